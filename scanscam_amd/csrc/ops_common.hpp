@@ -1,0 +1,161 @@
+// What the kernels of the state space layer's operators share: parameters of any type, sequences in a stream of tokens, the
+// activations' functions, column sums.
+#pragma once
+
+#include "scanscam_ops.h"
+
+#include "scan_kernels.hpp"
+
+namespace scanscam {
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A parameter's element, whatever its type; `fill` where there is no parameter.
+__device__ __forceinline__ float param(const scanscam_param &p, int64_t i, float fill = 0.0f)
+{
+    if (p.p == nullptr) return fill;
+    if (p.dtype == SCANSCAM_F32) return static_cast<const float *>(p.p)[i];
+    if (p.dtype == SCANSCAM_BF16) return (float)static_cast<const __bf16 *>(p.p)[i];
+    return (float)static_cast<const _Float16 *>(p.p)[i];
+}
+
+__device__ __forceinline__ int64_t index_at(const void *p, int wide, int64_t i)
+{
+    return wide ? static_cast<const int64_t *>(p)[i] : (int64_t)static_cast<const int32_t *>(p)[i];
+}
+
+// exp by the hardware's 2^x (one unit in the last place), 1/x likewise; both flush no result that fp32 sums would keep.
+__device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float sigmoid_(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_(-x)); }
+
+// log(1 + e^x) = max(x, 0) + log(1 + t), t = e^-|x| in (0, 1]. log(1 + t) = 2 artanh(w), w = t / (2 + t) <= 1/3, by its
+// series 2 w (1 + w^2/3 + w^4/5 + ...), cut after w^14: what is left out is below 2^-27 of the result, and small t (step
+// sizes of 0.001 are where a model starts) keep all their digits, which the logarithm of the rounded 1 + t loses.
+__device__ __forceinline__ float softplus_(float x)
+{
+    const float t = exp_(-__builtin_fabsf(x));
+    const float w = t * __builtin_amdgcn_rcpf(2.0f + t), q = w * w;
+    float s = 1.0f / 15;
+    s = __builtin_fmaf(s, q, 1.0f / 13);
+    s = __builtin_fmaf(s, q, 1.0f / 11);
+    s = __builtin_fmaf(s, q, 1.0f / 9);
+    s = __builtin_fmaf(s, q, 1.0f / 7);
+    s = __builtin_fmaf(s, q, 1.0f / 5);
+    s = __builtin_fmaf(s, q, 1.0f / 3);
+    s = __builtin_fmaf(s, q, 1.0f);
+    // (max() would lose a NaN: x + |x| keeps it)
+    return __builtin_fmaf(2.0f * w, s, 0.5f * (x + __builtin_fabsf(x)));
+}
+
+// VEC neighbouring elements, of which the first `count` are there; they need no more than their own alignment.
+template <typename ST, int VEC>
+__device__ __forceinline__ void load_part(const ST *p, int count, float (&f)[VEC])
+{
+    if (count >= VEC) {
+        constexpr int PIECE = VEC * sizeof(ST) > 16 ? 16 / sizeof(ST) : VEC;
+        using raw_t = typename RawT<sizeof(ST) * PIECE>::type;
+        typedef raw_t raw_unaligned_t __attribute__((aligned(sizeof(ST))));
+#pragma unroll
+        for (int j = 0; j < VEC; j += PIECE) {
+            const raw_t raw = *reinterpret_cast<const raw_unaligned_t *>(p + j);
+            const Elems<ST, PIECE> e = __builtin_bit_cast(Elems<ST, PIECE>, raw);
+#pragma unroll
+            for (int k = 0; k < PIECE; k++) f[j + k] = (float)e.e[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; k++) f[k] = k < count ? (float)p[k] : 0.0f;
+    }
+}
+template <typename ST, int VEC>
+__device__ __forceinline__ void store_some(ST *p, int count, const float (&f)[VEC])
+{
+    if (count >= VEC) {
+        constexpr int PIECE = VEC * sizeof(ST) > 16 ? 16 / sizeof(ST) : VEC;
+        using raw_t = typename RawT<sizeof(ST) * PIECE>::type;
+        typedef raw_t raw_unaligned_t __attribute__((aligned(sizeof(ST))));
+#pragma unroll
+        for (int j = 0; j < VEC; j += PIECE) {
+            Elems<ST, PIECE> e;
+#pragma unroll
+            for (int k = 0; k < PIECE; k++) e.e[k] = (ST)f[j + k];
+            *reinterpret_cast<raw_unaligned_t *>(p + j) = __builtin_bit_cast(raw_t, e);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; k++)
+            if (k < count) p[k] = (ST)f[k];
+    }
+}
+
+// The sequence that token t of a packed stream belongs to: the last one that starts at or before t.
+__device__ __forceinline__ int64_t sequence_of(const void *offsets, int wide, int64_t sequences, int64_t t)
+{
+    int64_t lo = 0, hi = sequences - 1;  // the answer lies in [lo, hi]
+    while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) >> 1;
+        if (index_at(offsets, wide, mid) <= t) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int64_t clamp_(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// out[m] = sum over p < parts of in[p * pitch + m], in an order that the sizes alone decide: 16 threads a column, each over every
+// 16th part, joined in order. The parts are themselves sums of some hundreds of values, so that no sum is one long chain.
+struct ColumnSum {
+    const float *in;
+    float *out;
+    int64_t parts, pitch, columns;
+};
+
+__global__ __launch_bounds__(1024) void column_sum_kernel(ColumnSum a);
+
+inline unsigned column_blocks(int64_t columns) { return (unsigned)ceil_div(columns, 64); }
+
+template <typename Kernel, typename Args>
+inline hipError_t launch_op(Kernel kernel, dim3 grid, dim3 block, size_t lds, hipStream_t stream, const Args &args)
+{
+    Args copy = args;
+    void *params[] = {&copy};
+    return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, params, lds, stream);
+}
+
+inline hipError_t column_sum(const float *in, float *out, int64_t parts, int64_t pitch, int64_t columns, hipStream_t stream)
+{
+    return launch_op(column_sum_kernel, dim3(column_blocks(columns)), dim3(1024), 0, stream, ColumnSum{in, out, parts, pitch, columns});
+}
+
+// --- checks of arguments ---------------------------------------------------------------------------------------------------
+inline int activation_size(int dtype)
+{
+    return dtype == SCANSCAM_F32 ? 4 : dtype == SCANSCAM_BF16 || dtype == SCANSCAM_F16 ? 2 : 0;
+}
+inline bool misaligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+inline int check_tokens(const scanscam_tokens &t, int size)
+{
+    if (t.p == nullptr || t.batch < 0 || t.token < 0 || t.group < 0) return SCANSCAM_EINVAL;
+    return misaligned(t.p, (size_t)size) ? SCANSCAM_EALIGN : SCANSCAM_OK;
+}
+inline int check_param(const scanscam_param &p, bool required)
+{
+    if (p.p == nullptr) return required ? SCANSCAM_EINVAL : SCANSCAM_OK;
+    const int size = activation_size(p.dtype);
+    if (size == 0) return SCANSCAM_EDTYPE;
+    return misaligned(p.p, (size_t)size) ? SCANSCAM_EALIGN : SCANSCAM_OK;
+}
+
+constexpr int64_t kMostTokens = (int64_t(1) << 31) - (int64_t(1) << 20), kMostChannels = int64_t(1) << 20;
+
+#define SCANSCAM_CHECK(expr)                      \
+    do {                                          \
+        const int rc_ = (expr);                   \
+        if (rc_ != SCANSCAM_OK) return rc_;       \
+    } while (0)
+
+}  // namespace scanscam

@@ -1,0 +1,179 @@
+// C ABI of the selective scan (declared in include/scanscam_ops.h): argument checks, launch shapes, launches.
+#include "selective_kernels.hpp"
+
+namespace {
+
+using namespace scanscam;
+
+constexpr int kTokensALane = 8;  // K
+constexpr int kTile = Geometry<kTokensALane>::kTile;
+constexpr int64_t kMostStates = 256;
+
+int check_sizes(int64_t channels, int64_t groups, int64_t N, int dtype)
+{
+    if (channels < 0 || channels > kMostChannels || groups < 1 || channels % groups != 0 || N < 1 || N > kMostStates) return SCANSCAM_EINVAL;
+    return activation_size(dtype) == 0 ? SCANSCAM_EDTYPE : SCANSCAM_OK;
+}
+
+int check_selective(const scanscam_selective *a)
+{
+    if (a == nullptr) return SCANSCAM_EINVAL;
+    SCANSCAM_CHECK(check_sizes(a->channels, a->groups, a->N, a->dtype));
+    if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->sequences > 65535 || a->parts < 0) return SCANSCAM_EINVAL;
+    if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
+    if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
+    SCANSCAM_CHECK(check_param(a->A, true));
+    SCANSCAM_CHECK(check_param(a->D, false));
+    SCANSCAM_CHECK(check_param(a->dt_bias, false));
+    if (misaligned(a->offsets, a->offsets64 ? 8 : 4) || misaligned(a->state_in, 4) || misaligned(a->state_out, 4) || misaligned(a->saved, 16))
+        return SCANSCAM_EALIGN;
+    if (a->batch * a->T == 0) return SCANSCAM_OK;
+    const int size = activation_size(a->dtype);
+    for (const scanscam_tokens *t : {&a->x, &a->dt, &a->B, &a->C}) SCANSCAM_CHECK(check_tokens(*t, size));
+    return a->z.p != nullptr ? check_tokens(a->z, size) : SCANSCAM_OK;
+}
+
+template <typename Kernel, typename Args>
+hipError_t launch_wide(Kernel kernel, dim3 grid, int threads, int words, hipStream_t stream, const Args &args)
+{
+    const size_t bytes = (size_t)words * sizeof(float);
+    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return err != hipSuccess ? err : launch_op(kernel, grid, dim3((unsigned)threads), bytes, stream, args);
+}
+
+// Waves that share the states of a channel out: more where there are too few channels to give every CU two workgroups.
+int forward_split(const scanscam_selective &a)
+{
+    int split = 1;
+    while (split < kFwdWaves && split < a.N && a.sequences * a.groups * ceil_div(a.channels / a.groups, kFwdWaves / split * kRows) < 512) split *= 2;
+    return split;
+}
+
+int64_t forward_blocks(const scanscam_selective &a, int split) { return ceil_div(a.channels / a.groups, kFwdWaves / split * kRows); }
+int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels); }
+
+size_t bc_words(const scanscam_selective &a)
+{
+    return (size_t)(a.groups * backward_blocks(a) * a.batch * a.T * 2 * a.N);
+}
+
+template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream_t stream)
+{
+    const int split = forward_split(a);
+    const SelectiveArgs args{a, split, forward_blocks(a, split)};
+    return launch_wide(selective_fwd_kernel<ST, kTokensALane>, dim3((unsigned)(a.groups * args.blocks), (unsigned)a.sequences), kFwdWaves * 64,
+                       ForwardLds<kTokensALane>::words(kFwdWaves / split * kRows, (int)a.N), stream, args);
+}
+
+template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream_t stream)
+{
+    const int64_t blocks = backward_blocks(a);
+    float *bc = static_cast<float *>(a.workspace), *sums = bc + bc_words(a);
+    const BackwardArgs args{{a, 0, blocks}, bc, sums};
+    hipError_t err = launch_wide(selective_bwd_kernel<ST, kTokensALane>, dim3((unsigned)(a.groups * blocks), (unsigned)a.sequences), kBwdWaves * 64,
+                                 BackwardLds<kTokensALane>::words((int)a.N), stream, args);
+    const int64_t values = a.batch * a.T * 2 * a.N;
+    if (err == hipSuccess && values > 0)
+        err = launch_op(selective_bc_kernel<ST>, dim3((unsigned)ceil_div(values, 256), (unsigned)a.groups), dim3(256), 0, stream, GroupSum{a, bc, blocks});
+    const int64_t pitch = (a.N + 2) * a.channels;
+    if (err == hipSuccess) err = column_sum(sums, a.gA, a.sequences, pitch, a.N * a.channels, stream);
+    if (err == hipSuccess && a.gD != nullptr) err = column_sum(sums + a.N * a.channels, a.gD, a.sequences, pitch, a.channels, stream);
+    if (err == hipSuccess && a.gdt_bias != nullptr)
+        err = column_sum(sums + (a.N + 1) * a.channels, a.gdt_bias, a.sequences, pitch, a.channels, stream);
+    return err;
+}
+
+template <typename ST> hipError_t run_step(const scanscam_selective_step &a, hipStream_t stream)
+{
+    int lanes = 1;
+    while (lanes < 32 && lanes * 4 < a.N) lanes *= 2;
+    const dim3 grid((unsigned)a.rows, (unsigned)ceil_div(a.channels, 256 / lanes));
+    switch (lanes) {
+    case 1: return launch_op(selective_step_kernel<ST, 1>, grid, dim3(256), 0, stream, a);
+    case 2: return launch_op(selective_step_kernel<ST, 2>, grid, dim3(256), 0, stream, a);
+    case 4: return launch_op(selective_step_kernel<ST, 4>, grid, dim3(256), 0, stream, a);
+    case 8: return launch_op(selective_step_kernel<ST, 8>, grid, dim3(256), 0, stream, a);
+    case 16: return launch_op(selective_step_kernel<ST, 16>, grid, dim3(256), 0, stream, a);
+    default: return launch_op(selective_step_kernel<ST, 32>, grid, dim3(256), 0, stream, a);
+    }
+}
+
+int status(hipError_t err) { return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH; }
+
+}  // namespace
+
+extern "C" {
+
+size_t scanscam_selective_saved_bytes(const scanscam_selective *a)
+{
+    if (a == nullptr || check_sizes(a->channels, a->groups, a->N, a->dtype) != SCANSCAM_OK || a->batch <= 0 || a->T <= 0 || a->sequences <= 0) return 0;
+    return (size_t)(all_tiles(*a, kTile) * a->N * a->channels) * sizeof(float);
+}
+
+size_t scanscam_selective_workspace_bytes(const scanscam_selective *a, int direction)
+{
+    if (a == nullptr || check_sizes(a->channels, a->groups, a->N, a->dtype) != SCANSCAM_OK || a->batch <= 0 || a->T < 0 || a->sequences <= 0) return 0;
+    if (direction == SCANSCAM_FORWARD) return 0;
+    return (bc_words(*a) + (size_t)(a->sequences * (a->N + 2) * a->channels)) * sizeof(float);
+}
+
+int scanscam_selective_fwd(const scanscam_selective *a, void *stream)
+{
+    SCANSCAM_CHECK(check_selective(a));
+    if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
+    if (a->batch * a->T > 0) SCANSCAM_CHECK(check_tokens(a->y, activation_size(a->dtype)));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return status(a->dtype == SCANSCAM_F32    ? run_fwd<float>(*a, s)
+                  : a->dtype == SCANSCAM_BF16 ? run_fwd<__bf16>(*a, s)
+                                              : run_fwd<_Float16>(*a, s));
+}
+
+int scanscam_selective_bwd(const scanscam_selective *a, void *stream)
+{
+    SCANSCAM_CHECK(check_selective(a));
+    if (a->channels == 0) return SCANSCAM_OK;
+    if (a->gA == nullptr) return SCANSCAM_EINVAL;
+    if (a->sequences > 0) {
+        if (a->batch * a->T > 0) {
+            const int size = activation_size(a->dtype);
+            for (const scanscam_tokens *t : {&a->gy, &a->gx, &a->gdt, &a->gB, &a->gC}) SCANSCAM_CHECK(check_tokens(*t, size));
+            if (a->z.p != nullptr) SCANSCAM_CHECK(check_tokens(a->gz, size));
+            if (a->saved == nullptr) return SCANSCAM_EINVAL;
+        }
+        if (misaligned(a->gstate_out, 4) || misaligned(a->gstate_in, 4)) return SCANSCAM_EALIGN;
+        if (a->workspace == nullptr || a->workspace_bytes < scanscam_selective_workspace_bytes(a, SCANSCAM_BACKWARD)) return SCANSCAM_EWORKSPACE;
+        if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a->sequences == 0) {
+        hipError_t err = column_sum(nullptr, a->gA, 0, 0, a->N * a->channels, s);
+        if (err == hipSuccess && a->gD != nullptr) err = column_sum(nullptr, a->gD, 0, 0, a->channels, s);
+        if (err == hipSuccess && a->gdt_bias != nullptr) err = column_sum(nullptr, a->gdt_bias, 0, 0, a->channels, s);
+        return status(err);
+    }
+    return status(a->dtype == SCANSCAM_F32    ? run_bwd<float>(*a, s)
+                  : a->dtype == SCANSCAM_BF16 ? run_bwd<__bf16>(*a, s)
+                                              : run_bwd<_Float16>(*a, s));
+}
+
+int scanscam_selective_step_fwd(const scanscam_selective_step *a, void *stream)
+{
+    if (a == nullptr) return SCANSCAM_EINVAL;
+    SCANSCAM_CHECK(check_sizes(a->channels, a->groups, a->N, a->dtype));
+    if (a->rows < 0 || a->rows >= (int64_t(1) << 24) || a->slots < 0) return SCANSCAM_EINVAL;
+    if (a->rows == 0 || a->channels == 0) return SCANSCAM_OK;
+    const int size = activation_size(a->dtype);
+    for (const scanscam_tokens *t : {&a->x, &a->dt, &a->B, &a->C, &a->y}) SCANSCAM_CHECK(check_tokens(*t, size));
+    if (a->z.p != nullptr) SCANSCAM_CHECK(check_tokens(a->z, size));
+    SCANSCAM_CHECK(check_param(a->A, true));
+    SCANSCAM_CHECK(check_param(a->D, false));
+    SCANSCAM_CHECK(check_param(a->dt_bias, false));
+    if (a->state == nullptr) return SCANSCAM_EINVAL;
+    if (misaligned(a->state, 4) || misaligned(a->slot, a->slot64 ? 8 : 4)) return SCANSCAM_EALIGN;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return status(a->dtype == SCANSCAM_F32    ? run_step<float>(*a, s)
+                  : a->dtype == SCANSCAM_BF16 ? run_step<__bf16>(*a, s)
+                                              : run_step<_Float16>(*a, s));
+}
+
+}  // extern "C"

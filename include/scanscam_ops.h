@@ -61,8 +61,10 @@ typedef struct scanscam_param {
  * `saved`: for a backward call, the states that its tiles of time start from
  * (scanscam_selective_saved_bytes). The workspace (scanscam_selective_workspace_bytes)
  * is for calls that share the time of a sequence out over workgroups, and for
- * the sums of the backward call. Both need alignment to 16 bytes.
+ * the sums of the backward call. Both need alignment to 16 bytes. Strides from token to token must stay below
+ * SCANSCAM_MOST_TOKEN_STRIDE.
  */
+#define SCANSCAM_MOST_TOKEN_STRIDE (1 << 22)
 typedef struct scanscam_selective {
     int64_t batch, T, sequences, channels, groups, N;
     const void *offsets; /* or NULL */

@@ -7,7 +7,7 @@ using namespace scanscam;
 
 constexpr int kTokensALane = 8;  // K
 constexpr int kTile = Geometry<kTokensALane>::kTile;
-constexpr int64_t kMostStates = 256;
+constexpr int64_t kMostStates = 256, kMostParts = 1024;
 
 int check_sizes(int64_t channels, int64_t groups, int64_t N, int dtype)
 {
@@ -15,11 +15,18 @@ int check_sizes(int64_t channels, int64_t groups, int64_t N, int dtype)
     return activation_size(dtype) == 0 ? SCANSCAM_EDTYPE : SCANSCAM_OK;
 }
 
+// The kernels reach the tokens of a tile from its first one with 32-bit offsets.
+int check_near(const scanscam_tokens &t, int size)
+{
+    SCANSCAM_CHECK(check_tokens(t, size));
+    return t.token < SCANSCAM_MOST_TOKEN_STRIDE ? SCANSCAM_OK : SCANSCAM_EINVAL;
+}
+
 int check_selective(const scanscam_selective *a)
 {
     if (a == nullptr) return SCANSCAM_EINVAL;
     SCANSCAM_CHECK(check_sizes(a->channels, a->groups, a->N, a->dtype));
-    if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->sequences > 65535 || a->parts < 0) return SCANSCAM_EINVAL;
+    if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->parts < 0 || a->parts > kMostParts || a->sequences * (a->parts > 0 ? a->parts : 1) > 65535) return SCANSCAM_EINVAL;
     if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
     if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
     SCANSCAM_CHECK(check_param(a->A, true));
@@ -29,8 +36,8 @@ int check_selective(const scanscam_selective *a)
         return SCANSCAM_EALIGN;
     if (a->batch * a->T == 0) return SCANSCAM_OK;
     const int size = activation_size(a->dtype);
-    for (const scanscam_tokens *t : {&a->x, &a->dt, &a->B, &a->C}) SCANSCAM_CHECK(check_tokens(*t, size));
-    return a->z.p != nullptr ? check_tokens(a->z, size) : SCANSCAM_OK;
+    for (const scanscam_tokens *t : {&a->x, &a->dt, &a->B, &a->C}) SCANSCAM_CHECK(check_near(*t, size));
+    return a->z.p != nullptr ? check_near(a->z, size) : SCANSCAM_OK;
 }
 
 template <typename Kernel, typename Args>
@@ -41,45 +48,68 @@ hipError_t launch_wide(Kernel kernel, dim3 grid, int threads, int words, hipStre
     return err != hipSuccess ? err : launch_op(kernel, grid, dim3((unsigned)threads), bytes, stream, args);
 }
 
-// Waves that share the states of a channel out: more where there are too few channels to give every CU two workgroups.
-int forward_split(const scanscam_selective &a)
-{
-    int split = 1;
-    while (split < kFwdWaves && split < a.N && a.sequences * a.groups * ceil_div(a.channels / a.groups, kFwdWaves / split * kRows) < 512) split *= 2;
-    return split;
-}
+struct Plan {
+    int split;      // forwards: waves that share the states of a channel out among them
+    int64_t parts;  // that the time of every sequence is cut into
+};
 
 int64_t forward_blocks(const scanscam_selective &a, int split) { return ceil_div(a.channels / a.groups, kFwdWaves / split * kRows); }
 int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels); }
 
-size_t bc_words(const scanscam_selective &a)
+// Parts of time, at least `shortest` tiles each, where the channels alone give fewer than `wanted` workgroups.
+int64_t choose_parts(const scanscam_selective &a, int64_t workgroups, int64_t wanted, int64_t shortest)
 {
-    return (size_t)(a.groups * backward_blocks(a) * a.batch * a.T * 2 * a.N);
+    if (a.parts > 0) return a.parts;
+    const int64_t tiles = ceil_div(a.T, kTile), most = tiles / shortest;
+    const int64_t parts = ceil_div(wanted, workgroups > 0 ? workgroups : 1);  // (a grid's rows suffice: sequences x parts is below 2 x wanted)
+    return parts < 2 || most < 2 ? 1 : parts < most ? parts : most;
 }
+
+Plan forward_plan(const scanscam_selective &a)
+{
+    Plan p{1, 1};
+    while (p.split < kFwdWaves && p.split < a.N && a.sequences * a.groups * forward_blocks(a, p.split) < 512) p.split *= 2;
+    p.parts = choose_parts(a, a.sequences * a.groups * forward_blocks(a, p.split), 512, 4);
+    return p;
+}
+Plan backward_plan(const scanscam_selective &a) { return {1, choose_parts(a, a.sequences * a.groups * backward_blocks(a), 512, 4)}; }
+
+size_t ends_words(const scanscam_selective &a, int64_t parts) { return parts > 1 ? (size_t)(a.sequences * parts * (a.N + 1) * a.channels) : 0; }
+size_t bc_words(const scanscam_selective &a) { return (size_t)(a.groups * backward_blocks(a) * a.batch * a.T * 2 * a.N); }
 
 template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream_t stream)
 {
-    const int split = forward_split(a);
-    const SelectiveArgs args{a, split, forward_blocks(a, split)};
-    return launch_wide(selective_fwd_kernel<ST, kTokensALane>, dim3((unsigned)(a.groups * args.blocks), (unsigned)a.sequences), kFwdWaves * 64,
-                       ForwardLds<kTokensALane>::words(kFwdWaves / split * kRows, (int)a.N), stream, args);
+    constexpr int K = kTokensALane;
+    const Plan plan = forward_plan(a);
+    const SelectiveArgs args{a, plan.split, forward_blocks(a, plan.split), plan.parts, static_cast<float *>(a.workspace), nullptr, nullptr};
+    const dim3 grid((unsigned)(a.groups * args.blocks), (unsigned)(a.sequences * plan.parts));
+    const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
+    if (plan.parts > 1) {
+        const hipError_t err = launch_wide(selective_fwd_kernel<ST, K, true>, grid, kFwdWaves * 64, words, stream, args);
+        if (err != hipSuccess) return err;
+    }
+    return launch_wide(selective_fwd_kernel<ST, K, false>, grid, kFwdWaves * 64, words, stream, args);
 }
 
 template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream_t stream)
 {
+    constexpr int K = kTokensALane;
+    const Plan plan = backward_plan(a);
     const int64_t blocks = backward_blocks(a);
-    float *bc = static_cast<float *>(a.workspace), *sums = bc + bc_words(a);
-    const BackwardArgs args{{a, 0, blocks}, bc, sums};
-    hipError_t err = launch_wide(selective_bwd_kernel<ST, kTokensALane>, dim3((unsigned)(a.groups * blocks), (unsigned)a.sequences), kBwdWaves * 64,
-                                 BackwardLds<kTokensALane>::words((int)a.N), stream, args);
+    float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.parts), *sums = bc + bc_words(a);
+    const SelectiveArgs args{a, 1, blocks, plan.parts, ends, bc, sums};
+    const dim3 grid((unsigned)(a.groups * blocks), (unsigned)(a.sequences * plan.parts));
+    const int words = BackwardLds<K>::words((int)a.N);
+    hipError_t err = hipSuccess;
+    if (plan.parts > 1) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
+    if (err == hipSuccess) err = launch_wide(selective_bwd_kernel<ST, K, false>, grid, kBwdWaves * 64, words, stream, args);
     const int64_t values = a.batch * a.T * 2 * a.N;
     if (err == hipSuccess && values > 0)
         err = launch_op(selective_bc_kernel<ST>, dim3((unsigned)ceil_div(values, 256), (unsigned)a.groups), dim3(256), 0, stream, GroupSum{a, bc, blocks});
-    const int64_t pitch = (a.N + 2) * a.channels;
-    if (err == hipSuccess) err = column_sum(sums, a.gA, a.sequences, pitch, a.N * a.channels, stream);
-    if (err == hipSuccess && a.gD != nullptr) err = column_sum(sums + a.N * a.channels, a.gD, a.sequences, pitch, a.channels, stream);
-    if (err == hipSuccess && a.gdt_bias != nullptr)
-        err = column_sum(sums + (a.N + 1) * a.channels, a.gdt_bias, a.sequences, pitch, a.channels, stream);
+    const int64_t pitch = (a.N + 2) * a.channels, rows = a.sequences * plan.parts;
+    if (err == hipSuccess) err = column_sum(sums, a.gA, rows, pitch, a.N * a.channels, stream);
+    if (err == hipSuccess && a.gD != nullptr) err = column_sum(sums + a.N * a.channels, a.gD, rows, pitch, a.channels, stream);
+    if (err == hipSuccess && a.gdt_bias != nullptr) err = column_sum(sums + (a.N + 1) * a.channels, a.gdt_bias, rows, pitch, a.channels, stream);
     return err;
 }
 
@@ -98,6 +128,13 @@ template <typename ST> hipError_t run_step(const scanscam_selective_step &a, hip
     }
 }
 
+int check_workspace(const scanscam_selective &a, int direction)
+{
+    const size_t bytes = scanscam_selective_workspace_bytes(&a, direction);
+    if (bytes > 0 && (a.workspace == nullptr || a.workspace_bytes < bytes)) return SCANSCAM_EWORKSPACE;
+    return misaligned(a.workspace, 16) ? SCANSCAM_EALIGN : SCANSCAM_OK;
+}
+
 int status(hipError_t err) { return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH; }
 
 }  // namespace
@@ -113,15 +150,17 @@ size_t scanscam_selective_saved_bytes(const scanscam_selective *a)
 size_t scanscam_selective_workspace_bytes(const scanscam_selective *a, int direction)
 {
     if (a == nullptr || check_sizes(a->channels, a->groups, a->N, a->dtype) != SCANSCAM_OK || a->batch <= 0 || a->T < 0 || a->sequences <= 0) return 0;
-    if (direction == SCANSCAM_FORWARD) return 0;
-    return (bc_words(*a) + (size_t)(a->sequences * (a->N + 2) * a->channels)) * sizeof(float);
+    if (direction == SCANSCAM_FORWARD) return ends_words(*a, forward_plan(*a).parts) * sizeof(float);
+    const int64_t parts = backward_plan(*a).parts;
+    return (ends_words(*a, parts) + bc_words(*a) + (size_t)(a->sequences * parts * (a->N + 2) * a->channels)) * sizeof(float);
 }
 
 int scanscam_selective_fwd(const scanscam_selective *a, void *stream)
 {
     SCANSCAM_CHECK(check_selective(a));
     if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
-    if (a->batch * a->T > 0) SCANSCAM_CHECK(check_tokens(a->y, activation_size(a->dtype)));
+    if (a->batch * a->T > 0) SCANSCAM_CHECK(check_near(a->y, activation_size(a->dtype)));
+    SCANSCAM_CHECK(check_workspace(*a, SCANSCAM_FORWARD));
     hipStream_t s = static_cast<hipStream_t>(stream);
     return status(a->dtype == SCANSCAM_F32    ? run_fwd<float>(*a, s)
                   : a->dtype == SCANSCAM_BF16 ? run_fwd<__bf16>(*a, s)
@@ -136,13 +175,12 @@ int scanscam_selective_bwd(const scanscam_selective *a, void *stream)
     if (a->sequences > 0) {
         if (a->batch * a->T > 0) {
             const int size = activation_size(a->dtype);
-            for (const scanscam_tokens *t : {&a->gy, &a->gx, &a->gdt, &a->gB, &a->gC}) SCANSCAM_CHECK(check_tokens(*t, size));
-            if (a->z.p != nullptr) SCANSCAM_CHECK(check_tokens(a->gz, size));
+            for (const scanscam_tokens *t : {&a->gy, &a->gx, &a->gdt, &a->gB, &a->gC}) SCANSCAM_CHECK(check_near(*t, size));
+            if (a->z.p != nullptr) SCANSCAM_CHECK(check_near(a->gz, size));
             if (a->saved == nullptr) return SCANSCAM_EINVAL;
         }
         if (misaligned(a->gstate_out, 4) || misaligned(a->gstate_in, 4)) return SCANSCAM_EALIGN;
-        if (a->workspace == nullptr || a->workspace_bytes < scanscam_selective_workspace_bytes(a, SCANSCAM_BACKWARD)) return SCANSCAM_EWORKSPACE;
-        if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
+        SCANSCAM_CHECK(check_workspace(*a, SCANSCAM_BACKWARD));
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->sequences == 0) {

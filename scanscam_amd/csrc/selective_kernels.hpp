@@ -28,12 +28,6 @@ constexpr int kTimeLanes = 16;   // lanes of a row: tokens of one channel
 constexpr int kRows = 4;         // channels of a wave
 constexpr int kStateBlock = 16;  // states whose B and C are in LDS at a time
 
-struct SelectiveArgs {
-    scanscam_selective a;
-    int split;        // waves that share the states of a channel out among them
-    int64_t blocks;   // of channels, in a group
-};
-
 // What follows from K. Tokens lie in LDS as [K / 4][16 lanes][4], 4 floats of padding behind each 64, so that the 16-byte reads of
 // neighbouring lanes are neighbours and the single writes of a wave spread over the banks.
 template <int K> struct Geometry {
@@ -58,57 +52,82 @@ template <int K> struct Geometry {
     }
 };
 
-// A scan step over affine maps h -> a h + b inside rows of 16 lanes: lanes without a source are left as they are (their a is
-// finite, see finite_).
-template <int CTRL> __device__ __forceinline__ void row_step(float &a, float &b)
-{
-    const float a1 = dpp_move<CTRL, 0xf>(1.0f, a), b1 = dpp_move<CTRL, 0xf>(0.0f, b);
-    b = __builtin_fmaf(a, b1, b);
-    a = a * a1;
-}
-// Inclusive over ascending lanes (FORWARDS) or descending ones.
+// Inclusive scan over affine maps h -> a h + b inside rows of 16 lanes, over ascending lanes (FORWARDS) or descending ones, as
+// DPP operands of the multiply-add itself: b += a' s b, a *= a' s a; a lane without a source writes nothing, so neither
+// an identity nor a mask is needed and a channel never meets another one's values. Two instructions and a wait state a step; as builtins
+// (moves with identities to fill) it was seven, a quarter of the forward kernel's instructions. A DPP source needs two
+// wait states behind its write: the first nop covers whatever wrote a and b, the others the step before.
+#define SCANSCAM_ROW_STEP(DIR, N)                                                       \
+    "v_fmac_f32_dpp %1, %1, %0 row_" DIR ":" N " row_mask:0xf bank_mask:0xf\n\t"       \
+    "v_mul_f32_dpp %0, %0, %0 row_" DIR ":" N " row_mask:0xf bank_mask:0xf\n\t"        \
+    "s_nop 0\n\t"
 template <bool FORWARDS> __device__ __forceinline__ void row_scan(float &a, float &b)
 {
     if constexpr (FORWARDS) {
-        row_step<0x111>(a, b);
-        row_step<0x112>(a, b);
-        row_step<0x114>(a, b);
-        row_step<0x118>(a, b);
+        asm volatile("s_nop 1\n\t" SCANSCAM_ROW_STEP("shr", "1") SCANSCAM_ROW_STEP("shr", "2") SCANSCAM_ROW_STEP("shr", "4")
+                     "v_fmac_f32_dpp %1, %1, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\t" "s_nop 1"
+                     : "+v"(a), "+v"(b));
     } else {
-        row_step<0x101>(a, b);
-        row_step<0x102>(a, b);
-        row_step<0x104>(a, b);
-        row_step<0x108>(a, b);
+        asm volatile("s_nop 1\n\t" SCANSCAM_ROW_STEP("shl", "1") SCANSCAM_ROW_STEP("shl", "2") SCANSCAM_ROW_STEP("shl", "4")
+                     "v_fmac_f32_dpp %1, %1, %0 row_shl:8 row_mask:0xf bank_mask:0xf\n\t" "s_nop 1"
+                     : "+v"(a), "+v"(b));
     }
 }
+#undef SCANSCAM_ROW_STEP
 __device__ __forceinline__ float row_prev(float v, float fill) { return dpp_move<0x111, 0xf>(fill, v); }
 __device__ __forceinline__ float row_next(float v, float fill) { return dpp_move<0x101, 0xf>(fill, v); }
+// The sum over a row's lanes, in lane 15.
 __device__ __forceinline__ float row_sum(float v)
 {
-    v += dpp_move<0x111, 0xf>(0.0f, v);
-    v += dpp_move<0x112, 0xf>(0.0f, v);
-    v += dpp_move<0x114, 0xf>(0.0f, v);
-    v += dpp_move<0x118, 0xf>(0.0f, v);
-    return v;  // in lane 15
+    asm volatile("s_nop 1\n\t"
+                 "v_add_f32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+                 "v_add_f32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+                 "v_add_f32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
+                 "v_add_f32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf"
+                 : "+v"(v));
+    return v;
 }
-// A lane's whole decay. It multiplies zeros where a lane has no source: an overflow (growing states only) must not make those NaN.
-__device__ __forceinline__ float finite_(float a) { return __builtin_fminf(a, __FLT_MAX__); }
+// The sums over the four rows of four values, the sum of value r in row r. A swap of halves puts two values' lanes behind each
+// other, so that an addition serves both: six instructions, where four sums of their own take sixteen.
+__device__ __forceinline__ float halves_sum(float a, float b)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+__device__ __forceinline__ float rows_sum(float v0, float v1, float v2, float v3)
+{
+    const float a = halves_sum(v0, v2), b = halves_sum(v1, v3);
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
 
-// The stretch of tokens that a workgroup goes through.
+// The stretch of tokens that a workgroup goes through: one of `parts` of a sequence, whole tiles from the sequence's start on.
 struct Stretch {
-    int64_t seq, batch, start, end;
+    int64_t seq, batch, part, start, end, tile;  // tile: number of its first tile among all sequences', for `saved`
 };
-__device__ __forceinline__ Stretch stretch_of(const scanscam_selective &a, int64_t unit)
+// A sequence of L tokens has at most L / TILE + 1 tiles, so that packed ones can be counted from their starts.
+template <int TILE> __device__ __forceinline__ Stretch stretch_of(const scanscam_selective &a, int64_t unit, int64_t parts)
 {
-    if (a.offsets == nullptr) return {unit, unit, 0, a.T};
-    const int64_t start = clamp_(index_at(a.offsets, a.offsets64, unit), 0, a.T);
-    return {unit, 0, start, clamp_(index_at(a.offsets, a.offsets64, unit + 1), start, a.T)};
-}
-// Tiles of the stretches before this one, for `saved`: a sequence of L tokens has at most L / TILE + 1 of them.
-template <int TILE> __device__ __forceinline__ int64_t first_tile(const scanscam_selective &a, const Stretch &s)
-{
-    if (a.offsets == nullptr) return s.seq * ((a.T + TILE - 1) / TILE);
-    return s.start / TILE + s.seq;
+    Stretch s;
+    s.seq = unit / parts;
+    s.part = unit - s.seq * parts;
+    s.batch = 0;
+    if (a.offsets == nullptr) {
+        s.batch = s.seq;
+        s.start = 0;
+        s.end = a.T;
+        s.tile = s.seq * ((a.T + TILE - 1) / TILE);
+    } else {
+        s.start = clamp_(index_at(a.offsets, a.offsets64, s.seq), 0, a.T);
+        s.end = clamp_(index_at(a.offsets, a.offsets64, s.seq + 1), s.start, a.T);
+        s.tile = s.start / TILE + s.seq;
+    }
+    const int64_t tiles = (s.end - s.start + TILE - 1) / TILE, each = (tiles + parts - 1) / parts;
+    const int64_t from = s.part * each < tiles ? s.part * each : tiles, to = from + each < tiles ? from + each : tiles;
+    s.end = to < tiles ? s.start + to * TILE : s.end;
+    s.start = from < tiles ? s.start + from * TILE : s.end;
+    s.tile += from;
+    return s;
 }
 __host__ __device__ inline int64_t all_tiles(const scanscam_selective &a, int64_t tile)
 {
@@ -121,23 +140,128 @@ __device__ __forceinline__ const ST *token_at(const scanscam_tokens &x, int64_t 
     return static_cast<const ST *>(x.p) + batch * x.batch + t * x.token + c;
 }
 
+// An element a 32-bit number of them behind a place that is the same for all lanes: an address of a scalar base and a vector offset.
+template <typename ST> __device__ __forceinline__ ST *behind(const ST *base, uint32_t elements)
+{
+    return reinterpret_cast<ST *>(reinterpret_cast<uintptr_t>(base) + (uint64_t)(uint32_t)(elements * (uint32_t)sizeof(ST)));
+}
+
+// Four neighbouring elements as they are stored. Where not all quads of a workgroup are whole, they are read one by one, those
+// past the end as the last one.
+template <typename ST> struct Quad {
+    ST e[4];
+    using raw_t = typename RawT<sizeof(ST) * 4>::type;
+    typedef raw_t raw_unaligned_t __attribute__((aligned(sizeof(ST))));
+    __device__ __forceinline__ void load(const ST *base, uint32_t at, int count, bool whole)
+    {
+        if (whole) {
+            const raw_t raw = *reinterpret_cast<const raw_unaligned_t *>(behind(base, at));
+            *this = __builtin_bit_cast(Quad, raw);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[i] = *behind(base, at + (uint32_t)(i < count ? i : count - 1));
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return (float)e[i]; }
+};
+template <typename ST> __device__ __forceinline__ void store_quad(ST *base, uint32_t at, int count, bool whole, const float (&f)[4])
+{
+    Quad<ST> q;
+#pragma unroll
+    for (int i = 0; i < 4; i++) q.e[i] = (ST)f[i];
+    if (whole) {
+        *reinterpret_cast<typename Quad<ST>::raw_unaligned_t *>(behind(base, at)) = __builtin_bit_cast(typename Quad<ST>::raw_t, q);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < count) *behind(base, at + (uint32_t)i) = q.e[i];
+    }
+}
+
+// The same value, of which the compiler does not know that it is: what is derived from it is computed again for every tile, where
+// it would otherwise be kept in registers (or spilled) through the scan of one.
+__device__ __forceinline__ int again(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// What a thread brings in of B and C for a block of states: quads of neighbouring states of a token each.
+template <typename ST, int TILE, int THREADS> struct StateInputs {
+    static constexpr int kQuads = kStateBlock / 4, kCount = TILE * kQuads / THREADS;
+    static_assert(TILE * kQuads % THREADS == 0, "every thread has as many quads");
+    Quad<ST> B[kCount], C[kCount];
+    __device__ __forceinline__ void load(const scanscam_selective &a, int64_t batch, int64_t group, int64_t t0, int length, int n0)
+    {
+        const ST *fromB = token_at<ST>(a.B, batch, t0, group * a.B.group), *fromC = token_at<ST>(a.C, batch, t0, group * a.C.group);
+        const int thread = again((int)threadIdx.x), N = (int)a.N, n = n0 + thread % kQuads * 4;
+        const int at = n < N ? n : 0;  // (past the last state: any that is there)
+        const bool whole = N % 4 == 0;
+#pragma unroll
+        for (int j = 0; j < kCount; j++) {
+            const int t = (thread + j * THREADS) / kQuads, row = t < length ? t : length - 1;
+            B[j].load(fromB, (uint32_t)row * (uint32_t)a.B.token + (uint32_t)at, N - at, whole);
+            C[j].load(fromC, (uint32_t)row * (uint32_t)a.C.token + (uint32_t)at, N - at, whole);
+        }
+    }
+    template <typename G> __device__ __forceinline__ void store(float *lB, float *lC, int length, int states) const
+    {
+        const int thread = again((int)threadIdx.x), n = thread % kQuads * 4;
+#pragma unroll
+        for (int j = 0; j < kCount; j++) {
+            const int t = (thread + j * THREADS) / kQuads;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool there = t < length && n + k < states;
+                lB[(n + k) * G::kPitch + G::place(t)] = there ? B[j][k] : 0.0f;
+                lC[(n + k) * G::kPitch + G::place(t)] = there ? C[j][k] : 0.0f;
+            }
+        }
+    }
+};
+
+struct SelectiveArgs {
+    scanscam_selective a;
+    int split;        // forwards: waves that share the states of a channel out among them
+    int64_t blocks;   // of channels, in a group
+    int64_t parts;    // that the time of every sequence is cut into
+    float *ends;      // [sequences][parts][N + 1][channels]: the states that a part alone ends with (backwards: starts with), its sum of d
+    float *bc;        // backwards: [blocks of all groups][tokens][2][N], sums of gB and gC over a workgroup's channels
+    float *sums;      // backwards: [sequences][parts][N + 2][channels], sums over a part's tokens for A, D and dt_bias
+};
+
+// The state before a part (the gradient behind it): that of the sequence's end, taken through the parts between. A part alone
+// is the map h -> exp(A * sum of d) h + its own end.
+__device__ __forceinline__ float carried(const SelectiveArgs &args, const Stretch &s, int n, int64_t channel, float A, float h, bool forwards)
+{
+    const scanscam_selective &a = args.a;
+    const int64_t pitch = (a.N + 1) * a.channels;
+    const float *ends = args.ends + s.seq * args.parts * pitch + channel;
+    for (int64_t q = forwards ? 0 : args.parts - 1; forwards ? q < s.part : q > s.part; q += forwards ? 1 : -1)
+        h = __builtin_fmaf(__builtin_amdgcn_exp2f(A * ends[q * pitch + a.N * a.channels]), h, ends[q * pitch + n * a.channels]);
+    return h;
+}
+
+struct Carry { float A, h; };  // A log2(e), and the state
+
 // ---------------------------------------------------------------------------------------------------------------------------
-// Forwards. A workgroup of 8 waves takes 8 / split groups of 4 channels through a stretch, tile by tile.
+// Forwards. A workgroup of 8 waves takes 8 / split groups of 4 channels through a stretch, tile by tile; the next tile's tensors
+// are loaded while this one is scanned. With ENDS only the states at the stretch's end are found, from zeros.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kFwdWaves = 8;
 
 template <int K> struct ForwardLds {
     using G = Geometry<K>;
-    static constexpr int kRowsOut = kFwdWaves * kRows;  // channels x split: rows of sums over n
+    static constexpr int kSums = kFwdWaves * kRows;  // channels x split: rows of sums over n
     // floats: d and u of the channels, sums, B and C; then A and the carries of all states
     static __host__ __device__ constexpr int words(int channels, int N)
     {
-        return 2 * channels * G::kPitch + kRowsOut * G::kPitch + 2 * kStateBlock * G::kPitch + 2 * channels * N;
+        return 2 * channels * G::kPitch + kSums * G::kPitch + 2 * kStateBlock * G::kPitch + 2 * channels * N;
     }
 };
 
-template <typename ST, int K>
-__global__ __launch_bounds__(kFwdWaves * 64) void selective_fwd_kernel(SelectiveArgs args)
+template <typename ST, int K, bool ENDS>
+__global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(SelectiveArgs args)
 {
     using G = Geometry<K>;
     constexpr int TILE = G::kTile, P = G::kPitch;
@@ -146,100 +270,123 @@ __global__ __launch_bounds__(kFwdWaves * 64) void selective_fwd_kernel(Selective
     const int N = (int)a.N, split = args.split, sets = kFwdWaves / split, channels = sets * kRows;
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *ly = lu + channels * P, *lB = ly + kFwdWaves * kRows * P, *lC = lB + kStateBlock * P;
-    float *lA = lC + kStateBlock * P, *lh = lA + channels * N;  // [N][channels] each
+    Carry *lh = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
 
     const int64_t per_group = a.channels / a.groups;
     const int64_t group = blockIdx.x / args.blocks, c0 = (blockIdx.x - group * args.blocks) * channels;  // c0: inside the group
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;  // first channel
-    const Stretch s = stretch_of(a, blockIdx.y);
+    const Stretch s = stretch_of<TILE>(a, blockIdx.y, args.parts);
+    if (ENDS && s.part == args.parts - 1) return;  // (nothing follows it)
+    const bool gated = !ENDS && a.z.p != nullptr;
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = lane >> 4, tl = lane & 15;
-    const int set = wave / split, part = wave % split;
-    const int ch = set * kRows + row;
+    const int part = wave % split, ch = wave / split * kRows + row;
 
     for (int i = threadIdx.x; i < channels * N; i += kThreads) {
         const int n = i / channels, c = i - n * channels;
-        const bool there = c < here;
-        const int64_t at = (first + c) * N + n;
-        lA[i] = there ? param(a.A, at) * kLog2e : 0.0f;
-        lh[i] = there && a.state_in != nullptr ? a.state_in[s.seq * a.channels * N + at] : 0.0f;
+        Carry q{0.0f, 0.0f};
+        if (c < here) {
+            const int64_t at = (first + c) * N + n;
+            q.A = param(a.A, at) * kLog2e;
+            if (!ENDS) {
+                if (a.state_in != nullptr) q.h = a.state_in[s.seq * a.channels * N + at];
+                q.h = carried(args, s, n, first + c, q.A, q.h, true);
+            }
+        }
+        lh[i] = q;
     }
 
-    // This thread's items on the way in and out: 4 channels at one token each.
+    // This thread's items on the way in and out: 4 channels at one token each. Tokens past the end and channels that are not there
+    // are read from places that are, and have no decay and add nothing.
     const int set_in = threadIdx.x % sets, c_in = set_in * kRows, count = (int)clamp_(here - c_in, 0, 4);
-    float bias[4], skip[4];
+    const int t_in = threadIdx.x / sets, t_step = kThreads / sets;
+    const uint32_t c_from = count > 0 ? c_in : 0;
+    const int c_count = count > 0 ? count : here;
+    const bool whole = here % 4 == 0;
+    float bias[4], skip[4], sum_d[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         bias[i] = i < count ? param(a.dt_bias, first + c_in + i) : 0.0f;
         skip[i] = i < count ? param(a.D, first + c_in + i) : 0.0f;
     }
-    int64_t tile = first_tile<TILE>(a, s);
-    for (int64_t t0 = s.start; t0 < s.end; t0 += TILE, tile++) {
-        const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
-        float x[kItems][4], z[kItems][4];
+    Quad<ST> x[kItems], dt[kItems], z[kItems];
+    StateInputs<ST, TILE, kThreads> bc;
+    auto fetch = [&](int64_t t0) {
+        const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE), t_mine = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
-            const int t = threadIdx.x / sets + j * (kThreads / sets);
-            if (t >= TILE) continue;
-            float d[4];
-            const bool there = t < length && count > 0;
+            const uint32_t t = t_mine + j * t_step < length ? t_mine + j * t_step : length - 1;
+            x[j].load(token_at<ST>(a.x, s.batch, t0, first), t * (uint32_t)a.x.token + c_from, c_count, whole);
+            dt[j].load(token_at<ST>(a.dt, s.batch, t0, first), t * (uint32_t)a.dt.token + c_from, c_count, whole);
+            if (gated) z[j].load(token_at<ST>(a.z, s.batch, t0, first), t * (uint32_t)a.z.token + c_from, c_count, whole);
+        }
+        bc.load(a, s.batch, group, t0, length, 0);
+    };
+    if (s.start < s.end) fetch(s.start);
+    int64_t tile = s.tile;
+    for (int64_t t0 = s.start; t0 < s.end; t0 += TILE, tile++) {
+        const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
+        Quad<ST> x_now[kItems], z_now[kItems];
+        const int t_mine = again(t_in);
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[j][i] = z[j][i] = d[i] = 0.0f;
-            if (there) {
-                load_part(token_at<ST>(a.x, s.batch, t0 + t, first + c_in), count, x[j]);
-                load_part(token_at<ST>(a.dt, s.batch, t0 + t, first + c_in), count, d);
-                if (a.z.p != nullptr) load_part(token_at<ST>(a.z, s.batch, t0 + t, first + c_in), count, z[j]);
-            }
+        for (int j = 0; j < kItems; j++) {
+            const int t = t_mine + j * t_step;
+            x_now[j] = x[j];
+            z_now[j] = z[j];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                // (tokens past the end and channels that are not there: no decay, nothing added)
-                d[i] = there && i < count ? (a.softplus ? softplus_(d[i] + bias[i]) : d[i] + bias[i]) : 0.0f;
-                ld[(c_in + i) * P + G::place(t)] = d[i];
-                lu[(c_in + i) * P + G::place(t)] = d[i] * x[j][i];
+                const float raw = dt[j][i] + bias[i];
+                float d = a.softplus ? softplus_(raw) : raw, u = d * x[j][i];
+                const bool there = t < length && i < count;
+                d = there ? d : 0.0f;
+                u = there ? u : 0.0f;
+                if (ENDS) sum_d[i] += d;
+                if (t < TILE) {
+                    ld[(c_in + i) * P + G::place(t)] = d;
+                    lu[(c_in + i) * P + G::place(t)] = u;
+                }
             }
         }
         float y[K] = {};
         for (int n0 = 0; n0 < N; n0 += kStateBlock) {
             const int states = N - n0 < kStateBlock ? N - n0 : kStateBlock;
             if (n0 > 0) __syncthreads();
-            for (int i = threadIdx.x; i < TILE * kStateBlock; i += kThreads) {
-                const int n = i % kStateBlock, t = i / kStateBlock;
-                const bool there = t < length && n < states;
-                lB[n * P + G::place(t)] = there ? (float)token_at<ST>(a.B, s.batch, t0 + t, group * a.B.group + n0 + n)[0] : 0.0f;
-                lC[n * P + G::place(t)] = there ? (float)token_at<ST>(a.C, s.batch, t0 + t, group * a.C.group + n0 + n)[0] : 0.0f;
-            }
+            bc.template store<G>(lB, lC, length, states);
             __syncthreads();
-            if (n0 == 0 && a.saved != nullptr) {
+            if (!ENDS && n0 == 0 && a.saved != nullptr) {
                 // The states that this tile starts from, [tile][N][channels]; the barriers around keep them from moving on.
                 float *to = static_cast<float *>(a.saved) + tile * N * a.channels + first;
                 for (int i = threadIdx.x; i < channels * N; i += kThreads) {
                     const int n = i / channels, c = i - n * channels;
-                    if (c < here) to[(int64_t)n * a.channels + c] = lh[i];
+                    if (c < here) to[(int64_t)n * a.channels + c] = lh[i].h;
                 }
                 __syncthreads();
             }
+            if (n0 + kStateBlock < N) bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
+            else if (t0 + TILE < s.end) fetch(t0 + TILE);
             float d[K], u[K], total = 0.0f;
             G::read(ld + ch * P, tl, d);
             G::read(lu + ch * P, tl, u);
 #pragma unroll
             for (int k = 0; k < K; k++) total += d[k];
             for (int n = part; n < states; n += split) {
-                float *carry = lh + (n0 + n) * channels + ch;
-                const float A = lA[(n0 + n) * channels + ch], h0 = *carry;
+                Carry *carry = lh + (n0 + n) * channels + ch;
+                const Carry c = *carry;
                 float e[K], b[K];
                 G::read(lB + n * P, tl, b);
-                float h = tl == 0 ? h0 : 0.0f;
+                float h = tl == 0 ? c.h : 0.0f;
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    e[k] = __builtin_amdgcn_exp2f(d[k] * A);
+                    e[k] = __builtin_amdgcn_exp2f(d[k] * c.A);
                     b[k] *= u[k];
                     h = __builtin_fmaf(e[k], h, b[k]);
                 }
-                float decay = finite_(__builtin_amdgcn_exp2f(total * A));
+                float decay = __builtin_amdgcn_exp2f(total * c.A);
                 row_scan<true>(decay, h);
-                if (tl == kTimeLanes - 1) *carry = h;
-                h = row_prev(h, h0);
+                if (tl == kTimeLanes - 1) carry->h = h;
+                if (ENDS) continue;
+                h = row_prev(h, c.h);
                 float C[K];
                 G::read(lC + n * P, tl, C);
 #pragma unroll
@@ -249,85 +396,111 @@ __global__ __launch_bounds__(kFwdWaves * 64) void selective_fwd_kernel(Selective
                 }
             }
         }
-        G::write(ly + (part * channels + ch) * P, tl, y);
+        if (!ENDS) G::write(ly + (part * channels + ch) * P, tl, y);
         __syncthreads();
+        if (ENDS) continue;
+        const int t_out = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
-            const int t = threadIdx.x / sets + j * (kThreads / sets);
+            const int t = t_out + j * t_step;
             if (t >= length || count <= 0) continue;
             float out[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float v = skip[i] * x[j][i];
+                float v = skip[i] * x_now[j][i];
                 for (int q = 0; q < split; q++) v += ly[(q * channels + c_in + i) * P + G::place(t)];
-                out[i] = a.z.p != nullptr ? v * (z[j][i] * sigmoid_(z[j][i])) : v;
+                out[i] = gated ? v * (z_now[j][i] * sigmoid_(z_now[j][i])) : v;
             }
-            store_some(const_cast<ST *>(token_at<ST>(a.y, s.batch, t0 + t, first + c_in)), count, out);
+            store_quad(const_cast<ST *>(token_at<ST>(a.y, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.y.token + c_from, count, whole, out);
         }
     }
-    if (a.state_out == nullptr) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < channels * N; i += kThreads) {
-        const int c = i / N, n = i - c * N;
-        if (c < here) a.state_out[(s.seq * a.channels + first + c) * N + n] = lh[n * channels + c];
+    if (ENDS) {
+        float *to = args.ends + (s.seq * args.parts + s.part) * (N + 1) * a.channels + first;
+        for (int i = threadIdx.x; i < channels * N; i += kThreads) {
+            const int n = i / channels, c = i - n * channels;
+            if (c < here) to[(int64_t)n * a.channels + c] = lh[i].h;
+        }
+        // The sum of d, over the threads of a channel in order.
+        float *red = lds;  // [threads a set][channels]
+#pragma unroll
+        for (int i = 0; i < 4; i++) red[t_in * channels + c_in + i] = sum_d[i];
+        __syncthreads();
+        if ((int)threadIdx.x < here) {
+            float sum = 0.0f;
+            for (int t = 0; t < t_step; t++) sum += red[t * channels + threadIdx.x];
+            to[(int64_t)N * a.channels + threadIdx.x] = sum;
+        }
+    } else if (a.state_out != nullptr && s.part == args.parts - 1) {
+        for (int i = threadIdx.x; i < channels * N; i += kThreads) {
+            const int c = i / N, n = i - c * N;
+            if (c < here) a.state_out[(s.seq * a.channels + first + c) * N + n] = lh[n * channels + c].h;
+        }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Backwards. A workgroup of 4 waves takes 16 channels back through a stretch. The sums over n (s1, s2, v) belong to a channel, the
 // sums over channels (gB, gC) to a state: a wave keeps the latter for its 4 of 16 states in registers while it goes over the
-// 4 groups of channels, and the former are added up in LDS, where in every step each group of channels is one wave's alone.
+// 4 groups of channels, and the former are added up in LDS, where in every step each group of channels is one wave's alone. With
+// ENDS only the gradient at the stretch's start is found, from zeros.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kBwdWaves = 4, kBwdChannels = kBwdWaves * kRows, kBwdStates = kStateBlock / kBwdWaves;
 
-struct BackwardArgs {
-    SelectiveArgs f;
-    float *bc;     // [blocks of all groups][tokens][2][N]: sums of gB and gC over a workgroup's channels
-    float *sums;   // [stretches][channels][N + 2]: sums over a stretch's tokens for A, D and dt_bias
-};
-
 template <int K> struct BackwardLds {
     using G = Geometry<K>;
-    // d, u, g0 and s1, s2, v; B and C; A, the states' and the gradients' carries and the sums for A
+    // d, u, g0 and s1, s2, v; B and C; A and the gradients' carries, the states and the sums for A
     static __host__ __device__ constexpr int words(int N)
     {
         return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 4 * kBwdChannels * N;
     }
 };
 
-template <typename ST, int K>
-__global__ __launch_bounds__(kBwdWaves * 64) void selective_bwd_kernel(BackwardArgs args)
+template <typename ST, int K, bool ENDS>
+__global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(SelectiveArgs args)
 {
     using G = Geometry<K>;
     constexpr int TILE = G::kTile, P = G::kPitch, channels = kBwdChannels;
     constexpr int kThreads = kBwdWaves * 64, kItems = kBwdWaves * TILE / kThreads;
-    const scanscam_selective &a = args.f.a;
+    const scanscam_selective &a = args.a;
     const int N = (int)a.N;
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *lg = lu + channels * P;
     float *l1 = lg + channels * P, *l2 = l1 + channels * P, *lv = l2 + channels * P;
     float *lB = lv + channels * P, *lC = lB + kStateBlock * P;
-    float *lA = lC + kStateBlock * P, *lh = lA + channels * N, *lG = lh + channels * N, *lS = lG + channels * N;  // [N][channels]
+    Carry *lG = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
+    float *lh = reinterpret_cast<float *>(lG + channels * N), *lS = lh + channels * N;
 
     const int64_t per_group = a.channels / a.groups;
-    const int64_t group = blockIdx.x / args.f.blocks, c0 = (blockIdx.x - group * args.f.blocks) * channels;
+    const int64_t group = blockIdx.x / args.blocks, c0 = (blockIdx.x - group * args.blocks) * channels;
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;
-    const Stretch s = stretch_of(a, blockIdx.y);
+    const Stretch s = stretch_of<TILE>(a, blockIdx.y, args.parts);
+    if (ENDS && s.part == 0) return;
     const bool gated = a.z.p != nullptr;
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = lane >> 4, tl = lane & 15;
 
     for (int i = threadIdx.x; i < channels * N; i += kThreads) {
         const int n = i / channels, c = i - n * channels;
-        const bool there = c < here;
-        const int64_t at = (first + c) * N + n;
-        lA[i] = there ? param(a.A, at) * kLog2e : 0.0f;
-        lG[i] = there && a.gstate_out != nullptr ? a.gstate_out[s.seq * a.channels * N + at] : 0.0f;
+        Carry q{0.0f, 0.0f};
+        if (c < here) {
+            const int64_t at = (first + c) * N + n;
+            q.A = param(a.A, at) * kLog2e;
+            if (!ENDS) {
+                if (a.gstate_out != nullptr) q.h = a.gstate_out[s.seq * a.channels * N + at];
+                q.h = carried(args, s, n, first + c, q.A, q.h, false);
+            }
+        }
+        lG[i] = q;
         lS[i] = 0.0f;
     }
 
     const int set_in = threadIdx.x % kBwdWaves, c_in = set_in * kRows, count = (int)clamp_(here - c_in, 0, 4);
+    const int t_in = threadIdx.x / kBwdWaves, t_step = kThreads / kBwdWaves;
+    const uint32_t c_from = count > 0 ? c_in : 0;
+    const int c_count = count > 0 ? count : here;
+    const bool whole = here % 4 == 0;
     float bias[4], skip[4], sum_skip[4] = {}, sum_bias[4] = {};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -335,59 +508,75 @@ __global__ __launch_bounds__(kBwdWaves * 64) void selective_bwd_kernel(BackwardA
         skip[i] = i < count ? param(a.D, first + c_in + i) : 0.0f;
     }
     const int64_t tiles = (s.end - s.start + TILE - 1) / TILE;
+    Quad<ST> x[kItems], dt[kItems], gy[kItems], z[kItems];
+    StateInputs<ST, TILE, kThreads> bc;
+    auto fetch = [&](int64_t t0) {
+        const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE), t_mine = again(t_in);
+#pragma unroll
+        for (int j = 0; j < kItems; j++) {
+            const uint32_t t = t_mine + j * t_step < length ? t_mine + j * t_step : length - 1;
+            x[j].load(token_at<ST>(a.x, s.batch, t0, first), t * (uint32_t)a.x.token + c_from, c_count, whole);
+            dt[j].load(token_at<ST>(a.dt, s.batch, t0, first), t * (uint32_t)a.dt.token + c_from, c_count, whole);
+            gy[j].load(token_at<ST>(a.gy, s.batch, t0, first), t * (uint32_t)a.gy.token + c_from, c_count, whole);
+            if (gated) z[j].load(token_at<ST>(a.z, s.batch, t0, first), t * (uint32_t)a.z.token + c_from, c_count, whole);
+        }
+        bc.load(a, s.batch, group, t0, length, 0);
+    };
+    if (tiles > 0) fetch(s.start + (tiles - 1) * TILE);
     for (int64_t tile = tiles - 1; tile >= 0; tile--) {
         const int64_t t0 = s.start + tile * TILE;
         const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
-        const float *from = static_cast<const float *>(a.saved) + (first_tile<TILE>(a, s) + tile) * N * a.channels + first;
         __syncthreads();
-        for (int i = threadIdx.x; i < channels * N; i += kThreads) {
-            const int n = i / channels, c = i - n * channels;
-            lh[i] = c < here ? from[(int64_t)n * a.channels + c] : 0.0f;
+        if (!ENDS) {
+            const float *from = static_cast<const float *>(a.saved) + (s.tile + tile) * N * a.channels + first;
+            for (int i = threadIdx.x; i < channels * N; i += kThreads) {
+                const int n = i / channels, c = i - n * channels;
+                lh[i] = c < here ? from[(int64_t)n * a.channels + c] : 0.0f;
+            }
         }
-        float x[kItems][4], raw[kItems][4], d[kItems][4], z[kItems][4], gy[kItems][4];
+        Quad<ST> x_now[kItems], dt_now[kItems], gy_now[kItems], z_now[kItems];
+        const int t_mine = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
-            const int t = threadIdx.x / kBwdWaves + j * (kThreads / kBwdWaves);
-            const bool there = t < length && count > 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[j][i] = raw[j][i] = z[j][i] = gy[j][i] = 0.0f;
-            if (there) {
-                load_part(token_at<ST>(a.x, s.batch, t0 + t, first + c_in), count, x[j]);
-                load_part(token_at<ST>(a.dt, s.batch, t0 + t, first + c_in), count, raw[j]);
-                load_part(token_at<ST>(a.gy, s.batch, t0 + t, first + c_in), count, gy[j]);
-                if (gated) load_part(token_at<ST>(a.z, s.batch, t0 + t, first + c_in), count, z[j]);
-            }
+            const int t = t_mine + j * t_step;
+            x_now[j] = x[j];
+            dt_now[j] = dt[j];
+            gy_now[j] = gy[j];
+            z_now[j] = z[j];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                raw[j][i] += bias[i];
-                d[j][i] = there && i < count ? (a.softplus ? softplus_(raw[j][i]) : raw[j][i]) : 0.0f;
+                const float raw = dt[j][i] + bias[i];
+                float d = a.softplus ? softplus_(raw) : raw, u = d * x[j][i], g = gated ? gy[j][i] * (z[j][i] * sigmoid_(z[j][i])) : gy[j][i];
+                const bool there = t < length && i < count;
                 const int at = (c_in + i) * P + G::place(t);
-                ld[at] = d[j][i];
-                lu[at] = d[j][i] * x[j][i];
-                lg[at] = gated ? gy[j][i] * (z[j][i] * sigmoid_(z[j][i])) : gy[j][i];
-                l1[at] = l2[at] = lv[at] = 0.0f;
+                ld[at] = there ? d : 0.0f;
+                lu[at] = there ? u : 0.0f;
+                lg[at] = there ? g : 0.0f;
+                if (!ENDS) l1[at] = l2[at] = lv[at] = 0.0f;
+                else sum_bias[i] += there ? d : 0.0f;
             }
         }
         for (int n0 = 0; n0 < N; n0 += kStateBlock) {
             const int states = N - n0 < kStateBlock ? N - n0 : kStateBlock;
             if (n0 > 0) __syncthreads();
-            for (int i = threadIdx.x; i < TILE * kStateBlock; i += kThreads) {
-                const int n = i % kStateBlock, t = i / kStateBlock;
-                const bool there = t < length && n < states;
-                lB[n * P + G::place(t)] = there ? (float)token_at<ST>(a.B, s.batch, t0 + t, group * a.B.group + n0 + n)[0] : 0.0f;
-                lC[n * P + G::place(t)] = there ? (float)token_at<ST>(a.C, s.batch, t0 + t, group * a.C.group + n0 + n)[0] : 0.0f;
-            }
+            bc.template store<G>(lB, lC, length, states);
             float gB[kBwdStates][K] = {}, gC[kBwdStates][K] = {};
             for (int step = 0; step < kBwdWaves; step++) {
                 __syncthreads();
+                if (step == 0) {
+                    if (n0 + kStateBlock < N) bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
+                    else if (tile > 0) fetch(t0 - TILE);
+                }
                 const int ch = ((wave + step) % kBwdWaves) * kRows + row;
                 float d[K], u[K], g0[K], s1[K], s2[K], v[K], total = 0.0f;
                 G::read(ld + ch * P, tl, d);
-                G::read(lu + ch * P, tl, u);
                 G::read(lg + ch * P, tl, g0);
-                G::read(l1 + ch * P, tl, s1);
-                G::read(l2 + ch * P, tl, s2);
-                G::read(lv + ch * P, tl, v);
+                if (!ENDS) {
+                    G::read(lu + ch * P, tl, u);
+                    G::read(l1 + ch * P, tl, s1);
+                    G::read(l2 + ch * P, tl, s2);
+                    G::read(lv + ch * P, tl, v);
+                }
 #pragma unroll
                 for (int k = 0; k < K; k++) total += d[k];
 #pragma unroll
@@ -395,26 +584,30 @@ __global__ __launch_bounds__(kBwdWaves * 64) void selective_bwd_kernel(BackwardA
                     const int n = wave * kBwdStates + q;
                     if (n >= states) continue;
                     const int at = (n0 + n) * channels + ch;
-                    const float A = lA[at], h0 = lh[at], G0 = lG[at];
+                    const Carry c = lG[at];
                     float e[K], h[K], B[K], C[K];
-                    G::read(lB + n * P, tl, B);
                     G::read(lC + n * P, tl, C);
-                    float fold = tl == 0 ? h0 : 0.0f, back = tl == kTimeLanes - 1 ? G0 : 0.0f;
+                    float back = tl == kTimeLanes - 1 ? c.h : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < K; k++) e[k] = __builtin_amdgcn_exp2f(d[k] * c.A);
+#pragma unroll
+                    for (int k = K - 1; k >= 0; k--) back = e[k] * __builtin_fmaf(g0[k], C[k], back);
+                    const float decay = __builtin_amdgcn_exp2f(total * c.A);
+                    float a2 = decay;
+                    row_scan<false>(a2, back);
+                    if (tl == 0) lG[at].h = back;
+                    if (ENDS) continue;
+                    const float h0 = lh[at];
+                    G::read(lB + n * P, tl, B);
+                    float fold = tl == 0 ? h0 : 0.0f, a1 = decay;
 #pragma unroll
                     for (int k = 0; k < K; k++) {
-                        e[k] = __builtin_amdgcn_exp2f(d[k] * A);
                         h[k] = u[k] * B[k];
                         fold = __builtin_fmaf(e[k], fold, h[k]);
                     }
-#pragma unroll
-                    for (int k = K - 1; k >= 0; k--) back = e[k] * __builtin_fmaf(g0[k], C[k], back);
-                    const float decay = finite_(__builtin_amdgcn_exp2f(total * A));
-                    float a1 = decay, a2 = decay;
                     row_scan<true>(a1, fold);
-                    row_scan<false>(a2, back);
-                    if (tl == 0) lG[at] = back;
                     const float before = row_prev(fold, h0);
-                    float g = row_next(back, G0);
+                    float g = row_next(back, c.h);
                     float state = before;
 #pragma unroll
                     for (int k = 0; k < K; k++) {
@@ -431,82 +624,95 @@ __global__ __launch_bounds__(kBwdWaves * 64) void selective_bwd_kernel(BackwardA
                         s1[k] = __builtin_fmaf(B[k], g, s1[k]);
                         g *= e[k];
                         const float r = g * (k > 0 ? h[k - 1] : before);
-                        s2[k] = __builtin_fmaf(A, r, s2[k]);
+                        s2[k] = __builtin_fmaf(c.A, r, s2[k]);
                         sum = __builtin_fmaf(d[k], r, sum);
                     }
                     sum = row_sum(sum);
                     if (tl == kTimeLanes - 1) lS[at] += sum;
                 }
+                if (ENDS) continue;
                 G::write(l1 + ch * P, tl, s1);
                 G::write(l2 + ch * P, tl, s2);
                 G::write(lv + ch * P, tl, v);
             }
-            // gB and gC over the 4 channels of the rows: lanes 0-15 end up with the first, ... of every four values.
+            if (ENDS) continue;
+            // gB and gC over the 4 channels of the rows, into the places of B and C (a state's are one wave's alone), and out.
 #pragma unroll
             for (int q = 0; q < kBwdStates; q++) {
-                const int n = wave * kBwdStates + q;
+                const int at = (wave * kBwdStates + q) * P + tl * 4 + row;
 #pragma unroll
-                for (int k = 0; k < K; k++) {
-                    float b = gB[q][k], c = gC[q][k];
-                    b += __shfl_xor(b, 16);
-                    b += __shfl_xor(b, 32);
-                    c += __shfl_xor(c, 16);
-                    c += __shfl_xor(c, 32);
-                    const int t = tl * K + k;
-                    if (row == 0 && n < states && t < length) {
-                        float *to = args.bc + (((int64_t)blockIdx.x * a.batch + s.batch) * a.T + t0 + t) * 2 * N + n0 + n;
-                        to[0] = b;
-                        to[N] = c;
-                    }
+                for (int m = 0; m < K / 4; m++) {
+                    lB[at + m * G::kLine] = rows_sum(gB[q][4 * m], gB[q][4 * m + 1], gB[q][4 * m + 2], gB[q][4 * m + 3]);
+                    lC[at + m * G::kLine] = rows_sum(gC[q][4 * m], gC[q][4 * m + 1], gC[q][4 * m + 2], gC[q][4 * m + 3]);
                 }
             }
+            __syncthreads();
+            float *to = args.bc + (((int64_t)blockIdx.x * a.batch + s.batch) * a.T + t0) * 2 * N + n0;
+            const int thread = again((int)threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < TILE * 2 * kStateBlock / 4 / kThreads; j++) {
+                const int i = thread + j * kThreads, n = i % 4 * 4, which = i / 4 % 2, t = i / 8;
+                const float *from = (which ? lC : lB) + n * P + G::place(t);
+                const float f[4] = {from[0], from[P], from[2 * P], from[3 * P]};
+                if (t < length && n < states) store_quad(to, (uint32_t)((2 * t + which) * N + n), states - n, states - n >= 4, f);
+            }
         }
-        __syncthreads();
+        if (ENDS) continue;
+        const int t_out = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
-            const int t = threadIdx.x / kBwdWaves + j * (kThreads / kBwdWaves);
+            const int t = t_out + j * t_step;
             if (t >= length || count <= 0) continue;
             float gx[4], gd[4], gz[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int at = (c_in + i) * P + G::place(t);
-                const float s1 = l1[at], s2 = l2[at] * (1.0f / kLog2e), v = lv[at] + skip[i] * x[j][i], g0 = lg[at];
-                gx[i] = __builtin_fmaf(d[j][i], s1, skip[i] * g0);
-                gd[i] = __builtin_fmaf(x[j][i], s1, s2);
-                if (a.softplus) gd[i] *= sigmoid_(raw[j][i]);
-                sum_skip[i] = __builtin_fmaf(g0, x[j][i], sum_skip[i]);
+                const float xi = x_now[j][i], zi = z_now[j][i];
+                const float s1 = l1[at], s2 = l2[at] * (1.0f / kLog2e), v = __builtin_fmaf(skip[i], xi, lv[at]), g0 = lg[at];
+                gx[i] = __builtin_fmaf(ld[at], s1, skip[i] * g0);
+                gd[i] = __builtin_fmaf(xi, s1, s2);
+                if (a.softplus) gd[i] *= sigmoid_(dt_now[j][i] + bias[i]);
+                sum_skip[i] = __builtin_fmaf(g0, xi, sum_skip[i]);
                 sum_bias[i] += gd[i];
-                const float sg = sigmoid_(z[j][i]);
-                gz[i] = gy[j][i] * v * (sg * __builtin_fmaf(z[j][i], 1.0f - sg, 1.0f));
+                if (gated) {
+                    const float sg = sigmoid_(zi);
+                    gz[i] = gy_now[j][i] * v * (sg * __builtin_fmaf(zi, 1.0f - sg, 1.0f));
+                }
             }
-            store_some(const_cast<ST *>(token_at<ST>(a.gx, s.batch, t0 + t, first + c_in)), count, gx);
-            store_some(const_cast<ST *>(token_at<ST>(a.gdt, s.batch, t0 + t, first + c_in)), count, gd);
-            if (gated) store_some(const_cast<ST *>(token_at<ST>(a.gz, s.batch, t0 + t, first + c_in)), count, gz);
+            store_quad(const_cast<ST *>(token_at<ST>(a.gx, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gx.token + c_from, count, whole, gx);
+            store_quad(const_cast<ST *>(token_at<ST>(a.gdt, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gdt.token + c_from, count, whole, gd);
+            if (gated) store_quad(const_cast<ST *>(token_at<ST>(a.gz, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gz.token + c_from, count, whole, gz);
         }
     }
     __syncthreads();
+    float *to = ENDS ? args.ends + (s.seq * args.parts + s.part) * (N + 1) * a.channels + first
+                     : args.sums + (s.seq * args.parts + s.part) * (N + 2) * a.channels + first * N;
     for (int i = threadIdx.x; i < channels * N; i += kThreads) {
-        const int c = i / N, n = i - c * N;
-        if (c >= here) continue;
-        const int64_t at = (s.seq * a.channels + first + c) * N + n;
-        if (a.gstate_in != nullptr) a.gstate_in[at] = lG[n * channels + c];
-        args.sums[(s.seq * (N + 2)) * a.channels + (first + c) * N + n] = lS[n * channels + c];
+        if (ENDS) {
+            const int n = i / channels, c = i - n * channels;
+            if (c < here) to[(int64_t)n * a.channels + c] = lG[i].h;
+        } else {
+            const int c = i / N, n = i - c * N;
+            if (c >= here) continue;
+            if (a.gstate_in != nullptr && s.part == 0) a.gstate_in[(s.seq * a.channels + first + c) * N + n] = lG[n * channels + c].h;
+            to[i] = lS[n * channels + c];
+        }
     }
-    // D's and the bias's: over the threads of a channel, through the tokens' rows (64 threads a set of 4 channels).
-    __syncthreads();
+    // D's and the bias's (ENDS: the sum of d): over the threads of a channel, in order.
     float *red = lds;  // [64][2][channels]
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int t = threadIdx.x / kBwdWaves;
-        red[(t * 2 + 0) * channels + c_in + i] = sum_skip[i];
-        red[(t * 2 + 1) * channels + c_in + i] = sum_bias[i];
+        red[(t_in * 2 + 0) * channels + c_in + i] = sum_skip[i];
+        red[(t_in * 2 + 1) * channels + c_in + i] = sum_bias[i];
     }
     __syncthreads();
     if (threadIdx.x < 2 * channels) {
         const int which = threadIdx.x / channels, c = threadIdx.x % channels;
         float sum = 0.0f;
-        for (int t = 0; t < 64; t++) sum += red[(t * 2 + which) * channels + c];
-        if (c < here) args.sums[(s.seq * (N + 2) + N + which) * a.channels + first + c] = sum;
+        for (int t = 0; t < t_step; t++) sum += red[(t * 2 + which) * channels + c];
+        if (c >= here) return;
+        if (!ENDS) args.sums[((s.seq * args.parts + s.part) * (N + 2) + N + which) * a.channels + first + c] = sum;
+        else if (which == 1) to[(int64_t)N * a.channels + c] = sum;
     }
 }
 

@@ -22,7 +22,7 @@ from . import baseline, hip
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _EIGHT = {torch.int8: 16, torch.float8_e4m3fn: 17}
 _ACTIVATIONS = {None: 0, "silu": 1}
-_MOST_STATES, _MOST_TAPS, _MOST_NORM_CHANNELS = 256, 8, 32768
+_MOST_STATES, _MOST_TAPS, _MOST_NORM_CHANNELS, _MOST_TOKEN_STRIDE = 256, 8, 32768, 1 << 22
 
 _p, _i32, _i64, _f32, _size = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -71,6 +71,8 @@ class _Norm(ctypes.Structure):
 
 
 _entry_points = None
+# Parts of time that the selective scan's workgroups share a sequence out in; 0: the library chooses (the tests force others).
+_parts = 0
 
 
 def _lib():
@@ -171,6 +173,12 @@ def _unit(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t.contiguous()
 
 
+def _near(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The same for the selective scan of whole sequences, whose kernels take tokens at most so far apart."""
+    t = _unit(t)
+    return t if t is None or t.stride(1) < _MOST_TOKEN_STRIDE else t.contiguous()
+
+
 def _tokens(t: Optional[torch.Tensor], lead: int = 2) -> _Tokens:
     """``lead``: 2 for [batch, T, ...], 1 for [rows, ...]."""
     if t is None:
@@ -255,7 +263,7 @@ def _selective_args(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus) -> 
     a.sequences = x.shape[0] if offsets is None else offsets.shape[0] - 1
     a.groups, a.N = B.shape[2], A.shape[1]
     a.offsets, a.offsets64 = _ptr(offsets), int(offsets is not None and offsets.dtype == torch.int64)
-    a.dtype, a.softplus = _TYPES[x.dtype], int(softplus)
+    a.dtype, a.softplus, a.parts = _TYPES[x.dtype], int(softplus), _parts
     a.x, a.dt, a.B, a.C, a.z = (_tokens(t) for t in (x, dt, B, C, z))
     a.A, a.D, a.dt_bias = _param(A), _param(D), _param(dt_bias)
     a.state_in = _ptr(state)
@@ -266,7 +274,7 @@ def _selective_forward(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus, 
     """``(y, new state or None, saved or None, the tensors as the library saw them)``."""
     L = _lib()
     with hip._on(x.device):
-        seen = tuple(_unit(t) for t in (x, dt)) + (_dense(A), _unit(B), _unit(C), _dense(D), _unit(z), _dense(dt_bias), _dense(state), _dense(offsets))
+        seen = (_near(x), _near(dt), _dense(A), _near(B), _near(C), _dense(D), _near(z), _dense(dt_bias), _dense(state), _dense(offsets))
         a = _selective_args(*seen, softplus)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         a.y = _tokens(y)
@@ -303,7 +311,7 @@ class SelectiveScan(torch.autograd.Function):
             return (None,) * 12
         L = _lib()
         with hip._on(x.device):
-            gy = _unit(gy) if gy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
+            gy = _near(gy) if gy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
             gnew = _dense(gnew)
             a = _selective_args(*seen, ctx.softplus)
             new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=x.device)  # noqa: E731

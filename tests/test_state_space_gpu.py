@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import scanscam_amd as f
-from scanscam_amd import baseline
+from scanscam_amd import baseline, state_space
 
 pytestmark = pytest.mark.gpu
 
@@ -71,12 +71,14 @@ SCANS = [
     (torch.bfloat16, 0, 0, 64, 16, {"lengths": [128, 5, 0, 300], "state": True}),
     (torch.bfloat16, 1, 33, 31, 8, {"param": torch.bfloat16}),
     (torch.float16, 2, 140, 48, 16, {"param": torch.float16}),
+    (torch.float32, 1, 1500, 9, 16, {"state": True}),
 ]
 
 
 @pytest.mark.parametrize("dtype,batch,T,D,N,more", SCANS, ids=lambda v: str(v).replace("torch.", "").replace(" ", ""))
-@pytest.mark.parametrize("softplus", [True, False])
-def test_scan_and_gradients(gpu, dtype, batch, T, D, N, more, softplus):
+@pytest.mark.parametrize("softplus,parts", [(True, 0), (False, 0), (True, 2), (True, 5)])
+def test_scan_and_gradients(gpu, monkeypatch, dtype, batch, T, D, N, more, softplus, parts):
+    monkeypatch.setattr(state_space, "_parts", parts)  # parts of time to share out, also where there is less than a tile for each
     v = make_scan(5, dtype, batch, T, D, N, **more)
     if not softplus:  # step sizes themselves
         v["dt"] = (v["dt"].float().abs() * 0.2).to(dtype)

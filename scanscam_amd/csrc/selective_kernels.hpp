@@ -207,18 +207,49 @@ template <typename ST, int TILE, int THREADS> struct StateInputs {
     template <typename G> __device__ __forceinline__ void store(float *lB, float *lC, int length, int states) const
     {
         const int thread = again((int)threadIdx.x), n = thread % kQuads * 4;
+        const bool full = length == TILE && states == kStateBlock;
 #pragma unroll
         for (int j = 0; j < kCount; j++) {
-            const int t = (thread + j * THREADS) / kQuads;
+            const int t = (thread + j * THREADS) / kQuads, at = n * G::kPitch + G::place(t);
+            float b[4], c[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const bool there = t < length && n + k < states;
-                lB[(n + k) * G::kPitch + G::place(t)] = there ? B[j][k] : 0.0f;
-                lC[(n + k) * G::kPitch + G::place(t)] = there ? C[j][k] : 0.0f;
+                b[k] = B[j][k];
+                c[k] = C[j][k];
+            }
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const bool there = t < length && n + k < states;
+                    b[k] = there ? b[k] : 0.0f;
+                    c[k] = there ? c[k] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                lB[at + k * G::kPitch] = b[k];
+                lC[at + k * G::kPitch] = c[k];
             }
         }
     }
 };
+
+// Step sizes of a thread's items from what is stored: four channels at a token each. (The branches are the same for all lanes and
+// stand outside of the loops, which then run without them.)
+template <typename ST, int ITEMS>
+__device__ __forceinline__ void step_sizes(const Quad<ST> (&dt)[ITEMS], const float (&bias)[4], bool softplus, float (&d)[ITEMS][4])
+{
+#pragma unroll
+    for (int j = 0; j < ITEMS; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[j][i] = dt[j][i] + bias[i];
+    if (softplus) {
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[j][i] = softplus_(d[j][i]);
+    }
+}
 
 struct SelectiveArgs {
     scanscam_selective a;
@@ -253,10 +284,10 @@ constexpr int kFwdWaves = 8;
 template <int K> struct ForwardLds {
     using G = Geometry<K>;
     static constexpr int kSums = kFwdWaves * kRows;  // channels x split: rows of sums over n
-    // floats: d and u of the channels, sums, B and C; then A and the carries of all states
+    // floats: d and u of the channels, sums, B and C; A and the carries of all states; where lanes write that have nothing to say
     static __host__ __device__ constexpr int words(int channels, int N)
     {
-        return 2 * channels * G::kPitch + kSums * G::kPitch + 2 * kStateBlock * G::kPitch + 2 * channels * N;
+        return 2 * channels * G::kPitch + kSums * G::kPitch + 2 * kStateBlock * G::kPitch + 2 * channels * N + 2;
     }
 };
 
@@ -270,7 +301,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     const int N = (int)a.N, split = args.split, sets = kFwdWaves / split, channels = sets * kRows;
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *ly = lu + channels * P, *lB = ly + kFwdWaves * kRows * P, *lC = lB + kStateBlock * P;
-    Carry *lh = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
+    Carry *lh = reinterpret_cast<Carry *>(lC + kStateBlock * P), *nowhere = lh + channels * N;  // [N][channels]
 
     const int64_t per_group = a.channels / a.groups;
     const int64_t group = blockIdx.x / args.blocks, c0 = (blockIdx.x - group * args.blocks) * channels;  // c0: inside the group
@@ -329,23 +360,35 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
         const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
         Quad<ST> x_now[kItems], z_now[kItems];
         const int t_mine = again(t_in);
+        const bool full = length == TILE && here == channels;
+        float d_in[kItems][4], u_in[kItems][4];
+        step_sizes(dt, bias, a.softplus, d_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
-            const int t = t_mine + j * t_step;
             x_now[j] = x[j];
             z_now[j] = z[j];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float raw = dt[j][i] + bias[i];
-                float d = a.softplus ? softplus_(raw) : raw, u = d * x[j][i];
-                const bool there = t < length && i < count;
-                d = there ? d : 0.0f;
-                u = there ? u : 0.0f;
-                if (ENDS) sum_d[i] += d;
-                if (t < TILE) {
-                    ld[(c_in + i) * P + G::place(t)] = d;
-                    lu[(c_in + i) * P + G::place(t)] = u;
+            for (int i = 0; i < 4; i++) u_in[j][i] = d_in[j][i] * x[j][i];
+        }
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < kItems; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool there = t_mine + j * t_step < length && i < count;
+                    d_in[j][i] = there ? d_in[j][i] : 0.0f;
+                    u_in[j][i] = there ? u_in[j][i] : 0.0f;
                 }
+        }
+#pragma unroll
+        for (int j = 0; j < kItems; j++) {
+            const int t = t_mine + j * t_step, at = c_in * P + G::place(t);
+            if (t >= TILE) continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (ENDS) sum_d[i] += d_in[j][i];
+                ld[at + i * P] = d_in[j][i];
+                lu[at + i * P] = u_in[j][i];
             }
         }
         float y[K] = {};
@@ -370,6 +413,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
             G::read(lu + ch * P, tl, u);
 #pragma unroll
             for (int k = 0; k < K; k++) total += d[k];
+#pragma unroll 2
             for (int n = part; n < states; n += split) {
                 Carry *carry = lh + (n0 + n) * channels + ch;
                 const Carry c = *carry;
@@ -384,7 +428,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
                 }
                 float decay = __builtin_amdgcn_exp2f(total * c.A);
                 row_scan<true>(decay, h);
-                if (tl == kTimeLanes - 1) carry->h = h;
+                (tl == kTimeLanes - 1 ? carry : nowhere)->h = h;
                 if (ENDS) continue;
                 h = row_prev(h, c.h);
                 float C[K];
@@ -405,11 +449,18 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
             const int t = t_out + j * t_step;
             if (t >= length || count <= 0) continue;
             float out[4];
+            const float *sums = ly + c_in * P + G::place(t);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float v = skip[i] * x_now[j][i];
-                for (int q = 0; q < split; q++) v += ly[(q * channels + c_in + i) * P + G::place(t)];
-                out[i] = gated ? v * (z_now[j][i] * sigmoid_(z_now[j][i])) : v;
+            for (int i = 0; i < 4; i++) out[i] = __builtin_fmaf(skip[i], x_now[j][i], sums[i * P]);
+#pragma unroll 1
+            for (int q = 1; q < split; q++) {
+                sums += channels * P;
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[i] += sums[i * P];
+            }
+            if (gated) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) out[i] *= z_now[j][i] * sigmoid_(z_now[j][i]);
             }
             store_quad(const_cast<ST *>(token_at<ST>(a.y, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.y.token + c_from, count, whole, out);
         }
@@ -452,8 +503,11 @@ template <int K> struct BackwardLds {
     // d, u, g0 and s1, s2, v; B and C; A and the gradients' carries, the states and the sums for A
     static __host__ __device__ constexpr int words(int N)
     {
-        return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 4 * kBwdChannels * N;
+        return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 4 * kBwdChannels * padded(N) + kNowhere;
     }
+    // A wave goes through its states without a branch: those past the last one have no decay, no B and no C.
+    static constexpr int kNowhere = 3 * kBwdChannels * kBwdStates;  // where lanes write that have nothing to say
+    static __host__ __device__ constexpr int padded(int N) { return (N + kBwdStates - 1) / kBwdStates * kBwdStates; }
 };
 
 template <typename ST, int K, bool ENDS>
@@ -463,13 +517,13 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     constexpr int TILE = G::kTile, P = G::kPitch, channels = kBwdChannels;
     constexpr int kThreads = kBwdWaves * 64, kItems = kBwdWaves * TILE / kThreads;
     const scanscam_selective &a = args.a;
-    const int N = (int)a.N;
+    const int N = (int)a.N, slots = channels * BackwardLds<K>::padded(N);
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *lg = lu + channels * P;
     float *l1 = lg + channels * P, *l2 = l1 + channels * P, *lv = l2 + channels * P;
     float *lB = lv + channels * P, *lC = lB + kStateBlock * P;
     Carry *lG = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
-    float *lh = reinterpret_cast<float *>(lG + channels * N), *lS = lh + channels * N;
+    float *lh = reinterpret_cast<float *>(lG + slots), *lS = lh + slots, *nowhere = lS + slots;
 
     const int64_t per_group = a.channels / a.groups;
     const int64_t group = blockIdx.x / args.blocks, c0 = (blockIdx.x - group * args.blocks) * channels;
@@ -481,10 +535,10 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = lane >> 4, tl = lane & 15;
 
-    for (int i = threadIdx.x; i < channels * N; i += kThreads) {
+    for (int i = threadIdx.x; i < slots; i += kThreads) {
         const int n = i / channels, c = i - n * channels;
         Carry q{0.0f, 0.0f};
-        if (c < here) {
+        if (c < here && n < N) {
             const int64_t at = (first + c) * N + n;
             q.A = param(a.A, at) * kLog2e;
             if (!ENDS) {
@@ -529,31 +583,55 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
         __syncthreads();
         if (!ENDS) {
             const float *from = static_cast<const float *>(a.saved) + (s.tile + tile) * N * a.channels + first;
-            for (int i = threadIdx.x; i < channels * N; i += kThreads) {
+            for (int i = threadIdx.x; i < slots; i += kThreads) {
                 const int n = i / channels, c = i - n * channels;
-                lh[i] = c < here ? from[(int64_t)n * a.channels + c] : 0.0f;
+                lh[i] = c < here && n < N ? from[(int64_t)n * a.channels + c] : 0.0f;
             }
         }
         Quad<ST> x_now[kItems], dt_now[kItems], gy_now[kItems], z_now[kItems];
         const int t_mine = again(t_in);
+        const bool full = length == TILE && here == channels;
+        float d_in[kItems][4], u_in[kItems][4], g_in[kItems][4];
+        step_sizes(dt, bias, a.softplus, d_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
-            const int t = t_mine + j * t_step;
             x_now[j] = x[j];
             dt_now[j] = dt[j];
             gy_now[j] = gy[j];
             z_now[j] = z[j];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float raw = dt[j][i] + bias[i];
-                float d = a.softplus ? softplus_(raw) : raw, u = d * x[j][i], g = gated ? gy[j][i] * (z[j][i] * sigmoid_(z[j][i])) : gy[j][i];
-                const bool there = t < length && i < count;
-                const int at = (c_in + i) * P + G::place(t);
-                ld[at] = there ? d : 0.0f;
-                lu[at] = there ? u : 0.0f;
-                lg[at] = there ? g : 0.0f;
-                if (!ENDS) l1[at] = l2[at] = lv[at] = 0.0f;
-                else sum_bias[i] += there ? d : 0.0f;
+                u_in[j][i] = d_in[j][i] * x[j][i];
+                g_in[j][i] = gy[j][i];
+            }
+        }
+        if (gated) {
+#pragma unroll
+            for (int j = 0; j < kItems; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) g_in[j][i] *= z[j][i] * sigmoid_(z[j][i]);
+        }
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < kItems; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool there = t_mine + j * t_step < length && i < count;
+                    d_in[j][i] = there ? d_in[j][i] : 0.0f;
+                    u_in[j][i] = there ? u_in[j][i] : 0.0f;
+                    g_in[j][i] = there ? g_in[j][i] : 0.0f;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < kItems; j++) {
+            const int at = c_in * P + G::place(t_mine + j * t_step);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ld[at + i * P] = d_in[j][i];
+                lu[at + i * P] = u_in[j][i];
+                lg[at + i * P] = g_in[j][i];
+                if (!ENDS) l1[at + i * P] = l2[at + i * P] = lv[at + i * P] = 0.0f;
+                else sum_bias[i] += d_in[j][i];
             }
         }
         for (int n0 = 0; n0 < N; n0 += kStateBlock) {
@@ -567,7 +645,11 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                     if (n0 + kStateBlock < N) bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
                     else if (tile > 0) fetch(t0 - TILE);
                 }
-                const int ch = ((wave + step) % kBwdWaves) * kRows + row;
+                if (wave * kBwdStates >= states) continue;
+                const int ch = ((wave + step) % kBwdWaves) * kRows + row, from = (n0 + wave * kBwdStates) * channels + ch;
+                // (an address for every lane instead of a branch around the one that writes: the four states below stay one block)
+                Carry *out = tl == 0 ? lG + from : reinterpret_cast<Carry *>(nowhere);
+                float *sums = tl == kTimeLanes - 1 ? lS + from : nowhere + 2 * channels * kBwdStates;
                 float d[K], u[K], g0[K], s1[K], s2[K], v[K], total = 0.0f;
                 G::read(ld + ch * P, tl, d);
                 G::read(lg + ch * P, tl, g0);
@@ -582,9 +664,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
 #pragma unroll
                 for (int q = 0; q < kBwdStates; q++) {
                     const int n = wave * kBwdStates + q;
-                    if (n >= states) continue;
-                    const int at = (n0 + n) * channels + ch;
-                    const Carry c = lG[at];
+                    const Carry c = lG[from + q * channels];
                     float e[K], h[K], B[K], C[K];
                     G::read(lC + n * P, tl, C);
                     float back = tl == kTimeLanes - 1 ? c.h : 0.0f;
@@ -595,9 +675,9 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                     const float decay = __builtin_amdgcn_exp2f(total * c.A);
                     float a2 = decay;
                     row_scan<false>(a2, back);
-                    if (tl == 0) lG[at].h = back;
+                    out[q * channels].h = back;
                     if (ENDS) continue;
-                    const float h0 = lh[at];
+                    const float h0 = lh[from + q * channels];
                     G::read(lB + n * P, tl, B);
                     float fold = tl == 0 ? h0 : 0.0f, a1 = decay;
 #pragma unroll
@@ -628,7 +708,8 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                         sum = __builtin_fmaf(d[k], r, sum);
                     }
                     sum = row_sum(sum);
-                    if (tl == kTimeLanes - 1) lS[at] += sum;
+                    sums[q * channels] += sum;
+                    __builtin_amdgcn_sched_barrier(0x104);  // the next state's reads may go ahead, its arithmetic would need more registers
                 }
                 if (ENDS) continue;
                 G::write(l1 + ch * P, tl, s1);
@@ -664,21 +745,27 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
             const int t = t_out + j * t_step;
             if (t >= length || count <= 0) continue;
             float gx[4], gd[4], gz[4];
+            const int at = c_in * P + G::place(t);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int at = (c_in + i) * P + G::place(t);
-                const float xi = x_now[j][i], zi = z_now[j][i];
-                const float s1 = l1[at], s2 = l2[at] * (1.0f / kLog2e), v = __builtin_fmaf(skip[i], xi, lv[at]), g0 = lg[at];
-                gx[i] = __builtin_fmaf(ld[at], s1, skip[i] * g0);
+                const float xi = x_now[j][i], s1 = l1[at + i * P], s2 = l2[at + i * P] * (1.0f / kLog2e), g0 = lg[at + i * P];
+                gx[i] = __builtin_fmaf(ld[at + i * P], s1, skip[i] * g0);
                 gd[i] = __builtin_fmaf(xi, s1, s2);
-                if (a.softplus) gd[i] *= sigmoid_(dt_now[j][i] + bias[i]);
                 sum_skip[i] = __builtin_fmaf(g0, xi, sum_skip[i]);
-                sum_bias[i] += gd[i];
-                if (gated) {
-                    const float sg = sigmoid_(zi);
+            }
+            if (a.softplus) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) gd[i] *= sigmoid_(dt_now[j][i] + bias[i]);
+            }
+            if (gated) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float zi = z_now[j][i], sg = sigmoid_(zi), v = __builtin_fmaf(skip[i], x_now[j][i], lv[at + i * P]);
                     gz[i] = gy_now[j][i] * v * (sg * __builtin_fmaf(zi, 1.0f - sg, 1.0f));
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum_bias[i] += gd[i];
             store_quad(const_cast<ST *>(token_at<ST>(a.gx, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gx.token + c_from, count, whole, gx);
             store_quad(const_cast<ST *>(token_at<ST>(a.gdt, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gdt.token + c_from, count, whole, gd);
             if (gated) store_quad(const_cast<ST *>(token_at<ST>(a.gz, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gz.token + c_from, count, whole, gz);

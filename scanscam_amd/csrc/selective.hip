@@ -56,23 +56,36 @@ struct Plan {
 int64_t forward_blocks(const scanscam_selective &a, int split) { return ceil_div(a.channels / a.groups, kFwdWaves / split * kRows); }
 int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels); }
 
-// Parts of time, at least `shortest` tiles each, where the channels alone give fewer than `wanted` workgroups.
-int64_t choose_parts(const scanscam_selective &a, int64_t workgroups, int64_t wanted, int64_t shortest)
+// Parts of time for `wanted` workgroups, whole tiles each. (Sequences x parts is below 2 x wanted: a grid's rows suffice.)
+int64_t parts_for(const scanscam_selective &a, int64_t workgroups, int64_t wanted)
 {
-    if (a.parts > 0) return a.parts;
-    const int64_t tiles = ceil_div(a.T, kTile), most = tiles / shortest;
-    const int64_t parts = ceil_div(wanted, workgroups > 0 ? workgroups : 1);  // (a grid's rows suffice: sequences x parts is below 2 x wanted)
-    return parts < 2 || most < 2 ? 1 : parts < most ? parts : most;
+    const int64_t tiles = ceil_div(a.T, kTile), parts = ceil_div(wanted, workgroups > 0 ? workgroups : 1);
+    return tiles < 1 ? 1 : parts < tiles ? parts : tiles;
 }
 
+// Two workgroups fit a CU, and one keeps it nearly as busy, so that from 192 workgroups on nothing is cut. Below, sharing the states
+// of a channel out costs less than parts of time, whose first pass repeats most of the arithmetic, as long as it is two waves
+// (bf16, N = 16, us: [4, 2048, 1024] 128 whole, 93 by two waves, 105 in 4 parts; [6, 2048, 1024] 139, 137, 156); four
+// or eight waves have too little to do for the tokens' own work and the barriers, so that with fewer channels parts win where there are
+// tiles for them ([2, 2048, 1024] 127 whole, 72 by four waves, 63 in 8 parts; [1, 2048, 1024] 128, 70, 40 in 16), and not in
+// short sequences ([1, 512, 2048] 39 whole, 26 by four waves, 30 in 4 parts).
 Plan forward_plan(const scanscam_selective &a)
 {
-    Plan p{1, 1};
-    while (p.split < kFwdWaves && p.split < a.N && a.sequences * a.groups * forward_blocks(a, p.split) < 512) p.split *= 2;
-    p.parts = choose_parts(a, a.sequences * a.groups * forward_blocks(a, p.split), 512, 4);
+    Plan p{1, a.parts > 0 ? a.parts : 1};
+    const int64_t whole = a.sequences * a.groups * forward_blocks(a, 1);
+    const bool long_enough = ceil_div(a.T, kTile) >= 8;
+    if (whole < 192 && (whole >= 96 || !long_enough)) {
+        while (p.split < kFwdWaves && p.split < a.N && (whole >= 96 ? p.split < 2 : a.sequences * a.groups * forward_blocks(a, p.split) < 256)) p.split *= 2;
+    } else if (whole < 96 && a.parts == 0) {
+        p.parts = parts_for(a, whole, 512);
+    }
     return p;
 }
-Plan backward_plan(const scanscam_selective &a) { return {1, choose_parts(a, a.sequences * a.groups * backward_blocks(a), 512, 4)}; }
+Plan backward_plan(const scanscam_selective &a)
+{
+    const int64_t whole = a.sequences * a.groups * backward_blocks(a);
+    return {1, a.parts > 0 ? a.parts : whole < 256 ? parts_for(a, whole, 512) : 1};
+}
 
 size_t ends_words(const scanscam_selective &a, int64_t parts) { return parts > 1 ? (size_t)(a.sequences * parts * (a.N + 1) * a.channels) : 0; }
 size_t bc_words(const scanscam_selective &a) { return (size_t)(a.groups * backward_blocks(a) * a.batch * a.T * 2 * a.N); }

@@ -141,9 +141,13 @@ __device__ __forceinline__ const ST *token_at(const scanscam_tokens &x, int64_t 
 }
 
 // An element a 32-bit number of them behind a place that is the same for all lanes: an address of a scalar base and a vector offset.
-template <typename ST> __device__ __forceinline__ ST *behind(const ST *base, uint32_t elements)
+template <typename ST> __device__ __forceinline__ const ST *behind(const ST *base, uint32_t elements)
 {
-    return reinterpret_cast<ST *>(reinterpret_cast<uintptr_t>(base) + (uint64_t)(uint32_t)(elements * (uint32_t)sizeof(ST)));
+    return reinterpret_cast<const ST *>(reinterpret_cast<const char *>(base) + (uint64_t)(uint32_t)(elements * (uint32_t)sizeof(ST)));
+}
+template <typename ST> __device__ __forceinline__ ST *behind(ST *base, uint32_t elements)
+{
+    return reinterpret_cast<ST *>(reinterpret_cast<char *>(base) + (uint64_t)(uint32_t)(elements * (uint32_t)sizeof(ST)));
 }
 
 // Four neighbouring elements as they are stored. Where not all quads of a workgroup are whole, they are read one by one, those

@@ -26,8 +26,11 @@ int check_selective(const scanscam_selective *a)
 {
     if (a == nullptr) return SCANSCAM_EINVAL;
     SCANSCAM_CHECK(check_sizes(a->channels, a->groups, a->N, a->dtype));
-    if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->parts < 0 || a->parts > kMostParts || a->sequences * (a->parts > 0 ? a->parts : 1) > 65535) return SCANSCAM_EINVAL;
+    if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->sequences >= kMostTokens || a->parts < 0 || a->parts > kMostParts) return SCANSCAM_EINVAL;
     if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
+    // (a launch has fewer than 2^32 threads)
+    if (a->sequences * (a->groups + a->channels / kBwdChannels) * (a->parts > 0 ? a->parts : 1) >= int64_t(1) << 23) return SCANSCAM_EINVAL;
+    if (a->batch > 0 && a->T >= (int64_t(1) << 31) / a->N / a->batch) return SCANSCAM_EINVAL;
     if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
     SCANSCAM_CHECK(check_param(a->A, true));
     SCANSCAM_CHECK(check_param(a->D, false));
@@ -56,7 +59,7 @@ struct Plan {
 int64_t forward_blocks(const scanscam_selective &a, int split) { return ceil_div(a.channels / a.groups, kFwdWaves / split * kRows); }
 int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels); }
 
-// Parts of time for `wanted` workgroups, whole tiles each. (Sequences x parts is below 2 x wanted: a grid's rows suffice.)
+// Parts of time for `wanted` workgroups, whole tiles each.
 int64_t parts_for(const scanscam_selective &a, int64_t workgroups, int64_t wanted)
 {
     const int64_t tiles = ceil_div(a.T, kTile), parts = ceil_div(wanted, workgroups > 0 ? workgroups : 1);
@@ -95,7 +98,7 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
     constexpr int K = kTokensALane;
     const Plan plan = forward_plan(a);
     const SelectiveArgs args{a, plan.split, forward_blocks(a, plan.split), plan.parts, static_cast<float *>(a.workspace), nullptr, nullptr};
-    const dim3 grid((unsigned)(a.groups * args.blocks), (unsigned)(a.sequences * plan.parts));
+    const dim3 grid((unsigned)(a.groups * args.blocks * a.sequences * plan.parts));
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
     if (plan.parts > 1) {
         const hipError_t err = launch_wide(selective_fwd_kernel<ST, K, true>, grid, kFwdWaves * 64, words, stream, args);
@@ -111,7 +114,7 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     const int64_t blocks = backward_blocks(a);
     float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.parts), *sums = bc + bc_words(a);
     const SelectiveArgs args{a, 1, blocks, plan.parts, ends, bc, sums};
-    const dim3 grid((unsigned)(a.groups * blocks), (unsigned)(a.sequences * plan.parts));
+    const dim3 grid((unsigned)(a.groups * blocks * a.sequences * plan.parts));
     const int words = BackwardLds<K>::words((int)a.N);
     hipError_t err = hipSuccess;
     if (plan.parts > 1) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);

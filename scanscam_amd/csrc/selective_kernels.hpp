@@ -73,19 +73,35 @@ template <bool FORWARDS> __device__ __forceinline__ void row_scan(float &a, floa
                      : "+v"(a), "+v"(b));
     }
 }
+// Both at once: each fills the other's wait states.
+#define SCANSCAM_ROW_STEPS(N)                                                      \
+    "v_fmac_f32_dpp %1, %1, %0 row_shr:" N " row_mask:0xf bank_mask:0xf\n\t"       \
+    "v_fmac_f32_dpp %3, %3, %2 row_shl:" N " row_mask:0xf bank_mask:0xf\n\t"
+#define SCANSCAM_ROW_DECAYS(N)                                                     \
+    "v_mul_f32_dpp %0, %0, %0 row_shr:" N " row_mask:0xf bank_mask:0xf\n\t"        \
+    "v_mul_f32_dpp %2, %2, %2 row_shl:" N " row_mask:0xf bank_mask:0xf\n\t"
+__device__ __forceinline__ void row_scans(float &a, float &up, float &b, float &down)
+{
+    asm volatile("s_nop 1\n\t" SCANSCAM_ROW_STEPS("1") SCANSCAM_ROW_DECAYS("1") SCANSCAM_ROW_STEPS("2") SCANSCAM_ROW_DECAYS("2")
+                 SCANSCAM_ROW_STEPS("4") SCANSCAM_ROW_DECAYS("4") SCANSCAM_ROW_STEPS("8") "s_nop 1"
+                 : "+v"(a), "+v"(up), "+v"(b), "+v"(down));
+}
+#undef SCANSCAM_ROW_DECAYS
+#undef SCANSCAM_ROW_STEPS
 #undef SCANSCAM_ROW_STEP
 __device__ __forceinline__ float row_prev(float v, float fill) { return dpp_move<0x111, 0xf>(fill, v); }
 __device__ __forceinline__ float row_next(float v, float fill) { return dpp_move<0x101, 0xf>(fill, v); }
-// The sum over a row's lanes, in lane 15.
-__device__ __forceinline__ float row_sum(float v)
+// The sums of four values over a row's lanes, in lane 15: four chains that fill each other's wait states.
+__device__ __forceinline__ void row_sums(float (&v)[4])
 {
-    asm volatile("s_nop 1\n\t"
-                 "v_add_f32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
-                 "v_add_f32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
-                 "v_add_f32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\ts_nop 1\n\t"
-                 "v_add_f32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf"
-                 : "+v"(v));
-    return v;
+#define SCANSCAM_ROW_ADDS(N)                                                       \
+    "v_add_f32_dpp %0, %0, %0 row_shr:" N " row_mask:0xf bank_mask:0xf\n\t"        \
+    "v_add_f32_dpp %1, %1, %1 row_shr:" N " row_mask:0xf bank_mask:0xf\n\t"        \
+    "v_add_f32_dpp %2, %2, %2 row_shr:" N " row_mask:0xf bank_mask:0xf\n\t"        \
+    "v_add_f32_dpp %3, %3, %3 row_shr:" N " row_mask:0xf bank_mask:0xf\n\t"
+    asm volatile("s_nop 1\n\t" SCANSCAM_ROW_ADDS("1") SCANSCAM_ROW_ADDS("2") SCANSCAM_ROW_ADDS("4") SCANSCAM_ROW_ADDS("8")
+                 : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+#undef SCANSCAM_ROW_ADDS
 }
 // The sums over the four rows of four values, the sum of value r in row r. A swap of halves puts two values' lanes behind each
 // other, so that an addition serves both: six instructions, where four sums of their own take sixteen.
@@ -167,6 +183,13 @@ template <typename ST> struct Quad {
         }
     }
     __device__ __forceinline__ float operator[](int i) const { return (float)e[i]; }
+    // Waits here for what load() asked for.
+    __device__ __forceinline__ void arrive()
+    {
+        raw_t raw = __builtin_bit_cast(raw_t, *this);
+        asm volatile("" : "+v"(raw));
+        *this = __builtin_bit_cast(Quad, raw);
+    }
 };
 template <typename ST> __device__ __forceinline__ void store_quad(ST *base, uint32_t at, int count, bool whole, const float (&f)[4])
 {
@@ -206,6 +229,14 @@ template <typename ST, int TILE, int THREADS> struct StateInputs {
             const int t = (thread + j * THREADS) / kQuads, row = t < length ? t : length - 1;
             B[j].load(fromB, (uint32_t)row * (uint32_t)a.B.token + (uint32_t)at, N - at, whole);
             C[j].load(fromC, (uint32_t)row * (uint32_t)a.C.token + (uint32_t)at, N - at, whole);
+        }
+    }
+    __device__ __forceinline__ void arrive()
+    {
+#pragma unroll
+        for (int j = 0; j < kCount; j++) {
+            B[j].arrive();
+            C[j].arrive();
         }
     }
     template <typename G> __device__ __forceinline__ void store(float *lB, float *lC, int length, int states) const
@@ -265,6 +296,24 @@ struct SelectiveArgs {
     float *sums;      // backwards: [sequences][parts][N + 2][channels], sums over a part's tokens for A, D and dt_bias
 };
 
+// Workgroups are dealt out to the 8 dies in turn, each with an L2 cache of its own, while neighbouring blocks of channels share the
+// 128-byte lines of every token (a block of 16 channels of 16 bits is a quarter of one) and all of B and C: dealt out one by
+// one, a line is fetched by up to four dies, and written by them in pieces. So a die takes neighbours: an eighth of all work where
+// sequences are of one length, and 8 blocks in turn where they are not, as dies would then be done at different times. (Backward
+// kernel of the layer [8, 4096, 2048] in bf16: one by one 1328 us, 8 in turn 1282, eighths 1234; packed prompts forwards: 135,
+// 139 and 170 us.)
+struct Work {
+    int64_t block, unit;  // block of channels among all groups'; part of a sequence
+};
+__device__ __forceinline__ Work work_of(int64_t blocks, bool even)
+{
+    constexpr uint32_t kDies = 8;
+    const uint32_t near = even ? gridDim.x / kDies : 8u, round = near * kDies;
+    uint32_t i = blockIdx.x;
+    if (near > 0 && i < gridDim.x / round * round) i = i / round * round + i % kDies * near + i % round / kDies;
+    return {i % blocks, i / blocks};
+}
+
 // The state before a part (the gradient behind it): that of the sequence's end, taken through the parts between. A part alone
 // is the map h -> exp(A * sum of d) h + its own end.
 __device__ __forceinline__ float carried(const SelectiveArgs &args, const Stretch &s, int n, int64_t channel, float A, float h, bool forwards)
@@ -308,10 +357,11 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     Carry *lh = reinterpret_cast<Carry *>(lC + kStateBlock * P), *nowhere = lh + channels * N;  // [N][channels]
 
     const int64_t per_group = a.channels / a.groups;
-    const int64_t group = blockIdx.x / args.blocks, c0 = (blockIdx.x - group * args.blocks) * channels;  // c0: inside the group
+    const Work w = work_of(a.groups * args.blocks, a.offsets == nullptr);
+    const int64_t group = w.block / args.blocks, c0 = (w.block - group * args.blocks) * channels;  // c0: inside the group
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;  // first channel
-    const Stretch s = stretch_of<TILE>(a, blockIdx.y, args.parts);
+    const Stretch s = stretch_of<TILE>(a, w.unit, args.parts);
     if (ENDS && s.part == args.parts - 1) return;  // (nothing follows it)
     const bool gated = !ENDS && a.z.p != nullptr;
 
@@ -447,6 +497,14 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
         if (!ENDS) G::write(ly + (part * channels + ch) * P, tl, y);
         __syncthreads();
         if (ENDS) continue;
+        // What was asked for ahead is waited for before anything is stored: a wait behind the stores would be one for them too.
+#pragma unroll
+        for (int j = 0; j < kItems; j++) {
+            x[j].arrive();
+            dt[j].arrive();
+            z[j].arrive();
+        }
+        bc.arrive();
         const int t_out = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
@@ -504,10 +562,10 @@ constexpr int kBwdWaves = 4, kBwdChannels = kBwdWaves * kRows, kBwdStates = kSta
 
 template <int K> struct BackwardLds {
     using G = Geometry<K>;
-    // d, u, g0 and s1, s2, v; B and C; A and the gradients' carries, the states and the sums for A
+    // d, u, g0 and s1, s2, v; B and C; A and the gradients' carries and the sums for A; a block's states
     static __host__ __device__ constexpr int words(int N)
     {
-        return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 4 * kBwdChannels * padded(N) + kNowhere;
+        return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 3 * kBwdChannels * padded(N) + kBwdChannels * kStateBlock + kNowhere;
     }
     // A wave goes through its states without a branch: those past the last one have no decay, no B and no C.
     static constexpr int kNowhere = 3 * kBwdChannels * kBwdStates;  // where lanes write that have nothing to say
@@ -527,13 +585,14 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     float *l1 = lg + channels * P, *l2 = l1 + channels * P, *lv = l2 + channels * P;
     float *lB = lv + channels * P, *lC = lB + kStateBlock * P;
     Carry *lG = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
-    float *lh = reinterpret_cast<float *>(lG + slots), *lS = lh + slots, *nowhere = lS + slots;
+    float *lS = reinterpret_cast<float *>(lG + slots), *lh = lS + slots, *nowhere = lh + channels * kStateBlock;  // lh: [16][channels]
 
     const int64_t per_group = a.channels / a.groups;
-    const int64_t group = blockIdx.x / args.blocks, c0 = (blockIdx.x - group * args.blocks) * channels;
+    const Work w = work_of(a.groups * args.blocks, a.offsets == nullptr);
+    const int64_t group = w.block / args.blocks, c0 = (w.block - group * args.blocks) * channels;
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;
-    const Stretch s = stretch_of<TILE>(a, blockIdx.y, args.parts);
+    const Stretch s = stretch_of<TILE>(a, w.unit, args.parts);
     if (ENDS && s.part == 0) return;
     const bool gated = a.z.p != nullptr;
 
@@ -580,18 +639,23 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
         }
         bc.load(a, s.batch, group, t0, length, 0);
     };
-    if (tiles > 0) fetch(s.start + (tiles - 1) * TILE);
+    // The states that a tile starts from, one a thread in a block of 16.
+    static_assert(channels * kStateBlock == kThreads, "one a thread");
+    float h_saved = 0.0f;
+    auto fetch_states = [&](int64_t tile, int n0) {
+        if (ENDS) return;
+        const int thread = again((int)threadIdx.x), n = n0 + thread / channels, c = thread % channels;
+        const float *from = static_cast<const float *>(a.saved) + (s.tile + tile) * N * a.channels + first;
+        h_saved = c < here && n < N ? *(from + (int64_t)n * a.channels + c) : 0.0f;
+    };
+    if (tiles > 0) {
+        fetch(s.start + (tiles - 1) * TILE);
+        fetch_states(tiles - 1, 0);
+    }
     for (int64_t tile = tiles - 1; tile >= 0; tile--) {
         const int64_t t0 = s.start + tile * TILE;
         const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
         __syncthreads();
-        if (!ENDS) {
-            const float *from = static_cast<const float *>(a.saved) + (s.tile + tile) * N * a.channels + first;
-            for (int i = threadIdx.x; i < slots; i += kThreads) {
-                const int n = i / channels, c = i - n * channels;
-                lh[i] = c < here && n < N ? from[(int64_t)n * a.channels + c] : 0.0f;
-            }
-        }
         Quad<ST> x_now[kItems], dt_now[kItems], gy_now[kItems], z_now[kItems];
         const int t_mine = again(t_in);
         const bool full = length == TILE && here == channels;
@@ -642,12 +706,18 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
             const int states = N - n0 < kStateBlock ? N - n0 : kStateBlock;
             if (n0 > 0) __syncthreads();
             bc.template store<G>(lB, lC, length, states);
+            if (!ENDS) lh[threadIdx.x] = h_saved;
             float gB[kBwdStates][K] = {}, gC[kBwdStates][K] = {};
             for (int step = 0; step < kBwdWaves; step++) {
                 __syncthreads();
                 if (step == 0) {
-                    if (n0 + kStateBlock < N) bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
-                    else if (tile > 0) fetch(t0 - TILE);
+                    if (n0 + kStateBlock < N) {
+                        bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
+                        fetch_states(tile, n0 + kStateBlock);
+                    } else if (tile > 0) {
+                        fetch(t0 - TILE);
+                        fetch_states(tile - 1, 0);
+                    }
                 }
                 if (wave * kBwdStates >= states) continue;
                 const int ch = ((wave + step) % kBwdWaves) * kRows + row, from = (n0 + wave * kBwdStates) * channels + ch;
@@ -665,57 +735,67 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 }
 #pragma unroll
                 for (int k = 0; k < K; k++) total += d[k];
+                float sum_A[kBwdStates];
+                static_assert(kBwdStates == 4, "row_sums takes a wave's states");
 #pragma unroll
                 for (int q = 0; q < kBwdStates; q++) {
                     const int n = wave * kBwdStates + q;
                     const Carry c = lG[from + q * channels];
-                    float e[K], h[K], B[K], C[K];
+                    float e[K], C[K];
                     G::read(lC + n * P, tl, C);
-                    float back = tl == kTimeLanes - 1 ? c.h : 0.0f;
+                    float back = tl == kTimeLanes - 1 ? c.h : 0.0f, a2 = __builtin_amdgcn_exp2f(total * c.A);
 #pragma unroll
                     for (int k = 0; k < K; k++) e[k] = __builtin_amdgcn_exp2f(d[k] * c.A);
+                    if constexpr (ENDS) {
 #pragma unroll
-                    for (int k = K - 1; k >= 0; k--) back = e[k] * __builtin_fmaf(g0[k], C[k], back);
-                    const float decay = __builtin_amdgcn_exp2f(total * c.A);
-                    float a2 = decay;
-                    row_scan<false>(a2, back);
-                    out[q * channels].h = back;
-                    if (ENDS) continue;
-                    const float h0 = lh[from + q * channels];
-                    G::read(lB + n * P, tl, B);
-                    float fold = tl == 0 ? h0 : 0.0f, a1 = decay;
-#pragma unroll
-                    for (int k = 0; k < K; k++) {
-                        h[k] = u[k] * B[k];
-                        fold = __builtin_fmaf(e[k], fold, h[k]);
+                        for (int k = K - 1; k >= 0; k--) back = e[k] * __builtin_fmaf(g0[k], C[k], back);
+                        row_scan<false>(a2, back);
+                        out[q * channels].h = back;
+                        continue;
                     }
-                    row_scan<true>(a1, fold);
-                    const float before = row_prev(fold, h0);
-                    float g = row_next(back, c.h);
-                    float state = before;
+                    // Forwards in time and backwards side by side: each is one chain of dependent operations.
+                    float h[K], B[K];
+                    G::read(lB + n * P, tl, B);
+                    const float h0 = lh[(wave * kBwdStates + q) * channels + ch];
+                    float fold = tl == 0 ? h0 : 0.0f, a1 = a2;
+#pragma unroll
+                    for (int k = 0; k < K; k++) h[k] = u[k] * B[k];
 #pragma unroll
                     for (int k = 0; k < K; k++) {
+                        fold = __builtin_fmaf(e[k], fold, h[k]);
+                        back = e[K - 1 - k] * __builtin_fmaf(g0[K - 1 - k], C[K - 1 - k], back);
+                    }
+                    row_scans(a1, fold, a2, back);
+                    out[q * channels].h = back;
+                    const float before = row_prev(fold, h0);
+                    float g = row_next(back, c.h), state = before;
+#pragma unroll
+                    for (int k = 0; k < K; k++) {
+                        const int r = K - 1 - k;
                         state = __builtin_fmaf(e[k], state, h[k]);
+                        g = __builtin_fmaf(g0[r], C[r], g);  // G[t]
                         h[k] = state;
                         v[k] = __builtin_fmaf(C[k], state, v[k]);
                         gC[q][k] = __builtin_fmaf(g0[k], state, gC[q][k]);
+                        gB[q][r] = __builtin_fmaf(u[r], g, gB[q][r]);
+                        s1[r] = __builtin_fmaf(B[r], g, s1[r]);
+                        g *= e[r];
+                        B[r] = g;  // e G: what G hands to the token before
                     }
                     float sum = 0.0f;
 #pragma unroll
-                    for (int k = K - 1; k >= 0; k--) {
-                        g = __builtin_fmaf(g0[k], C[k], g);  // G[t]
-                        gB[q][k] = __builtin_fmaf(u[k], g, gB[q][k]);
-                        s1[k] = __builtin_fmaf(B[k], g, s1[k]);
-                        g *= e[k];
-                        const float r = g * (k > 0 ? h[k - 1] : before);
+                    for (int k = 0; k < K; k++) {
+                        const float r = B[k] * (k > 0 ? h[k - 1] : before);
                         s2[k] = __builtin_fmaf(c.A, r, s2[k]);
                         sum = __builtin_fmaf(d[k], r, sum);
                     }
-                    sum = row_sum(sum);
-                    sums[q * channels] += sum;
+                    sum_A[q] = sum;
                     __builtin_amdgcn_sched_barrier(0x104);  // the next state's reads may go ahead, its arithmetic would need more registers
                 }
                 if (ENDS) continue;
+                row_sums(sum_A);
+#pragma unroll
+                for (int q = 0; q < kBwdStates; q++) sums[q * channels] += sum_A[q];
                 G::write(l1 + ch * P, tl, s1);
                 G::write(l2 + ch * P, tl, s2);
                 G::write(lv + ch * P, tl, v);
@@ -732,7 +812,17 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 }
             }
             __syncthreads();
-            float *to = args.bc + (((int64_t)blockIdx.x * a.batch + s.batch) * a.T + t0) * 2 * N + n0;
+            // (waited for before anything is stored, as in the forward kernel)
+#pragma unroll
+            for (int j = 0; j < kItems; j++) {
+                x[j].arrive();
+                dt[j].arrive();
+                gy[j].arrive();
+                z[j].arrive();
+            }
+            bc.arrive();
+            asm volatile("" : "+v"(h_saved));
+            float *to = args.bc + ((w.block * a.batch + s.batch) * a.T + t0) * 2 * N + n0;
             const int thread = again((int)threadIdx.x);
 #pragma unroll
             for (int j = 0; j < TILE * 2 * kStateBlock / 4 / kThreads; j++) {

@@ -33,6 +33,7 @@
 #include <unordered_map>
 
 #include "scanscam_hip.h"
+#include "scanscam_ops.h"
 
 namespace {
 
@@ -408,11 +409,404 @@ PyObject *bind(PyObject *, PyObject *args)
     return reinterpret_cast<PyObject *>(&node_type);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// The operators of a state space layer: calls that need no gradient. In Python the checks, the struct of arguments and the
+// outputs took 13 to 20 us a call, against 4 us of the kernel at one token. As above, None is returned for every call that is not
+// covered (gradients, CPU tensors, mismatched arguments, views that have to be copied first), and the Python path goes on with it.
+// ---------------------------------------------------------------------------------------------------------------------------
+struct Operators {
+    decltype(&scanscam_selective_fwd) selective = nullptr;
+    decltype(&scanscam_selective_workspace_bytes) selective_workspace = nullptr;
+    decltype(&scanscam_selective_step_fwd) selective_step = nullptr;
+    decltype(&scanscam_conv_fwd) conv = nullptr;
+    decltype(&scanscam_conv_step_fwd) conv_step = nullptr;
+    decltype(&scanscam_norm_fwd) norm = nullptr;
+} operators;
+
+constexpr int64_t kMostStates = 256, kMostTaps = 8, kMostNormChannels = 32768;
+
+// The arguments of one call, looked at one after the other; `ok` says whether it is covered so far.
+struct Arguments {
+    PyObject *const *args;
+    bool ok;
+    at::Tensor first;  // the activations: what the others are compared with
+
+    Arguments(PyObject *const *args, Py_ssize_t nargs, Py_ssize_t expected, int first_at) : args(args)
+    {
+        ok = nargs == expected && operators.norm && !left_to_python && !modes_active() && !torch::jit::tracer::isTracing() &&
+             !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+        if (!ok) return;
+        first = tensor(first_at);
+        if (!ok || !first.defined()) {
+            ok = false;
+            return;
+        }
+        code();
+    }
+    // An argument that may be None (then undefined).
+    at::Tensor tensor(int i)
+    {
+        if (!ok || args[i] == Py_None) return {};
+        if (!THPVariable_CheckExact(args[i])) {
+            ok = false;
+            return {};
+        }
+        at::Tensor t = THPVariable_Unpack(args[i]);
+        ok = plain(t) && !(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(/*level=*/0).defined() &&
+             (!first.defined() || t.device() == first.device());
+        return t;
+    }
+    int code()
+    {
+        const int c = dtype_code(first.scalar_type());
+        if (c < 0 || c == SCANSCAM_F64) ok = false;
+        return c;
+    }
+    bool flag(int i)
+    {
+        const int v = PyObject_IsTrue(args[i]);
+        if (v < 0) {
+            PyErr_Clear();
+            ok = false;
+        }
+        return v == 1;
+    }
+    int activation(int i)
+    {
+        if (args[i] == Py_None) return SCANSCAM_ACT_NONE;
+        if (PyUnicode_Check(args[i]) && PyUnicode_CompareWithASCIIString(args[i], "silu") == 0) return SCANSCAM_ACT_SILU;
+        ok = false;
+        return 0;
+    }
+    void shape(const at::Tensor &t, at::IntArrayRef sizes)
+    {
+        if (t.defined() && t.sizes() != sizes) ok = false;
+    }
+    // [batch, T, ...] (lead 2) or [rows, ...] (lead 1) of the activations' type, unit-stride at the end.
+    scanscam_tokens tokens(const at::Tensor &t, int lead)
+    {
+        scanscam_tokens k{};
+        if (!ok || !t.defined()) return k;
+        if (t.scalar_type() != first.scalar_type() || (t.size(-1) != 1 && t.stride(-1) != 1) || t.stride(lead - 1) >= SCANSCAM_MOST_TOKEN_STRIDE) {
+            ok = false;
+            return k;
+        }
+        k.p = t.data_ptr();
+        k.batch = lead == 2 ? t.stride(0) : 0;
+        k.token = t.stride(lead - 1);
+        k.group = t.dim() > lead + 1 ? t.stride(lead) : 0;
+        return k;
+    }
+    scanscam_param parameter(const at::Tensor &t)
+    {
+        scanscam_param k{};
+        if (!ok || !t.defined()) return k;
+        const int c = dtype_code(t.scalar_type());
+        if (c < 0 || c == SCANSCAM_F64 || !t.is_contiguous()) ok = false;
+        k.p = t.data_ptr();
+        k.dtype = c;
+        return k;
+    }
+    void *dense(const at::Tensor &t, at::ScalarType type)
+    {
+        if (!ok || !t.defined()) return nullptr;
+        if (t.scalar_type() != type || !t.is_contiguous()) ok = false;
+        return t.data_ptr();
+    }
+    const void *indices(const at::Tensor &t, int32_t *wide)
+    {
+        *wide = t.defined() && t.scalar_type() == at::kLong;
+        return dense(t, *wide ? at::kLong : at::kInt);
+    }
+    at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type) const { return at::empty(sizes, at::TensorOptions().dtype(type).device(first.device())); }
+    void *stream() const { return c10::hip::getCurrentHIPStream(first.device().index()).stream(); }
+};
+
+void check_launch(int rc, const char *what)
+{
+    if (rc != SCANSCAM_OK) throw std::runtime_error(std::string("scanscam_") + what + ": " + error_text(rc));
+}
+
+// The device that the tensors are on must be the current one when a call is made.
+#define SCANSCAM_LAUNCH(call, what)                             \
+    {                                                           \
+        pybind11::gil_scoped_release no_gil;                    \
+        const c10::DeviceGuard guard(in.first.device());        \
+        check_launch(call, what);                               \
+    }
+
+// norm(x, weight, residual, eps, quant code): the tuple that rms_norm returns, or y alone.
+PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 5, 0);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &x = in.first, weight = in.tensor(1), residual = in.tensor(2);
+    const int64_t dims = x.dim();
+    if (!in.ok || dims < 1 || x.numel() == 0 || x.size(-1) > kMostNormChannels || !weight.defined()) Py_RETURN_NONE;
+    const int64_t channels = x.size(-1);
+    in.shape(weight, {channels});
+    in.shape(residual, x.sizes());
+    // Rows of one stride: the leading dimensions merge into one level.
+    const auto row_stride = [&](const at::Tensor &t) {
+        if (t.is_contiguous()) return channels;
+        if (channels != 1 && t.stride(-1) != 1) in.ok = false;
+        int64_t stride = channels, size = 1;
+        bool any = false;
+        for (int64_t d = dims - 2; d >= 0; d--) {
+            if (t.size(d) == 1) continue;
+            if (!any) stride = t.stride(d);
+            else if (t.stride(d) != stride * size) in.ok = false;
+            any = true;
+            size *= t.size(d);
+        }
+        return stride;
+    };
+    scanscam_norm a{};
+    a.rows = x.numel() / channels;
+    a.channels = channels;
+    a.x = x.data_ptr();
+    a.x_stride = row_stride(x);
+    a.weight = in.parameter(weight);
+    a.eps = (float)PyFloat_AsDouble(args[3]);
+    a.dtype = in.code();
+    const long quant = PyLong_AsLong(args[4]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (quant != 0 && quant != SCANSCAM_I8 && quant != SCANSCAM_F8) Py_RETURN_NONE;
+    a.out_dtype = quant != 0 ? (int)quant : a.dtype;
+    at::Tensor sum, scale;
+    if (residual.defined()) {
+        a.residual_dtype = dtype_code(residual.scalar_type());
+        if (a.residual_dtype < 0 || a.residual_dtype == SCANSCAM_F64) in.ok = false;
+        a.residual = residual.data_ptr();
+        a.residual_stride = row_stride(residual);
+    }
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(x.sizes(), quant == SCANSCAM_I8 ? at::kChar : quant == SCANSCAM_F8 ? at::kFloat8_e4m3fn : x.scalar_type());
+    a.y = y.data_ptr();
+    if (residual.defined()) {
+        sum = in.empty(x.sizes(), residual.scalar_type());
+        a.sum = sum.data_ptr();
+    }
+    if (quant != 0) {
+        scale = in.empty(x.sizes().slice(0, (size_t)dims - 1), at::kFloat);
+        a.scale = static_cast<float *>(scale.data_ptr());
+    }
+    SCANSCAM_LAUNCH(operators.norm(&a, in.stream()), "norm_fwd")
+    if (quant == 0 && !residual.defined()) return THPVariable_Wrap(std::move(y));
+    pybind11::list out;
+    for (at::Tensor *t : {&y, &scale, &sum})
+        if (t->defined()) out.append(pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(*t))));
+    return PyList_AsTuple(out.ptr());
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *with_state(at::Tensor &&y, at::Tensor &&state)
+{
+    pybind11::object a = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(y)));
+    if (!state.defined()) return a.release().ptr();
+    pybind11::object b = pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(state)));
+    return PyTuple_Pack(2, a.ptr(), b.ptr());
+}
+
+// conv(x, weight, bias, activation, state, offsets, return_state)
+PyObject *conv(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 7, 0);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &x = in.first, weight = in.tensor(1), bias = in.tensor(2), state = in.tensor(4), offsets = in.tensor(5);
+    if (!in.ok || x.dim() != 3 || x.numel() == 0 || !weight.defined() || weight.dim() != 2 || (offsets.defined() && (offsets.dim() != 1 || offsets.numel() < 2 || x.size(0) != 1)))
+        Py_RETURN_NONE;
+    scanscam_conv a{};
+    a.batch = x.size(0);
+    a.T = x.size(1);
+    a.channels = x.size(2);
+    a.K = weight.size(1);
+    a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+    if (a.K < 1 || a.K > kMostTaps) Py_RETURN_NONE;
+    in.shape(weight, {a.channels, a.K});
+    in.shape(bias, {a.channels});
+    in.shape(state, {a.sequences, a.K - 1, a.channels});
+    a.offsets = in.indices(offsets, &a.offsets64);
+    a.dtype = in.code();
+    a.activation = in.activation(3);
+    a.x = in.tokens(x, 2);
+    a.weight = in.parameter(weight);
+    a.bias = in.parameter(bias);
+    a.state_in = in.dense(state, x.scalar_type());
+    const bool keep = in.flag(6);
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(x.sizes(), x.scalar_type()), new_state;
+    a.y = in.tokens(y, 2);
+    if (keep) {
+        new_state = in.empty({a.sequences, a.K - 1, a.channels}, x.scalar_type());
+        a.state_out = new_state.data_ptr();
+    }
+    SCANSCAM_LAUNCH(operators.conv(&a, in.stream()), "conv_fwd")
+    return with_state(std::move(y), std::move(new_state));
+    END_HANDLE_TH_ERRORS
+}
+
+// conv_step(state, x, weight, bias, activation, slots)
+PyObject *conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 6, 1);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &x = in.first, state = in.tensor(0), weight = in.tensor(2), bias = in.tensor(3), slots = in.tensor(5);
+    if (!in.ok || x.dim() != 2 || x.numel() == 0 || !state.defined() || state.dim() != 3 || !weight.defined() || weight.dim() != 2) Py_RETURN_NONE;
+    scanscam_conv_step a{};
+    a.rows = x.size(0);
+    a.channels = x.size(1);
+    a.K = weight.size(1);
+    a.slots = state.size(0);
+    if (a.K < 1 || a.K > kMostTaps || (!slots.defined() && a.slots != a.rows)) Py_RETURN_NONE;
+    in.shape(weight, {a.channels, a.K});
+    in.shape(bias, {a.channels});
+    in.shape(state, {a.slots, a.K - 1, a.channels});
+    in.shape(slots, {a.rows});
+    a.slot = in.indices(slots, &a.slot64);
+    a.dtype = in.code();
+    a.activation = in.activation(4);
+    a.x = in.tokens(x, 1);
+    a.weight = in.parameter(weight);
+    a.bias = in.parameter(bias);
+    a.state = in.dense(state, x.scalar_type());
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(x.sizes(), x.scalar_type());
+    a.y = in.tokens(y, 1);
+    SCANSCAM_LAUNCH(operators.conv_step(&a, in.stream()), "conv_step_fwd")
+    state.unsafeGetTensorImpl()->bump_version();  // (written in place)
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// What the selective scan's two forms have in common: x, dt, A, B, C, D, z, dt_bias from `at` on.
+template <typename Args> bool selective_arguments(Arguments &in, int at, int lead, Args &a)
+{
+    const at::Tensor &x = in.first, dt = in.tensor(at + 1), A = in.tensor(at + 2), B = in.tensor(at + 3), C = in.tensor(at + 4), D = in.tensor(at + 5),
+                     z = in.tensor(at + 6), bias = in.tensor(at + 7);
+    if (!in.ok || x.dim() != lead + 1 || x.numel() == 0 || !dt.defined() || !A.defined() || !B.defined() || !C.defined() || A.dim() != 2 ||
+        (B.dim() != lead + 1 && B.dim() != lead + 2))
+        return false;
+    a.channels = x.size(-1);
+    a.N = A.size(1);
+    a.groups = B.dim() == lead + 2 ? B.size(lead) : 1;
+    if (a.N < 1 || a.N > kMostStates || a.groups < 1 || a.channels % a.groups != 0 || B.size(-1) != a.N) return false;
+    for (int d = 0; d < lead; d++)
+        if (B.size(d) != x.size(d)) return false;
+    in.shape(dt, x.sizes());
+    in.shape(z, x.sizes());
+    in.shape(A, {a.channels, a.N});
+    in.shape(C, B.sizes());
+    in.shape(D, {a.channels});
+    in.shape(bias, {a.channels});
+    a.dtype = in.code();
+    a.x = in.tokens(x, lead);
+    a.dt = in.tokens(dt, lead);
+    a.B = in.tokens(B, lead);
+    a.C = in.tokens(C, lead);
+    a.z = in.tokens(z, lead);
+    a.A = in.parameter(A);
+    a.D = in.parameter(D);
+    a.dt_bias = in.parameter(bias);
+    return in.ok;
+}
+
+// selective(x, dt, A, B, C, D, z, dt_bias, softplus, state, offsets, return_state)
+PyObject *selective(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 12, 0);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &x = in.first, state = in.tensor(9), offsets = in.tensor(10);
+    scanscam_selective a{};
+    if (!in.ok || !selective_arguments(in, 0, 2, a) || (offsets.defined() && (offsets.dim() != 1 || offsets.numel() < 2 || x.size(0) != 1))) Py_RETURN_NONE;
+    a.batch = x.size(0);
+    a.T = x.size(1);
+    a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+    in.shape(state, {a.sequences, a.channels, a.N});
+    a.offsets = in.indices(offsets, &a.offsets64);
+    a.state_in = static_cast<const float *>(in.dense(state, at::kFloat));
+    a.softplus = in.flag(8);
+    const bool keep = in.flag(11);
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(x.sizes(), x.scalar_type()), new_state, workspace;
+    a.y = in.tokens(y, 2);
+    if (keep) {
+        new_state = in.empty({a.sequences, a.channels, a.N}, at::kFloat);
+        a.state_out = static_cast<float *>(new_state.data_ptr());
+    }
+    a.workspace_bytes = operators.selective_workspace(&a, SCANSCAM_FORWARD);
+    if (a.workspace_bytes != 0) {
+        workspace = in.empty({(int64_t)a.workspace_bytes}, at::kByte);
+        a.workspace = workspace.data_ptr();
+    }
+    SCANSCAM_LAUNCH(operators.selective(&a, in.stream()), "selective_fwd")
+    return with_state(std::move(y), std::move(new_state));
+    END_HANDLE_TH_ERRORS
+}
+
+// selective_step(state, x, dt, A, B, C, D, z, dt_bias, softplus, slots)
+PyObject *selective_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 11, 1);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &x = in.first, state = in.tensor(0), slots = in.tensor(10);
+    scanscam_selective_step a{};
+    if (!in.ok || !state.defined() || state.dim() != 3 || !selective_arguments(in, 1, 1, a)) Py_RETURN_NONE;
+    a.rows = x.size(0);
+    a.slots = state.size(0);
+    if (!slots.defined() && a.slots != a.rows) Py_RETURN_NONE;
+    in.shape(state, {a.slots, a.channels, a.N});
+    in.shape(slots, {a.rows});
+    a.slot = in.indices(slots, &a.slot64);
+    a.softplus = in.flag(9);
+    a.state = static_cast<float *>(in.dense(state, at::kFloat));
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(x.sizes(), x.scalar_type());
+    a.y = in.tokens(y, 1);
+    SCANSCAM_LAUNCH(operators.selective_step(&a, in.stream()), "selective_step_fwd")
+    state.unsafeGetTensorImpl()->bump_version();
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// bind_operators(selective_fwd, selective_workspace_bytes, selective_step_fwd, conv_fwd, conv_step_fwd, norm_fwd): addresses.
+PyObject *bind_operators(PyObject *, PyObject *args)
+{
+    unsigned long long p[6];
+    if (!PyArg_ParseTuple(args, "KKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5)) return nullptr;
+    operators.selective = reinterpret_cast<decltype(operators.selective)>(p[0]);
+    operators.selective_workspace = reinterpret_cast<decltype(operators.selective_workspace)>(p[1]);
+    operators.selective_step = reinterpret_cast<decltype(operators.selective_step)>(p[2]);
+    operators.conv = reinterpret_cast<decltype(operators.conv)>(p[3]);
+    operators.conv_step = reinterpret_cast<decltype(operators.conv_step)>(p[4]);
+    operators.norm = reinterpret_cast<decltype(operators.norm)>(p[5]);
+    Py_RETURN_NONE;
+}
+
+template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)> PyCFunction fast()
+{
+    return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F));
+}
+
 PyMethodDef methods[] = {{"scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(scan)), METH_FASTCALL, nullptr},
                          {"leave_to_python", leave_to_python, METH_O, nullptr},
                          {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
                          {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(backward)), METH_FASTCALL, nullptr},
                          {"bind", bind, METH_VARARGS, nullptr},
+                         {"norm", fast<norm>(), METH_FASTCALL, nullptr},
+                         {"conv", fast<conv>(), METH_FASTCALL, nullptr},
+                         {"conv_step", fast<conv_step>(), METH_FASTCALL, nullptr},
+                         {"selective", fast<selective>(), METH_FASTCALL, nullptr},
+                         {"selective_step", fast<selective_step>(), METH_FASTCALL, nullptr},
+                         {"bind_operators", bind_operators, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -95,6 +95,24 @@ def _lib():
     return _entry_points
 
 
+def _bind_native():
+    """The host path of calls without gradients in native code (csrc/torch_binding.cpp), or ``None`` where it is not built or the
+    library is a build without these operators; such calls then go through the functions below, three times as slowly on the host."""
+    if hip._native is None or not hasattr(hip._native, "bind_operators"):
+        return None
+    try:
+        lib = _lib()
+    except RuntimeError:
+        return None
+    hip._native.bind_operators(*(ctypes.cast(fn, _p).value for fn in (
+        lib.scanscam_selective_fwd, lib.scanscam_selective_workspace_bytes, lib.scanscam_selective_step_fwd, lib.scanscam_conv_fwd,
+        lib.scanscam_conv_step_fwd, lib.scanscam_norm_fwd)))
+    return hip._native
+
+
+_native = _bind_native()
+
+
 def _raise(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"scanscam_{what}: {hip.strerror(rc)}")
@@ -228,6 +246,10 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     :param return_state: hand back the states after the last tokens as well, in float32
     :return: y, or ``(y, state)``. Differentiable in every tensor but ``offsets``.
     """
+    if _native is not None and _parts == 0 and not torch.compiler.is_compiling():
+        out = _native.selective(x, dt, A, B, C, D, z, dt_bias, softplus, state, offsets, return_state)  # None: a call it leaves to the code below
+        if out is not None:
+            return out
     what = "selective_scan"
     if x.dim() != 3:
         raise AssertionError(f"{what}: x must be [batch, T, channels], got shape {tuple(x.shape)}")
@@ -340,6 +362,10 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         slot is not in ``state``, such as -1, is left out: its output is zero and no state changes.
     :return: y, [rows, channels]. Not differentiable.
     """
+    if _native is not None and not torch.compiler.is_compiling():
+        out = _native.selective_step(state, x, dt, A, B, C, D, z, dt_bias, softplus, slots)
+        if out is not None:
+            return out
     what = "selective_scan_step"
     if x.dim() != 2 or state.dim() != 3 or A.dim() != 2 or B.dim() not in (2, 3) or not 1 <= A.shape[1] <= _MOST_STATES:
         raise AssertionError(f"{what}: x must be [rows, channels], state [slots, channels, N], A [channels, N], B [rows, (groups,) N], "
@@ -372,6 +398,7 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
                            _TYPES[x.dtype], int(softplus), 0, _tokens(x, 1), _tokens(dt, 1), _tokens(B, 1), _tokens(C, 1), _tokens(z, 1),
                            _tokens(y, 1), _param(A), _param(D), _param(dt_bias), state.data_ptr())
         _raise(L.scanscam_selective_step_fwd(a, _stream(x.device)), "selective_step_fwd")
+    torch.autograd.graph.increment_version(state)  # (written in place)
     return y
 
 
@@ -390,6 +417,10 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     :param return_state: hand back the K - 1 inputs before the next token as well
     :return: y, or ``(y, state)``. Differentiable in every tensor but ``offsets``.
     """
+    if _native is not None and not torch.compiler.is_compiling():
+        out = _native.conv(x, weight, bias, activation, state, offsets, return_state)
+        if out is not None:
+            return out
     what = "causal_conv"
     if x.dim() != 3 or weight.dim() != 2 or not 1 <= weight.shape[1] <= _MOST_TAPS:
         raise AssertionError(f"{what}: x must be [batch, T, channels] and weight [channels, 1 to {_MOST_TAPS} taps], got {tuple(x.shape)} and {tuple(weight.shape)}")
@@ -477,6 +508,10 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     :param x: [rows, channels]; weight, bias, activation as for ``causal_conv``; slots as for ``selective_scan_step``
     :return: y, [rows, channels]. Not differentiable.
     """
+    if _native is not None and not torch.compiler.is_compiling():
+        out = _native.conv_step(state, x, weight, bias, activation, slots)
+        if out is not None:
+            return out
     what = "causal_conv_step"
     if x.dim() != 2 or state.dim() != 3 or weight.dim() != 2 or not 1 <= weight.shape[1] <= _MOST_TAPS:
         raise AssertionError(f"{what}: x must be [rows, channels], state [slots, K - 1, channels], weight [channels, 1 to {_MOST_TAPS} taps], "
@@ -501,6 +536,7 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         a = _ConvStep(rows, channels, K, state.shape[0], _ptr(slots), int(slots is not None and slots.dtype == torch.int64), _TYPES[x.dtype],
                       _ACTIVATIONS[activation], 0, _tokens(x, 1), _tokens(y, 1), _param(weight), _param(bias), state.data_ptr())
         _raise(L.scanscam_conv_step_fwd(a, _stream(x.device)), "conv_step_fwd")
+    torch.autograd.graph.increment_version(state)
     return y
 
 
@@ -521,6 +557,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     :return: y; with a residual ``(y, sum)``; with ``quant`` ``(q, scale)`` or ``(q, scale, sum)``, scale being float32 and of x's
         leading shape. Differentiable (in x, weight and residual) unless ``quant`` is given.
     """
+    if _native is not None and not torch.compiler.is_compiling():
+        out = _native.norm(x, weight, residual, eps, _EIGHT.get(quant, -1) if quant is not None else 0)
+        if out is not None:
+            return out
     what = "rms_norm"
     if x.dim() < 1 or x.shape[-1] > _MOST_NORM_CHANNELS:
         raise AssertionError(f"{what}: x must be [..., up to {_MOST_NORM_CHANNELS} channels], got shape {tuple(x.shape)}")

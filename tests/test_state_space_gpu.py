@@ -389,3 +389,67 @@ def test_calls_use_the_current_stream(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, f.selective_scan(**dict(d, x=f.causal_conv(f.rms_norm(d["x"] * scale, col), w)), softplus=True))
+
+
+def test_native_host_path_is_the_python_path(gpu, monkeypatch):
+    """Calls without gradients take the native host path, and give what the Python one gives; what it does not cover it leaves alone."""
+    assert state_space._native is not None
+    taken = []
+
+    class Counted:
+        def __getattr__(self, name):
+            def call(*args):
+                out = getattr(state_space.hip._native, name)(*args)
+                taken.append((name, out is not None))
+                return out
+            return call
+
+    def both(fn, *args, covered=True, **kwargs):
+        fresh = lambda: ([a.clone() if torch.is_tensor(a) and a.is_contiguous() else a for a in args], kwargs)  # noqa: E731
+        outs = []
+        for native in (Counted(), None):
+            monkeypatch.setattr(state_space, "_native", native)
+            a, k = fresh()
+            versions = a[0]._version
+            out = fn(*a, **k)
+            outs.append([*(out if isinstance(out, tuple) else (out,)), *([a[0], torch.tensor(a[0]._version - versions)] if fn.__name__.endswith("step") else [])])
+        assert taken.pop()[1] == covered and len(outs[0]) == len(outs[1]), fn.__name__
+        for p, q in zip(*outs):
+            assert p.dtype == q.dtype and p.shape == q.shape and torch.equal(p.float(), q.float()), fn.__name__
+
+    for dtype in (torch.bfloat16, torch.float32):
+        v = make_scan(17, dtype, 0, 0, 40, 16, groups=2, lengths=[70, 0, 33], state=True)
+        d = {k: None if t is None else t.to(gpu) for k, t in v.items()}
+        args = [d[k] for k in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")]
+        both(f.selective_scan, *args, softplus=True, state=d["state"], offsets=d["offsets"], return_state=True)
+        both(f.selective_scan, *args[:5], softplus=True)
+        both(f.selective_scan, *args[:3], d["B"][:, :, 0], d["C"][:, :, 0], d["D"], softplus=True)
+        both(f.selective_scan, *args[:2], d["A"].t().contiguous().t(), *args[3:], softplus=True, covered=False)
+        wide = torch.cat((d["x"], d["z"]), -1)
+        both(f.selective_scan, wide[..., :40], d["dt"], *args[2:6], wide[..., 40:], d["dt_bias"], softplus=True)
+        token = [None if t is None else t[0, :5] if t.dim() > 2 else t for t in args]
+        both(f.selective_scan_step, torch.randn(7, 40, 16, device=gpu), *token, softplus=True, slots=torch.tensor([3, 0, -1, 6, 2], device=gpu))
+        both(f.selective_scan_step, torch.randn(5, 40, 16, device=gpu), *token, softplus=True)
+        w, b = torch.randn(40, 4, device=gpu), torch.randn(40, device=gpu)
+        kept = torch.randn(3, 3, 40, device=gpu).to(dtype)
+        both(f.causal_conv, d["x"], w, b, activation="silu", state=kept, offsets=d["offsets"], return_state=True)
+        both(f.causal_conv, wide[..., :40], w)
+        both(f.causal_conv_step, torch.randn(7, 3, 40, device=gpu).to(dtype), token[0], w, b, activation="silu", slots=torch.tensor([3, 0, -1, 6, 2], dtype=torch.int32, device=gpu))
+        for quant in (None, torch.int8, torch.float8_e4m3fn):
+            both(f.rms_norm, d["x"], b, quant=quant)
+            both(f.rms_norm, wide[..., :40], b, d["z"].float(), quant=quant, eps=1e-3)
+        both(f.rms_norm, d["x"].transpose(0, 1).expand(103, 2, 40), b, covered=False)
+    with torch.no_grad():
+        both(f.rms_norm, d["x"].requires_grad_(), b)
+    for name, call in (("norm", lambda: f.rms_norm(d["x"], b)), ("selective", lambda: f.selective_scan(*[d[k] for k in ("x", "dt", "A", "B", "C")]))):
+        monkeypatch.setattr(state_space, "_native", Counted())
+        assert call().requires_grad and taken.pop() == (name, False)
+    with pytest.raises(TypeError):
+        f.rms_norm(b, b, quant=torch.uint8)
+
+
+def test_calls_on_a_device_that_is_not_current_and_errors(gpu):
+    with pytest.raises(RuntimeError, match="on cpu"):
+        f.rms_norm(torch.ones(3, device=gpu), torch.ones(3))
+    with pytest.raises(RuntimeError, match="on cpu"):
+        f.causal_conv_step(torch.ones(1, 3, 2), torch.ones(1, 2, device=gpu), torch.ones(2, 4, device=gpu))

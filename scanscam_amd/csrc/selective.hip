@@ -29,7 +29,7 @@ int check_selective(const scanscam_selective *a)
     if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->sequences >= kMostTokens || a->parts < 0 || a->parts > kMostParts) return SCANSCAM_EINVAL;
     if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
     // (a launch has fewer than 2^32 threads)
-    if (a->sequences * (a->groups + a->channels / kBwdChannels) * (a->parts > 0 ? a->parts : 1) >= int64_t(1) << 23) return SCANSCAM_EINVAL;
+    if ((a->sequences * (a->parts > 0 ? a->parts : 1) + 512) * (a->groups + a->channels / kBwdChannels) >= int64_t(1) << 23) return SCANSCAM_EINVAL;
     if (a->batch > 0 && a->T >= (int64_t(1) << 31) / a->N / a->batch) return SCANSCAM_EINVAL;
     if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
     SCANSCAM_CHECK(check_param(a->A, true));
@@ -52,18 +52,25 @@ hipError_t launch_wide(Kernel kernel, dim3 grid, int threads, int words, hipStre
 }
 
 struct Plan {
-    int split;      // forwards: waves that share the states of a channel out among them
-    int64_t parts;  // that the time of every sequence is cut into
+    int split;     // forwards: waves that share the states of a channel out among them
+    int64_t span;  // tokens of a part that the time of a sequence is cut into; packed ones that are not longer stay whole
 };
 
 int64_t forward_blocks(const scanscam_selective &a, int split) { return ceil_div(a.channels / a.groups, kFwdWaves / split * kRows); }
 int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels); }
 
-// Parts of time for `wanted` workgroups, whole tiles each.
-int64_t parts_for(const scanscam_selective &a, int64_t workgroups, int64_t wanted)
+// Parts of one length for about two workgroups a CU, whole tiles each.
+int64_t span_for(const scanscam_selective &a, int64_t blocks, int64_t shortest)
 {
-    const int64_t tiles = ceil_div(a.T, kTile), parts = ceil_div(wanted, workgroups > 0 ? workgroups : 1);
-    return tiles < 1 ? 1 : parts < tiles ? parts : tiles;
+    const int64_t tiles = (a.offsets != nullptr ? 1 : a.sequences) * ceil_div(a.T, kTile) * a.groups * blocks, each = ceil_div(tiles, 512);
+    return (each > shortest ? each : shortest) * kTile;
+}
+
+// Parts that were asked for (a measurement's, or a test's).
+int64_t span_of(const scanscam_selective &a)
+{
+    const int64_t each = ceil_div(ceil_div(a.T, kTile), a.parts);
+    return (each > 0 ? each : 1) * kTile;
 }
 
 // Two workgroups fit a CU, and one keeps it nearly as busy, so that from 192 workgroups on nothing is cut. Below, sharing the states
@@ -71,36 +78,46 @@ int64_t parts_for(const scanscam_selective &a, int64_t workgroups, int64_t wante
 // (bf16, N = 16, us: [4, 2048, 1024] 128 whole, 93 by two waves, 105 in 4 parts; [6, 2048, 1024] 139, 137, 156); four
 // or eight waves have too little to do for the tokens' own work and the barriers, so that with fewer channels parts win where there are
 // tiles for them ([2, 2048, 1024] 127 whole, 72 by four waves, 63 in 8 parts; [1, 2048, 1024] 128, 70, 40 in 16), and not in
-// short sequences ([1, 512, 2048] 39 whole, 26 by four waves, 30 in 4 parts).
+// short sequences ([1, 512, 2048] 39 whole, 26 by four waves, 30 in 4 parts). Packed sequences differ in length, and the longest may take
+// longer than all work shared out evenly: two waves then halve the time that one workgroup is busy with it (13 sequences, 8021
+// tokens, 2048 channels, six sets of lengths, one wave / two waves / cut into parts of four tiles: 130/159/224, 149/146/187, 311/219/209,
+// 132/143/180, 162/146/191, 118/141/206 us).
 Plan forward_plan(const scanscam_selective &a)
 {
-    Plan p{1, a.parts > 0 ? a.parts : 1};
+    if (a.parts > 0) return {1, span_of(a)};
     const int64_t whole = a.sequences * a.groups * forward_blocks(a, 1);
-    const bool long_enough = ceil_div(a.T, kTile) >= 8;
-    if (whole < 192 && (whole >= 96 || !long_enough)) {
-        while (p.split < kFwdWaves && p.split < a.N && (whole >= 96 ? p.split < 2 : a.sequences * a.groups * forward_blocks(a, p.split) < 256)) p.split *= 2;
-    } else if (whole < 96 && a.parts == 0) {
-        p.parts = parts_for(a, whole, 512);
+    if (whole >= 192) return {a.offsets != nullptr && whole < 1024 && a.N > 1 ? 2 : 1, kWhole};
+    Plan p{1, kWhole};
+    if (whole >= 96) {
+        p.split = a.N > 1 ? 2 : 1;
+    } else if (ceil_div(a.T, kTile) >= 8) {
+        p.span = span_for(a, forward_blocks(a, 1), 1);
+    } else {
+        while (p.split < kFwdWaves && p.split < a.N && a.sequences * a.groups * forward_blocks(a, p.split) < 256) p.split *= 2;
     }
     return p;
 }
 Plan backward_plan(const scanscam_selective &a)
 {
-    const int64_t whole = a.sequences * a.groups * backward_blocks(a);
-    return {1, a.parts > 0 ? a.parts : whole < 256 ? parts_for(a, whole, 512) : 1};
+    if (a.parts > 0) return {1, span_of(a)};
+    const int64_t blocks = backward_blocks(a), whole = a.sequences * a.groups * blocks;
+    return {1, whole < 256 ? span_for(a, blocks, 1) : a.offsets != nullptr ? span_for(a, blocks, 4) : kWhole};
 }
 
-size_t ends_words(const scanscam_selective &a, int64_t parts) { return parts > 1 ? (size_t)(a.sequences * parts * (a.N + 1) * a.channels) : 0; }
+// Whether any sequence can be longer than a part.
+bool cut(const scanscam_selective &a, int64_t span) { return a.T > span; }
+
+size_t ends_words(const scanscam_selective &a, int64_t span) { return cut(a, span) ? (size_t)(all_units(a, span) * (a.N + 1) * a.channels) : 0; }
 size_t bc_words(const scanscam_selective &a) { return (size_t)(a.groups * backward_blocks(a) * a.batch * a.T * 2 * a.N); }
 
 template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream_t stream)
 {
     constexpr int K = kTokensALane;
     const Plan plan = forward_plan(a);
-    const SelectiveArgs args{a, plan.split, forward_blocks(a, plan.split), plan.parts, static_cast<float *>(a.workspace), nullptr, nullptr};
-    const dim3 grid((unsigned)(a.groups * args.blocks * a.sequences * plan.parts));
+    const SelectiveArgs args{a, plan.split, forward_blocks(a, plan.split), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
+    const dim3 grid((unsigned)(a.groups * args.blocks * all_units(a, plan.span)));
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
-    if (plan.parts > 1) {
+    if (cut(a, plan.span)) {
         const hipError_t err = launch_wide(selective_fwd_kernel<ST, K, true>, grid, kFwdWaves * 64, words, stream, args);
         if (err != hipSuccess) return err;
     }
@@ -111,21 +128,21 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
 {
     constexpr int K = kTokensALane;
     const Plan plan = backward_plan(a);
-    const int64_t blocks = backward_blocks(a);
-    float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.parts), *sums = bc + bc_words(a);
-    const SelectiveArgs args{a, 1, blocks, plan.parts, ends, bc, sums};
-    const dim3 grid((unsigned)(a.groups * blocks * a.sequences * plan.parts));
+    const int64_t blocks = backward_blocks(a), units = all_units(a, plan.span);
+    float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.span), *sums = bc + bc_words(a);
+    const SelectiveArgs args{a, 1, blocks, plan.span, ends, bc, sums};
+    const dim3 grid((unsigned)(a.groups * blocks * units));
     const int words = BackwardLds<K>::words((int)a.N);
     hipError_t err = hipSuccess;
-    if (plan.parts > 1) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
+    if (cut(a, plan.span)) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
     if (err == hipSuccess) err = launch_wide(selective_bwd_kernel<ST, K, false>, grid, kBwdWaves * 64, words, stream, args);
     const int64_t values = a.batch * a.T * 2 * a.N;
     if (err == hipSuccess && values > 0)
         err = launch_op(selective_bc_kernel<ST>, dim3((unsigned)ceil_div(values, 256), (unsigned)a.groups), dim3(256), 0, stream, GroupSum{a, bc, blocks});
-    const int64_t pitch = (a.N + 2) * a.channels, rows = a.sequences * plan.parts;
-    if (err == hipSuccess) err = column_sum(sums, a.gA, rows, pitch, a.N * a.channels, stream);
-    if (err == hipSuccess && a.gD != nullptr) err = column_sum(sums + a.N * a.channels, a.gD, rows, pitch, a.channels, stream);
-    if (err == hipSuccess && a.gdt_bias != nullptr) err = column_sum(sums + (a.N + 1) * a.channels, a.gdt_bias, rows, pitch, a.channels, stream);
+    const int64_t pitch = (a.N + 2) * a.channels;
+    if (err == hipSuccess) err = column_sum(sums, a.gA, units, pitch, a.N * a.channels, stream);
+    if (err == hipSuccess && a.gD != nullptr) err = column_sum(sums + a.N * a.channels, a.gD, units, pitch, a.channels, stream);
+    if (err == hipSuccess && a.gdt_bias != nullptr) err = column_sum(sums + (a.N + 1) * a.channels, a.gdt_bias, units, pitch, a.channels, stream);
     return err;
 }
 
@@ -166,9 +183,9 @@ size_t scanscam_selective_saved_bytes(const scanscam_selective *a)
 size_t scanscam_selective_workspace_bytes(const scanscam_selective *a, int direction)
 {
     if (a == nullptr || check_sizes(a->channels, a->groups, a->N, a->dtype) != SCANSCAM_OK || a->batch <= 0 || a->T < 0 || a->sequences <= 0) return 0;
-    if (direction == SCANSCAM_FORWARD) return ends_words(*a, forward_plan(*a).parts) * sizeof(float);
-    const int64_t parts = backward_plan(*a).parts;
-    return (ends_words(*a, parts) + bc_words(*a) + (size_t)(a->sequences * parts * (a->N + 2) * a->channels)) * sizeof(float);
+    if (direction == SCANSCAM_FORWARD) return ends_words(*a, forward_plan(*a).span) * sizeof(float);
+    const int64_t span = backward_plan(*a).span;
+    return (ends_words(*a, span) + bc_words(*a) + (size_t)(all_units(*a, span) * (a->N + 2) * a->channels)) * sizeof(float);
 }
 
 int scanscam_selective_fwd(const scanscam_selective *a, void *stream)

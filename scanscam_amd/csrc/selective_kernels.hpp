@@ -117,33 +117,69 @@ __device__ __forceinline__ float rows_sum(float v0, float v1, float v2, float v3
     return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
 
-// The stretch of tokens that a workgroup goes through: one of `parts` of a sequence, whole tiles from the sequence's start on.
+// The stretch of tokens that a workgroup goes through: a part of a sequence, `span` tokens (whole tiles) from its start on, one of
+// `parts`. Parts are numbered through all sequences. Those of packed ones are counted from their starts, without a look at the
+// sequences before: one of L tokens has at most L / span + 1 parts, so that sequence s begins with number start / span + s.
+// Numbers that no part has (`part` is then past the last one) get a stretch without tokens.
 struct Stretch {
-    int64_t seq, batch, part, start, end, tile;  // tile: number of its first tile among all sequences', for `saved`
+    int64_t seq, batch, part, parts, unit, start, end, tile;  // unit: its number; tile: that of its first tile, for `saved`, counted likewise
+    __device__ __forceinline__ bool last() const { return part == parts - 1; }
 };
-// A sequence of L tokens has at most L / TILE + 1 tiles, so that packed ones can be counted from their starts.
-template <int TILE> __device__ __forceinline__ Stretch stretch_of(const scanscam_selective &a, int64_t unit, int64_t parts)
+constexpr int64_t kWhole = int64_t(1) << 40;  // a span that cuts nothing
+
+// The longest of up to 64 packed sequences, the next one, ...: what runs longest has to begin first (a workgroup has a sequence's
+// whole time to go through). A lane has a sequence; every wave counts for each of them those that come before it.
+__device__ __forceinline__ int64_t by_length(const scanscam_selective &a, int64_t unit)
+{
+    const int lane = threadIdx.x & 63, sequences = (int)a.sequences;
+    const int at = lane < sequences ? lane : sequences - 1;
+    const int length = (int)(clamp_(index_at(a.offsets, a.offsets64, at + 1), 0, a.T) - clamp_(index_at(a.offsets, a.offsets64, at), 0, a.T));
+    int before = 0;
+    for (int j = 0; j < sequences; j++) {
+        const int other = __builtin_amdgcn_readlane(length, j);
+        before += other > length || (other == length && j < lane);
+    }
+    return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < sequences && before == (int)unit));
+}
+
+template <int TILE> __device__ __forceinline__ Stretch stretch_of(const scanscam_selective &a, int64_t unit, int64_t span)
 {
     Stretch s;
-    s.seq = unit / parts;
-    s.part = unit - s.seq * parts;
+    if (a.offsets != nullptr && span == kWhole && a.sequences <= 64) unit = by_length(a, unit);
+    s.unit = unit;
     s.batch = 0;
     if (a.offsets == nullptr) {
-        s.batch = s.seq;
+        const int64_t each = a.T > span ? (a.T + span - 1) / span : 1;
+        s.seq = s.batch = unit / each;
+        s.part = unit - s.seq * each;
         s.start = 0;
         s.end = a.T;
         s.tile = s.seq * ((a.T + TILE - 1) / TILE);
     } else {
-        s.start = clamp_(index_at(a.offsets, a.offsets64, s.seq), 0, a.T);
-        s.end = clamp_(index_at(a.offsets, a.offsets64, s.seq + 1), s.start, a.T);
-        s.tile = s.start / TILE + s.seq;
+        int64_t lo = 0, hi = a.sequences - 1;  // the last sequence that begins with this number or a lower one
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) >> 1;
+            if (clamp_(index_at(a.offsets, a.offsets64, mid), 0, a.T) / span + mid <= unit) lo = mid;
+            else hi = mid - 1;
+        }
+        s.seq = lo;
+        s.start = clamp_(index_at(a.offsets, a.offsets64, lo), 0, a.T);
+        s.end = clamp_(index_at(a.offsets, a.offsets64, lo + 1), s.start, a.T);
+        s.part = unit - s.start / span - lo;
+        s.part = s.part < 0 ? 0 : s.part;
+        s.tile = s.start / TILE + lo;
     }
-    const int64_t tiles = (s.end - s.start + TILE - 1) / TILE, each = (tiles + parts - 1) / parts;
-    const int64_t from = s.part * each < tiles ? s.part * each : tiles, to = from + each < tiles ? from + each : tiles;
-    s.end = to < tiles ? s.start + to * TILE : s.end;
-    s.start = from < tiles ? s.start + from * TILE : s.end;
-    s.tile += from;
+    const int64_t length = s.end - s.start, from = s.part * span < length ? s.part * span : length;
+    s.parts = length > span ? (length + span - 1) / span : 1;
+    s.tile += from / TILE;
+    s.start += from;
+    s.end = s.start + span < s.end ? s.start + span : s.end;
     return s;
+}
+// The numbers that there are.
+__host__ __device__ inline int64_t all_units(const scanscam_selective &a, int64_t span)
+{
+    return a.offsets == nullptr ? a.sequences * (a.T > span ? ceil_div(a.T, span) : 1) : a.T / span + a.sequences;
 }
 __host__ __device__ inline int64_t all_tiles(const scanscam_selective &a, int64_t tile)
 {
@@ -290,10 +326,10 @@ struct SelectiveArgs {
     scanscam_selective a;
     int split;        // forwards: waves that share the states of a channel out among them
     int64_t blocks;   // of channels, in a group
-    int64_t parts;    // that the time of every sequence is cut into
-    float *ends;      // [sequences][parts][N + 1][channels]: the states that a part alone ends with (backwards: starts with), its sum of d
+    int64_t span;     // tokens of a part of a sequence
+    float *ends;      // [parts of all sequences][N + 1][channels]: the states that a part alone ends with (backwards: starts with), its sum of d
     float *bc;        // backwards: [blocks of all groups][tokens][2][N], sums of gB and gC over a workgroup's channels
-    float *sums;      // backwards: [sequences][parts][N + 2][channels], sums over a part's tokens for A, D and dt_bias
+    float *sums;      // backwards: [parts of all sequences][N + 2][channels], sums over a part's tokens for A, D and dt_bias
 };
 
 // Workgroups are dealt out to the 8 dies in turn, each with an L2 cache of its own, while neighbouring blocks of channels share the
@@ -320,8 +356,9 @@ __device__ __forceinline__ float carried(const SelectiveArgs &args, const Stretc
 {
     const scanscam_selective &a = args.a;
     const int64_t pitch = (a.N + 1) * a.channels;
-    const float *ends = args.ends + s.seq * args.parts * pitch + channel;
-    for (int64_t q = forwards ? 0 : args.parts - 1; forwards ? q < s.part : q > s.part; q += forwards ? 1 : -1)
+    const float *ends = args.ends + (s.unit - s.part) * pitch + channel;
+    if (s.part >= s.parts) return h;
+    for (int64_t q = forwards ? 0 : s.parts - 1; forwards ? q < s.part : q > s.part; q += forwards ? 1 : -1)
         h = __builtin_fmaf(__builtin_amdgcn_exp2f(A * ends[q * pitch + a.N * a.channels]), h, ends[q * pitch + n * a.channels]);
     return h;
 }
@@ -361,8 +398,8 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     const int64_t group = w.block / args.blocks, c0 = (w.block - group * args.blocks) * channels;  // c0: inside the group
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;  // first channel
-    const Stretch s = stretch_of<TILE>(a, w.unit, args.parts);
-    if (ENDS && s.part == args.parts - 1) return;  // (nothing follows it)
+    const Stretch s = stretch_of<TILE>(a, w.unit, args.span);
+    if (ENDS && s.part >= s.parts - 1) return;  // (nothing follows it)
     const bool gated = !ENDS && a.z.p != nullptr;
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = lane >> 4, tl = lane & 15;
@@ -467,7 +504,6 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
             G::read(lu + ch * P, tl, u);
 #pragma unroll
             for (int k = 0; k < K; k++) total += d[k];
-#pragma unroll 2
             for (int n = part; n < states; n += split) {
                 Carry *carry = lh + (n0 + n) * channels + ch;
                 const Carry c = *carry;
@@ -529,7 +565,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     }
     __syncthreads();
     if (ENDS) {
-        float *to = args.ends + (s.seq * args.parts + s.part) * (N + 1) * a.channels + first;
+        float *to = args.ends + s.unit * (N + 1) * a.channels + first;
         for (int i = threadIdx.x; i < channels * N; i += kThreads) {
             const int n = i / channels, c = i - n * channels;
             if (c < here) to[(int64_t)n * a.channels + c] = lh[i].h;
@@ -544,7 +580,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
             for (int t = 0; t < t_step; t++) sum += red[t * channels + threadIdx.x];
             to[(int64_t)N * a.channels + threadIdx.x] = sum;
         }
-    } else if (a.state_out != nullptr && s.part == args.parts - 1) {
+    } else if (a.state_out != nullptr && s.last()) {
         for (int i = threadIdx.x; i < channels * N; i += kThreads) {
             const int c = i / N, n = i - c * N;
             if (c < here) a.state_out[(s.seq * a.channels + first + c) * N + n] = lh[n * channels + c].h;
@@ -592,8 +628,8 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     const int64_t group = w.block / args.blocks, c0 = (w.block - group * args.blocks) * channels;
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;
-    const Stretch s = stretch_of<TILE>(a, w.unit, args.parts);
-    if (ENDS && s.part == 0) return;
+    const Stretch s = stretch_of<TILE>(a, w.unit, args.span);
+    if (ENDS && (s.part == 0 || s.part >= s.parts)) return;
     const bool gated = a.z.p != nullptr;
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = lane >> 4, tl = lane & 15;
@@ -866,8 +902,8 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
         }
     }
     __syncthreads();
-    float *to = ENDS ? args.ends + (s.seq * args.parts + s.part) * (N + 1) * a.channels + first
-                     : args.sums + (s.seq * args.parts + s.part) * (N + 2) * a.channels + first * N;
+    float *to = ENDS ? args.ends + s.unit * (N + 1) * a.channels + first
+                     : args.sums + s.unit * (N + 2) * a.channels + first * N;
     for (int i = threadIdx.x; i < channels * N; i += kThreads) {
         if (ENDS) {
             const int n = i / channels, c = i - n * channels;
@@ -892,7 +928,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
         float sum = 0.0f;
         for (int t = 0; t < t_step; t++) sum += red[(t * 2 + which) * channels + c];
         if (c >= here) return;
-        if (!ENDS) args.sums[((s.seq * args.parts + s.part) * (N + 2) + N + which) * a.channels + first + c] = sum;
+        if (!ENDS) args.sums[(s.unit * (N + 2) + N + which) * a.channels + first + c] = sum;
         else if (which == 1) to[(int64_t)N * a.channels + c] = sum;
     }
 }

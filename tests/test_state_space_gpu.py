@@ -294,7 +294,8 @@ NORMS = [
     (torch.float32, None, (3, 5, 64)), (torch.float32, torch.float32, (7, 1)), (torch.float32, torch.bfloat16, (2, 2049)), (torch.float32, None, (0, 16)),
     (torch.bfloat16, None, (65, 1000)), (torch.bfloat16, torch.bfloat16, (4, 2, 2048)), (torch.bfloat16, torch.float32, (9, 4096)),
     (torch.bfloat16, torch.float32, (3, 5000)), (torch.float16, torch.float16, (5, 9001)), (torch.float16, torch.float32, (2, 32768)),
-    (torch.bfloat16, torch.float32, (3000, 40)), (torch.float16, None, (33,)),
+    (torch.bfloat16, torch.float32, (3000, 40)), (torch.float16, None, (33,)), (torch.bfloat16, torch.float32, (5, 32767)), (torch.bfloat16, None, (4, 32763)),
+    (torch.bfloat16, torch.bfloat16, (1100, 2047)), (torch.float32, None, (1030, 513)), (torch.bfloat16, torch.float32, (1024, 2560)),
 ]
 
 

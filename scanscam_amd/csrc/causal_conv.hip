@@ -5,7 +5,9 @@
 //
 // Memory bounds it: x in, y out (backwards x and gy in, gx out). A lane owns a 16-byte vector of neighbouring channels and
 // walks over a stretch of time with the last K - 1 inputs in registers, so that an element is loaded once but for the K - 1 at
-// the border of two stretches, which the caches still hold.
+// the border of two stretches, which the caches still hold. A lane whose vector would reach past the last channel takes
+// the last whole one instead and does some of its neighbour's work again, the same (fewer channels than a vector's go
+// element by element); tokens are asked for several at a time, as one token's latency is longer than its arithmetic.
 #include "ops_common.hpp"
 
 namespace scanscam {
@@ -53,14 +55,36 @@ __device__ __forceinline__ void conv_input(const scanscam_conv &a, int64_t b, co
     }
 }
 
+// Tokens asked for at a time.
+constexpr int kAhead = 4;
+
+// This lane's vector of channels: the first one, and how many there are (VEC but where there are fewer channels than that).
+template <int VEC> __device__ __forceinline__ int64_t lane_channels(int64_t channels, int64_t c, int &count)
+{
+    count = channels < VEC ? (int)channels : VEC;
+    return c < channels - count ? c : channels - count;
+}
+
+// Taps and bias of a lane's channels.
+template <int VEC, int K> struct Taps {
+    float w[VEC * K], bias[VEC];
+    __device__ __forceinline__ void load(const scanscam_param &weight, const scanscam_param &b, int64_t c, int count)
+    {
+        params(weight, c * K, count * K, w);
+        params(b, c, count, bias);
+    }
+    __device__ __forceinline__ float operator()(int i, int k) const { return w[i * K + k]; }
+};
+
 template <typename ST, int K>
 __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs args)
 {
     constexpr int VEC = 16 / sizeof(ST);
     const scanscam_conv &a = args.a;
-    const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    if (c >= a.channels) return;
-    const int count = (int)clamp_(a.channels - c, 0, VEC);
+    const int64_t mine = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    if (mine >= a.channels) return;
+    int count;
+    const int64_t c = lane_channels<VEC>(a.channels, mine, count);
     const int64_t unit = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;  // a stretch of a batch element, or a sequence's state
     const int64_t walks = a.batch * args.stretches;
     if (unit >= walks) {  // the states after the last tokens
@@ -83,36 +107,46 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs args)
     const int64_t b = unit / args.stretches, t0 = (unit - b * args.stretches) * args.stretch;
     const int64_t t1 = t0 + args.stretch < a.T ? t0 + args.stretch : a.T;
     if (t0 >= t1) return;
-    float w[K][VEC], bias[VEC];
+    Taps<VEC, K> taps;
+    taps.load(a.weight, a.bias, c, count);
+    const ST *from = static_cast<const ST *>(a.x.p) + b * a.x.batch + c;
+    ST *to = static_cast<ST *>(a.y.p) + b * a.y.batch + c;
+    float x[K][VEC];  // x[k]: the input that tap k reads
+    const auto token = [&](int64_t t) {  // x[K - 1] is there
+        float y[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; i++) {
-        const int64_t ch = c + (i < count ? i : 0);
-        bias[i] = param(a.bias, ch);
+        for (int i = 0; i < VEC; i++) {
+            y[i] = taps.bias[i];
 #pragma unroll
-        for (int k = 0; k < K; k++) w[k][i] = param(a.weight, ch * K + k);
-    }
+            for (int k = 0; k < K; k++) y[i] = __builtin_fmaf(taps(i, k), x[k][i], y[i]);
+            y[i] = act_(y[i], a.activation);
+        }
+        store_some(to + t * a.y.token, count, y);
+#pragma unroll
+        for (int k = 0; k + 1 < K; k++) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) x[k][i] = x[k + 1][i];
+        }
+    };
     for (int64_t t = t0; t < t1;) {
         const Span s = span_at(a, b, t);
         const int64_t last = s.end < t1 ? s.end : t1;
-        float x[K][VEC];  // x[k]: the input that tap k reads
 #pragma unroll
-        for (int k = 0; k < K - 1; k++) conv_input<ST, VEC>(a, b, s, t - s.start - (K - 1) + k, K, c, count, x[k + 1]);
+        for (int k = 0; k < K - 1; k++) conv_input<ST, VEC>(a, b, s, t - s.start - (K - 1) + k, K, c, count, x[k]);
+        for (; count == VEC && t + kAhead <= last; t += kAhead) {
+            Stored<ST, VEC> ahead[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) ahead[j].load(from + (t + j) * a.x.token);
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) x[K - 1][i] = ahead[j][i];
+                token(t + j);
+            }
+        }
         for (; t < last; t++) {
-#pragma unroll
-            for (int k = 0; k + 1 < K; k++) {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) x[k][i] = x[k + 1][i];
-            }
-            load_part(static_cast<const ST *>(a.x.p) + b * a.x.batch + t * a.x.token + c, count, x[K - 1]);
-            float y[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                y[i] = bias[i];
-#pragma unroll
-                for (int k = 0; k < K; k++) y[i] = __builtin_fmaf(w[k][i], x[k][i], y[i]);
-                y[i] = act_(y[i], a.activation);
-            }
-            store_some(static_cast<ST *>(a.y.p) + b * a.y.batch + t * a.y.token + c, count, y);
+            load_part(from + t * a.x.token, count, x[K - 1]);
+            token(t);
         }
     }
 }
@@ -123,9 +157,10 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
 {
     constexpr int VEC = 16 / sizeof(ST);
     const scanscam_conv &a = args.a;
-    const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    if (c >= a.channels) return;
-    const int count = (int)clamp_(a.channels - c, 0, VEC);
+    const int64_t mine = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
+    if (mine >= a.channels) return;
+    int count;
+    const int64_t c = lane_channels<VEC>(a.channels, mine, count);
     const int64_t unit = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (unit >= a.batch * args.stretches) {
         // Sequences without a token: the state goes through as it is.
@@ -142,30 +177,47 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
     }
     const int64_t b = unit / args.stretches, t0 = (unit - b * args.stretches) * args.stretch;
     const int64_t t1 = t0 + args.stretch < a.T ? t0 + args.stretch : a.T;
-    float w[K][VEC], bias[VEC], gw[K][VEC], gb[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-        const int64_t ch = c + (i < count ? i : 0);
-        bias[i] = param(a.bias, ch);
-        gb[i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            w[k][i] = param(a.weight, ch * K + k);
-            gw[k][i] = 0.0f;
-        }
-    }
+    Taps<VEC, K> taps;
+    taps.load(a.weight, a.bias, c, count);
+    float gw[VEC * K] = {}, gb[VEC] = {};
+    const ST *from = static_cast<const ST *>(a.x.p) + b * a.x.batch + c, *from_gy = static_cast<const ST *>(a.gy.p) + b * a.gy.batch + c;
     for (int64_t t = t0; t < t1;) {
         const Span s = span_at(a, b, t);
         const int64_t first = t, last = s.end < t1 ? s.end : t1, length = s.end - s.start;
-        float x[K][VEC], gp[K][VEC];  // gp[k]: of token t - (K-1) + k
+        float x[K][VEC], gp[K][VEC];  // of the tokens t - (K-1) + k
 #pragma unroll
         for (int k = 0; k < K - 1; k++) {
-            conv_input<ST, VEC>(a, b, s, t - s.start - (K - 1) + k, K, c, count, x[k + 1]);
+            conv_input<ST, VEC>(a, b, s, t - s.start - (K - 1) + k, K, c, count, x[k]);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) gp[k + 1][i] = 0.0f;
+            for (int i = 0; i < VEC; i++) gp[k][i] = 0.0f;  // (not needed: their gx is another stretch's, or the state's)
         }
-        // (gp of the tokens before the stretch is not needed: their gx is another stretch's, or the state's)
-        for (; t < last + K - 1; t++) {
+        // gp of token t, whose x is there, from its gy; `sums`: it is the stretch's own.
+        const auto slope = [&](const float (&g)[VEC], bool sums) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                float p = taps.bias[i];
+#pragma unroll
+                for (int k = 0; k < K; k++) p = __builtin_fmaf(taps(i, k), x[k][i], p);
+                gp[K - 1][i] = g[i] * act_slope(p, a.activation);
+            }
+            if (!sums) return;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                gb[i] += gp[K - 1][i];
+#pragma unroll
+                for (int k = 0; k < K; k++) gw[i * K + k] = __builtin_fmaf(gp[K - 1][i], x[k][i], gw[i * K + k]);
+            }
+        };
+        // The input K - 1 tokens back has met all its taps.
+        const auto input_gradient = [&](float (&g)[VEC]) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                g[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; k++) g[i] = __builtin_fmaf(taps(i, K - 1 - k), gp[k][i], g[i]);
+            }
+        };
+        const auto move_on = [&]() {
 #pragma unroll
             for (int k = 0; k + 1 < K; k++) {
 #pragma unroll
@@ -174,55 +226,69 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
                     gp[k][i] = gp[k + 1][i];
                 }
             }
-#pragma unroll
-            for (int i = 0; i < VEC; i++) gp[K - 1][i] = 0.0f;
+        };
+        // Any token: at the borders of stretches and sequences.
+        const auto token = [&]() {
             if (t < s.end) {
                 float g[VEC];
-                load_part(static_cast<const ST *>(a.x.p) + b * a.x.batch + t * a.x.token + c, count, x[K - 1]);
-                load_part(static_cast<const ST *>(a.gy.p) + b * a.gy.batch + t * a.gy.token + c, count, g);
+                load_part(from + t * a.x.token, count, x[K - 1]);
+                load_part(from_gy + t * a.gy.token, count, g);
+                slope(g, t < last);
+            } else {
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    float p = bias[i];
-#pragma unroll
-                    for (int k = 0; k < K; k++) p = __builtin_fmaf(w[k][i], x[k][i], p);
-                    gp[K - 1][i] = g[i] * act_slope(p, a.activation);
-                    if (t < last) {
-                        gb[i] += gp[K - 1][i];
-#pragma unroll
-                        for (int k = 0; k < K; k++) gw[k][i] = __builtin_fmaf(gp[K - 1][i], x[k][i], gw[k][i]);
-                    }
-                }
+                for (int i = 0; i < VEC; i++) gp[K - 1][i] = 0.0f;
             }
-            // The input K - 1 tokens back has met all its taps.
             const int64_t at = t - (K - 1) - s.start;  // counted from the sequence's start; the state's rows are below 0
             const bool own = t - (K - 1) >= first, state = at < 0 && first == s.start;
-            if (!own && !(state && a.gstate_in != nullptr)) continue;
-            float g[VEC];
+            if (own || (state && a.gstate_in != nullptr)) {
+                float g[VEC];
+                input_gradient(g);
+                const int64_t kept = at - (length - (K - 1));  // its row of the state after the sequence, if it is one
+                if (kept >= 0 && a.gstate_out != nullptr) {
+                    float more[VEC];
+                    load_part(static_cast<const ST *>(a.gstate_out) + (s.seq * (K - 1) + kept) * a.channels + c, count, more);
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                g[i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < K; k++) g[i] = __builtin_fmaf(w[K - 1 - k][i], gp[k][i], g[i]);
+                    for (int i = 0; i < VEC; i++) g[i] += more[i];
+                }
+                if (own) store_some(static_cast<ST *>(a.gx.p) + b * a.gx.batch + (t - (K - 1)) * a.gx.token + c, count, g);
+                else store_some(static_cast<ST *>(a.gstate_in) + (s.seq * (K - 1) + (K - 1) + at) * a.channels + c, count, g);
             }
-            const int64_t kept = at - (length - (K - 1));  // its row of the state after the sequence, if it is one
-            if (kept >= 0 && a.gstate_out != nullptr) {
-                float more[VEC];
-                load_part(static_cast<const ST *>(a.gstate_out) + (s.seq * (K - 1) + kept) * a.channels + c, count, more);
+            move_on();
+        };
+        for (; t < first + K - 1 && t < last + K - 1; t++) token();
+        // Tokens inside the stretch whose gx goes out to K - 1 tokens back, a token's row of its own, kept by no state.
+        ST *to = static_cast<ST *>(a.gx.p) + b * a.gx.batch + c;
+        for (; count == VEC && t + kAhead <= last; t += kAhead) {
+            Stored<ST, VEC> ahead[kAhead], ahead_gy[kAhead];
 #pragma unroll
-                for (int i = 0; i < VEC; i++) g[i] += more[i];
+            for (int j = 0; j < kAhead; j++) {
+                ahead[j].load(from + (t + j) * a.x.token);
+                ahead_gy[j].load(from_gy + (t + j) * a.gy.token);
             }
-            if (own) store_some(static_cast<ST *>(a.gx.p) + b * a.gx.batch + (t - (K - 1)) * a.gx.token + c, count, g);
-            else store_some(static_cast<ST *>(a.gstate_in) + (s.seq * (K - 1) + (K - 1) + at) * a.channels + c, count, g);
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                float g[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    x[K - 1][i] = ahead[j][i];
+                    g[i] = ahead_gy[j][i];
+                }
+                slope(g, true);
+                input_gradient(g);
+                store_some(to + (t + j - (K - 1)) * a.gx.token, count, g);
+                move_on();
+            }
         }
+        for (; t < last + K - 1; t++) token();
         t = last;
     }
-    float *part = args.part + unit * (K + 1) * a.channels + c;
+    float *part = args.part + unit * (K + 1) * a.channels;
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
         if (i >= count) break;
 #pragma unroll
-        for (int k = 0; k < K; k++) part[(int64_t)i * K + k + c * (K - 1)] = gw[k][i];
-        part[(int64_t)K * a.channels + i] = gb[i];
+        for (int k = 0; k < K; k++) part[(c + i) * K + k] = gw[i * K + k];
+        part[(int64_t)K * a.channels + c + i] = gb[i];
     }
 }
 
@@ -234,23 +300,38 @@ __global__ __launch_bounds__(256) void conv_step_kernel(scanscam_conv_step a)
     const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (c >= a.channels || row >= a.rows) return;
-    const int count = (int)clamp_(a.channels - c, 0, VEC);
+    const int count = (int)clamp_(a.channels - c, 0, VEC);  // (no lane does another's work again here: the state is read and written in place)
     const int64_t slot = a.slot != nullptr ? index_at(a.slot, a.slot64, row) : row;
     float y[VEC] = {};
     if (slot >= 0 && slot < a.slots) {
         ST *state = static_cast<ST *>(a.state) + slot * (K - 1) * a.channels + c;
+        const ST *from = static_cast<const ST *>(a.x.p) + row * a.x.token + c;
+        Taps<VEC, K> taps;
         float x[K][VEC];
+        if (count == VEC) {
+            Stored<ST, VEC> ahead[K];
 #pragma unroll
-        for (int k = 0; k < K - 1; k++) load_part(state + (int64_t)k * a.channels, count, x[k]);
-        load_part(static_cast<const ST *>(a.x.p) + row * a.x.token + c, count, x[K - 1]);
+            for (int k = 0; k < K - 1; k++) ahead[k].load(state + (int64_t)k * a.channels);
+            ahead[K - 1].load(from);
+            taps.load(a.weight, a.bias, c, count);
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) x[k][i] = ahead[k][i];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K - 1; k++) load_part(state + (int64_t)k * a.channels, count, x[k]);
+            load_part(from, count, x[K - 1]);
+            taps.load(a.weight, a.bias, c, count);
+        }
 #pragma unroll
         for (int k = 0; k < K - 1; k++) store_some(state + (int64_t)k * a.channels, count, x[k + 1]);
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
-            const int64_t ch = c + (i < count ? i : 0);
-            y[i] = param(a.bias, ch);
+            y[i] = taps.bias[i];
 #pragma unroll
-            for (int k = 0; k < K; k++) y[i] = __builtin_fmaf(param(a.weight, ch * K + k), x[k][i], y[i]);
+            for (int k = 0; k < K; k++) y[i] = __builtin_fmaf(taps(i, k), x[k][i], y[i]);
             y[i] = act_(y[i], a.activation);
         }
     }

@@ -92,6 +92,58 @@ __device__ __forceinline__ void store_some(ST *p, int count, const float (&f)[VE
     }
 }
 
+// Whole vectors of neighbouring elements, as they are stored: what is asked for is waited for where it is taken apart.
+template <typename ST, int VEC> struct Stored {
+    Elems<ST, VEC> e;
+    __device__ __forceinline__ void load(const ST *p)
+    {
+        constexpr int PIECE = VEC * sizeof(ST) > 16 ? 16 / sizeof(ST) : VEC;
+        using raw_t = typename RawT<sizeof(ST) * PIECE>::type;
+        typedef raw_t raw_unaligned_t __attribute__((aligned(sizeof(ST))));
+        struct Raw { raw_t r[VEC / PIECE]; } raw;
+#pragma unroll
+        for (int i = 0; i < VEC / PIECE; i++) raw.r[i] = *reinterpret_cast<const raw_unaligned_t *>(p + i * PIECE);
+        e = __builtin_bit_cast(decltype(e), raw);
+    }
+    __device__ __forceinline__ float operator[](int i) const { return (float)e.e[i]; }
+};
+
+// COUNT neighbouring elements of a parameter, of which the first `there` are there (all: in vectors).
+template <int COUNT> __device__ __forceinline__ void params(const scanscam_param &p, int64_t at, int there, float (&f)[COUNT], float fill = 0.0f)
+{
+    if (p.p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) f[i] = fill;
+    } else if (there < COUNT || COUNT % 4 != 0) {
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) f[i] = i < there ? param(p, at + i) : 0.0f;
+    } else if (p.dtype == SCANSCAM_F32) {
+#pragma unroll
+        for (int i = 0; i < COUNT; i += 4) {
+            Stored<float, 4> s;
+            s.load(static_cast<const float *>(p.p) + at + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) f[i + k] = s[k];
+        }
+    } else if (p.dtype == SCANSCAM_BF16) {
+#pragma unroll
+        for (int i = 0; i < COUNT; i += 4) {
+            Stored<__bf16, 4> s;
+            s.load(static_cast<const __bf16 *>(p.p) + at + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) f[i + k] = s[k];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; i += 4) {
+            Stored<_Float16, 4> s;
+            s.load(static_cast<const _Float16 *>(p.p) + at + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) f[i + k] = s[k];
+        }
+    }
+}
+
 // The sequence that token t of a packed stream belongs to: the last one that starts at or before t.
 __device__ __forceinline__ int64_t sequence_of(const void *offsets, int wide, int64_t sequences, int64_t t)
 {

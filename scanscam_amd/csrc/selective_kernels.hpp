@@ -971,38 +971,59 @@ __global__ __launch_bounds__(256) void selective_step_kernel(scanscam_selective_
         if (there && lane == 0) const_cast<ST *>(token_at<ST>(a.y, 0, row, c))[0] = (ST)0.0f;
         return;
     }
-    float y = 0.0f, x = 0.0f;
+    float y = 0.0f, x = 0.0f, z = 0.0f, skip = 0.0f;
     if (there) {
-        const int64_t group = c / (a.channels / a.groups);
-        x = (float)token_at<ST>(a.x, 0, row, c)[0];
-        float d = (float)token_at<ST>(a.dt, 0, row, c)[0] + param(a.dt_bias, c);
-        if (a.softplus) d = softplus_(d);
+        // (everything is asked for before any of it is used)
+        const ST x_in = token_at<ST>(a.x, 0, row, c)[0], dt_in = token_at<ST>(a.dt, 0, row, c)[0];
+        const ST z_in = a.z.p != nullptr ? token_at<ST>(a.z, 0, row, c)[0] : (ST)0.0f;
+        const int64_t group = (uint32_t)c / (uint32_t)(a.channels / a.groups);
         const ST *B = token_at<ST>(a.B, 0, row, group * a.B.group), *C = token_at<ST>(a.C, 0, row, group * a.C.group);
         float *state = a.state + (slot * a.channels + c) * N;
+        const float bias = param(a.dt_bias, c);
+        skip = param(a.D, c);
+        float d = 0.0f;
         for (int n0 = lane * 4; n0 < N; n0 += LANES * 4) {
             const int count = N - n0 < 4 ? N - n0 : 4;
-            float h[4], b[4], w[4];
-            load_part(state + n0, count, h);
-            load_part(B + n0, count, b);
-            load_part(C + n0, count, w);
+            float h[4], b[4], w[4], A[4];
+            if (count == 4) {
+                Stored<float, 4> h_in;
+                Stored<ST, 4> b_in, w_in;
+                h_in.load(state + n0);
+                b_in.load(B + n0);
+                w_in.load(C + n0);
+                params(a.A, c * N + n0, 4, A);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    h[i] = h_in[i];
+                    b[i] = b_in[i];
+                    w[i] = w_in[i];
+                }
+            } else {
+                load_part(state + n0, count, h);
+                load_part(B + n0, count, b);
+                load_part(C + n0, count, w);
+                params(a.A, c * N + n0, count, A);
+            }
+            if (n0 < LANES * 4) {
+                x = (float)x_in;
+                d = (float)dt_in + bias;
+                if (a.softplus) d = softplus_(d);
+            }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (i >= count) break;
-                const float A = param(a.A, c * N + n0 + i);
-                h[i] = __builtin_fmaf(exp_(d * A), h[i], d * x * b[i]);
+                h[i] = __builtin_fmaf(exp_(d * A[i]), h[i], d * x * b[i]);  // (past the last state: zeros)
                 y = __builtin_fmaf(w[i], h[i], y);
             }
             store_some(state + n0, count, h);
         }
+        x = (float)x_in;
+        z = (float)z_in;
     }
 #pragma unroll
     for (int m = LANES / 2; m > 0; m >>= 1) y += __shfl_xor(y, m);
     if (there && lane == 0) {
-        y = __builtin_fmaf(param(a.D, c), x, y);
-        if (a.z.p != nullptr) {
-            const float z = (float)token_at<ST>(a.z, 0, row, c)[0];
-            y *= z * sigmoid_(z);
-        }
+        y = __builtin_fmaf(skip, x, y);
+        if (a.z.p != nullptr) y *= z * sigmoid_(z);
         const_cast<ST *>(token_at<ST>(a.y, 0, row, c))[0] = (ST)y;
     }
 }

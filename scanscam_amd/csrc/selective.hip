@@ -107,6 +107,7 @@ Plan backward_plan(const scanscam_selective &a)
 // Whether any sequence can be longer than a part.
 bool cut(const scanscam_selective &a, int64_t span) { return a.T > span; }
 
+uint32_t each_of(const scanscam_selective &a, int64_t span) { return (uint32_t)(a.T > span ? ceil_div(a.T, span) : 1); }
 size_t ends_words(const scanscam_selective &a, int64_t span) { return cut(a, span) ? (size_t)(all_units(a, span) * (a.N + 1) * a.channels) : 0; }
 size_t bc_words(const scanscam_selective &a) { return (size_t)(a.groups * backward_blocks(a) * a.batch * a.T * 2 * a.N); }
 
@@ -114,8 +115,8 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
 {
     constexpr int K = kTokensALane;
     const Plan plan = forward_plan(a);
-    const SelectiveArgs args{a, plan.split, forward_blocks(a, plan.split), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
-    const dim3 grid((unsigned)(a.groups * args.blocks * all_units(a, plan.span)));
+    const SelectiveArgs args{a, plan.split, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
+    const dim3 grid((unsigned)(a.groups * (int64_t)args.blocks * all_units(a, plan.span)));
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
     if (cut(a, plan.span)) {
         const hipError_t err = launch_wide(selective_fwd_kernel<ST, K, true>, grid, kFwdWaves * 64, words, stream, args);
@@ -130,7 +131,7 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     const Plan plan = backward_plan(a);
     const int64_t blocks = backward_blocks(a), units = all_units(a, plan.span);
     float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.span), *sums = bc + bc_words(a);
-    const SelectiveArgs args{a, 1, blocks, plan.span, ends, bc, sums};
+    const SelectiveArgs args{a, 1, (uint32_t)blocks, each_of(a, plan.span), plan.span, ends, bc, sums};
     const dim3 grid((unsigned)(a.groups * blocks * units));
     const int words = BackwardLds<K>::words((int)a.N);
     hipError_t err = hipSuccess;

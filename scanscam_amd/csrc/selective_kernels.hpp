@@ -142,19 +142,27 @@ __device__ __forceinline__ int64_t by_length(const scanscam_selective &a, int64_
     return __builtin_ctzll(__builtin_amdgcn_ballot_w64(lane < sequences && before == (int)unit));
 }
 
-template <int TILE> __device__ __forceinline__ Stretch stretch_of(const scanscam_selective &a, int64_t unit, int64_t span)
+// `each`: the parts of a sequence where all have one length. (Numbers of parts and tiles have 32 bits, a division of 64 takes the
+// hundred instructions that a short call cannot hide; only packed sequences that are cut need it.)
+template <int TILE> __device__ __forceinline__ Stretch stretch_of(const scanscam_selective &a, uint32_t unit, int64_t span, uint32_t each)
 {
     Stretch s;
-    if (a.offsets != nullptr && span == kWhole && a.sequences <= 64) unit = by_length(a, unit);
-    s.unit = unit;
-    s.batch = 0;
     if (a.offsets == nullptr) {
-        const int64_t each = a.T > span ? (a.T + span - 1) / span : 1;
-        s.seq = s.batch = unit / each;
-        s.part = unit - s.seq * each;
+        const uint32_t seq = each > 1 ? unit / each : unit;
+        s.seq = s.batch = seq;
+        s.unit = unit;
+        s.part = unit - seq * each;
+        s.parts = each;
         s.start = 0;
         s.end = a.T;
-        s.tile = s.seq * ((a.T + TILE - 1) / TILE);
+        s.tile = (int64_t)seq * ((a.T + TILE - 1) / TILE);
+    } else if (span == kWhole) {
+        s.seq = s.unit = a.sequences <= 64 ? by_length(a, unit) : unit;
+        s.batch = s.part = 0;
+        s.parts = 1;
+        s.start = clamp_(index_at(a.offsets, a.offsets64, s.seq), 0, a.T);
+        s.end = clamp_(index_at(a.offsets, a.offsets64, s.seq + 1), s.start, a.T);
+        s.tile = s.start / TILE + s.seq;
     } else {
         int64_t lo = 0, hi = a.sequences - 1;  // the last sequence that begins with this number or a lower one
         while (lo < hi) {
@@ -163,17 +171,21 @@ template <int TILE> __device__ __forceinline__ Stretch stretch_of(const scanscam
             else hi = mid - 1;
         }
         s.seq = lo;
+        s.batch = 0;
+        s.unit = unit;
         s.start = clamp_(index_at(a.offsets, a.offsets64, lo), 0, a.T);
         s.end = clamp_(index_at(a.offsets, a.offsets64, lo + 1), s.start, a.T);
         s.part = unit - s.start / span - lo;
         s.part = s.part < 0 ? 0 : s.part;
+        s.parts = s.end - s.start > span ? (s.end - s.start + span - 1) / span : 1;
         s.tile = s.start / TILE + lo;
     }
-    const int64_t length = s.end - s.start, from = s.part * span < length ? s.part * span : length;
-    s.parts = length > span ? (length + span - 1) / span : 1;
-    s.tile += from / TILE;
-    s.start += from;
-    s.end = s.start + span < s.end ? s.start + span : s.end;
+    if (span != kWhole) {
+        const int64_t length = s.end - s.start, from = s.part * span < length ? s.part * span : length;
+        s.tile += from / TILE;
+        s.start += from;
+        s.end = s.start + span < s.end ? s.start + span : s.end;
+    }
     return s;
 }
 // The numbers that there are.
@@ -325,7 +337,8 @@ __device__ __forceinline__ void step_sizes(const Quad<ST> (&dt)[ITEMS], const fl
 struct SelectiveArgs {
     scanscam_selective a;
     int split;        // forwards: waves that share the states of a channel out among them
-    int64_t blocks;   // of channels, in a group
+    uint32_t blocks;  // of channels, in a group
+    uint32_t each;    // parts of a sequence where all are of one length
     int64_t span;     // tokens of a part of a sequence
     float *ends;      // [parts of all sequences][N + 1][channels]: the states that a part alone ends with (backwards: starts with), its sum of d
     float *bc;        // backwards: [blocks of all groups][tokens][2][N], sums of gB and gC over a workgroup's channels
@@ -339,15 +352,16 @@ struct SelectiveArgs {
 // kernel of the layer [8, 4096, 2048] in bf16: one by one 1328 us, 8 in turn 1282, eighths 1234; packed prompts forwards: 135,
 // 139 and 170 us.)
 struct Work {
-    int64_t block, unit;  // block of channels among all groups'; part of a sequence
+    uint32_t block, unit;  // block of channels among all groups'; part of a sequence
 };
-__device__ __forceinline__ Work work_of(int64_t blocks, bool even)
+__device__ __forceinline__ Work work_of(uint32_t blocks, bool even)
 {
     constexpr uint32_t kDies = 8;
     const uint32_t near = even ? gridDim.x / kDies : 8u, round = near * kDies;
     uint32_t i = blockIdx.x;
     if (near > 0 && i < gridDim.x / round * round) i = i / round * round + i % kDies * near + i % round / kDies;
-    return {i % blocks, i / blocks};
+    const uint32_t unit = i / blocks;
+    return {i - unit * blocks, unit};
 }
 
 // The state before a part (the gradient behind it): that of the sequence's end, taken through the parts between. A part alone
@@ -374,10 +388,10 @@ constexpr int kFwdWaves = 8;
 template <int K> struct ForwardLds {
     using G = Geometry<K>;
     static constexpr int kSums = kFwdWaves * kRows;  // channels x split: rows of sums over n
-    // floats: d and u of the channels, sums, B and C; A and the carries of all states; where lanes write that have nothing to say
+    // floats: d and u of the channels, sums, B and C; D; A and the carries of all states; where lanes write that have nothing to say
     static __host__ __device__ constexpr int words(int channels, int N)
     {
-        return 2 * channels * G::kPitch + kSums * G::kPitch + 2 * kStateBlock * G::kPitch + 2 * channels * N + 2;
+        return 2 * channels * G::kPitch + kSums * G::kPitch + 2 * kStateBlock * G::kPitch + channels + 2 * channels * N + 2;
     }
 };
 
@@ -391,14 +405,15 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     const int N = (int)a.N, split = args.split, sets = kFwdWaves / split, channels = sets * kRows;
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *ly = lu + channels * P, *lB = ly + kFwdWaves * kRows * P, *lC = lB + kStateBlock * P;
-    Carry *lh = reinterpret_cast<Carry *>(lC + kStateBlock * P), *nowhere = lh + channels * N;  // [N][channels]
+    float *lskip = lC + kStateBlock * P;
+    Carry *lh = reinterpret_cast<Carry *>(lskip + channels), *nowhere = lh + channels * N;  // [N][channels]
 
-    const int64_t per_group = a.channels / a.groups;
-    const Work w = work_of(a.groups * args.blocks, a.offsets == nullptr);
-    const int64_t group = w.block / args.blocks, c0 = (w.block - group * args.blocks) * channels;  // c0: inside the group
+    const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
+    const Work w = work_of((uint32_t)a.groups * args.blocks, a.offsets == nullptr);
+    const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * channels;  // c0: inside the group
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;  // first channel
-    const Stretch s = stretch_of<TILE>(a, w.unit, args.span);
+    const Stretch s = stretch_of<TILE>(a, w.unit, args.span, args.each);
     if (ENDS && s.part >= s.parts - 1) return;  // (nothing follows it)
     const bool gated = !ENDS && a.z.p != nullptr;
 
@@ -426,30 +441,34 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     const uint32_t c_from = count > 0 ? c_in : 0;
     const int c_count = count > 0 ? count : here;
     const bool whole = here % 4 == 0;
-    float bias[4], skip[4], sum_d[4] = {};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        bias[i] = i < count ? param(a.dt_bias, first + c_in + i) : 0.0f;
-        skip[i] = i < count ? param(a.D, first + c_in + i) : 0.0f;
-    }
+    float bias[4], sum_d[4] = {};
+    params(a.dt_bias, first + c_in, count, bias);
+    if ((int)threadIdx.x < channels) lskip[threadIdx.x] = (int)threadIdx.x < here ? param(a.D, first + threadIdx.x) : 0.0f;
     Quad<ST> x[kItems], dt[kItems], z[kItems];
     StateInputs<ST, TILE, kThreads> bc;
-    auto fetch = [&](int64_t t0) {
+    const auto fetch = [&](int64_t t0) {
         const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE), t_mine = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
             const uint32_t t = t_mine + j * t_step < length ? t_mine + j * t_step : length - 1;
             x[j].load(token_at<ST>(a.x, s.batch, t0, first), t * (uint32_t)a.x.token + c_from, c_count, whole);
             dt[j].load(token_at<ST>(a.dt, s.batch, t0, first), t * (uint32_t)a.dt.token + c_from, c_count, whole);
-            if (gated) z[j].load(token_at<ST>(a.z, s.batch, t0, first), t * (uint32_t)a.z.token + c_from, c_count, whole);
         }
         bc.load(a, s.batch, group, t0, length, 0);
+    };
+    const auto fetch_gate = [&](int64_t t0, int length) {
+        const int t_mine = again(t_in);
+#pragma unroll
+        for (int j = 0; j < kItems; j++) {
+            const uint32_t t = t_mine + j * t_step < length ? t_mine + j * t_step : length - 1;
+            z[j].load(token_at<ST>(a.z, s.batch, t0, first), t * (uint32_t)a.z.token + c_from, c_count, whole);
+        }
     };
     if (s.start < s.end) fetch(s.start);
     int64_t tile = s.tile;
     for (int64_t t0 = s.start; t0 < s.end; t0 += TILE, tile++) {
         const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
-        Quad<ST> x_now[kItems], z_now[kItems];
+        Quad<ST> x_now[kItems];
         const int t_mine = again(t_in);
         const bool full = length == TILE && here == channels;
         float d_in[kItems][4], u_in[kItems][4];
@@ -457,7 +476,6 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
             x_now[j] = x[j];
-            z_now[j] = z[j];
 #pragma unroll
             for (int i = 0; i < 4; i++) u_in[j][i] = d_in[j][i] * x[j][i];
         }
@@ -497,6 +515,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
                 }
                 __syncthreads();
             }
+            if (gated && n0 == 0) fetch_gate(t0, length);
             if (n0 + kStateBlock < N) bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
             else if (t0 + TILE < s.end) fetch(t0 + TILE);
             float d[K], u[K], total = 0.0f;
@@ -548,6 +567,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
             if (t >= length || count <= 0) continue;
             float out[4];
             const float *sums = ly + c_in * P + G::place(t);
+            const float4v skip = *reinterpret_cast<const float4v *>(lskip + c_in);
 #pragma unroll
             for (int i = 0; i < 4; i++) out[i] = __builtin_fmaf(skip[i], x_now[j][i], sums[i * P]);
 #pragma unroll 1
@@ -558,7 +578,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
             }
             if (gated) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) out[i] *= z_now[j][i] * sigmoid_(z_now[j][i]);
+                for (int i = 0; i < 4; i++) out[i] *= z[j][i] * sigmoid_(z[j][i]);
             }
             store_quad(const_cast<ST *>(token_at<ST>(a.y, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.y.token + c_from, count, whole, out);
         }
@@ -623,12 +643,12 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     Carry *lG = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
     float *lS = reinterpret_cast<float *>(lG + slots), *lh = lS + slots, *nowhere = lh + channels * kStateBlock;  // lh: [16][channels]
 
-    const int64_t per_group = a.channels / a.groups;
-    const Work w = work_of(a.groups * args.blocks, a.offsets == nullptr);
-    const int64_t group = w.block / args.blocks, c0 = (w.block - group * args.blocks) * channels;
+    const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
+    const Work w = work_of((uint32_t)a.groups * args.blocks, a.offsets == nullptr);
+    const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * channels;
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;
-    const Stretch s = stretch_of<TILE>(a, w.unit, args.span);
+    const Stretch s = stretch_of<TILE>(a, w.unit, args.span, args.each);
     if (ENDS && (s.part == 0 || s.part >= s.parts)) return;
     const bool gated = a.z.p != nullptr;
 
@@ -655,11 +675,8 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     const int c_count = count > 0 ? count : here;
     const bool whole = here % 4 == 0;
     float bias[4], skip[4], sum_skip[4] = {}, sum_bias[4] = {};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        bias[i] = i < count ? param(a.dt_bias, first + c_in + i) : 0.0f;
-        skip[i] = i < count ? param(a.D, first + c_in + i) : 0.0f;
-    }
+    params(a.dt_bias, first + c_in, count, bias);
+    params(a.D, first + c_in, count, skip);
     const int64_t tiles = (s.end - s.start + TILE - 1) / TILE;
     Quad<ST> x[kItems], dt[kItems], gy[kItems], z[kItems];
     StateInputs<ST, TILE, kThreads> bc;
@@ -858,7 +875,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
             }
             bc.arrive();
             asm volatile("" : "+v"(h_saved));
-            float *to = args.bc + ((w.block * a.batch + s.batch) * a.T + t0) * 2 * N + n0;
+            float *to = args.bc + (((int64_t)w.block * a.batch + s.batch) * a.T + t0) * 2 * N + n0;
             const int thread = again((int)threadIdx.x);
 #pragma unroll
             for (int j = 0; j < TILE * 2 * kStateBlock / 4 / kThreads; j++) {

@@ -57,7 +57,13 @@ struct Plan {
 };
 
 int64_t forward_blocks(const scanscam_selective &a, int split) { return ceil_div(a.channels / a.groups, kFwdWaves / split * kRows); }
-int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels); }
+// Two sets of 16 channels a workgroup where that leaves two workgroups for every CU.
+int backward_sets(const scanscam_selective &a)
+{
+    const int64_t wide = kBwdMostSets * kBwdChannels;
+    return a.N <= kStateBlock && a.sequences * a.groups * ceil_div(a.channels / a.groups, wide) >= 512 ? kBwdMostSets : 1;
+}
+int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels * backward_sets(a)); }
 
 // Parts of one length for about two workgroups a CU, whole tiles each.
 int64_t span_for(const scanscam_selective &a, int64_t blocks, int64_t shortest)
@@ -115,7 +121,7 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
 {
     constexpr int K = kTokensALane;
     const Plan plan = forward_plan(a);
-    const SelectiveArgs args{a, plan.split, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
+    const SelectiveArgs args{a, plan.split, 1, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
     const dim3 grid((unsigned)(a.groups * (int64_t)args.blocks * all_units(a, plan.span)));
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
     if (cut(a, plan.span)) {
@@ -129,11 +135,12 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
 {
     constexpr int K = kTokensALane;
     const Plan plan = backward_plan(a);
+    const int sets = backward_sets(a);
     const int64_t blocks = backward_blocks(a), units = all_units(a, plan.span);
     float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.span), *sums = bc + bc_words(a);
-    const SelectiveArgs args{a, 1, (uint32_t)blocks, each_of(a, plan.span), plan.span, ends, bc, sums};
+    const SelectiveArgs args{a, 1, sets, (uint32_t)blocks, each_of(a, plan.span), plan.span, ends, bc, sums};
     const dim3 grid((unsigned)(a.groups * blocks * units));
-    const int words = BackwardLds<K>::words((int)a.N);
+    const int words = BackwardLds<K>::words((int)a.N, sets);
     hipError_t err = hipSuccess;
     if (cut(a, plan.span)) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
     if (err == hipSuccess) err = launch_wide(selective_bwd_kernel<ST, K, false>, grid, kBwdWaves * 64, words, stream, args);

@@ -29,11 +29,12 @@ constexpr int kRows = 4;         // channels of a wave
 constexpr int kStateBlock = 16;  // states whose B and C are in LDS at a time
 
 // What follows from K. Tokens lie in LDS as [K / 4][16 lanes][4], 4 floats of padding behind each 64, so that the 16-byte reads of
-// neighbouring lanes are neighbours and the single writes of a wave spread over the banks.
+// neighbouring lanes are neighbours and the single writes of a wave spread over the banks: the pitch is 4 or 12 modulo 16, which
+// sends the 4 groups of channels that a wave writes to different quarters of them.
 template <int K> struct Geometry {
     static constexpr int kTile = kTimeLanes * K;
     static constexpr int kLine = 68;
-    static constexpr int kPitch = K / 4 * kLine + (K / 4 % 4 == 1 ? 0 : K / 4 % 4 == 2 ? 12 : K / 4 % 4 == 3 ? 8 : 4);
+    static constexpr int kPitch = K / 4 * kLine + (K / 4 % 2 == 1 ? 0 : 4);
     static __device__ __forceinline__ int place(int t) { return (t % K) / 4 * kLine + t / K * 4 + (t & 3); }
     static __device__ __forceinline__ void read(const float *row, int lane, float (&f)[K])
     {
@@ -337,6 +338,7 @@ __device__ __forceinline__ void step_sizes(const Quad<ST> (&dt)[ITEMS], const fl
 struct SelectiveArgs {
     scanscam_selective a;
     int split;        // forwards: waves that share the states of a channel out among them
+    int sets;         // backwards: sets of 16 channels that a workgroup takes
     uint32_t blocks;  // of channels, in a group
     uint32_t each;    // parts of a sequence where all are of one length
     int64_t span;     // tokens of a part of a sequence
@@ -611,21 +613,25 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
 // ---------------------------------------------------------------------------------------------------------------------------
 // Backwards. A workgroup of 4 waves takes 16 channels back through a stretch. The sums over n (s1, s2, v) belong to a channel, the
 // sums over channels (gB, gC) to a state: a wave keeps the latter for its 4 of 16 states in registers while it goes over the
-// 4 groups of channels, and the former are added up in LDS, where in every step each group of channels is one wave's alone. With
-// ENDS only the gradient at the stretch's start is found, from zeros.
+// 4 groups of channels, and the former are added up in LDS, where in every step each group of channels is one wave's alone. Of
+// many channels with up to 16 states it takes two times 16, one after the other in every tile, before gB and gC go out: half
+// the sums for selective_bc_kernel to join. With ENDS only the gradient at the stretch's start is found, from zeros.
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kBwdWaves = 4, kBwdChannels = kBwdWaves * kRows, kBwdStates = kStateBlock / kBwdWaves;
 
+constexpr int kBwdMostSets = 2;  // of 16 channels
+
 template <int K> struct BackwardLds {
     using G = Geometry<K>;
-    // d, u, g0 and s1, s2, v; B and C; A and the gradients' carries and the sums for A; a block's states
-    static __host__ __device__ constexpr int words(int N)
+    // d, u, g0 and s1, s2, v; B and C; A, the gradients' carries and the sums for A; a block's states; bias, D and the sums for them
+    static __host__ __device__ constexpr int words(int N, int sets)
     {
-        return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 3 * kBwdChannels * padded(N) + kBwdChannels * kStateBlock + kNowhere;
+        return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 3 * sets * kBwdChannels * padded(N) + kBwdChannels * kStateBlock +
+               (2 + 2 * kBwdWaves) * sets * kBwdChannels + nowhere(sets);
     }
     // A wave goes through its states without a branch: those past the last one have no decay, no B and no C.
-    static constexpr int kNowhere = 3 * kBwdChannels * kBwdStates;  // where lanes write that have nothing to say
     static __host__ __device__ constexpr int padded(int N) { return (N + kBwdStates - 1) / kBwdStates * kBwdStates; }
+    static __host__ __device__ constexpr int nowhere(int sets) { return 3 * sets * kBwdChannels * kBwdStates; }  // where lanes write that have nothing to say
 };
 
 template <typename ST, int K, bool ENDS>
@@ -635,18 +641,20 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     constexpr int TILE = G::kTile, P = G::kPitch, channels = kBwdChannels;
     constexpr int kThreads = kBwdWaves * 64, kItems = kBwdWaves * TILE / kThreads;
     const scanscam_selective &a = args.a;
-    const int N = (int)a.N, slots = channels * BackwardLds<K>::padded(N);
+    const int N = (int)a.N, wide = args.sets * channels, slots = wide * BackwardLds<K>::padded(N);  // wide: all channels of the workgroup
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *lg = lu + channels * P;
     float *l1 = lg + channels * P, *l2 = l1 + channels * P, *lv = l2 + channels * P;
     float *lB = lv + channels * P, *lC = lB + kStateBlock * P;
-    Carry *lG = reinterpret_cast<Carry *>(lC + kStateBlock * P);  // [N][channels]
-    float *lS = reinterpret_cast<float *>(lG + slots), *lh = lS + slots, *nowhere = lh + channels * kStateBlock;  // lh: [16][channels]
+    Carry *lG = reinterpret_cast<Carry *>(lC + kStateBlock * P);                   // [N][wide]
+    float *lS = reinterpret_cast<float *>(lG + slots), *lh = lS + slots;           // [N][wide], [16][channels]
+    float *lbias = lh + channels * kStateBlock, *lskip = lbias + wide, *lsum = lskip + wide;  // lsum: [waves][2][wide]
+    float *nowhere = lsum + 2 * kBwdWaves * wide;
 
     const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
     const Work w = work_of((uint32_t)a.groups * args.blocks, a.offsets == nullptr);
-    const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * channels;
-    const int here = (int)clamp_(per_group - c0, 0, channels);
+    const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * wide;
+    const int here = (int)clamp_(per_group - c0, 0, wide), sets = (here + channels - 1) / channels;
     const int64_t first = group * per_group + c0;
     const Stretch s = stretch_of<TILE>(a, w.unit, args.span, args.each);
     if (ENDS && (s.part == 0 || s.part >= s.parts)) return;
@@ -655,7 +663,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, row = lane >> 4, tl = lane & 15;
 
     for (int i = threadIdx.x; i < slots; i += kThreads) {
-        const int n = i / channels, c = i - n * channels;
+        const int n = i / wide, c = i - n * wide;
         Carry q{0.0f, 0.0f};
         if (c < here && n < N) {
             const int64_t at = (first + c) * N + n;
@@ -669,49 +677,76 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
         lS[i] = 0.0f;
     }
 
-    const int set_in = threadIdx.x % kBwdWaves, c_in = set_in * kRows, count = (int)clamp_(here - c_in, 0, 4);
+    for (int i = threadIdx.x; i < wide; i += kThreads) {
+        lbias[i] = i < here ? param(a.dt_bias, first + i) : 0.0f;
+        lskip[i] = i < here ? param(a.D, first + i) : 0.0f;
+    }
+    for (int i = threadIdx.x; i < 2 * kBwdWaves * wide; i += kThreads) lsum[i] = 0.0f;
+
+    const int c_in = threadIdx.x % kBwdWaves * kRows;
     const int t_in = threadIdx.x / kBwdWaves, t_step = kThreads / kBwdWaves;
-    const uint32_t c_from = count > 0 ? c_in : 0;
-    const int c_count = count > 0 ? count : here;
     const bool whole = here % 4 == 0;
-    float bias[4], skip[4], sum_skip[4] = {}, sum_bias[4] = {};
-    params(a.dt_bias, first + c_in, count, bias);
-    params(a.D, first + c_in, count, skip);
+    // Channels from c_in on that set `set` has, and where they are read: those that are not there from places that are.
+    const auto count_of = [&](int set) { return (int)clamp_(here - set * channels - c_in, 0, 4); };
     const int64_t tiles = (s.end - s.start + TILE - 1) / TILE;
     Quad<ST> x[kItems], dt[kItems], gy[kItems], z[kItems];
     StateInputs<ST, TILE, kThreads> bc;
-    auto fetch = [&](int64_t t0) {
-        const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE), t_mine = again(t_in);
+    const auto fetch = [&](int64_t t0, int set) {
+        const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE), t_mine = again(t_in), have = count_of(set);
+        const int count = have > 0 ? have : here - set * channels;
+        const int64_t from = first + set * channels;
+        const uint32_t c = have > 0 ? c_in : 0;
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
             const uint32_t t = t_mine + j * t_step < length ? t_mine + j * t_step : length - 1;
-            x[j].load(token_at<ST>(a.x, s.batch, t0, first), t * (uint32_t)a.x.token + c_from, c_count, whole);
-            dt[j].load(token_at<ST>(a.dt, s.batch, t0, first), t * (uint32_t)a.dt.token + c_from, c_count, whole);
-            gy[j].load(token_at<ST>(a.gy, s.batch, t0, first), t * (uint32_t)a.gy.token + c_from, c_count, whole);
-            if (gated) z[j].load(token_at<ST>(a.z, s.batch, t0, first), t * (uint32_t)a.z.token + c_from, c_count, whole);
+            x[j].load(token_at<ST>(a.x, s.batch, t0, from), t * (uint32_t)a.x.token + c, count, whole);
+            dt[j].load(token_at<ST>(a.dt, s.batch, t0, from), t * (uint32_t)a.dt.token + c, count, whole);
+            gy[j].load(token_at<ST>(a.gy, s.batch, t0, from), t * (uint32_t)a.gy.token + c, count, whole);
+            if (gated) z[j].load(token_at<ST>(a.z, s.batch, t0, from), t * (uint32_t)a.z.token + c, count, whole);
         }
-        bc.load(a, s.batch, group, t0, length, 0);
     };
+    const auto fetch_bc = [&](int64_t t0, int n0) { bc.load(a, s.batch, group, t0, (int)(s.end - t0 < TILE ? s.end - t0 : TILE), n0); };
     // The states that a tile starts from, one a thread in a block of 16.
     static_assert(channels * kStateBlock == kThreads, "one a thread");
     float h_saved = 0.0f;
-    auto fetch_states = [&](int64_t tile, int n0) {
+    const auto fetch_states = [&](int64_t tile, int set, int n0) {
         if (ENDS) return;
-        const int thread = again((int)threadIdx.x), n = n0 + thread / channels, c = thread % channels;
+        const int thread = again((int)threadIdx.x), n = n0 + thread / channels, c = set * channels + thread % channels;
         const float *from = static_cast<const float *>(a.saved) + (s.tile + tile) * N * a.channels + first;
         h_saved = c < here && n < N ? *(from + (int64_t)n * a.channels + c) : 0.0f;
     };
     if (tiles > 0) {
-        fetch(s.start + (tiles - 1) * TILE);
-        fetch_states(tiles - 1, 0);
+        fetch(s.start + (tiles - 1) * TILE, 0);
+        fetch_bc(s.start + (tiles - 1) * TILE, 0);
+        fetch_states(tiles - 1, 0, 0);
     }
+    // What was asked for ahead is waited for before anything is stored, as in the forward kernel.
+    const auto arrive = [&]() {
+#pragma unroll
+        for (int j = 0; j < kItems; j++) {
+            x[j].arrive();
+            dt[j].arrive();
+            gy[j].arrive();
+            z[j].arrive();
+        }
+        bc.arrive();
+        asm volatile("" : "+v"(h_saved));
+    };
+    // Whether every wave has states in the first block: then what it finds in its first step is the first there is of s1, s2 and v.
+    const bool busy = N > (kBwdWaves - 1) * kBwdStates;
     for (int64_t tile = tiles - 1; tile >= 0; tile--) {
         const int64_t t0 = s.start + tile * TILE;
         const int length = (int)(s.end - t0 < TILE ? s.end - t0 : TILE);
+        float gB[kBwdStates][K], gC[kBwdStates][K];
+        for (int set = 0; set < sets; set++) {
+        const int count = count_of(set);
         __syncthreads();
         Quad<ST> x_now[kItems], dt_now[kItems], gy_now[kItems], z_now[kItems];
         const int t_mine = again(t_in);
-        const bool full = length == TILE && here == channels;
+        const bool full = length == TILE && here - set * channels >= channels;
+        const float4v bias4 = *reinterpret_cast<const float4v *>(lbias + set * channels + c_in);
+        const float bias[4] = {bias4[0], bias4[1], bias4[2], bias4[3]};
+        float sums_in[2][4] = {};
         float d_in[kItems][4], u_in[kItems][4], g_in[kItems][4];
         step_sizes(dt, bias, a.softplus, d_in);
 #pragma unroll
@@ -751,40 +786,54 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 ld[at + i * P] = d_in[j][i];
                 lu[at + i * P] = u_in[j][i];
                 lg[at + i * P] = g_in[j][i];
-                if (!ENDS) l1[at + i * P] = l2[at + i * P] = lv[at + i * P] = 0.0f;
-                else sum_bias[i] += d_in[j][i];
+                if (!ENDS && !busy) l1[at + i * P] = l2[at + i * P] = lv[at + i * P] = 0.0f;
+                if (ENDS) sums_in[1][i] += d_in[j][i];
             }
         }
         for (int n0 = 0; n0 < N; n0 += kStateBlock) {
             const int states = N - n0 < kStateBlock ? N - n0 : kStateBlock;
             if (n0 > 0) __syncthreads();
-            bc.template store<G>(lB, lC, length, states);
+            if (set == 0) bc.template store<G>(lB, lC, length, states);
             if (!ENDS) lh[threadIdx.x] = h_saved;
-            float gB[kBwdStates][K] = {}, gC[kBwdStates][K] = {};
+            if (set == 0) {
+#pragma unroll
+                for (int q = 0; q < kBwdStates; q++)
+#pragma unroll
+                    for (int k = 0; k < K; k++) gB[q][k] = gC[q][k] = 0.0f;
+            }
             for (int step = 0; step < kBwdWaves; step++) {
                 __syncthreads();
                 if (step == 0) {
                     if (n0 + kStateBlock < N) {
-                        bc.load(a, s.batch, group, t0, length, n0 + kStateBlock);
-                        fetch_states(tile, n0 + kStateBlock);
+                        fetch_bc(t0, n0 + kStateBlock);
+                        fetch_states(tile, set, n0 + kStateBlock);
+                    } else if (set + 1 < sets) {
+                        fetch(t0, set + 1);
+                        fetch_states(tile, set + 1, 0);
                     } else if (tile > 0) {
-                        fetch(t0 - TILE);
-                        fetch_states(tile - 1, 0);
+                        fetch(t0 - TILE, 0);
+                        fetch_bc(t0 - TILE, 0);
+                        fetch_states(tile - 1, 0, 0);
                     }
                 }
                 if (wave * kBwdStates >= states) continue;
-                const int ch = ((wave + step) % kBwdWaves) * kRows + row, from = (n0 + wave * kBwdStates) * channels + ch;
+                const int ch = ((wave + step) % kBwdWaves) * kRows + row, from = (n0 + wave * kBwdStates) * wide + set * channels + ch;
                 // (an address for every lane instead of a branch around the one that writes: the four states below stay one block)
                 Carry *out = tl == 0 ? lG + from : reinterpret_cast<Carry *>(nowhere);
-                float *sums = tl == kTimeLanes - 1 ? lS + from : nowhere + 2 * channels * kBwdStates;
+                float *sums = tl == kTimeLanes - 1 ? lS + from : nowhere + 2 * wide * kBwdStates;
                 float d[K], u[K], g0[K], s1[K], s2[K], v[K], total = 0.0f;
                 G::read(ld + ch * P, tl, d);
                 G::read(lg + ch * P, tl, g0);
                 if (!ENDS) {
                     G::read(lu + ch * P, tl, u);
-                    G::read(l1 + ch * P, tl, s1);
-                    G::read(l2 + ch * P, tl, s2);
-                    G::read(lv + ch * P, tl, v);
+                    if (busy && step == 0 && n0 == 0) {
+#pragma unroll
+                        for (int k = 0; k < K; k++) s1[k] = s2[k] = v[k] = 0.0f;
+                    } else {
+                        G::read(l1 + ch * P, tl, s1);
+                        G::read(l2 + ch * P, tl, s2);
+                        G::read(lv + ch * P, tl, v);
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < K; k++) total += d[k];
@@ -793,7 +842,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
 #pragma unroll
                 for (int q = 0; q < kBwdStates; q++) {
                     const int n = wave * kBwdStates + q;
-                    const Carry c = lG[from + q * channels];
+                    const Carry c = lG[from + q * wide];
                     float e[K], C[K];
                     G::read(lC + n * P, tl, C);
                     float back = tl == kTimeLanes - 1 ? c.h : 0.0f, a2 = __builtin_amdgcn_exp2f(total * c.A);
@@ -803,7 +852,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
 #pragma unroll
                         for (int k = K - 1; k >= 0; k--) back = e[k] * __builtin_fmaf(g0[k], C[k], back);
                         row_scan<false>(a2, back);
-                        out[q * channels].h = back;
+                        out[q * wide].h = back;
                         continue;
                     }
                     // Forwards in time and backwards side by side: each is one chain of dependent operations.
@@ -819,7 +868,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                         back = e[K - 1 - k] * __builtin_fmaf(g0[K - 1 - k], C[K - 1 - k], back);
                     }
                     row_scans(a1, fold, a2, back);
-                    out[q * channels].h = back;
+                    out[q * wide].h = back;
                     const float before = row_prev(fold, h0);
                     float g = row_next(back, c.h), state = before;
 #pragma unroll
@@ -848,12 +897,17 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 if (ENDS) continue;
                 row_sums(sum_A);
 #pragma unroll
-                for (int q = 0; q < kBwdStates; q++) sums[q * channels] += sum_A[q];
+                for (int q = 0; q < kBwdStates; q++) sums[q * wide] += sum_A[q];
                 G::write(l1 + ch * P, tl, s1);
                 G::write(l2 + ch * P, tl, s2);
                 G::write(lv + ch * P, tl, v);
             }
             if (ENDS) continue;
+            if (set + 1 < sets) {
+                __syncthreads();
+                arrive();
+                continue;
+            }
             // gB and gC over the 4 channels of the rows, into the places of B and C (a state's are one wave's alone), and out.
 #pragma unroll
             for (int q = 0; q < kBwdStates; q++) {
@@ -865,16 +919,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 }
             }
             __syncthreads();
-            // (waited for before anything is stored, as in the forward kernel)
-#pragma unroll
-            for (int j = 0; j < kItems; j++) {
-                x[j].arrive();
-                dt[j].arrive();
-                gy[j].arrive();
-                z[j].arrive();
-            }
-            bc.arrive();
-            asm volatile("" : "+v"(h_saved));
+            arrive();
             float *to = args.bc + (((int64_t)w.block * a.batch + s.batch) * a.T + t0) * 2 * N + n0;
             const int thread = again((int)threadIdx.x);
 #pragma unroll
@@ -885,7 +930,9 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 if (t < length && n < states) store_quad(to, (uint32_t)((2 * t + which) * N + n), states - n, states - n >= 4, f);
             }
         }
-        if (ENDS) continue;
+        if (!ENDS) {
+        const float4v skip = *reinterpret_cast<const float4v *>(lskip + set * channels + c_in);
+        const int64_t from = first + set * channels;
         const int t_out = again(t_in);
 #pragma unroll
         for (int j = 0; j < kItems; j++) {
@@ -898,7 +945,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 const float xi = x_now[j][i], s1 = l1[at + i * P], s2 = l2[at + i * P] * (1.0f / kLog2e), g0 = lg[at + i * P];
                 gx[i] = __builtin_fmaf(ld[at + i * P], s1, skip[i] * g0);
                 gd[i] = __builtin_fmaf(xi, s1, s2);
-                sum_skip[i] = __builtin_fmaf(g0, xi, sum_skip[i]);
+                sums_in[0][i] = __builtin_fmaf(g0, xi, sums_in[0][i]);
             }
             if (a.softplus) {
 #pragma unroll
@@ -912,39 +959,46 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) sum_bias[i] += gd[i];
-            store_quad(const_cast<ST *>(token_at<ST>(a.gx, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gx.token + c_from, count, whole, gx);
-            store_quad(const_cast<ST *>(token_at<ST>(a.gdt, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gdt.token + c_from, count, whole, gd);
-            if (gated) store_quad(const_cast<ST *>(token_at<ST>(a.gz, s.batch, t0, first)), (uint32_t)t * (uint32_t)a.gz.token + c_from, count, whole, gz);
+            for (int i = 0; i < 4; i++) sums_in[1][i] += gd[i];
+            store_quad(const_cast<ST *>(token_at<ST>(a.gx, s.batch, t0, from)), (uint32_t)t * (uint32_t)a.gx.token + c_in, count, whole, gx);
+            store_quad(const_cast<ST *>(token_at<ST>(a.gdt, s.batch, t0, from)), (uint32_t)t * (uint32_t)a.gdt.token + c_in, count, whole, gd);
+            if (gated) store_quad(const_cast<ST *>(token_at<ST>(a.gz, s.batch, t0, from)), (uint32_t)t * (uint32_t)a.gz.token + c_in, count, whole, gz);
+        }
+        }
+        // The sums for D and the bias (ENDS: of d) over the wave's tokens: over the 4 lanes of a row that have the same channels, then over
+        // the rows, which leaves channel r of every 4 in row r's last lanes.
+#pragma unroll
+        for (int which = ENDS ? 1 : 0; which < 2; which++) {
+            float (&v)[4] = sums_in[which];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i] += dpp_move<0x114, 0xf>(0.0f, v[i]);
+                v[i] += dpp_move<0x118, 0xf>(0.0f, v[i]);
+            }
+            const float sum = rows_sum(v[0], v[1], v[2], v[3]);
+            if (tl >= 12) lsum[(wave * 2 + which) * wide + set * channels + (tl - 12) * 4 + row] += sum;
+        }
         }
     }
     __syncthreads();
     float *to = ENDS ? args.ends + s.unit * (N + 1) * a.channels + first
                      : args.sums + s.unit * (N + 2) * a.channels + first * N;
-    for (int i = threadIdx.x; i < channels * N; i += kThreads) {
+    for (int i = threadIdx.x; i < wide * N; i += kThreads) {
         if (ENDS) {
-            const int n = i / channels, c = i - n * channels;
+            const int n = i / wide, c = i - n * wide;
             if (c < here) to[(int64_t)n * a.channels + c] = lG[i].h;
         } else {
             const int c = i / N, n = i - c * N;
             if (c >= here) continue;
-            if (a.gstate_in != nullptr && s.part == 0) a.gstate_in[(s.seq * a.channels + first + c) * N + n] = lG[n * channels + c].h;
-            to[i] = lS[n * channels + c];
+            if (a.gstate_in != nullptr && s.part == 0) a.gstate_in[(s.seq * a.channels + first + c) * N + n] = lG[n * wide + c].h;
+            to[i] = lS[n * wide + c];
         }
     }
-    // D's and the bias's (ENDS: the sum of d): over the threads of a channel, in order.
-    float *red = lds;  // [64][2][channels]
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        red[(t_in * 2 + 0) * channels + c_in + i] = sum_skip[i];
-        red[(t_in * 2 + 1) * channels + c_in + i] = sum_bias[i];
-    }
-    __syncthreads();
-    if (threadIdx.x < 2 * channels) {
-        const int which = threadIdx.x / channels, c = threadIdx.x % channels;
+    for (int i = threadIdx.x; i < 2 * wide; i += kThreads) {
+        const int which = i / wide, c = i - which * wide;
+        if (c >= here) continue;
         float sum = 0.0f;
-        for (int t = 0; t < t_step; t++) sum += red[(t * 2 + which) * channels + c];
-        if (c >= here) return;
+        for (int q = 0; q < kBwdWaves; q++) sum += lsum[(q * 2 + which) * wide + c];
         if (!ENDS) args.sums[(s.unit * (N + 2) + N + which) * a.channels + first + c] = sum;
         else if (which == 1) to[(int64_t)N * a.channels + c] = sum;
     }

@@ -111,6 +111,14 @@ def test_scan_and_gradients(gpu, monkeypatch, dtype, batch, T, D, N, more, softp
         close(a, torch.zeros(v[k].shape, dtype=torch.float64) if w is None else w, Tn, f"gradient of {k}")
 
 
+@pytest.mark.parametrize("dtype,batch,T,D,N,more", [(torch.float32, 2, 140, 8190, 16, {}), (torch.bfloat16, 64, 9, 255, 5, {"state": True}),
+                                                     (torch.float32, 0, 0, 64, 16, {"lengths": [3, 0, 1, 7] * 66})],
+                         ids=lambda v: str(v).replace("torch.", "").replace(" ", "")[:30])
+def test_scan_of_many_channels(gpu, monkeypatch, dtype, batch, T, D, N, more):
+    """Enough workgroups for the backward kernel to take two sets of channels each."""
+    test_scan_and_gradients(gpu, monkeypatch, dtype, batch, T, D, N, more, True, 0)
+
+
 def test_scan_of_projections_parts(gpu):
     """Views of wider projections, odd offsets, broadcast inputs and other orders of dimensions give what dense tensors give."""
     v = make_scan(11, torch.bfloat16, 2, 70, 24, 8)

@@ -484,8 +484,7 @@ int scanscam_conv_bwd(const scanscam_conv *a, void *stream)
     hipError_t err = hipSuccess;
     if (p.grid.x > 0) err = run_conv({*a, part, p.stretch, p.stretches}, p, true, s);
     const int64_t parts = a->batch * p.stretches, wide = a->K * a->channels, pitch = wide + a->channels;
-    if (err == hipSuccess) err = column_sum(part, a->gweight, parts, pitch, wide, s);
-    if (err == hipSuccess && a->gbias != nullptr) err = column_sum(part + wide, a->gbias, parts, pitch, a->channels, s);
+    if (err == hipSuccess) err = column_sum({part, parts, pitch, {a->gweight, a->gbias}, {wide, a->channels}}, s);
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
 }
 

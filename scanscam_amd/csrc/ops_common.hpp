@@ -158,17 +158,17 @@ __device__ __forceinline__ int64_t sequence_of(const void *offsets, int wide, in
 
 __device__ __forceinline__ int64_t clamp_(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// out[m] = sum over p < parts of in[p * pitch + m], in an order that the sizes alone decide: 16 threads a column, each over every
-// 16th part, joined in order. The parts are themselves sums of some hundreds of values, so that no sum is one long chain.
+// Sums over p < parts of in[p * pitch + m], in an order that the sizes alone decide: 16 threads a column, each over every 16th
+// part, joined in order. The parts are themselves sums of some hundreds of values, so that no sum is one long chain. The
+// columns are those of up to three outputs, one behind the other; an output may be NULL.
 struct ColumnSum {
     const float *in;
-    float *out;
-    int64_t parts, pitch, columns;
+    int64_t parts, pitch;
+    float *out[3];
+    int64_t columns[3];
 };
 
 __global__ __launch_bounds__(1024) void column_sum_kernel(ColumnSum a);
-
-inline unsigned column_blocks(int64_t columns) { return (unsigned)ceil_div(columns, 64); }
 
 template <typename Kernel, typename Args>
 inline hipError_t launch_op(Kernel kernel, dim3 grid, dim3 block, size_t lds, hipStream_t stream, const Args &args)
@@ -178,9 +178,10 @@ inline hipError_t launch_op(Kernel kernel, dim3 grid, dim3 block, size_t lds, hi
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, params, lds, stream);
 }
 
-inline hipError_t column_sum(const float *in, float *out, int64_t parts, int64_t pitch, int64_t columns, hipStream_t stream)
+inline hipError_t column_sum(const ColumnSum &a, hipStream_t stream)
 {
-    return launch_op(column_sum_kernel, dim3(column_blocks(columns)), dim3(1024), 0, stream, ColumnSum{in, out, parts, pitch, columns});
+    const int64_t columns = a.columns[0] + a.columns[1] + a.columns[2];
+    return launch_op(column_sum_kernel, dim3((unsigned)ceil_div(columns, 64)), dim3(1024), 0, stream, a);
 }
 
 // --- checks of arguments ---------------------------------------------------------------------------------------------------

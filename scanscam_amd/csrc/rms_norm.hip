@@ -8,17 +8,20 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(ColumnSum a)
 {
     __shared__ float sums[16][64];
     const int col = threadIdx.x & 63, slice = threadIdx.x >> 6;
-    const int64_t m = (int64_t)blockIdx.x * 64 + col;
+    const int64_t column = (int64_t)blockIdx.x * 64 + col, all = a.columns[0] + a.columns[1] + a.columns[2];
     float s = 0.0f;
-    if (m < a.columns) {
+    if (column < all) {
 #pragma unroll 8
-        for (int64_t p = slice; p < a.parts; p += 16) s += a.in[p * a.pitch + m];
+        for (int64_t p = slice; p < a.parts; p += 16) s += a.in[p * a.pitch + column];
     }
     sums[slice][col] = s;
     __syncthreads();
-    if (slice != 0 || m >= a.columns) return;
+    if (slice != 0 || column >= all) return;
     for (int i = 1; i < 16; i++) s += sums[i][col];
-    a.out[m] = s;
+    const int which = column < a.columns[0] ? 0 : column < a.columns[0] + a.columns[1] ? 1 : 2;
+    const int64_t m = column - (which > 0 ? a.columns[0] : 0) - (which > 1 ? a.columns[1] : 0);
+    float *out = which == 0 ? a.out[0] : which == 1 ? a.out[1] : a.out[2];
+    if (out != nullptr) out[m] = s;
 }
 
 }  // namespace scanscam
@@ -106,7 +109,7 @@ int scanscam_norm_bwd(const scanscam_norm *a, void *stream)
     if (a->channels == 0) return SCANSCAM_OK;
     if (a->gweight == nullptr) return SCANSCAM_EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (a->rows == 0) return column_sum(nullptr, a->gweight, 0, 0, a->channels, s) == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
+    if (a->rows == 0) return column_sum({nullptr, 0, 0, {a->gweight}, {a->channels}}, s) == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
     if (a->gy == nullptr || a->gx == nullptr || a->rstd == nullptr || (a->gsum != nullptr && a->residual == nullptr) ||
         (a->gresidual != nullptr && a->residual == nullptr))
         return SCANSCAM_EINVAL;
@@ -118,7 +121,7 @@ int scanscam_norm_bwd(const scanscam_norm *a, void *stream)
     const int64_t grid = norm_bwd_workgroups(*a, plan);
     float *part = static_cast<float *>(a->workspace);
     hipError_t err = run_norm(true, plan, (unsigned)grid, plan.groups > 1 ? (size_t)a->channels * sizeof(float) : 0, s, NormArgs{*a, plan.waves, false, part});
-    if (err == hipSuccess) err = column_sum(part, a->gweight, grid, a->channels, a->channels, s);
+    if (err == hipSuccess) err = column_sum({part, grid, a->channels, {a->gweight}, {a->channels}}, s);
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
 }
 

@@ -148,9 +148,7 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     if (err == hipSuccess && values > 0)
         err = launch_op(selective_bc_kernel<ST>, dim3((unsigned)ceil_div(values, 256), (unsigned)a.groups), dim3(256), 0, stream, GroupSum{a, bc, blocks});
     const int64_t pitch = (a.N + 2) * a.channels;
-    if (err == hipSuccess) err = column_sum(sums, a.gA, units, pitch, a.N * a.channels, stream);
-    if (err == hipSuccess && a.gD != nullptr) err = column_sum(sums + a.N * a.channels, a.gD, units, pitch, a.channels, stream);
-    if (err == hipSuccess && a.gdt_bias != nullptr) err = column_sum(sums + (a.N + 1) * a.channels, a.gdt_bias, units, pitch, a.channels, stream);
+    if (err == hipSuccess) err = column_sum({sums, units, pitch, {a.gA, a.gD, a.gdt_bias}, {a.N * a.channels, a.channels, a.channels}}, stream);
     return err;
 }
 
@@ -225,10 +223,7 @@ int scanscam_selective_bwd(const scanscam_selective *a, void *stream)
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->sequences == 0) {
-        hipError_t err = column_sum(nullptr, a->gA, 0, 0, a->N * a->channels, s);
-        if (err == hipSuccess && a->gD != nullptr) err = column_sum(nullptr, a->gD, 0, 0, a->channels, s);
-        if (err == hipSuccess && a->gdt_bias != nullptr) err = column_sum(nullptr, a->gdt_bias, 0, 0, a->channels, s);
-        return status(err);
+        return status(column_sum({nullptr, 0, 0, {a->gA, a->gD, a->gdt_bias}, {a->N * a->channels, a->channels, a->channels}}, s));
     }
     return status(a->dtype == SCANSCAM_F32    ? run_bwd<float>(*a, s)
                   : a->dtype == SCANSCAM_BF16 ? run_bwd<__bf16>(*a, s)

@@ -16,6 +16,7 @@
 // runs.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -24,6 +25,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/record_function.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -410,9 +412,10 @@ PyObject *bind(PyObject *, PyObject *args)
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// The operators of a state space layer: calls that need no gradient. In Python the checks, the struct of arguments and the
-// outputs took 13 to 20 us a call, against 4 us of the kernel at one token. As above, None is returned for every call that is not
-// covered (gradients, CPU tensors, mismatched arguments, views that have to be copied first), and the Python path goes on with it.
+// The operators of a state space layer. In Python the checks, the struct of arguments and the outputs took 13 to 20 us a call,
+// against 4 us of the kernel at one token, and a training step of a small call 145 (norm) to 250 us (selective scan); with
+// nodes in C++ as for scan(), STEPS. As above, None is returned for every call that is not covered (CPU tensors,
+// mismatched arguments, views that have to be copied first), and the Python path goes on with it.
 // ---------------------------------------------------------------------------------------------------------------------------
 struct Operators {
     decltype(&scanscam_selective_fwd) selective = nullptr;
@@ -421,6 +424,12 @@ struct Operators {
     decltype(&scanscam_conv_fwd) conv = nullptr;
     decltype(&scanscam_conv_step_fwd) conv_step = nullptr;
     decltype(&scanscam_norm_fwd) norm = nullptr;
+    decltype(&scanscam_selective_bwd) selective_back = nullptr;
+    decltype(&scanscam_selective_saved_bytes) selective_saved = nullptr;
+    decltype(&scanscam_conv_bwd) conv_back = nullptr;
+    decltype(&scanscam_conv_workspace_bytes) conv_workspace = nullptr;
+    decltype(&scanscam_norm_bwd) norm_back = nullptr;
+    decltype(&scanscam_norm_workspace_bytes) norm_workspace = nullptr;
 } operators;
 
 constexpr int64_t kMostStates = 256, kMostTaps = 8, kMostNormChannels = 32768;
@@ -429,7 +438,8 @@ constexpr int64_t kMostStates = 256, kMostTaps = 8, kMostNormChannels = 32768;
 struct Arguments {
     PyObject *const *args;
     bool ok;
-    at::Tensor first;  // the activations: what the others are compared with
+    bool gradients = false;  // an argument requires one
+    at::Tensor first;        // the activations: what the others are compared with
 
     Arguments(PyObject *const *args, Py_ssize_t nargs, Py_ssize_t expected, int first_at) : args(args)
     {
@@ -452,8 +462,8 @@ struct Arguments {
             return {};
         }
         at::Tensor t = THPVariable_Unpack(args[i]);
-        ok = plain(t) && !(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(/*level=*/0).defined() &&
-             (!first.defined() || t.device() == first.device());
+        ok = plain(t) && !t._fw_grad(/*level=*/0).defined() && (!first.defined() || t.device() == first.device());
+        if (at::GradMode::is_enabled() && t.requires_grad()) gradients = true;
         return t;
     }
     int code()
@@ -535,6 +545,249 @@ void check_launch(int rc, const char *what)
         check_launch(call, what);                               \
     }
 
+using torch::autograd::AutogradContext;
+
+// An argument that may be absent, as a node takes it: an undefined tensor has no metadata for the node to record, none at all is no input.
+using Maybe = std::optional<at::Tensor>;
+Maybe maybe(const at::Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; }
+
+// What a backward call has of its own: outputs, a workspace, gradients as the library takes them.
+struct Gradients {
+    const at::Tensor &like;
+    at::Tensor empty(const at::Tensor &t, at::ScalarType type) const
+    {
+        return t.defined() ? at::empty(t.sizes(), at::TensorOptions().dtype(type).device(like.device())) : at::Tensor();
+    }
+    at::Tensor empty(const at::Tensor &t) const { return t.defined() ? empty(t, t.scalar_type()) : at::Tensor(); }
+    at::Tensor bytes(size_t n) const { return n != 0 ? at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(like.device())) : at::Tensor(); }
+    // Zeros where there is no gradient; a copy where the last dimension is not unit-stride or tokens are too far apart.
+    at::Tensor tokens(const at::Tensor &g) const
+    {
+        if (!g.defined()) return at::zeros(like.sizes(), like.options());
+        return (g.size(-1) == 1 || g.stride(-1) == 1) && g.stride(1) < SCANSCAM_MOST_TOKEN_STRIDE ? g : g.contiguous();
+    }
+    static scanscam_tokens view(const at::Tensor &t)
+    {
+        if (!t.defined()) return {};
+        return {t.data_ptr(), t.stride(0), t.stride(1), t.dim() > 3 ? t.stride(2) : 0};
+    }
+    static scanscam_param parameter(const at::Tensor &t) { return t.defined() ? scanscam_param{t.data_ptr(), dtype_code(t.scalar_type()), 0} : scanscam_param{}; }
+    template <typename T = void> static T *at(const at::Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr; }
+    static at::Tensor as(at::Tensor &&g, const at::Tensor &t) { return g.defined() && g.scalar_type() != t.scalar_type() ? g.to(t.scalar_type()) : std::move(g); }
+    void *stream() const { return c10::hip::getCurrentHIPStream(like.device().index()).stream(); }
+};
+
+// The gradients, which have none themselves: asking for one is an error, as with a Python function that is differentiable once.
+variable_list once(variable_list &&grads, const variable_list &saved, const variable_list &from)
+{
+    if (!at::GradMode::is_enabled()) return std::move(grads);
+    bool any = false;
+    for (const variable_list *list : {&saved, &from})
+        for (const at::Tensor &t : *list) any = any || (t.defined() && t.requires_grad());
+    if (!any) return std::move(grads);
+    variable_list given;
+    for (const at::Tensor &t : grads)
+        if (t.defined()) given.push_back(t.detach().set_requires_grad(true));
+    const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)given.size());
+    variable_list marked = (*error)(std::move(given));
+    size_t i = 0;
+    for (at::Tensor &t : grads)
+        if (t.defined()) t = marked[i++];
+    return std::move(grads);
+}
+
+// The distance between rows where the leading dimensions merge into one level of rows with unit-stride channels, else -1.
+int64_t row_stride(const at::Tensor &t)
+{
+    const int64_t channels = t.size(-1);
+    if (t.is_contiguous()) return channels;
+    if (channels != 1 && t.stride(-1) != 1) return -1;
+    int64_t stride = channels, size = 1;
+    bool any = false;
+    for (int64_t d = t.dim() - 2; d >= 0; d--) {
+        if (t.size(d) == 1) continue;
+        if (!any) stride = t.stride(d);
+        else if (t.stride(d) != stride * size) return -1;
+        any = true;
+        size *= t.size(d);
+    }
+    return stride;
+}
+
+struct NormBackward : torch::autograd::Function<NormBackward> {
+    struct Done {
+        at::Tensor y, sum, rstd;
+    };
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &residual, Done *done)
+    {
+        ctx->save_for_backward({residual ? done->sum : x, weight, done->rstd});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
+        ctx->saved_data["residual"] = residual.has_value();
+        return residual ? variable_list{done->y, done->sum} : variable_list{done->y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        // (a hook on saved tensors may lay out what it gives back as it likes)
+        const at::Tensor kept = row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous();
+        const at::Tensor &weight = saved[1], &rstd = saved[2];
+        const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+        const bool added = ctx->saved_data["residual"].toBool();
+        at::Tensor gy = grads[0], gsum = added ? grads[1] : at::Tensor();
+        if (!gy.defined() && !gsum.defined()) return {{}, {}, {}, {}};
+        const c10::DeviceGuard guard(kept.device());
+        const Gradients make{kept};
+        gy = gy.defined() ? gy.contiguous() : at::zeros(kept.sizes(), kept.options().dtype(type));
+        if (gsum.defined()) gsum = gsum.contiguous();
+        scanscam_norm a{};
+        a.channels = kept.size(-1);
+        a.rows = kept.numel() / a.channels;
+        a.dtype = dtype_code(type);
+        a.weight = Gradients::parameter(weight);
+        a.rstd = Gradients::at<float>(rstd);
+        a.x = kept.data_ptr();
+        a.x_stride = row_stride(kept);
+        at::Tensor gx = make.empty(kept, type), gresidual, gweight = make.empty(weight, at::kFloat);
+        if (added) {
+            a.residual = a.sum = kept.data_ptr();
+            a.residual_dtype = dtype_code(kept.scalar_type());
+            a.gsum = Gradients::at(gsum);
+            gresidual = kept.scalar_type() == type ? gx : make.empty(kept);  // (where the types agree the two are the same values)
+            if (kept.scalar_type() != type) a.gresidual = gresidual.data_ptr();
+        }
+        a.gy = gy.data_ptr();
+        a.gx = gx.data_ptr();
+        a.gweight = Gradients::at<float>(gweight);
+        a.workspace_bytes = operators.norm_workspace(&a);
+        const at::Tensor workspace = make.bytes(a.workspace_bytes);
+        a.workspace = Gradients::at(workspace);
+        check_launch(operators.norm_back(&a, make.stream()), "norm_bwd");
+        return once({gx, Gradients::as(std::move(gweight), weight), gresidual, {}}, saved, grads);
+    }
+};
+
+struct ConvBackward : torch::autograd::Function<ConvBackward> {
+    struct Done {
+        at::Tensor y, state, offsets;
+        int activation;
+    };
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &bias, const Maybe &state, Done *done)
+    {
+        ctx->save_for_backward({x, weight, bias.value_or(at::Tensor()), state.value_or(at::Tensor()), done->offsets});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["activation"] = (int64_t)done->activation;
+        return done->state.defined() ? variable_list{done->y, done->state} : variable_list{done->y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &offsets = saved[4];
+        at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
+        if (!grads[0].defined() && !gstate_out.defined()) return {{}, {}, {}, {}, {}};
+        const c10::DeviceGuard guard(x.device());
+        const Gradients make{x};
+        const at::Tensor gy = make.tokens(grads[0]);
+        if (gstate_out.defined()) gstate_out = gstate_out.contiguous();
+        at::Tensor gx = make.empty(x), gweight = make.empty(weight, at::kFloat), gbias = make.empty(bias, at::kFloat);
+        // (inputs of the node are counted without the absent ones)
+        at::Tensor gstate = state.defined() && ctx->needs_input_grad(2 + bias.defined()) ? make.empty(state) : at::Tensor();
+        scanscam_conv a{};
+        a.batch = x.size(0);
+        a.T = x.size(1);
+        a.channels = x.size(2);
+        a.K = weight.size(1);
+        a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+        a.offsets = Gradients::at(offsets);
+        a.offsets64 = offsets.defined() && offsets.scalar_type() == at::kLong;
+        a.dtype = dtype_code(x.scalar_type());
+        a.activation = (int32_t)ctx->saved_data["activation"].toInt();
+        a.x = Gradients::view(x);
+        a.weight = Gradients::parameter(weight);
+        a.bias = Gradients::parameter(bias);
+        a.state_in = Gradients::at(state);
+        a.gy = Gradients::view(gy);
+        a.gx = Gradients::view(gx);
+        a.gweight = Gradients::at<float>(gweight);
+        a.gbias = Gradients::at<float>(gbias);
+        a.gstate_out = Gradients::at(gstate_out);
+        a.gstate_in = Gradients::at(gstate);
+        a.workspace_bytes = operators.conv_workspace(&a);
+        const at::Tensor workspace = make.bytes(a.workspace_bytes);
+        a.workspace = Gradients::at(workspace);
+        check_launch(operators.conv_back(&a, make.stream()), "conv_bwd");
+        return once({gx, Gradients::as(std::move(gweight), weight), Gradients::as(std::move(gbias), bias), gstate, {}}, saved, grads);
+    }
+};
+
+struct SelectiveBackward : torch::autograd::Function<SelectiveBackward> {
+    struct Done {
+        at::Tensor y, state, saved, offsets;
+        bool softplus;
+    };
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &dt, const at::Tensor &A, const at::Tensor &B, const at::Tensor &C,
+                                 const Maybe &D, const Maybe &z, const Maybe &bias, const Maybe &state, Done *done)
+    {
+        const at::Tensor none;
+        ctx->save_for_backward({x, dt, A, B, C, D.value_or(none), z.value_or(none), bias.value_or(none), state.value_or(none), done->offsets, done->saved});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["softplus"] = done->softplus;
+        return done->state.defined() ? variable_list{done->y, done->state} : variable_list{done->y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const variable_list kept = ctx->get_saved_variables();
+        const at::Tensor &x = kept[0], &dt = kept[1], &A = kept[2], &B = kept[3], &C = kept[4], &D = kept[5], &z = kept[6], &bias = kept[7], &state = kept[8],
+                         &offsets = kept[9], &saved = kept[10];
+        at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
+        if (!grads[0].defined() && !gstate_out.defined()) return variable_list(10);
+        const c10::DeviceGuard guard(x.device());
+        const Gradients make{x};
+        const at::Tensor gy = make.tokens(grads[0]);
+        if (gstate_out.defined()) gstate_out = gstate_out.contiguous();
+        at::Tensor gx = make.empty(x), gdt = make.empty(dt), gB = make.empty(B), gC = make.empty(C), gz = make.empty(z);
+        at::Tensor gA = make.empty(A, at::kFloat), gD = make.empty(D, at::kFloat), gbias = make.empty(bias, at::kFloat);
+        at::Tensor gstate = state.defined() && ctx->needs_input_grad(5 + D.defined() + z.defined() + bias.defined()) ? make.empty(state) : at::Tensor();
+        scanscam_selective a{};
+        a.batch = x.size(0);
+        a.T = x.size(1);
+        a.channels = x.size(2);
+        a.N = A.size(1);
+        a.groups = B.dim() == 4 ? B.size(2) : 1;
+        a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+        a.offsets = Gradients::at(offsets);
+        a.offsets64 = offsets.defined() && offsets.scalar_type() == at::kLong;
+        a.dtype = dtype_code(x.scalar_type());
+        a.softplus = ctx->saved_data["softplus"].toBool();
+        a.x = Gradients::view(x);
+        a.dt = Gradients::view(dt);
+        a.B = Gradients::view(B);
+        a.C = Gradients::view(C);
+        a.z = Gradients::view(z);
+        a.A = Gradients::parameter(A);
+        a.D = Gradients::parameter(D);
+        a.dt_bias = Gradients::parameter(bias);
+        a.state_in = Gradients::at<float>(state);
+        a.saved = Gradients::at(saved);
+        a.gy = Gradients::view(gy);
+        a.gx = Gradients::view(gx);
+        a.gdt = Gradients::view(gdt);
+        a.gB = Gradients::view(gB);
+        a.gC = Gradients::view(gC);
+        a.gz = Gradients::view(gz);
+        a.gA = Gradients::at<float>(gA);
+        a.gD = Gradients::at<float>(gD);
+        a.gdt_bias = Gradients::at<float>(gbias);
+        a.gstate_out = Gradients::at<float>(gstate_out);
+        a.gstate_in = Gradients::at<float>(gstate);
+        a.workspace_bytes = operators.selective_workspace(&a, SCANSCAM_BACKWARD);
+        const at::Tensor workspace = make.bytes(a.workspace_bytes);
+        a.workspace = Gradients::at(workspace);
+        check_launch(operators.selective_back(&a, make.stream()), "selective_bwd");
+        return once({gx, gdt, Gradients::as(std::move(gA), A), gB, gC, Gradients::as(std::move(gD), D), gz, Gradients::as(std::move(gbias), bias), gstate, {}}, kept, grads);
+    }
+};
+
 // norm(x, weight, residual, eps, quant code): the tuple that rms_norm returns, or y alone.
 PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
@@ -547,30 +800,17 @@ PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     const int64_t channels = x.size(-1);
     in.shape(weight, {channels});
     in.shape(residual, x.sizes());
-    // Rows of one stride: the leading dimensions merge into one level.
-    const auto row_stride = [&](const at::Tensor &t) {
-        if (t.is_contiguous()) return channels;
-        if (channels != 1 && t.stride(-1) != 1) in.ok = false;
-        int64_t stride = channels, size = 1;
-        bool any = false;
-        for (int64_t d = dims - 2; d >= 0; d--) {
-            if (t.size(d) == 1) continue;
-            if (!any) stride = t.stride(d);
-            else if (t.stride(d) != stride * size) in.ok = false;
-            any = true;
-            size *= t.size(d);
-        }
-        return stride;
-    };
     scanscam_norm a{};
     a.rows = x.numel() / channels;
     a.channels = channels;
     a.x = x.data_ptr();
     a.x_stride = row_stride(x);
+    if (a.x_stride < 0) in.ok = false;
     a.weight = in.parameter(weight);
     a.eps = (float)PyFloat_AsDouble(args[3]);
     a.dtype = in.code();
     const long quant = PyLong_AsLong(args[4]);
+    if (in.gradients && quant != 0) Py_RETURN_NONE;
     if (PyErr_Occurred()) {
         PyErr_Clear();
         Py_RETURN_NONE;
@@ -583,6 +823,7 @@ PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         if (a.residual_dtype < 0 || a.residual_dtype == SCANSCAM_F64) in.ok = false;
         a.residual = residual.data_ptr();
         a.residual_stride = row_stride(residual);
+        if (a.residual_stride < 0) in.ok = false;
     }
     if (!in.ok) Py_RETURN_NONE;
     at::Tensor y = in.empty(x.sizes(), quant == SCANSCAM_I8 ? at::kChar : quant == SCANSCAM_F8 ? at::kFloat8_e4m3fn : x.scalar_type());
@@ -595,7 +836,18 @@ PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         scale = in.empty(x.sizes().slice(0, (size_t)dims - 1), at::kFloat);
         a.scale = static_cast<float *>(scale.data_ptr());
     }
+    at::Tensor rstd;
+    if (in.gradients) {
+        rstd = in.empty({a.rows}, at::kFloat);
+        a.rstd = static_cast<float *>(rstd.data_ptr());
+    }
     SCANSCAM_LAUNCH(operators.norm(&a, in.stream()), "norm_fwd")
+    if (in.gradients) {
+        NormBackward::Done done{y, sum, rstd};
+        variable_list out = NormBackward::apply(x, weight, maybe(residual), &done);
+        y = out[0];
+        if (residual.defined()) sum = out[1];
+    }
     if (quant == 0 && !residual.defined()) return THPVariable_Wrap(std::move(y));
     pybind11::list out;
     for (at::Tensor *t : {&y, &scale, &sum})
@@ -647,6 +899,12 @@ PyObject *conv(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         a.state_out = new_state.data_ptr();
     }
     SCANSCAM_LAUNCH(operators.conv(&a, in.stream()), "conv_fwd")
+    if (in.gradients) {
+        ConvBackward::Done done{y, new_state, offsets, a.activation};
+        variable_list out = ConvBackward::apply(x, weight, maybe(bias), maybe(state), &done);
+        y = out[0];
+        if (keep) new_state = out[1];
+    }
     return with_state(std::move(y), std::move(new_state));
     END_HANDLE_TH_ERRORS
 }
@@ -658,7 +916,7 @@ PyObject *conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     Arguments in(args, nargs, 6, 1);
     if (!in.ok) Py_RETURN_NONE;
     const at::Tensor &x = in.first, state = in.tensor(0), weight = in.tensor(2), bias = in.tensor(3), slots = in.tensor(5);
-    if (!in.ok || x.dim() != 2 || x.numel() == 0 || !state.defined() || state.dim() != 3 || !weight.defined() || weight.dim() != 2) Py_RETURN_NONE;
+    if (!in.ok || in.gradients || x.dim() != 2 || x.numel() == 0 || !state.defined() || state.dim() != 3 || !weight.defined() || weight.dim() != 2) Py_RETURN_NONE;
     scanscam_conv_step a{};
     a.rows = x.size(0);
     a.channels = x.size(1);
@@ -741,12 +999,24 @@ PyObject *selective(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         new_state = in.empty({a.sequences, a.channels, a.N}, at::kFloat);
         a.state_out = static_cast<float *>(new_state.data_ptr());
     }
+    at::Tensor saved;
+    if (in.gradients) {
+        saved = in.empty({(int64_t)operators.selective_saved(&a)}, at::kByte);
+        a.saved = saved.data_ptr();
+    }
     a.workspace_bytes = operators.selective_workspace(&a, SCANSCAM_FORWARD);
     if (a.workspace_bytes != 0) {
         workspace = in.empty({(int64_t)a.workspace_bytes}, at::kByte);
         a.workspace = workspace.data_ptr();
     }
     SCANSCAM_LAUNCH(operators.selective(&a, in.stream()), "selective_fwd")
+    if (in.gradients) {
+        SelectiveBackward::Done done{y, new_state, saved, offsets, a.softplus != 0};
+        const auto given = [&](int i) { return args[i] == Py_None ? Maybe() : Maybe(THPVariable_Unpack(args[i])); };
+        variable_list out = SelectiveBackward::apply(x, *given(1), *given(2), *given(3), *given(4), given(5), given(6), given(7), maybe(state), &done);
+        y = out[0];
+        if (keep) new_state = out[1];
+    }
     return with_state(std::move(y), std::move(new_state));
     END_HANDLE_TH_ERRORS
 }
@@ -759,7 +1029,7 @@ PyObject *selective_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     if (!in.ok) Py_RETURN_NONE;
     const at::Tensor &x = in.first, state = in.tensor(0), slots = in.tensor(10);
     scanscam_selective_step a{};
-    if (!in.ok || !state.defined() || state.dim() != 3 || !selective_arguments(in, 1, 1, a)) Py_RETURN_NONE;
+    if (!in.ok || !state.defined() || state.dim() != 3 || !selective_arguments(in, 1, 1, a) || in.gradients) Py_RETURN_NONE;
     a.rows = x.size(0);
     a.slots = state.size(0);
     if (!slots.defined() && a.slots != a.rows) Py_RETURN_NONE;
@@ -777,11 +1047,18 @@ PyObject *selective_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
-// bind_operators(selective_fwd, selective_workspace_bytes, selective_step_fwd, conv_fwd, conv_step_fwd, norm_fwd): addresses.
+// bind_operators(selective_fwd, selective_workspace_bytes, selective_step_fwd, conv_fwd, conv_step_fwd, norm_fwd, and of the backward calls
+// selective_bwd, selective_saved_bytes, conv_bwd, conv_workspace_bytes, norm_bwd, norm_workspace_bytes): addresses.
 PyObject *bind_operators(PyObject *, PyObject *args)
 {
-    unsigned long long p[6];
-    if (!PyArg_ParseTuple(args, "KKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5)) return nullptr;
+    unsigned long long p[12];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9, p + 10, p + 11)) return nullptr;
+    operators.selective_back = reinterpret_cast<decltype(operators.selective_back)>(p[6]);
+    operators.selective_saved = reinterpret_cast<decltype(operators.selective_saved)>(p[7]);
+    operators.conv_back = reinterpret_cast<decltype(operators.conv_back)>(p[8]);
+    operators.conv_workspace = reinterpret_cast<decltype(operators.conv_workspace)>(p[9]);
+    operators.norm_back = reinterpret_cast<decltype(operators.norm_back)>(p[10]);
+    operators.norm_workspace = reinterpret_cast<decltype(operators.norm_workspace)>(p[11]);
     operators.selective = reinterpret_cast<decltype(operators.selective)>(p[0]);
     operators.selective_workspace = reinterpret_cast<decltype(operators.selective_workspace)>(p[1]);
     operators.selective_step = reinterpret_cast<decltype(operators.selective_step)>(p[2]);

@@ -96,8 +96,8 @@ def _lib():
 
 
 def _bind_native():
-    """The host path of calls without gradients in native code (csrc/torch_binding.cpp), or ``None`` where it is not built or the
-    library is a build without these operators; such calls then go through the functions below, three times as slowly on the host."""
+    """The host path in native code, autograd nodes included (csrc/torch_binding.cpp), or ``None`` where it is not built or the library is
+    a build without these operators; calls then go through the functions below, three times as slowly on the host."""
     if hip._native is None or not hasattr(hip._native, "bind_operators"):
         return None
     try:
@@ -106,7 +106,8 @@ def _bind_native():
         return None
     hip._native.bind_operators(*(ctypes.cast(fn, _p).value for fn in (
         lib.scanscam_selective_fwd, lib.scanscam_selective_workspace_bytes, lib.scanscam_selective_step_fwd, lib.scanscam_conv_fwd,
-        lib.scanscam_conv_step_fwd, lib.scanscam_norm_fwd)))
+        lib.scanscam_conv_step_fwd, lib.scanscam_norm_fwd, lib.scanscam_selective_bwd, lib.scanscam_selective_saved_bytes,
+        lib.scanscam_conv_bwd, lib.scanscam_conv_workspace_bytes, lib.scanscam_norm_bwd, lib.scanscam_norm_workspace_bytes)))
     return hip._native
 
 

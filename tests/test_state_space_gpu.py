@@ -401,7 +401,7 @@ def test_calls_use_the_current_stream(gpu):
 
 
 def test_native_host_path_is_the_python_path(gpu, monkeypatch):
-    """Calls without gradients take the native host path, and give what the Python one gives; what it does not cover it leaves alone."""
+    """Calls take the native host path, and give what the Python one gives; what it does not cover it leaves alone."""
     assert state_space._native is not None
     taken = []
 
@@ -450,11 +450,59 @@ def test_native_host_path_is_the_python_path(gpu, monkeypatch):
         both(f.rms_norm, d["x"].transpose(0, 1).expand(103, 2, 40), b, covered=False)
     with torch.no_grad():
         both(f.rms_norm, d["x"].requires_grad_(), b)
-    for name, call in (("norm", lambda: f.rms_norm(d["x"], b)), ("selective", lambda: f.selective_scan(*[d[k] for k in ("x", "dt", "A", "B", "C")]))):
-        monkeypatch.setattr(state_space, "_native", Counted())
-        assert call().requires_grad and taken.pop() == (name, False)
     with pytest.raises(TypeError):
         f.rms_norm(b, b, quant=torch.uint8)
+
+
+def test_native_autograd_nodes_are_the_python_ones(gpu, monkeypatch):
+    """The same gradients, bit for bit, from the nodes in C++ as from those in Python: of every argument or of some, of every output or of
+    one, of expanded and transposed gradients; a second derivative is refused by both."""
+    native = state_space._native
+    assert native is not None
+
+    def both(fn, args, kwargs, some=None, only=None):
+        results = []
+        for path in (native, None):
+            monkeypatch.setattr(state_space, "_native", path)
+            leaves = {k: t.detach().clone().requires_grad_(some is None or k in some) if torch.is_tensor(t) and t.is_floating_point() else t for k, t in args.items()}
+            out = fn(**leaves, **kwargs)
+            out = out if isinstance(out, tuple) else (out,)
+            assert all(o.requires_grad for o in out)
+            assert ("CppNode" in out[0].grad_fn.name()) == (path is not None), out[0].grad_fn.name()
+            torch.manual_seed(5)
+            grads = [torch.randn(o.shape, device=gpu).to(o.dtype) for o in out]
+            used = range(len(out)) if only is None else [only]
+            torch.autograd.backward([out[i] for i in used], [grads[i] for i in used])
+            results.append([*out, *(t.grad for t in leaves.values() if torch.is_tensor(t))])
+        for p, q in zip(*results):
+            assert (p is None) == (q is None) and (p is None or (p.dtype == q.dtype and torch.equal(p, q))), (fn.__name__, some, only)
+
+    for dtype in (torch.bfloat16, torch.float32):
+        for offsets in (None, [70, 0, 33]):
+            v = make_scan(19, dtype, 2, 103, 40, 16, groups=2, lengths=offsets, state=True)
+            d = {k: None if t is None else t.to(gpu) for k, t in v.items()}
+            d["A"] = d["A"].to(torch.float32)
+            kept = torch.randn(d["state"].shape[0], 3, 40, device=gpu).to(dtype)
+            conv = dict(x=d["x"], weight=torch.randn(40, 4, device=gpu).to(dtype), bias=torch.randn(40, device=gpu), state=kept, offsets=d["offsets"])
+            for kwargs, only in (({}, None), ({"return_state": True}, None), ({"return_state": True}, 0), ({"return_state": True}, 1)):
+                both(f.selective_scan, d, dict(softplus=True, **kwargs), only=only)
+                both(f.causal_conv, conv, dict(activation="silu", **kwargs), only=only)
+            both(f.selective_scan, {k: None if k in ("z", "D", "dt_bias", "state") else t for k, t in d.items()}, dict(softplus=True), some=("A", "x"))
+            both(f.selective_scan, d, dict(softplus=True), some=("state",))
+            both(f.causal_conv, dict(conv, bias=None, state=None), {}, some=("weight",))
+        x, w, r = torch.randn(3, 5, 40, device=gpu).to(dtype), torch.randn(40, device=gpu), torch.randn(3, 5, 40, device=gpu)
+        both(f.rms_norm, dict(x=x, weight=w), {})
+        both(f.rms_norm, dict(x=x, weight=w.to(dtype)), {}, some=("weight",))
+        for residual in (r, r.to(dtype)):
+            for only in (None, 0, 1):
+                both(f.rms_norm, dict(x=x, weight=w, residual=residual), dict(eps=1e-3), only=only)
+    for path in (native, None):
+        monkeypatch.setattr(state_space, "_native", path)
+        wide = torch.randn(4, 6, 80, device=gpu, requires_grad=True)
+        results = [f.rms_norm(wide[..., :40], w), f.causal_conv(wide[..., 40:], torch.ones(40, 4, device=gpu))]
+        total = torch.autograd.grad(sum(t.square().sum() for t in results) + (results[1].transpose(0, 1) * 2).sum(), wide, create_graph=True)[0]
+        with pytest.raises(RuntimeError, match="differentiate twice|once_differentiable"):
+            total.square().sum().backward()
 
 
 def test_calls_on_a_device_that_is_not_current_and_errors(gpu):

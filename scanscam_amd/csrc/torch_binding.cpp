@@ -413,9 +413,9 @@ PyObject *bind(PyObject *, PyObject *args)
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // The operators of a state space layer. In Python the checks, the struct of arguments and the outputs took 13 to 20 us a call,
-// against 4 us of the kernel at one token, and a training step of a small call 145 (norm) to 250 us (selective scan); with
-// nodes in C++ as for scan(), STEPS. As above, None is returned for every call that is not covered (CPU tensors,
-// mismatched arguments, views that have to be copied first), and the Python path goes on with it.
+// against 3 to 6 us here (4 us of the kernel at one token); a forward and backward pass over 9 x 1 x 32 values took 142 us
+// (norm), 145 (conv) and 222 (selective scan), and 64, 62 and 89 with nodes in C++ as for scan(). As above, None is returned for every
+// call that is not covered (CPU tensors, mismatched arguments, views that have to be copied first), and the Python path goes on with it.
 // ---------------------------------------------------------------------------------------------------------------------------
 struct Operators {
     decltype(&scanscam_selective_fwd) selective = nullptr;

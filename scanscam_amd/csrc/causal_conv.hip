@@ -58,6 +58,14 @@ __device__ __forceinline__ void conv_input(const scanscam_conv &a, int64_t b, co
 // Tokens asked for at a time.
 constexpr int kAhead = 4;
 
+// kAhead rows of a tensor from token t on (those past its end: the last one again), asked for without a wait between them.
+template <typename ST, int VEC>
+__device__ __forceinline__ void ask(Stored<ST, VEC> (&rows)[kAhead], const ST *from, int64_t stride, int64_t t, int64_t T)
+{
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) rows[j].load(from + (t + j < T ? t + j : T - 1) * stride);
+}
+
 // This lane's vector of channels: the first one, and how many there are (VEC but where there are fewer channels than that).
 template <int VEC> __device__ __forceinline__ int64_t lane_channels(int64_t channels, int64_t c, int &count)
 {
@@ -152,10 +160,15 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs args)
 }
 
 // A stretch's gx needs gp of the K - 1 tokens after it: they are computed again. The sums for gw and gbias cover the stretch itself.
+// A lane has 4 channels whatever the type: 8 of 16 bits leave two waves a SIMD, 4 leave three, and cover twice as much time in the same
+// number of waves, so that fewer tokens are at a stretch's border. Those are loaded kAhead at a time as well. (A training step of
+// [8, 4096, 2048] in bf16, K = 4, borders' tokens one by one / together: 8 channels and 64 tokens 159 / 155 us, 4 channels and 128 tokens
+// 160 / 144, of which 87 are this kernel's: 4.6 TB/s. The next group asked for before this one is worked on: 166, for its registers.)
+constexpr int kBackChannels = 4;
 template <typename ST, int K>
-__global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
+__global__ __launch_bounds__(256, 2) void conv_bwd_kernel(ConvArgs args)
 {
-    constexpr int VEC = 16 / sizeof(ST);
+    constexpr int VEC = kBackChannels;
     const scanscam_conv &a = args.a;
     const int64_t mine = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
     if (mine >= a.channels) return;
@@ -228,11 +241,19 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
             }
         };
         // Any token: at the borders of stretches and sequences.
-        const auto token = [&]() {
+        const auto token = [&](const Stored<ST, VEC> &x_row, const Stored<ST, VEC> &gy_row) {
             if (t < s.end) {
                 float g[VEC];
-                load_part(from + t * a.x.token, count, x[K - 1]);
-                load_part(from_gy + t * a.gy.token, count, g);
+                if (count == VEC) {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        x[K - 1][i] = x_row[i];
+                        g[i] = gy_row[i];
+                    }
+                } else {
+                    load_part(from + t * a.x.token, count, x[K - 1]);
+                    load_part(from_gy + t * a.gy.token, count, g);
+                }
                 slope(g, t < last);
             } else {
 #pragma unroll
@@ -255,7 +276,28 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
             }
             move_on();
         };
-        for (; t < first + K - 1 && t < last + K - 1; t++) token();
+        // The first K - 1 tokens and the last: theirs are asked for kAhead at a time too.
+        const auto border = [&](int64_t stop) {
+#pragma unroll 1
+            while (t < stop) {
+                Stored<ST, VEC> ahead[kAhead], ahead_gy[kAhead];
+                if (count == VEC) {
+                    ask(ahead, from, a.x.token, t, a.T);
+                    ask(ahead_gy, from_gy, a.gy.token, t, a.T);
+                }
+                int64_t n = stop - t < kAhead ? stop - t : kAhead;
+#pragma unroll 1
+                for (; n > 0; n--, t++) {
+                    token(ahead[0], ahead_gy[0]);
+#pragma unroll
+                    for (int q = 0; q + 1 < kAhead; q++) {
+                        ahead[q] = ahead[q + 1];
+                        ahead_gy[q] = ahead_gy[q + 1];
+                    }
+                }
+            }
+        };
+        border(first + K - 1 < last + K - 1 ? first + K - 1 : last + K - 1);
         // Tokens inside the stretch whose gx goes out to K - 1 tokens back, a token's row of its own, kept by no state.
         ST *to = static_cast<ST *>(a.gx.p) + b * a.gx.batch + c;
         for (; count == VEC && t + kAhead <= last; t += kAhead) {
@@ -279,7 +321,7 @@ __global__ __launch_bounds__(256) void conv_bwd_kernel(ConvArgs args)
                 move_on();
             }
         }
-        for (; t < last + K - 1; t++) token();
+        border(last + K - 1);
         t = last;
     }
     float *part = args.part + unit * (K + 1) * a.channels;
@@ -377,12 +419,12 @@ struct ConvPlan {
     dim3 grid, block;
 };
 
-// Stretches of up to 64 tokens, shorter where there are too few to give every SIMD two waves.
-ConvPlan conv_plan(const scanscam_conv &a, bool states)
+// Stretches of up to 64 tokens (backwards 128: their borders cost more), shorter where there are too few to give every SIMD two waves.
+ConvPlan conv_plan(const scanscam_conv &a, bool back, bool states)
 {
-    const int64_t vec = 16 / activation_size(a.dtype), lanes = ceil_div(a.channels, vec);
+    const int64_t vec = back ? kBackChannels : 16 / activation_size(a.dtype), lanes = ceil_div(a.channels, vec);
     ConvPlan p;
-    p.stretch = 64;
+    p.stretch = back ? 128 : 64;
     while (p.stretch > 8 && ceil_div(lanes * a.batch * ceil_div(a.T, p.stretch), 64) < 2048) p.stretch /= 2;
     p.stretches = ceil_div(a.T, p.stretch);
     int x = 1;
@@ -449,7 +491,7 @@ int scanscam_conv_fwd(const scanscam_conv *a, void *stream)
         SCANSCAM_CHECK(check_tokens(a->x, size));
         SCANSCAM_CHECK(check_tokens(a->y, size));
     }
-    const ConvPlan p = conv_plan(*a, states);
+    const ConvPlan p = conv_plan(*a, false, states);
     if (p.grid.x == 0) return SCANSCAM_OK;
     const hipError_t err = run_conv({*a, nullptr, p.stretch, p.stretches}, p, false, static_cast<hipStream_t>(stream));
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
@@ -460,7 +502,7 @@ size_t scanscam_conv_workspace_bytes(const scanscam_conv *a)
     if (check_conv_sizes(a != nullptr ? a->channels : -1, a != nullptr ? a->K : 0, a != nullptr ? a->dtype : 0, 0) != SCANSCAM_OK ||
         a->batch <= 0 || a->T <= 0 || a->channels == 0)
         return 0;
-    const ConvPlan p = conv_plan(*a, false);
+    const ConvPlan p = conv_plan(*a, true, false);
     return (size_t)(a->batch * p.stretches * (a->K + 1) * a->channels) * sizeof(float);
 }
 
@@ -479,7 +521,7 @@ int scanscam_conv_bwd(const scanscam_conv *a, void *stream)
         if (a->workspace == nullptr || a->workspace_bytes < scanscam_conv_workspace_bytes(a)) return SCANSCAM_EWORKSPACE;
         if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
     }
-    const ConvPlan p = conv_plan(*a, states);
+    const ConvPlan p = conv_plan(*a, true, states);
     float *part = static_cast<float *>(a->workspace);
     hipError_t err = hipSuccess;
     if (p.grid.x > 0) err = run_conv({*a, part, p.stretch, p.stretches}, p, true, s);

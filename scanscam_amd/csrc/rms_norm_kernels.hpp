@@ -5,7 +5,9 @@
 //   8 bits: scale = max |y| / limit,  q = round(y / scale)
 //   backwards, u = gy * weight, v = sum * rstd:  gx = rstd * (u - v * mean(u * v)) + gsum,  gweight = sum over rows of gy * v
 //
-// Memory bounds it: each tensor once. A row stays in the registers of one to sixteen waves, so that nothing is read twice.
+// Memory bounds it: each tensor once. A row stays in the registers of one to sixteen waves, so that nothing is read twice. [32768, 2048] in
+// bf16 with a float32 residual: 146 us forwards (805 MB, 5.5 TB/s), 215 backwards (1074 MB, 5.0 TB/s); [16384, 2049] in bf16 to 8 bits,
+// where three rows in four begin inside a vector: 52 us (235 MB, 4.5 TB/s); 16 rows of 2048: 4 us, a launch and one trip to memory.
 #pragma once
 
 #include "ops_common.hpp"

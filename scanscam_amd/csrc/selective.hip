@@ -145,8 +145,11 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     if (cut(a, plan.span)) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
     if (err == hipSuccess) err = launch_wide(selective_bwd_kernel<ST, K, false>, grid, kBwdWaves * 64, words, stream, args);
     const int64_t values = a.batch * a.T * 2 * a.N;
-    if (err == hipSuccess && values > 0)
-        err = launch_op(selective_bc_kernel<ST>, dim3((unsigned)ceil_div(values, 256), (unsigned)a.groups), dim3(256), 0, stream, GroupSum{a, bc, blocks});
+    if (err == hipSuccess && values > 0) {
+        const bool four = a.N % 4 == 0;
+        err = launch_op(four ? selective_bc_kernel<ST, 4> : selective_bc_kernel<ST, 1>, dim3((unsigned)ceil_div(values, four ? 1024 : 256), (unsigned)a.groups), dim3(256), 0,
+                        stream, GroupSum{a, bc, blocks});
+    }
     const int64_t pitch = (a.N + 2) * a.channels;
     if (err == hipSuccess) err = column_sum({sums, units, pitch, {a.gA, a.gD, a.gdt_bias}, {a.N * a.channels, a.channels, a.channels}}, stream);
     return err;

@@ -16,8 +16,11 @@
 // the sum over n in registers, and B and C, the same for all channels, come from LDS. What a token costs once (softplus, the gate,
 // rounding) is done by other lanes on the way between the channel-fastest tensors and the token-fastest rows in LDS.
 //
-// The vector unit bounds it: per token, channel and state one exponential (two issue slots) and five multiply-adds forwards,
-// with N = 16 some 130 slots for 8 bytes of 16-bit tensors.
+// The vector unit bounds it. Forwards a lane's 8 tokens take 74 issue slots a state (65 instructions; 9 exponentials take two), of which 56
+// are the formula's: 148 a token and channel at N = 16, with some 70 more for what a token costs once, for 8 bytes of 16-bit tensors.
+// Backwards they take 171 a state and 120 a token. At 2.4 GHz and 4 cycles a slot that is 360 and 850 us for [8, 4096, 2048] with N = 16; in
+// bf16 with the gate it takes 378 us forwards (2.8e12 states a second, 1.6 TB/s) and 1086 backwards, where two waves a SIMD (256
+// registers, 80 KB of LDS a workgroup) leave a fifth of the slots empty. More waves of 4 tokens a lane were slower: they scan twice as often.
 #pragma once
 
 #include "ops_common.hpp"
@@ -406,7 +409,8 @@ struct Carry { float A, h; };  // A log2(e), and the state
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // Forwards. A workgroup of 8 waves takes 8 / split groups of 4 channels through a stretch, tile by tile; the next tile's tensors
-// are loaded while this one is scanned. With ENDS only the states at the stretch's end are found, from zeros.
+// are loaded while this one is scanned. With ENDS only the states at the stretch's end are found, from zeros: [1, 30001, 256] in fp32,
+// in 59 parts, 47 us and then 66 (backwards 74 and 183, in 30).
 // ---------------------------------------------------------------------------------------------------------------------------
 constexpr int kFwdWaves = 8;
 
@@ -1036,32 +1040,49 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     }
 }
 
-// gB and gC: the sums of the workgroups of a group of channels, in order.
+// gB and gC: the sums of the workgroups of a group of channels, in order. Memory bounds it: what the workgroups wrote, read once. Eight
+// loads of 16 bytes are under way at a time: [8, 4096, 2048], N = 16, 64 workgroups a token, 268 MB: 58 us, 4.6 TB/s (4 bytes a lane,
+// as many loads as the compiler took together: 75).
 struct GroupSum {
     scanscam_selective a;
     const float *bc;
     int64_t blocks;
 };
-template <typename ST>
+// VEC: neighbouring states of a lane, 4 where their number allows it.
+template <typename ST, int VEC>
 __global__ __launch_bounds__(256) void selective_bc_kernel(GroupSum args)
 {
+    constexpr int kTogether = 8;
     const scanscam_selective &a = args.a;
-    const int64_t wide = 2 * a.N, tokens = a.batch * a.T;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, group = blockIdx.y;
+    const uint32_t wide = 2 * (uint32_t)a.N, tokens = (uint32_t)(a.batch * a.T), i = (blockIdx.x * 256 + threadIdx.x) * VEC, group = blockIdx.y;
     if (i >= tokens * wide) return;
-    const int64_t token = i / wide;
-    int64_t n = i - token * wide;
-    const float *from = args.bc + group * args.blocks * tokens * wide + i;
-    float sum = 0.0f;
-    for (int64_t b = 0; b < args.blocks; b++) sum += from[b * tokens * wide];
+    typedef float vec_t __attribute__((ext_vector_type(VEC), aligned(4)));
+    const int64_t pitch = (int64_t)tokens * wide;
+    const float *from = args.bc + group * args.blocks * pitch + i;
+    vec_t sum = 0.0f;
+    int64_t b = 0;
+    for (; b + kTogether <= args.blocks; b += kTogether, from += kTogether * pitch) {
+        vec_t v[kTogether];
+#pragma unroll
+        for (int j = 0; j < kTogether; j++) v[j] = *reinterpret_cast<const vec_t *>(from + j * pitch);
+#pragma unroll
+        for (int j = 0; j < kTogether; j++) sum += v[j];
+    }
+    for (; b < args.blocks; b++, from += pitch) sum += *reinterpret_cast<const vec_t *>(from);
+    const uint32_t token = i / wide, batch = token / (uint32_t)a.T;
+    uint32_t n = i - token * wide;
     const scanscam_tokens &to = n < a.N ? a.gB : a.gC;
-    if (n >= a.N) n -= a.N;
-    const int64_t batch = token / a.T;
-    const_cast<ST *>(token_at<ST>(to, batch, token - batch * a.T, group * to.group + n))[0] = (ST)sum;
+    if (n >= a.N) n -= (uint32_t)a.N;
+    float f[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; k++) f[k] = sum[k];
+    store_some(const_cast<ST *>(token_at<ST>(to, batch, token - batch * (uint32_t)a.T, group * to.group + n)), VEC, f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------
-// One token: LANES lanes a channel, each with 4 neighbouring states at a time.
+// One token: LANES lanes a channel, each with 4 neighbouring states at a time, so that a wave reads and writes the states, which are nearly
+// all there is, in one piece; everything is asked for before any of it is used. 512 rows of 2048 channels, N = 16, bf16: 29 us for 143 MB,
+// 4.9 TB/s. One row: 4 us, which are a launch and one trip to memory.
 // ---------------------------------------------------------------------------------------------------------------------------
 template <typename ST, int LANES>
 __global__ __launch_bounds__(256) void selective_step_kernel(scanscam_selective_step a)

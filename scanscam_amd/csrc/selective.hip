@@ -81,13 +81,13 @@ int64_t span_of(const scanscam_selective &a)
 
 // Two workgroups fit a CU, and one keeps it nearly as busy, so that from 192 workgroups on nothing is cut. Below, sharing the states
 // of a channel out costs less than parts of time, whose first pass repeats most of the arithmetic, as long as it is two waves
-// (bf16, N = 16, us: [4, 2048, 1024] 128 whole, 93 by two waves, 105 in 4 parts; [6, 2048, 1024] 139, 137, 156); four
+// (bf16, N = 16, us: [4, 2048, 1024] 120 whole, 83 by two waves, 92 in 4 parts; [6, 2048, 1024] 117, 113, 134); four
 // or eight waves have too little to do for the tokens' own work and the barriers, so that with fewer channels parts win where there are
-// tiles for them ([2, 2048, 1024] 127 whole, 72 by four waves, 63 in 8 parts; [1, 2048, 1024] 128, 70, 40 in 16), and not in
-// short sequences ([1, 512, 2048] 39 whole, 26 by four waves, 30 in 4 parts). Packed sequences differ in length, and the longest may take
+// tiles for them ([2, 2048, 1024] 114 whole, 61 by four waves, 56 in 8 parts; [1, 2048, 1024] 113, 59, 38 in 16), and not in
+// short sequences ([1, 512, 2048] 34 whole, 24 by four waves, 28 in 4 parts). Packed sequences differ in length, and the longest may take
 // longer than all work shared out evenly: two waves then halve the time that one workgroup is busy with it (13 sequences, 8021
-// tokens, 2048 channels, six sets of lengths, one wave / two waves / cut into parts of four tiles: 130/159/224, 149/146/187, 311/219/209,
-// 132/143/180, 162/146/191, 118/141/206 us).
+// tokens, 2048 channels, six sets of lengths, one wave / two waves / cut into parts of four tiles: 113/133/189, 136/126/173, 292/207/188,
+// 123/125/170, 151/128/179, 104/124/184 us).
 Plan forward_plan(const scanscam_selective &a)
 {
     if (a.parts > 0) return {1, span_of(a)};

@@ -19,7 +19,7 @@
 // The vector unit bounds it. Forwards a lane's 8 tokens take 74 issue slots a state (65 instructions; 9 exponentials take two), of which 56
 // are the formula's: 148 a token and channel at N = 16, with some 70 more for what a token costs once, for 8 bytes of 16-bit tensors.
 // Backwards they take 171 a state and 120 a token. At 2.4 GHz and 4 cycles a slot that is 360 and 850 us for [8, 4096, 2048] with N = 16; in
-// bf16 with the gate it takes 378 us forwards (2.8e12 states a second, 1.6 TB/s) and 1086 backwards, where two waves a SIMD (256
+// bf16 with the gate it takes 371 us forwards (2.9e12 states a second, 1.6 TB/s) and 1080 backwards, where two waves a SIMD (256
 // registers, 80 KB of LDS a workgroup) leave a fifth of the slots empty. More waves of 4 tokens a lane were slower: they scan twice as often.
 #pragma once
 
@@ -352,19 +352,17 @@ struct SelectiveArgs {
 
 // Workgroups are dealt out to the 8 dies in turn, each with an L2 cache of its own, while neighbouring blocks of channels share the
 // 128-byte lines of every token (a block of 16 channels of 16 bits is a quarter of one) and all of B and C: dealt out one by
-// one, a line is fetched by up to four dies, and written by them in pieces. So a die takes neighbours: an eighth of all work where
-// sequences are of one length, and 8 blocks in turn where they are not, as dies would then be done at different times. (Backward
-// kernel of the layer [8, 4096, 2048] in bf16: one by one 1328 us, 8 in turn 1282, eighths 1234; packed prompts forwards: 135,
-// 139 and 170 us.)
+// one, a line is fetched by up to four dies, and written by them in pieces. So a die takes 8 neighbours in turn. (Layer [8, 4096, 2048]
+// in bf16, forwards / forwards and backwards, and packed prompts forwards, us: one by one 388 / 1558, 133; 4 in turn 381 / 1533, 126; 8
+// 371 / 1522, 127; 16 377 / 1532, 127; 32 381 / 1530, 133; an eighth of all work each 388 / 1535, 170.)
 struct Work {
     uint32_t block, unit;  // block of channels among all groups'; part of a sequence
 };
-__device__ __forceinline__ Work work_of(uint32_t blocks, bool even)
+__device__ __forceinline__ Work work_of(uint32_t blocks)
 {
-    constexpr uint32_t kDies = 8;
-    const uint32_t near = even ? gridDim.x / kDies : 8u, round = near * kDies;
+    constexpr uint32_t kDies = 8, near = 8, round = near * kDies;
     uint32_t i = blockIdx.x;
-    if (near > 0 && i < gridDim.x / round * round) i = i / round * round + i % kDies * near + i % round / kDies;
+    if (i < gridDim.x / round * round) i = i / round * round + i % kDies * near + i % round / kDies;
     const uint32_t unit = i / blocks;
     return {i - unit * blocks, unit};
 }
@@ -438,7 +436,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     Carry *lh = reinterpret_cast<Carry *>(lskip + channels), *nowhere = lh + channels * N;  // [N][channels]
 
     const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
-    const Work w = work_of((uint32_t)a.groups * args.blocks, a.offsets == nullptr);
+    const Work w = work_of((uint32_t)a.groups * args.blocks);
     const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * channels;  // c0: inside the group
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;  // first channel
@@ -684,7 +682,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     float *nowhere = lsum + 2 * kBwdWaves * wide;
 
     const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
-    const Work w = work_of((uint32_t)a.groups * args.blocks, a.offsets == nullptr);
+    const Work w = work_of((uint32_t)a.groups * args.blocks);
     const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * wide;
     const int here = (int)clamp_(per_group - c0, 0, wide), sets = (here + channels - 1) / channels;
     const int64_t first = group * per_group + c0;

@@ -17,10 +17,11 @@
 // rounding) is done by other lanes on the way between the channel-fastest tensors and the token-fastest rows in LDS.
 //
 // The vector unit bounds it. Forwards a lane's 8 tokens take 74 issue slots a state (65 instructions; 9 exponentials take two), of which 56
-// are the formula's: 148 a token and channel at N = 16, with some 70 more for what a token costs once, for 8 bytes of 16-bit tensors.
-// Backwards they take 171 a state and 120 a token. At 2.4 GHz and 4 cycles a slot that is 360 and 850 us for [8, 4096, 2048] with N = 16; in
-// bf16 with the gate it takes 371 us forwards (2.9e12 states a second, 1.6 TB/s) and 1080 backwards, where two waves a SIMD (256
-// registers, 80 KB of LDS a workgroup) leave a fifth of the slots empty. More waves of 4 tokens a lane were slower: they scan twice as often.
+// are the formula's: 148 a token and channel at N = 16, with 63 more for what a token costs once, for 8 bytes of 16-bit tensors.
+// Backwards they take 171 a state, 342 a token and channel, with 162 more. At 2.4 GHz and 4 cycles a slot that is 360 and 860 us for
+// [8, 4096, 2048] with N = 16; in bf16 with the gate it takes 371 us forwards (2.9e12 states a second, 1.6 TB/s) and 1075 backwards, where
+// two waves a SIMD (256 registers, 80 KB of LDS a workgroup) leave a fifth of the slots empty. More waves of 4 tokens a lane were
+// slower: they scan twice as often.
 #pragma once
 
 #include "ops_common.hpp"

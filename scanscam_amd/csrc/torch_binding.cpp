@@ -565,11 +565,13 @@ struct Gradients {
     at::Tensor empty(const at::Tensor &t) const { return t.defined() ? empty(t, t.scalar_type()) : at::Tensor(); }
     at::Tensor bytes(size_t n) const { return n != 0 ? output({(int64_t)n}, at::kByte, like.device()) : at::Tensor(); }
     // Zeros where there is no gradient; a copy where the last dimension is not unit-stride or tokens are too far apart.
-    at::Tensor tokens(const at::Tensor &g) const
+    at::Tensor tokens(const at::Tensor &g) const { return g.defined() ? near(g) : at::zeros(like.sizes(), like.options()); }
+    // What was saved, as the kernels take it: a hook on saved tensors may lay out what it gives back in its own way.
+    static at::Tensor near(const at::Tensor &t)
     {
-        if (!g.defined()) return at::zeros(like.sizes(), like.options());
-        return (g.size(-1) == 1 || g.stride(-1) == 1) && g.stride(1) < SCANSCAM_MOST_TOKEN_STRIDE ? g : g.contiguous();
+        return !t.defined() || ((t.size(-1) == 1 || t.stride(-1) == 1) && t.stride(1) < SCANSCAM_MOST_TOKEN_STRIDE) ? t : t.contiguous();
     }
+    static at::Tensor dense(const at::Tensor &t) { return t.defined() ? t.contiguous() : t; }
     static scanscam_tokens view(const at::Tensor &t)
     {
         if (!t.defined()) return {};
@@ -633,9 +635,7 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         const variable_list saved = ctx->get_saved_variables();
-        // (a hook on saved tensors may lay out what it gives back as it likes)
-        const at::Tensor kept = row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous();
-        const at::Tensor &weight = saved[1], &rstd = saved[2];
+        const at::Tensor kept = row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous(), weight = Gradients::dense(saved[1]), rstd = Gradients::dense(saved[2]);
         const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
         const bool added = ctx->saved_data["residual"].toBool();
         at::Tensor gy = grads[0], gsum = added ? grads[1] : at::Tensor();
@@ -686,7 +686,8 @@ struct ConvBackward : torch::autograd::Function<ConvBackward> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &offsets = saved[4];
+        const at::Tensor x = Gradients::near(saved[0]), weight = Gradients::dense(saved[1]), bias = Gradients::dense(saved[2]), state = Gradients::dense(saved[3]),
+                         offsets = Gradients::dense(saved[4]);
         at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
         if (!grads[0].defined() && !gstate_out.defined()) return {{}, {}, {}, {}, {}};
         const c10::DeviceGuard guard(x.device());
@@ -741,8 +742,10 @@ struct SelectiveBackward : torch::autograd::Function<SelectiveBackward> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         const variable_list kept = ctx->get_saved_variables();
-        const at::Tensor &x = kept[0], &dt = kept[1], &A = kept[2], &B = kept[3], &C = kept[4], &D = kept[5], &z = kept[6], &bias = kept[7], &state = kept[8],
-                         &offsets = kept[9], &saved = kept[10];
+        const auto near = [&](int i) { return Gradients::near(kept[i]); };
+        const auto dense = [&](int i) { return Gradients::dense(kept[i]); };
+        const at::Tensor x = near(0), dt = near(1), A = dense(2), B = near(3), C = near(4), D = dense(5), z = near(6), bias = dense(7), state = dense(8),
+                         offsets = dense(9), saved = dense(10);
         at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
         if (!grads[0].defined() && !gstate_out.defined()) return variable_list(10);
         const c10::DeviceGuard guard(x.device());

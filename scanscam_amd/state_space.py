@@ -328,10 +328,13 @@ class SelectiveScan(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gnew):
-        *seen, saved = ctx.saved_tensors
-        x, dt, A, B, C, D, z, dt_bias, state, offsets = seen
         if gy is None and gnew is None:
             return (None,) * 12
+        x, dt, A, B, C, D, z, dt_bias, state, offsets, saved = ctx.saved_tensors
+        # (a hook on saved tensors may lay out what it gives back in its own way)
+        x, dt, B, C, z = (_near(t) for t in (x, dt, B, C, z))
+        A, D, dt_bias, state, offsets, saved = (_dense(t) for t in (A, D, dt_bias, state, offsets, saved))
+        seen = x, dt, A, B, C, D, z, dt_bias, state, offsets
         L = _lib()
         with hip._on(x.device):
             gy = _near(gy) if gy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
@@ -478,9 +481,10 @@ class CausalConv(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gnew):
-        x, weight, bias, state, offsets = ctx.saved_tensors
         if gy is None and gnew is None:
             return (None,) * 7
+        x, *others = ctx.saved_tensors
+        x, (weight, bias, state, offsets) = _unit(x), (_dense(t) for t in others)  # (as above)
         L = _lib()
         with hip._on(x.device):
             gy = _unit(gy) if gy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
@@ -643,7 +647,7 @@ class RmsNorm(torch.autograd.Function):
         with hip._on(device):
             gy = torch.zeros(shape, dtype=dtype, device=device) if gy is None else gy.contiguous()
             gtotal = _dense(gtotal)
-            rows = kept.reshape(-1, shape[-1]) if kept.numel() else kept.reshape(0, shape[-1])
+            rows, weight, rstd = _rows(kept), _dense(weight), _dense(rstd)
             a = _norm_args(rows, weight, residual_dtype, 0.0)
             a.dtype, a.rstd, a.gy, a.gsum = _TYPES[dtype], rstd.data_ptr(), gy.data_ptr(), _ptr(gtotal)
             gx = torch.empty(shape, dtype=dtype, device=device)

@@ -496,6 +496,23 @@ def test_native_autograd_nodes_are_the_python_ones(gpu, monkeypatch):
         for residual in (r, r.to(dtype)):
             for only in (None, 0, 1):
                 both(f.rms_norm, dict(x=x, weight=w, residual=residual), dict(eps=1e-3), only=only)
+    def spread(t):  # the same values at other strides
+        if t.dim() == 0 or t.numel() == 0:
+            return t
+        out = torch.empty([2 * n for n in t.shape], dtype=t.dtype, device=t.device)[tuple(slice(None, None, 2) for _ in t.shape)]
+        return out.copy_(t)
+
+    v = {k: None if t is None else t.to(gpu) for k, t in make_scan(20, torch.float32, 2, 140, 24, 16, groups=2, state=True).items()}
+    leaves = [t.requires_grad_() for t in v.values() if t is not None]
+    w4, wide = torch.randn(24, 4, device=gpu, requires_grad=True), torch.randn(24, device=gpu, requires_grad=True)
+    for path in (native, None):
+        monkeypatch.setattr(state_space, "_native", path)
+        got = []
+        for unpack in (lambda t: t, spread):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+                y = f.selective_scan(**dict(v, x=f.causal_conv(f.rms_norm(v["x"], wide), w4, activation="silu")), softplus=True)
+            got.append(torch.autograd.grad(y.square().sum(), [*leaves, w4, wide]))
+        assert all(torch.equal(p, q) for p, q in zip(*got))
     for path in (native, None):
         monkeypatch.setattr(state_space, "_native", path)
         wide = torch.randn(4, 6, 80, device=gpu, requires_grad=True)

@@ -7,7 +7,7 @@
 //
 // Memory bounds it: each tensor once. A row stays in the registers of one to sixteen waves, so that nothing is read twice. [32768, 2048] in
 // bf16 with a float32 residual: 146 us forwards (805 MB, 5.5 TB/s), 215 backwards (1074 MB, 5.0 TB/s); [16384, 2049] in bf16 to 8 bits,
-// where three rows in four begin inside a vector: 52 us (235 MB, 4.5 TB/s); 16 rows of 2048: 4 us, a launch and one trip to memory.
+// where seven rows in eight begin inside a vector: 53 us (235 MB, 4.5 TB/s); 16 rows of 2048: 4 us, a launch and one trip to memory.
 #pragma once
 
 #include "ops_common.hpp"
@@ -147,9 +147,13 @@ template <int VEC> struct Weights {
     }
 };
 
+// Waves a SIMD at least: rows of 6 vectors of 8 that begin inside one take 132 registers and three waves if they may; in the 128 of four, three
+// of them spilled, [16384, 2049] to 8 bits takes 53 us instead of 56 (whole vectors, [16384, 2048]: 47).
+template <typename ST, typename RT, int NV, bool EXACT> constexpr int norm_fwd_least() { return !EXACT && NV == 6 && norm_vec<ST, RT>() == 8 ? 4 : 1; }
+
 // A workgroup holds 4 waves, or the row's. RT: the residual's type (the activations' where there is none).
 template <typename ST, typename RT, int NV, int THREADS, bool EXACT>
-__global__ __launch_bounds__(THREADS) void norm_fwd_kernel(NormArgs args)
+__global__ __launch_bounds__(THREADS, (norm_fwd_least<ST, RT, NV, EXACT>())) void norm_fwd_kernel(NormArgs args)
 {
     constexpr int VEC = norm_vec<ST, RT>();
     const scanscam_norm &a = args.a;

@@ -227,6 +227,12 @@ def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether a forward-mode derivative is asked for, which no kernel here has: calls with gradients go through their autograd
+    function, which refuses it as scan()'s does, and the others refuse it themselves."""
+    return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 # -------------------------------------------------------------------------------------------------------------------- selective scan
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
                    D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, *,
@@ -273,7 +279,8 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         return baseline.naive_selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus=softplus, state=state, offsets=offsets, return_state=return_state)
     if B.dim() == 3:
         B, C = _grouped(B), _grouped(C)
-    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
+    given = (x, dt, A, B, C, D, z, dt_bias, state)
+    if _wants_grad(*given) or _has_tangent(*given):
         y, new = SelectiveScan.apply(x, dt, A, B, C, D, z, dt_bias, state, offsets, bool(softplus), bool(return_state))
     else:
         y, new, _, _ = _selective_forward(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus, return_state, False)
@@ -387,7 +394,7 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         raise TypeError(f"{what}: state must be float32, got {state.dtype}")
     _check_slots(what, rows, state, slots)
     _check_in_place(what, state)
-    if _wants_grad(x, dt, A, B, C, D, z, dt_bias):
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias) or _has_tangent(state, x, dt, A, B, C, D, z, dt_bias):
         raise RuntimeError(f"{what}: a single token's step has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_selective_scan_step(state, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, slots=slots)
@@ -437,7 +444,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         _check_shape(what, name, t, shape)
     if x.device.type != "cuda":
         return baseline.naive_causal_conv(x, weight, bias, activation=activation, state=state, offsets=offsets, return_state=return_state)
-    if _wants_grad(x, weight, bias, state):
+    if _wants_grad(x, weight, bias, state) or _has_tangent(x, weight, bias, state):
         y, new = CausalConv.apply(x, weight, bias, state, offsets, activation, bool(return_state))
     else:
         y, new, _ = _conv_forward(x, weight, bias, state, offsets, activation, return_state)
@@ -529,7 +536,7 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         _check_shape(what, name, t, shape)
     _check_slots(what, rows, state, slots)
     _check_in_place(what, state)
-    if _wants_grad(x, weight, bias):
+    if _wants_grad(x, weight, bias) or _has_tangent(state, x, weight, bias):
         raise RuntimeError(f"{what}: a single token's step has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_causal_conv_step(state, x, weight, bias, activation=activation, slots=slots)
@@ -575,7 +582,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     _check_shape(what, "residual", residual, x.shape)
     if quant is not None and quant not in _EIGHT:
         raise TypeError(f"{what}: quant must be None, int8 or float8_e4m3fn, got {quant}")
-    grad = _wants_grad(x, weight, residual)
+    grad = _wants_grad(x, weight, residual) or _has_tangent(x, weight, residual)
     if grad and quant is not None:
         raise RuntimeError(f"{what}: an output in 8 bits has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":

@@ -1,0 +1,58 @@
+"""
+Calls of the state space layer's operators that are not plain ones: forward-mode derivatives, recorded calls. None of them may give
+an answer that looks right and is not.
+"""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import scanscam_amd as f
+
+pytestmark = pytest.mark.gpu
+
+
+def calls(gpu, seed=0):
+    """name: (function of tensors, the tensors), without gradients of their own."""
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=gpu)  # noqa: E731
+    x, dt, z, B, C = r(2, 37, 24), r(2, 37, 24), r(2, 37, 24), r(2, 37, 2, 8), r(2, 37, 2, 8)
+    A, D, bias, state, w, kept = -r(24, 8).exp(), r(24), r(24), r(2, 24, 8), r(24, 4), r(2, 3, 24)
+    return {
+        "rms_norm": (lambda x, w: f.rms_norm(x, w), (x, D)),
+        "rms_norm_residual": (lambda x, w, r: f.rms_norm(x, w, r), (x, D, z)),
+        "causal_conv": (lambda x, w, b: f.causal_conv(x, w, b, activation="silu"), (x, w, bias)),
+        "causal_conv_state": (lambda x, w, b, s: f.causal_conv(x, w, b, state=s, return_state=True), (x, w, bias, kept)),
+        "selective_scan": (lambda *t: f.selective_scan(*t, softplus=True), (x, dt, A, B, C, D, z, bias)),
+        "selective_scan_state": (lambda s, *t: f.selective_scan(*t, state=s, return_state=True), (state, x, dt.abs(), A, B, C)),
+    }
+
+
+def single(gpu, seed=0):
+    """The calls that have no gradient, the steps with their state first."""
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=gpu)  # noqa: E731
+    slots = torch.tensor([4, 0, -1, 2], device=gpu)
+    return {
+        "rms_norm_int8": (lambda x, w: f.rms_norm(x, w, quant=torch.int8), (r(5, 40), r(40))),
+        "rms_norm_int8_residual": (lambda x, w, s: f.rms_norm(x, w, s, quant=torch.int8), (r(5, 40), r(40), r(5, 40))),
+        "selective_scan_step": (lambda s, *t: f.selective_scan_step(s, *t, softplus=True, slots=slots), (r(6, 24, 8), r(4, 24), r(4, 24), -r(24, 8).exp(), r(4, 8), r(4, 8))),
+        "causal_conv_step": (lambda s, *t: f.causal_conv_step(s, *t, activation="silu", slots=slots), (r(6, 3, 24), r(4, 24), r(24, 4), r(24))),
+    }
+
+
+def listed(out):
+    return list(out) if isinstance(out, (tuple, list)) else [out]
+
+
+@pytest.mark.parametrize("name", list(calls("cpu")) + list(single("cpu")))
+def test_forward_mode_is_refused(gpu, name):
+    """As scan() refuses it; an output without a tangent would be a derivative of zero."""
+    fn, tensors = {**calls(gpu), **single(gpu)}[name]
+    for i in range(len(tensors)):
+        for grads in (True, False):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grads):
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if k == i else t for k, t in enumerate(tensors)]
+                with pytest.raises(RuntimeError):  # (NotImplementedError is one)
+                    fn(*dual)
+    with forward_ad.dual_level():  # nothing of the call's has a tangent
+        assert all(torch.isfinite(o.float()).all() for o in listed(fn(*[t.clone() for t in tensors])))

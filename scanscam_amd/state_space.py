@@ -233,6 +233,12 @@ def _has_tangent(*tensors) -> bool:
     return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def _needs_node(*tensors) -> bool:
+    """Whether a call has to go through its autograd function: for gradients, and where torch.jit.trace records it, which sees the function but
+    not a launch (it would record the allocation of the outputs and nothing that writes them)."""
+    return _wants_grad(*tensors) or _has_tangent(*tensors) or torch.jit.is_tracing()
+
+
 # -------------------------------------------------------------------------------------------------------------------- selective scan
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
                    D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, *,
@@ -279,8 +285,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         return baseline.naive_selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus=softplus, state=state, offsets=offsets, return_state=return_state)
     if B.dim() == 3:
         B, C = _grouped(B), _grouped(C)
-    given = (x, dt, A, B, C, D, z, dt_bias, state)
-    if _wants_grad(*given) or _has_tangent(*given):
+    if _needs_node(x, dt, A, B, C, D, z, dt_bias, state):
         y, new = SelectiveScan.apply(x, dt, A, B, C, D, z, dt_bias, state, offsets, bool(softplus), bool(return_state))
     else:
         y, new, _, _ = _selective_forward(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus, return_state, False)
@@ -400,10 +405,17 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         return baseline.naive_selective_scan_step(state, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, slots=slots)
     if B.dim() == 2:
         B, C = _grouped(B), _grouped(C)
+    if torch.jit.is_tracing():
+        return SelectiveScanStep.apply(state, x, dt, A, B, C, D, z, dt_bias, slots, bool(softplus))
+    return _selective_step(state, x, dt, A, B, C, D, z, dt_bias, slots, softplus)
+
+
+def _selective_step(state, x, dt, A, B, C, D, z, dt_bias, slots, softplus):
     L = _lib()
     with hip._on(x.device):
         x, dt, B, C, z = (_unit(t) for t in (x, dt, B, C, z))
         A, D, dt_bias, slots = (_dense(t) for t in (A, D, dt_bias, slots))
+        (rows, channels), groups, N = x.shape, B.shape[1], A.shape[1]
         y = torch.empty((rows, channels), dtype=x.dtype, device=x.device)
         a = _SelectiveStep(rows, channels, groups, N, state.shape[0], _ptr(slots), int(slots is not None and slots.dtype == torch.int64),
                            _TYPES[x.dtype], int(softplus), 0, _tokens(x, 1), _tokens(dt, 1), _tokens(B, 1), _tokens(C, 1), _tokens(z, 1),
@@ -411,6 +423,17 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         _raise(L.scanscam_selective_step_fwd(a, _stream(x.device)), "selective_step_fwd")
     torch.autograd.graph.increment_version(state)  # (written in place)
     return y
+
+
+class SelectiveScanStep(torch.autograd.Function):
+    """What a trace records of a step (see ``_needs_node``); there is no gradient. A replay takes no function that is marked as changing
+    its arguments, but runs functions in their order."""
+
+    @staticmethod
+    def forward(ctx, state, x, dt, A, B, C, D, z, dt_bias, slots, softplus):
+        y = _selective_step(state, x, dt, A, B, C, D, z, dt_bias, slots, softplus)
+        ctx.mark_non_differentiable(y)
+        return y
 
 
 # ------------------------------------------------------------------------------------------------------------------- convolution
@@ -444,7 +467,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         _check_shape(what, name, t, shape)
     if x.device.type != "cuda":
         return baseline.naive_causal_conv(x, weight, bias, activation=activation, state=state, offsets=offsets, return_state=return_state)
-    if _wants_grad(x, weight, bias, state) or _has_tangent(x, weight, bias, state):
+    if _needs_node(x, weight, bias, state):
         y, new = CausalConv.apply(x, weight, bias, state, offsets, activation, bool(return_state))
     else:
         y, new, _ = _conv_forward(x, weight, bias, state, offsets, activation, return_state)
@@ -540,16 +563,31 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         raise RuntimeError(f"{what}: a single token's step has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_causal_conv_step(state, x, weight, bias, activation=activation, slots=slots)
+    if torch.jit.is_tracing():
+        return CausalConvStep.apply(state, x, weight, bias, slots, activation)
+    return _conv_step(state, x, weight, bias, slots, activation)
+
+
+def _conv_step(state, x, weight, bias, slots, activation):
     L = _lib()
     with hip._on(x.device):
         x = _unit(x)
         weight, bias, slots = (_dense(t) for t in (weight, bias, slots))
+        (rows, channels), K = x.shape, weight.shape[1]
         y = torch.empty((rows, channels), dtype=x.dtype, device=x.device)
         a = _ConvStep(rows, channels, K, state.shape[0], _ptr(slots), int(slots is not None and slots.dtype == torch.int64), _TYPES[x.dtype],
                       _ACTIVATIONS[activation], 0, _tokens(x, 1), _tokens(y, 1), _param(weight), _param(bias), state.data_ptr())
         _raise(L.scanscam_conv_step_fwd(a, _stream(x.device)), "conv_step_fwd")
     torch.autograd.graph.increment_version(state)
     return y
+
+
+class CausalConvStep(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, state, x, weight, bias, slots, activation):
+        y = _conv_step(state, x, weight, bias, slots, activation)
+        ctx.mark_non_differentiable(y)
+        return y
 
 
 # -------------------------------------------------------------------------------------------------------------------------- norm
@@ -582,15 +620,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     _check_shape(what, "residual", residual, x.shape)
     if quant is not None and quant not in _EIGHT:
         raise TypeError(f"{what}: quant must be None, int8 or float8_e4m3fn, got {quant}")
-    grad = _wants_grad(x, weight, residual) or _has_tangent(x, weight, residual)
-    if grad and quant is not None:
+    if quant is not None and (_wants_grad(x, weight, residual) or _has_tangent(x, weight, residual)):
         raise RuntimeError(f"{what}: an output in 8 bits has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_rms_norm(x, weight, residual, eps=eps, quant=quant)
-    if grad:
+    if quant is None and _needs_node(x, weight, residual):
         y, total = RmsNorm.apply(x, weight, residual, float(eps))
         return y if residual is None else (y, total)
-    y, scale, total, _ = _norm_forward(x, weight, residual, eps, quant, False)
+    if torch.jit.is_tracing():
+        y, scale, total = RmsNormEight.apply(x, weight, residual, float(eps), quant)
+    else:
+        y, scale, total, _ = _norm_forward(x, weight, residual, eps, quant, False)
     return y if quant is None and total is None else tuple(t for t in (y, scale, total) if t is not None)
 
 
@@ -670,3 +710,13 @@ class RmsNorm(torch.autograd.Function):
             a.workspace, a.workspace_bytes = _ptr(workspace), n
             _raise(L.scanscam_norm_bwd(a, _stream(device)), "norm_bwd")
             return gx, gweight.to(weight.dtype), gresidual, None
+
+
+class RmsNormEight(torch.autograd.Function):
+    """What a trace records of a norm in 8 bits; there is no gradient."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, quant):
+        y, scale, total, _ = _norm_forward(x, weight, residual, eps, quant, False)
+        ctx.mark_non_differentiable(*(t for t in (y, scale, total) if t is not None))
+        return y, scale, total

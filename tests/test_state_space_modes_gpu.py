@@ -56,3 +56,46 @@ def test_forward_mode_is_refused(gpu, name):
                     fn(*dual)
     with forward_ad.dual_level():  # nothing of the call's has a tangent
         assert all(torch.isfinite(o.float()).all() for o in listed(fn(*[t.clone() for t in tensors])))
+
+
+@pytest.mark.parametrize("name", list(calls("cpu")) + list(single("cpu")))
+def test_a_trace_runs_the_kernels(gpu, name):
+    """A call that torch.jit.trace recorded computes when it is replayed, with other inputs than those it saw, and updates states in place."""
+    fn, tensors = {**calls(gpu), **single(gpu)}[name]
+    with torch.no_grad():
+        traced = torch.jit.trace(fn, [t.clone() for t in tensors], check_trace=False)
+        for seed in (1, 2):
+            given = {**calls(gpu, seed), **single(gpu, seed)}[name][1]
+            outs = []
+            for call in (fn, traced):
+                for n in (1 << 16, 1 << 10):
+                    torch.full((n,), float("nan"), device=gpu)  # (memory that an output which nothing writes would show)
+                own = [t.clone() for t in given]
+                outs.append([*listed(call(*own)), *own])
+            assert len(outs[0]) == len(outs[1]) and all(torch.equal(p, q) for p, q in zip(*outs))
+    if name in calls("cpu"):  # recorded without gradients, replayed with them
+        grads = []
+        for call in (fn, traced):
+            leaves = [t.clone().requires_grad_() for t in tensors]
+            grads.append(torch.autograd.grad([o.square().sum() for o in listed(call(*leaves))], leaves))
+        assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+def test_a_trace_of_several_steps_takes_them_in_order(gpu):
+    (scan, state, *t), (conv, kept, *u) = ((fn, *given) for fn, given in (single(gpu)[n] for n in ("selective_scan_step", "causal_conv_step")))
+
+    def three(state, kept, x, *rest):
+        outs = []
+        for _ in range(3):
+            x = scan(state, conv(kept, x, *u[1:]), *t[1:])
+            outs += [x, state.sum()]
+        return tuple(outs)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(three, (state.clone(), kept.clone(), t[0]), check_trace=False)
+        for scale in (1.0, 0.5):
+            outs = []
+            for call in (three, traced):
+                own = [state.clone(), kept.clone(), t[0] * scale]
+                outs.append([*call(*own), *own])
+            assert all(torch.equal(p, q) for p, q in zip(*outs))

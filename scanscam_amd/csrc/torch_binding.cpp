@@ -555,6 +555,13 @@ using torch::autograd::AutogradContext;
 using Maybe = std::optional<at::Tensor>;
 Maybe maybe(const at::Tensor &t) { return t.defined() ? Maybe(t) : std::nullopt; }
 
+// make_fx records ATen calls, of which a launch is none: it would take gradients for constants.
+void check_unrecorded(const char *what)
+{
+    if (c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+        throw std::runtime_error(std::string(what) + ": make_fx cannot record this call, whose kernels are no ATen operators");
+}
+
 // What a backward call has of its own: outputs, a workspace, gradients as the library takes them.
 struct Gradients {
     const at::Tensor &like;
@@ -634,6 +641,7 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        check_unrecorded("rms_norm");
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor kept = row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous(), weight = Gradients::dense(saved[1]), rstd = Gradients::dense(saved[2]);
         const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
@@ -685,6 +693,7 @@ struct ConvBackward : torch::autograd::Function<ConvBackward> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        check_unrecorded("causal_conv");
         const variable_list saved = ctx->get_saved_variables();
         const at::Tensor x = Gradients::near(saved[0]), weight = Gradients::dense(saved[1]), bias = Gradients::dense(saved[2]), state = Gradients::dense(saved[3]),
                          offsets = Gradients::dense(saved[4]);
@@ -741,6 +750,7 @@ struct SelectiveBackward : torch::autograd::Function<SelectiveBackward> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
+        check_unrecorded("selective_scan");
         const variable_list kept = ctx->get_saved_variables();
         const auto near = [&](int i) { return Gradients::near(kept[i]); };
         const auto dense = [&](int i) { return Gradients::dense(kept[i]); };

@@ -13,6 +13,7 @@ else; CPU tensors take the loops of ``scanscam_amd.baseline``. None of this has 
 operator is the scan.
 """
 import ctypes
+import sys
 from typing import Optional, Tuple, Union
 
 import torch
@@ -93,6 +94,15 @@ def _lib():
             fn.argtypes, fn.restype = [ctypes.POINTER(args)] + more, _size
         _entry_points = lib
     return _entry_points
+
+
+def _launching(what: str):
+    """The library, for a call that launches kernels. make_fx records ATen calls, of which a launch is none: it would record outputs that
+    nothing writes."""
+    recorder = sys.modules.get("torch.fx.experimental.proxy_tensor")  # (where nothing has imported it nothing records)
+    if recorder is not None and recorder.get_proxy_mode() is not None:
+        raise RuntimeError(f"{what}: make_fx cannot record this call, whose kernels are no ATen operators")
+    return _lib()
 
 
 def _bind_native():
@@ -307,7 +317,7 @@ def _selective_args(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus) -> 
 
 def _selective_forward(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus, return_state, save):
     """``(y, new state or None, saved or None, the tensors as the library saw them)``."""
-    L = _lib()
+    L = _launching("selective_scan")
     with hip._on(x.device):
         seen = (_near(x), _near(dt), _dense(A), _near(B), _near(C), _dense(D), _near(z), _dense(dt_bias), _dense(state), _dense(offsets))
         a = _selective_args(*seen, softplus)
@@ -347,7 +357,7 @@ class SelectiveScan(torch.autograd.Function):
         x, dt, B, C, z = (_near(t) for t in (x, dt, B, C, z))
         A, D, dt_bias, state, offsets, saved = (_dense(t) for t in (A, D, dt_bias, state, offsets, saved))
         seen = x, dt, A, B, C, D, z, dt_bias, state, offsets
-        L = _lib()
+        L = _launching("selective_scan")
         with hip._on(x.device):
             gy = _near(gy) if gy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
             gnew = _dense(gnew)
@@ -411,7 +421,7 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
 
 
 def _selective_step(state, x, dt, A, B, C, D, z, dt_bias, slots, softplus):
-    L = _lib()
+    L = _launching("selective_scan_step")
     with hip._on(x.device):
         x, dt, B, C, z = (_unit(t) for t in (x, dt, B, C, z))
         A, D, dt_bias, slots = (_dense(t) for t in (A, D, dt_bias, slots))
@@ -485,7 +495,7 @@ def _conv_args(x, weight, bias, state, offsets, activation) -> _Conv:
 
 
 def _conv_forward(x, weight, bias, state, offsets, activation, return_state):
-    L = _lib()
+    L = _launching("causal_conv")
     with hip._on(x.device):
         seen = (_unit(x),) + tuple(_dense(t) for t in (weight, bias, state, offsets))
         a = _conv_args(*seen, activation)
@@ -515,7 +525,7 @@ class CausalConv(torch.autograd.Function):
             return (None,) * 7
         x, *others = ctx.saved_tensors
         x, (weight, bias, state, offsets) = _unit(x), (_dense(t) for t in others)  # (as above)
-        L = _lib()
+        L = _launching("causal_conv")
         with hip._on(x.device):
             gy = _unit(gy) if gy is not None else torch.zeros(x.shape, dtype=x.dtype, device=x.device)
             gnew = _dense(gnew)
@@ -569,7 +579,7 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
 
 
 def _conv_step(state, x, weight, bias, slots, activation):
-    L = _lib()
+    L = _launching("causal_conv_step")
     with hip._on(x.device):
         x = _unit(x)
         weight, bias, slots = (_dense(t) for t in (weight, bias, slots))
@@ -652,7 +662,7 @@ def _norm_args(x, weight, residual_dtype, eps) -> _Norm:
 
 def _norm_forward(x, weight, residual, eps, quant, save):
     """``(y, scale or None, sum or None, (what the backward call reads))``."""
-    L = _lib()
+    L = _launching("rms_norm")
     with hip._on(x.device):
         rows, more, weight = _rows(x), _rows(residual), _dense(weight)
         a = _norm_args(rows, weight, None if residual is None else residual.dtype, eps)
@@ -689,7 +699,7 @@ class RmsNorm(torch.autograd.Function):
         shape = (gy if gy is not None else gtotal).shape if gy is not None or gtotal is not None else None
         if shape is None:
             return None, None, None, None
-        L = _lib()
+        L = _launching("rms_norm")
         device = kept.device
         with hip._on(device):
             gy = torch.zeros(shape, dtype=dtype, device=device) if gy is None else gy.contiguous()

@@ -99,3 +99,27 @@ def test_a_trace_of_several_steps_takes_them_in_order(gpu):
                 own = [state.clone(), kept.clone(), t[0] * scale]
                 outs.append([*call(*own), *own])
             assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+@pytest.mark.parametrize("name", list(calls("cpu")) + list(single("cpu")))
+def test_make_fx_is_refused(gpu, name):
+    """It records ATen calls, of which these are none; its graph would return outputs that nothing writes. (CPU tensors' calls are.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    fn, tensors = {**calls(gpu), **single(gpu)}[name]
+    for mode in ("real", "fake"):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="make_fx"):
+            make_fx(fn, tracing_mode=mode)(*tensors)
+    if name in single("cpu"):
+        return
+
+    def gradients(*t):
+        leaves = [v.detach().requires_grad_() for v in t]
+        return torch.autograd.grad([o.sum() for o in listed(fn(*leaves))], leaves)
+
+    with pytest.raises(RuntimeError, match="make_fx"):
+        make_fx(gradients)(*tensors)
+    leaves = [t.clone().requires_grad_() for t in tensors]
+    outs = listed(fn(*leaves))
+    with pytest.raises(RuntimeError, match="make_fx"):  # the backward pass of a call made outside
+        make_fx(lambda *g: torch.autograd.grad(outs, leaves, g))(*[torch.ones_like(o) for o in outs])

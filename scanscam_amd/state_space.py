@@ -133,6 +133,25 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# ---------------------------------------------------------------------------------------------------------------- compiled callers
+_outside = {}
+
+
+def _eager(fn, *args, **kwargs):
+    """A call from a function that torch.compile traces: it breaks the graph there and runs as it does everywhere else. (Traced through, it
+    would come to the library's entry points, which no graph can hold.)"""
+    if fn not in _outside:
+        _outside[fn] = torch.compiler.disable(fn)
+    return _outside[fn](*args, **kwargs)
+
+
+_eager._torchdynamo_disable = True  # (what torch.compiler.disable marks, without its import of the compiler)
+
+
+def _compiling(x: torch.Tensor) -> bool:
+    return torch.compiler.is_dynamo_compiling() and x.device.type == "cuda"
+
+
 # --------------------------------------------------------------------------------------------------------- checks of arguments
 def _check_types(what: str, first: torch.Tensor, tensors, params) -> None:
     if first.dtype not in _TYPES:
@@ -269,7 +288,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     :param return_state: hand back the states after the last tokens as well, in float32
     :return: y, or ``(y, state)``. Differentiable in every tensor but ``offsets``.
     """
-    if _native is not None and _parts == 0 and not torch.compiler.is_compiling():
+    if _compiling(x):
+        return _eager(selective_scan, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, state=state, offsets=offsets, return_state=return_state)
+    if _native is not None and _parts == 0:
         out = _native.selective(x, dt, A, B, C, D, z, dt_bias, softplus, state, offsets, return_state)  # None: a call it leaves to the code below
         if out is not None:
             return out
@@ -388,7 +409,9 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         slot is not in ``state``, such as -1, is left out: its output is zero and no state changes.
     :return: y, [rows, channels]. Not differentiable.
     """
-    if _native is not None and not torch.compiler.is_compiling():
+    if _compiling(x):
+        return _eager(selective_scan_step, state, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, slots=slots)
+    if _native is not None:
         out = _native.selective_step(state, x, dt, A, B, C, D, z, dt_bias, softplus, slots)
         if out is not None:
             return out
@@ -461,7 +484,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     :param return_state: hand back the K - 1 inputs before the next token as well
     :return: y, or ``(y, state)``. Differentiable in every tensor but ``offsets``.
     """
-    if _native is not None and not torch.compiler.is_compiling():
+    if _compiling(x):
+        return _eager(causal_conv, x, weight, bias, activation=activation, state=state, offsets=offsets, return_state=return_state)
+    if _native is not None:
         out = _native.conv(x, weight, bias, activation, state, offsets, return_state)
         if out is not None:
             return out
@@ -553,7 +578,9 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     :param x: [rows, channels]; weight, bias, activation as for ``causal_conv``; slots as for ``selective_scan_step``
     :return: y, [rows, channels]. Not differentiable.
     """
-    if _native is not None and not torch.compiler.is_compiling():
+    if _compiling(x):
+        return _eager(causal_conv_step, state, x, weight, bias, activation=activation, slots=slots)
+    if _native is not None:
         out = _native.conv_step(state, x, weight, bias, activation, slots)
         if out is not None:
             return out
@@ -617,7 +644,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     :return: y; with a residual ``(y, sum)``; with ``quant`` ``(q, scale)`` or ``(q, scale, sum)``, scale being float32 and of x's
         leading shape. Differentiable (in x, weight and residual) unless ``quant`` is given.
     """
-    if _native is not None and not torch.compiler.is_compiling():
+    if _compiling(x):
+        return _eager(rms_norm, x, weight, residual, eps=eps, quant=quant)
+    if _native is not None:
         out = _native.norm(x, weight, residual, eps, _EIGHT.get(quant, -1) if quant is not None else 0)
         if out is not None:
             return out

@@ -123,3 +123,41 @@ def test_make_fx_is_refused(gpu, name):
     outs = listed(fn(*leaves))
     with pytest.raises(RuntimeError, match="make_fx"):  # the backward pass of a call made outside
         make_fx(lambda *g: torch.autograd.grad(outs, leaves, g))(*[torch.ones_like(o) for o in outs])
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_calls_from_compiled_functions(gpu, backend):
+    """torch.compile breaks its graph at a call, which then is what it is elsewhere, as scan()'s calls are."""
+    for name, (fn, tensors) in {**calls(gpu), **single(gpu)}.items():
+        def user(first, *rest):
+            return [o.float() * 2 for o in listed(fn(first, *rest))]
+
+        for grad in (False, True) if name in calls("cpu") else (False,):
+            torch._dynamo.reset()
+            results = []
+            for call in (user, torch.compile(user, backend=backend)):
+                own = [t.clone().requires_grad_(grad) for t in tensors]
+                outs = call(*own)
+                results.append(outs + (list(torch.autograd.grad([o.sum() for o in outs], own)) if grad else own))
+            assert all(torch.equal(p, q) for p, q in zip(*results)), (name, grad)
+    torch._dynamo.reset()
+
+
+def test_a_backward_pass_that_is_compiled(gpu):
+    """Compiled autograd calls the native nodes as they are."""
+    from torch._dynamo import compiled_autograd
+
+    for name, (fn, tensors) in calls(gpu).items():
+        grads = []
+        for compiled in (False, True):
+            torch._dynamo.reset()
+            leaves = [t.clone().requires_grad_() for t in tensors]
+            loss = sum(o.square().sum() for o in listed(fn(*leaves)))
+            if compiled:
+                with compiled_autograd._enable(torch.compile(backend="eager")):
+                    loss.backward()
+            else:
+                loss.backward()
+            grads.append([t.grad for t in leaves])
+        assert all(torch.equal(p, q) for p, q in zip(*grads)), name
+    torch._dynamo.reset()

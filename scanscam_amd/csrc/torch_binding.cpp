@@ -643,9 +643,10 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
     {
         check_unrecorded("rms_norm");
         const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor kept = row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous(), weight = Gradients::dense(saved[1]), rstd = Gradients::dense(saved[2]);
         const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
         const bool added = ctx->saved_data["residual"].toBool();
+        // (the library takes rows of x at any distance, those of a sum dense)
+        const at::Tensor kept = !added && row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous(), weight = Gradients::dense(saved[1]), rstd = Gradients::dense(saved[2]);
         at::Tensor gy = grads[0], gsum = added ? grads[1] : at::Tensor();
         if (!gy.defined() && !gsum.defined()) return {{}, {}, {}, {}};
         const c10::DeviceGuard guard(kept.device());

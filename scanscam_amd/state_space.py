@@ -733,7 +733,8 @@ class RmsNorm(torch.autograd.Function):
         with hip._on(device):
             gy = torch.zeros(shape, dtype=dtype, device=device) if gy is None else gy.contiguous()
             gtotal = _dense(gtotal)
-            rows, weight, rstd = _rows(kept), _dense(weight), _dense(rstd)
+            # (a hook on saved tensors may lay out what it gives back in its own way; the library takes rows of x at any distance, those of a sum dense)
+            rows, weight, rstd = _rows(kept if residual_dtype is None else kept.contiguous()), _dense(weight), _dense(rstd)
             a = _norm_args(rows, weight, residual_dtype, 0.0)
             a.dtype, a.rstd, a.gy, a.gsum = _TYPES[dtype], rstd.data_ptr(), gy.data_ptr(), _ptr(gtotal)
             gx = torch.empty(shape, dtype=dtype, device=device)

@@ -7,6 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 import scanscam_amd as f
+from scanscam_amd import state_space
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +162,37 @@ def test_a_backward_pass_that_is_compiled(gpu):
             grads.append([t.grad for t in leaves])
         assert all(torch.equal(p, q) for p, q in zip(*grads)), name
     torch._dynamo.reset()
+
+
+def rows_apart(t):
+    """The same values, unit-stride at the end, rows further apart than they are long."""
+    if t.dim() < 2:
+        return t
+    out = torch.full((*t.shape[:-1], 2, t.shape[-1]), float("nan"), dtype=t.dtype, device=t.device)[..., 0, :]
+    return out.copy_(t)
+
+
+def one_row(t):
+    """The same values, where all rows are alike, as one row at a distance of zero."""
+    return t if t.dim() < 2 else t[(slice(0, 1),) * (t.dim() - 1)].expand(t.shape)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("residual", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("unpack", [rows_apart, one_row])
+def test_norm_of_saved_rows_at_other_strides(gpu, monkeypatch, native, residual, unpack):
+    """What hooks on saved tensors give back may lie elsewhere in memory in a layout of its own: the gradients are the same bits."""
+    if not native:
+        monkeypatch.setattr(state_space, "_native", None)
+    g = torch.Generator(device=gpu).manual_seed(3)
+    row = torch.randn(1, 1, 40, generator=g, device=gpu)
+    x = row.expand(3, 7, 40).contiguous() if unpack is one_row else torch.randn(3, 7, 40, generator=g, device=gpu)
+    x, w, gy = x.to(torch.bfloat16), torch.randn(40, generator=g, device=gpu), torch.randn(3, 7, 40, generator=g, device=gpu).to(torch.bfloat16)
+    r = None if residual is None else (x * 3).to(residual)
+    grads = []
+    for give in (lambda t: t, unpack):
+        leaves = [t.clone().requires_grad_() for t in (x, w, r) if t is not None]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), give):
+            out = f.rms_norm(*leaves)
+        grads.append(torch.autograd.grad(out if residual is None else out[0], leaves, gy))
+    assert all(torch.equal(p, q) for p, q in zip(*grads))

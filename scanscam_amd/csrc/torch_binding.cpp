@@ -33,7 +33,9 @@
 
 #include <array>
 #include <atomic>
+#include <sstream>
 #include <unordered_map>
+#include <vector>
 
 #include "scanscam_hip.h"
 #include "scanscam_ops.h"
@@ -562,6 +564,39 @@ void check_unrecorded(const char *what)
         throw std::runtime_error(std::string(what) + ": make_fx cannot record this call, whose kernels are no ATen operators");
 }
 
+// What a node saves, with types and shapes (of each tensor its type and sizes, -1 where there is none): a hook on saved tensors may lay out
+// what it gives back in its own way, but the kernels take addresses.
+std::vector<int64_t> types_and_shapes(const variable_list &tensors)
+{
+    std::vector<int64_t> all;
+    all.reserve(tensors.size() * 5);
+    for (const at::Tensor &t : tensors) {
+        all.push_back(t.defined() ? (int64_t)t.scalar_type() : -1);
+        if (!t.defined()) continue;
+        all.push_back(t.dim());
+        for (const int64_t n : t.sizes()) all.push_back(n);
+    }
+    return all;
+}
+void keep(AutogradContext *ctx, variable_list &&tensors)
+{
+    ctx->saved_data["meta"] = types_and_shapes(tensors);
+    ctx->save_for_backward(std::move(tensors));
+}
+// ... and what it gets back, for gradients of which one is `grad`.
+variable_list returned(AutogradContext *ctx, const at::Tensor &grad, const char *what)
+{
+    variable_list tensors = ctx->get_saved_variables();
+    bool same = types_and_shapes(tensors) == ctx->saved_data["meta"].toIntVector();
+    for (const at::Tensor &t : tensors) same = same && (!t.defined() || (plain(t) && t.device() == grad.device()));
+    if (!same) {
+        std::ostringstream text;
+        text << what << ": a tensor that was saved for the backward pass came back with another type or shape, or not on " << grad.device() << " as it was";
+        throw std::runtime_error(text.str());
+    }
+    return tensors;
+}
+
 // What a backward call has of its own: outputs, a workspace, gradients as the library takes them.
 struct Gradients {
     const at::Tensor &like;
@@ -633,7 +668,7 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
     };
     static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &residual, Done *done)
     {
-        ctx->save_for_backward({residual ? done->sum : x, weight, done->rstd});
+        keep(ctx, {residual ? done->sum : x, weight, done->rstd});
         ctx->set_materialize_grads(false);
         ctx->saved_data["dtype"] = (int64_t)x.scalar_type();
         ctx->saved_data["residual"] = residual.has_value();
@@ -642,13 +677,13 @@ struct NormBackward : torch::autograd::Function<NormBackward> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         check_unrecorded("rms_norm");
-        const variable_list saved = ctx->get_saved_variables();
-        const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
         const bool added = ctx->saved_data["residual"].toBool();
-        // (the library takes rows of x at any distance, those of a sum dense)
-        const at::Tensor kept = !added && row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous(), weight = Gradients::dense(saved[1]), rstd = Gradients::dense(saved[2]);
         at::Tensor gy = grads[0], gsum = added ? grads[1] : at::Tensor();
         if (!gy.defined() && !gsum.defined()) return {{}, {}, {}, {}};
+        const variable_list saved = returned(ctx, gy.defined() ? gy : gsum, "rms_norm");
+        const auto type = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+        // (the library takes rows of x at any distance, those of a sum dense)
+        const at::Tensor kept = !added && row_stride(saved[0]) >= 0 ? saved[0] : saved[0].contiguous(), weight = Gradients::dense(saved[1]), rstd = Gradients::dense(saved[2]);
         const c10::DeviceGuard guard(kept.device());
         const Gradients make{kept};
         gy = gy.defined() ? gy.contiguous() : at::zeros(kept.sizes(), kept.options().dtype(type));
@@ -687,7 +722,7 @@ struct ConvBackward : torch::autograd::Function<ConvBackward> {
     };
     static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const Maybe &bias, const Maybe &state, Done *done)
     {
-        ctx->save_for_backward({x, weight, bias.value_or(at::Tensor()), state.value_or(at::Tensor()), done->offsets});
+        keep(ctx, {x, weight, bias.value_or(at::Tensor()), state.value_or(at::Tensor()), done->offsets});
         ctx->set_materialize_grads(false);
         ctx->saved_data["activation"] = (int64_t)done->activation;
         return done->state.defined() ? variable_list{done->y, done->state} : variable_list{done->y};
@@ -695,11 +730,11 @@ struct ConvBackward : torch::autograd::Function<ConvBackward> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         check_unrecorded("causal_conv");
-        const variable_list saved = ctx->get_saved_variables();
-        const at::Tensor x = Gradients::near(saved[0]), weight = Gradients::dense(saved[1]), bias = Gradients::dense(saved[2]), state = Gradients::dense(saved[3]),
-                         offsets = Gradients::dense(saved[4]);
         at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
         if (!grads[0].defined() && !gstate_out.defined()) return {{}, {}, {}, {}, {}};
+        const variable_list saved = returned(ctx, grads[0].defined() ? grads[0] : gstate_out, "causal_conv");
+        const at::Tensor x = Gradients::near(saved[0]), weight = Gradients::dense(saved[1]), bias = Gradients::dense(saved[2]), state = Gradients::dense(saved[3]),
+                         offsets = Gradients::dense(saved[4]);
         const c10::DeviceGuard guard(x.device());
         const Gradients make{x};
         const at::Tensor gy = make.tokens(grads[0]);
@@ -744,7 +779,7 @@ struct SelectiveBackward : torch::autograd::Function<SelectiveBackward> {
                                  const Maybe &D, const Maybe &z, const Maybe &bias, const Maybe &state, Done *done)
     {
         const at::Tensor none;
-        ctx->save_for_backward({x, dt, A, B, C, D.value_or(none), z.value_or(none), bias.value_or(none), state.value_or(none), done->offsets, done->saved});
+        keep(ctx, {x, dt, A, B, C, D.value_or(none), z.value_or(none), bias.value_or(none), state.value_or(none), done->offsets, done->saved});
         ctx->set_materialize_grads(false);
         ctx->saved_data["softplus"] = done->softplus;
         return done->state.defined() ? variable_list{done->y, done->state} : variable_list{done->y};
@@ -752,13 +787,13 @@ struct SelectiveBackward : torch::autograd::Function<SelectiveBackward> {
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
         check_unrecorded("selective_scan");
-        const variable_list kept = ctx->get_saved_variables();
+        at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
+        if (!grads[0].defined() && !gstate_out.defined()) return variable_list(10);
+        const variable_list kept = returned(ctx, grads[0].defined() ? grads[0] : gstate_out, "selective_scan");
         const auto near = [&](int i) { return Gradients::near(kept[i]); };
         const auto dense = [&](int i) { return Gradients::dense(kept[i]); };
         const at::Tensor x = near(0), dt = near(1), A = dense(2), B = near(3), C = near(4), D = dense(5), z = near(6), bias = dense(7), state = dense(8),
                          offsets = dense(9), saved = dense(10);
-        at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
-        if (!grads[0].defined() && !gstate_out.defined()) return variable_list(10);
         const c10::DeviceGuard guard(x.device());
         const Gradients make{x};
         const at::Tensor gy = make.tokens(grads[0]);

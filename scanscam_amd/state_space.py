@@ -213,6 +213,18 @@ def _grouped(t: torch.Tensor) -> torch.Tensor:
     return t.unsqueeze(-2)
 
 
+# What was saved for a backward pass, and what a hook on saved tensors gives back for it: in a layout of its own, but the kernels take addresses.
+def _meta(*tensors):
+    return [None if t is None else (t.shape, t.dtype) for t in tensors]
+
+
+def _check_saved(what: str, grad: torch.Tensor, tensors: dict, meta) -> None:
+    for (name, t), kept in zip(tensors.items(), meta):
+        if t is not None and (t.device != grad.device or (t.shape, t.dtype) != kept):
+            raise RuntimeError(f"{what}: {name} was saved for the backward pass as {kept[1]} {tuple(kept[0])} on {grad.device} and came back as "
+                               f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 # ---------------------------------------------------------------------------------------------------------- views for the library
 def _unit(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """The tensor itself where its last dimension is unit-stride, else a copy."""
@@ -364,6 +376,7 @@ class SelectiveScan(torch.autograd.Function):
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus, return_state):
         y, new, saved, seen = _selective_forward(x, dt, A, B, C, D, z, dt_bias, state, offsets, softplus, return_state, True)
         ctx.save_for_backward(*seen, saved)
+        ctx.meta = _meta(*seen, saved)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
         return y, new
@@ -374,6 +387,8 @@ class SelectiveScan(torch.autograd.Function):
         if gy is None and gnew is None:
             return (None,) * 12
         x, dt, A, B, C, D, z, dt_bias, state, offsets, saved = ctx.saved_tensors
+        given = {"x": x, "dt": dt, "A": A, "B": B, "C": C, "D": D, "z": z, "dt_bias": dt_bias, "state": state, "offsets": offsets, "saved states": saved}
+        _check_saved("selective_scan", gy if gy is not None else gnew, given, ctx.meta)
         # (a hook on saved tensors may lay out what it gives back in its own way)
         x, dt, B, C, z = (_near(t) for t in (x, dt, B, C, z))
         A, D, dt_bias, state, offsets, saved = (_dense(t) for t in (A, D, dt_bias, state, offsets, saved))
@@ -539,6 +554,7 @@ class CausalConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, state, offsets, activation, return_state):
         y, new, seen = _conv_forward(x, weight, bias, state, offsets, activation, return_state)
         ctx.save_for_backward(*seen)
+        ctx.meta = _meta(*seen)
         ctx.activation = activation
         ctx.set_materialize_grads(False)
         return y, new
@@ -549,6 +565,7 @@ class CausalConv(torch.autograd.Function):
         if gy is None and gnew is None:
             return (None,) * 7
         x, *others = ctx.saved_tensors
+        _check_saved("causal_conv", gy if gy is not None else gnew, dict(zip(("x", "weight", "bias", "state", "offsets"), (x, *others))), ctx.meta)
         x, (weight, bias, state, offsets) = _unit(x), (_dense(t) for t in others)  # (as above)
         L = _launching("causal_conv")
         with hip._on(x.device):
@@ -715,7 +732,9 @@ class RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         y, _, total, (rows, weight, total, rstd) = _norm_forward(x, weight, residual, eps, None, True)
-        ctx.save_for_backward(rows if residual is None else total, weight, rstd)
+        kept = rows if residual is None else total, weight, rstd
+        ctx.save_for_backward(*kept)
+        ctx.meta = _meta(*kept)
         ctx.types = x.dtype, None if residual is None else residual.dtype
         ctx.set_materialize_grads(False)
         return y, total
@@ -728,6 +747,7 @@ class RmsNorm(torch.autograd.Function):
         shape = (gy if gy is not None else gtotal).shape if gy is not None or gtotal is not None else None
         if shape is None:
             return None, None, None, None
+        _check_saved("rms_norm", gy if gy is not None else gtotal, {"rows": kept, "weight": weight, "rstd": rstd}, ctx.meta)
         L = _launching("rms_norm")
         device = kept.device
         with hip._on(device):

@@ -196,3 +196,42 @@ def test_norm_of_saved_rows_at_other_strides(gpu, monkeypatch, native, residual,
             out = f.rms_norm(*leaves)
         grads.append(torch.autograd.grad(out if residual is None else out[0], leaves, gy))
     assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("changed", ["device", "type", "shape"])
+def test_saved_tensors_that_hooks_changed_are_refused(gpu, monkeypatch, native, changed):
+    """A hook on saved tensors that gives back another device's memory, another type or fewer values: an error, for each of the saved ones."""
+    if not native:
+        monkeypatch.setattr(state_space, "_native", None)
+    give = {"device": lambda t: t.cpu(), "type": lambda t: t.double(), "shape": lambda t: t[:-1]}[changed]
+    g = torch.Generator(device=gpu).manual_seed(7)
+    r = lambda *s: torch.randn(s, generator=g, device=gpu)  # noqa: E731
+    offsets = torch.tensor([0, 30, 30, 70], dtype=torch.int32, device=gpu)
+    cases = {
+        "rms_norm": lambda p: f.rms_norm(r(4, 9, 40).requires_grad_(), p(40)),
+        "rms_norm_residual": lambda p: f.rms_norm(r(4, 9, 40).requires_grad_(), p(40), r(4, 9, 40)),
+        "causal_conv": lambda p: f.causal_conv(r(1, 70, 24).requires_grad_(), p(24, 4), p(24), state=r(3, 3, 24), offsets=offsets, return_state=True),
+        "selective_scan": lambda p: f.selective_scan(r(1, 70, 24).requires_grad_(), r(1, 70, 24), p(24, 8) - 3, r(1, 70, 2, 8), r(1, 70, 2, 8), p(24), r(1, 70, 24), p(24),
+                                                     softplus=True, state=r(3, 24, 8), offsets=offsets, return_state=True),
+    }
+    for name, call in cases.items():
+        seen = []
+
+        def pack(t):
+            seen.append(t)
+            return len(seen) - 1
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda i: seen[i].clone()):
+            call(lambda *s: r(*s).requires_grad_())
+        count = len(seen)
+        assert count >= 3
+        for k in range(count):
+            seen.clear()
+            own = []
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda i: give(seen[i]) if i == k else seen[i].clone()):
+                outs = listed(call(lambda *s: own.append(r(*s).requires_grad_()) or own[-1]))
+            for which in range(len(outs)):  # the gradient of one output or the other
+                print(name, changed, native, "saved tensor", k, tuple(seen[k].shape), "output", which, flush=True)
+                with pytest.raises(RuntimeError, match="saved for the backward pass"):
+                    torch.autograd.grad(outs[which].sum(), own, retain_graph=True)

@@ -79,7 +79,7 @@ def naive_selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, *, softpl
     if dt_bias is not None:
         d = d + _wide(dt_bias)
     if softplus:
-        d = d.clamp(min=0) + torch.log1p(torch.exp(-d.abs()))
+        d = torch.logaddexp(d, torch.zeros_like(d))  # log(e^d + e^0), with a gradient of sigmoid(d) at zero too
     outs, states = [], []
     for s, (b, start, end) in enumerate(_sequences(x, offsets)):
         h = _wide(state[s]) if state is not None else torch.zeros_like(A)

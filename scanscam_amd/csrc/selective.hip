@@ -131,6 +131,16 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
     return launch_wide(selective_fwd_kernel<ST, K, false>, grid, kFwdWaves * 64, words, stream, args);
 }
 
+// gB and gC from the sums of the blocks; of no blocks (no channels) they are zero.
+template <typename ST> hipError_t run_bc(const scanscam_selective &a, const float *bc, int64_t blocks, hipStream_t stream)
+{
+    const int64_t values = a.batch * a.T * 2 * a.N;
+    if (values == 0) return hipSuccess;
+    const bool four = a.N % 4 == 0;
+    return launch_op(four ? selective_bc_kernel<ST, 4> : selective_bc_kernel<ST, 1>, dim3((unsigned)ceil_div(values, four ? 1024 : 256), (unsigned)a.groups), dim3(256), 0,
+                     stream, GroupSum{a, bc, blocks});
+}
+
 template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream_t stream)
 {
     constexpr int K = kTokensALane;
@@ -144,12 +154,7 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     hipError_t err = hipSuccess;
     if (cut(a, plan.span)) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
     if (err == hipSuccess) err = launch_wide(selective_bwd_kernel<ST, K, false>, grid, kBwdWaves * 64, words, stream, args);
-    const int64_t values = a.batch * a.T * 2 * a.N;
-    if (err == hipSuccess && values > 0) {
-        const bool four = a.N % 4 == 0;
-        err = launch_op(four ? selective_bc_kernel<ST, 4> : selective_bc_kernel<ST, 1>, dim3((unsigned)ceil_div(values, four ? 1024 : 256), (unsigned)a.groups), dim3(256), 0,
-                        stream, GroupSum{a, bc, blocks});
-    }
+    if (err == hipSuccess) err = run_bc<ST>(a, bc, blocks, stream);
     const int64_t pitch = (a.N + 2) * a.channels;
     if (err == hipSuccess) err = column_sum({sums, units, pitch, {a.gA, a.gD, a.gdt_bias}, {a.N * a.channels, a.channels, a.channels}}, stream);
     return err;
@@ -212,7 +217,14 @@ int scanscam_selective_fwd(const scanscam_selective *a, void *stream)
 int scanscam_selective_bwd(const scanscam_selective *a, void *stream)
 {
     SCANSCAM_CHECK(check_selective(a));
-    if (a->channels == 0) return SCANSCAM_OK;
+    if (a->channels == 0) {
+        if (a->batch * a->T == 0) return SCANSCAM_OK;
+        for (const scanscam_tokens *t : {&a->gB, &a->gC}) SCANSCAM_CHECK(check_near(*t, activation_size(a->dtype)));
+        hipStream_t s = static_cast<hipStream_t>(stream);
+        return status(a->dtype == SCANSCAM_F32    ? run_bc<float>(*a, nullptr, 0, s)
+                      : a->dtype == SCANSCAM_BF16 ? run_bc<__bf16>(*a, nullptr, 0, s)
+                                                  : run_bc<_Float16>(*a, nullptr, 0, s));
+    }
     if (a->gA == nullptr) return SCANSCAM_EINVAL;
     if (a->sequences > 0) {
         if (a->batch * a->T > 0) {

@@ -140,7 +140,7 @@ def naive_rms_norm(x, weight, residual=None, *, eps=1e-6, quant=None):
         y = y.to(x.dtype)
         return y if residual is None else (y, total)
     limit = 127.0 if quant == torch.int8 else 448.0
-    most = y.abs().amax(-1)
+    most = y.abs().amax(-1) if y.shape[-1] else y.new_zeros(y.shape[:-1])
     scale = torch.where(most == 0, torch.ones_like(most), most / limit)
     q = (y / scale.unsqueeze(-1)).clamp(-limit, limit)
     q = q.round().to(quant) if quant == torch.int8 else q.to(quant)

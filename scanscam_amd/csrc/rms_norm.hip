@@ -24,6 +24,17 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(ColumnSum a)
     if (out != nullptr) out[m] = s;
 }
 
+// The scales of rows without channels.
+struct Ones {
+    float *to;
+    int64_t count;
+};
+__global__ __launch_bounds__(256) void ones_kernel(Ones a)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < a.count) a.to[i] = 1.0f;
+}
+
 }  // namespace scanscam
 
 namespace {
@@ -88,12 +99,17 @@ int scanscam_norm_fwd(const scanscam_norm *a, void *stream)
     SCANSCAM_CHECK(check_norm(a));
     const bool eight = a->out_dtype == SCANSCAM_I8 || a->out_dtype == SCANSCAM_F8;
     if (!eight && a->out_dtype != a->dtype) return SCANSCAM_EDTYPE;
-    if (a->rows == 0 || a->channels == 0) return SCANSCAM_OK;
-    if (a->y == nullptr || (eight && a->scale == nullptr)) return SCANSCAM_EINVAL;
+    if (a->rows == 0 || (a->channels == 0 && !eight)) return SCANSCAM_OK;
+    if ((a->y == nullptr && a->channels > 0) || (eight && a->scale == nullptr)) return SCANSCAM_EINVAL;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a->channels == 0) {
+        const hipError_t err = launch_op(ones_kernel, dim3((unsigned)ceil_div(a->rows, 256)), dim3(256), 0, s, Ones{a->scale, a->rows});
+        return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
+    }
     if (!eight && misaligned(a->y, (size_t)activation_size(a->dtype))) return SCANSCAM_EALIGN;
     const NormPlan plan = norm_plan(*a);
     if (ceil_div(a->rows, plan.groups) * plan.waves * plan.groups * 64 >= int64_t(1) << 32) return SCANSCAM_EINVAL;  // (threads of a launch)
-    const hipError_t err = run_norm(false, plan, (unsigned)ceil_div(a->rows, plan.groups), 0, static_cast<hipStream_t>(stream), NormArgs{*a, plan.waves, plan.shifted, nullptr});
+    const hipError_t err = run_norm(false, plan, (unsigned)ceil_div(a->rows, plan.groups), 0, s, NormArgs{*a, plan.waves, plan.shifted, nullptr});
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
 }
 

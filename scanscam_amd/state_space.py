@@ -695,7 +695,7 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if t is None:
         return None
     t = _unit(t)
-    return t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+    return t.reshape(t.shape[:-1].numel(), t.shape[-1])
 
 
 def _norm_args(x, weight, residual_dtype, eps) -> _Norm:

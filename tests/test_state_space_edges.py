@@ -3,7 +3,7 @@ The state space layer's operators at the edges of their arguments, without a GPU
 """
 import torch
 
-from scanscam_amd import baseline
+from scanscam_amd import baseline, rms_norm
 
 
 def test_softplus_has_its_gradient_at_zero():
@@ -16,3 +16,10 @@ def test_softplus_has_its_gradient_at_zero():
         (g,) = torch.autograd.grad(y[0, T, 0], dt)
         want = torch.sigmoid(dt.detach()) * (torch.arange(dt.shape[1]) <= T)[None, :, None]
         torch.testing.assert_close(g, want, rtol=1e-14, atol=0.0)
+
+
+def test_eight_bits_of_no_channels():
+    """A row without values is a row of zeros: its scale is 1."""
+    x = torch.zeros(2, 3, 0)
+    q, scale, total = rms_norm(x, torch.zeros(0), x, quant=torch.int8)
+    assert q.shape == x.shape and total.shape == x.shape and torch.equal(scale, torch.ones(2, 3))

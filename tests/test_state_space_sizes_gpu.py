@@ -21,3 +21,15 @@ def test_selections_of_no_channels_have_gradients_of_zero(gpu):
     spoil(gpu, [B.numel()] * 8)
     for g in torch.autograd.grad(y.sum(), (B, C)):
         assert torch.equal(g, torch.zeros_like(B))
+
+
+@pytest.mark.parametrize("quant", [torch.int8, torch.float8_e4m3fn])
+def test_eight_bits_of_no_channels(gpu, quant):
+    """A row without values is a row of zeros: its scale is 1."""
+    x, w = torch.empty(5, 60, 0, device=gpu, dtype=torch.bfloat16), torch.empty(0, device=gpu)
+    spoil(gpu, [300] * 8)
+    q, scale = f.rms_norm(x, w, quant=quant)
+    assert q.shape == x.shape and torch.equal(scale, torch.ones(5, 60, device=gpu))
+    spoil(gpu, [300] * 8)
+    q, scale, total = f.rms_norm(x, w, x.float(), quant=quant)
+    assert total.shape == x.shape and torch.equal(scale, torch.ones(5, 60, device=gpu))

@@ -156,14 +156,17 @@ __device__ __forceinline__ int64_t sequence_of(const void *offsets, int wide, in
 __device__ __forceinline__ int64_t clamp_(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // Sums over p < parts of in[p * pitch + m], in an order that the sizes alone decide: 16 threads a column, each over every 16th
-// part, joined in order. The parts are themselves sums of some hundreds of values, so that no sum is one long chain. The
-// columns are those of up to three outputs, one behind the other; an output may be NULL.
+// part, joined in order. More than kMostSummed parts are first summed in groups of kSummed, each into the place of its first one, so that
+// no thread adds up more than 64. (A part is itself a sum: of up to 128 tokens of a convolution; of a stretch of time of the selective scan, a value
+// a tile; of every 4096th row or more of a norm.) The columns are those of up to three outputs, one behind the other; an output may be NULL.
 struct ColumnSum {
-    const float *in;
+    float *in;
     int64_t parts, pitch;
     float *out[3];
     int64_t columns[3];
+    int64_t each, first;  // parts of a group, and the first group; each = 0: all parts, to the outputs
 };
+constexpr int64_t kMostSummed = 1024, kSummed = 256;
 
 __global__ __launch_bounds__(1024) void column_sum_kernel(ColumnSum a);
 
@@ -175,10 +178,20 @@ inline hipError_t launch_op(Kernel kernel, dim3 grid, dim3 block, size_t lds, hi
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, params, lds, stream);
 }
 
-inline hipError_t column_sum(const ColumnSum &a, hipStream_t stream)
+inline hipError_t column_sum(ColumnSum a, hipStream_t stream)
 {
-    const int64_t columns = a.columns[0] + a.columns[1] + a.columns[2];
-    return launch_op(column_sum_kernel, dim3((unsigned)ceil_div(columns, 64)), dim3(1024), 0, stream, a);
+    const unsigned grid = (unsigned)ceil_div(a.columns[0] + a.columns[1] + a.columns[2], 64);
+    for (; a.parts > kMostSummed; a.parts = ceil_div(a.parts, kSummed), a.pitch *= kSummed) {
+        const int64_t groups = ceil_div(a.parts, kSummed), most = 32768;  // (a launch has at most 65535 workgroups in its second dimension)
+        a.each = kSummed;
+        for (a.first = 0; a.first < groups; a.first += most) {
+            const int64_t now = groups - a.first < most ? groups - a.first : most;
+            const hipError_t err = launch_op(column_sum_kernel, dim3(grid, (unsigned)now), dim3(1024), 0, stream, a);
+            if (err != hipSuccess) return err;
+        }
+    }
+    a.each = a.first = 0;
+    return launch_op(column_sum_kernel, dim3(grid), dim3(1024), 0, stream, a);
 }
 
 // --- checks of arguments ---------------------------------------------------------------------------------------------------

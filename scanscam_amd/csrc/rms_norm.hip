@@ -9,15 +9,21 @@ __global__ __launch_bounds__(1024) void column_sum_kernel(ColumnSum a)
     __shared__ float sums[16][64];
     const int col = threadIdx.x & 63, slice = threadIdx.x >> 6;
     const int64_t column = (int64_t)blockIdx.x * 64 + col, all = a.columns[0] + a.columns[1] + a.columns[2];
+    const int64_t group = a.first + blockIdx.y, begin = group * a.each, parts = a.each > 0 && a.each < a.parts - begin ? a.each : a.parts - begin;
+    float *in = a.in + begin * a.pitch;
     float s = 0.0f;
     if (column < all) {
 #pragma unroll 8
-        for (int64_t p = slice; p < a.parts; p += 16) s += a.in[p * a.pitch + column];
+        for (int64_t p = slice; p < parts; p += 16) s += in[p * a.pitch + column];
     }
     sums[slice][col] = s;
     __syncthreads();
     if (slice != 0 || column >= all) return;
     for (int i = 1; i < 16; i++) s += sums[i][col];
+    if (a.each > 0) {  // (a group's columns are one workgroup's alone, and all of it has been read)
+        in[column] = s;
+        return;
+    }
     const int which = column < a.columns[0] ? 0 : column < a.columns[0] + a.columns[1] ? 1 : 2;
     const int64_t m = column - (which > 0 ? a.columns[0] : 0) - (which > 1 ? a.columns[1] : 0);
     float *out = which == 0 ? a.out[0] : which == 1 ? a.out[1] : a.out[2];

@@ -33,3 +33,20 @@ def test_eight_bits_of_no_channels(gpu, quant):
     spoil(gpu, [300] * 8)
     q, scale, total = f.rms_norm(x, w, x.float(), quant=quant)
     assert total.shape == x.shape and torch.equal(scale, torch.ones(5, 60, device=gpu))
+
+
+def test_sums_over_many_parts_are_no_long_chains(gpu):
+    """A parameter's gradient is joined from 65 536 stretches of 128 tokens here. Positive values that are all alike round the same way
+    every time; a path to the result has at most 128 additions of tokens and two levels of 64 + 16 of stretches, each of which
+    rounds by half a unit in the last place, 2^-24, of a partial sum that is no larger than the whole."""
+    batch, T, value = 64, 131072, 1.990972876548767
+    x = torch.ones(batch, T, 8, device=gpu)
+    w, b = torch.randn(8, 4, device=gpu, requires_grad=True), torch.randn(8, device=gpu, requires_grad=True)
+    gw, gb = torch.autograd.grad(f.causal_conv(x, w, b), (w, b), torch.full_like(x, value))
+    value = float(torch.tensor(value))  # (as float32 holds it)
+    bound = (128 + 2 * (64 + 16)) * 2.0 ** -24
+    for k in range(4):  # (tap k reads no token for the first 3 - k)
+        want = value * batch * (T - (3 - k))
+        assert (gw[:, k].double() - want).abs().max() <= bound * want, k
+    want = value * batch * T
+    assert (gb.double() - want).abs().max() <= bound * want

@@ -1,13 +1,16 @@
 // C ABI of the selective scan (declared in include/scanscam_ops.h): argument checks, launch shapes, launches.
 #include "selective_kernels.hpp"
 
+#include <atomic>
+
 namespace {
 
 using namespace scanscam;
 
 constexpr int kTokensALane = 8;  // K
 constexpr int kTile = Geometry<kTokensALane>::kTile;
-constexpr int64_t kMostStates = 256, kMostParts = 1024;
+constexpr int kMostStates = 256;
+constexpr int64_t kMostParts = 1024;
 
 int check_sizes(int64_t channels, int64_t groups, int64_t N, int dtype)
 {
@@ -43,12 +46,21 @@ int check_selective(const scanscam_selective *a)
     return a->z.p != nullptr ? check_near(a->z, size) : SCANSCAM_OK;
 }
 
-template <typename Kernel, typename Args>
-hipError_t launch_wide(Kernel kernel, dim3 grid, int threads, int words, hipStream_t stream, const Args &args)
+// A launch that may need more LDS than a kernel gets unasked. The limit belongs to the process: it is set once on each device, to the most
+// that any call needs (one that a call sets for itself could be lowered by another thread's before the launch).
+template <auto Kernel, typename Args> hipError_t launch_wide(dim3 grid, int threads, int words, int most_words, hipStream_t stream, const Args &args)
 {
-    const size_t bytes = (size_t)words * sizeof(float);
-    const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    return err != hipSuccess ? err : launch_op(kernel, grid, dim3((unsigned)threads), bytes, stream, args);
+    static std::atomic<uint64_t> ready{0};  // a bit a device
+    int device = 0;
+    hipError_t err = hipGetDevice(&device);
+    if (err != hipSuccess) return err;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if ((ready.load(std::memory_order_acquire) & bit) == 0) {
+        err = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, most_words * (int)sizeof(float));
+        if (err != hipSuccess) return err;
+        ready.fetch_or(bit, std::memory_order_release);
+    }
+    return launch_op(Kernel, grid, dim3((unsigned)threads), (size_t)words * sizeof(float), stream, args);
 }
 
 struct Plan {
@@ -124,11 +136,12 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
     const SelectiveArgs args{a, plan.split, 1, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
     const dim3 grid((unsigned)(a.groups * (int64_t)args.blocks * all_units(a, plan.span)));
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
+    constexpr int most = ForwardLds<K>::words(kFwdWaves * kRows, kMostStates);
     if (cut(a, plan.span)) {
-        const hipError_t err = launch_wide(selective_fwd_kernel<ST, K, true>, grid, kFwdWaves * 64, words, stream, args);
+        const hipError_t err = launch_wide<selective_fwd_kernel<ST, K, true>>(grid, kFwdWaves * 64, words, most, stream, args);
         if (err != hipSuccess) return err;
     }
-    return launch_wide(selective_fwd_kernel<ST, K, false>, grid, kFwdWaves * 64, words, stream, args);
+    return launch_wide<selective_fwd_kernel<ST, K, false>>(grid, kFwdWaves * 64, words, most, stream, args);
 }
 
 // gB and gC from the sums of the blocks; of no blocks (no channels) they are zero.
@@ -151,9 +164,10 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     const SelectiveArgs args{a, 1, sets, (uint32_t)blocks, each_of(a, plan.span), plan.span, ends, bc, sums};
     const dim3 grid((unsigned)(a.groups * blocks * units));
     const int words = BackwardLds<K>::words((int)a.N, sets);
+    constexpr int one = BackwardLds<K>::words(kMostStates, 1), two = BackwardLds<K>::words(kStateBlock, kBwdMostSets), most = one > two ? one : two;
     hipError_t err = hipSuccess;
-    if (cut(a, plan.span)) err = launch_wide(selective_bwd_kernel<ST, K, true>, grid, kBwdWaves * 64, words, stream, args);
-    if (err == hipSuccess) err = launch_wide(selective_bwd_kernel<ST, K, false>, grid, kBwdWaves * 64, words, stream, args);
+    if (cut(a, plan.span)) err = launch_wide<selective_bwd_kernel<ST, K, true>>(grid, kBwdWaves * 64, words, most, stream, args);
+    if (err == hipSuccess) err = launch_wide<selective_bwd_kernel<ST, K, false>>(grid, kBwdWaves * 64, words, most, stream, args);
     if (err == hipSuccess) err = run_bc<ST>(a, bc, blocks, stream);
     const int64_t pitch = (a.N + 2) * a.channels;
     if (err == hipSuccess) err = column_sum({sums, units, pitch, {a.gA, a.gD, a.gdt_bias}, {a.N * a.channels, a.channels, a.channels}}, stream);

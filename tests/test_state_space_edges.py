@@ -1,6 +1,12 @@
 """
 The state space layer's operators at the edges of their arguments, without a GPU.
 """
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
 import torch
 
 from scanscam_amd import baseline, rms_norm
@@ -23,3 +29,75 @@ def test_eight_bits_of_no_channels():
     x = torch.zeros(2, 3, 0)
     q, scale, total = rms_norm(x, torch.zeros(0), x, quant=torch.int8)
     assert q.shape == x.shape and total.shape == x.shape and torch.equal(scale, torch.ones(2, 3))
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+# Stands in for the runtime's launch: notes what is asked for, launches nothing.
+RECORDER = """
+#include <stdint.h>
+#include <stdio.h>
+#include <stddef.h>
+typedef struct { uint32_t x, y, z; } dim3;
+int hipGetDevice(int *device) { *device = 0; return 0; }
+int hipFuncSetAttribute(const void *kernel, int what, int value) { printf("limit %p %d\\n", kernel, value); fflush(stdout); return 0; }
+int hipLaunchKernel(const void *kernel, dim3 grid, dim3 block, void **args, size_t lds, void *stream)
+{
+    printf("launch %p %u %u %u %u %u %u %zu\\n", kernel, grid.x, grid.y, grid.z, block.x, block.y, block.z, lds);
+    fflush(stdout);
+    return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def recorded(tmp_path_factory):
+    """Runs statements in a process where launches of the library are only noted (the pointers that they get are never used): lines of
+    [what, kernel, numbers ...] and of what the statements print."""
+    folder = tmp_path_factory.mktemp("recorder")
+    (folder / "recorder.c").write_text(RECORDER)
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(folder / "recorder.so"), str(folder / "recorder.c")], check=True)
+    head = f"""
+        import ctypes
+        ctypes.CDLL({str(folder / "recorder.so")!r}, mode=ctypes.RTLD_GLOBAL)
+        from scanscam_amd import hip, state_space as s
+        L, fake = s._lib(), 0x100000
+        T = lambda token=1 << 12, group=0: s._Tokens(fake, token, token, group)
+        P = s._Param(fake, 0)
+        def scan(**k):
+            a = s._Selective(batch=1, T=4, sequences=1, channels=64, groups=1, N=16, dtype=1, saved=fake, gA=fake, workspace=fake, workspace_bytes=1 << 60, A=P)
+            for n in ("x", "dt", "B", "C", "y", "gy", "gx", "gdt", "gB", "gC"):
+                setattr(a, n, T())
+            for n, v in k.items():
+                setattr(a, n, v)
+            return a
+    """
+
+    def run(statements):
+        code = textwrap.dedent(head) + textwrap.dedent(statements)
+        out = subprocess.run([sys.executable, "-c", code], check=True, capture_output=True, text=True, cwd=ROOT, env={**os.environ, "PYTHONPATH": ROOT})
+        return [line.split() for line in out.stdout.splitlines()]
+
+    return run
+
+
+def test_the_limit_of_shared_memory_does_not_depend_on_the_call(recorded):
+    """It belongs to the process, so a call's own would be another thread's too. Once a kernel, and enough for every launch."""
+    lines = recorded("""
+        for N in (16, 256, 1, 40, 16):
+            assert L.scanscam_selective_fwd(scan(N=N), None) == 0 and L.scanscam_selective_bwd(scan(N=N), None) == 0
+            assert L.scanscam_selective_bwd(scan(N=N, T=5000, parts=4), None) == 0
+            assert L.scanscam_selective_fwd(scan(N=N, T=5000, parts=4), None) == 0
+            assert L.scanscam_selective_bwd(scan(N=min(N, 16), batch=600, sequences=600), None) == 0
+    """)
+    limits = {}
+    launches = 0
+    for what, kernel, *numbers in lines:
+        if what == "limit":
+            assert kernel not in limits
+            limits[kernel] = int(numbers[0])
+        else:
+            launches += 1
+            lds = int(numbers[6])
+            assert lds <= 160 * 1024 and (lds <= 64 * 1024 or lds <= limits[kernel])
+    assert len(limits) == 4 and launches > 30

@@ -133,7 +133,7 @@ typedef struct scanscam_conv {
 
 int scanscam_conv_fwd(const scanscam_conv *args, void *stream);
 int scanscam_conv_bwd(const scanscam_conv *args, void *stream);
-size_t scanscam_conv_workspace_bytes(const scanscam_conv *args);
+size_t scanscam_conv_workspace_bytes(const scanscam_conv *args); /* only the sizes and dtype are looked at */
 
 /* One token of each of `rows` sequences; `state` is [slots, K - 1, channels], slots as in the selective scan's step. */
 typedef struct scanscam_conv_step {
@@ -177,7 +177,7 @@ typedef struct scanscam_norm {
 
 int scanscam_norm_fwd(const scanscam_norm *args, void *stream);
 int scanscam_norm_bwd(const scanscam_norm *args, void *stream);
-size_t scanscam_norm_workspace_bytes(const scanscam_norm *args);
+size_t scanscam_norm_workspace_bytes(const scanscam_norm *args); /* only the sizes are looked at */
 
 #ifdef __cplusplus
 }

@@ -65,10 +65,11 @@ NormPlan norm_plan(const scanscam_norm &a)
 
 constexpr int64_t kNormMostChannels = 32768;
 
+constexpr int64_t kNormMostParts = 1024;
 int64_t norm_bwd_workgroups(const scanscam_norm &a, const NormPlan &p)
 {
     const int64_t all = ceil_div(a.rows, p.groups);
-    return all < 1024 ? all : 1024;
+    return all < kNormMostParts ? all : kNormMostParts;
 }
 
 int check_norm(const scanscam_norm *a)
@@ -122,7 +123,8 @@ int scanscam_norm_fwd(const scanscam_norm *a, void *stream)
 size_t scanscam_norm_workspace_bytes(const scanscam_norm *a)
 {
     if (a == nullptr || a->rows <= 0 || a->channels <= 0 || a->channels > kNormMostChannels) return 0;
-    return (size_t)(norm_bwd_workgroups(*a, norm_plan(*a)) * a->channels) * sizeof(float);
+    // (enough for every number of rows a workgroup, which depends on the residual: it may be asked for before the pointers are there)
+    return (size_t)((a->rows < kNormMostParts ? a->rows : kNormMostParts) * a->channels) * sizeof(float);
 }
 
 int scanscam_norm_bwd(const scanscam_norm *a, void *stream)

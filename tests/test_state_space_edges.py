@@ -101,3 +101,19 @@ def test_the_limit_of_shared_memory_does_not_depend_on_the_call(recorded):
             lds = int(numbers[6])
             assert lds <= 160 * 1024 and (lds <= 64 * 1024 or lds <= limits[kernel])
     assert len(limits) == 4 and launches > 30
+
+
+@pytest.mark.parametrize("rows,channels,dtype,residual", [(4000, 3000, 1, 0), (4000, 3000, 1, 1), (5, 3000, 1, 0), (1025, 2049, 0, 1), (9999, 40, 2, 0), (4096, 9000, 1, 0), (7, 1, 0, 0)])
+def test_the_norm_s_workspace_follows_from_its_sizes(recorded, rows, channels, dtype, residual):
+    """Asked for before the pointers are there, it is enough for the call that has them."""
+    lines = recorded(f"""
+        a = s._Norm(rows={rows}, channels={channels}, x_stride={channels}, dtype={dtype}, residual_dtype={residual})
+        n = L.scanscam_norm_workspace_bytes(a)
+        for pointer in ("x", "residual", "sum", "gy", "gx", "gresidual", "gweight", "rstd", "workspace"):
+            setattr(a, pointer, fake)
+        a.weight, a.workspace_bytes = P, n
+        print("rc", L.scanscam_norm_bwd(a, None), n == L.scanscam_norm_workspace_bytes(a))
+        a.workspace_bytes = n - 4
+        print("rc", L.scanscam_norm_bwd(a, None))
+    """)
+    assert [line for line in lines if line[0] == "rc"] == [["rc", "0", "True"], ["rc", "5"]]

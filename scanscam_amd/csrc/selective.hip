@@ -31,9 +31,7 @@ int check_selective(const scanscam_selective *a)
     SCANSCAM_CHECK(check_sizes(a->channels, a->groups, a->N, a->dtype));
     if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->sequences >= kMostTokens || a->parts < 0 || a->parts > kMostParts) return SCANSCAM_EINVAL;
     if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
-    // (a launch has fewer than 2^32 threads)
-    if ((a->sequences * (a->parts > 0 ? a->parts : 1) + 512) * (a->groups + a->channels / kBwdChannels) >= int64_t(1) << 23) return SCANSCAM_EINVAL;
-    if (a->batch > 0 && a->T >= (int64_t(1) << 31) / a->N / a->batch) return SCANSCAM_EINVAL;
+    if (a->batch > 0 && a->T > (kMostTokens - 1) / a->batch) return SCANSCAM_EINVAL;
     if (a->channels == 0 || a->sequences == 0) return SCANSCAM_OK;
     SCANSCAM_CHECK(check_param(a->A, true));
     SCANSCAM_CHECK(check_param(a->D, false));
@@ -61,6 +59,18 @@ template <auto Kernel, typename Args> hipError_t launch_wide(dim3 grid, int thre
         ready.fetch_or(bit, std::memory_order_release);
     }
     return launch_op(Kernel, grid, dim3((unsigned)threads), (size_t)words * sizeof(float), stream, args);
+}
+
+// A launch has fewer than 2^32 threads: more parts than that are several launches.
+template <auto Kernel> hipError_t launch_units(SelectiveArgs args, int64_t units, int threads, int words, int most_words, hipStream_t stream)
+{
+    const int64_t blocks = args.a.groups * args.blocks, most = ((int64_t(1) << 32) / threads - 1) / blocks;
+    hipError_t err = hipSuccess;
+    for (int64_t first = 0; first < units && err == hipSuccess; first += most) {
+        args.unit0 = (uint32_t)first;
+        err = launch_wide<Kernel>(dim3((unsigned)(blocks * (units - first < most ? units - first : most))), threads, words, most_words, stream, args);
+    }
+    return err;
 }
 
 struct Plan {
@@ -133,25 +143,33 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
 {
     constexpr int K = kTokensALane;
     const Plan plan = forward_plan(a);
-    const SelectiveArgs args{a, plan.split, 1, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
-    const dim3 grid((unsigned)(a.groups * (int64_t)args.blocks * all_units(a, plan.span)));
+    const SelectiveArgs args{a, plan.split, 1, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), 0, plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
+    const int64_t units = all_units(a, plan.span);
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
     constexpr int most = ForwardLds<K>::words(kFwdWaves * kRows, kMostStates);
     if (cut(a, plan.span)) {
-        const hipError_t err = launch_wide<selective_fwd_kernel<ST, K, true>>(grid, kFwdWaves * 64, words, most, stream, args);
+        const hipError_t err = launch_units<selective_fwd_kernel<ST, K, true>>(args, units, kFwdWaves * 64, words, most, stream);
         if (err != hipSuccess) return err;
     }
-    return launch_wide<selective_fwd_kernel<ST, K, false>>(grid, kFwdWaves * 64, words, most, stream, args);
+    return launch_units<selective_fwd_kernel<ST, K, false>>(args, units, kFwdWaves * 64, words, most, stream);
 }
 
 // gB and gC from the sums of the blocks; of no blocks (no channels) they are zero.
 template <typename ST> hipError_t run_bc(const scanscam_selective &a, const float *bc, int64_t blocks, hipStream_t stream)
 {
-    const int64_t values = a.batch * a.T * 2 * a.N;
-    if (values == 0) return hipSuccess;
+    // (a launch's values are numbered with 32 bits, its groups are its grid's second dimension)
+    const int64_t tokens = a.batch * a.T, wide = 2 * a.N, most = (int64_t(1) << 31) / wide, most_groups = 32768;
     const bool four = a.N % 4 == 0;
-    return launch_op(four ? selective_bc_kernel<ST, 4> : selective_bc_kernel<ST, 1>, dim3((unsigned)ceil_div(values, four ? 1024 : 256), (unsigned)a.groups), dim3(256), 0,
-                     stream, GroupSum{a, bc, blocks});
+    hipError_t err = hipSuccess;
+    for (int64_t token = 0; token < tokens; token += most) {
+        const int64_t now = tokens - token < most ? tokens - token : most;
+        for (int64_t group = 0; group < a.groups && err == hipSuccess; group += most_groups) {
+            const dim3 grid((unsigned)ceil_div(now * wide, four ? 1024 : 256), (unsigned)(a.groups - group < most_groups ? a.groups - group : most_groups));
+            err = launch_op(four ? selective_bc_kernel<ST, 4> : selective_bc_kernel<ST, 1>, grid, dim3(256), 0, stream,
+                            GroupSum{a, bc, blocks, (uint32_t)token, (uint32_t)now, (uint32_t)group});
+        }
+    }
+    return err;
 }
 
 template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream_t stream)
@@ -161,13 +179,12 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     const int sets = backward_sets(a);
     const int64_t blocks = backward_blocks(a), units = all_units(a, plan.span);
     float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.span), *sums = bc + bc_words(a);
-    const SelectiveArgs args{a, 1, sets, (uint32_t)blocks, each_of(a, plan.span), plan.span, ends, bc, sums};
-    const dim3 grid((unsigned)(a.groups * blocks * units));
+    const SelectiveArgs args{a, 1, sets, (uint32_t)blocks, each_of(a, plan.span), 0, plan.span, ends, bc, sums};
     const int words = BackwardLds<K>::words((int)a.N, sets);
     constexpr int one = BackwardLds<K>::words(kMostStates, 1), two = BackwardLds<K>::words(kStateBlock, kBwdMostSets), most = one > two ? one : two;
     hipError_t err = hipSuccess;
-    if (cut(a, plan.span)) err = launch_wide<selective_bwd_kernel<ST, K, true>>(grid, kBwdWaves * 64, words, most, stream, args);
-    if (err == hipSuccess) err = launch_wide<selective_bwd_kernel<ST, K, false>>(grid, kBwdWaves * 64, words, most, stream, args);
+    if (cut(a, plan.span)) err = launch_units<selective_bwd_kernel<ST, K, true>>(args, units, kBwdWaves * 64, words, most, stream);
+    if (err == hipSuccess) err = launch_units<selective_bwd_kernel<ST, K, false>>(args, units, kBwdWaves * 64, words, most, stream);
     if (err == hipSuccess) err = run_bc<ST>(a, bc, blocks, stream);
     const int64_t pitch = (a.N + 2) * a.channels;
     if (err == hipSuccess) err = column_sum({sums, units, pitch, {a.gA, a.gD, a.gdt_bias}, {a.N * a.channels, a.channels, a.channels}}, stream);

@@ -345,6 +345,7 @@ struct SelectiveArgs {
     int sets;         // backwards: sets of 16 channels that a workgroup takes
     uint32_t blocks;  // of channels, in a group
     uint32_t each;    // parts of a sequence where all are of one length
+    uint32_t unit0;   // the first part of this launch's
     int64_t span;     // tokens of a part of a sequence
     float *ends;      // [parts of all sequences][N + 1][channels]: the states that a part alone ends with (backwards: starts with), its sum of d
     float *bc;        // backwards: [blocks of all groups][tokens][2][N], sums of gB and gC over a workgroup's channels
@@ -359,13 +360,13 @@ struct SelectiveArgs {
 struct Work {
     uint32_t block, unit;  // block of channels among all groups'; part of a sequence
 };
-__device__ __forceinline__ Work work_of(uint32_t blocks)
+__device__ __forceinline__ Work work_of(uint32_t blocks, uint32_t unit0)
 {
     constexpr uint32_t kDies = 8, near = 8, round = near * kDies;
     uint32_t i = blockIdx.x;
     if (i < gridDim.x / round * round) i = i / round * round + i % kDies * near + i % round / kDies;
     const uint32_t unit = i / blocks;
-    return {i - unit * blocks, unit};
+    return {i - unit * blocks, unit0 + unit};
 }
 
 // The state before a part (the gradient behind it): that of the sequence's end, taken through the parts between. A part alone
@@ -437,7 +438,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     Carry *lh = reinterpret_cast<Carry *>(lskip + channels), *nowhere = lh + channels * N;  // [N][channels]
 
     const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
-    const Work w = work_of((uint32_t)a.groups * args.blocks);
+    const Work w = work_of((uint32_t)a.groups * args.blocks, args.unit0);
     const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * channels;  // c0: inside the group
     const int here = (int)clamp_(per_group - c0, 0, channels);
     const int64_t first = group * per_group + c0;  // first channel
@@ -683,7 +684,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     float *nowhere = lsum + 2 * kBwdWaves * wide;
 
     const int64_t per_group = a.groups > 1 ? (uint32_t)a.channels / (uint32_t)a.groups : a.channels;
-    const Work w = work_of((uint32_t)a.groups * args.blocks);
+    const Work w = work_of((uint32_t)a.groups * args.blocks, args.unit0);
     const uint32_t group = a.groups > 1 ? w.block / args.blocks : 0, c0 = (w.block - group * args.blocks) * wide;
     const int here = (int)clamp_(per_group - c0, 0, wide), sets = (here + channels - 1) / channels;
     const int64_t first = group * per_group + c0;
@@ -1046,6 +1047,7 @@ struct GroupSum {
     scanscam_selective a;
     const float *bc;
     int64_t blocks;
+    uint32_t token0, tokens, group0;  // of this launch
 };
 // VEC: neighbouring states of a lane, 4 where their number allows it.
 template <typename ST, int VEC>
@@ -1053,11 +1055,12 @@ __global__ __launch_bounds__(256) void selective_bc_kernel(GroupSum args)
 {
     constexpr int kTogether = 8;
     const scanscam_selective &a = args.a;
-    const uint32_t wide = 2 * (uint32_t)a.N, tokens = (uint32_t)(a.batch * a.T), i = (blockIdx.x * 256 + threadIdx.x) * VEC, group = blockIdx.y;
-    if (i >= tokens * wide) return;
+    const uint32_t wide = 2 * (uint32_t)a.N, i = (blockIdx.x * 256 + threadIdx.x) * VEC;
+    const int64_t group = args.group0 + blockIdx.y;
+    if (i >= args.tokens * wide) return;
     typedef float vec_t __attribute__((ext_vector_type(VEC), aligned(4)));
-    const int64_t pitch = (int64_t)tokens * wide;
-    const float *from = args.bc + group * args.blocks * pitch + i;
+    const int64_t pitch = a.batch * a.T * wide;
+    const float *from = args.bc + group * args.blocks * pitch + (int64_t)args.token0 * wide + i;
     vec_t sum = 0.0f;
     int64_t b = 0;
     for (; b + kTogether <= args.blocks; b += kTogether, from += kTogether * pitch) {
@@ -1068,8 +1071,8 @@ __global__ __launch_bounds__(256) void selective_bc_kernel(GroupSum args)
         for (int j = 0; j < kTogether; j++) sum += v[j];
     }
     for (; b < args.blocks; b++, from += pitch) sum += *reinterpret_cast<const vec_t *>(from);
-    const uint32_t token = i / wide, batch = token / (uint32_t)a.T;
-    uint32_t n = i - token * wide;
+    const uint32_t place = i / wide, token = args.token0 + place, batch = token / (uint32_t)a.T;
+    uint32_t n = i - place * wide;
     const scanscam_tokens &to = n < a.N ? a.gB : a.gC;
     if (n >= a.N) n -= (uint32_t)a.N;
     float f[VEC];

@@ -117,3 +117,31 @@ def test_the_norm_s_workspace_follows_from_its_sizes(recorded, rows, channels, d
         print("rc", L.scanscam_norm_bwd(a, None))
     """)
     assert [line for line in lines if line[0] == "rc"] == [["rc", "0", "True"], ["rc", "5"]]
+
+
+def launches(lines):
+    """(workgroups, threads of a workgroup) of each launch; every dimension of the grid has fewer than 2^32 threads, all but the first up to 65 535 workgroups."""
+    out = []
+    for what, _, *n in lines:
+        if what == "launch":
+            x, y, z, bx, by, bz, _ = map(int, n)
+            assert x * bx < 1 << 32 and y <= 65535 and z == 1 and x * y > 0
+            out.append((x * y, bx * by * bz))
+    return out
+
+
+def test_selective_scans_of_many_parts_are_several_launches(recorded):
+    """Workgroups: of 32 channels (16, or two sets of them, backwards) for each sequence; none is left out and none comes twice."""
+    for batch, channels in ((65536, 2048), (1 << 23, 64), (1 << 20, 65536)):
+        lines = recorded(f"assert L.scanscam_selective_fwd(scan(batch={batch}, sequences={batch}, T=1, channels={channels}, N=4), None) == 0")
+        assert sum(n for n, threads in launches(lines)) == batch * channels // 32
+        lines = recorded(f"assert L.scanscam_selective_bwd(scan(batch={batch}, sequences={batch}, T=1, channels={channels}, N=4), None) == 0")
+        assert sum(n for n, threads in launches(lines) if threads == 256) == batch * channels // 32 + batch * 8 // 1024 + (batch * 8 % 1024 > 0)
+    # gradients of B and C: tokens x 2 N values, four a lane
+    lines = recorded("assert L.scanscam_selective_bwd(scan(batch=1 << 20, sequences=1 << 20, T=100, channels=4, N=256), None) == 0")
+    assert sum(n for n, threads in launches(lines)[:-1] if threads == 256) == (1 << 20) + (100 << 20) * 512 // 1024
+    # packed: the numbers of parts that there may be
+    lines = recorded("assert L.scanscam_selective_fwd(scan(batch=1, sequences=3000000, T=4000000, channels=2048, offsets=fake), None) == 0")
+    assert sum(n for n, _ in launches(lines)) == 3000000 * 64
+    assert recorded("print(L.scanscam_selective_fwd(scan(batch=1 << 20, sequences=1 << 20, T=1 << 11), None))") == [["1"]]  # 2^31 tokens
+    assert recorded("print(L.scanscam_selective_fwd(scan(batch=1 << 25, sequences=1 << 25, T=0), None))")[-1] == ["0"]

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import scanscam_amd as f
+from scanscam_amd import baseline
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,74 @@ def test_sums_over_many_parts_are_no_long_chains(gpu):
         assert (gw[:, k].double() - want).abs().max() <= bound * want, k
     want = value * batch * T
     assert (gb.double() - want).abs().max() <= bound * want
+
+
+def test_selective_scan_of_many_sequences(gpu):
+    """65 536 sequences of one token: with h[-1] = 0, y = x (d (B . C) + D), and gradients that follow from that. Roundings of 2^-24: some
+    64 (softplus, products, sums over 16 states), for the gradients of B and C those of sums over channels (32 of a block, 64 blocks), for D's
+    those of sums over 65 536 parts in two levels, all of the sum of the terms' sizes; and one to bfloat16."""
+    S, D, N = 65536, 2048, 16
+    g = torch.Generator(device=gpu).manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g, device=gpu)  # noqa: E731
+    x, dt, gy = (r(S, 1, D).to(torch.bfloat16) for _ in range(3))
+    B, C = (r(S, 1, N).to(torch.bfloat16) for _ in range(2))
+    A, skip = -r(D, N).exp(), r(D)
+    leaves = [t.requires_grad_() for t in (x, dt, A, B, C, skip)]
+    y = f.selective_scan(*leaves, softplus=True)
+    gx, gdt, gA, gB, gC, gskip = torch.autograd.grad(y, leaves, gy)
+    assert torch.equal(gA, torch.zeros_like(A))
+    some = torch.tensor([0, 1, 7, 4095, 32767, 65007, 65024, 65025, 65535], device=gpu)  # (a launch's last parts and the next one's first among them)
+    with torch.no_grad():
+        w = {k: t[some, 0].double() for k, t in dict(x=x, dt=dt, gy=gy, B=B, C=C).items()}
+        d, mixed = torch.nn.functional.softplus(w["dt"], threshold=60.0), (w["B"] * w["C"]).sum(-1, keepdim=True)
+        terms = w["gy"] * d * w["x"]
+        along, whole = terms.sum(-1, keepdim=True), terms.abs().sum(-1, keepdim=True)
+        want = {"y": w["x"] * (d * mixed + skip.double()), "gx": w["gy"] * (d * mixed + skip.double()),
+                "gdt": w["gy"] * w["x"] * mixed * torch.sigmoid(w["dt"]), "gB": along * w["C"], "gC": along * w["B"]}
+        for name, got in (("y", y), ("gx", gx), ("gdt", gdt), ("gB", gB), ("gC", gC)):
+            got, ref = got[some, 0].double(), want[name]
+            size = whole * {"gB": w["C"], "gC": w["B"]}[name].abs() if name in ("gB", "gC") else ref.abs().max()
+            assert ((got - ref).abs() <= 2.0 ** -8 * 1.01 * ref.abs() + (64 + D // 16) * 2.0 ** -24 * size).all(), name
+        ref, size = torch.zeros(D, dtype=torch.float64, device=gpu), torch.zeros(D, dtype=torch.float64, device=gpu)
+        for a, b in zip(x.split(8192), gy.split(8192)):
+            part = a[:, 0].double() * b[:, 0].double()
+            ref, size = ref + part.sum(0), size + part.abs().sum(0)
+        assert ((gskip.double() - ref).abs() <= (16 + 2 * 80) * 2.0 ** -24 * size).all()
+
+
+def test_selective_scan_of_many_tokens_and_states(gpu):
+    """131 073 sequences of 64 tokens with 256 states: 2^31 values of B and C and more, numbered with more than 32 bits backwards."""
+    S, T, D, N = 131073, 64, 4, 256
+    g = torch.Generator(device=gpu).manual_seed(2)
+    r = lambda *s: torch.randn(s, generator=g, device=gpu)  # noqa: E731
+    x, dt, gy = r(S, T, D).to(torch.bfloat16), (r(S, T, D) - 2).to(torch.bfloat16), r(S, T, D).to(torch.bfloat16)
+    B, C = (torch.empty(S, T, N, dtype=torch.bfloat16, device=gpu).normal_(generator=g) for _ in range(2))
+    A = -r(D, N).exp()
+    leaves = [t.requires_grad_() for t in (x, dt, A, B, C)]
+    y = f.selective_scan(*leaves, softplus=True)
+    gx, gdt, gA, gB, gC = torch.autograd.grad(y, leaves, gy)
+    some = [0, 65535, 65536, 131072]
+    ref = [t.detach()[some].cpu().double().requires_grad_() if t is not A else A.detach().cpu().double().requires_grad_() for t in leaves]
+    want = baseline.naive_selective_scan(*ref, softplus=True)
+    wants = torch.autograd.grad(want, [ref[i] for i in (0, 1, 3, 4)], gy[some].cpu().double())
+    for name, got, w in (("y", y, want), ("gx", gx, wants[0]), ("gdt", gdt, wants[1]), ("gB", gB, wants[2]), ("gC", gC, wants[3])):
+        got, w = got.detach()[some].cpu().double(), w.detach()
+        bound = 2.0 ** -8 * 1.01 * w.abs() + (64 + 2 * T) * 2.0 ** -24 * w.abs().max()
+        assert ((got - w).abs() <= bound).all(), name
+    assert torch.isfinite(gA).all()
+
+
+def test_selective_scan_of_many_groups(gpu):
+    """A group a channel, more of them than a grid's second dimension holds workgroups."""
+    D = 70000
+    g = torch.Generator(device=gpu).manual_seed(3)
+    x, dt, B, C, gy = (torch.randn(1, 3, D, generator=g, device=gpu) for _ in range(5))
+    A = -torch.randn(D, 1, generator=g, device=gpu).exp()
+    leaves = [t.requires_grad_() for t in (x, dt, A, B[..., None], C[..., None])]
+    y = f.selective_scan(*leaves, softplus=True)
+    grads = torch.autograd.grad(y, leaves, gy)
+    ref = [t.detach().cpu().double().requires_grad_() for t in leaves]
+    want = baseline.naive_selective_scan(*ref, softplus=True)
+    for got, w in zip([y, *grads], [want, *torch.autograd.grad(want, ref, gy.cpu().double())]):
+        got, w = got.detach().cpu().double(), w.detach()
+        assert ((got - w).abs() <= 2.0 ** -24 * w.abs() + (64 + 2 * 3) * 2.0 ** -24 * w.abs().max()).all()

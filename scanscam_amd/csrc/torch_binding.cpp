@@ -503,13 +503,14 @@ struct Arguments {
     {
         scanscam_tokens k{};
         if (!ok || !t.defined()) return k;
-        if (t.scalar_type() != first.scalar_type() || (t.size(-1) != 1 && t.stride(-1) != 1) || t.stride(lead - 1) >= SCANSCAM_MOST_TOKEN_STRIDE) {
+        const int64_t token = t.size(lead - 1) > 1 ? t.stride(lead - 1) : 0;  // (a single token's distance to the next may be anything)
+        if (t.scalar_type() != first.scalar_type() || (t.size(-1) != 1 && t.stride(-1) != 1) || token >= SCANSCAM_MOST_TOKEN_STRIDE) {
             ok = false;
             return k;
         }
         k.p = t.data_ptr();
         k.batch = lead == 2 ? t.stride(0) : 0;
-        k.token = t.stride(lead - 1);
+        k.token = token;
         k.group = t.dim() > lead + 1 ? t.stride(lead) : 0;
         return k;
     }
@@ -611,13 +612,13 @@ struct Gradients {
     // What was saved, as the kernels take it: a hook on saved tensors may lay out what it gives back in its own way.
     static at::Tensor near(const at::Tensor &t)
     {
-        return !t.defined() || ((t.size(-1) == 1 || t.stride(-1) == 1) && t.stride(1) < SCANSCAM_MOST_TOKEN_STRIDE) ? t : t.contiguous();
+        return !t.defined() || ((t.size(-1) == 1 || t.stride(-1) == 1) && (t.size(1) <= 1 || t.stride(1) < SCANSCAM_MOST_TOKEN_STRIDE)) ? t : t.contiguous();
     }
     static at::Tensor dense(const at::Tensor &t) { return t.defined() ? t.contiguous() : t; }
     static scanscam_tokens view(const at::Tensor &t)
     {
         if (!t.defined()) return {};
-        return {t.data_ptr(), t.stride(0), t.stride(1), t.dim() > 3 ? t.stride(2) : 0};
+        return {t.data_ptr(), t.stride(0), t.size(1) > 1 ? t.stride(1) : 0, t.dim() > 3 ? t.stride(2) : 0};
     }
     static scanscam_param parameter(const at::Tensor &t) { return t.defined() ? scanscam_param{t.data_ptr(), dtype_code(t.scalar_type()), 0} : scanscam_param{}; }
     template <typename T = void> static T *at(const at::Tensor &t) { return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr; }
@@ -1008,6 +1009,7 @@ template <typename Args> bool selective_arguments(Arguments &in, int at, int lea
     a.N = A.size(1);
     a.groups = B.dim() == lead + 2 ? B.size(lead) : 1;
     if (a.N < 1 || a.N > kMostStates || a.groups < 1 || a.channels % a.groups != 0 || B.size(-1) != a.N) return false;
+    if (a.groups * a.N >= SCANSCAM_MOST_TOKEN_STRIDE) return false;  // (gradients of B and C need a layout of their own)
     for (int d = 0; d < lead; d++)
         if (B.size(d) != x.size(d)) return false;
     in.shape(dt, x.sizes());

@@ -234,9 +234,23 @@ def _unit(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 def _near(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """The same for the selective scan of whole sequences, whose kernels take tokens at most so far apart."""
+    """The same for the selective scan of whole sequences, whose kernels take tokens at most so far apart; B and C of very many groups
+    come group by group then."""
     t = _unit(t)
-    return t if t is None or t.stride(1) < _MOST_TOKEN_STRIDE else t.contiguous()
+    if t is None or t.shape[1] <= 1 or t.stride(1) < _MOST_TOKEN_STRIDE:
+        return t
+    t = t.contiguous()
+    return t if t.stride(1) < _MOST_TOKEN_STRIDE else t.permute(2, 0, 1, 3).contiguous().permute(1, 2, 0, 3)
+
+
+def _empty_near(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """An output of t's shape that the selective scan takes."""
+    if t is None:
+        return None
+    if t.dim() < 4 or t.shape[2] * t.shape[3] < _MOST_TOKEN_STRIDE:
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    batch, T, groups, N = t.shape
+    return torch.empty((groups, batch, T, N), dtype=t.dtype, device=t.device).permute(1, 2, 0, 3)
 
 
 def _tokens(t: Optional[torch.Tensor], lead: int = 2) -> _Tokens:
@@ -245,6 +259,8 @@ def _tokens(t: Optional[torch.Tensor], lead: int = 2) -> _Tokens:
         return _Tokens()
     st = t.stride()
     batch, token = (st[0], st[1]) if lead == 2 else (0, st[0])
+    if t.shape[lead - 1] == 1:
+        token = 0  # (a single token's distance to the next may be anything)
     return _Tokens(t.data_ptr(), batch, token, st[lead] if t.dim() > lead + 1 else 0)
 
 
@@ -399,7 +415,7 @@ class SelectiveScan(torch.autograd.Function):
             gnew = _dense(gnew)
             a = _selective_args(*seen, ctx.softplus)
             new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=x.device)  # noqa: E731
-            gx, gdt, gB, gC, gz = (new(t) for t in (x, dt, B, C, z))
+            gx, gdt, gB, gC, gz = (_empty_near(t) for t in (x, dt, B, C, z))
             gA, gD, gbias = (new(t, torch.float32) for t in (A, D, dt_bias))
             gstate = new(state) if ctx.needs_input_grad[8] else None
             a.gy, a.gx, a.gdt, a.gB, a.gC, a.gz = (_tokens(t) for t in (gy, gx, gdt, gB, gC, gz))

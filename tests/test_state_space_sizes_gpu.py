@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import scanscam_amd as f
-from scanscam_amd import baseline
+from scanscam_amd import baseline, state_space
 
 pytestmark = pytest.mark.gpu
 
@@ -122,3 +122,40 @@ def test_selective_scan_of_many_groups(gpu):
     for got, w in zip([y, *grads], [want, *torch.autograd.grad(want, ref, gy.cpu().double())]):
         got, w = got.detach().cpu().double(), w.detach()
         assert ((got - w).abs() <= 2.0 ** -24 * w.abs() + (64 + 2 * 3) * 2.0 ** -24 * w.abs().max()).all()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_single_token_stored_time_first(gpu, monkeypatch, native):
+    """[batch, 1, channels] as a view of [1, batch, channels]: where the next token would be is far away, and does not matter."""
+    if not native:
+        monkeypatch.setattr(state_space, "_native", None)
+    S, D, N = 4096, 1024, 4
+    g = torch.Generator(device=gpu).manual_seed(4)
+    first = [torch.randn(1, S, D, generator=g, device=gpu).transpose(0, 1) for _ in range(4)]
+    B, C = (torch.randn(1, S, N, generator=g, device=gpu).transpose(0, 1) for _ in range(2))
+    A = -torch.randn(D, N, generator=g, device=gpu).exp()
+    assert first[0].stride(1) == 1 << 22
+    results = []
+    for lay in (lambda t: t, lambda t: t[:, 0].clone()[:, None]):
+        x, dt, z, gy, b, c = (lay(t) for t in (*first, B, C))
+        leaves = [t.detach().requires_grad_() for t in (x, dt, A, b, c, z)]
+        y = f.selective_scan(leaves[0], leaves[1], leaves[2], leaves[3], leaves[4], z=leaves[5], softplus=True)
+        results.append([y, *torch.autograd.grad(y, leaves, gy)])
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+def test_selections_of_far_tokens(gpu):
+    """16 384 groups with 256 states: 2^22 values of B a token, more than the kernels reach over within a tile."""
+    G, N = 16384, 256
+    g = torch.Generator(device=gpu).manual_seed(5)
+    x, dt, gy = (torch.randn(1, 3, G, generator=g, device=gpu) for _ in range(3))
+    B, C = (torch.randn(1, 3, G, N, generator=g, device=gpu) for _ in range(2))
+    A = -torch.randn(G, N, generator=g, device=gpu).exp()
+    leaves = [t.requires_grad_() for t in (x, dt, A, B, C)]
+    y = f.selective_scan(*leaves, softplus=True)
+    grads = torch.autograd.grad(y, leaves, gy)
+    ref = [t.detach().cpu().double().requires_grad_() for t in leaves]
+    want = baseline.naive_selective_scan(*ref, softplus=True)
+    for got, w in zip([y, *grads], [want, *torch.autograd.grad(want, ref, gy.cpu().double())]):
+        got, w = got.detach().cpu().double(), w.detach()
+        assert got.shape == w.shape and ((got - w).abs() <= 2.0 ** -24 * w.abs() + (64 + 2 * 3) * 2.0 ** -24 * w.abs().max()).all()

@@ -88,6 +88,22 @@ int check_norm(const scanscam_norm *a)
     return SCANSCAM_OK;
 }
 
+// A forward call's arguments for `count` of its rows.
+scanscam_norm rows_from(const scanscam_norm &a, int64_t row, int64_t count)
+{
+    const auto moved = [](auto *p, int64_t bytes) { return p == nullptr ? p : (decltype(p))((const char *)p + bytes); };
+    const int size = activation_size(a.dtype), residual = activation_size(a.residual_dtype), out = activation_size(a.out_dtype);
+    scanscam_norm now = a;
+    now.rows = count;
+    now.x = moved(a.x, row * a.x_stride * size);
+    now.residual = moved(a.residual, row * a.residual_stride * residual);
+    now.y = moved(a.y, row * a.channels * (out > 0 ? out : 1));
+    now.sum = moved(a.sum, row * a.channels * residual);
+    now.rstd = moved(a.rstd, row * (int64_t)sizeof(float));
+    now.scale = moved(a.scale, row * (int64_t)sizeof(float));
+    return now;
+}
+
 hipError_t run_norm(bool back, const NormPlan &plan, unsigned grid, size_t lds, hipStream_t stream, const NormArgs &args)
 {
     switch (args.a.dtype) {
@@ -115,9 +131,15 @@ int scanscam_norm_fwd(const scanscam_norm *a, void *stream)
     }
     if (!eight && misaligned(a->y, (size_t)activation_size(a->dtype))) return SCANSCAM_EALIGN;
     const NormPlan plan = norm_plan(*a);
-    if (ceil_div(a->rows, plan.groups) * plan.waves * plan.groups * 64 >= int64_t(1) << 32) return SCANSCAM_EINVAL;  // (threads of a launch)
-    const hipError_t err = run_norm(false, plan, (unsigned)ceil_div(a->rows, plan.groups), 0, s, NormArgs{*a, plan.waves, plan.shifted, nullptr});
-    return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
+    // A launch has fewer than 2^32 threads: more rows than that are several launches, a multiple of 8 rows each, so that a launch's
+    // first row begins on a vector's border where the first one of all does.
+    const int64_t threads = 64 * plan.waves * plan.groups, most = ((int64_t(1) << 32) / threads - 1) * plan.groups / 8 * 8;
+    for (int64_t row = 0; row < a->rows; row += most) {
+        const scanscam_norm now = rows_from(*a, row, a->rows - row < most ? a->rows - row : most);
+        const hipError_t err = run_norm(false, plan, (unsigned)ceil_div(now.rows, plan.groups), 0, s, NormArgs{now, plan.waves, plan.shifted, nullptr});
+        if (err != hipSuccess) return SCANSCAM_ELAUNCH;
+    }
+    return SCANSCAM_OK;
 }
 
 size_t scanscam_norm_workspace_bytes(const scanscam_norm *a)

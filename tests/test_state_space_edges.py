@@ -145,3 +145,12 @@ def test_selective_scans_of_many_parts_are_several_launches(recorded):
     assert sum(n for n, _ in launches(lines)) == 3000000 * 64
     assert recorded("print(L.scanscam_selective_fwd(scan(batch=1 << 20, sequences=1 << 20, T=1 << 11), None))") == [["1"]]  # 2^31 tokens
     assert recorded("print(L.scanscam_selective_fwd(scan(batch=1 << 25, sequences=1 << 25, T=0), None))")[-1] == ["0"]
+
+
+def test_norms_of_many_rows_are_several_launches(recorded):
+    for rows, channels, eight in (((1 << 26) + 3, 8, 0), ((1 << 27) + 1, 64, 17), (1 << 30, 1, 0), (1 << 25, 16384, 16), (100, 5, 0)):
+        lines = recorded(f"""
+            a = s._Norm(rows={rows}, channels={channels}, x_stride={channels}, dtype=1, out_dtype={eight or 1}, x=fake, y=fake, scale=fake, weight=P)
+            assert L.scanscam_norm_fwd(a, None) == 0
+        """)
+        assert sum(n * threads // 64 for n, threads in launches(lines)) >= rows  # (a row has a wave or more)

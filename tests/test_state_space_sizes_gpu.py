@@ -159,3 +159,32 @@ def test_selections_of_far_tokens(gpu):
     for got, w in zip([y, *grads], [want, *torch.autograd.grad(want, ref, gy.cpu().double())]):
         got, w = got.detach().cpu().double(), w.detach()
         assert got.shape == w.shape and ((got - w).abs() <= 2.0 ** -24 * w.abs() + (64 + 2 * 3) * 2.0 ** -24 * w.abs().max()).all()
+
+
+@pytest.mark.parametrize("quant", [None, torch.float8_e4m3fn])
+def test_norm_of_many_rows(gpu, quant):
+    """More rows than a launch has waves for, of a width at which rows begin inside vectors: every row is its own norm."""
+    rows, D = (1 << 26) + 3, 9
+    g = torch.Generator(device=gpu).manual_seed(6)
+    x = torch.empty(rows, D, dtype=torch.bfloat16, device=gpu).normal_(generator=g)
+    r = torch.empty(rows, D, dtype=torch.bfloat16, device=gpu).normal_(generator=g)
+    w = torch.randn(D, generator=g, device=gpu)
+    outs = f.rms_norm(x, w, r, quant=quant)
+    if quant is None:
+        leaves = [t.clone().requires_grad_() for t in (x, w, r)]
+        gx, gw, _ = torch.autograd.grad(f.rms_norm(*leaves)[0], leaves, x)
+        assert torch.isfinite(gw).all()
+    for start in range(0, rows, 1 << 23):  # (each piece is a call of one launch)
+        piece = slice(start, min(rows, start + (1 << 23)))
+        want = f.rms_norm(x[piece], w, r[piece], quant=quant)
+        for got, one in zip(outs, want):
+            assert torch.equal(got[piece].view(torch.uint8), one.view(torch.uint8)), start
+    last = slice(rows - 5, rows)
+    total = (x[last].float() + r[last].float()).to(torch.bfloat16)
+    assert torch.equal(outs[-1][last], total)
+    if quant is None:
+        leaf, wide = total.double().requires_grad_(), w.double()
+        y = leaf / torch.sqrt(leaf.square().mean(-1, keepdim=True) + 1e-6) * wide
+        (want,) = torch.autograd.grad(y, leaf, x[last].double())
+        for got, one in ((outs[0][last], y.detach()), (gx[last], want)):
+            assert ((got.double() - one).abs() <= 2.0 ** -8 * 1.01 * one.abs() + 64 * 2.0 ** -24 * one.abs().max()).all()

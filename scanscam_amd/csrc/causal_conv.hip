@@ -20,6 +20,7 @@ struct ConvArgs {
     float *part;      // backward: [stretches][K + 1][channels] sums of gp x and of gp
     int64_t stretch;  // tokens of a lane
     int64_t stretches;
+    int64_t unit0;    // the first unit of this launch: a stretch of a batch element, or a sequence's state
 };
 
 __device__ __forceinline__ float act_(float p, int kind) { return kind == SCANSCAM_ACT_SILU ? p * sigmoid_(p) : p; }
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(256) void conv_fwd_kernel(ConvArgs args)
     if (mine >= a.channels) return;
     int count;
     const int64_t c = lane_channels<VEC>(a.channels, mine, count);
-    const int64_t unit = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;  // a stretch of a batch element, or a sequence's state
+    const int64_t unit = args.unit0 + (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int64_t walks = a.batch * args.stretches;
     if (unit >= walks) {  // the states after the last tokens
         const int64_t s = unit - walks;
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256, 2) void conv_bwd_kernel(ConvArgs args)
     if (mine >= a.channels) return;
     int count;
     const int64_t c = lane_channels<VEC>(a.channels, mine, count);
-    const int64_t unit = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int64_t unit = args.unit0 + (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (unit >= a.batch * args.stretches) {
         // Sequences without a token: the state goes through as it is.
         const int64_t s = unit - a.batch * args.stretches;
@@ -406,8 +407,7 @@ int check_conv(const scanscam_conv *a)
     if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->batch >= kMostTokens || a->sequences < 0 || a->sequences >= kMostTokens)
         return SCANSCAM_EINVAL;
     if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
-    // (a launch has fewer than 2^32 threads, and a stretch at least 8 tokens)
-    if (a->batch > 0 && a->T / 8 + 1 > (int64_t(1) << 23) / a->batch) return SCANSCAM_EINVAL;
+    if (a->batch > 0 && a->T > (kMostTokens - 1) / a->batch) return SCANSCAM_EINVAL;
     if (a->channels == 0) return SCANSCAM_OK;
     SCANSCAM_CHECK(check_param(a->weight, true));
     SCANSCAM_CHECK(check_param(a->bias, false));
@@ -420,7 +420,8 @@ int check_conv(const scanscam_conv *a)
 
 struct ConvPlan {
     int64_t stretch, stretches, units;
-    dim3 grid, block;
+    dim3 block;
+    unsigned blocks;  // of channels
 };
 
 // Stretches of up to 64 tokens (backwards 128: their borders cost more), shorter where there are too few to give every SIMD two waves.
@@ -436,14 +437,21 @@ ConvPlan conv_plan(const scanscam_conv &a, bool back, bool states)
     const int y = 256 / x;
     p.units = a.batch * p.stretches + (states ? a.sequences : 0);
     p.block = dim3(x, y);
-    p.grid = dim3((unsigned)ceil_div(p.units, y), (unsigned)ceil_div(lanes, x));
+    p.blocks = (unsigned)ceil_div(lanes, x);
     return p;
 }
 
-template <typename ST, int K> hipError_t run_conv(const ConvArgs &args, const ConvPlan &p, bool back, hipStream_t stream)
+// A launch has fewer than 2^32 threads along each of its dimensions: more units than that are several launches.
+template <typename ST, int K> hipError_t run_conv(ConvArgs args, const ConvPlan &p, bool back, hipStream_t stream)
 {
-    return back ? launch_op(conv_bwd_kernel<ST, K>, p.grid, p.block, 0, stream, args)
-                : launch_op(conv_fwd_kernel<ST, K>, p.grid, p.block, 0, stream, args);
+    const int64_t most = ((int64_t(1) << 32) / p.block.x - 1) * p.block.y;
+    hipError_t err = hipSuccess;
+    for (; args.unit0 < p.units && err == hipSuccess; args.unit0 += most) {
+        const int64_t now = p.units - args.unit0 < most ? p.units - args.unit0 : most;
+        const dim3 grid((unsigned)ceil_div(now, p.block.y), p.blocks);
+        err = back ? launch_op(conv_bwd_kernel<ST, K>, grid, p.block, 0, stream, args) : launch_op(conv_fwd_kernel<ST, K>, grid, p.block, 0, stream, args);
+    }
+    return err;
 }
 template <typename ST> hipError_t run_conv(const ConvArgs &args, const ConvPlan &p, bool back, hipStream_t stream)
 {
@@ -496,8 +504,7 @@ int scanscam_conv_fwd(const scanscam_conv *a, void *stream)
         SCANSCAM_CHECK(check_tokens(a->y, size));
     }
     const ConvPlan p = conv_plan(*a, false, states);
-    if (p.grid.x == 0) return SCANSCAM_OK;
-    const hipError_t err = run_conv({*a, nullptr, p.stretch, p.stretches}, p, false, static_cast<hipStream_t>(stream));
+    const hipError_t err = run_conv({*a, nullptr, p.stretch, p.stretches, 0}, p, false, static_cast<hipStream_t>(stream));
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
 }
 
@@ -527,8 +534,7 @@ int scanscam_conv_bwd(const scanscam_conv *a, void *stream)
     }
     const ConvPlan p = conv_plan(*a, true, states);
     float *part = static_cast<float *>(a->workspace);
-    hipError_t err = hipSuccess;
-    if (p.grid.x > 0) err = run_conv({*a, part, p.stretch, p.stretches}, p, true, s);
+    hipError_t err = run_conv({*a, part, p.stretch, p.stretches, 0}, p, true, s);
     const int64_t parts = a->batch * p.stretches, wide = a->K * a->channels, pitch = wide + a->channels;
     if (err == hipSuccess) err = column_sum({part, parts, pitch, {a->gweight, a->gbias}, {wide, a->channels}}, s);
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;

@@ -154,3 +154,19 @@ def test_norms_of_many_rows_are_several_launches(recorded):
             assert L.scanscam_norm_fwd(a, None) == 0
         """)
         assert sum(n * threads // 64 for n, threads in launches(lines)) >= rows  # (a row has a wave or more)
+
+
+def test_convolutions_of_many_stretches_are_several_launches(recorded):
+    for batch, T, channels, packed in (((1 << 23) + 9, 1, 4, 0), (1, (1 << 30) + 5, 64, 0), (1 << 24, 3, 4096, 0), (1, 5, 4096, 1 << 26), (2, 9, 24, 0)):
+        lines = recorded(f"""
+            a = s._Conv(batch={batch}, T={T}, sequences={packed or batch}, channels={channels}, K=4, dtype=1, x=T(), y=T(), gy=T(), gx=T(), weight=P, gweight=fake,
+                        offsets={'fake' if packed else 'None'}, state_in=fake, state_out=fake, gstate_in=fake, workspace=fake, workspace_bytes=1 << 62)
+            assert L.scanscam_conv_fwd(a, None) == 0
+            print("backwards", flush=True)
+            assert L.scanscam_conv_bwd(a, None) == 0
+        """)
+        back = lines.index(["backwards"])
+        for part, vec in ((lines[:back], 8), (lines[back + 1:], 4)):
+            lanes = sum(n * threads for n, threads in launches(part) if threads == 256)
+            assert lanes >= channels // vec * ((packed or batch) + batch * -(-T // 128))  # (a lane a vector of each state and of each stretch at least)
+    assert recorded("print(L.scanscam_conv_fwd(s._Conv(batch=4, T=1 << 29, sequences=4, channels=8, K=4, x=T(), y=T(), weight=P), None))") == [["1"]]  # 2^31 tokens

@@ -188,3 +188,25 @@ def test_norm_of_many_rows(gpu, quant):
         (want,) = torch.autograd.grad(y, leaf, x[last].double())
         for got, one in ((outs[0][last], y.detach()), (gx[last], want)):
             assert ((got.double() - one).abs() <= 2.0 ** -8 * 1.01 * one.abs() + 64 * 2.0 ** -24 * one.abs().max()).all()
+
+
+def test_convolution_of_many_sequences(gpu):
+    """More sequences than a launch has lanes for, one token each: y = w[1] x + w[0] state, and gradients that follow from that. Roundings of
+    2^-24: 3 of an output; 3 x 80 + 16 of a parameter's gradient (8 388 617 parts in three levels)."""
+    S, D = (1 << 23) + 9, 4
+    g = torch.Generator(device=gpu).manual_seed(7)
+    x, gy, kept, gkept = (torch.randn(S, 1, D, generator=g, device=gpu) for _ in range(4))
+    w = torch.randn(D, 2, generator=g, device=gpu)
+    leaves = [t.requires_grad_() for t in (x, w, kept)]
+    y, new = f.causal_conv(leaves[0], leaves[1], state=leaves[2], return_state=True)
+    assert torch.equal(new, x)
+    gx, gw, gstate = torch.autograd.grad((y, new), leaves, (gy, gkept))
+    with torch.no_grad():
+        a, b = w[:, 1].double(), w[:, 0].double()
+        for start in range(0, S, 1 << 21):
+            p = slice(start, start + (1 << 21))
+            for got, terms in ((y, (a * x[p], b * kept[p])), (gx, (a * gy[p], gkept[p].double())), (gstate, (b * gy[p],))):
+                assert ((got[p] - sum(terms)).abs() <= 3 * 2.0 ** -24 * sum(t.abs() for t in terms)).all()
+        for k, rows in ((0, kept), (1, x)):
+            terms = gy.double() * rows
+            assert ((gw[:, k] - terms.sum((0, 1))).abs() <= (16 + 3 * 80) * 2.0 ** -24 * terms.abs().sum((0, 1))).all()

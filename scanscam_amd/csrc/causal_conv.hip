@@ -341,11 +341,12 @@ __global__ __launch_bounds__(256, 2) void conv_bwd_kernel(ConvArgs args)
 // A lane's vector of one row: the window moves on by a token. 512 rows of 2048 channels in bf16, K = 4: 6 us (17 MB, 2.7 TB/s), mostly a launch and
 // one trip to memory.
 template <typename ST, int K>
-__global__ __launch_bounds__(256) void conv_step_kernel(scanscam_conv_step a)
+__global__ __launch_bounds__(256) void conv_step_kernel(StepPart<scanscam_conv_step> args)
 {
+    const scanscam_conv_step &a = args.a;
     constexpr int VEC = 16 / sizeof(ST);
-    const int64_t c = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int64_t c = ((int64_t)(args.block0 + blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+    const int64_t row = args.row0 + (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (c >= a.channels || row >= a.rows) return;
     const int count = (int)clamp_(a.channels - c, 0, VEC);  // (no lane does another's work again here: the state is read and written in place)
     const int64_t slot = a.slot != nullptr ? index_at(a.slot, a.slot64, row) : row;
@@ -475,17 +476,17 @@ hipError_t run_conv(const ConvArgs &args, const ConvPlan &p, bool back, hipStrea
     }
 }
 
-template <typename ST> hipError_t run_step(const scanscam_conv_step &a, dim3 grid, dim3 block, hipStream_t stream)
+template <typename ST> hipError_t run_step(const scanscam_conv_step &a, int64_t blocks, dim3 block, hipStream_t stream)
 {
     switch (a.K) {
-    case 1: return launch_op(conv_step_kernel<ST, 1>, grid, block, 0, stream, a);
-    case 2: return launch_op(conv_step_kernel<ST, 2>, grid, block, 0, stream, a);
-    case 3: return launch_op(conv_step_kernel<ST, 3>, grid, block, 0, stream, a);
-    case 4: return launch_op(conv_step_kernel<ST, 4>, grid, block, 0, stream, a);
-    case 5: return launch_op(conv_step_kernel<ST, 5>, grid, block, 0, stream, a);
-    case 6: return launch_op(conv_step_kernel<ST, 6>, grid, block, 0, stream, a);
-    case 7: return launch_op(conv_step_kernel<ST, 7>, grid, block, 0, stream, a);
-    default: return launch_op(conv_step_kernel<ST, 8>, grid, block, 0, stream, a);
+    case 1: return launch_step(conv_step_kernel<ST, 1>, a.rows, blocks, block, stream, a);
+    case 2: return launch_step(conv_step_kernel<ST, 2>, a.rows, blocks, block, stream, a);
+    case 3: return launch_step(conv_step_kernel<ST, 3>, a.rows, blocks, block, stream, a);
+    case 4: return launch_step(conv_step_kernel<ST, 4>, a.rows, blocks, block, stream, a);
+    case 5: return launch_step(conv_step_kernel<ST, 5>, a.rows, blocks, block, stream, a);
+    case 6: return launch_step(conv_step_kernel<ST, 6>, a.rows, blocks, block, stream, a);
+    case 7: return launch_step(conv_step_kernel<ST, 7>, a.rows, blocks, block, stream, a);
+    default: return launch_step(conv_step_kernel<ST, 8>, a.rows, blocks, block, stream, a);
     }
 }
 
@@ -556,11 +557,12 @@ int scanscam_conv_step_fwd(const scanscam_conv_step *a, void *stream)
     const int64_t lanes = ceil_div(a->channels, 16 / size);
     int x = 1;
     while (x < 256 && x < lanes) x *= 2;
-    const dim3 block(x, 256 / x), grid((unsigned)ceil_div(a->rows, 256 / x), (unsigned)ceil_div(lanes, x));
+    const dim3 block(x, 256 / x);
+    const int64_t blocks = ceil_div(lanes, x);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const hipError_t err = a->dtype == SCANSCAM_F32    ? run_step<float>(*a, grid, block, s)
-                           : a->dtype == SCANSCAM_BF16 ? run_step<__bf16>(*a, grid, block, s)
-                                                       : run_step<_Float16>(*a, grid, block, s);
+    const hipError_t err = a->dtype == SCANSCAM_F32    ? run_step<float>(*a, blocks, block, s)
+                           : a->dtype == SCANSCAM_BF16 ? run_step<__bf16>(*a, blocks, block, s)
+                                                       : run_step<_Float16>(*a, blocks, block, s);
     return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH;
 }
 

@@ -194,6 +194,26 @@ inline hipError_t column_sum(ColumnSum a, hipStream_t stream)
     return launch_op(column_sum_kernel, dim3(grid), dim3(1024), 0, stream, a);
 }
 
+// A single token's step in launches of fewer than 2^32 threads along each dimension and of a second dimension that a grid can have.
+template <typename Step> struct StepPart {
+    Step a;
+    int64_t row0;     // the first row of this launch
+    uint32_t block0;  // and its first block of channels
+};
+template <typename Kernel, typename Step>
+inline hipError_t launch_step(Kernel kernel, int64_t rows, int64_t blocks, dim3 block, hipStream_t stream, const Step &a)
+{
+    const int64_t most_rows = ((int64_t(1) << 32) / block.x - 1) * block.y, most_blocks = 32768;
+    hipError_t err = hipSuccess;
+    for (int64_t row = 0; row < rows; row += most_rows) {
+        for (int64_t first = 0; first < blocks && err == hipSuccess; first += most_blocks) {
+            const dim3 grid((unsigned)ceil_div(rows - row < most_rows ? rows - row : most_rows, block.y), (unsigned)(blocks - first < most_blocks ? blocks - first : most_blocks));
+            err = launch_op(kernel, grid, block, 0, stream, StepPart<Step>{a, row, (uint32_t)first});
+        }
+    }
+    return err;
+}
+
 // --- checks of arguments ---------------------------------------------------------------------------------------------------
 inline int activation_size(int dtype)
 {

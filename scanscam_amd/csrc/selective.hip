@@ -195,14 +195,14 @@ template <typename ST> hipError_t run_step(const scanscam_selective_step &a, hip
 {
     int lanes = 1;
     while (lanes < 32 && lanes * 4 < a.N) lanes *= 2;
-    const dim3 grid((unsigned)a.rows, (unsigned)ceil_div(a.channels, 256 / lanes));
+    const int64_t blocks = ceil_div(a.channels, 256 / lanes);
     switch (lanes) {
-    case 1: return launch_op(selective_step_kernel<ST, 1>, grid, dim3(256), 0, stream, a);
-    case 2: return launch_op(selective_step_kernel<ST, 2>, grid, dim3(256), 0, stream, a);
-    case 4: return launch_op(selective_step_kernel<ST, 4>, grid, dim3(256), 0, stream, a);
-    case 8: return launch_op(selective_step_kernel<ST, 8>, grid, dim3(256), 0, stream, a);
-    case 16: return launch_op(selective_step_kernel<ST, 16>, grid, dim3(256), 0, stream, a);
-    default: return launch_op(selective_step_kernel<ST, 32>, grid, dim3(256), 0, stream, a);
+    case 1: return launch_step(selective_step_kernel<ST, 1>, a.rows, blocks, dim3(256), stream, a);
+    case 2: return launch_step(selective_step_kernel<ST, 2>, a.rows, blocks, dim3(256), stream, a);
+    case 4: return launch_step(selective_step_kernel<ST, 4>, a.rows, blocks, dim3(256), stream, a);
+    case 8: return launch_step(selective_step_kernel<ST, 8>, a.rows, blocks, dim3(256), stream, a);
+    case 16: return launch_step(selective_step_kernel<ST, 16>, a.rows, blocks, dim3(256), stream, a);
+    default: return launch_step(selective_step_kernel<ST, 32>, a.rows, blocks, dim3(256), stream, a);
     }
 }
 
@@ -280,7 +280,7 @@ int scanscam_selective_step_fwd(const scanscam_selective_step *a, void *stream)
 {
     if (a == nullptr) return SCANSCAM_EINVAL;
     SCANSCAM_CHECK(check_sizes(a->channels, a->groups, a->N, a->dtype));
-    if (a->rows < 0 || a->rows >= (int64_t(1) << 24) || a->slots < 0) return SCANSCAM_EINVAL;
+    if (a->rows < 0 || a->rows >= kMostTokens || a->slots < 0) return SCANSCAM_EINVAL;
     if (a->rows == 0 || a->channels == 0) return SCANSCAM_OK;
     const int size = activation_size(a->dtype);
     for (const scanscam_tokens *t : {&a->x, &a->dt, &a->B, &a->C, &a->y}) SCANSCAM_CHECK(check_tokens(*t, size));

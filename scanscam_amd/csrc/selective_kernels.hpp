@@ -1087,10 +1087,11 @@ __global__ __launch_bounds__(256) void selective_bc_kernel(GroupSum args)
 // 4.9 TB/s. One row: 4 us, which are a launch and one trip to memory.
 // ---------------------------------------------------------------------------------------------------------------------------
 template <typename ST, int LANES>
-__global__ __launch_bounds__(256) void selective_step_kernel(scanscam_selective_step a)
+__global__ __launch_bounds__(256) void selective_step_kernel(StepPart<scanscam_selective_step> args)
 {
+    const scanscam_selective_step &a = args.a;
     const int lane = threadIdx.x % LANES, N = (int)a.N;
-    const int64_t c = (int64_t)blockIdx.y * (256 / LANES) + threadIdx.x / LANES, row = blockIdx.x;
+    const int64_t c = (int64_t)(args.block0 + blockIdx.y) * (256 / LANES) + threadIdx.x / LANES, row = args.row0 + blockIdx.x;
     const int64_t slot = a.slot != nullptr ? index_at(a.slot, a.slot64, row) : row;
     const bool there = c < a.channels;
     if (slot < 0 || slot >= a.slots) {

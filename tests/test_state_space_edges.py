@@ -170,3 +170,20 @@ def test_convolutions_of_many_stretches_are_several_launches(recorded):
             lanes = sum(n * threads for n, threads in launches(part) if threads == 256)
             assert lanes >= channels // vec * ((packed or batch) + batch * -(-T // 128))  # (a lane a vector of each state and of each stretch at least)
     assert recorded("print(L.scanscam_conv_fwd(s._Conv(batch=4, T=1 << 29, sequences=4, channels=8, K=4, x=T(), y=T(), weight=P), None))") == [["1"]]  # 2^31 tokens
+
+
+def test_steps_of_many_rows_or_channels_are_several_launches(recorded):
+    for rows, channels, N in ((1 << 24, 32, 16), (3, 1 << 20, 128), ((1 << 25) + 1, 8, 1), (1, 1, 1)):
+        lines = recorded(f"""
+            a = s._SelectiveStep(rows={rows}, channels={channels}, groups=1, N={N}, slots=1, slot=fake, state=fake, A=P)
+            for n in ("x", "dt", "B", "C", "y"):
+                setattr(a, n, T())
+            assert L.scanscam_selective_step_fwd(a, None) == 0
+        """)
+        lanes = min(32, 1 << max(0, (N - 1).bit_length() - 2))
+        assert sum(n for n, _ in launches(lines)) == rows * -(-channels * lanes // 256)
+        lines = recorded(f"""
+            a = s._ConvStep(rows={rows}, channels={channels}, K=4, slots=1, slot=fake, state=fake, weight=P, x=T(), y=T())
+            assert L.scanscam_conv_step_fwd(a, None) == 0
+        """)
+        assert sum(n * threads for n, threads in launches(lines)) >= rows * -(-channels // 4)

@@ -210,3 +210,22 @@ def test_convolution_of_many_sequences(gpu):
         for k, rows in ((0, kept), (1, x)):
             terms = gy.double() * rows
             assert ((gw[:, k] - terms.sum((0, 1))).abs() <= (16 + 3 * 80) * 2.0 ** -24 * terms.abs().sum((0, 1))).all()
+
+
+@pytest.mark.parametrize("rows,D,N", [((1 << 24) + 5, 4, 1), (2, 1 << 20, 128)])
+def test_steps_of_many_rows_or_channels(gpu, rows, D, N):
+    """More than a launch has threads or a grid's second dimension workgroups for: the rows and channels of calls of their own."""
+    g = torch.Generator(device=gpu).manual_seed(8)
+    x, dt = (torch.randn(rows, D, generator=g, device=gpu) for _ in range(2))
+    B, C = (torch.randn(rows, N, generator=g, device=gpu) for _ in range(2))
+    A, state = -torch.rand(D, N, generator=g, device=gpu), torch.randn(rows, D, N, generator=g, device=gpu)
+    kept, w = torch.randn(rows, 2, D, generator=g, device=gpu), torch.randn(D, 3, generator=g, device=gpu)
+    slots = torch.randperm(rows, generator=g, device=gpu)
+    new, new_kept = state.clone(), kept.clone()
+    y, u = f.selective_scan_step(new, x, dt, A, B, C, softplus=True, slots=slots), f.causal_conv_step(new_kept, x, w, slots=slots)
+    for r in (slice(0, min(rows, 9)), slice(max(0, rows - 9), rows)):
+        for c in (slice(0, min(D, 64)), slice(D - min(D, 64), D)):
+            mine = slots[r]
+            one, one_kept = state[mine][:, c].contiguous(), kept[mine][..., c].contiguous()
+            assert torch.equal(f.selective_scan_step(one, x[r, c], dt[r, c], A[c], B[r], C[r], softplus=True), y[r, c]) and torch.equal(new[mine][:, c], one)
+            assert torch.equal(f.causal_conv_step(one_kept, x[r, c], w[c]), u[r, c]) and torch.equal(new_kept[mine][..., c], one_kept)

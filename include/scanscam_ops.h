@@ -27,6 +27,10 @@
 
 #include "scanscam_hip.h"
 
+/* A call takes up to so many channels (the norm 32768), and fewer than so many tokens of all batch elements, sequences or rows. */
+#define SCANSCAM_MOST_CHANNELS (1 << 20)
+#define SCANSCAM_MOST_TOKENS ((INT64_C(1) << 31) - (INT64_C(1) << 20))
+
 #ifdef __cplusplus
 extern "C" {
 #endif

@@ -233,7 +233,7 @@ inline int check_param(const scanscam_param &p, bool required)
     return misaligned(p.p, (size_t)size) ? SCANSCAM_EALIGN : SCANSCAM_OK;
 }
 
-constexpr int64_t kMostTokens = (int64_t(1) << 31) - (int64_t(1) << 20), kMostChannels = int64_t(1) << 20;
+constexpr int64_t kMostTokens = SCANSCAM_MOST_TOKENS, kMostChannels = SCANSCAM_MOST_CHANNELS;
 
 #define SCANSCAM_CHECK(expr)                      \
     do {                                          \

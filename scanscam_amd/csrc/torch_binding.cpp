@@ -494,6 +494,11 @@ struct Arguments {
         ok = false;
         return 0;
     }
+    // What one call takes; the Python path says so.
+    void sizes(int64_t channels, int64_t tokens, int64_t sequences = 0)
+    {
+        if (channels > SCANSCAM_MOST_CHANNELS || tokens >= SCANSCAM_MOST_TOKENS || sequences >= SCANSCAM_MOST_TOKENS) ok = false;
+    }
     void shape(const at::Tensor &t, at::IntArrayRef sizes)
     {
         if (t.defined() && t.sizes() != sizes) ok = false;
@@ -857,6 +862,7 @@ PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     scanscam_norm a{};
     a.rows = x.numel() / channels;
     a.channels = channels;
+    in.sizes(channels, a.rows);
     a.x = x.data_ptr();
     a.x_stride = row_stride(x);
     if (a.x_stride < 0) in.ok = false;
@@ -934,6 +940,7 @@ PyObject *conv(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     a.K = weight.size(1);
     a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
     if (a.K < 1 || a.K > kMostTaps) Py_RETURN_NONE;
+    in.sizes(a.channels, a.batch * a.T, a.sequences);
     in.shape(weight, {a.channels, a.K});
     in.shape(bias, {a.channels});
     in.shape(state, {a.sequences, a.K - 1, a.channels});
@@ -977,6 +984,7 @@ PyObject *conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     a.K = weight.size(1);
     a.slots = state.size(0);
     if (a.K < 1 || a.K > kMostTaps || (!slots.defined() && a.slots != a.rows)) Py_RETURN_NONE;
+    in.sizes(a.channels, a.rows);
     in.shape(weight, {a.channels, a.K});
     in.shape(bias, {a.channels});
     in.shape(state, {a.slots, a.K - 1, a.channels});
@@ -1042,6 +1050,7 @@ PyObject *selective(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     a.batch = x.size(0);
     a.T = x.size(1);
     a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+    in.sizes(a.channels, a.batch * a.T, a.sequences);
     in.shape(state, {a.sequences, a.channels, a.N});
     a.offsets = in.indices(offsets, &a.offsets64);
     a.state_in = static_cast<const float *>(in.dense(state, at::kFloat));
@@ -1088,6 +1097,7 @@ PyObject *selective_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     a.rows = x.size(0);
     a.slots = state.size(0);
     if (!slots.defined() && a.slots != a.rows) Py_RETURN_NONE;
+    in.sizes(a.channels, a.rows);
     in.shape(state, {a.slots, a.channels, a.N});
     in.shape(slots, {a.rows});
     a.slot = in.indices(slots, &a.slot64);

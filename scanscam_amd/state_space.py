@@ -24,6 +24,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _EIGHT = {torch.int8: 16, torch.float8_e4m3fn: 17}
 _ACTIVATIONS = {None: 0, "silu": 1}
 _MOST_STATES, _MOST_TAPS, _MOST_NORM_CHANNELS, _MOST_TOKEN_STRIDE = 256, 8, 32768, 1 << 22
+_MOST_CHANNELS, _MOST_TOKENS = 1 << 20, (1 << 31) - (1 << 20)
 
 _p, _i32, _i64, _f32, _size = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -173,6 +174,13 @@ def _check_devices(what: str, first: torch.Tensor, tensors) -> None:
 def _check_shape(what: str, name: str, t: Optional[torch.Tensor], shape) -> None:
     if t is not None and tuple(t.shape) != tuple(shape):
         raise AssertionError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _check_sizes(what: str, channels: int, tokens: int, sequences: int = 0) -> None:
+    """What one call on the GPU takes (CPU tensors have no such limits)."""
+    if channels > _MOST_CHANNELS or max(tokens, sequences) >= _MOST_TOKENS:
+        raise AssertionError(f"{what}: a call takes up to {_MOST_CHANNELS} channels and fewer than {_MOST_TOKENS} tokens, rows or sequences, "
+                             f"got {channels} channels, {tokens} tokens" + (f", {sequences} sequences" if sequences else ""))
 
 
 def _check_offsets(what: str, x: torch.Tensor, offsets: Optional[torch.Tensor]) -> int:
@@ -342,6 +350,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         raise TypeError(f"{what}: state must be float32, got {state.dtype}")
     if x.device.type != "cuda":
         return baseline.naive_selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus=softplus, state=state, offsets=offsets, return_state=return_state)
+    _check_sizes(what, channels, batch * T, sequences)
     if B.dim() == 3:
         B, C = _grouped(B), _grouped(C)
     if _needs_node(x, dt, A, B, C, D, z, dt_bias, state):
@@ -467,6 +476,7 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         raise RuntimeError(f"{what}: a single token's step has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_selective_scan_step(state, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, slots=slots)
+    _check_sizes(what, channels, rows)
     if B.dim() == 2:
         B, C = _grouped(B), _grouped(C)
     if torch.jit.is_tracing():
@@ -533,6 +543,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         _check_shape(what, name, t, shape)
     if x.device.type != "cuda":
         return baseline.naive_causal_conv(x, weight, bias, activation=activation, state=state, offsets=offsets, return_state=return_state)
+    _check_sizes(what, channels, x.shape[0] * x.shape[1], sequences)
     if _needs_node(x, weight, bias, state):
         y, new = CausalConv.apply(x, weight, bias, state, offsets, activation, bool(return_state))
     else:
@@ -633,6 +644,7 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         raise RuntimeError(f"{what}: a single token's step has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_causal_conv_step(state, x, weight, bias, activation=activation, slots=slots)
+    _check_sizes(what, channels, rows)
     if torch.jit.is_tracing():
         return CausalConvStep.apply(state, x, weight, bias, slots, activation)
     return _conv_step(state, x, weight, bias, slots, activation)
@@ -696,6 +708,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
         raise RuntimeError(f"{what}: an output in 8 bits has no gradient; call it under torch.no_grad()")
     if x.device.type != "cuda":
         return baseline.naive_rms_norm(x, weight, residual, eps=eps, quant=quant)
+    _check_sizes(what, x.shape[-1], x.shape[:-1].numel())
     if quant is None and _needs_node(x, weight, residual):
         y, total = RmsNorm.apply(x, weight, residual, float(eps))
         return y if residual is None else (y, total)

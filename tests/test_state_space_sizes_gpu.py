@@ -229,3 +229,24 @@ def test_steps_of_many_rows_or_channels(gpu, rows, D, N):
             one, one_kept = state[mine][:, c].contiguous(), kept[mine][..., c].contiguous()
             assert torch.equal(f.selective_scan_step(one, x[r, c], dt[r, c], A[c], B[r], C[r], softplus=True), y[r, c]) and torch.equal(new[mine][:, c], one)
             assert torch.equal(f.causal_conv_step(one_kept, x[r, c], w[c]), u[r, c]) and torch.equal(new_kept[mine][..., c], one_kept)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_what_is_too_large_is_named(gpu, monkeypatch, native):
+    """Sizes that no call takes, of expanded tensors that hold one value: refused by name before anything is allocated."""
+    if not native:
+        monkeypatch.setattr(state_space, "_native", None)
+    one = torch.ones(1, device=gpu)
+    many, wide = 1 << 31, (1 << 20) + 16
+    for call in (lambda: f.rms_norm(one.expand(many, 1), one),
+                 lambda: f.causal_conv(one.expand(1, many, 1), one[None]), lambda: f.causal_conv(one.expand(2, many // 2, 1), one[None]),
+                 lambda: f.causal_conv(one.expand(1, 1, wide), one[None].expand(wide, 1)),
+                 lambda: f.causal_conv_step(torch.empty(1, 0, 1, device=gpu).expand(many, 0, 1).contiguous(), one.expand(many, 1), one[None]),
+                 lambda: f.selective_scan(one.expand(1, many, 1), one.expand(1, many, 1), one[None], one.expand(1, many, 1), one.expand(1, many, 1)),
+                 lambda: f.selective_scan(one.expand(1, 1, wide), one.expand(1, 1, wide), one[None].expand(wide, 1), one.expand(1, 1, 1), one.expand(1, 1, 1)),
+                 lambda: f.selective_scan_step(torch.ones(1, 1, 1, device=gpu), one.expand(many, 1), one.expand(many, 1), one[None], one.expand(many, 1), one.expand(many, 1),
+                                               slots=torch.zeros(1, dtype=torch.int32, device=gpu).expand(many))):
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(AssertionError, match="a call takes up to"):
+            call()
+        assert torch.cuda.memory_allocated() == before

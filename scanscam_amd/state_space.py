@@ -294,8 +294,8 @@ def _wants_grad(*tensors) -> bool:
 
 def _has_tangent(*tensors) -> bool:
     """Whether a forward-mode derivative is asked for, which no kernel here has: calls with gradients go through their autograd
-    function, which refuses it as scan()'s does, and the others refuse it themselves."""
-    return any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    function, which refuses it as scan()'s does, and the others refuse it themselves. (The CPU's loops have them.)"""
+    return any(t is not None and t.device.type == "cuda" and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _needs_node(*tensors) -> bool:

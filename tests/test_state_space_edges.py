@@ -8,8 +8,9 @@ import textwrap
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from scanscam_amd import baseline, rms_norm
+from scanscam_amd import baseline, causal_conv_step, rms_norm, selective_scan_step
 
 
 def test_softplus_has_its_gradient_at_zero():
@@ -187,3 +188,16 @@ def test_steps_of_many_rows_or_channels_are_several_launches(recorded):
             assert L.scanscam_conv_step_fwd(a, None) == 0
         """)
         assert sum(n * threads for n, threads in launches(lines)) >= rows * -(-channels // 4)
+
+
+def test_steps_on_the_cpu_keep_tangents():
+    """Their loops are ordinary operations: what a step's input adds to its output and to the state, forwards."""
+    state, w = torch.zeros(1, 2, 3), torch.rand(3, 3)
+    x, tangent = torch.rand(1, 3), torch.rand(1, 3)
+    A, B = -torch.rand(3, 4), torch.rand(1, 4)
+    with forward_ad.dual_level():
+        dual, kept = forward_ad.make_dual(x, tangent), forward_ad.make_dual(torch.zeros(1, 3, 4), torch.zeros(1, 3, 4))
+        y = causal_conv_step(state.clone(), dual, w)
+        assert torch.equal(forward_ad.unpack_dual(y).tangent, w[:, 2] * tangent)
+        y = selective_scan_step(kept, dual, torch.ones(1, 3), A, B, B)
+        torch.testing.assert_close(forward_ad.unpack_dual(y).tangent, tangent * (B * B).sum())

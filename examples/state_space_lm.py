@@ -135,6 +135,10 @@ def train(model, steps, device, batch=16, T=96, vocabulary=32, seed=0):
 @torch.no_grad()
 def generate(model, prompts, count, eight=None):
     """``count`` tokens after each of the prompts (lists of tokens, of any lengths), which go through the model as one packed batch."""
+    if any(len(p) == 0 for p in prompts):
+        raise ValueError("an empty prompt has no token to go on from")
+    if not prompts or count < 1:
+        return [[] for _ in prompts]
     device = model.norm.device
     offsets = torch.tensor([0] + [len(p) for p in prompts], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(device)
     packed = torch.tensor([t for p in prompts for t in p], device=device).unsqueeze(0)

@@ -250,3 +250,39 @@ def test_what_is_too_large_is_named(gpu, monkeypatch, native):
         with pytest.raises(AssertionError, match="a call takes up to"):
             call()
         assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.parametrize("quant,limit", [(torch.int8, 127.0), (torch.float8_e4m3fn, 448.0)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("residual", [None, "same", torch.float32])
+@pytest.mark.parametrize("D", [2047, 2049, 2500])
+def test_eight_bits_of_many_rows(gpu, quant, limit, dtype, residual, D):
+    """A wave a row, several vectors a lane, rows that begin inside a vector (or not), of a number that is no multiple of a workgroup's. q stands for
+    y to half a step of its type (1/2 for integers; a 16th of the value, or 2^-10, for floats), after three roundings of 2^-24, and a
+    row that holds a NaN or an infinity has neither values nor a scale."""
+    rows = 1030
+    g = torch.Generator(device=gpu).manual_seed(9)
+    x, w = torch.randn(rows, D, generator=g, device=gpu).to(dtype), 1 + 0.2 * torch.randn(D, generator=g, device=gpu)
+    r = None if residual is None else (3 * torch.randn(rows, D, generator=g, device=gpu)).to(dtype if residual == "same" else residual)
+    x[7], x[11, 0], x[12, D - 1], x[1029, D // 2] = 0, float("nan"), float("inf"), float("-inf")
+    if r is not None:
+        r[7] = 0
+    total = x if r is None else (x.float() + r.float()).to(r.dtype)
+    q, scale, *more = f.rms_norm(x, w, r, eps=1e-5, quant=quant)
+    if r is not None:
+        assert torch.equal(more[0].isnan(), total.isnan()) and torch.equal(more[0].nan_to_num(), total.nan_to_num())
+    lost = torch.zeros(rows, dtype=torch.bool, device=gpu)
+    lost[[11, 12, 1029]] = True
+    assert torch.equal(scale.isnan(), lost)
+    if quant == torch.int8:
+        assert (q[lost] == 0).all()
+    else:
+        assert torch.equal(q.float().isnan().all(1), lost) and torch.equal(q.float().isnan().any(1), lost)
+    wide = total[~lost].double()
+    want = wide / torch.sqrt(wide.square().mean(-1, keepdim=True) + 1e-5) * w.double()
+    q, scale = q[~lost].double(), scale[~lost].double().unsqueeze(-1)
+    most = want.abs().amax(-1, keepdim=True)
+    assert ((scale - torch.where(most == 0, 1.0, most / limit)).abs() <= 64 * 2.0 ** -24 * scale).all()
+    step = torch.full_like(want, 0.5) if quant == torch.int8 else torch.maximum(want.abs() / scale / 16, torch.full_like(want, 2.0 ** -10))
+    assert ((q * scale - want).abs() <= step * scale * (1 + 1e-4)).all()
+    assert (q[want == 0] == 0).all() and (q.abs().amax(-1) == torch.where(most[:, 0] == 0, 0.0, limit)).all()

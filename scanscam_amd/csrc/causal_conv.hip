@@ -340,13 +340,13 @@ __global__ __launch_bounds__(256, 2) void conv_bwd_kernel(ConvArgs args)
 
 // A lane's vector of one row: the window moves on by a token. 512 rows of 2048 channels in bf16, K = 4: 6 us (17 MB, 2.7 TB/s), mostly a launch and
 // one trip to memory.
-template <typename ST, int K>
+template <typename ST, int K, bool PART>
 __global__ __launch_bounds__(256) void conv_step_kernel(StepPart<scanscam_conv_step> args)
 {
     const scanscam_conv_step &a = args.a;
     constexpr int VEC = 16 / sizeof(ST);
-    const int64_t c = ((int64_t)(args.block0 + blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
-    const int64_t row = args.row0 + (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int64_t c = ((int64_t)((PART ? args.block0 : 0) + blockIdx.y) * blockDim.x + threadIdx.x) * VEC;
+    const int64_t row = (PART ? args.row0 : 0) + (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (c >= a.channels || row >= a.rows) return;
     const int count = (int)clamp_(a.channels - c, 0, VEC);  // (no lane does another's work again here: the state is read and written in place)
     const int64_t slot = a.slot != nullptr ? index_at(a.slot, a.slot64, row) : row;
@@ -479,14 +479,14 @@ hipError_t run_conv(const ConvArgs &args, const ConvPlan &p, bool back, hipStrea
 template <typename ST> hipError_t run_step(const scanscam_conv_step &a, int64_t blocks, dim3 block, hipStream_t stream)
 {
     switch (a.K) {
-    case 1: return launch_step(conv_step_kernel<ST, 1>, a.rows, blocks, block, stream, a);
-    case 2: return launch_step(conv_step_kernel<ST, 2>, a.rows, blocks, block, stream, a);
-    case 3: return launch_step(conv_step_kernel<ST, 3>, a.rows, blocks, block, stream, a);
-    case 4: return launch_step(conv_step_kernel<ST, 4>, a.rows, blocks, block, stream, a);
-    case 5: return launch_step(conv_step_kernel<ST, 5>, a.rows, blocks, block, stream, a);
-    case 6: return launch_step(conv_step_kernel<ST, 6>, a.rows, blocks, block, stream, a);
-    case 7: return launch_step(conv_step_kernel<ST, 7>, a.rows, blocks, block, stream, a);
-    default: return launch_step(conv_step_kernel<ST, 8>, a.rows, blocks, block, stream, a);
+    case 1: return launch_step(conv_step_kernel<ST, 1, false>, conv_step_kernel<ST, 1, true>, a.rows, blocks, block, stream, a);
+    case 2: return launch_step(conv_step_kernel<ST, 2, false>, conv_step_kernel<ST, 2, true>, a.rows, blocks, block, stream, a);
+    case 3: return launch_step(conv_step_kernel<ST, 3, false>, conv_step_kernel<ST, 3, true>, a.rows, blocks, block, stream, a);
+    case 4: return launch_step(conv_step_kernel<ST, 4, false>, conv_step_kernel<ST, 4, true>, a.rows, blocks, block, stream, a);
+    case 5: return launch_step(conv_step_kernel<ST, 5, false>, conv_step_kernel<ST, 5, true>, a.rows, blocks, block, stream, a);
+    case 6: return launch_step(conv_step_kernel<ST, 6, false>, conv_step_kernel<ST, 6, true>, a.rows, blocks, block, stream, a);
+    case 7: return launch_step(conv_step_kernel<ST, 7, false>, conv_step_kernel<ST, 7, true>, a.rows, blocks, block, stream, a);
+    default: return launch_step(conv_step_kernel<ST, 8, false>, conv_step_kernel<ST, 8, true>, a.rows, blocks, block, stream, a);
     }
 }
 

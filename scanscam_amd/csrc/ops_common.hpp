@@ -200,15 +200,18 @@ template <typename Step> struct StepPart {
     int64_t row0;     // the first row of this launch
     uint32_t block0;  // and its first block of channels
 };
+// `whole` does what one launch can, `part` each of several.
 template <typename Kernel, typename Step>
-inline hipError_t launch_step(Kernel kernel, int64_t rows, int64_t blocks, dim3 block, hipStream_t stream, const Step &a)
+inline hipError_t launch_step(Kernel whole, Kernel part, int64_t rows, int64_t blocks, dim3 block, hipStream_t stream, const Step &a)
 {
     const int64_t most_rows = ((int64_t(1) << 32) / block.x - 1) * block.y, most_blocks = 32768;
+    if (rows <= most_rows && blocks <= most_blocks)
+        return launch_op(whole, dim3((unsigned)ceil_div(rows, block.y), (unsigned)blocks), block, 0, stream, StepPart<Step>{a, 0, 0});
     hipError_t err = hipSuccess;
     for (int64_t row = 0; row < rows; row += most_rows) {
         for (int64_t first = 0; first < blocks && err == hipSuccess; first += most_blocks) {
             const dim3 grid((unsigned)ceil_div(rows - row < most_rows ? rows - row : most_rows, block.y), (unsigned)(blocks - first < most_blocks ? blocks - first : most_blocks));
-            err = launch_op(kernel, grid, block, 0, stream, StepPart<Step>{a, row, (uint32_t)first});
+            err = launch_op(part, grid, block, 0, stream, StepPart<Step>{a, row, (uint32_t)first});
         }
     }
     return err;

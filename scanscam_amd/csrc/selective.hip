@@ -143,7 +143,7 @@ template <typename ST> hipError_t run_fwd(const scanscam_selective &a, hipStream
 {
     constexpr int K = kTokensALane;
     const Plan plan = forward_plan(a);
-    const SelectiveArgs args{a, plan.split, 1, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), 0, plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
+    const SelectiveArgs args{a, plan.split, 0, (uint32_t)forward_blocks(a, plan.split), each_of(a, plan.span), plan.span, static_cast<float *>(a.workspace), nullptr, nullptr};
     const int64_t units = all_units(a, plan.span);
     const int words = ForwardLds<K>::words(kFwdWaves / plan.split * kRows, (int)a.N);
     constexpr int most = ForwardLds<K>::words(kFwdWaves * kRows, kMostStates);
@@ -179,7 +179,7 @@ template <typename ST> hipError_t run_bwd(const scanscam_selective &a, hipStream
     const int sets = backward_sets(a);
     const int64_t blocks = backward_blocks(a), units = all_units(a, plan.span);
     float *ends = static_cast<float *>(a.workspace), *bc = ends + ends_words(a, plan.span), *sums = bc + bc_words(a);
-    const SelectiveArgs args{a, 1, sets, (uint32_t)blocks, each_of(a, plan.span), 0, plan.span, ends, bc, sums};
+    const SelectiveArgs args{a, sets, 0, (uint32_t)blocks, each_of(a, plan.span), plan.span, ends, bc, sums};
     const int words = BackwardLds<K>::words((int)a.N, sets);
     constexpr int one = BackwardLds<K>::words(kMostStates, 1), two = BackwardLds<K>::words(kStateBlock, kBwdMostSets), most = one > two ? one : two;
     hipError_t err = hipSuccess;
@@ -197,12 +197,12 @@ template <typename ST> hipError_t run_step(const scanscam_selective_step &a, hip
     while (lanes < 32 && lanes * 4 < a.N) lanes *= 2;
     const int64_t blocks = ceil_div(a.channels, 256 / lanes);
     switch (lanes) {
-    case 1: return launch_step(selective_step_kernel<ST, 1>, a.rows, blocks, dim3(256), stream, a);
-    case 2: return launch_step(selective_step_kernel<ST, 2>, a.rows, blocks, dim3(256), stream, a);
-    case 4: return launch_step(selective_step_kernel<ST, 4>, a.rows, blocks, dim3(256), stream, a);
-    case 8: return launch_step(selective_step_kernel<ST, 8>, a.rows, blocks, dim3(256), stream, a);
-    case 16: return launch_step(selective_step_kernel<ST, 16>, a.rows, blocks, dim3(256), stream, a);
-    default: return launch_step(selective_step_kernel<ST, 32>, a.rows, blocks, dim3(256), stream, a);
+    case 1: return launch_step(selective_step_kernel<ST, 1, false>, selective_step_kernel<ST, 1, true>, a.rows, blocks, dim3(256), stream, a);
+    case 2: return launch_step(selective_step_kernel<ST, 2, false>, selective_step_kernel<ST, 2, true>, a.rows, blocks, dim3(256), stream, a);
+    case 4: return launch_step(selective_step_kernel<ST, 4, false>, selective_step_kernel<ST, 4, true>, a.rows, blocks, dim3(256), stream, a);
+    case 8: return launch_step(selective_step_kernel<ST, 8, false>, selective_step_kernel<ST, 8, true>, a.rows, blocks, dim3(256), stream, a);
+    case 16: return launch_step(selective_step_kernel<ST, 16, false>, selective_step_kernel<ST, 16, true>, a.rows, blocks, dim3(256), stream, a);
+    default: return launch_step(selective_step_kernel<ST, 32, false>, selective_step_kernel<ST, 32, true>, a.rows, blocks, dim3(256), stream, a);
     }
 }
 

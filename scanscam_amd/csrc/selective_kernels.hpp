@@ -341,11 +341,10 @@ __device__ __forceinline__ void step_sizes(const Quad<ST> (&dt)[ITEMS], const fl
 
 struct SelectiveArgs {
     scanscam_selective a;
-    int split;        // forwards: waves that share the states of a channel out among them
-    int sets;         // backwards: sets of 16 channels that a workgroup takes
+    int share;        // forwards: waves that share the states of a channel out among them; backwards: sets of 16 channels that a workgroup takes
+    uint32_t unit0;   // the first part of this launch's
     uint32_t blocks;  // of channels, in a group
     uint32_t each;    // parts of a sequence where all are of one length
-    uint32_t unit0;   // the first part of this launch's
     int64_t span;     // tokens of a part of a sequence
     float *ends;      // [parts of all sequences][N + 1][channels]: the states that a part alone ends with (backwards: starts with), its sum of d
     float *bc;        // backwards: [blocks of all groups][tokens][2][N], sums of gB and gC over a workgroup's channels
@@ -431,7 +430,7 @@ __global__ __launch_bounds__(kFwdWaves * 64, 4) void selective_fwd_kernel(Select
     constexpr int TILE = G::kTile, P = G::kPitch;
     constexpr int kThreads = kFwdWaves * 64, kItems = kFwdWaves * TILE / kThreads;  // groups of 4 channels x tokens, a thread
     const scanscam_selective &a = args.a;
-    const int N = (int)a.N, split = args.split, sets = kFwdWaves / split, channels = sets * kRows;
+    const int N = (int)a.N, split = args.share, sets = kFwdWaves / split, channels = sets * kRows;
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *ly = lu + channels * P, *lB = ly + kFwdWaves * kRows * P, *lC = lB + kStateBlock * P;
     float *lskip = lC + kStateBlock * P;
@@ -673,7 +672,7 @@ __global__ __launch_bounds__(kBwdWaves * 64, 2) void selective_bwd_kernel(Select
     constexpr int TILE = G::kTile, P = G::kPitch, channels = kBwdChannels;
     constexpr int kThreads = kBwdWaves * 64, kItems = kBwdWaves * TILE / kThreads;
     const scanscam_selective &a = args.a;
-    const int N = (int)a.N, wide = args.sets * channels, slots = wide * BackwardLds<K>::padded(N);  // wide: all channels of the workgroup
+    const int N = (int)a.N, wide = args.share * channels, slots = wide * BackwardLds<K>::padded(N);  // wide: all channels of the workgroup
     extern __shared__ float lds[];
     float *ld = lds, *lu = ld + channels * P, *lg = lu + channels * P;
     float *l1 = lg + channels * P, *l2 = l1 + channels * P, *lv = l2 + channels * P;
@@ -1086,12 +1085,13 @@ __global__ __launch_bounds__(256) void selective_bc_kernel(GroupSum args)
 // all there is, in one piece; everything is asked for before any of it is used. 512 rows of 2048 channels, N = 16, bf16: 29 us for 143 MB,
 // 4.9 TB/s. One row: 4 us, which are a launch and one trip to memory.
 // ---------------------------------------------------------------------------------------------------------------------------
-template <typename ST, int LANES>
+// (PART: one of several launches, whose place only they look up: 29.3 us where all did, 28.8 so.)
+template <typename ST, int LANES, bool PART>
 __global__ __launch_bounds__(256) void selective_step_kernel(StepPart<scanscam_selective_step> args)
 {
     const scanscam_selective_step &a = args.a;
     const int lane = threadIdx.x % LANES, N = (int)a.N;
-    const int64_t c = (int64_t)(args.block0 + blockIdx.y) * (256 / LANES) + threadIdx.x / LANES, row = args.row0 + blockIdx.x;
+    const int64_t c = (int64_t)((PART ? args.block0 : 0) + blockIdx.y) * (256 / LANES) + threadIdx.x / LANES, row = (PART ? args.row0 : 0) + blockIdx.x;
     const int64_t slot = a.slot != nullptr ? index_at(a.slot, a.slot64, row) : row;
     const bool there = c < a.channels;
     if (slot < 0 || slot >= a.slots) {

@@ -17,6 +17,7 @@ import sys
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import baseline, hip
 
@@ -149,8 +150,7 @@ def _eager(fn, *args, **kwargs):
 _eager._torchdynamo_disable = True  # (what torch.compiler.disable marks, without its import of the compiler)
 
 
-def _compiling(x: torch.Tensor) -> bool:
-    return torch.compiler.is_dynamo_compiling() and x.device.type == "cuda"
+_traced_through = torch.compiler.is_dynamo_compiling
 
 
 # --------------------------------------------------------------------------------------------------------- checks of arguments
@@ -295,7 +295,9 @@ def _wants_grad(*tensors) -> bool:
 def _has_tangent(*tensors) -> bool:
     """Whether a forward-mode derivative is asked for, which no kernel here has: calls with gradients go through their autograd
     function, which refuses it as scan()'s does, and the others refuse it themselves. (The CPU's loops have them.)"""
-    return any(t is not None and t.device.type == "cuda" and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if getattr(forward_ad, "_current_level", 0) < 0:  # (no call under dual_level() is under way: unpack_dual() would look there first)
+        return False
+    return any(t is not None and t.device.type == "cuda" and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _needs_node(*tensors) -> bool:
@@ -324,9 +326,10 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     :param return_state: hand back the states after the last tokens as well, in float32
     :return: y, or ``(y, state)``. Differentiable in every tensor but ``offsets``.
     """
-    if _compiling(x):
-        return _eager(selective_scan, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, state=state, offsets=offsets, return_state=return_state)
-    if _native is not None and _parts == 0:
+    if _traced_through():
+        if x.device.type == "cuda":
+            return _eager(selective_scan, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, state=state, offsets=offsets, return_state=return_state)
+    elif _native is not None and _parts == 0:
         out = _native.selective(x, dt, A, B, C, D, z, dt_bias, softplus, state, offsets, return_state)  # None: a call it leaves to the code below
         if out is not None:
             return out
@@ -449,9 +452,10 @@ def selective_scan_step(state: torch.Tensor, x: torch.Tensor, dt: torch.Tensor, 
         slot is not in ``state``, such as -1, is left out: its output is zero and no state changes.
     :return: y, [rows, channels]. Not differentiable.
     """
-    if _compiling(x):
-        return _eager(selective_scan_step, state, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, slots=slots)
-    if _native is not None:
+    if _traced_through():
+        if x.device.type == "cuda":
+            return _eager(selective_scan_step, state, x, dt, A, B, C, D, z, dt_bias, softplus=softplus, slots=slots)
+    elif _native is not None:
         out = _native.selective_step(state, x, dt, A, B, C, D, z, dt_bias, softplus, slots)
         if out is not None:
             return out
@@ -525,9 +529,10 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     :param return_state: hand back the K - 1 inputs before the next token as well
     :return: y, or ``(y, state)``. Differentiable in every tensor but ``offsets``.
     """
-    if _compiling(x):
-        return _eager(causal_conv, x, weight, bias, activation=activation, state=state, offsets=offsets, return_state=return_state)
-    if _native is not None:
+    if _traced_through():
+        if x.device.type == "cuda":
+            return _eager(causal_conv, x, weight, bias, activation=activation, state=state, offsets=offsets, return_state=return_state)
+    elif _native is not None:
         out = _native.conv(x, weight, bias, activation, state, offsets, return_state)
         if out is not None:
             return out
@@ -622,9 +627,10 @@ def causal_conv_step(state: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
     :param x: [rows, channels]; weight, bias, activation as for ``causal_conv``; slots as for ``selective_scan_step``
     :return: y, [rows, channels]. Not differentiable.
     """
-    if _compiling(x):
-        return _eager(causal_conv_step, state, x, weight, bias, activation=activation, slots=slots)
-    if _native is not None:
+    if _traced_through():
+        if x.device.type == "cuda":
+            return _eager(causal_conv_step, state, x, weight, bias, activation=activation, slots=slots)
+    elif _native is not None:
         out = _native.conv_step(state, x, weight, bias, activation, slots)
         if out is not None:
             return out
@@ -689,9 +695,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     :return: y; with a residual ``(y, sum)``; with ``quant`` ``(q, scale)`` or ``(q, scale, sum)``, scale being float32 and of x's
         leading shape. Differentiable (in x, weight and residual) unless ``quant`` is given.
     """
-    if _compiling(x):
-        return _eager(rms_norm, x, weight, residual, eps=eps, quant=quant)
-    if _native is not None:
+    if _traced_through():
+        if x.device.type == "cuda":
+            return _eager(rms_norm, x, weight, residual, eps=eps, quant=quant)
+    elif _native is not None:
         out = _native.norm(x, weight, residual, eps, _EIGHT.get(quant, -1) if quant is not None else 0)
         if out is not None:
             return out

@@ -157,7 +157,8 @@ int scanscam_conv_step_fwd(const scanscam_conv_step *args, void *stream);
  *     y = sum * rstd * weight,  rstd = 1 / sqrt(mean(sum^2) + eps)
  * What is stored in `sum` is what is normalised, so that the backward call, which has only that, gives the gradient of
  * what was computed. With out_dtype SCANSCAM_I8 or SCANSCAM_F8 a row is stored in 8 bits: scale = max |y| / 127 or / 448
- * (1 where the row is zero) and y / scale, rounded to nearest even. Up to 32768 channels.
+ * (1 where the row is zero) and y / scale, rounded to nearest even; a row that holds a NaN or an infinity has the scale NaN (its integers are 0).
+ * Rows whose squares add up to more than fp32 holds (values of some 1e19) come out as zeros, as rstd does. Up to 32768 channels.
  */
 typedef struct scanscam_norm {
     int64_t rows, channels;

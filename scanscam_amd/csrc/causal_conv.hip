@@ -8,7 +8,7 @@
 // the border of two stretches, which the caches still hold. A lane whose vector would reach past the last channel takes
 // the last whole one instead and does some of its neighbour's work again, the same (fewer channels than a vector's go
 // element by element); tokens are asked for several at a time, as one token's latency is longer than its arithmetic. [8, 4096, 2048] in bf16
-// with K = 4: 53 us forwards (268 MB, 5.1 TB/s). 8021 packed tokens: 20 us (66 MB, 3.4 TB/s), where a wave's stretch of 8 tokens is a search for
+// with K = 4: 53 us forwards (268 MB, 5.1 TB/s). 8021 packed tokens, 66 MB: 26 us from memory, 20 from the caches, where a wave's stretch of 8 tokens is a search for
 // its sequence and three trips to memory; with the first tokens asked for before the search it took 23, with two groups under way
 // at once 24: both cost registers and so waves.
 #include "ops_common.hpp"
@@ -338,8 +338,9 @@ __global__ __launch_bounds__(256, 2) void conv_bwd_kernel(ConvArgs args)
     }
 }
 
-// A lane's vector of one row: the window moves on by a token. 512 rows of 2048 channels in bf16, K = 4: 6 us (17 MB, 2.7 TB/s), mostly a launch and
-// one trip to memory.
+// A lane's vector of one row: the window moves on by a token. 512 rows of 2048 channels in bf16, K = 4, 17 MB: 7 us where other
+// states are stepped in between, 6 where the same ones are and stay in the caches; mostly a launch and one trip to memory.
+// (PART: one of several launches, whose place only they look up.)
 template <typename ST, int K, bool PART>
 __global__ __launch_bounds__(256) void conv_step_kernel(StepPart<scanscam_conv_step> args)
 {

@@ -87,7 +87,7 @@ int backward_sets(const scanscam_selective &a)
 }
 int64_t backward_blocks(const scanscam_selective &a) { return ceil_div(a.channels / a.groups, kBwdChannels * backward_sets(a)); }
 
-// Parts of one length for about two workgroups a CU, whole tiles each.
+// Parts of one length for about two workgroups a CU, whole tiles each. (Known at N = 16; from N = 40 on a CU holds one.)
 int64_t span_for(const scanscam_selective &a, int64_t blocks, int64_t shortest)
 {
     const int64_t tiles = (a.offsets != nullptr ? 1 : a.sequences) * ceil_div(a.T, kTile) * a.groups * blocks, each = ceil_div(tiles, 512);
@@ -101,7 +101,7 @@ int64_t span_of(const scanscam_selective &a)
     return (each > 0 ? each : 1) * kTile;
 }
 
-// Two workgroups fit a CU, and one keeps it nearly as busy, so that from 192 workgroups on nothing is cut. Below, sharing the states
+// Two workgroups fit a CU (one from N = 40 on; all figures here are of N = 16), and one keeps it nearly as busy, so that from 192 workgroups on nothing is cut. Below, sharing the states
 // of a channel out costs less than parts of time, whose first pass repeats most of the arithmetic, as long as it is two waves
 // (bf16, N = 16, us: [4, 2048, 1024] 120 whole, 83 by two waves, 92 in 4 parts; [6, 2048, 1024] 117, 113, 134); four
 // or eight waves have too little to do for the tokens' own work and the barriers, so that with fewer channels parts win where there are

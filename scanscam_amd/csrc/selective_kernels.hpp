@@ -416,7 +416,8 @@ constexpr int kFwdWaves = 8;
 template <int K> struct ForwardLds {
     using G = Geometry<K>;
     static constexpr int kSums = kFwdWaves * kRows;  // channels x split: rows of sums over n
-    // floats: d and u of the channels, sums, B and C; D; A and the carries of all states; where lanes write that have nothing to say
+    // floats: d and u of the channels, sums, B and C; D; A and the carries of all states; where lanes write that have nothing to say. (Of 32
+    // channels 76 KB at N = 16, two workgroups a CU up to N = 39, one from 40 on: [8, 4096, 2048] in bf16 takes 621 us at N = 32, 973 at 40.)
     static __host__ __device__ constexpr int words(int channels, int N)
     {
         return 2 * channels * G::kPitch + kSums * G::kPitch + 2 * kStateBlock * G::kPitch + channels + 2 * channels * N + 2;
@@ -654,7 +655,8 @@ constexpr int kBwdMostSets = 2;  // of 16 channels
 
 template <int K> struct BackwardLds {
     using G = Geometry<K>;
-    // d, u, g0 and s1, s2, v; B and C; A, the gradients' carries and the sums for A; a block's states; bias, D and the sums for them
+    // d, u, g0 and s1, s2, v; B and C; A, the gradients' carries and the sums for A; a block's states; bias, D and the sums for them. (Two
+    // workgroups a CU up to N = 40.)
     static __host__ __device__ constexpr int words(int N, int sets)
     {
         return 6 * kBwdChannels * G::kPitch + 2 * kStateBlock * G::kPitch + 3 * sets * kBwdChannels * padded(N) + kBwdChannels * kStateBlock +
@@ -1082,8 +1084,9 @@ __global__ __launch_bounds__(256) void selective_bc_kernel(GroupSum args)
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // One token: LANES lanes a channel, each with 4 neighbouring states at a time, so that a wave reads and writes the states, which are nearly
-// all there is, in one piece; everything is asked for before any of it is used. 512 rows of 2048 channels, N = 16, bf16: 29 us for 143 MB,
-// 4.9 TB/s. One row: 4 us, which are a launch and one trip to memory.
+// all there is, in one piece; everything is asked for before any of it is used. 512 rows of 2048 channels, N = 16, bf16, 143 MB: 44 us, 3.2 TB/s,
+// where other states are stepped in between; 29 us where the same 67 MB of states are stepped again, which stay in the card's cache of 256 MB.
+// One row: 3 us, which are a launch and one trip to memory.
 // ---------------------------------------------------------------------------------------------------------------------------
 // (PART: one of several launches, whose place only they look up: 29.3 us where all did, 28.8 so.)
 template <typename ST, int LANES, bool PART>

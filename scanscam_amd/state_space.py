@@ -9,7 +9,9 @@ element whose tokens belong to sequence ``s`` from ``offsets[s]`` up to ``offset
 more than there are sequences, on the same device, from 0 to T, not decreasing; it is not looked at on the host).
 
 GPU tensors run the kernels of ``libscanscam_hip.so`` (C ABI in ``include/scanscam_ops.h``) on the current stream and nothing
-else; CPU tensors take the loops of ``scanscam_amd.baseline``. None of this has a counterpart in the reference, whose one
+else, up to 2^20 channels and 2^31 - 2^20 tokens, rows or sequences a call; CPU tensors take the loops of ``scanscam_amd.baseline``. Calls can be recorded by
+``torch.jit.trace`` and by graphs, and made from functions under ``torch.compile``, whose graph they break; ``make_fx`` and forward-mode derivatives
+are refused on the GPU. None of this has a counterpart in the reference, whose one
 operator is the scan.
 """
 import ctypes
@@ -687,7 +689,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
         sum = x + residual                     (in the residual's type; x itself without one)
         y = sum / sqrt(mean(sum^2) + eps) * weight
 
-    What is stored in ``sum`` is what is normalised, so the gradient is that of what was computed.
+    What is stored in ``sum`` is what is normalised, so the gradient is that of what was computed. Squares are added up in float32: rows of values
+    past some 1e19 come out as zeros.
 
     :param x: [..., channels], up to 32768 channels; residual: of the same shape and any supported type; weight: [channels]
     :param quant: None, ``torch.int8`` or ``torch.float8_e4m3fn``: y in 8 bits with a scale a row, ``scale = max |y| / 127`` or

@@ -6,7 +6,7 @@ This is the package's counterpart of the reference's ``scanscam/baseline.py:8-40
 It is differentiable by ``torch.autograd``. GPU tensors never come here: they
 go to the HIP kernels or raise.
 
-Below it are the operators of a state space layer (``scanscam_amd.state_space``) in
+Below it are the operators of state space and linear attention layers (``scanscam_amd.state_space``, ``scanscam_amd.attention``) in
 the same manner: loops over time on tensors, differentiable by ``torch.autograd``,
 in float64 where the inputs are and in float32 otherwise, rounded once at the end.
 """
@@ -145,3 +145,47 @@ def naive_rms_norm(x, weight, residual=None, *, eps=1e-6, quant=None):
     q = (y / scale.unsqueeze(-1)).clamp(-limit, limit)
     q = q.round().to(quant) if quant == torch.int8 else q.to(quant)
     return (q, scale) if residual is None else (q, scale, total)
+
+
+def naive_linear_attention(q, k, v, decay=None, *, scale=1.0, state=None, offsets=None, return_state=False):
+    heads, each = v.shape[2], v.shape[2] // q.shape[2]
+    wq, wk, wv = _wide(q).repeat_interleave(each, dim=2) * scale, _wide(k).repeat_interleave(each, dim=2), _wide(v)
+    gate = None if decay is None else torch.exp(_wide(decay)).expand(*v.shape[:3])
+    outs, states = [], []
+    for s, (b, start, end) in enumerate(_sequences(v, offsets)):
+        h = _wide(state[s]) if state is not None else wv.new_zeros((heads, q.shape[3], v.shape[3]))
+        ys = []
+        for t in range(start, end):
+            h = h if gate is None else gate[b, t, :, None, None] * h
+            h = h + wk[b, t, :, :, None] * wv[b, t, :, None, :]
+            ys.append((wq[b, t, :, :, None] * h).sum(-2))
+        outs.append(torch.stack(ys) if ys else wv[b, :0])
+        states.append(h)
+    y = _join(outs, offsets, v)
+    return (y, torch.stack(states) if states else wv.new_empty((0, heads, q.shape[3], v.shape[3]))) if return_state else y
+
+
+def naive_linear_attention_step(state, q, k, v, decay=None, *, scale=1.0, slots=None):
+    y = torch.zeros_like(v)
+    for i, s in _rows_of(slots, v.shape[0], state.shape[0]):
+        gate = decay if decay is None or decay.dim() == 1 else decay[i][None, None]
+        out, new = naive_linear_attention(q[i][None, None], k[i][None, None], v[i][None, None], gate, scale=scale, state=state[s][None], return_state=True)
+        y[i], state[s] = out[0, 0], new[0]
+    return y
+
+
+def naive_group_norm(x, groups, weight=None, bias=None, z=None, *, eps=1e-5, activation=None):
+    if x.numel() == 0:
+        return x * 1 if z is None else x * z
+    wide = _wide(x).unflatten(-1, (groups, -1))
+    wide = wide - wide.mean(-1, keepdim=True)
+    y = (wide * torch.rsqrt((wide * wide).mean(-1, keepdim=True) + eps)).flatten(-2)
+    if weight is not None:
+        y = y * _wide(weight)
+    if bias is not None:
+        y = y + _wide(bias)
+    if activation == "silu":
+        y = silu(y)
+    if z is not None:
+        y = y * silu(_wide(z))
+    return y.to(x.dtype)

@@ -1,0 +1,409 @@
+// C ABI of linear attention (declared in include/scanscam_attention.h): argument checks, launch shapes, launches; single tokens' steps; and the
+// kernels whose work does not depend on the activations' type.
+#include "linear_attention_kernels.hpp"
+
+namespace scanscam {
+
+// The states that parts start from, out of what each adds: in the parts' order, or from the last part on (gradients).
+struct Joined {
+    float *ends;
+    const double *logs;
+    const float *from;  // [pairs][values], or NULL
+    int64_t pairs, pair0;
+    int32_t parts, values, back;
+};
+__global__ __launch_bounds__(256) void join_kernel(Joined a)
+{
+    const int at = blockIdx.y * 256 + threadIdx.x;
+    const int64_t pair = a.pair0 + blockIdx.x;
+    if (at >= a.values) return;
+    float run = a.from == nullptr ? 0.0f : a.from[pair * a.values + at];
+    for (int i = 0; i < a.parts; i++) {
+        const int64_t unit = pair * a.parts + (a.back ? a.parts - 1 - i : i);
+        float *p = a.ends + unit * a.values + at;
+        const float adds = i + 1 < a.parts ? *p : 0.0f;  // (the last one's was not computed)
+        *p = run;
+        if (i + 1 < a.parts) run = run * exp2_(a.logs[unit]) + adds;
+    }
+}
+
+// Gradients of decays out of what every token reads and writes (the formula is in linear_attention_kernels.hpp). A workgroup takes the chunks
+// between two borders, a wave each, backwards from the later one's product of state and gradient.
+template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(AttendArgs args)
+{
+    const scanscam_attend &a = args.a;
+    AttendArgs whole = args;
+    whole.parts = 1;
+    const Span span = span_of(whole, args.first + blockIdx.x, C);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ double over[kBorder];
+    const int64_t chunks = (span.length + C - 1) / C, base = span.head * args.tokens + span.batch * a.T;
+    for (int64_t first = (int64_t)blockIdx.y * kBorder; first < chunks; first += (int64_t)gridDim.y * kBorder) {
+        const int64_t c = first + kBorder - 1 - wave, t = span.begin + c * C + lane;
+        const bool there = lane < C && t < span.end;
+        const double read = there ? args.reads[base + t] : 0.0, write = there ? args.writes[base + t] : 0.0;
+        const double reads = sums_upto(read), writes = sums_upto(write), all_reads = read_lane(reads, 63), all_writes = read_lane(writes, 63);
+        if (lane == 0) over[wave] = all_reads - all_writes;
+        __syncthreads();
+        double end = first + kBorder < chunks ? args.cross[border_at(args, span.batch, span.from + (first + kBorder) * C, C, span.head)] : args.last[span.unit];
+        for (int w = 0; w < wave; w++) end += over[w];
+        if (there) args.decays[(span.batch * a.T + t) * a.heads + span.head] = (float)((end - all_writes) + (all_reads - reads + read) + (writes - write));
+        __syncthreads();
+    }
+}
+
+// Gradients of shared queries or keys: over the heads that share them, in order.
+struct Shared {
+    const float *part;  // [tokens][heads][K]
+    scanscam_tokens out;
+    int64_t tokens, T, token0;
+    int32_t heads, each, K, dtype;
+};
+template <typename ST> __global__ __launch_bounds__(256) void shared_kernel(Shared a)
+{
+    const int fours = (a.K + 3) / 4, groups = a.heads / a.each, row = groups * fours;
+    const int64_t index = (int64_t)blockIdx.x * 256 + threadIdx.x, token = a.token0 + index / row;
+    if (token >= a.tokens) return;
+    const int rest = (int)(index % row), group = rest / fours, at = rest % fours * 4, count = a.K - at;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float *p = a.part + (token * a.heads + (int64_t)group * a.each) * a.K + at;
+    for (int h = 0; h < a.each; h++, p += a.K) {
+        float f[4];
+        load_part<float, 4>(p, count, f);
+#pragma unroll
+        for (int r = 0; r < 4; r++) sum[r] += f[r];
+    }
+    store_some<ST, 4>(static_cast<ST *>(a.out.p) + token / a.T * a.out.batch + token % a.T * a.out.token + group * a.out.group + at, count, sum);
+}
+
+// One token: S = e^g S + k v^T, y = scale S^T q. Memory bounds it, the states read and written. A workgroup takes `width` columns of a head's
+// state; `lanes` lanes hold four columns each, and rows go round the workgroup, eight under way at once.
+struct StepArgs {
+    scanscam_attend_step a;
+    int32_t lanes, pieces, each;
+    int64_t first;
+};
+template <typename ST> __global__ __launch_bounds__(256) void attend_step_kernel(StepArgs args)
+{
+    const scanscam_attend_step &a = args.a;
+    __shared__ float keys[256], queries[256];
+    __shared__ __attribute__((aligned(16))) float4v sums[256];
+    const int64_t unit = args.first + blockIdx.x, row = unit / args.pieces / a.heads;
+    const int piece = (int)(unit % args.pieces), head = (int)(unit / args.pieces % a.heads), shared = head / args.each;
+    const int K = (int)a.K, V = (int)a.V, lane = threadIdx.x % args.lanes, row0 = threadIdx.x / args.lanes, stride = 256 / args.lanes;
+    const int col = (piece * args.lanes + lane) * 4, count = V - col;
+    const int64_t slot = a.slot == nullptr ? row : index_at(a.slot, a.slot64, row);
+    ST *y = static_cast<ST *>(a.y.p) + row * a.y.token + head * a.y.group + col;
+    if (slot < 0 || slot >= a.slots) {
+        const float zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (row0 == 0 && count > 0) store_some<ST, 4>(y, count, zeros);
+        return;
+    }
+    float *state = a.state + (slot * a.heads + head) * (int64_t)K * V + col;
+    constexpr int UNROLL = 8;
+    float4v s[UNROLL];
+    const auto ask = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const int i = i0 + u * stride;
+            float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (i < K && count > 0) load_part<float, 4>(state + i * V, count, f);
+            s[u] = float4v{f[0], f[1], f[2], f[3]};
+        }
+    };
+    ask(row0);
+    if ((int)threadIdx.x < K) {
+        keys[threadIdx.x] = (float)static_cast<const ST *>(a.k.p)[row * a.k.token + shared * a.k.group + threadIdx.x];
+        queries[threadIdx.x] = (float)static_cast<const ST *>(a.q.p)[row * a.q.token + shared * a.q.group + threadIdx.x];
+    }
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (count > 0) load_part<ST, 4>(static_cast<const ST *>(a.v.p) + row * a.v.token + head * a.v.group + col, count, v);
+    const float g = a.decay.p == nullptr ? 0.0f : param(scanscam_param{a.decay.p, a.decay_dtype, 0}, row * a.decay.token + head);
+    const float decay = __builtin_amdgcn_exp2f((float)((double)g * 1.4426950408889634074));
+    __syncthreads();
+    float4v sum{0, 0, 0, 0};
+    for (int i0 = row0; i0 < K; i0 += UNROLL * stride) {
+        if (i0 != row0) ask(i0);
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const int i = i0 + u * stride;
+            if (i >= K) continue;
+            const float k = keys[i], q = queries[i];
+            float f[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                f[r] = __builtin_fmaf(decay, s[u][r], k * v[r]);
+                sum[r] = __builtin_fmaf(q, f[r], sum[r]);
+            }
+            if (count > 0) store_some<float, 4>(state + i * V, count, f);
+        }
+    }
+    sums[threadIdx.x] = sum;
+    for (int half = stride / 2; half > 0; half /= 2) {  // (both are powers of two)
+        __syncthreads();
+        if (row0 < half) sums[threadIdx.x] = sum = sum + sums[threadIdx.x + half * args.lanes];
+    }
+    if (row0 == 0 && count > 0) {
+        const float out[4] = {sum[0] * a.scale, sum[1] * a.scale, sum[2] * a.scale, sum[3] * a.scale};
+        store_some<ST, 4>(y, count, out);
+    }
+}
+
+}  // namespace scanscam
+
+namespace {
+
+using namespace scanscam;
+
+int check_near(const scanscam_tokens &t, int size)
+{
+    SCANSCAM_CHECK(check_tokens(t, size));
+    return t.token >= SCANSCAM_MOST_TOKEN_STRIDE ? SCANSCAM_EINVAL : SCANSCAM_OK;
+}
+
+int check_heads(int64_t heads, int64_t groups, int64_t K, int64_t V, int dtype, const scanscam_tokens &decay, int decay_dtype)
+{
+    if (heads < 0 || groups < 1 || heads % groups != 0 || K < 1 || K > SCANSCAM_MOST_HEAD || V < 1 || V > SCANSCAM_MOST_HEAD) return SCANSCAM_EINVAL;
+    if (heads * (K > V ? K : V) > kMostChannels) return SCANSCAM_EINVAL;
+    if (activation_size(dtype) == 0) return SCANSCAM_EDTYPE;
+    if (decay.p == nullptr) return SCANSCAM_OK;
+    if (activation_size(decay_dtype) == 0) return SCANSCAM_EDTYPE;
+    return check_tokens(decay, activation_size(decay_dtype));
+}
+
+constexpr int64_t kAttendMostParts = 1024;
+
+// `back`: also what a backward call reads and writes.
+int check_attend(const scanscam_attend *a, bool back)
+{
+    if (a == nullptr) return SCANSCAM_EINVAL;
+    if (a->batch < 0 || a->T < 0 || a->T >= kMostTokens || a->sequences < 0 || a->sequences >= kMostTokens || a->parts < 0 || a->parts > kAttendMostParts) return SCANSCAM_EINVAL;
+    if (a->offsets != nullptr ? a->batch != 1 || a->sequences < 1 : a->sequences != a->batch) return SCANSCAM_EINVAL;
+    if (a->batch > 0 && a->T > (kMostTokens - 1) / a->batch) return SCANSCAM_EINVAL;
+    SCANSCAM_CHECK(check_heads(a->heads, a->groups, a->K, a->V, a->dtype, a->decay, a->decay_dtype));
+    if (misaligned(a->offsets, a->offsets64 ? 8 : 4)) return SCANSCAM_EALIGN;
+    for (const void *p : {(const void *)a->state_in, (const void *)a->state_out, (const void *)a->gdecay, (const void *)a->gstate_out, (const void *)a->gstate_in})
+        if (misaligned(p, 4)) return SCANSCAM_EALIGN;
+    if (a->batch * a->T == 0 || a->heads == 0) return SCANSCAM_OK;
+    const int size = activation_size(a->dtype);
+    for (const scanscam_tokens *t : {&a->q, &a->k, &a->v}) SCANSCAM_CHECK(check_near(*t, size));
+    if (!back) return check_tokens(a->y, size);
+    SCANSCAM_CHECK(check_near(a->gy, size));
+    for (const scanscam_tokens *t : {&a->gq, &a->gk, &a->gv}) SCANSCAM_CHECK(check_tokens(*t, size));
+    return SCANSCAM_OK;
+}
+
+int chunk_of(const scanscam_attend &a) { return a.dtype == SCANSCAM_F32 ? Operand<float>::CHUNK : Operand<__bf16>::CHUNK; }
+
+int parts_of(const scanscam_attend &a)
+{
+    if (a.parts > 0) return a.parts;
+    const int64_t pairs = a.sequences * a.heads, chunks = ceil_div(a.T, chunk_of(a));
+    if (pairs == 0 || pairs >= 256) return 1;
+    int64_t parts = 512 / pairs;
+    parts = parts < chunks / 4 ? parts : chunks / 4;
+    return parts < 2 ? 1 : (int)parts;
+}
+
+// What the workspace holds, in order; each piece begins on 16 bytes.
+struct Pieces {
+    size_t ends, back_ends, logs, reads, writes, last, borders, cross, part_q, part_k, decays, bytes;
+    int64_t most_borders;
+};
+Pieces pieces_of(const scanscam_attend &a, bool back, int parts)
+{
+    Pieces p{};
+    const auto take = [&](bool there, int64_t count, size_t size) {
+        const size_t at = p.bytes;
+        if (there) p.bytes += ((size_t)count * size + 15) / 16 * 16;
+        return at;
+    };
+    const int64_t pairs = a.sequences * a.heads, values = pairs * parts * a.K * a.V, tokens = a.batch * a.T;
+    p.ends = take(parts > 1, values, 4);
+    p.logs = take(parts > 1, pairs * parts, 8);
+    if (!back) return p;
+    p.back_ends = take(parts > 1, values, 4);
+    p.reads = take(true, tokens * a.heads, 4);
+    p.writes = take(true, tokens * a.heads, 4);
+    p.last = take(true, pairs, 8);
+    p.most_borders = a.T / (kBorder * chunk_of(a)) + 1;
+    const int64_t borders = a.T > kBorder * chunk_of(a) ? a.batch * p.most_borders * a.heads : 0, width = attend_width(a);
+    p.borders = take(borders > 0, borders * width * width, 4);
+    p.cross = take(borders > 0, borders, 8);
+    p.part_q = take(a.groups < a.heads, tokens * a.heads * a.K, 4);
+    p.part_k = take(a.groups < a.heads, tokens * a.heads * a.K, 4);
+    p.decays = take(a.decay_fixed != 0, tokens * a.heads, 4);
+    return p;
+}
+
+hipError_t run(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
+{
+    switch (args.a.dtype) {
+    case SCANSCAM_F32: return launch_attend<float>(pass, units, stream, args);
+    case SCANSCAM_BF16: return launch_attend<__bf16>(pass, units, stream, args);
+    default: return launch_attend<_Float16>(pass, units, stream, args);
+    }
+}
+
+// The states that parts start from.
+hipError_t starts(const AttendArgs &args, bool back, hipStream_t stream)
+{
+    const scanscam_attend &a = args.a;
+    const int64_t pairs = a.sequences * a.heads;
+    hipError_t err = run(back ? kBackEnds : kEnds, pairs * args.parts, stream, args);
+    Joined j{back ? args.back_ends : args.ends, args.logs, back ? a.gstate_out : a.state_in, pairs, 0, args.parts, (int32_t)(a.K * a.V), back};
+    constexpr int64_t most = 1 << 22;
+    for (; j.pair0 < pairs && err == hipSuccess; j.pair0 += most)
+        err = launch_op(join_kernel, dim3((unsigned)(pairs - j.pair0 < most ? pairs - j.pair0 : most), (unsigned)ceil_div(a.K * a.V, 256)), dim3(256), 0, stream, j);
+    return err;
+}
+
+template <typename ST> hipError_t join_shared(Shared s, hipStream_t stream)
+{
+    const int64_t row = (int64_t)(s.heads / s.each) * ceil_div(s.K, 4), most = (int64_t(1) << 31) / row;
+    const int64_t all = s.tokens;
+    hipError_t err = hipSuccess;
+    for (; s.token0 < all && err == hipSuccess; s.token0 += most) {
+        const int64_t now = all - s.token0 < most ? all - s.token0 : most;
+        s.tokens = s.token0 + now;
+        err = launch_op(shared_kernel<ST>, dim3((unsigned)ceil_div(now * row, 256)), dim3(256), 0, stream, s);
+    }
+    return err;
+}
+
+template <typename ST> hipError_t launch_attend_step(const StepArgs &step, hipStream_t stream)
+{
+    StepArgs args = step;
+    const int64_t units = args.a.rows * args.a.heads * args.pieces, most = (int64_t(1) << 32) / 256 - 1;
+    hipError_t err = hipSuccess;
+    for (args.first = 0; args.first < units && err == hipSuccess; args.first += most)
+        err = launch_op(attend_step_kernel<ST>, dim3((unsigned)(units - args.first < most ? units - args.first : most)), dim3(256), 0, stream, args);
+    return err;
+}
+
+int code(hipError_t err) { return err == hipSuccess ? SCANSCAM_OK : SCANSCAM_ELAUNCH; }
+
+bool sizes_fit(const scanscam_attend *a)
+{
+    return a != nullptr && a->batch >= 0 && a->T >= 0 && a->T < kMostTokens && a->sequences >= 0 && a->sequences < kMostTokens && a->parts >= 0 && a->parts <= kAttendMostParts &&
+           (a->batch == 0 || a->T <= (kMostTokens - 1) / a->batch) && check_heads(a->heads, a->groups, a->K, a->V, a->dtype, scanscam_tokens{}, 0) == SCANSCAM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t scanscam_attend_workspace_bytes(const scanscam_attend *a, int direction)
+{
+    return sizes_fit(a) ? pieces_of(*a, direction == SCANSCAM_BACKWARD, parts_of(*a)).bytes : 0;
+}
+
+int scanscam_attend_fwd(const scanscam_attend *a, void *stream)
+{
+    SCANSCAM_CHECK(check_attend(a, false));
+    if (a->sequences == 0 || a->heads == 0 || (a->batch * a->T == 0 && a->state_out == nullptr)) return SCANSCAM_OK;
+    const int parts = parts_of(*a);
+    const Pieces at = pieces_of(*a, false, parts);
+    if (at.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < at.bytes)) return SCANSCAM_EWORKSPACE;
+    if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
+    char *w = static_cast<char *>(a->workspace);
+    AttendArgs args{};
+    args.a = *a;
+    args.tokens = a->batch * a->T;
+    args.parts = parts;
+    args.each = (int32_t)(a->heads / a->groups);
+    args.ends = reinterpret_cast<float *>(w + at.ends);
+    args.logs = reinterpret_cast<double *>(w + at.logs);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipError_t err = hipSuccess;
+    if (parts > 1) err = starts(args, false, s);
+    if (err == hipSuccess) err = run(kOutputs, a->sequences * a->heads * parts, s, args);
+    return code(err);
+}
+
+int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
+{
+    SCANSCAM_CHECK(check_attend(a, true));
+    if (a->gdecay != nullptr && a->decay.p == nullptr) return SCANSCAM_EINVAL;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a->heads == 0) return SCANSCAM_OK;
+    if (a->sequences == 0 || (a->batch * a->T == 0 && a->gstate_in == nullptr))
+        return a->gdecay != nullptr && a->decay_fixed ? code(column_sum({nullptr, 0, 0, {a->gdecay}, {a->heads}}, s)) : SCANSCAM_OK;
+    const int parts = parts_of(*a);
+    const Pieces at = pieces_of(*a, true, parts);
+    if (at.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < at.bytes)) return SCANSCAM_EWORKSPACE;
+    if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
+    char *w = static_cast<char *>(a->workspace);
+    AttendArgs args{};
+    args.a = *a;
+    args.tokens = a->batch * a->T;
+    args.parts = parts;
+    args.each = (int32_t)(a->heads / a->groups);
+    args.ends = reinterpret_cast<float *>(w + at.ends);
+    args.back_ends = reinterpret_cast<float *>(w + at.back_ends);
+    args.logs = reinterpret_cast<double *>(w + at.logs);
+    if (a->gdecay != nullptr) {
+        args.reads = reinterpret_cast<float *>(w + at.reads);
+        args.writes = reinterpret_cast<float *>(w + at.writes);
+        args.last = reinterpret_cast<double *>(w + at.last);
+        args.most_borders = at.most_borders;
+        if (at.cross > at.borders) {  // (some sequence may have one)
+            args.borders = reinterpret_cast<float *>(w + at.borders);
+            args.cross = reinterpret_cast<double *>(w + at.cross);
+        }
+        args.decays = a->decay_fixed ? reinterpret_cast<float *>(w + at.decays) : a->gdecay;
+    }
+    if (args.each > 1) {
+        args.part_q = reinterpret_cast<float *>(w + at.part_q);
+        args.part_k = reinterpret_cast<float *>(w + at.part_k);
+    }
+    const int64_t pairs = a->sequences * a->heads;
+    hipError_t err = hipSuccess;
+    if (parts > 1) err = starts(args, false, s);
+    if (parts > 1 && err == hipSuccess) err = starts(args, true, s);
+    if (err == hipSuccess) err = run(kQueries, pairs * parts, s, args);
+    if (err == hipSuccess) err = run(kKeysAndValues, pairs * parts, s, args);
+    if (a->gdecay != nullptr && err == hipSuccess) {
+        constexpr int64_t most = 1 << 21;
+        for (args.first = 0; args.first < pairs && err == hipSuccess; args.first += most) {
+            const int64_t batches = ceil_div(a->T, kBorder * chunk_of(*a)), rounds = batches < 1 ? 1 : batches < 64 ? batches : 64;
+            const dim3 grid((unsigned)(pairs - args.first < most ? pairs - args.first : most), (unsigned)rounds), block(64 * kBorder);
+            err = chunk_of(*a) == 32 ? launch_op(decays_kernel<32>, grid, block, 0, s, args) : launch_op(decays_kernel<64>, grid, block, 0, s, args);
+        }
+        if (a->decay_fixed && err == hipSuccess) err = column_sum({args.decays, args.tokens, a->heads, {a->gdecay}, {a->heads}}, s);
+    }
+    if (args.each > 1 && err == hipSuccess) {
+        for (int i = 0; i < 2 && err == hipSuccess; i++) {
+            const Shared sum{i == 0 ? args.part_q : args.part_k, i == 0 ? a->gq : a->gk, args.tokens, a->T, 0, (int32_t)a->heads, args.each, (int32_t)a->K, a->dtype};
+            err = a->dtype == SCANSCAM_F32 ? join_shared<float>(sum, s) : a->dtype == SCANSCAM_BF16 ? join_shared<__bf16>(sum, s) : join_shared<_Float16>(sum, s);
+        }
+    }
+    return code(err);
+}
+
+int scanscam_attend_step_fwd(const scanscam_attend_step *a, void *stream)
+{
+    if (a == nullptr || a->rows < 0 || a->rows >= kMostTokens || a->slots < 0) return SCANSCAM_EINVAL;
+    SCANSCAM_CHECK(check_heads(a->heads, a->groups, a->K, a->V, a->dtype, a->decay, a->decay_dtype));
+    if (a->rows == 0 || a->heads == 0) return SCANSCAM_OK;
+    const int size = activation_size(a->dtype);
+    for (const scanscam_tokens *t : {&a->q, &a->k, &a->v, &a->y}) SCANSCAM_CHECK(check_tokens(*t, size));
+    if (a->slots > 0 && a->state == nullptr) return SCANSCAM_EINVAL;
+    if (misaligned(a->slot, a->slot64 ? 8 : 4) || misaligned(a->state, 4)) return SCANSCAM_EALIGN;
+    // Lanes for a whole row of the state, or fewer where that leaves CUs without a workgroup.
+    StepArgs args{};
+    args.a = *a;
+    args.lanes = 1;
+    while (args.lanes * 4 < a->V) args.lanes *= 2;
+    while (args.lanes > 8 && a->rows * a->heads * ceil_div(a->V, 4 * args.lanes) < 256) args.lanes /= 2;
+    args.pieces = (int32_t)ceil_div(a->V, 4 * args.lanes);
+    args.each = (int32_t)(a->heads / a->groups);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (a->dtype) {
+    case SCANSCAM_F32: return code(launch_attend_step<float>(args, s));
+    case SCANSCAM_BF16: return code(launch_attend_step<__bf16>(args, s));
+    default: return code(launch_attend_step<_Float16>(args, s));
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,929 @@
+// Linear attention with a decay for each head, whole sequences: device code.
+//
+//   S[t] = e^g[t] S[t-1] + k[t] v[t]^T          (K x V values a head, in fp32)
+//   o[t] = scale S[t]^T q[t]
+//   backwards, H[t] the gradient of S[t]:  H[t] = scale q[t] do[t]^T + e^g[t+1] H[t+1]
+//   dq[t] = scale S[t] do[t],  dk[t] = H[t] v[t],  dv[t] = H[t]^T k[t],  dg[t] = <H[t], e^g[t] S[t-1]>
+//
+// Chunks of C tokens turn it into matrix products. With G the sums of g from the chunk's first token on and S the state before it,
+//   o[t] = scale (e^G[t] S^T q[t] + sum over s <= t of e^(G[t]-G[s]) (q[t] k[s]) v[s]),
+//   S'   = e^G[end] S + sum over s of e^(G[end]-G[s]) k[s] v[s]^T.
+// dq is the same with (do, v, k) in place of (q, k, v), dk and dv the same backwards in time with (v, do, q) and (k, q, do).
+//
+// The gradient of a decay is summed up from what passes it, never from differences of what does not: inside of a chunk the pairs
+// s < t, M[t,s] = e^(G[t]-G[s]) (q[t] k[s]) (do[t] v[s]), in fp32; across its borders R[t] = q[t] (what dq[t] takes from S) and
+// W[s] = k[s] (what dk[s] takes from H). With X[c] = e^G[end] <H, S>, which passes the whole chunk,
+//   dg[t] = X[c] + sum over u >= t of R[u] + sum over s < t of W[s] + sum over s < t <= u of M[u,s],
+//   X[c] + sum of W = X[c+1] + sum of the next chunk's R  (both are the product of state and gradient at the border),
+// so that X follows from a border on without either state. What the sums' roundings leave in it grows with the chunks: at every eighth border the
+// pass over queries stores its state, and the pass over keys takes the product anew. W and R are fp32's: states go into products in several terms.
+//
+// Layout. A workgroup takes a head of a sequence (or of a part of it) through its chunks. A wave holds all rows of its own columns of the
+// state in the matrix unit's accumulators; these are, as they lie, operands of the next product: with lane = 16 g + n a 16 x 16 tile
+// holds rows 4 g + r of column n, and an operand of 32 rows (16 bits) may have its rows in any order that both operands share: rows
+// 4 g + (0..3) and 16 + 4 g + (0..3). So the state is rounded to an operand without leaving the registers, and so are the scores, by way of
+// LDS (they are shared by the waves) in the operand's own order. Tiles of the tensors lie in LDS as they are in memory; products over
+// time read them by transposing loads.
+#pragma once
+
+#include "ops_common.hpp"
+#include "scanscam_attention.h"
+
+#include <type_traits>
+
+namespace scanscam {
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef uint32_t raw16 __attribute__((ext_vector_type(4)));
+
+struct AttendArgs {
+    scanscam_attend a;
+    int64_t first;            // the first unit of this launch; a unit is a part of a head of a sequence
+    int64_t tokens;           // batch * T
+    int32_t parts, each;      // parts of a sequence, heads that share queries and keys
+    float *ends, *back_ends;  // [sequences][heads][parts][K][V]: what a part adds to the state; then the state that it starts from
+    double *logs;             // [sequences][heads][parts]: the part's sum of decays
+    float *reads, *writes;    // [heads][tokens]: R[t] + sum of M[t,s] - sum of M[s,t], and W[t]
+    double *last;             // [sequences][heads]: <gradient of the last state, last state>
+    float *borders;           // [border][heads]: the state at a border, as its workgroup's lanes hold it
+    double *cross;            // [border][heads]: its product with the gradient there
+    int64_t most_borders;     // of a batch element
+    float *part_q, *part_k;   // [tokens][heads][K]: gradients of shared queries and keys by head; NULL where none are shared
+    float *decays;            // [tokens][heads]: gradients of decays
+};
+
+// What differs with the activations' type: an operand is 16 bytes a lane, KS rows of 16 columns.
+template <typename ST> struct Operand {
+    typedef ST frag __attribute__((ext_vector_type(8)));
+    static constexpr int KS = 32, CHUNK = 64, PAD = 16;  // rows of an operand; tokens of a chunk; elements between a tile's rows, against bank conflicts
+};
+// (float32's operands are four steps of the matrix unit's instruction, its tiles twice the size: half the tokens)
+template <> struct Operand<float> {
+    typedef float4v frag;
+    static constexpr int KS = 16, CHUNK = 32, PAD = 4;
+};
+template <typename ST> using frag_t = typename Operand<ST>::frag;
+
+__device__ __forceinline__ float4v mma(const frag_t<__bf16> &a, const frag_t<__bf16> &b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float4v mma(const frag_t<_Float16> &a, const frag_t<_Float16> &b, float4v c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ float4v mma(const float4v &a, const float4v &b, float4v c)
+{
+#pragma unroll
+    for (int r = 0; r < 4; r++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+    return c;
+}
+
+// Terms of the activations' type that a float32 factor is taken apart into: all 24 bits. (What only 16-bit results come from has one term.)
+template <typename ST> constexpr int kTerms = 3;
+template <> inline constexpr int kTerms<_Float16> = 2;
+template <> inline constexpr int kTerms<float> = 1;
+
+// fp16 has five bits of exponent: what is taken apart is first brought to a largest value of 2^14 in the wave, by a power of two, so that the second
+// term's smallest step is 2^-38 of it and nothing overflows.
+__device__ __forceinline__ float most_of(float v)
+{
+    const auto top = [](float a, float b) { return a > b ? a : b; };
+    v = top(v, dpp_move<0x111, 0xf>(0.0f, v));
+    v = top(v, dpp_move<0x112, 0xf>(0.0f, v));
+    v = top(v, dpp_move<0x114, 0xf>(0.0f, v));
+    v = top(v, dpp_move<0x118, 0xf>(0.0f, v));
+    v = top(v, dpp_move<0x142, 0xa>(0.0f, v));
+    v = top(v, dpp_move<0x143, 0xc>(0.0f, v));
+    return read_lane(v, 63);
+}
+// (zero, infinities and NaN are left at 1; the power's inverse is finite too)
+__device__ __forceinline__ float scale_to_fp16(float most)
+{
+    if (!(most > 1e-30f && most < __builtin_inff())) return 1.0f;
+    return __builtin_ldexpf(1.0f, 14 - (int)(__builtin_bit_cast(uint32_t, most) >> 23) + 127);
+}
+
+template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(const float (&x)[N], frag_t<ST> (&out)[TERMS])
+{
+    if constexpr (sizeof(ST) == 4) {
+#pragma unroll
+        for (int e = 0; e < N; e++) out[0][e] = x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            float rest = x[e];
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+                const ST h = (ST)rest;
+                out[t][e] = h;
+                if (t + 1 < TERMS) rest = __builtin_isfinite((float)h) ? rest - (float)h : 0.0f;  // (an infinity stays one)
+            }
+        }
+    }
+}
+
+template <typename ST, int D> struct Tile {
+    static constexpr int LD = D + Operand<ST>::PAD, WORDS = Operand<ST>::CHUNK * LD * (int)sizeof(ST) / 4;
+    ST *p;
+    // Operand of 16 of the tile's rows; its own rows are the tile's columns k0 ... k0 + KS - 1.
+    __device__ __forceinline__ frag_t<ST> rows(int row0, int k0) const
+    {
+        const int lane = threadIdx.x & 63;
+        const ST *at = p + (row0 + (lane & 15)) * LD + k0 + 4 * (lane >> 4);
+        if constexpr (sizeof(ST) == 4) {
+            return *reinterpret_cast<const float4v *>(at);
+        } else {
+            typedef uint32_t raw8 __attribute__((ext_vector_type(2)));
+            const raw8 lo = *reinterpret_cast<const raw8 *>(at), hi = *reinterpret_cast<const raw8 *>(at + 16);
+            return __builtin_bit_cast(frag_t<ST>, raw16{lo[0], lo[1], hi[0], hi[1]});
+        }
+    }
+    // Operand of 16 of the tile's columns; its own rows are the tile's rows k0 ... k0 + KS - 1.
+    __device__ __forceinline__ frag_t<ST> columns(int col0, int k0) const
+    {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        if constexpr (sizeof(ST) == 4) {
+            const float *at = p + (k0 + 4 * g) * LD + col0 + n;
+            return float4v{at[0], at[LD], at[2 * LD], at[3 * LD]};
+        } else {
+            typedef __attribute__((address_space(3))) short4v lds4;
+            const ST *at = p + (k0 + 4 * g + (n >> 2)) * LD + col0 + 4 * (n & 3);
+            struct Both { short4v lo, hi; };
+            return __builtin_bit_cast(frag_t<ST>, Both{__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)at), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(at + 16 * LD))});
+        }
+    }
+    // Four neighbouring columns of a row.
+    __device__ __forceinline__ void four(int row, int col, float (&f)[4]) const
+    {
+        const ST *at = p + row * LD + col;
+        const Elems<ST, 4> v = __builtin_bit_cast(Elems<ST, 4>, *reinterpret_cast<const typename RawT<4 * sizeof(ST)>::type *>(at));
+#pragma unroll
+        for (int r = 0; r < 4; r++) f[r] = (float)v.e[r];
+    }
+};
+
+// A tile on its way from memory: asked for a chunk ahead, in registers. Rows from `n` on and columns from `d` on are zeros.
+template <typename ST, int D, int NT> struct Staged {
+    static constexpr int VE = 16 / sizeof(ST), ROW = D / VE, COUNT = Operand<ST>::CHUNK * ROW / NT;
+    raw16 v[COUNT];
+    __device__ __forceinline__ void load(const ST *base, int stride, int n, int d)
+    {
+        using raw_t = typename RawT<sizeof(ST) * VE>::type;
+        typedef raw_t unaligned __attribute__((aligned(sizeof(ST))));
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) {
+            const int index = threadIdx.x + i * NT, row = index / ROW, col = index % ROW * VE;
+            v[i] = raw16{0, 0, 0, 0};
+            if (row < n && col < d) {
+                const ST *at = base + row * stride + col;
+                if (col + VE <= d) {
+                    v[i] = *reinterpret_cast<const unaligned *>(at);
+                } else {
+                    Elems<ST, VE> e;
+#pragma unroll
+                    for (int k = 0; k < VE; k++) e.e[k] = col + k < d ? at[k] : (ST)0.0f;
+                    v[i] = __builtin_bit_cast(raw16, e);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(Tile<ST, D> tile) const
+    {
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) {
+            const int index = threadIdx.x + i * NT;
+            *reinterpret_cast<raw16 *>(tile.p + index / ROW * Tile<ST, D>::LD + index % ROW * VE) = v[i];
+        }
+    }
+};
+
+// The tokens that a workgroup goes through: a part of a sequence, of whole chunks but for the last.
+struct Span {
+    int64_t sequence, batch, from, begin, end, length;  // from, begin and end: tokens of the batch element; from and length: of the sequence
+    int head, part;
+    int64_t unit;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs &args, int64_t unit, int chunk)
+{
+    const scanscam_attend &a = args.a;
+    Span s;
+    s.unit = unit;
+    s.part = (int)(unit % args.parts);
+    const int64_t rest = unit / args.parts;
+    s.head = (int)(rest % a.heads);
+    s.sequence = rest / a.heads;
+    int64_t from = 0, to = a.T;
+    s.batch = s.sequence;
+    if (a.offsets != nullptr) {
+        s.batch = 0;
+        from = clamp_(index_at(a.offsets, a.offsets64, s.sequence), 0, a.T);
+        to = clamp_(index_at(a.offsets, a.offsets64, s.sequence + 1), from, a.T);
+    }
+    s.from = from;
+    s.length = to - from;
+    const int64_t chunks = (s.length + chunk - 1) / chunk, per = (chunks + args.parts - 1) / args.parts * chunk;
+    s.begin = from + (s.part * per < s.length ? s.part * per : s.length);
+    s.end = from + ((s.part + 1) * per < s.length ? (s.part + 1) * per : s.length);
+    return s;
+}
+
+template <typename ST> __device__ __forceinline__ const ST *tensor_at(const scanscam_tokens &t, const Span &s, int64_t head)
+{
+    return static_cast<const ST *>(t.p) + s.batch * t.batch + head * t.group;
+}
+
+// A token's decay in powers of two. An infinitely strong one is 2^-1000000, which is zero in fp32 but has differences.
+__device__ __forceinline__ double decay_at(const scanscam_attend &a, const Span &s, int64_t token, bool there)
+{
+    if (!there || a.decay.p == nullptr) return 0.0;
+    const float g = param(scanscam_param{a.decay.p, a.decay_dtype, 0}, s.batch * a.decay.batch + token * a.decay.token + s.head);
+    const double d = (double)g * 1.4426950408889634074;
+    return d < -1e6 ? -1e6 : d > 1e6 ? 1e6 : d;  // (a NaN stays one)
+}
+// Sums over the lanes up to each, in 64 bits: differences of them are exponents, and 32 bits would lose what small decays add to large ones.
+__device__ __forceinline__ double sums_upto(double v)
+{
+    v += dpp_move<0x111, 0xf>(0.0, v);
+    v += dpp_move<0x112, 0xf>(0.0, v);
+    v += dpp_move<0x114, 0xf>(0.0, v);
+    v += dpp_move<0x118, 0xf>(0.0, v);
+    v += dpp_move<0x142, 0xa>(0.0, v);
+    v += dpp_move<0x143, 0xc>(0.0, v);
+    return v;
+}
+__device__ __forceinline__ float exp2_(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
+// Of a chunk, in LDS: the sums of decays, e^G[t] and e^(G[end] - G[t]).
+template <int C> struct Decays {
+    double *sums;
+    float *upto, *after;
+    // By the first wave.
+    __device__ __forceinline__ void fill(double g)
+    {
+        const double G = sums_upto(g), end = read_lane(G, 63);
+        if (threadIdx.x < C) {
+            sums[threadIdx.x] = G;
+            upto[threadIdx.x] = exp2_(G);
+            after[threadIdx.x] = exp2_(end - G);
+        }
+    }
+    __device__ __forceinline__ float whole() const { return upto[C - 1]; }  // (tokens past the end have no decay)
+    static constexpr int WORDS = 4 * C;
+};
+
+// sum over 16 neighbouring lanes, in the last of them
+__device__ __forceinline__ float row_sum(float v)
+{
+    v += dpp_move<0x111, 0xf>(0.0f, v);
+    v += dpp_move<0x112, 0xf>(0.0f, v);
+    v += dpp_move<0x114, 0xf>(0.0f, v);
+    v += dpp_move<0x118, 0xf>(0.0f, v);
+    return v;
+}
+// sum over the four lanes that hold the same column, in all of them
+__device__ __forceinline__ float column_sum4(float v)
+{
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// A wave's columns of a state: all rows, in accumulators.
+template <typename ST, int D, int JT> struct State {
+    static constexpr int KS = Operand<ST>::KS, PER = KS / 16, RT = D / 16, C = Operand<ST>::CHUNK, STEPS = C / KS;
+    float4v s[RT][JT];
+    // Rows below `rows` and columns below `cols` of memory where neighbouring rows and columns are so far apart; zeros elsewhere or without memory.
+    __device__ __forceinline__ void read(const float *p, int rows, int cols, int row_step, int col_step, int col0)
+    {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = rt * 16 + 4 * g + r, col = col0 + jt * 16 + n;
+                    s[rt][jt][r] = p != nullptr && row < rows && col < cols ? p[row * row_step + col * col_step] : 0.0f;
+                }
+    }
+    __device__ __forceinline__ void write(float *p, int rows, int cols, int row_step, int col_step, int col0) const
+    {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = rt * 16 + 4 * g + r, col = col0 + jt * 16 + n;
+                    if (row < rows && col < cols) p[row * row_step + col * col_step] = s[rt][jt][r];
+                }
+    }
+    // This lane's part of the product with what lies in memory.
+    __device__ __forceinline__ double dot(const float *p, int rows, int cols, int row_step, int col_step, int col0) const
+    {
+        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+        double sum = 0.0;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int row = rt * 16 + 4 * g + r, col = col0 + jt * 16 + n;
+                    if (row < rows && col < cols) sum += (double)s[rt][jt][r] * (double)p[row * row_step + col * col_step];
+                }
+        return sum;
+    }
+    // The power of two that the state is multiplied with in operands.
+    __device__ __forceinline__ float scale() const
+    {
+        if constexpr (!std::is_same_v<ST, _Float16>) return 1.0f;
+        float most = 0.0f;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) most = __builtin_fmaxf(most, __builtin_fabsf(s[rt][jt][r]));
+        return scale_to_fp16(most_of(most));
+    }
+    // Rows ks * KS ... of column tile jt as an operand.
+    template <int TERMS> __device__ __forceinline__ void operand(int ks, int jt, float scale, frag_t<ST> (&out)[TERMS]) const
+    {
+        float x[4 * PER];
+#pragma unroll
+        for (int h = 0; h < PER; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[4 * h + r] = s[ks * PER + h][jt][r] * scale;
+        split<ST, TERMS>(x, out);
+    }
+    // acc[tt][jt], columns: rows of `of` (tokens), rows: the state's columns: the state's product with them, times the power of two that is returned.
+    template <int TERMS> __device__ __forceinline__ float times(Tile<ST, D> of, float4v (&acc)[C / 16][JT]) const
+    {
+        const float factor = scale();
+#pragma unroll
+        for (int tt = 0; tt < C / 16; tt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) acc[tt][jt] = float4v{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < D / KS; ks++) {
+            frag_t<ST> own[JT][TERMS];
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) operand<TERMS>(ks, jt, factor, own[jt]);
+#pragma unroll
+            for (int tt = 0; tt < C / 16; tt++) {
+                const frag_t<ST> token = of.rows(tt * 16, ks * KS);
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                    for (int t = 0; t < TERMS; t++) acc[tt][jt] = mma(own[jt][t], token, acc[tt][jt]);
+            }
+        }
+        return factor;
+    }
+    // s = decay s + sum over the chunk's tokens of rows[t] (weight[t] factor own[t])^T
+    template <int TERMS> __device__ __forceinline__ void update(Tile<ST, D> rows, const frag_t<ST> (&own)[JT][STEPS], const float *weight, float factor, float decay)
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+        float bring = 1.0f;
+        if constexpr (std::is_same_v<ST, _Float16>) {
+            float most = 0.0f;
+#pragma unroll
+            for (int step = 0; step < STEPS; step++)
+#pragma unroll
+                for (int h = 0; h < PER; h++) {
+                    const float4v w = *reinterpret_cast<const float4v *>(weight + step * KS + 16 * h + 4 * g);
+#pragma unroll
+                    for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) most = __builtin_fmaxf(most, __builtin_fabsf((float)own[jt][step][4 * h + r] * (w[r] * factor)));
+                }
+            bring = scale_to_fp16(most_of(most));
+            bring = bring < 1048576.0f ? bring : 1048576.0f;  // (the state is multiplied with it as well)
+            factor *= bring;
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) s[rt][jt] *= decay * bring;
+#pragma unroll
+        for (int step = 0; step < STEPS; step++) {
+            frag_t<ST> scaled[JT][TERMS];
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) {
+                float x[4 * PER];
+#pragma unroll
+                for (int h = 0; h < PER; h++) {
+                    const float4v w = *reinterpret_cast<const float4v *>(weight + step * KS + 16 * h + 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[4 * h + r] = (float)own[jt][step][4 * h + r] * (w[r] * factor);
+                }
+                split<ST, TERMS>(x, scaled[jt]);
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const frag_t<ST> row = rows.columns(rt * 16, step * KS);
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                    for (int t = 0; t < TERMS; t++) s[rt][jt] = mma(row, scaled[jt][t], s[rt][jt]);
+            }
+        }
+        if constexpr (std::is_same_v<ST, _Float16>) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++) s[rt][jt] *= 1.0f / bring;
+        }
+    }
+    // As the lanes hold it: to memory, and this lane's part of the product with one from there.
+    __device__ __forceinline__ void keep(float *p, int waves) const
+    {
+        const int64_t lanes = 64 * waves, lane = threadIdx.x % lanes;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) reinterpret_cast<float4v *>(p)[(rt * JT + jt) * lanes + lane] = s[rt][jt];
+    }
+    __device__ __forceinline__ double kept(const float *p, int waves) const
+    {
+        const int64_t lanes = 64 * waves, lane = threadIdx.x % lanes;
+        double sum = 0.0;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) {
+                const float4v other = reinterpret_cast<const float4v *>(p)[(rt * JT + jt) * lanes + lane];
+#pragma unroll
+                for (int r = 0; r < 4; r++) sum += (double)s[rt][jt][r] * (double)other[r];
+            }
+        return sum;
+    }
+};
+
+// Chunks between borders whose products are taken from the states. For 128 x 128 values a head the states stored are 7 % of the bytes of a backward pass.
+constexpr int kBorder = 8;
+// Of the border before token t of a sequence that begins at token `from`, at a multiple of kBorder chunks: borders of a sequence are so far apart, and
+// of the next one's first token's at least the same as of this one's last border, so that each has a place of its own.
+__device__ __forceinline__ int64_t border_at(const AttendArgs &args, int64_t batch, int64_t t, int chunk, int head)
+{
+    return (batch * args.most_borders + t / (kBorder * chunk)) * args.a.heads + head;
+}
+
+// The scores of a chunk in LDS, as operands: [tile of 16 columns][step of KS rows][lane] of 16 bytes each.
+template <typename ST> struct Scores {
+    static constexpr int KS = Operand<ST>::KS, PER = KS / 16, C = Operand<ST>::CHUNK, STEPS = C / KS, WORDS = C * C * (int)sizeof(ST) / 4;
+    frag_t<ST> *p;
+    __device__ __forceinline__ frag_t<ST> operand(int tile, int step) const { return p[(tile * STEPS + step) * 64 + (threadIdx.x & 63)]; }
+    // A 16 x 16 tile of rows row_tile * 16 ... and columns tile * 16 ...
+    __device__ __forceinline__ void put(int tile, int row_tile, float4v v) const
+    {
+        ST *at = reinterpret_cast<ST *>(p + (tile * STEPS + row_tile / PER) * 64 + (threadIdx.x & 63)) + row_tile % PER * 4;
+        using raw_t = typename RawT<4 * sizeof(ST)>::type;
+        Elems<ST, 4> four;
+#pragma unroll
+        for (int r = 0; r < 4; r++) four.e[r] = (ST)v[r];
+        *reinterpret_cast<raw_t *>(at) = __builtin_bit_cast(raw_t, four);
+    }
+    __device__ __forceinline__ float at(int row, int column) const
+    {
+        const ST *e = reinterpret_cast<const ST *>(p + (column / 16 * STEPS + row / KS) * 64 + row % 16 / 4 * 16 + column % 16);
+        return (float)e[row % KS / 16 * 4 + row % 4];
+    }
+    // Tiles beyond the diagonal that operands reach are zeros, and nobody writes them.
+    __device__ __forceinline__ void clear() const
+    {
+        for (int i = threadIdx.x; i < C / 16 * STEPS * 64; i += blockDim.x) reinterpret_cast<raw16 *>(p)[i] = raw16{0, 0, 0, 0};
+    }
+};
+
+// The id-th pair (i, j) with j <= i.
+__device__ __forceinline__ void pair_of(int id, int &i, int &j)
+{
+    i = id < 1 ? 0 : id < 3 ? 1 : id < 6 ? 2 : 3;
+    j = id - i * (i + 1) / 2;
+}
+
+// Four neighbouring values of a token's output.
+template <typename ST> __device__ __forceinline__ void put4(ST *row, int col, int cols, float4v v)
+{
+    const float f[4] = {v[0], v[1], v[2], v[3]};
+    if (col < cols) store_some<ST, 4>(row + col, cols - col, f);
+}
+
+template <typename ST, int D> constexpr int attend_waves() { return D == 256 ? 8 : 4; }
+
+// --- outputs (x, y, z = q, k, v) and, with GRAD, gradients of queries (x, y, z = do, v, k) with what decays read -----------------------
+template <typename ST, int D, bool GRAD> struct AttendLds {
+    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<ST, D>();
+    static constexpr int TILES = GRAD ? 4 : 3;
+    static constexpr int WORDS = TILES * Tile<ST, D>::WORDS + Scores<ST>::WORDS + Decays<C>::WORDS + (GRAD ? 2 * (C / 16) * C + W * C + 2 * W : 0);
+};
+template <typename ST, int D, bool GRAD> __global__ __launch_bounds__((64 * attend_waves<ST, D>()), 2) void attend_kernel(AttendArgs args)
+{
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * attend_waves<ST, D>(), W = NT / 64, JT = D / 16 / W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
+    constexpr int TERMS = kTerms<ST>, READ_TERMS = GRAD ? kTerms<ST> : 1;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const scanscam_attend &a = args.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4, col0 = wave * JT * 16;
+    float *at = lds;
+    const auto take = [&](int words) { float *p = at; at += words; return p; };
+    Tile<ST, D> X{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Y{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Z{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))};
+    Tile<ST, D> Q{GRAD ? reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS)) : nullptr};
+    Scores<ST> scores{reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS))};
+    Decays<C> decays{reinterpret_cast<double *>(take(2 * C)), take(C), take(C)};
+    float *rows = GRAD ? take(TT * C) : nullptr, *cols = GRAD ? take(TT * C) : nullptr, *red = GRAD ? take(W * C) : nullptr;
+    double *last = GRAD ? reinterpret_cast<double *>(take(2 * W)) : nullptr;
+
+    const Span span = span_of(args, args.first + blockIdx.x, C);
+    const int64_t shared = span.head / args.each;
+    const int K = (int)a.K, V = (int)a.V;
+    const scanscam_tokens &xt = GRAD ? a.gy : a.q, &yt = GRAD ? a.v : a.k, &zt = GRAD ? a.k : a.v;
+    const ST *x = tensor_at<ST>(xt, span, GRAD ? span.head : shared), *y = tensor_at<ST>(yt, span, GRAD ? span.head : shared), *z = tensor_at<ST>(zt, span, GRAD ? shared : span.head);
+    const ST *q = GRAD ? tensor_at<ST>(a.q, span, shared) : nullptr;
+    const int inner = GRAD ? V : K, outer = GRAD ? K : V;  // rows and columns of the state as it is held here
+    const int row_step = GRAD ? 1 : V, col_step = GRAD ? V : 1;
+    const int64_t pair = span.sequence * a.heads + span.head;
+
+    State<ST, D, JT> S;
+    const float *from = args.parts > 1 ? args.ends + span.unit * K * V : a.state_in == nullptr ? nullptr : a.state_in + pair * K * V;
+    S.read(from, inner, outer, row_step, col_step, col0);
+    scores.clear();
+
+    Staged<ST, D, NT> sx, sy, sz, sq;
+    double decay = 0.0;
+    const auto ask = [&](int64_t t) {
+        const int n = (int)(span.end - t < C ? span.end - t : C);
+        if (wave == 0) decay = decay_at(a, span, t + lane, lane < n);
+        sx.load(x + t * xt.token, (int)xt.token, n, inner);
+        sy.load(y + t * yt.token, (int)yt.token, n, inner);
+        sz.load(z + t * zt.token, (int)zt.token, n, outer);
+        if constexpr (GRAD) sq.load(q + t * a.q.token, (int)a.q.token, n, outer);
+    };
+    if (span.begin < span.end) ask(span.begin);
+    for (int64_t t0 = span.begin; t0 < span.end; t0 += C) {
+        const int n = (int)(span.end - t0 < C ? span.end - t0 : C);
+        sx.store(X);
+        sy.store(Y);
+        sz.store(Z);
+        if constexpr (GRAD) sq.store(Q);
+        if (wave == 0) decays.fill(decay);
+        __syncthreads();
+        if (t0 + C < span.end) ask(t0 + C);
+
+        // Scores: tiles of 16 tokens s (rows) by 16 tokens t (columns), t >= s.
+        for (int id = wave; id < TT * (TT + 1) / 2; id += W) {
+            int tt, st;
+            pair_of(id, tt, st);
+            float4v p{0, 0, 0, 0}, other{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < D; k += KS) {
+                p = mma(Y.rows(st * 16, k), X.rows(tt * 16, k), p);
+                if constexpr (GRAD) other = mma(Z.rows(st * 16, k), Q.rows(tt * 16, k), other);
+            }
+            const double upto = decays.sums[tt * 16 + n16];
+            float over_s = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int s = st * 16 + 4 * g + r, t = tt * 16 + n16;
+                const float w = exp2_(upto - decays.sums[s]);
+                p[r] = s <= t ? p[r] * w : 0.0f;
+                if constexpr (GRAD) {
+                    const float m = s < t ? p[r] * other[r] * a.scale : 0.0f;
+                    over_s += m;
+                    const float over_t = row_sum(m);
+                    if (n16 == 15) cols[tt * C + s] = over_t;
+                }
+            }
+            if constexpr (GRAD) {
+                over_s = column_sum4(over_s);
+                if (g == 0) rows[st * C + tt * 16 + n16] = over_s;
+            }
+            scores.put(tt, st, p);
+        }
+        frag_t<ST> own[JT][STEPS];
+#pragma unroll
+        for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+            for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(col0 + jt * 16, step * KS);
+        float4v acc[TT][JT];
+        const float unscale = 1.0f / S.template times<READ_TERMS>(X, acc);
+        if constexpr (GRAD)
+            if (args.borders != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0) S.keep(args.borders + border_at(args, span.batch, t0, C, span.head) * D * D, W);
+        __syncthreads();
+
+#pragma unroll
+        for (int tt = 0; tt < TT; tt++) {
+            const int t = tt * 16 + n16;
+            const float upto = decays.upto[t] * unscale;
+            float read = 0.0f, finite = 0.0f;
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) {
+                acc[tt][jt] *= upto;
+                if constexpr (GRAD) {
+                    float query[4];
+                    Q.four(t, col0 + jt * 16 + 4 * g, query);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) read += query[r] * acc[tt][jt][r];
+                }
+                float4v sum = acc[tt][jt];
+#pragma unroll
+                for (int step = 0; step <= tt / PER; step++) sum = mma(own[jt][step], scores.operand(tt, step), sum);
+                if constexpr (!GRAD) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) finite += sum[r] * 0.0f;
+                    if (__builtin_expect(__ballot(finite != 0.0f) != 0, 0)) {
+                        // A value that is not finite may be a later token's, times a score of zero: the tokens up to t alone.
+                        sum = acc[tt][jt];
+                        for (int s = 0; s <= t; s++) {
+                            float value[4];
+                            Z.four(s, col0 + jt * 16 + 4 * g, value);
+                            const float p = scores.at(s, t);
+#pragma unroll
+                            for (int r = 0; r < 4; r++) sum[r] += p * value[r];
+                        }
+                    }
+                }
+                sum *= a.scale;
+                if (t < n) {
+                    const int col = col0 + jt * 16 + 4 * g;
+                    if constexpr (!GRAD) {
+                        put4(static_cast<ST *>(a.y.p) + span.batch * a.y.batch + (t0 + t) * a.y.token + span.head * a.y.group, col, V, sum);
+                    } else if (args.part_q != nullptr) {
+                        put4(args.part_q + ((span.batch * a.T + t0 + t) * a.heads + span.head) * K, col, K, sum);
+                    } else {
+                        put4(static_cast<ST *>(a.gq.p) + span.batch * a.gq.batch + (t0 + t) * a.gq.token + span.head * a.gq.group, col, K, sum);
+                    }
+                }
+            }
+            if constexpr (GRAD) {
+                read = column_sum4(read);
+                if (g == 0) red[wave * C + t] = read;
+            }
+        }
+        S.template update<TERMS>(Y, own, decays.after, 1.0f, decays.whole());
+        __syncthreads();
+        if constexpr (GRAD) {
+            if (threadIdx.x < (unsigned)n && args.reads != nullptr) {
+                const int t = threadIdx.x;
+                float read = 0.0f, inside = 0.0f;
+                for (int w = 0; w < W; w++) read += red[w * C + t];
+                for (int st = 0; st <= t / 16; st++) inside += rows[st * C + t];
+                for (int tt = t / 16; tt < TT; tt++) inside -= cols[tt * C + t];
+                args.reads[span.head * args.tokens + span.batch * a.T + t0 + t] = read * a.scale + inside;
+            }
+        }
+    }
+    if (span.part == args.parts - 1) {
+        if constexpr (!GRAD) {
+            if (a.state_out != nullptr) S.write(a.state_out + pair * K * V, inner, outer, row_step, col_step, col0);
+        } else if (args.last != nullptr) {
+            double sum = a.gstate_out == nullptr ? 0.0 : S.dot(a.gstate_out + pair * K * V, inner, outer, row_step, col_step, col0);
+            sum = sums_upto(sum);
+            if (lane == 63) last[wave] = sum;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                double total = 0.0;
+                for (int w = 0; w < W; w++) total += last[w];
+                args.last[pair] = total;
+            }
+        }
+    }
+}
+
+// --- what a part of a sequence adds to the state (y, z = k, v), or backwards in time to the state's gradient (do, q) --------------------
+template <typename ST, int D> struct EndsLds {
+    static constexpr int WORDS = 2 * Tile<ST, D>::WORDS + Decays<Operand<ST>::CHUNK>::WORDS;
+};
+template <typename ST, int D, bool BACK> __global__ __launch_bounds__((64 * attend_waves<ST, D>()), 2) void ends_kernel(AttendArgs args)
+{
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * attend_waves<ST, D>(), W = NT / 64, JT = D / 16 / W, STEPS = C / KS;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const scanscam_attend &a = args.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col0 = wave * JT * 16;
+    Tile<ST, D> Y{reinterpret_cast<ST *>(lds)}, Z{reinterpret_cast<ST *>(lds + Tile<ST, D>::WORDS)};
+    float *rest = lds + 2 * Tile<ST, D>::WORDS;
+    Decays<C> decays{reinterpret_cast<double *>(rest), rest + 2 * C, rest + 3 * C};
+    const Span span = span_of(args, args.first + blockIdx.x, C);
+    if (span.part == (BACK ? 0 : args.parts - 1)) return;  // (nothing starts from its end)
+    const int K = (int)a.K, V = (int)a.V;
+    const scanscam_tokens &yt = BACK ? a.gy : a.k, &zt = BACK ? a.q : a.v;
+    const int64_t shared = span.head / args.each;
+    const ST *y = tensor_at<ST>(yt, span, BACK ? span.head : shared), *z = tensor_at<ST>(zt, span, BACK ? shared : span.head);
+    const int inner = BACK ? V : K, outer = BACK ? K : V, row_step = BACK ? 1 : V, col_step = BACK ? V : 1;
+    State<ST, D, JT> S;
+    S.read(nullptr, inner, outer, row_step, col_step, col0);
+    Staged<ST, D, NT> sy, sz;
+    double decay = 0.0, whole = 0.0;
+    const auto ask = [&](int64_t t) {
+        const int n = (int)(span.end - t < C ? span.end - t : C);
+        if (wave == 0) decay = decay_at(a, span, t + lane, lane < n);
+        sy.load(y + t * yt.token, (int)yt.token, n, inner);
+        sz.load(z + t * zt.token, (int)zt.token, n, outer);
+    };
+    const int64_t chunks = (span.end - span.begin + C - 1) / C;
+    const auto token = [&](int64_t c) { return span.begin + (BACK ? chunks - 1 - c : c) * C; };
+    if (chunks > 0) ask(token(0));
+    for (int64_t c = 0; c < chunks; c++) {
+        sy.store(Y);
+        sz.store(Z);
+        if (wave == 0) {
+            decays.fill(decay);
+            whole += read_lane(sums_upto(decay), 63);
+        }
+        __syncthreads();
+        if (c + 1 < chunks) ask(token(c + 1));
+        frag_t<ST> own[JT][STEPS];
+#pragma unroll
+        for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+            for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(col0 + jt * 16, step * KS);
+        S.template update<kTerms<ST>>(Y, own, BACK ? decays.upto : decays.after, BACK ? a.scale : 1.0f, decays.whole());
+        __syncthreads();
+    }
+    S.write((BACK ? args.back_ends : args.ends) + span.unit * K * V, inner, outer, row_step, col_step, col0);
+    if (threadIdx.x == 0) args.logs[span.unit] = whole;
+}
+
+// --- gradients of keys and values, backwards in time ------------------------------------------------------------------------------------
+// Two kinds of waves share the tiles: those of dk hold H with the values' channels as rows, those of dv with the keys'. BOTH: four waves of each;
+// else (256 channels: one kind's accumulators alone are half of a CU's registers) a workgroup is of one kind.
+template <typename ST, int D> constexpr bool attend_both() { return D < 256; }
+template <typename ST, int D> struct BackLds {
+    static constexpr int C = Operand<ST>::CHUNK, W = attend_both<ST, D>() ? 4 : 8;
+    static constexpr int WORDS = 4 * Tile<ST, D>::WORDS + (attend_both<ST, D>() ? 2 : 1) * Scores<ST>::WORDS + Decays<C>::WORDS + W * C + 2 * W;
+};
+template <typename ST, int D> __global__ __launch_bounds__(512, 2) void attend_back_kernel(AttendArgs args)
+{
+    constexpr bool BOTH = attend_both<ST, D>();
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 512, W = BOTH ? 4 : 8, JT = D / 16 / W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const scanscam_attend &a = args.a;
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
+    const bool keys = BOTH ? all < W : blockIdx.y == 0;  // dk
+    const int wave = BOTH ? all % W : all, col0 = wave * JT * 16;
+    float *at = lds;
+    const auto take = [&](int words) { float *p = at; at += words; return p; };
+    Tile<ST, D> Q{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Kt{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Vt{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))},
+        O{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))};
+    // Of the waves' own kind: do v (dk) or q k (dv).
+    frag_t<ST> *first_scores = reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS)), *second_scores = BOTH ? reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS)) : first_scores;
+    Scores<ST> scores{keys ? first_scores : second_scores};
+    Decays<C> decays{reinterpret_cast<double *>(take(2 * C)), take(C), take(C)};
+    float *red = take(W * C);
+    double *over = reinterpret_cast<double *>(take(2 * W));
+
+    const Span span = span_of(args, args.first + blockIdx.x, C);
+    const int64_t shared = span.head / args.each, pair = span.sequence * a.heads + span.head;
+    const int K = (int)a.K, V = (int)a.V;
+    const ST *q = tensor_at<ST>(a.q, span, shared), *k = tensor_at<ST>(a.k, span, shared), *v = tensor_at<ST>(a.v, span, span.head), *o = tensor_at<ST>(a.gy, span, span.head);
+    const Tile<ST, D> inter = keys ? Vt : Kt, update_rows = keys ? O : Q, mine = keys ? Q : O;
+    const int inner = keys ? V : K, outer = keys ? K : V, row_step = keys ? 1 : V, col_step = keys ? V : 1;
+
+    State<ST, D, JT> H;
+    const float *from = args.parts > 1 ? args.back_ends + span.unit * K * V : a.gstate_out == nullptr ? nullptr : a.gstate_out + pair * K * V;
+    H.read(from, inner, outer, row_step, col_step, col0);
+    Scores<ST>{first_scores}.clear();
+    if constexpr (BOTH) Scores<ST>{second_scores}.clear();
+
+    Staged<ST, D, NT> sq, sk, sv, so;
+    double decay = 0.0;
+    const auto ask = [&](int64_t t) {
+        const int n = (int)(span.end - t < C ? span.end - t : C);
+        if (all == 0) decay = decay_at(a, span, t + lane, lane < n);
+        sq.load(q + t * a.q.token, (int)a.q.token, n, K);
+        sk.load(k + t * a.k.token, (int)a.k.token, n, K);
+        sv.load(v + t * a.v.token, (int)a.v.token, n, V);
+        so.load(o + t * a.gy.token, (int)a.gy.token, n, V);
+    };
+    const int64_t chunks = (span.end - span.begin + C - 1) / C;
+    if (chunks > 0) ask(span.begin + (chunks - 1) * C);
+    for (int64_t c = chunks - 1; c >= 0; c--) {
+        const int64_t t0 = span.begin + c * C;
+        const int n = (int)(span.end - t0 < C ? span.end - t0 : C);
+        sq.store(Q);
+        sk.store(Kt);
+        sv.store(Vt);
+        so.store(O);
+        if (all == 0) decays.fill(decay);
+        __syncthreads();
+        if (c > 0) ask(t0 - C);
+
+        // Scores: tiles of 16 tokens t (rows) by 16 tokens s (columns), t >= s.
+        for (int id = wave; id < TT * (TT + 1) / 2; id += W) {
+            int tt, st;
+            pair_of(id, tt, st);
+            float4v p{0, 0, 0, 0};
+            const Tile<ST, D> of = keys ? O : Q;
+#pragma unroll
+            for (int d = 0; d < D; d += KS) p = mma(of.rows(tt * 16, d), inter.rows(st * 16, d), p);
+            const double from_s = decays.sums[st * 16 + n16];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int s = st * 16 + n16, t = tt * 16 + 4 * g + r;
+                const float w = exp2_(decays.sums[t] - from_s);
+                p[r] = s <= t ? p[r] * (w * a.scale) : 0.0f;
+            }
+            scores.put(st, tt, p);
+        }
+        frag_t<ST> own[JT][STEPS];
+#pragma unroll
+        for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+            for (int step = 0; step < STEPS; step++) own[jt][step] = mine.columns(col0 + jt * 16, step * KS);
+        float4v acc[TT][JT];
+        const float unscale = 1.0f / H.template times<kTerms<ST>>(inter, acc);
+        __syncthreads();
+
+#pragma unroll
+        for (int st = 0; st < TT; st++) {
+            const int s = st * 16 + n16;
+            const float after = decays.after[s] * unscale;
+            float write = 0.0f;
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) {
+                acc[st][jt] *= after;
+                float key[4];
+                Kt.four(s, col0 + jt * 16 + 4 * g, key);
+#pragma unroll
+                for (int r = 0; r < 4; r++) write += key[r] * acc[st][jt][r];
+                float4v sum = acc[st][jt];
+#pragma unroll
+                for (int step = st / PER; step < STEPS; step++) sum = mma(own[jt][step], scores.operand(st, step), sum);
+                if (s < n) {
+                    const int col = col0 + jt * 16 + 4 * g;
+                    if (!keys) {
+                        put4(static_cast<ST *>(a.gv.p) + span.batch * a.gv.batch + (t0 + s) * a.gv.token + span.head * a.gv.group, col, V, sum);
+                    } else if (args.part_k != nullptr) {
+                        put4(args.part_k + ((span.batch * a.T + t0 + s) * a.heads + span.head) * K, col, K, sum);
+                    } else {
+                        put4(static_cast<ST *>(a.gk.p) + span.batch * a.gk.batch + (t0 + s) * a.gk.token + span.head * a.gk.group, col, K, sum);
+                    }
+                }
+            }
+            write = column_sum4(write);
+            if (keys && g == 0) red[wave * C + s] = write;
+        }
+        H.template update<kTerms<ST>>(update_rows, own, decays.upto, a.scale, decays.whole());
+        const bool border = args.cross != nullptr && keys && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0;
+        const int64_t at_border = border ? border_at(args, span.batch, t0, C, span.head) : 0;
+        if (border) {
+            const double sum = sums_upto(H.kept(args.borders + at_border * D * D, W));
+            if (lane == 63) over[wave] = sum;
+        }
+        __syncthreads();
+        if (border && threadIdx.x == 0) {
+            double sum = 0.0;
+            for (int w = 0; w < W; w++) sum += over[w];
+            args.cross[at_border] = sum;
+        }
+        if (keys && args.writes != nullptr && threadIdx.x < (unsigned)n) {
+            float write = 0.0f;
+            for (int w = 0; w < W; w++) write += red[w * C + threadIdx.x];
+            args.writes[span.head * args.tokens + span.batch * a.T + t0 + threadIdx.x] = write;
+        }
+    }
+    if (keys && span.part == 0 && a.gstate_in != nullptr) H.write(a.gstate_in + pair * K * V, inner, outer, row_step, col_step, col0);
+}
+
+// --- launches by type ---------------------------------------------------------------------------------------------------------------------
+enum AttendPass { kOutputs, kQueries, kKeysAndValues, kEnds, kBackEnds };
+
+// A workgroup's lanes' values of a state.
+inline int attend_width(const scanscam_attend &a)
+{
+    const int64_t most = a.K > a.V ? a.K : a.V;
+    return most <= 64 ? 64 : most <= 128 ? 128 : 256;
+}
+
+template <typename ST> hipError_t launch_attend(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args);
+
+// Units of several launches where one would have 2^32 threads.
+template <auto Kernel, int WORDS> hipError_t launch_attend_units(int64_t units, unsigned kinds, int threads, hipStream_t stream, AttendArgs args)
+{
+    static_assert(WORDS * 4 <= 160 * 1024, "a workgroup's shared memory");
+    constexpr int64_t most = 1 << 22;
+    for (int64_t first = 0; first < units; first += most) {
+        args.first = first;
+        const hipError_t err = launch_wide<Kernel>(dim3((unsigned)(units - first < most ? units - first : most), kinds), threads, WORDS, WORDS, stream, args);
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
+}
+
+template <typename ST, int D> hipError_t launch_attend_with(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
+{
+    constexpr int threads = 64 * attend_waves<ST, D>();
+    switch (pass) {
+    case kOutputs: return launch_attend_units<attend_kernel<ST, D, false>, AttendLds<ST, D, false>::WORDS>(units, 1, threads, stream, args);
+    case kQueries: return launch_attend_units<attend_kernel<ST, D, true>, AttendLds<ST, D, true>::WORDS>(units, 1, threads, stream, args);
+    case kKeysAndValues: return launch_attend_units<attend_back_kernel<ST, D>, BackLds<ST, D>::WORDS>(units, attend_both<ST, D>() ? 1 : 2, 512, stream, args);
+    case kBackEnds: return launch_attend_units<ends_kernel<ST, D, true>, EndsLds<ST, D>::WORDS>(units, 1, threads, stream, args);
+    default: return launch_attend_units<ends_kernel<ST, D, false>, EndsLds<ST, D>::WORDS>(units, 1, threads, stream, args);
+    }
+}
+#define SCANSCAM_DEFINE_ATTEND_LAUNCH(ST)                                                                                                        \
+    template <> hipError_t launch_attend<ST>(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)                         \
+    {                                                                                                                                            \
+        const int width = attend_width(args.a);                                                                                                  \
+        return width == 64    ? launch_attend_with<ST, 64>(pass, units, stream, args)                                                            \
+               : width == 128 ? launch_attend_with<ST, 128>(pass, units, stream, args)                                                           \
+                              : launch_attend_with<ST, 256>(pass, units, stream, args);                                                          \
+    }
+
+}  // namespace scanscam

@@ -6,6 +6,8 @@
 
 #include "scan_kernels.hpp"
 
+#include <atomic>
+
 namespace scanscam {
 
 typedef float float4v __attribute__((ext_vector_type(4)));
@@ -176,6 +178,23 @@ inline hipError_t launch_op(Kernel kernel, dim3 grid, dim3 block, size_t lds, hi
     Args copy = args;
     void *params[] = {&copy};
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, params, lds, stream);
+}
+
+// A launch that may need more LDS than a kernel gets unasked. The limit belongs to the process: it is set once on each device, to the most
+// that any call needs (one that a call sets for itself could be lowered by another thread's before the launch).
+template <auto Kernel, typename Args> inline hipError_t launch_wide(dim3 grid, int threads, int words, int most_words, hipStream_t stream, const Args &args)
+{
+    static std::atomic<uint64_t> ready{0};  // a bit a device
+    int device = 0;
+    hipError_t err = hipGetDevice(&device);
+    if (err != hipSuccess) return err;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if ((ready.load(std::memory_order_acquire) & bit) == 0) {
+        err = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, most_words * (int)sizeof(float));
+        if (err != hipSuccess) return err;
+        ready.fetch_or(bit, std::memory_order_release);
+    }
+    return launch_op(Kernel, grid, dim3((unsigned)threads), (size_t)words * sizeof(float), stream, args);
 }
 
 inline hipError_t column_sum(ColumnSum a, hipStream_t stream)

@@ -44,23 +44,6 @@ int check_selective(const scanscam_selective *a)
     return a->z.p != nullptr ? check_near(a->z, size) : SCANSCAM_OK;
 }
 
-// A launch that may need more LDS than a kernel gets unasked. The limit belongs to the process: it is set once on each device, to the most
-// that any call needs (one that a call sets for itself could be lowered by another thread's before the launch).
-template <auto Kernel, typename Args> hipError_t launch_wide(dim3 grid, int threads, int words, int most_words, hipStream_t stream, const Args &args)
-{
-    static std::atomic<uint64_t> ready{0};  // a bit a device
-    int device = 0;
-    hipError_t err = hipGetDevice(&device);
-    if (err != hipSuccess) return err;
-    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
-    if ((ready.load(std::memory_order_acquire) & bit) == 0) {
-        err = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, most_words * (int)sizeof(float));
-        if (err != hipSuccess) return err;
-        ready.fetch_or(bit, std::memory_order_release);
-    }
-    return launch_op(Kernel, grid, dim3((unsigned)threads), (size_t)words * sizeof(float), stream, args);
-}
-
 // A launch has fewer than 2^32 threads: more parts than that are several launches.
 template <auto Kernel> hipError_t launch_units(SelectiveArgs args, int64_t units, int threads, int words, int most_words, hipStream_t stream)
 {

@@ -63,6 +63,25 @@ def _lib():
     return _entry_points
 
 
+def _bind_native():
+    """The host path in native code, autograd nodes included (csrc/torch_binding.cpp), or ``None`` where it or the library is a build without
+    these operators; calls then go through the functions below, several times as slowly on the host."""
+    native = state_space._native
+    if native is None or not hasattr(native, "bind_attention"):
+        return None
+    try:
+        lib = _lib()
+    except RuntimeError:
+        return None
+    native.bind_attention(*(ctypes.cast(fn, _p).value for fn in (
+        lib.scanscam_attend_fwd, lib.scanscam_attend_bwd, lib.scanscam_attend_workspace_bytes, lib.scanscam_attend_step_fwd, lib.scanscam_group_norm_fwd,
+        lib.scanscam_group_norm_bwd, lib.scanscam_group_norm_workspace_bytes)))
+    return native
+
+
+_native = _bind_native()
+
+
 def _launching(what: str):
     """The library, for a call that launches kernels (what records ATen calls only is refused)."""
     state_space._launching(what)
@@ -113,6 +132,10 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
     if _traced_through():
         if v.device.type == "cuda":
             return _eager(linear_attention, q, k, v, decay, scale=scale, state=state, offsets=offsets, return_state=return_state)
+    elif _native is not None and _parts == 0:
+        out = _native.attend(q, k, v, decay, scale, state, offsets, return_state)  # None: a call it leaves to the code below
+        if out is not None:
+            return out
     what = "linear_attention"
     _check_heads(what, q, k, v, decay, 2)
     _check_devices(what, v, (("q", q), ("k", k), ("decay", decay), ("state", state), ("offsets", offsets)))
@@ -221,6 +244,10 @@ def linear_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     if _traced_through():
         if v.device.type == "cuda":
             return _eager(linear_attention_step, state, q, k, v, decay, scale=scale, slots=slots)
+    elif _native is not None:
+        out = _native.attend_step(state, q, k, v, decay, scale, slots)
+        if out is not None:
+            return out
     what = "linear_attention_step"
     _check_heads(what, q, k, v, decay, 1)
     _check_devices(what, v, (("state", state), ("q", q), ("k", k), ("decay", decay), ("slots", slots)))
@@ -287,6 +314,10 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     if _traced_through():
         if x.device.type == "cuda":
             return _eager(group_norm, x, groups, weight, bias, z, eps=eps, activation=activation)
+    elif _native is not None:
+        out = _native.group_norm(x, groups, weight, bias, z, eps, activation)
+        if out is not None:
+            return out
     what = "group_norm"
     groups = int(groups)
     if x.dim() < 1 or groups < 1 or x.shape[-1] % groups:

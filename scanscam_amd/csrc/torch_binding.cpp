@@ -39,6 +39,7 @@
 
 #include "scanscam_hip.h"
 #include "scanscam_ops.h"
+#include "scanscam_attention.h"
 
 namespace {
 
@@ -1133,6 +1134,315 @@ PyObject *bind_operators(PyObject *, PyObject *args)
     Py_RETURN_NONE;
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------
+// The operators of a linear attention layer, in the same manner: 20 us a call in Python (a step of one token, a norm of 16), 170 for a small
+// norm's forward and backward pass; the figures here are beside the cases in the documents.
+// ---------------------------------------------------------------------------------------------------------------------------
+struct Attention {
+    decltype(&scanscam_attend_fwd) forward = nullptr;
+    decltype(&scanscam_attend_bwd) back = nullptr;
+    decltype(&scanscam_attend_workspace_bytes) workspace = nullptr;
+    decltype(&scanscam_attend_step_fwd) step = nullptr;
+    decltype(&scanscam_group_norm_fwd) norm = nullptr;
+    decltype(&scanscam_group_norm_bwd) norm_back = nullptr;
+    decltype(&scanscam_group_norm_workspace_bytes) norm_workspace = nullptr;
+} attention;
+
+// Logs of decays, [batch, T, heads] (lead 2), [rows, heads] (lead 1) or [heads], of any of the three types.
+bool logs_of(const at::Tensor &t, const at::Tensor &v, int lead, scanscam_tokens &k, int32_t &dtype)
+{
+    if (!t.defined()) return true;
+    dtype = dtype_code(t.scalar_type());
+    if (dtype < 0 || dtype == SCANSCAM_F64) return false;
+    if (t.dim() == 1) {
+        k.p = t.data_ptr();
+        return t.size(0) == v.size(lead) && t.is_contiguous();
+    }
+    if (t.sizes() != v.sizes().slice(0, (size_t)lead + 1) || (t.size(lead) != 1 && t.stride(lead) != 1)) return false;
+    k = {t.data_ptr(), lead == 2 ? t.stride(0) : 0, t.size(lead - 1) > 1 ? t.stride(lead - 1) : 0, 0};
+    return true;
+}
+
+struct AttendBackward : torch::autograd::Function<AttendBackward> {
+    struct Done {
+        at::Tensor y, state, offsets;
+        float scale;
+    };
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const Maybe &decay, const Maybe &state, Done *done)
+    {
+        keep(ctx, {q, k, v, decay.value_or(at::Tensor()), state.value_or(at::Tensor()), done->offsets});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["scale"] = (double)done->scale;
+        return done->state.defined() ? variable_list{done->y, done->state} : variable_list{done->y};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        check_unrecorded("linear_attention");
+        at::Tensor gstate_out = grads.size() > 1 ? grads[1] : at::Tensor();
+        if (!grads[0].defined() && !gstate_out.defined()) return variable_list(6);
+        const variable_list saved = returned(ctx, grads[0].defined() ? grads[0] : gstate_out, "linear_attention");
+        const at::Tensor q = Gradients::near(saved[0]), k = Gradients::near(saved[1]), v = Gradients::near(saved[2]), state = Gradients::dense(saved[4]),
+                         offsets = Gradients::dense(saved[5]);
+        at::Tensor decay = saved[3];
+        const c10::DeviceGuard guard(v.device());
+        const Gradients make{v};
+        const at::Tensor gy = make.tokens(grads[0]);
+        if (gstate_out.defined()) gstate_out = gstate_out.contiguous();
+        scanscam_attend a{};
+        if (!logs_of(decay, v, 2, a.decay, a.decay_dtype)) {
+            decay = decay.contiguous();
+            logs_of(decay, v, 2, a.decay, a.decay_dtype);
+        }
+        a.decay_fixed = decay.defined() && decay.dim() == 1;
+        a.batch = v.size(0);
+        a.T = v.size(1);
+        a.heads = v.size(2);
+        a.V = v.size(3);
+        a.groups = q.size(2);
+        a.K = q.size(3);
+        a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+        a.offsets = Gradients::at(offsets);
+        a.offsets64 = offsets.defined() && offsets.scalar_type() == at::kLong;
+        a.dtype = dtype_code(v.scalar_type());
+        a.scale = (float)ctx->saved_data["scale"].toDouble();
+        at::Tensor gq = make.empty(q), gk = make.empty(k), gv = make.empty(v);
+        // (inputs of the node are counted without the absent ones)
+        at::Tensor gdecay = decay.defined() && ctx->needs_input_grad(3) ? make.empty(decay, at::kFloat) : at::Tensor();
+        at::Tensor gstate = state.defined() && ctx->needs_input_grad(3 + decay.defined()) ? make.empty(state) : at::Tensor();
+        a.q = Gradients::view(q);
+        a.k = Gradients::view(k);
+        a.v = Gradients::view(v);
+        a.state_in = Gradients::at<float>(state);
+        a.gy = Gradients::view(gy);
+        a.gq = Gradients::view(gq);
+        a.gk = Gradients::view(gk);
+        a.gv = Gradients::view(gv);
+        a.gdecay = Gradients::at<float>(gdecay);
+        a.gstate_out = Gradients::at<float>(gstate_out);
+        a.gstate_in = Gradients::at<float>(gstate);
+        a.workspace_bytes = attention.workspace(&a, SCANSCAM_BACKWARD);
+        const at::Tensor workspace = make.bytes(a.workspace_bytes);
+        a.workspace = Gradients::at(workspace);
+        check_launch(attention.back(&a, make.stream()), "attend_bwd");
+        return once({gq, gk, gv, Gradients::as(std::move(gdecay), decay), gstate, {}}, saved, grads);
+    }
+};
+
+struct GroupNormBackward : torch::autograd::Function<GroupNormBackward> {
+    struct Done {
+        at::Tensor y;
+        int64_t groups;
+        float eps;
+        int activation;
+    };
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const Maybe &weight, const Maybe &bias, const Maybe &z, Done *done)
+    {
+        const at::Tensor none;
+        keep(ctx, {x, weight.value_or(none), bias.value_or(none), z.value_or(none)});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["groups"] = done->groups;
+        ctx->saved_data["eps"] = (double)done->eps;
+        ctx->saved_data["activation"] = (int64_t)done->activation;
+        return done->y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        check_unrecorded("group_norm");
+        if (!grads[0].defined()) return variable_list(5);
+        const variable_list saved = returned(ctx, grads[0], "group_norm");
+        const auto rows = [&](const at::Tensor &t) { return !t.defined() || row_stride(t) >= 0 ? t : t.contiguous(); };
+        const at::Tensor x = rows(saved[0]), weight = Gradients::dense(saved[1]), bias = Gradients::dense(saved[2]), z = rows(saved[3]);
+        const c10::DeviceGuard guard(x.device());
+        const Gradients make{x};
+        const at::Tensor gy = grads[0].contiguous();
+        scanscam_group_norm a{};
+        a.channels = x.size(-1);
+        a.rows = x.numel() / a.channels;
+        a.groups = ctx->saved_data["groups"].toInt();
+        a.eps = (float)ctx->saved_data["eps"].toDouble();
+        a.activation = (int32_t)ctx->saved_data["activation"].toInt();
+        a.dtype = dtype_code(x.scalar_type());
+        a.x = x.data_ptr();
+        a.x_stride = row_stride(x);
+        a.z = Gradients::at(z);
+        a.z_stride = z.defined() ? row_stride(z) : 0;
+        a.weight = Gradients::parameter(weight);
+        a.bias = Gradients::parameter(bias);
+        at::Tensor gx = make.empty(x), gz = make.empty(z), gweight = make.empty(weight, at::kFloat), gbias = make.empty(bias, at::kFloat);
+        a.gy = gy.data_ptr();
+        a.gx = gx.data_ptr();
+        a.gz = Gradients::at(gz);
+        a.gweight = Gradients::at<float>(gweight);
+        a.gbias = Gradients::at<float>(gbias);
+        a.workspace_bytes = attention.norm_workspace(&a);
+        const at::Tensor workspace = make.bytes(a.workspace_bytes);
+        a.workspace = Gradients::at(workspace);
+        check_launch(attention.norm_back(&a, make.stream()), "group_norm_bwd");
+        return once({gx, Gradients::as(std::move(gweight), weight), Gradients::as(std::move(gbias), bias), gz, {}}, saved, grads);
+    }
+};
+
+// A number, or not covered.
+double number(Arguments &in, int i)
+{
+    const double v = PyFloat_AsDouble(in.args[i]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        in.ok = false;
+    }
+    return v;
+}
+
+// What both forms of the attention have in common: q, k, v, decay from `at` on; v is `first`.
+template <typename Args> bool attend_arguments(Arguments &in, int at, int lead, Args &a)
+{
+    const at::Tensor &v = in.first, q = in.tensor(at), k = in.tensor(at + 1), decay = in.tensor(at + 3);
+    if (at::GradMode::is_enabled() && v.requires_grad()) in.gradients = true;
+    if (!in.ok || !attention.norm || v.dim() != lead + 2 || v.numel() == 0 || !q.defined() || !k.defined() || q.dim() != lead + 2) return false;
+    a.heads = v.size(lead);
+    a.V = v.size(lead + 1);
+    a.groups = q.size(lead);
+    a.K = q.size(lead + 1);
+    if (a.groups < 1 || a.heads % a.groups != 0 || a.K < 1 || a.K > SCANSCAM_MOST_HEAD || a.V > SCANSCAM_MOST_HEAD) return false;
+    in.shape(k, q.sizes());
+    for (int d = 0; d < lead; d++)
+        if (q.size(d) != v.size(d)) return false;
+    a.dtype = in.code();
+    a.q = in.tokens(q, lead);
+    a.k = in.tokens(k, lead);
+    a.v = in.tokens(v, lead);
+    if (!logs_of(decay, v, lead, a.decay, a.decay_dtype)) return false;
+    return in.ok;
+}
+
+// attend(q, k, v, decay, scale, state, offsets, return_state)
+PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 8, 2);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &v = in.first, state = in.tensor(5), offsets = in.tensor(6);
+    scanscam_attend a{};
+    if (!in.ok || !attend_arguments(in, 0, 2, a) || (offsets.defined() && (offsets.dim() != 1 || offsets.numel() < 2 || v.size(0) != 1))) Py_RETURN_NONE;
+    a.decay_fixed = args[3] != Py_None && THPVariable_Unpack(args[3]).dim() == 1;
+    a.batch = v.size(0);
+    a.T = v.size(1);
+    a.sequences = offsets.defined() ? offsets.numel() - 1 : a.batch;
+    in.sizes(a.heads * (a.K > a.V ? a.K : a.V), a.batch * a.T, a.sequences);
+    in.shape(state, {a.sequences, a.heads, a.K, a.V});
+    a.offsets = in.indices(offsets, &a.offsets64);
+    a.state_in = static_cast<const float *>(in.dense(state, at::kFloat));
+    a.scale = (float)number(in, 4);
+    const bool keep = in.flag(7);
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(v.sizes(), v.scalar_type()), new_state, workspace;
+    a.y = in.tokens(y, 2);
+    if (keep) {
+        new_state = in.empty({a.sequences, a.heads, a.K, a.V}, at::kFloat);
+        a.state_out = static_cast<float *>(new_state.data_ptr());
+    }
+    a.workspace_bytes = attention.workspace(&a, SCANSCAM_FORWARD);
+    if (a.workspace_bytes != 0) {
+        workspace = in.empty({(int64_t)a.workspace_bytes}, at::kByte);
+        a.workspace = workspace.data_ptr();
+    }
+    SCANSCAM_LAUNCH(attention.forward(&a, in.stream()), "attend_fwd")
+    if (in.gradients) {
+        AttendBackward::Done done{y, new_state, offsets, a.scale};
+        const auto given = [&](int i) { return args[i] == Py_None ? Maybe() : Maybe(THPVariable_Unpack(args[i])); };
+        variable_list out = AttendBackward::apply(*given(0), *given(1), v, given(3), maybe(state), &done);
+        y = out[0];
+        if (keep) new_state = out[1];
+    }
+    return with_state(std::move(y), std::move(new_state));
+    END_HANDLE_TH_ERRORS
+}
+
+// attend_step(state, q, k, v, decay, scale, slots)
+PyObject *attend_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 7, 3);
+    if (!in.ok) Py_RETURN_NONE;
+    const at::Tensor &v = in.first, state = in.tensor(0), slots = in.tensor(6);
+    scanscam_attend_step a{};
+    if (!in.ok || !state.defined() || state.dim() != 4 || !attend_arguments(in, 1, 1, a) || in.gradients) Py_RETURN_NONE;
+    a.rows = v.size(0);
+    a.slots = state.size(0);
+    if (!slots.defined() && a.slots != a.rows) Py_RETURN_NONE;
+    in.sizes(a.heads * (a.K > a.V ? a.K : a.V), a.rows);
+    in.shape(state, {a.slots, a.heads, a.K, a.V});
+    in.shape(slots, {a.rows});
+    a.slot = in.indices(slots, &a.slot64);
+    a.scale = (float)number(in, 5);
+    a.state = static_cast<float *>(in.dense(state, at::kFloat));
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(v.sizes(), v.scalar_type());
+    a.y = in.tokens(y, 1);
+    SCANSCAM_LAUNCH(attention.step(&a, in.stream()), "attend_step_fwd")
+    state.unsafeGetTensorImpl()->bump_version();
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// group_norm(x, groups, weight, bias, z, eps, activation)
+PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    Arguments in(args, nargs, 7, 0);
+    if (!in.ok || !PyLong_CheckExact(args[1])) Py_RETURN_NONE;
+    const at::Tensor &x = in.first, weight = in.tensor(2), bias = in.tensor(3), z = in.tensor(4);
+    if (!in.ok || !attention.norm || x.dim() < 1 || x.numel() == 0) Py_RETURN_NONE;
+    scanscam_group_norm a{};
+    int overflow = 0;
+    a.groups = PyLong_AsLongAndOverflow(args[1], &overflow);
+    a.channels = x.size(-1);
+    if (overflow != 0 || a.groups < 1 || a.channels % a.groups != 0 || a.channels / a.groups > SCANSCAM_MOST_GROUP) Py_RETURN_NONE;
+    a.rows = x.numel() / a.channels;
+    in.sizes(a.channels, a.rows);
+    in.shape(weight, {a.channels});
+    in.shape(bias, {a.channels});
+    in.shape(z, x.sizes());
+    a.x = x.data_ptr();
+    a.x_stride = row_stride(x);
+    if (z.defined()) {
+        a.z = z.data_ptr();
+        a.z_stride = row_stride(z);
+        if (z.scalar_type() != x.scalar_type()) in.ok = false;
+    }
+    if (a.x_stride < 0 || a.z_stride < 0) in.ok = false;
+    a.weight = in.parameter(weight);
+    a.bias = in.parameter(bias);
+    a.eps = (float)number(in, 5);
+    a.activation = in.activation(6);
+    a.dtype = in.code();
+    if (!in.ok) Py_RETURN_NONE;
+    at::Tensor y = in.empty(x.sizes(), x.scalar_type());
+    a.y = y.data_ptr();
+    SCANSCAM_LAUNCH(attention.norm(&a, in.stream()), "group_norm_fwd")
+    if (in.gradients) {
+        GroupNormBackward::Done done{y, a.groups, a.eps, a.activation};
+        y = GroupNormBackward::apply(x, maybe(weight), maybe(bias), maybe(z), &done);
+    }
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// bind_attention(attend_fwd, attend_bwd, attend_workspace_bytes, attend_step_fwd, group_norm_fwd, group_norm_bwd, group_norm_workspace_bytes): addresses.
+PyObject *bind_attention(PyObject *, PyObject *args)
+{
+    unsigned long long p[7];
+    if (!PyArg_ParseTuple(args, "KKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6)) return nullptr;
+    attention.forward = reinterpret_cast<decltype(attention.forward)>(p[0]);
+    attention.back = reinterpret_cast<decltype(attention.back)>(p[1]);
+    attention.workspace = reinterpret_cast<decltype(attention.workspace)>(p[2]);
+    attention.step = reinterpret_cast<decltype(attention.step)>(p[3]);
+    attention.norm_back = reinterpret_cast<decltype(attention.norm_back)>(p[5]);
+    attention.norm_workspace = reinterpret_cast<decltype(attention.norm_workspace)>(p[6]);
+    attention.norm = reinterpret_cast<decltype(attention.norm)>(p[4]);
+    Py_RETURN_NONE;
+}
+
 template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)> PyCFunction fast()
 {
     return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F));
@@ -1149,6 +1459,10 @@ PyMethodDef methods[] = {{"scan", reinterpret_cast<PyCFunction>(reinterpret_cast
                          {"selective", fast<selective>(), METH_FASTCALL, nullptr},
                          {"selective_step", fast<selective_step>(), METH_FASTCALL, nullptr},
                          {"bind_operators", bind_operators, METH_VARARGS, nullptr},
+                         {"attend", fast<attend>(), METH_FASTCALL, nullptr},
+                         {"attend_step", fast<attend_step>(), METH_FASTCALL, nullptr},
+                         {"group_norm", fast<group_norm>(), METH_FASTCALL, nullptr},
+                         {"bind_attention", bind_attention, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -96,9 +96,11 @@ CASES = [
 
 
 @pytest.mark.parametrize("dtype,batch,T,heads,K,V,more", CASES, ids=lambda v: str(v).replace("torch.", "").replace(" ", ""))
-@pytest.mark.parametrize("parts", [0, 1, 3])
-def test_attention_and_gradients(gpu, monkeypatch, dtype, batch, T, heads, K, V, more, parts):
+@pytest.mark.parametrize("parts,native", [(0, True), (0, False), (1, False), (3, False)])
+def test_attention_and_gradients(gpu, monkeypatch, dtype, batch, T, heads, K, V, more, parts, native):
     monkeypatch.setattr(attention, "_parts", parts)  # parts of time to share out, also where there is less than a chunk for each
+    if not native:  # the host path in Python
+        monkeypatch.setattr(attention, "_native", None)
     v, scale = make(5, dtype, batch, T, heads, K, V, **more), K ** -0.5
     state = v["state"] is not None
     names = [n for n, t in v.items() if t is not None and n != "offsets"]
@@ -137,8 +139,10 @@ def test_attention_and_gradients(gpu, monkeypatch, dtype, batch, T, heads, K, V,
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,heads,K,V,groups,decay", [(1, 1, 1, 1, 1, "token"), (3, 2, 16, 16, 1, "token"), (5, 3, 33, 65, 3, "head"), (2, 4, 128, 128, 2, None),
                                                          (2, 1, 256, 256, 1, "token"), (70, 2, 8, 130, 2, "token"), (1, 16, 128, 128, 16, "token")])
-@pytest.mark.parametrize("wide_slots", [True, False])
-def test_attention_step(gpu, dtype, rows, heads, K, V, groups, decay, wide_slots):
+@pytest.mark.parametrize("wide_slots,native", [(True, True), (False, True), (False, False)])
+def test_attention_step(gpu, monkeypatch, dtype, rows, heads, K, V, groups, decay, wide_slots, native):
+    if not native:
+        monkeypatch.setattr(attention, "_native", None)
     v = make(8, dtype, rows, 1, heads, K, V, groups, decay)
     slots = torch.randperm(rows + 4, generator=torch.Generator().manual_seed(1))[:rows]
     if rows > 2:
@@ -189,7 +193,10 @@ def norm_close(got, want, what, terms=1.0):
 
 
 @pytest.mark.parametrize("dtype,rows,channels,groups,affine,gate,activation", NORMS, ids=lambda v: str(v).replace("torch.", ""))
-def test_group_norm_and_gradients(gpu, dtype, rows, channels, groups, affine, gate, activation):
+@pytest.mark.parametrize("native", [True, False])
+def test_group_norm_and_gradients(gpu, monkeypatch, dtype, rows, channels, groups, affine, gate, activation, native):
+    if not native:
+        monkeypatch.setattr(attention, "_native", None)
     g = torch.Generator().manual_seed(3)
     r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
     v = {"x": (r(rows, channels) * 3 + 1).to(dtype), "weight": r(channels) + 1 if affine else None, "bias": r(channels) if affine else None,

@@ -27,8 +27,9 @@ extern "C" {
  * [heads] where `decay_fixed` is set (strides 0), or NULL (no decay). -infinity forgets everything. Logs above 0 let states
  * grow, as far as fp32 holds them.
  *
- * The workspace (scanscam_attend_workspace_bytes, aligned to 16 bytes) is for calls that share the time of a sequence out over
- * workgroups, and for the sums of the backward call. Strides from token to token must stay below SCANSCAM_MOST_TOKEN_STRIDE (decay's may be any), and
+ * `saved`: for a backward call, the states that its parts of time start from (scanscam_attend_saved_bytes, which may be 0). The
+ * workspace (scanscam_attend_workspace_bytes) is for calls that share the time of a sequence out over
+ * workgroups, and for the sums of the backward call. Both need alignment to 16 bytes. Strides from token to token must stay below SCANSCAM_MOST_TOKEN_STRIDE (decay's may be any), and
  * heads * K, heads * V are SCANSCAM_MOST_CHANNELS at most.
  */
 #define SCANSCAM_MOST_HEAD 256
@@ -42,6 +43,7 @@ typedef struct scanscam_attend {
     scanscam_tokens decay;         /* or NULL */
     const float *state_in;         /* [sequences, heads, K, V], or NULL */
     float *state_out;              /* or NULL */
+    void *saved;                   /* forward: written, or NULL; backward: read (NULL where it has no bytes) */
     /* Backward call only. */
     scanscam_tokens gy, gq, gk, gv;
     float *gdecay;                 /* [batch, T, heads], or [heads] where decay_fixed is set; or NULL */
@@ -54,6 +56,7 @@ typedef struct scanscam_attend {
 int scanscam_attend_fwd(const scanscam_attend *args, void *stream);
 int scanscam_attend_bwd(const scanscam_attend *args, void *stream);
 /* Only the sizes, dtype, parts, decay_fixed and whether offsets are given are looked at. */
+size_t scanscam_attend_saved_bytes(const scanscam_attend *args);
 size_t scanscam_attend_workspace_bytes(const scanscam_attend *args, int direction);
 
 /*

@@ -23,7 +23,7 @@ _MOST_HEAD, _MOST_GROUP = 256, 8192
 class _Attend(ctypes.Structure):
     _fields_ = ([(n, _i64) for n in ("batch", "T", "sequences", "heads", "groups", "K", "V")] + [("offsets", _p)] +
                 [(n, _i32) for n in ("offsets64", "dtype", "decay_dtype", "decay_fixed")] + [("scale", _f32), ("parts", _i32)] +
-                [(n, _Tokens) for n in ("q", "k", "v", "y", "decay")] + [("state_in", _p), ("state_out", _p)] +
+                [(n, _Tokens) for n in ("q", "k", "v", "y", "decay")] + [(n, _p) for n in ("state_in", "state_out", "saved")] +
                 [(n, _Tokens) for n in ("gy", "gq", "gk", "gv")] + [(n, _p) for n in ("gdecay", "gstate_out", "gstate_in", "workspace")] +
                 [("workspace_bytes", _size)])
 
@@ -56,7 +56,7 @@ def _lib():
             if fn is None:
                 raise RuntimeError(f"scanscam_amd: {hip.LIB_PATH} has no scanscam_{name}: it is a build without these operators")
             fn.argtypes, fn.restype = [ctypes.POINTER(args), _p], ctypes.c_int
-        for name, args, more in (("attend_workspace", _Attend, [ctypes.c_int]), ("group_norm_workspace", _GroupNorm, [])):
+        for name, args, more in (("attend_saved", _Attend, []), ("attend_workspace", _Attend, [ctypes.c_int]), ("group_norm_workspace", _GroupNorm, [])):
             fn = getattr(lib, f"scanscam_{name}_bytes")
             fn.argtypes, fn.restype = [ctypes.POINTER(args)] + more, _size
         _entry_points = lib
@@ -75,7 +75,7 @@ def _bind_native():
         return None
     native.bind_attention(*(ctypes.cast(fn, _p).value for fn in (
         lib.scanscam_attend_fwd, lib.scanscam_attend_bwd, lib.scanscam_attend_workspace_bytes, lib.scanscam_attend_step_fwd, lib.scanscam_group_norm_fwd,
-        lib.scanscam_group_norm_bwd, lib.scanscam_group_norm_workspace_bytes)))
+        lib.scanscam_group_norm_bwd, lib.scanscam_group_norm_workspace_bytes, lib.scanscam_attend_saved_bytes)))
     return native
 
 
@@ -150,7 +150,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
     if _needs_node(q, k, v, decay, state):
         y, new = LinearAttention.apply(q, k, v, decay, state, offsets, float(scale), bool(return_state))
     else:
-        y, new, _ = _attend_forward(q, k, v, decay, state, offsets, scale, return_state)
+        y, new, _, _ = _attend_forward(q, k, v, decay, state, offsets, scale, return_state, False)
     return (y, new) if return_state else y
 
 
@@ -177,32 +177,35 @@ def _seen(q, k, v, decay, state, offsets):
     return _near(q), _near(k), _near(v), _unit(decay), _dense(state), _dense(offsets)
 
 
-def _attend_forward(q, k, v, decay, state, offsets, scale, return_state):
-    """``(y, new state or None, the tensors as the library saw them)``."""
+def _attend_forward(q, k, v, decay, state, offsets, scale, return_state, save):
+    """``(y, new state or None, saved or None, the tensors as the library saw them)``."""
     L = _launching("linear_attention")
     with hip._on(v.device):
         seen = _seen(q, k, v, decay, state, offsets)
         a = _attend_args(*seen, scale)
         y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         a.y = _tokens(y)
-        new = workspace = None
+        new = saved = workspace = None
         if return_state:
             new = torch.empty((a.sequences, a.heads, a.K, a.V), dtype=torch.float32, device=v.device)
             a.state_out = new.data_ptr()
+        if save:
+            saved = _bytes(L.scanscam_attend_saved_bytes(a), v.device)
+            a.saved = _ptr(saved)
         n = L.scanscam_attend_workspace_bytes(a, hip.FORWARD)
         if n:
             workspace = _bytes(n, v.device)
             a.workspace, a.workspace_bytes = workspace.data_ptr(), n
         _raise(L.scanscam_attend_fwd(a, _stream(v.device)), "attend_fwd")
-    return y, new, seen
+    return y, new, saved, seen
 
 
 class LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, decay, state, offsets, scale, return_state):
-        y, new, seen = _attend_forward(q, k, v, decay, state, offsets, scale, return_state)
-        ctx.save_for_backward(*seen)
-        ctx.meta = _meta(*seen)
+        y, new, saved, seen = _attend_forward(q, k, v, decay, state, offsets, scale, return_state, True)
+        ctx.save_for_backward(*seen, saved)
+        ctx.meta = _meta(*seen, saved)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return y, new
@@ -213,8 +216,8 @@ class LinearAttention(torch.autograd.Function):
         if gy is None and gnew is None:
             return (None,) * 8
         kept = ctx.saved_tensors
-        _check_saved("linear_attention", gy if gy is not None else gnew, dict(zip(("q", "k", "v", "decay", "state", "offsets"), kept)), ctx.meta)
-        q, k, v, decay, state, offsets = seen = _seen(*kept)  # (a hook on saved tensors may lay out what it gives back in its own way)
+        _check_saved("linear_attention", gy if gy is not None else gnew, dict(zip(("q", "k", "v", "decay", "state", "offsets", "saved states"), kept)), ctx.meta)
+        q, k, v, decay, state, offsets = seen = _seen(*kept[:6])  # (a hook on saved tensors may lay out what it gives back in its own way)
         L = _launching("linear_attention")
         with hip._on(v.device):
             gy = _near(gy) if gy is not None else torch.zeros(v.shape, dtype=v.dtype, device=v.device)
@@ -224,7 +227,8 @@ class LinearAttention(torch.autograd.Function):
             gdecay = torch.empty(decay.shape, dtype=torch.float32, device=v.device) if ctx.needs_input_grad[3] else None
             gstate = torch.empty(state.shape, dtype=torch.float32, device=v.device) if ctx.needs_input_grad[4] else None
             a.gy, a.gq, a.gk, a.gv = (_tokens(t) for t in (gy, gq, gk, gv))
-            a.gdecay, a.gstate_out, a.gstate_in = _ptr(gdecay), _ptr(gnew), _ptr(gstate)
+            saved = _dense(kept[6])
+            a.gdecay, a.gstate_out, a.gstate_in, a.saved = _ptr(gdecay), _ptr(gnew), _ptr(gstate), _ptr(saved)
             n = L.scanscam_attend_workspace_bytes(a, hip.BACKWARD)
             workspace = _bytes(n, v.device)
             a.workspace, a.workspace_bytes = _ptr(workspace), n

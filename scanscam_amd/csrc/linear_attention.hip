@@ -18,12 +18,22 @@ __global__ __launch_bounds__(256) void join_kernel(Joined a)
     const int64_t pair = a.pair0 + blockIdx.x;
     if (at >= a.values) return;
     float run = a.from == nullptr ? 0.0f : a.from[pair * a.values + at];
-    for (int i = 0; i < a.parts; i++) {
-        const int64_t unit = pair * a.parts + (a.back ? a.parts - 1 - i : i);
-        float *p = a.ends + unit * a.values + at;
-        const float adds = i + 1 < a.parts ? *p : 0.0f;  // (the last one's was not computed)
-        *p = run;
-        if (i + 1 < a.parts) run = run * exp2_(a.logs[unit]) + adds;
+    constexpr int AHEAD = 16;  // parts asked for together: one after the other each is a trip to memory
+    for (int i0 = 0; i0 < a.parts; i0 += AHEAD) {
+        float adds[AHEAD], decay[AHEAD];
+        const auto unit = [&](int i) { return pair * a.parts + (a.back ? a.parts - 1 - i : i); };
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {  // (the last one's was not computed)
+            const bool there = i0 + i + 1 < a.parts;
+            adds[i] = there ? a.ends[unit(i0 + i) * a.values + at] : 0.0f;
+            decay[i] = there ? exp2_(a.logs[unit(i0 + i)]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (i0 + i < a.parts) {
+                a.ends[unit(i0 + i) * a.values + at] = run;
+                run = run * decay[i] + adds[i];
+            }
     }
 }
 
@@ -41,7 +51,7 @@ template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(A
     for (int64_t first = (int64_t)blockIdx.y * kBorder; first < chunks; first += (int64_t)gridDim.y * kBorder) {
         const int64_t c = first + kBorder - 1 - wave, t = span.begin + c * C + lane;
         const bool there = lane < C && t < span.end;
-        const double read = there ? args.reads[base + t] : 0.0, write = there ? args.writes[base + t] : 0.0;
+        const double read = there ? (double)args.reads[base + t] + (double)args.inside[base + t] : 0.0, write = there ? args.writes[base + t] : 0.0;
         const double reads = sums_upto(read), writes = sums_upto(write), all_reads = read_lane(reads, 63), all_writes = read_lane(writes, 63);
         if (lane == 0) over[wave] = all_reads - all_writes;
         __syncthreads();
@@ -182,6 +192,7 @@ int check_attend(const scanscam_attend *a, bool back)
     if (a->batch > 0 && a->T > (kMostTokens - 1) / a->batch) return SCANSCAM_EINVAL;
     SCANSCAM_CHECK(check_heads(a->heads, a->groups, a->K, a->V, a->dtype, a->decay, a->decay_dtype));
     if (misaligned(a->offsets, a->offsets64 ? 8 : 4)) return SCANSCAM_EALIGN;
+    if (misaligned(a->saved, 16)) return SCANSCAM_EALIGN;
     for (const void *p : {(const void *)a->state_in, (const void *)a->state_out, (const void *)a->gdecay, (const void *)a->gstate_out, (const void *)a->gstate_in})
         if (misaligned(p, 4)) return SCANSCAM_EALIGN;
     if (a->batch * a->T == 0 || a->heads == 0) return SCANSCAM_OK;
@@ -207,9 +218,10 @@ int parts_of(const scanscam_attend &a)
 
 // What the workspace holds, in order; each piece begins on 16 bytes.
 struct Pieces {
-    size_t ends, back_ends, logs, reads, writes, last, borders, cross, part_q, part_k, decays, bytes;
+    size_t ends, back_ends, logs, reads, writes, inside, last, borders, cross, part_q, part_k, decays, bytes;
     int64_t most_borders;
 };
+int64_t ends_values(const scanscam_attend &a, int parts) { return a.sequences * a.heads * parts * a.K * a.V; }
 Pieces pieces_of(const scanscam_attend &a, bool back, int parts)
 {
     Pieces p{};
@@ -218,13 +230,14 @@ Pieces pieces_of(const scanscam_attend &a, bool back, int parts)
         if (there) p.bytes += ((size_t)count * size + 15) / 16 * 16;
         return at;
     };
-    const int64_t pairs = a.sequences * a.heads, values = pairs * parts * a.K * a.V, tokens = a.batch * a.T;
-    p.ends = take(parts > 1, values, 4);
+    const int64_t pairs = a.sequences * a.heads, values = ends_values(a, parts), tokens = a.batch * a.T;
+    p.ends = take(parts > 1 && !back, values, 4);  // (a backward call has the forward one's)
     p.logs = take(parts > 1, pairs * parts, 8);
     if (!back) return p;
     p.back_ends = take(parts > 1, values, 4);
     p.reads = take(true, tokens * a.heads, 4);
     p.writes = take(true, tokens * a.heads, 4);
+    p.inside = take(true, tokens * a.heads, 4);
     p.last = take(true, pairs, 8);
     p.most_borders = a.T / (kBorder * chunk_of(a)) + 1;
     const int64_t borders = a.T > kBorder * chunk_of(a) ? a.batch * p.most_borders * a.heads : 0, width = attend_width(a);
@@ -246,11 +259,11 @@ hipError_t run(AttendPass pass, int64_t units, hipStream_t stream, const AttendA
 }
 
 // The states that parts start from.
-hipError_t starts(const AttendArgs &args, bool back, hipStream_t stream)
+hipError_t starts(const AttendArgs &args, bool back, AttendPass pass, hipStream_t stream)
 {
     const scanscam_attend &a = args.a;
     const int64_t pairs = a.sequences * a.heads;
-    hipError_t err = run(back ? kBackEnds : kEnds, pairs * args.parts, stream, args);
+    hipError_t err = run(pass, pairs * args.parts, stream, args);
     Joined j{back ? args.back_ends : args.ends, args.logs, back ? a.gstate_out : a.state_in, pairs, 0, args.parts, (int32_t)(a.K * a.V), back};
     constexpr int64_t most = 1 << 22;
     for (; j.pair0 < pairs && err == hipSuccess; j.pair0 += most)
@@ -293,6 +306,12 @@ bool sizes_fit(const scanscam_attend *a)
 
 extern "C" {
 
+size_t scanscam_attend_saved_bytes(const scanscam_attend *a)
+{
+    const int parts = sizes_fit(a) ? parts_of(*a) : 1;
+    return parts > 1 ? (size_t)ends_values(*a, parts) * sizeof(float) : 0;
+}
+
 size_t scanscam_attend_workspace_bytes(const scanscam_attend *a, int direction)
 {
     return sizes_fit(a) ? pieces_of(*a, direction == SCANSCAM_BACKWARD, parts_of(*a)).bytes : 0;
@@ -312,12 +331,12 @@ int scanscam_attend_fwd(const scanscam_attend *a, void *stream)
     args.tokens = a->batch * a->T;
     args.parts = parts;
     args.each = (int32_t)(a->heads / a->groups);
-    args.ends = reinterpret_cast<float *>(w + at.ends);
+    args.ends = a->saved != nullptr ? static_cast<float *>(a->saved) : reinterpret_cast<float *>(w + at.ends);
     args.logs = reinterpret_cast<double *>(w + at.logs);
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t err = hipSuccess;
-    if (parts > 1) err = starts(args, false, s);
-    if (err == hipSuccess) err = run(kOutputs, a->sequences * a->heads * parts, s, args);
+    if (parts > 1) err = starts(args, false, kEnds, s);
+    if (err == hipSuccess) err = run(a->state_out != nullptr ? kOutputs : kOutputsOnce, a->sequences * a->heads * parts, s, args);
     return code(err);
 }
 
@@ -333,18 +352,20 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     const Pieces at = pieces_of(*a, true, parts);
     if (at.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < at.bytes)) return SCANSCAM_EWORKSPACE;
     if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
+    if (parts > 1 && a->saved == nullptr) return SCANSCAM_EINVAL;
     char *w = static_cast<char *>(a->workspace);
     AttendArgs args{};
     args.a = *a;
     args.tokens = a->batch * a->T;
     args.parts = parts;
     args.each = (int32_t)(a->heads / a->groups);
-    args.ends = reinterpret_cast<float *>(w + at.ends);
+    args.ends = static_cast<float *>(a->saved);
     args.back_ends = reinterpret_cast<float *>(w + at.back_ends);
     args.logs = reinterpret_cast<double *>(w + at.logs);
     if (a->gdecay != nullptr) {
         args.reads = reinterpret_cast<float *>(w + at.reads);
         args.writes = reinterpret_cast<float *>(w + at.writes);
+        args.inside = reinterpret_cast<float *>(w + at.inside);
         args.last = reinterpret_cast<double *>(w + at.last);
         args.most_borders = at.most_borders;
         if (at.cross > at.borders) {  // (some sequence may have one)
@@ -359,8 +380,7 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     }
     const int64_t pairs = a->sequences * a->heads;
     hipError_t err = hipSuccess;
-    if (parts > 1) err = starts(args, false, s);
-    if (parts > 1 && err == hipSuccess) err = starts(args, true, s);
+    if (parts > 1) err = starts(args, true, kBackEnds, s);
     if (err == hipSuccess) err = run(kQueries, pairs * parts, s, args);
     if (err == hipSuccess) err = run(kKeysAndValues, pairs * parts, s, args);
     if (a->gdecay != nullptr && err == hipSuccess) {

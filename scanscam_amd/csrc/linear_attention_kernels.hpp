@@ -43,9 +43,9 @@ struct AttendArgs {
     int32_t parts, each;      // parts of a sequence, heads that share queries and keys
     float *ends, *back_ends;  // [sequences][heads][parts][K][V]: what a part adds to the state; then the state that it starts from
     double *logs;             // [sequences][heads][parts]: the part's sum of decays
-    float *reads, *writes;    // [heads][tokens]: R[t] + sum of M[t,s] - sum of M[s,t], and W[t]
+    float *reads, *writes, *inside;  // [heads][tokens]: R[t], W[t], and the sum of M[t,s] over s less that of M[s,t]
     double *last;             // [sequences][heads]: <gradient of the last state, last state>
-    float *borders;           // [border][heads]: the state at a border, as its workgroup's lanes hold it
+    float *borders;           // [border][heads]: the state at a border, tile by tile as the lanes hold it
     double *cross;            // [border][heads]: its product with the gradient there
     int64_t most_borders;     // of a batch element
     float *part_q, *part_k;   // [tokens][heads][K]: gradients of shared queries and keys by head; NULL where none are shared
@@ -55,12 +55,12 @@ struct AttendArgs {
 // What differs with the activations' type: an operand is 16 bytes a lane, KS rows of 16 columns.
 template <typename ST> struct Operand {
     typedef ST frag __attribute__((ext_vector_type(8)));
-    static constexpr int KS = 32, CHUNK = 64, PAD = 16;  // rows of an operand; tokens of a chunk; elements between a tile's rows, against bank conflicts
+    static constexpr int KS = 32, CHUNK = 64;  // rows of an operand; tokens of a chunk
 };
 // (float32's operands are four steps of the matrix unit's instruction, its tiles twice the size: half the tokens)
 template <> struct Operand<float> {
     typedef float4v frag;
-    static constexpr int KS = 16, CHUNK = 32, PAD = 4;
+    static constexpr int KS = 16, CHUNK = 32;
 };
 template <typename ST> using frag_t = typename Operand<ST>::frag;
 
@@ -73,7 +73,8 @@ __device__ __forceinline__ float4v mma(const float4v &a, const float4v &b, float
     return c;
 }
 
-// Terms of the activations' type that a float32 factor is taken apart into: all 24 bits. (What only 16-bit results come from has one term.)
+// Terms of the activations' type that a float32 factor is taken apart into where float32 results come from it (states that are handed over, gradients
+// of states and of decays): all 24 bits, 22 in fp16. What only 16-bit results come from has one: a rounding that is half of the result's own.
 template <typename ST> constexpr int kTerms = 3;
 template <> inline constexpr int kTerms<_Float16> = 2;
 template <> inline constexpr int kTerms<float> = 1;
@@ -111,25 +112,34 @@ template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(c
             for (int t = 0; t < TERMS; t++) {
                 const ST h = (ST)rest;
                 out[t][e] = h;
-                if (t + 1 < TERMS) rest = __builtin_isfinite((float)h) ? rest - (float)h : 0.0f;  // (an infinity stays one)
+                if (t + 1 < TERMS) rest -= (float)h;  // (an infinity becomes a NaN)
             }
         }
     }
 }
 
+// A chunk's tokens by up to D channels in LDS. Sixteen bytes of a row lie where an exclusive or with its number puts them, so that neither
+// operand's reads meet in a bank: 16 lanes that read 16 rows at a column have 16 places, and 8 rows of 32 bytes eight times two.
 template <typename ST, int D> struct Tile {
-    static constexpr int LD = D + Operand<ST>::PAD, WORDS = Operand<ST>::CHUNK * LD * (int)sizeof(ST) / 4;
+    static constexpr int VE = 16 / sizeof(ST), ROW = D / VE, WORDS = Operand<ST>::CHUNK * D * (int)sizeof(ST) / 4;
     ST *p;
+    static __device__ __forceinline__ int turn(int row)
+    {
+        if constexpr (sizeof(ST) == 4) return row & 15;
+        else if constexpr (D == 64) return (row >> 1 & 3) * 2 + (row >> 3 & 1);
+        else return (row & 7) * 2 + (row >> 3 & 1);
+    }
+    // Column `col` of a row, a multiple of four.
+    __device__ __forceinline__ ST *at(int row, int col) const { return p + row * D + ((col / VE ^ turn(row)) * VE + col % VE); }
     // Operand of 16 of the tile's rows; its own rows are the tile's columns k0 ... k0 + KS - 1.
     __device__ __forceinline__ frag_t<ST> rows(int row0, int k0) const
     {
-        const int lane = threadIdx.x & 63;
-        const ST *at = p + (row0 + (lane & 15)) * LD + k0 + 4 * (lane >> 4);
+        const int lane = threadIdx.x & 63, row = row0 + (lane & 15), col = k0 + 4 * (lane >> 4);
         if constexpr (sizeof(ST) == 4) {
-            return *reinterpret_cast<const float4v *>(at);
+            return *reinterpret_cast<const float4v *>(at(row, col));
         } else {
             typedef uint32_t raw8 __attribute__((ext_vector_type(2)));
-            const raw8 lo = *reinterpret_cast<const raw8 *>(at), hi = *reinterpret_cast<const raw8 *>(at + 16);
+            const raw8 lo = *reinterpret_cast<const raw8 *>(at(row, col)), hi = *reinterpret_cast<const raw8 *>(at(row, col + 16));
             return __builtin_bit_cast(frag_t<ST>, raw16{lo[0], lo[1], hi[0], hi[1]});
         }
     }
@@ -138,56 +148,75 @@ template <typename ST, int D> struct Tile {
     {
         const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
         if constexpr (sizeof(ST) == 4) {
-            const float *at = p + (k0 + 4 * g) * LD + col0 + n;
-            return float4v{at[0], at[LD], at[2 * LD], at[3 * LD]};
+            frag_t<ST> f;
+#pragma unroll
+            for (int r = 0; r < 4; r++) f[r] = at(k0 + 4 * g + r, col0 + (n & 12))[n & 3];
+            return f;
         } else {
             typedef __attribute__((address_space(3))) short4v lds4;
-            const ST *at = p + (k0 + 4 * g + (n >> 2)) * LD + col0 + 4 * (n & 3);
+            const int row = k0 + 4 * g + (n >> 2), col = col0 + 4 * (n & 3);
             struct Both { short4v lo, hi; };
-            return __builtin_bit_cast(frag_t<ST>, Both{__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)at), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(at + 16 * LD))});
+            return __builtin_bit_cast(frag_t<ST>, Both{__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)at(row, col)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)at(row + 16, col))});
         }
     }
     // Four neighbouring columns of a row.
     __device__ __forceinline__ void four(int row, int col, float (&f)[4]) const
     {
-        const ST *at = p + row * LD + col;
-        const Elems<ST, 4> v = __builtin_bit_cast(Elems<ST, 4>, *reinterpret_cast<const typename RawT<4 * sizeof(ST)>::type *>(at));
+        const Elems<ST, 4> v = __builtin_bit_cast(Elems<ST, 4>, *reinterpret_cast<const typename RawT<4 * sizeof(ST)>::type *>(at(row, col)));
 #pragma unroll
         for (int r = 0; r < 4; r++) f[r] = (float)v.e[r];
     }
 };
 
-// A tile on its way from memory: asked for a chunk ahead, in registers. Rows from `n` on and columns from `d` on are zeros.
-template <typename ST, int D, int NT> struct Staged {
-    static constexpr int VE = 16 / sizeof(ST), ROW = D / VE, COUNT = Operand<ST>::CHUNK * ROW / NT;
+// A tile on its way from memory: asked for a chunk ahead, in registers. Rows from `n` on and columns from `d` on are zeros. EXACT: d is a whole
+// number of vectors; then every lane loads, rows past the end the last one again, and what is not there becomes zero on the way to LDS.
+template <typename ST, int D, int NT, bool EXACT> struct Staged {
+    static constexpr int VE = 16 / sizeof(ST), ROW = D / VE, COUNT = Operand<ST>::CHUNK * ROW / NT, STEP = NT / ROW;
+    static_assert(NT % ROW == 0 && Operand<ST>::CHUNK * ROW % NT == 0, "whole rows for all threads");
     raw16 v[COUNT];
     __device__ __forceinline__ void load(const ST *base, int stride, int n, int d)
     {
         using raw_t = typename RawT<sizeof(ST) * VE>::type;
         typedef raw_t unaligned __attribute__((aligned(sizeof(ST))));
+        const int row0 = threadIdx.x / ROW, col = threadIdx.x % ROW * VE;
+        if constexpr (EXACT) {
+            const ST *at = base + (col < d ? col : 0);
 #pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            const int index = threadIdx.x + i * NT, row = index / ROW, col = index % ROW * VE;
-            v[i] = raw16{0, 0, 0, 0};
-            if (row < n && col < d) {
-                const ST *at = base + row * stride + col;
-                if (col + VE <= d) {
-                    v[i] = *reinterpret_cast<const unaligned *>(at);
-                } else {
-                    Elems<ST, VE> e;
+            for (int i = 0; i < COUNT; i++) {
+                const int row = row0 + i * STEP;
+                v[i] = *reinterpret_cast<const unaligned *>(at + (row < n ? row : n - 1) * stride);
+            }
+        } else {
 #pragma unroll
-                    for (int k = 0; k < VE; k++) e.e[k] = col + k < d ? at[k] : (ST)0.0f;
-                    v[i] = __builtin_bit_cast(raw16, e);
+            for (int i = 0; i < COUNT; i++) {
+                const int row = row0 + i * STEP;
+                v[i] = raw16{0, 0, 0, 0};
+                if (row < n && col < d) {
+                    const ST *at = base + row * stride + col;
+                    if (col + VE <= d) {
+                        v[i] = *reinterpret_cast<const unaligned *>(at);
+                    } else {
+                        Elems<ST, VE> e;
+#pragma unroll
+                        for (int k = 0; k < VE; k++) e.e[k] = col + k < d ? at[k] : (ST)0.0f;
+                        v[i] = __builtin_bit_cast(raw16, e);
+                    }
                 }
             }
         }
     }
-    __device__ __forceinline__ void store(Tile<ST, D> tile) const
+    __device__ __forceinline__ void store(Tile<ST, D> tile, int n, int d) const
     {
+        const int row0 = threadIdx.x / ROW, col = threadIdx.x % ROW * VE;
+        if (!EXACT || (n == Operand<ST>::CHUNK && d == D)) {
 #pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            const int index = threadIdx.x + i * NT;
-            *reinterpret_cast<raw16 *>(tile.p + index / ROW * Tile<ST, D>::LD + index % ROW * VE) = v[i];
+            for (int i = 0; i < COUNT; i++) *reinterpret_cast<raw16 *>(tile.at(row0 + i * STEP, col)) = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < COUNT; i++) {
+                const bool there = row0 + i * STEP < n && col < d;
+                *reinterpret_cast<raw16 *>(tile.at(row0 + i * STEP, col)) = there ? v[i] : raw16{0, 0, 0, 0};
+            }
         }
     }
 };
@@ -282,12 +311,15 @@ __device__ __forceinline__ float column_sum4(float v)
     return v + __shfl_xor(v, 32);
 }
 
-// A wave's columns of a state: all rows, in accumulators.
-template <typename ST, int D, int JT> struct State {
+// A wave's columns of a state: all rows, in accumulators. Column tile jt of wave w is the state's tile jt * WAVES + w. Products go over the rows that
+// there are, 64 at a time.
+template <typename ST, int D, int JT, int WAVES> struct State {
     static constexpr int KS = Operand<ST>::KS, PER = KS / 16, RT = D / 16, C = Operand<ST>::CHUNK, STEPS = C / KS;
     float4v s[RT][JT];
-    // Rows below `rows` and columns below `cols` of memory where neighbouring rows and columns are so far apart; zeros elsewhere or without memory.
-    __device__ __forceinline__ void read(const float *p, int rows, int cols, int row_step, int col_step, int col0)
+    int wave;
+    __device__ __forceinline__ int column(int jt) const { return (jt * WAVES + wave) * 16; }
+    // value = f(value, row, column) for this lane's values below `rows` and `cols`.
+    template <typename F> __device__ __forceinline__ void each(int rows, int cols, F f)
     {
         const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -296,36 +328,56 @@ template <typename ST, int D, int JT> struct State {
             for (int jt = 0; jt < JT; jt++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int row = rt * 16 + 4 * g + r, col = col0 + jt * 16 + n;
-                    s[rt][jt][r] = p != nullptr && row < rows && col < cols ? p[row * row_step + col * col_step] : 0.0f;
+                    const int row = rt * 16 + 4 * g + r, col = column(jt) + n;
+                    if (row < rows && col < cols) s[rt][jt][r] = f(s[rt][jt][r], row, col);
                 }
     }
-    __device__ __forceinline__ void write(float *p, int rows, int cols, int row_step, int col_step, int col0) const
+    __device__ __forceinline__ void clear()
     {
-        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) s[rt][jt] = float4v{0, 0, 0, 0};
+    }
+    // From and to memory where neighbouring rows and columns are so far apart (zeros without memory), and this lane's part of the product with it.
+    __device__ __forceinline__ void read(const float *p, int rows, int cols, int row_step, int col_step)
+    {
+        clear();
+        if (p != nullptr) each(rows, cols, [&](float, int row, int col) { return p[row * row_step + col * col_step]; });
+    }
+    __device__ __forceinline__ void write(float *p, int rows, int cols, int row_step, int col_step)
+    {
+        each(rows, cols, [&](float v, int row, int col) { return p[row * row_step + col * col_step] = v; });
+    }
+    __device__ __forceinline__ double dot(const float *p, int rows, int cols, int row_step, int col_step)
+    {
+        double sum = 0.0;
+        each(rows, cols, [&](float v, int row, int col) {
+            sum += (double)v * (double)p[row * row_step + col * col_step];
+            return v;
+        });
+        return sum;
+    }
+    // As the lanes hold it, tile by tile: to memory, and this lane's part of the product with one from there.
+    __device__ __forceinline__ void keep(float *p, int rows, int cols) const
+    {
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int jt = 0; jt < JT; jt++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = rt * 16 + 4 * g + r, col = col0 + jt * 16 + n;
-                    if (row < rows && col < cols) p[row * row_step + col * col_step] = s[rt][jt][r];
-                }
+                if (rt * 16 < rows && column(jt) < cols) reinterpret_cast<float4v *>(p)[(rt * RT + column(jt) / 16) * 64 + (threadIdx.x & 63)] = s[rt][jt];
     }
-    // This lane's part of the product with what lies in memory.
-    __device__ __forceinline__ double dot(const float *p, int rows, int cols, int row_step, int col_step, int col0) const
+    __device__ __forceinline__ double kept(const float *p, int rows, int cols) const
     {
-        const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
         double sum = 0.0;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int jt = 0; jt < JT; jt++)
+                if (rt * 16 < rows && column(jt) < cols) {
+                    const float4v other = reinterpret_cast<const float4v *>(p)[(rt * RT + column(jt) / 16) * 64 + (threadIdx.x & 63)];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = rt * 16 + 4 * g + r, col = col0 + jt * 16 + n;
-                    if (row < rows && col < cols) sum += (double)s[rt][jt][r] * (double)p[row * row_step + col * col_step];
+                    for (int r = 0; r < 4; r++) sum += (double)s[rt][jt][r] * (double)other[r];
                 }
         return sum;
     }
@@ -342,18 +394,8 @@ template <typename ST, int D, int JT> struct State {
                 for (int r = 0; r < 4; r++) most = __builtin_fmaxf(most, __builtin_fabsf(s[rt][jt][r]));
         return scale_to_fp16(most_of(most));
     }
-    // Rows ks * KS ... of column tile jt as an operand.
-    template <int TERMS> __device__ __forceinline__ void operand(int ks, int jt, float scale, frag_t<ST> (&out)[TERMS]) const
-    {
-        float x[4 * PER];
-#pragma unroll
-        for (int h = 0; h < PER; h++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) x[4 * h + r] = s[ks * PER + h][jt][r] * scale;
-        split<ST, TERMS>(x, out);
-    }
     // acc[tt][jt], columns: rows of `of` (tokens), rows: the state's columns: the state's product with them, times the power of two that is returned.
-    template <int TERMS> __device__ __forceinline__ float times(Tile<ST, D> of, float4v (&acc)[C / 16][JT]) const
+    template <int TERMS> __device__ __forceinline__ float times(Tile<ST, D> of, int rows, float4v (&acc)[C / 16][JT]) const
     {
         const float factor = scale();
 #pragma unroll
@@ -361,23 +403,35 @@ template <typename ST, int D, int JT> struct State {
 #pragma unroll
             for (int jt = 0; jt < JT; jt++) acc[tt][jt] = float4v{0, 0, 0, 0};
 #pragma unroll
-        for (int ks = 0; ks < D / KS; ks++) {
-            frag_t<ST> own[JT][TERMS];
+        for (int k0 = 0; k0 < D; k0 += 64) {
+            if (k0 >= rows) break;
 #pragma unroll
-            for (int jt = 0; jt < JT; jt++) operand<TERMS>(ks, jt, factor, own[jt]);
+            for (int k = k0; k < k0 + 64; k += KS) {
+                frag_t<ST> own[JT][TERMS];
 #pragma unroll
-            for (int tt = 0; tt < C / 16; tt++) {
-                const frag_t<ST> token = of.rows(tt * 16, ks * KS);
+                for (int jt = 0; jt < JT; jt++) {
+                    float x[4 * PER];
 #pragma unroll
-                for (int jt = 0; jt < JT; jt++)
+                    for (int h = 0; h < PER; h++)
 #pragma unroll
-                    for (int t = 0; t < TERMS; t++) acc[tt][jt] = mma(own[jt][t], token, acc[tt][jt]);
+                        for (int r = 0; r < 4; r++) x[4 * h + r] = s[k / 16 + h][jt][r] * factor;
+                    split<ST, TERMS>(x, own[jt]);
+                }
+#pragma unroll
+                for (int tt = 0; tt < C / 16; tt++) {
+                    const frag_t<ST> token = of.rows(tt * 16, k);
+#pragma unroll
+                    for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                        for (int t = 0; t < TERMS; t++) acc[tt][jt] = mma(own[jt][t], token, acc[tt][jt]);
+                }
             }
         }
         return factor;
     }
-    // s = decay s + sum over the chunk's tokens of rows[t] (weight[t] factor own[t])^T
-    template <int TERMS> __device__ __forceinline__ void update(Tile<ST, D> rows, const frag_t<ST> (&own)[JT][STEPS], const float *weight, float factor, float decay)
+    // s = decay s + sum over the chunk's tokens of from[t] (weight[t] factor own[t])^T
+    template <int TERMS>
+    __device__ __forceinline__ void update(Tile<ST, D> from, int rows, const frag_t<ST> (&own)[JT][STEPS], const float *weight, float factor, float decay)
     {
         const int g = (threadIdx.x & 63) >> 4;
         float bring = 1.0f;
@@ -416,12 +470,16 @@ template <typename ST, int D, int JT> struct State {
                 split<ST, TERMS>(x, scaled[jt]);
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                const frag_t<ST> row = rows.columns(rt * 16, step * KS);
+            for (int row0 = 0; row0 < D; row0 += 64) {
+                if (row0 >= rows) break;
 #pragma unroll
-                for (int jt = 0; jt < JT; jt++)
+                for (int rt = row0 / 16; rt < row0 / 16 + 4; rt++) {
+                    const frag_t<ST> row = from.columns(rt * 16, step * KS);
 #pragma unroll
-                    for (int t = 0; t < TERMS; t++) s[rt][jt] = mma(row, scaled[jt][t], s[rt][jt]);
+                    for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                        for (int t = 0; t < TERMS; t++) s[rt][jt] = mma(row, scaled[jt][t], s[rt][jt]);
+                }
             }
         }
         if constexpr (std::is_same_v<ST, _Float16>) {
@@ -431,30 +489,20 @@ template <typename ST, int D, int JT> struct State {
                 for (int jt = 0; jt < JT; jt++) s[rt][jt] *= 1.0f / bring;
         }
     }
-    // As the lanes hold it: to memory, and this lane's part of the product with one from there.
-    __device__ __forceinline__ void keep(float *p, int waves) const
-    {
-        const int64_t lanes = 64 * waves, lane = threadIdx.x % lanes;
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-            for (int jt = 0; jt < JT; jt++) reinterpret_cast<float4v *>(p)[(rt * JT + jt) * lanes + lane] = s[rt][jt];
-    }
-    __device__ __forceinline__ double kept(const float *p, int waves) const
-    {
-        const int64_t lanes = 64 * waves, lane = threadIdx.x % lanes;
-        double sum = 0.0;
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-            for (int jt = 0; jt < JT; jt++) {
-                const float4v other = reinterpret_cast<const float4v *>(p)[(rt * JT + jt) * lanes + lane];
-#pragma unroll
-                for (int r = 0; r < 4; r++) sum += (double)s[rt][jt][r] * (double)other[r];
-            }
-        return sum;
-    }
 };
+
+// A product of 16 tokens by 16 over their channels, 64 at a time.
+template <typename ST, int D> __device__ __forceinline__ float4v score(Tile<ST, D> a, int a0, Tile<ST, D> b, int b0, int channels)
+{
+    float4v p{0, 0, 0, 0};
+#pragma unroll
+    for (int k0 = 0; k0 < D; k0 += 64) {
+        if (k0 >= channels) break;
+#pragma unroll
+        for (int k = k0; k < k0 + 64; k += Operand<ST>::KS) p = mma(a.rows(a0, k), b.rows(b0, k), p);
+    }
+    return p;
+}
 
 // Chunks between borders whose products are taken from the states. For 128 x 128 values a head the states stored are 7 % of the bytes of a backward pass.
 constexpr int kBorder = 8;
@@ -499,35 +547,40 @@ __device__ __forceinline__ void pair_of(int id, int &i, int &j)
     j = id - i * (i + 1) / 2;
 }
 
-// Four neighbouring values of a token's output.
-template <typename ST> __device__ __forceinline__ void put4(ST *row, int col, int cols, float4v v)
+// Four neighbouring values of a token's output. EXACT: `cols` is a multiple of four.
+template <bool EXACT, typename ST> __device__ __forceinline__ void put4(ST *row, int col, int cols, float4v v)
 {
     const float f[4] = {v[0], v[1], v[2], v[3]};
-    if (col < cols) store_some<ST, 4>(row + col, cols - col, f);
+    if (col < cols) store_some<ST, 4>(row + col, EXACT ? 4 : cols - col, f);
 }
 
-template <typename ST, int D> constexpr int attend_waves() { return D == 256 ? 8 : 4; }
+// Waves of a workgroup, or in the pass over keys and values of each of its kinds: four with up to two tiles of 16 columns each. (Eight waves of one tile
+// read the shared operands twice as often: [8, 4096, 16 x 128] in bf16 201 us forwards, 164 so.)
+#ifndef GWPS
+#define GWPS 2
+#endif
+#ifndef GW
+#define GW 4
+#endif
+template <int D, bool GRAD = false> constexpr int attend_waves() { return D == 256 ? 8 : GRAD && D == 128 ? GW : 4; }
 
 // --- outputs (x, y, z = q, k, v) and, with GRAD, gradients of queries (x, y, z = do, v, k) with what decays read -----------------------
 template <typename ST, int D, bool GRAD> struct AttendLds {
-    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<ST, D>();
-    static constexpr int TILES = GRAD ? 4 : 3;
-    static constexpr int WORDS = TILES * Tile<ST, D>::WORDS + Scores<ST>::WORDS + Decays<C>::WORDS + (GRAD ? 2 * (C / 16) * C + W * C + 2 * W : 0);
+    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<D, GRAD>();
+    static constexpr int WORDS = 3 * Tile<ST, D>::WORDS + Scores<ST>::WORDS + Decays<C>::WORDS + (GRAD ? W * C + 2 * W : 0);
 };
-template <typename ST, int D, bool GRAD> __global__ __launch_bounds__((64 * attend_waves<ST, D>()), 2) void attend_kernel(AttendArgs args)
+template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global__ __launch_bounds__((64 * attend_waves<D, GRAD>()), (GRAD && D == 128 && GW == 8 ? GWPS : 2)) void attend_kernel(AttendArgs args)
 {
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * attend_waves<ST, D>(), W = NT / 64, JT = D / 16 / W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
-    constexpr int TERMS = kTerms<ST>, READ_TERMS = GRAD ? kTerms<ST> : 1;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D, GRAD>(), NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const scanscam_attend &a = args.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4, col0 = wave * JT * 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
     float *at = lds;
     const auto take = [&](int words) { float *p = at; at += words; return p; };
     Tile<ST, D> X{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Y{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Z{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))};
-    Tile<ST, D> Q{GRAD ? reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS)) : nullptr};
     Scores<ST> scores{reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS))};
     Decays<C> decays{reinterpret_cast<double *>(take(2 * C)), take(C), take(C)};
-    float *rows = GRAD ? take(TT * C) : nullptr, *cols = GRAD ? take(TT * C) : nullptr, *red = GRAD ? take(W * C) : nullptr;
+    float *red = GRAD ? take(W * C) : nullptr;
     double *last = GRAD ? reinterpret_cast<double *>(take(2 * W)) : nullptr;
 
     const Span span = span_of(args, args.first + blockIdx.x, C);
@@ -539,13 +592,17 @@ template <typename ST, int D, bool GRAD> __global__ __launch_bounds__((64 * atte
     const int inner = GRAD ? V : K, outer = GRAD ? K : V;  // rows and columns of the state as it is held here
     const int row_step = GRAD ? 1 : V, col_step = GRAD ? V : 1;
     const int64_t pair = span.sequence * a.heads + span.head;
+    // Where this lane's outputs go: token n16 of a tile, four columns from 4 g on of each of its tiles.
+    const int64_t out_step = GRAD ? args.part_q != nullptr ? a.heads * K : a.gq.token : a.y.token;
+    const int64_t out_first = GRAD ? args.part_q != nullptr ? (span.batch * a.T * a.heads + span.head) * K : span.batch * a.gq.batch + span.head * a.gq.group
+                                   : span.batch * a.y.batch + span.head * a.y.group;
 
-    State<ST, D, JT> S;
-    const float *from = args.parts > 1 ? args.ends + span.unit * K * V : a.state_in == nullptr ? nullptr : a.state_in + pair * K * V;
-    S.read(from, inner, outer, row_step, col_step, col0);
+    State<ST, D, JT, W> S;
+    S.wave = wave;
+    S.read(args.parts > 1 ? args.ends + span.unit * K * V : a.state_in == nullptr ? nullptr : a.state_in + pair * K * V, inner, outer, row_step, col_step);
     scores.clear();
 
-    Staged<ST, D, NT> sx, sy, sz, sq;
+    Staged<ST, D, NT, EXACT> sx, sy, sz;
     double decay = 0.0;
     const auto ask = [&](int64_t t) {
         const int n = (int)(span.end - t < C ? span.end - t : C);
@@ -553,101 +610,113 @@ template <typename ST, int D, bool GRAD> __global__ __launch_bounds__((64 * atte
         sx.load(x + t * xt.token, (int)xt.token, n, inner);
         sy.load(y + t * yt.token, (int)yt.token, n, inner);
         sz.load(z + t * zt.token, (int)zt.token, n, outer);
-        if constexpr (GRAD) sq.load(q + t * a.q.token, (int)a.q.token, n, outer);
     };
     if (span.begin < span.end) ask(span.begin);
     for (int64_t t0 = span.begin; t0 < span.end; t0 += C) {
         const int n = (int)(span.end - t0 < C ? span.end - t0 : C);
-        sx.store(X);
-        sy.store(Y);
-        sz.store(Z);
-        if constexpr (GRAD) sq.store(Q);
+        sx.store(X, n, inner);
+        sy.store(Y, n, inner);
+        sz.store(Z, n, outer);
         if (wave == 0) decays.fill(decay);
         __syncthreads();
+        // This lane's part of the queries, which only the sums over channels need.
+        Elems<ST, 4> queries[TT][JT];
+        if constexpr (GRAD) {
+            using raw_t = typename RawT<4 * sizeof(ST)>::type;
+            typedef raw_t unaligned __attribute__((aligned(sizeof(ST))));
+#pragma unroll
+            for (int tt = 0; tt < TT; tt++)
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++) {
+                    const int t = tt * 16 + n16, col = S.column(jt) + 4 * g;
+                    const ST *from = q + (t0 + (t < n ? t : n - 1)) * a.q.token + (col < outer ? col : 0);
+                    if (EXACT || col + 4 <= outer) {
+                        const raw_t raw = *reinterpret_cast<const unaligned *>(from);
+                        queries[tt][jt] = __builtin_bit_cast(Elems<ST, 4>, raw);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) queries[tt][jt].e[r] = col + r < outer ? from[r] : (ST)0.0f;
+                    }
+                }
+        }
         if (t0 + C < span.end) ask(t0 + C);
 
-        // Scores: tiles of 16 tokens s (rows) by 16 tokens t (columns), t >= s.
-        for (int id = wave; id < TT * (TT + 1) / 2; id += W) {
+        // Scores: tiles of 16 tokens s (rows) by 16 tokens t (columns), t >= s. (The first wave, which has the decays, is not among those with one more.)
+        for (int id = (wave + 2) % W; id < TT * (TT + 1) / 2; id += W) {
             int tt, st;
             pair_of(id, tt, st);
-            float4v p{0, 0, 0, 0}, other{0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < D; k += KS) {
-                p = mma(Y.rows(st * 16, k), X.rows(tt * 16, k), p);
-                if constexpr (GRAD) other = mma(Z.rows(st * 16, k), Q.rows(tt * 16, k), other);
-            }
+            float4v p = score(Y, st * 16, X, tt * 16, inner);
             const double upto = decays.sums[tt * 16 + n16];
-            float over_s = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int s = st * 16 + 4 * g + r, t = tt * 16 + n16;
-                const float w = exp2_(upto - decays.sums[s]);
-                p[r] = s <= t ? p[r] * w : 0.0f;
-                if constexpr (GRAD) {
-                    const float m = s < t ? p[r] * other[r] * a.scale : 0.0f;
-                    over_s += m;
-                    const float over_t = row_sum(m);
-                    if (n16 == 15) cols[tt * C + s] = over_t;
-                }
-            }
-            if constexpr (GRAD) {
-                over_s = column_sum4(over_s);
-                if (g == 0) rows[st * C + tt * 16 + n16] = over_s;
+                p[r] = s <= t ? p[r] * (exp2_(upto - decays.sums[s]) * a.scale) : 0.0f;
             }
             scores.put(tt, st, p);
         }
+        float4v acc[TT][JT];
+        const float factor = a.scale / S.template times<GRAD ? TERMS : 1>(X, inner, acc);
+        if constexpr (GRAD)
+            if (args.borders != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0)
+                S.keep(args.borders + border_at(args, span.batch, t0, C, span.head) * D * D, inner, outer);
         frag_t<ST> own[JT][STEPS];
 #pragma unroll
         for (int jt = 0; jt < JT; jt++)
 #pragma unroll
-            for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(col0 + jt * 16, step * KS);
-        float4v acc[TT][JT];
-        const float unscale = 1.0f / S.template times<READ_TERMS>(X, acc);
-        if constexpr (GRAD)
-            if (args.borders != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0) S.keep(args.borders + border_at(args, span.batch, t0, C, span.head) * D * D, W);
+            for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(S.column(jt), step * KS);
         __syncthreads();
 
 #pragma unroll
         for (int tt = 0; tt < TT; tt++) {
             const int t = tt * 16 + n16;
-            const float upto = decays.upto[t] * unscale;
+            const float upto = decays.upto[t] * factor;
             float read = 0.0f, finite = 0.0f;
+            float4v sum[JT];
 #pragma unroll
             for (int jt = 0; jt < JT; jt++) {
                 acc[tt][jt] *= upto;
                 if constexpr (GRAD) {
-                    float query[4];
-                    Q.four(t, col0 + jt * 16 + 4 * g, query);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) read += query[r] * acc[tt][jt][r];
+                    for (int r = 0; r < 4; r++) read += (float)queries[tt][jt].e[r] * acc[tt][jt][r];
                 }
-                float4v sum = acc[tt][jt];
+                sum[jt] = acc[tt][jt];
+            }
 #pragma unroll
-                for (int step = 0; step <= tt / PER; step++) sum = mma(own[jt][step], scores.operand(tt, step), sum);
-                if constexpr (!GRAD) {
+            for (int step = 0; step <= tt / PER; step++) {
+                const frag_t<ST> p = scores.operand(tt, step);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) finite += sum[r] * 0.0f;
-                    if (__builtin_expect(__ballot(finite != 0.0f) != 0, 0)) {
-                        // A value that is not finite may be a later token's, times a score of zero: the tokens up to t alone.
-                        sum = acc[tt][jt];
+                for (int jt = 0; jt < JT; jt++) sum[jt] = mma(own[jt][step], p, sum[jt]);
+            }
+            if constexpr (!GRAD) {
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) finite += sum[jt][r] * 0.0f;
+                if (__builtin_expect(__ballot(finite != 0.0f) != 0, 0)) {
+                    // A value that is not finite may be a later token's, times a score of zero: the tokens up to t alone.
+                    for (int jt = 0; jt < JT; jt++) {
+                        sum[jt] = acc[tt][jt];
                         for (int s = 0; s <= t; s++) {
                             float value[4];
-                            Z.four(s, col0 + jt * 16 + 4 * g, value);
+                            Z.four(s, S.column(jt) + 4 * g, value);
                             const float p = scores.at(s, t);
 #pragma unroll
-                            for (int r = 0; r < 4; r++) sum[r] += p * value[r];
+                            for (int r = 0; r < 4; r++) sum[jt][r] += p * value[r];
                         }
                     }
                 }
-                sum *= a.scale;
-                if (t < n) {
-                    const int col = col0 + jt * 16 + 4 * g;
+            }
+            if (t < n) {
+                const int64_t row = out_first + (t0 + t) * out_step;
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++) {
+                    const int col = S.column(jt) + 4 * g;
                     if constexpr (!GRAD) {
-                        put4(static_cast<ST *>(a.y.p) + span.batch * a.y.batch + (t0 + t) * a.y.token + span.head * a.y.group, col, V, sum);
+                        put4<EXACT>(static_cast<ST *>(a.y.p) + row, col, V, sum[jt]);
                     } else if (args.part_q != nullptr) {
-                        put4(args.part_q + ((span.batch * a.T + t0 + t) * a.heads + span.head) * K, col, K, sum);
+                        put4<EXACT>(args.part_q + row, col, K, sum[jt]);
                     } else {
-                        put4(static_cast<ST *>(a.gq.p) + span.batch * a.gq.batch + (t0 + t) * a.gq.token + span.head * a.gq.group, col, K, sum);
+                        put4<EXACT>(static_cast<ST *>(a.gq.p) + row, col, K, sum[jt]);
                     }
                 }
             }
@@ -656,24 +725,22 @@ template <typename ST, int D, bool GRAD> __global__ __launch_bounds__((64 * atte
                 if (g == 0) red[wave * C + t] = read;
             }
         }
-        S.template update<TERMS>(Y, own, decays.after, 1.0f, decays.whole());
+        S.template update<TERMS>(Y, inner, own, decays.after, 1.0f, decays.whole());
         __syncthreads();
         if constexpr (GRAD) {
             if (threadIdx.x < (unsigned)n && args.reads != nullptr) {
                 const int t = threadIdx.x;
-                float read = 0.0f, inside = 0.0f;
+                float read = 0.0f;
                 for (int w = 0; w < W; w++) read += red[w * C + t];
-                for (int st = 0; st <= t / 16; st++) inside += rows[st * C + t];
-                for (int tt = t / 16; tt < TT; tt++) inside -= cols[tt * C + t];
-                args.reads[span.head * args.tokens + span.batch * a.T + t0 + t] = read * a.scale + inside;
+                args.reads[span.head * args.tokens + span.batch * a.T + t0 + t] = read;
             }
         }
     }
     if (span.part == args.parts - 1) {
         if constexpr (!GRAD) {
-            if (a.state_out != nullptr) S.write(a.state_out + pair * K * V, inner, outer, row_step, col_step, col0);
+            if (a.state_out != nullptr) S.write(a.state_out + pair * K * V, inner, outer, row_step, col_step);
         } else if (args.last != nullptr) {
-            double sum = a.gstate_out == nullptr ? 0.0 : S.dot(a.gstate_out + pair * K * V, inner, outer, row_step, col_step, col0);
+            double sum = a.gstate_out == nullptr ? 0.0 : S.dot(a.gstate_out + pair * K * V, inner, outer, row_step, col_step);
             sum = sums_upto(sum);
             if (lane == 63) last[wave] = sum;
             __syncthreads();
@@ -690,12 +757,12 @@ template <typename ST, int D, bool GRAD> __global__ __launch_bounds__((64 * atte
 template <typename ST, int D> struct EndsLds {
     static constexpr int WORDS = 2 * Tile<ST, D>::WORDS + Decays<Operand<ST>::CHUNK>::WORDS;
 };
-template <typename ST, int D, bool BACK> __global__ __launch_bounds__((64 * attend_waves<ST, D>()), 2) void ends_kernel(AttendArgs args)
+template <typename ST, int D, int JT, bool BACK, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * attend_waves<D>(), 2) void ends_kernel(AttendArgs args)
 {
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * attend_waves<ST, D>(), W = NT / 64, JT = D / 16 / W, STEPS = C / KS;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * W, STEPS = C / KS;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const scanscam_attend &a = args.a;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col0 = wave * JT * 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Tile<ST, D> Y{reinterpret_cast<ST *>(lds)}, Z{reinterpret_cast<ST *>(lds + Tile<ST, D>::WORDS)};
     float *rest = lds + 2 * Tile<ST, D>::WORDS;
     Decays<C> decays{reinterpret_cast<double *>(rest), rest + 2 * C, rest + 3 * C};
@@ -706,9 +773,10 @@ template <typename ST, int D, bool BACK> __global__ __launch_bounds__((64 * atte
     const int64_t shared = span.head / args.each;
     const ST *y = tensor_at<ST>(yt, span, BACK ? span.head : shared), *z = tensor_at<ST>(zt, span, BACK ? shared : span.head);
     const int inner = BACK ? V : K, outer = BACK ? K : V, row_step = BACK ? 1 : V, col_step = BACK ? V : 1;
-    State<ST, D, JT> S;
-    S.read(nullptr, inner, outer, row_step, col_step, col0);
-    Staged<ST, D, NT> sy, sz;
+    State<ST, D, JT, W> S;
+    S.wave = wave;
+    S.clear();
+    Staged<ST, D, NT, EXACT> sy, sz;
     double decay = 0.0, whole = 0.0;
     const auto ask = [&](int64_t t) {
         const int n = (int)(span.end - t < C ? span.end - t : C);
@@ -720,8 +788,9 @@ template <typename ST, int D, bool BACK> __global__ __launch_bounds__((64 * atte
     const auto token = [&](int64_t c) { return span.begin + (BACK ? chunks - 1 - c : c) * C; };
     if (chunks > 0) ask(token(0));
     for (int64_t c = 0; c < chunks; c++) {
-        sy.store(Y);
-        sz.store(Z);
+        const int n = (int)(span.end - token(c) < C ? span.end - token(c) : C);
+        sy.store(Y, n, inner);
+        sz.store(Z, n, outer);
         if (wave == 0) {
             decays.fill(decay);
             whole += read_lane(sums_upto(decay), 63);
@@ -732,56 +801,59 @@ template <typename ST, int D, bool BACK> __global__ __launch_bounds__((64 * atte
 #pragma unroll
         for (int jt = 0; jt < JT; jt++)
 #pragma unroll
-            for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(col0 + jt * 16, step * KS);
-        S.template update<kTerms<ST>>(Y, own, BACK ? decays.upto : decays.after, BACK ? a.scale : 1.0f, decays.whole());
+            for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(S.column(jt), step * KS);
+        S.template update<TERMS>(Y, inner, own, BACK ? decays.upto : decays.after, BACK ? a.scale : 1.0f, decays.whole());
         __syncthreads();
     }
-    S.write((BACK ? args.back_ends : args.ends) + span.unit * K * V, inner, outer, row_step, col_step, col0);
+    S.write((BACK ? args.back_ends : args.ends) + span.unit * K * V, inner, outer, row_step, col_step);
     if (threadIdx.x == 0) args.logs[span.unit] = whole;
 }
 
 // --- gradients of keys and values, backwards in time ------------------------------------------------------------------------------------
-// Two kinds of waves share the tiles: those of dk hold H with the values' channels as rows, those of dv with the keys'. BOTH: four waves of each;
-// else (256 channels: one kind's accumulators alone are half of a CU's registers) a workgroup is of one kind.
-template <typename ST, int D> constexpr bool attend_both() { return D < 256; }
+// Two kinds of waves share the tiles: those of dk hold H with the values' channels as rows, those of dv with the keys'. Up to 128 channels four waves of
+// each; else (one kind's accumulators alone are half of a CU's registers) a workgroup is of one kind. float32 results come from dk's waves: theirs
+// are the products in several terms, and dv's waves compute the scores of both.
+template <int D> constexpr bool attend_both() { return D < 256; }
+template <int D> constexpr int back_waves() { return attend_waves<D>() * (attend_both<D>() ? 2 : 1); }
 template <typename ST, int D> struct BackLds {
-    static constexpr int C = Operand<ST>::CHUNK, W = attend_both<ST, D>() ? 4 : 8;
-    static constexpr int WORDS = 4 * Tile<ST, D>::WORDS + (attend_both<ST, D>() ? 2 : 1) * Scores<ST>::WORDS + Decays<C>::WORDS + W * C + 2 * W;
+    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<D>();
+    static constexpr int WORDS = 4 * Tile<ST, D>::WORDS + (attend_both<D>() ? 2 : 1) * Scores<ST>::WORDS + Decays<C>::WORDS + W * C + 2 * W + 2 * (C / 16) * C;
 };
-template <typename ST, int D> __global__ __launch_bounds__(512, 2) void attend_back_kernel(AttendArgs args)
+template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forceinline__ void back_pass(const AttendArgs &args, float *lds)
 {
-    constexpr bool BOTH = attend_both<ST, D>();
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 512, W = BOTH ? 4 : 8, JT = D / 16 / W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
-    extern __shared__ __attribute__((aligned(16))) float lds[];
+    constexpr bool BOTH = attend_both<D>();
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * back_waves<D>(), STEPS = C / KS, TT = C / 16, PER = KS / 16, TERMS = KEYS ? kTerms<ST> : 1;
     const scanscam_attend &a = args.a;
-    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
-    const bool keys = BOTH ? all < W : blockIdx.y == 0;  // dk
-    const int wave = BOTH ? all % W : all, col0 = wave * JT * 16;
+    const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % W, n16 = lane & 15, g = lane >> 4;
     float *at = lds;
     const auto take = [&](int words) { float *p = at; at += words; return p; };
     Tile<ST, D> Q{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Kt{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))}, Vt{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))},
         O{reinterpret_cast<ST *>(take(Tile<ST, D>::WORDS))};
-    // Of the waves' own kind: do v (dk) or q k (dv).
-    frag_t<ST> *first_scores = reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS)), *second_scores = BOTH ? reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS)) : first_scores;
-    Scores<ST> scores{keys ? first_scores : second_scores};
+    // do v, of which dk is made, and q k, of which dv is.
+    Scores<ST> of_keys{reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS))}, of_values{BOTH ? reinterpret_cast<frag_t<ST> *>(take(Scores<ST>::WORDS)) : of_keys.p};
+    const Scores<ST> scores = KEYS ? of_keys : of_values;
     Decays<C> decays{reinterpret_cast<double *>(take(2 * C)), take(C), take(C)};
     float *red = take(W * C);
     double *over = reinterpret_cast<double *>(take(2 * W));
+    float *rows = take(TT * C), *cols = take(TT * C);  // sums of M over each tile's rows and columns
 
     const Span span = span_of(args, args.first + blockIdx.x, C);
     const int64_t shared = span.head / args.each, pair = span.sequence * a.heads + span.head;
     const int K = (int)a.K, V = (int)a.V;
     const ST *q = tensor_at<ST>(a.q, span, shared), *k = tensor_at<ST>(a.k, span, shared), *v = tensor_at<ST>(a.v, span, span.head), *o = tensor_at<ST>(a.gy, span, span.head);
-    const Tile<ST, D> inter = keys ? Vt : Kt, update_rows = keys ? O : Q, mine = keys ? Q : O;
-    const int inner = keys ? V : K, outer = keys ? K : V, row_step = keys ? 1 : V, col_step = keys ? V : 1;
+    const Tile<ST, D> inter = KEYS ? Vt : Kt, update_rows = KEYS ? O : Q, mine = KEYS ? Q : O;
+    const int inner = KEYS ? V : K, outer = KEYS ? K : V, row_step = KEYS ? 1 : V, col_step = KEYS ? V : 1;
+    const int64_t out_step = !KEYS ? a.gv.token : args.part_k != nullptr ? a.heads * K : a.gk.token;
+    const int64_t out_first = !KEYS ? span.batch * a.gv.batch + span.head * a.gv.group
+                              : args.part_k != nullptr ? (span.batch * a.T * a.heads + span.head) * K : span.batch * a.gk.batch + span.head * a.gk.group;
 
-    State<ST, D, JT> H;
-    const float *from = args.parts > 1 ? args.back_ends + span.unit * K * V : a.gstate_out == nullptr ? nullptr : a.gstate_out + pair * K * V;
-    H.read(from, inner, outer, row_step, col_step, col0);
-    Scores<ST>{first_scores}.clear();
-    if constexpr (BOTH) Scores<ST>{second_scores}.clear();
+    State<ST, D, JT, W> H;
+    H.wave = wave;
+    H.read(args.parts > 1 ? args.back_ends + span.unit * K * V : a.gstate_out == nullptr ? nullptr : a.gstate_out + pair * K * V, inner, outer, row_step, col_step);
+    of_keys.clear();
+    if constexpr (BOTH) of_values.clear();
 
-    Staged<ST, D, NT> sq, sk, sv, so;
+    Staged<ST, D, NT, EXACT> sq, sk, sv, so;
     double decay = 0.0;
     const auto ask = [&](int64_t t) {
         const int n = (int)(span.end - t < C ? span.end - t : C);
@@ -796,38 +868,51 @@ template <typename ST, int D> __global__ __launch_bounds__(512, 2) void attend_b
     for (int64_t c = chunks - 1; c >= 0; c--) {
         const int64_t t0 = span.begin + c * C;
         const int n = (int)(span.end - t0 < C ? span.end - t0 : C);
-        sq.store(Q);
-        sk.store(Kt);
-        sv.store(Vt);
-        so.store(O);
+        sq.store(Q, n, K);
+        sk.store(Kt, n, K);
+        sv.store(Vt, n, V);
+        so.store(O, n, V);
         if (all == 0) decays.fill(decay);
         __syncthreads();
         if (c > 0) ask(t0 - C);
 
-        // Scores: tiles of 16 tokens t (rows) by 16 tokens s (columns), t >= s.
-        for (int id = wave; id < TT * (TT + 1) / 2; id += W) {
-            int tt, st;
-            pair_of(id, tt, st);
-            float4v p{0, 0, 0, 0};
-            const Tile<ST, D> of = keys ? O : Q;
+        // Scores: tiles of 16 tokens t (rows) by 16 tokens s (columns), t >= s, and of both M.
+        if (!BOTH || !KEYS) {
+            for (int id = (wave + 2) % W; id < TT * (TT + 1) / 2; id += W) {
+                int tt, st;
+                pair_of(id, tt, st);
+                float4v p{0, 0, 0, 0}, other{0, 0, 0, 0};
+                if (BOTH || KEYS) p = score(O, tt * 16, Vt, st * 16, V);
+                other = score(Q, tt * 16, Kt, st * 16, K);
+                const double from_s = decays.sums[st * 16 + n16];
+                float over_t = 0.0f;
 #pragma unroll
-            for (int d = 0; d < D; d += KS) p = mma(of.rows(tt * 16, d), inter.rows(st * 16, d), p);
-            const double from_s = decays.sums[st * 16 + n16];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int s = st * 16 + n16, t = tt * 16 + 4 * g + r;
-                const float w = exp2_(decays.sums[t] - from_s);
-                p[r] = s <= t ? p[r] * (w * a.scale) : 0.0f;
+                for (int r = 0; r < 4; r++) {
+                    const int s = st * 16 + n16, t = tt * 16 + 4 * g + r;
+                    const float w = exp2_(decays.sums[t] - from_s) * a.scale;
+                    if (BOTH || KEYS) {
+                        const float m = s < t ? p[r] * other[r] * w : 0.0f, over_s = row_sum(m);
+                        over_t += m;
+                        if (n16 == 15) rows[st * C + t] = over_s;
+                    }
+                    p[r] = s <= t ? p[r] * w : 0.0f;
+                    other[r] = s <= t ? other[r] * w : 0.0f;
+                }
+                if (BOTH || KEYS) {
+                    over_t = column_sum4(over_t);
+                    if (g == 0) cols[tt * C + st * 16 + n16] = over_t;
+                    of_keys.put(st, tt, p);
+                }
+                if (BOTH || !KEYS) of_values.put(st, tt, other);
             }
-            scores.put(st, tt, p);
         }
+        float4v acc[TT][JT];
+        const float unscale = 1.0f / H.template times<TERMS>(inter, inner, acc);
         frag_t<ST> own[JT][STEPS];
 #pragma unroll
         for (int jt = 0; jt < JT; jt++)
 #pragma unroll
-            for (int step = 0; step < STEPS; step++) own[jt][step] = mine.columns(col0 + jt * 16, step * KS);
-        float4v acc[TT][JT];
-        const float unscale = 1.0f / H.template times<kTerms<ST>>(inter, acc);
+            for (int step = 0; step < STEPS; step++) own[jt][step] = mine.columns(H.column(jt), step * KS);
         __syncthreads();
 
 #pragma unroll
@@ -838,53 +923,84 @@ template <typename ST, int D> __global__ __launch_bounds__(512, 2) void attend_b
 #pragma unroll
             for (int jt = 0; jt < JT; jt++) {
                 acc[st][jt] *= after;
-                float key[4];
-                Kt.four(s, col0 + jt * 16 + 4 * g, key);
+                if constexpr (KEYS) {
+                    float key[4];
+                    Kt.four(s, H.column(jt) + 4 * g, key);
 #pragma unroll
-                for (int r = 0; r < 4; r++) write += key[r] * acc[st][jt][r];
-                float4v sum = acc[st][jt];
+                    for (int r = 0; r < 4; r++) write += key[r] * acc[st][jt][r];
+                }
+            }
 #pragma unroll
-                for (int step = st / PER; step < STEPS; step++) sum = mma(own[jt][step], scores.operand(st, step), sum);
-                if (s < n) {
-                    const int col = col0 + jt * 16 + 4 * g;
-                    if (!keys) {
-                        put4(static_cast<ST *>(a.gv.p) + span.batch * a.gv.batch + (t0 + s) * a.gv.token + span.head * a.gv.group, col, V, sum);
+            for (int step = st / PER; step < STEPS; step++) {
+                const frag_t<ST> p = scores.operand(st, step);
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++) acc[st][jt] = mma(own[jt][step], p, acc[st][jt]);
+            }
+            if (s < n) {
+                const int64_t row = out_first + (t0 + s) * out_step;
+#pragma unroll
+                for (int jt = 0; jt < JT; jt++) {
+                    const int col = H.column(jt) + 4 * g;
+                    if constexpr (!KEYS) {
+                        put4<EXACT>(static_cast<ST *>(a.gv.p) + row, col, V, acc[st][jt]);
                     } else if (args.part_k != nullptr) {
-                        put4(args.part_k + ((span.batch * a.T + t0 + s) * a.heads + span.head) * K, col, K, sum);
+                        put4<EXACT>(args.part_k + row, col, K, acc[st][jt]);
                     } else {
-                        put4(static_cast<ST *>(a.gk.p) + span.batch * a.gk.batch + (t0 + s) * a.gk.token + span.head * a.gk.group, col, K, sum);
+                        put4<EXACT>(static_cast<ST *>(a.gk.p) + row, col, K, acc[st][jt]);
                     }
                 }
             }
-            write = column_sum4(write);
-            if (keys && g == 0) red[wave * C + s] = write;
+            if constexpr (KEYS) {
+                write = column_sum4(write);
+                if (g == 0) red[wave * C + s] = write;
+            }
         }
-        H.template update<kTerms<ST>>(update_rows, own, decays.upto, a.scale, decays.whole());
-        const bool border = args.cross != nullptr && keys && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0;
-        const int64_t at_border = border ? border_at(args, span.batch, t0, C, span.head) : 0;
-        if (border) {
-            const double sum = sums_upto(H.kept(args.borders + at_border * D * D, W));
-            if (lane == 63) over[wave] = sum;
-        }
-        __syncthreads();
-        if (border && threadIdx.x == 0) {
-            double sum = 0.0;
-            for (int w = 0; w < W; w++) sum += over[w];
-            args.cross[at_border] = sum;
-        }
-        if (keys && args.writes != nullptr && threadIdx.x < (unsigned)n) {
-            float write = 0.0f;
-            for (int w = 0; w < W; w++) write += red[w * C + threadIdx.x];
-            args.writes[span.head * args.tokens + span.batch * a.T + t0 + threadIdx.x] = write;
+        H.template update<TERMS>(update_rows, inner, own, decays.upto, a.scale, decays.whole());
+        if constexpr (KEYS) {
+            const bool border = args.cross != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0;
+            const int64_t at_border = border ? border_at(args, span.batch, t0, C, span.head) : 0;
+            if (border) {
+                const double sum = sums_upto(H.kept(args.borders + at_border * D * D, inner, outer));
+                if (lane == 63) over[wave] = sum;
+            }
+            __syncthreads();
+            if (border && all == 0 && lane == 0) {
+                double sum = 0.0;
+                for (int w = 0; w < W; w++) sum += over[w];
+                args.cross[at_border] = sum;
+            }
+            if (args.writes != nullptr && threadIdx.x < (unsigned)n) {
+                float write = 0.0f;
+                for (int w = 0; w < W; w++) write += red[w * C + threadIdx.x];
+                const int t = threadIdx.x;
+                float inside = 0.0f;
+                for (int st = 0; st <= t / 16; st++) inside += rows[st * C + t];
+                for (int tt = t / 16; tt < TT; tt++) inside -= cols[tt * C + t];
+                const int64_t at = span.head * args.tokens + span.batch * a.T + t0 + t;
+                args.writes[at] = write;
+                args.inside[at] = inside;
+            }
+        } else {
+            __syncthreads();
         }
     }
-    if (keys && span.part == 0 && a.gstate_in != nullptr) H.write(a.gstate_in + pair * K * V, inner, outer, row_step, col_step, col0);
+    if constexpr (KEYS)
+        if (span.part == 0 && a.gstate_in != nullptr) H.write(a.gstate_in + pair * K * V, inner, outer, row_step, col_step);
+}
+// JK, JV: column tiles of dk's and dv's waves. (The kinds meet at the same barriers: each pass has three a chunk.)
+template <typename ST, int D, int JK, int JV, bool EXACT> __global__ __launch_bounds__(64 * back_waves<D>(), 2) void attend_back_kernel(AttendArgs args)
+{
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (attend_both<D>() ? wave < attend_waves<D>() : blockIdx.y == 0) back_pass<ST, D, JK, true, EXACT>(args, lds);
+    else back_pass<ST, D, JV, false, EXACT>(args, lds);
 }
 
 // --- launches by type ---------------------------------------------------------------------------------------------------------------------
-enum AttendPass { kOutputs, kQueries, kKeysAndValues, kEnds, kBackEnds };
+// kOutputsOnce: no state is handed over, so that what is added to it is rounded to one term.
+enum AttendPass { kOutputs, kOutputsOnce, kQueries, kKeysAndValues, kEnds, kBackEnds };
 
-// A workgroup's lanes' values of a state.
+// Channels that a call's tiles have room for.
 inline int attend_width(const scanscam_attend &a)
 {
     const int64_t most = a.K > a.V ? a.K : a.V;
@@ -906,24 +1022,47 @@ template <auto Kernel, int WORDS> hipError_t launch_attend_units(int64_t units, 
     return hipSuccess;
 }
 
-template <typename ST, int D> hipError_t launch_attend_with(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
+// Column tiles of a wave by the columns that there are: a head of up to 64 (of the 256 kind 128) leaves half of the waves' registers and products out.
+template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
 {
-    constexpr int threads = 64 * attend_waves<ST, D>();
+    constexpr int threads = 64 * attend_waves<D>(), grad_threads = 64 * attend_waves<D, true>(), back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, T = kTerms<ST>;
+    constexpr int out = AttendLds<ST, D, false>::WORDS, grad = AttendLds<ST, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
+    const bool k_half = ALL == 2 && args.a.K <= D / 2, v_half = ALL == 2 && args.a.V <= D / 2;
+    const unsigned kinds = attend_both<D>() ? 1 : 2;
     switch (pass) {
-    case kOutputs: return launch_attend_units<attend_kernel<ST, D, false>, AttendLds<ST, D, false>::WORDS>(units, 1, threads, stream, args);
-    case kQueries: return launch_attend_units<attend_kernel<ST, D, true>, AttendLds<ST, D, true>::WORDS>(units, 1, threads, stream, args);
-    case kKeysAndValues: return launch_attend_units<attend_back_kernel<ST, D>, BackLds<ST, D>::WORDS>(units, attend_both<ST, D>() ? 1 : 2, 512, stream, args);
-    case kBackEnds: return launch_attend_units<ends_kernel<ST, D, true>, EndsLds<ST, D>::WORDS>(units, 1, threads, stream, args);
-    default: return launch_attend_units<ends_kernel<ST, D, false>, EndsLds<ST, D>::WORDS>(units, 1, threads, stream, args);
+    case kOutputs:
+        return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, T, EXACT>, out>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, false, T, EXACT>, out>(units, 1, threads, stream, args);
+    case kOutputsOnce:
+        return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, 1, EXACT>, out>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, false, 1, EXACT>, out>(units, 1, threads, stream, args);
+    case kQueries:
+        return k_half ? launch_attend_units<attend_kernel<ST, D, 1, true, T, EXACT>, grad>(units, 1, grad_threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, D / 16 / attend_waves<D, true>(), true, T, EXACT>, grad>(units, 1, grad_threads, stream, args);
+    case kKeysAndValues:  // (both are not halves at once)
+        if (k_half) return launch_attend_units<attend_back_kernel<ST, D, 1, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
+        if (v_half) return launch_attend_units<attend_back_kernel<ST, D, ALL, 1, EXACT>, back>(units, kinds, back_threads, stream, args);
+        return launch_attend_units<attend_back_kernel<ST, D, ALL, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
+    case kEnds:
+        return v_half ? launch_attend_units<ends_kernel<ST, D, 1, false, T, EXACT>, ends>(units, 1, threads, stream, args)
+                      : launch_attend_units<ends_kernel<ST, D, ALL, false, T, EXACT>, ends>(units, 1, threads, stream, args);
+    default:
+        return k_half ? launch_attend_units<ends_kernel<ST, D, 1, true, T, EXACT>, ends>(units, 1, threads, stream, args)
+                      : launch_attend_units<ends_kernel<ST, D, ALL, true, T, EXACT>, ends>(units, 1, threads, stream, args);
     }
+}
+template <typename ST, int D> hipError_t launch_attend_of(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
+{
+    constexpr int64_t vector = 16 / sizeof(ST);
+    return args.a.K % vector == 0 && args.a.V % vector == 0 ? launch_attend_with<ST, D, true>(pass, units, stream, args) : launch_attend_with<ST, D, false>(pass, units, stream, args);
 }
 #define SCANSCAM_DEFINE_ATTEND_LAUNCH(ST)                                                                                                        \
     template <> hipError_t launch_attend<ST>(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)                         \
     {                                                                                                                                            \
         const int width = attend_width(args.a);                                                                                                  \
-        return width == 64    ? launch_attend_with<ST, 64>(pass, units, stream, args)                                                            \
-               : width == 128 ? launch_attend_with<ST, 128>(pass, units, stream, args)                                                           \
-                              : launch_attend_with<ST, 256>(pass, units, stream, args);                                                          \
+        return width == 64    ? launch_attend_of<ST, 64>(pass, units, stream, args)                                                              \
+               : width == 128 ? launch_attend_of<ST, 128>(pass, units, stream, args)                                                             \
+                              : launch_attend_of<ST, 256>(pass, units, stream, args);                                                            \
     }
 
 }  // namespace scanscam

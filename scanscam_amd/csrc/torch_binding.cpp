@@ -1146,6 +1146,7 @@ struct Attention {
     decltype(&scanscam_group_norm_fwd) norm = nullptr;
     decltype(&scanscam_group_norm_bwd) norm_back = nullptr;
     decltype(&scanscam_group_norm_workspace_bytes) norm_workspace = nullptr;
+    decltype(&scanscam_attend_saved_bytes) saved = nullptr;
 } attention;
 
 // Logs of decays, [batch, T, heads] (lead 2), [rows, heads] (lead 1) or [heads], of any of the three types.
@@ -1165,12 +1166,12 @@ bool logs_of(const at::Tensor &t, const at::Tensor &v, int lead, scanscam_tokens
 
 struct AttendBackward : torch::autograd::Function<AttendBackward> {
     struct Done {
-        at::Tensor y, state, offsets;
+        at::Tensor y, state, saved, offsets;
         float scale;
     };
     static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const Maybe &decay, const Maybe &state, Done *done)
     {
-        keep(ctx, {q, k, v, decay.value_or(at::Tensor()), state.value_or(at::Tensor()), done->offsets});
+        keep(ctx, {q, k, v, decay.value_or(at::Tensor()), state.value_or(at::Tensor()), done->offsets, done->saved});
         ctx->set_materialize_grads(false);
         ctx->saved_data["scale"] = (double)done->scale;
         return done->state.defined() ? variable_list{done->y, done->state} : variable_list{done->y};
@@ -1182,7 +1183,7 @@ struct AttendBackward : torch::autograd::Function<AttendBackward> {
         if (!grads[0].defined() && !gstate_out.defined()) return variable_list(6);
         const variable_list saved = returned(ctx, grads[0].defined() ? grads[0] : gstate_out, "linear_attention");
         const at::Tensor q = Gradients::near(saved[0]), k = Gradients::near(saved[1]), v = Gradients::near(saved[2]), state = Gradients::dense(saved[4]),
-                         offsets = Gradients::dense(saved[5]);
+                         offsets = Gradients::dense(saved[5]), parts = Gradients::dense(saved[6]);
         at::Tensor decay = saved[3];
         const c10::DeviceGuard guard(v.device());
         const Gradients make{v};
@@ -1217,6 +1218,7 @@ struct AttendBackward : torch::autograd::Function<AttendBackward> {
         a.gq = Gradients::view(gq);
         a.gk = Gradients::view(gk);
         a.gv = Gradients::view(gv);
+        a.saved = Gradients::at(parts);
         a.gdecay = Gradients::at<float>(gdecay);
         a.gstate_out = Gradients::at<float>(gstate_out);
         a.gstate_in = Gradients::at<float>(gstate);
@@ -1341,6 +1343,11 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         new_state = in.empty({a.sequences, a.heads, a.K, a.V}, at::kFloat);
         a.state_out = static_cast<float *>(new_state.data_ptr());
     }
+    at::Tensor saved;
+    if (in.gradients) {
+        if (const size_t n = attention.saved(&a)) saved = in.empty({(int64_t)n}, at::kByte);
+        a.saved = saved.defined() ? saved.data_ptr() : nullptr;
+    }
     a.workspace_bytes = attention.workspace(&a, SCANSCAM_FORWARD);
     if (a.workspace_bytes != 0) {
         workspace = in.empty({(int64_t)a.workspace_bytes}, at::kByte);
@@ -1348,7 +1355,7 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     }
     SCANSCAM_LAUNCH(attention.forward(&a, in.stream()), "attend_fwd")
     if (in.gradients) {
-        AttendBackward::Done done{y, new_state, offsets, a.scale};
+        AttendBackward::Done done{y, new_state, saved, offsets, a.scale};
         const auto given = [&](int i) { return args[i] == Py_None ? Maybe() : Maybe(THPVariable_Unpack(args[i])); };
         variable_list out = AttendBackward::apply(*given(0), *given(1), v, given(3), maybe(state), &done);
         y = out[0];
@@ -1428,11 +1435,13 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
-// bind_attention(attend_fwd, attend_bwd, attend_workspace_bytes, attend_step_fwd, group_norm_fwd, group_norm_bwd, group_norm_workspace_bytes): addresses.
+// bind_attention(attend_fwd, attend_bwd, attend_workspace_bytes, attend_step_fwd, group_norm_fwd, group_norm_bwd, group_norm_workspace_bytes,
+// attend_saved_bytes): addresses.
 PyObject *bind_attention(PyObject *, PyObject *args)
 {
-    unsigned long long p[7];
-    if (!PyArg_ParseTuple(args, "KKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6)) return nullptr;
+    unsigned long long p[8];
+    if (!PyArg_ParseTuple(args, "KKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7)) return nullptr;
+    attention.saved = reinterpret_cast<decltype(attention.saved)>(p[7]);
     attention.forward = reinterpret_cast<decltype(attention.forward)>(p[0]);
     attention.back = reinterpret_cast<decltype(attention.back)>(p[1]);
     attention.workspace = reinterpret_cast<decltype(attention.workspace)>(p[2]);

@@ -132,7 +132,7 @@ def test_header_is_plain_c_and_every_symbol_is_exported(tmp_path):
     assert sizes == [ctypes.sizeof(s) for s in structs.values()]
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
     names = set(re.findall(r"\b(scanscam_[a-z_]+)\s*\(", text))
-    assert len(names) == 7
+    assert len(names) == 8
     raw = ctypes.CDLL(hip.LIB_PATH)
     for name in names:
         assert hasattr(raw, name), name
@@ -157,7 +157,7 @@ def test_the_library_checks_its_arguments_before_any_launch():
               (E_INVAL, {"heads": 1 << 18, "groups": 1}), (E_INVAL, {"parts": -1}), (E_INVAL, {"T": 1 << 31}))
     for rc, k in shared + ((E_INVAL, {"y": T(None, 1, 1, 1)}), (E_WORKSPACE, {"parts": 3})):
         assert L.scanscam_attend_fwd(attend(**k), None) == rc, k
-    for rc, k in shared + ((E_INVAL, {"gq": T(None, 1, 1, 1)}), (E_INVAL, {"gy": T(fake, 1, 1 << 22, 1)}), (E_WORKSPACE, {}), (E_INVAL, {"gdecay": fake}), (E_ALIGN, {"gstate_in": fake + 1})):
+    for rc, k in shared + ((E_INVAL, {"gq": T(None, 1, 1, 1)}), (E_INVAL, {"gy": T(fake, 1, 1 << 22, 1)}), (E_WORKSPACE, {}), (E_INVAL, {"parts": 3, "workspace": fake, "workspace_bytes": 1 << 40}), (E_INVAL, {"gdecay": fake}), (E_ALIGN, {"gstate_in": fake + 1})):
         assert L.scanscam_attend_bwd(attend(**k), None) == rc, k
     assert L.scanscam_attend_fwd(None, None) == L.scanscam_attend_bwd(None, None) == L.scanscam_attend_step_fwd(None, None) == E_INVAL
     assert L.scanscam_attend_fwd(attend(T=0), None) == L.scanscam_attend_fwd(attend(heads=0), None) == E_OK

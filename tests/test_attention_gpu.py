@@ -4,7 +4,8 @@ against those that torch.autograd takes of these loops.
 
 Bounds. Every output is a sum of products, of which the same call on the inputs' absolute values (and its gradients) gives the sum of absolute values, A.
 With h half a unit in the last place of the activations' type, relative (2^-8 bf16, 2^-11 fp16, 2^-24 fp32):
-  * each product passes one rounding to that type on its way (its score's or the state's): h A; and the result one more: h |want|;
+  * each product passes up to two roundings to that type on its way (its score's; or where no state is handed over that of what is added to the state,
+    and the state's): 2 h A; and the result one more: h |want|;
   * in fp32 a product is rounded once for each addition on its way, at most K + V + C + 2 T of them and some 64 of exponentials and factors:
     (600 + 2 T) 2^-24 A;
   * float32 results (states, gradients of states and of decays) have no rounding to the type, but two terms of it, 2^-17 A (bf16; fp16 2^-21);
@@ -33,7 +34,7 @@ def close(got, want, total, dtype, T, what, exact=False):
     half = HALF[got.dtype]
     got, want, total = got.detach().cpu().double(), want.detach().cpu().double(), total.detach().cpu().double()
     assert torch.isfinite(got).all(), what
-    bound = 1.01 * half * want.abs() + (600 + 2 * T) * 2.0 ** -24 * total + (TERMS[dtype] if exact else 1.01 * HALF[dtype]) * total
+    bound = 1.01 * half * want.abs() + (600 + 2 * T) * 2.0 ** -24 * total + (TERMS[dtype] if exact else 2.02 * HALF[dtype]) * total
     if dtype == torch.float16:
         bound = bound + 2.0 ** -16 * total.max()
     over = (got - want).abs() - bound
@@ -121,8 +122,9 @@ def test_attention_and_gradients(gpu, monkeypatch, dtype, batch, T, heads, K, V,
         plain = f.linear_attention(**dev, scale=scale)
     got = f.linear_attention(**dev, scale=scale, return_state=state)
     got, got_state = got if state else (got, None)
-    assert torch.equal(plain, got.detach())
     Tn = v["v"].shape[1]
+    assert state or torch.equal(plain, got.detach())
+    close(plain, want, size, dtype, Tn, "y of a call without gradients")
     close(got, want, size, dtype, Tn, "y")
     if state:
         close(got_state, want_state, size_state, dtype, Tn, "state", exact=True)

@@ -174,25 +174,35 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
     static constexpr int VE = 16 / sizeof(ST), ROW = D / VE, COUNT = Operand<ST>::CHUNK * ROW / NT, STEP = NT / ROW;
     static_assert(NT % ROW == 0 && Operand<ST>::CHUNK * ROW % NT == 0, "whole rows for all threads");
     raw16 v[COUNT];
-    __device__ __forceinline__ void load(const ST *base, int stride, int n, int d)
+    const ST *from;  // this lane's first vector in a tile that would begin at the tensor's first token
+    int64_t stride;
+    int d, col;
+    __device__ __forceinline__ Staged(const ST *base, int64_t token_stride, int channels) : stride(token_stride), d(channels)
+    {
+        col = threadIdx.x % ROW * VE;
+        from = base + threadIdx.x / ROW * stride + (col < d ? col : 0);
+    }
+    // Of the tokens from t on, of which there are n.
+    __device__ __forceinline__ void load(int64_t t, int n)
     {
         using raw_t = typename RawT<sizeof(ST) * VE>::type;
         typedef raw_t unaligned __attribute__((aligned(sizeof(ST))));
-        const int row0 = threadIdx.x / ROW, col = threadIdx.x % ROW * VE;
-        if constexpr (EXACT) {
-            const ST *at = base + (col < d ? col : 0);
+        const int row0 = threadIdx.x / ROW;
+        if (EXACT && n == Operand<ST>::CHUNK) {
+#pragma unroll
+            for (int i = 0; i < COUNT; i++) v[i] = *reinterpret_cast<const unaligned *>(from + (t + i * STEP) * stride);
+        } else if constexpr (EXACT) {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) {
                 const int row = row0 + i * STEP;
-                v[i] = *reinterpret_cast<const unaligned *>(at + (row < n ? row : n - 1) * stride);
+                v[i] = *reinterpret_cast<const unaligned *>(from + (t + (row < n ? row : n - 1) - row0) * stride);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) {
-                const int row = row0 + i * STEP;
                 v[i] = raw16{0, 0, 0, 0};
-                if (row < n && col < d) {
-                    const ST *at = base + row * stride + col;
+                if (row0 + i * STEP < n && col < d) {
+                    const ST *at = from + (t + i * STEP) * stride;
                     if (col + VE <= d) {
                         v[i] = *reinterpret_cast<const unaligned *>(at);
                     } else {
@@ -205,9 +215,9 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
             }
         }
     }
-    __device__ __forceinline__ void store(Tile<ST, D> tile, int n, int d) const
+    __device__ __forceinline__ void store(Tile<ST, D> tile, int n) const
     {
-        const int row0 = threadIdx.x / ROW, col = threadIdx.x % ROW * VE;
+        const int row0 = threadIdx.x / ROW;
         if (!EXACT || (n == Operand<ST>::CHUNK && d == D)) {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) *reinterpret_cast<raw16 *>(tile.at(row0 + i * STEP, col)) = v[i];
@@ -256,11 +266,23 @@ template <typename ST> __device__ __forceinline__ const ST *tensor_at(const scan
     return static_cast<const ST *>(t.p) + s.batch * t.batch + head * t.group;
 }
 
-// A token's decay in powers of two. An infinitely strong one is 2^-1000000, which is zero in fp32 but has differences.
-__device__ __forceinline__ double decay_at(const scanscam_attend &a, const Span &s, int64_t token, bool there)
+// A token's log of a decay as it is stored: taken apart only where it is used, a chunk after it is asked for.
+__device__ __forceinline__ uint32_t decay_at(const scanscam_attend &a, const Span &s, int64_t token, bool there)
 {
-    if (!there || a.decay.p == nullptr) return 0.0;
-    const float g = param(scanscam_param{a.decay.p, a.decay_dtype, 0}, s.batch * a.decay.batch + token * a.decay.token + s.head);
+    uint32_t raw = 0;
+    if (there && a.decay.p != nullptr) {
+        const int64_t at = s.batch * a.decay.batch + token * a.decay.token + s.head;
+        if (a.decay_dtype == SCANSCAM_F32) raw = static_cast<const uint32_t *>(a.decay.p)[at];
+        else raw = static_cast<const uint16_t *>(a.decay.p)[at];
+    }
+    return raw;
+}
+// ... in powers of two. An infinitely strong one is 2^-1000000, which is zero in fp32 but has differences.
+__device__ __forceinline__ double decay_of(const scanscam_attend &a, uint32_t raw)
+{
+    const float g = a.decay_dtype == SCANSCAM_F32    ? __builtin_bit_cast(float, raw)
+                    : a.decay_dtype == SCANSCAM_BF16 ? __builtin_bit_cast(float, raw << 16)
+                                                     : (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
     const double d = (double)g * 1.4426950408889634074;
     return d < -1e6 ? -1e6 : d > 1e6 ? 1e6 : d;  // (a NaN stays one)
 }
@@ -309,6 +331,22 @@ __device__ __forceinline__ float column_sum4(float v)
 {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
+}
+
+// Waits for everything asked for before a loop. What is still under way where a loop begins (the state's first values) the compiler takes to be so in every
+// turn, and waits there for what the turn itself has asked for meanwhile.
+__device__ __forceinline__ void settle()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt 0
+    asm volatile("" ::: "memory");
+}
+
+// A value that is not known before: what is computed with it is computed there, and not ahead of a loop, to lie in registers all the while.
+__device__ __forceinline__ int later(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // A wave's columns of a state: all rows, in accumulators. Column tile jt of wave w is the state's tile jt * WAVES + w. Products go over the rows that
@@ -361,21 +399,23 @@ template <typename ST, int D, int JT, int WAVES> struct State {
     // As the lanes hold it, tile by tile: to memory, and this lane's part of the product with one from there.
     __device__ __forceinline__ void keep(float *p, int rows, int cols) const
     {
+        float4v *at = reinterpret_cast<float4v *>(p) + later(threadIdx.x & 63);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int jt = 0; jt < JT; jt++)
-                if (rt * 16 < rows && column(jt) < cols) reinterpret_cast<float4v *>(p)[(rt * RT + column(jt) / 16) * 64 + (threadIdx.x & 63)] = s[rt][jt];
+                if (rt * 16 < rows && column(jt) < cols) at[(rt * RT + column(jt) / 16) * 64] = s[rt][jt];
     }
     __device__ __forceinline__ double kept(const float *p, int rows, int cols) const
     {
+        const float4v *at = reinterpret_cast<const float4v *>(p) + later(threadIdx.x & 63);
         double sum = 0.0;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int jt = 0; jt < JT; jt++)
                 if (rt * 16 < rows && column(jt) < cols) {
-                    const float4v other = reinterpret_cast<const float4v *>(p)[(rt * RT + column(jt) / 16) * 64 + (threadIdx.x & 63)];
+                    const float4v other = at[(rt * RT + column(jt) / 16) * 64];
 #pragma unroll
                     for (int r = 0; r < 4; r++) sum += (double)s[rt][jt][r] * (double)other[r];
                 }
@@ -596,28 +636,30 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
     const int64_t out_step = GRAD ? args.part_q != nullptr ? a.heads * K : a.gq.token : a.y.token;
     const int64_t out_first = GRAD ? args.part_q != nullptr ? (span.batch * a.T * a.heads + span.head) * K : span.batch * a.gq.batch + span.head * a.gq.group
                                    : span.batch * a.y.batch + span.head * a.y.group;
+    const int64_t out_lane = out_first + n16 * out_step + 4 * g;
 
     State<ST, D, JT, W> S;
     S.wave = wave;
     S.read(args.parts > 1 ? args.ends + span.unit * K * V : a.state_in == nullptr ? nullptr : a.state_in + pair * K * V, inner, outer, row_step, col_step);
     scores.clear();
 
-    Staged<ST, D, NT, EXACT> sx, sy, sz;
-    double decay = 0.0;
+    Staged<ST, D, NT, EXACT> sx(x, xt.token, inner), sy(y, yt.token, inner), sz(z, zt.token, outer);
+    uint32_t decay = 0;
     const auto ask = [&](int64_t t) {
         const int n = (int)(span.end - t < C ? span.end - t : C);
         if (wave == 0) decay = decay_at(a, span, t + lane, lane < n);
-        sx.load(x + t * xt.token, (int)xt.token, n, inner);
-        sy.load(y + t * yt.token, (int)yt.token, n, inner);
-        sz.load(z + t * zt.token, (int)zt.token, n, outer);
+        sx.load(t, n);
+        sy.load(t, n);
+        sz.load(t, n);
     };
     if (span.begin < span.end) ask(span.begin);
+    settle();
     for (int64_t t0 = span.begin; t0 < span.end; t0 += C) {
         const int n = (int)(span.end - t0 < C ? span.end - t0 : C);
-        sx.store(X, n, inner);
-        sy.store(Y, n, inner);
-        sz.store(Z, n, outer);
-        if (wave == 0) decays.fill(decay);
+        sx.store(X, n);
+        sy.store(Y, n);
+        sz.store(Z, n);
+        if (wave == 0) decays.fill(decay_of(a, decay));
         __syncthreads();
         // This lane's part of the queries, which only the sums over channels need.
         Elems<ST, 4> queries[TT][JT];
@@ -694,6 +736,7 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
                     for (int r = 0; r < 4; r++) finite += sum[jt][r] * 0.0f;
                 if (__builtin_expect(__ballot(finite != 0.0f) != 0, 0)) {
                     // A value that is not finite may be a later token's, times a score of zero: the tokens up to t alone.
+#pragma unroll
                     for (int jt = 0; jt < JT; jt++) {
                         sum[jt] = acc[tt][jt];
                         for (int s = 0; s <= t; s++) {
@@ -704,19 +747,20 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
                             for (int r = 0; r < 4; r++) sum[jt][r] += p * value[r];
                         }
                     }
+                    settle();
                 }
             }
             if (t < n) {
-                const int64_t row = out_first + (t0 + t) * out_step;
+                const int64_t row = out_lane + (t0 + tt * 16) * out_step;
 #pragma unroll
                 for (int jt = 0; jt < JT; jt++) {
-                    const int col = S.column(jt) + 4 * g;
+                    const int col = S.column(jt), there = outer - 4 * g;
                     if constexpr (!GRAD) {
-                        put4<EXACT>(static_cast<ST *>(a.y.p) + row, col, V, sum[jt]);
+                        put4<EXACT>(static_cast<ST *>(a.y.p) + row, col, there, sum[jt]);
                     } else if (args.part_q != nullptr) {
-                        put4<EXACT>(args.part_q + row, col, K, sum[jt]);
+                        put4<EXACT>(args.part_q + row, col, there, sum[jt]);
                     } else {
-                        put4<EXACT>(static_cast<ST *>(a.gq.p) + row, col, K, sum[jt]);
+                        put4<EXACT>(static_cast<ST *>(a.gq.p) + row, col, there, sum[jt]);
                     }
                 }
             }
@@ -776,24 +820,26 @@ template <typename ST, int D, int JT, bool BACK, int TERMS, bool EXACT> __global
     State<ST, D, JT, W> S;
     S.wave = wave;
     S.clear();
-    Staged<ST, D, NT, EXACT> sy, sz;
-    double decay = 0.0, whole = 0.0;
+    Staged<ST, D, NT, EXACT> sy(y, yt.token, inner), sz(z, zt.token, outer);
+    uint32_t decay = 0;
+    double whole = 0.0;
     const auto ask = [&](int64_t t) {
         const int n = (int)(span.end - t < C ? span.end - t : C);
         if (wave == 0) decay = decay_at(a, span, t + lane, lane < n);
-        sy.load(y + t * yt.token, (int)yt.token, n, inner);
-        sz.load(z + t * zt.token, (int)zt.token, n, outer);
+        sy.load(t, n);
+        sz.load(t, n);
     };
     const int64_t chunks = (span.end - span.begin + C - 1) / C;
     const auto token = [&](int64_t c) { return span.begin + (BACK ? chunks - 1 - c : c) * C; };
     if (chunks > 0) ask(token(0));
+    settle();
     for (int64_t c = 0; c < chunks; c++) {
         const int n = (int)(span.end - token(c) < C ? span.end - token(c) : C);
-        sy.store(Y, n, inner);
-        sz.store(Z, n, outer);
+        sy.store(Y, n);
+        sz.store(Z, n);
         if (wave == 0) {
-            decays.fill(decay);
-            whole += read_lane(sums_upto(decay), 63);
+            decays.fill(decay_of(a, decay));
+            whole += decays.sums[C - 1];
         }
         __syncthreads();
         if (c + 1 < chunks) ask(token(c + 1));
@@ -846,6 +892,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
     const int64_t out_step = !KEYS ? a.gv.token : args.part_k != nullptr ? a.heads * K : a.gk.token;
     const int64_t out_first = !KEYS ? span.batch * a.gv.batch + span.head * a.gv.group
                               : args.part_k != nullptr ? (span.batch * a.T * a.heads + span.head) * K : span.batch * a.gk.batch + span.head * a.gk.group;
+    const int64_t out_lane = out_first + n16 * out_step + 4 * g;
 
     State<ST, D, JT, W> H;
     H.wave = wave;
@@ -853,26 +900,27 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
     of_keys.clear();
     if constexpr (BOTH) of_values.clear();
 
-    Staged<ST, D, NT, EXACT> sq, sk, sv, so;
-    double decay = 0.0;
+    Staged<ST, D, NT, EXACT> sq(q, a.q.token, K), sk(k, a.k.token, K), sv(v, a.v.token, V), so(o, a.gy.token, V);
+    uint32_t decay = 0;
     const auto ask = [&](int64_t t) {
         const int n = (int)(span.end - t < C ? span.end - t : C);
         if (all == 0) decay = decay_at(a, span, t + lane, lane < n);
-        sq.load(q + t * a.q.token, (int)a.q.token, n, K);
-        sk.load(k + t * a.k.token, (int)a.k.token, n, K);
-        sv.load(v + t * a.v.token, (int)a.v.token, n, V);
-        so.load(o + t * a.gy.token, (int)a.gy.token, n, V);
+        sq.load(t, n);
+        sk.load(t, n);
+        sv.load(t, n);
+        so.load(t, n);
     };
     const int64_t chunks = (span.end - span.begin + C - 1) / C;
     if (chunks > 0) ask(span.begin + (chunks - 1) * C);
+    settle();
     for (int64_t c = chunks - 1; c >= 0; c--) {
         const int64_t t0 = span.begin + c * C;
         const int n = (int)(span.end - t0 < C ? span.end - t0 : C);
-        sq.store(Q, n, K);
-        sk.store(Kt, n, K);
-        sv.store(Vt, n, V);
-        so.store(O, n, V);
-        if (all == 0) decays.fill(decay);
+        sq.store(Q, n);
+        sk.store(Kt, n);
+        sv.store(Vt, n);
+        so.store(O, n);
+        if (all == 0) decays.fill(decay_of(a, decay));
         __syncthreads();
         if (c > 0) ask(t0 - C);
 
@@ -937,16 +985,16 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                 for (int jt = 0; jt < JT; jt++) acc[st][jt] = mma(own[jt][step], p, acc[st][jt]);
             }
             if (s < n) {
-                const int64_t row = out_first + (t0 + s) * out_step;
+                const int64_t row = out_lane + (t0 + st * 16) * out_step;
 #pragma unroll
                 for (int jt = 0; jt < JT; jt++) {
-                    const int col = H.column(jt) + 4 * g;
+                    const int col = H.column(jt), there = outer - 4 * g;
                     if constexpr (!KEYS) {
-                        put4<EXACT>(static_cast<ST *>(a.gv.p) + row, col, V, acc[st][jt]);
+                        put4<EXACT>(static_cast<ST *>(a.gv.p) + row, col, there, acc[st][jt]);
                     } else if (args.part_k != nullptr) {
-                        put4<EXACT>(args.part_k + row, col, K, acc[st][jt]);
+                        put4<EXACT>(args.part_k + row, col, there, acc[st][jt]);
                     } else {
-                        put4<EXACT>(static_cast<ST *>(a.gk.p) + row, col, K, acc[st][jt]);
+                        put4<EXACT>(static_cast<ST *>(a.gk.p) + row, col, there, acc[st][jt]);
                     }
                 }
             }

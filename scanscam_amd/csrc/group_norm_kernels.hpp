@@ -55,10 +55,13 @@ template <int L, bool WAVES> __device__ __forceinline__ float over_team(float v,
 
 __device__ __forceinline__ float silu_slope(float z, float s) { return s * __builtin_fmaf(z, 1.0f - s, 1.0f); }
 
-template <typename ST, int L, int NV, bool WAVES> struct Team {
+// EXACT: a group is a whole number of vectors. Else its last vector ends where the group does and covers some of the channels of the one before a second
+// time, which its sums leave out and both write alike: loads and stores of single channels took half of the time (groups of 205: 63 us of
+// [16384, 2050]). A group smaller than a vector is one lane's, channel by channel.
+template <typename ST, int L, int NV, bool WAVES, bool EXACT> struct Team {
     static constexpr int VEC = group_vec<ST>();
     int64_t group, part;
-    int at[NV], count[NV];  // channels of the group
+    int at[NV], count[NV], skip[NV];  // channels of the group: the first, how many of a vector's are there, and how many of them are another's
     bool there;
     __device__ __forceinline__ explicit Team(const GroupNormArgs &args)
     {
@@ -69,10 +72,13 @@ template <typename ST, int L, int NV, bool WAVES> struct Team {
         part = team / args.a.groups;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            at[j] = (j * lanes + lane) * VEC;
-            count[j] = args.size - at[j];
+            const int first = (j * lanes + lane) * VEC, left = args.size - first;
+            at[j] = EXACT || left >= VEC || left <= 0 || args.size < VEC ? first : args.size - VEC;
+            skip[j] = first - at[j];
+            count[j] = left + skip[j];
         }
     }
+    __device__ __forceinline__ bool own(int j, int k) const { return EXACT ? count[j] > 0 : k >= skip[j] && k < count[j]; }
     __device__ __forceinline__ void load(const ST *p, Elems<ST, VEC> (&e)[NV]) const
     {
         using raw_t = typename RawT<sizeof(ST) * VEC>::type;
@@ -80,15 +86,20 @@ template <typename ST, int L, int NV, bool WAVES> struct Team {
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             e[j] = __builtin_bit_cast(Elems<ST, VEC>, raw_t{0, 0, 0, 0});
-            if (count[j] >= VEC) {
+            if (EXACT ? count[j] > 0 : count[j] >= VEC) {
                 const raw_t raw = *reinterpret_cast<const unaligned *>(p + at[j]);
                 e[j] = __builtin_bit_cast(Elems<ST, VEC>, raw);
-            } else {
+            } else if constexpr (!EXACT && L == 1) {
 #pragma unroll
                 for (int k = 0; k < VEC; k++)
                     if (k < count[j]) e[j].e[k] = p[at[j] + k];
             }
         }
+    }
+    template <typename T> __device__ __forceinline__ void store(T *p, int j, const float (&f)[VEC]) const
+    {
+        if (EXACT ? count[j] > 0 : count[j] >= VEC) store_some<T, VEC>(p + at[j], VEC, f);
+        else if constexpr (!EXACT && L == 1) store_some<T, VEC>(p + at[j], count[j], f);
     }
     __device__ __forceinline__ void parameter(const scanscam_param &p, int64_t first, float (&f)[NV][VEC], float fill) const
     {
@@ -103,15 +114,19 @@ template <typename ST, int L, int NV, bool WAVES> struct Team {
 #pragma unroll
         for (int j = 0; j < NV; j++)
 #pragma unroll
-            for (int k = 0; k < VEC; k++) sum += h[j][k] = (float)e[j].e[k];  // (zeros where there is no channel)
+            for (int k = 0; k < VEC; k++) {
+                h[j][k] = (float)e[j].e[k];
+                sum += EXACT || own(j, k) ? h[j][k] : 0.0f;  // (zeros where there is no channel)
+            }
         const float mean = over_team<L, WAVES>(sum, args.waves, slots, turn) * share;
         sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; j++)
 #pragma unroll
             for (int k = 0; k < VEC; k++) {
-                h[j][k] = k < count[j] ? h[j][k] - mean : 0.0f;
-                sum = __builtin_fmaf(h[j][k], h[j][k], sum);
+                h[j][k] -= mean;
+                const float mine = own(j, k) ? h[j][k] : 0.0f;
+                sum = __builtin_fmaf(mine, mine, sum);
             }
         const float rstd = __builtin_amdgcn_rsqf(over_team<L, WAVES>(sum, args.waves, slots, turn) * share + args.a.eps);
 #pragma unroll
@@ -122,9 +137,9 @@ template <typename ST, int L, int NV, bool WAVES> struct Team {
     }
 };
 
-template <typename ST, int L, int NV, bool WAVES> __global__ __launch_bounds__(WAVES ? 512 : 256) void group_norm_kernel(GroupNormArgs args)
+template <typename ST, int L, int NV, bool WAVES, bool EXACT> __global__ __launch_bounds__(WAVES ? 512 : 256) void group_norm_kernel(GroupNormArgs args)
 {
-    using T = Team<ST, L, NV, WAVES>;
+    using T = Team<ST, L, NV, WAVES, EXACT>;
     constexpr int VEC = T::VEC;
     __shared__ float slots[2][8];
     const scanscam_group_norm &a = args.a;
@@ -165,14 +180,14 @@ template <typename ST, int L, int NV, bool WAVES> __global__ __launch_bounds__(W
                 if (a.z != nullptr) u *= gate[j][k] * sigmoid_(gate[j][k]);
                 h[j][k] = u;
             }
-            store_some(y + r * a.channels + team.at[j], team.count[j], h[j]);
+            team.store(y + r * a.channels, j, h[j]);
         }
     }
 }
 
-template <typename ST, int L, int NV, bool WAVES> __global__ __launch_bounds__(WAVES ? 512 : 256) void group_norm_back_kernel(GroupNormArgs args)
+template <typename ST, int L, int NV, bool WAVES, bool EXACT> __global__ __launch_bounds__(WAVES ? 512 : 256) void group_norm_back_kernel(GroupNormArgs args)
 {
-    using T = Team<ST, L, NV, WAVES>;
+    using T = Team<ST, L, NV, WAVES, EXACT>;
     constexpr int VEC = T::VEC;
     __shared__ float slots[2][8];
     const scanscam_group_norm &a = args.a;
@@ -226,12 +241,12 @@ template <typename ST, int L, int NV, bool WAVES> __global__ __launch_bounds__(W
                 if (a.activation == SCANSCAM_ACT_SILU) e *= silu_slope(u, su);
                 gw[j][k] = __builtin_fmaf(e, h[j][k], gw[j][k]);
                 gb[j][k] += e;
-                e = k < team.count[j] ? e * w[j][k] : 0.0f;
-                g[j][k] = e;
-                sum += e;
-                along = __builtin_fmaf(e, h[j][k], along);
+                g[j][k] = e *= w[j][k];
+                const float mine = team.own(j, k) ? e : 0.0f;
+                sum += mine;
+                along = __builtin_fmaf(mine, h[j][k], along);
             }
-            if (a.gz != nullptr) store_some(gz + r * a.channels + team.at[j], team.count[j], s[j]);
+            if (a.gz != nullptr) team.store(gz + r * a.channels, j, s[j]);
         }
         sum = over_team<L, WAVES>(sum, args.waves, slots, turn) * share;
         along = over_team<L, WAVES>(along, args.waves, slots, turn) * share;
@@ -239,7 +254,7 @@ template <typename ST, int L, int NV, bool WAVES> __global__ __launch_bounds__(W
         for (int j = 0; j < NV; j++) {
 #pragma unroll
             for (int k = 0; k < VEC; k++) g[j][k] = rstd * (g[j][k] - sum - h[j][k] * along);
-            store_some(gx + r * a.channels + team.at[j], team.count[j], g[j]);
+            team.store(gx + r * a.channels, j, g[j]);
         }
     }
     const int64_t columns = a.gweight != nullptr ? a.channels : 0, pitch = columns + (a.gbias != nullptr ? a.channels : 0);
@@ -247,8 +262,8 @@ template <typename ST, int L, int NV, bool WAVES> __global__ __launch_bounds__(W
     float *part = args.part + team.part * pitch + first;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        if (a.gweight != nullptr) store_some(part + team.at[j], team.count[j], gw[j]);
-        if (a.gbias != nullptr) store_some(part + columns + team.at[j], team.count[j], gb[j]);
+        if (a.gweight != nullptr) team.store(part, j, gw[j]);
+        if (a.gbias != nullptr) team.store(part + columns, j, gb[j]);
     }
 }
 
@@ -259,24 +274,29 @@ struct GroupNormPlan {
 // One per storage type, in a file of its own.
 template <typename ST> hipError_t launch_group_norm(bool back, const GroupNormPlan &plan, hipStream_t stream, const GroupNormArgs &args);
 
-template <typename ST, int L, int NV, bool WAVES> hipError_t launch_team(bool back, hipStream_t stream, const GroupNormArgs &args)
+template <typename ST, int L, int NV, bool WAVES, bool EXACT> hipError_t launch_team(bool back, hipStream_t stream, const GroupNormArgs &args)
 {
     const int64_t teams = args.a.groups * args.parts, grid = WAVES ? teams : ceil_div(teams, 256 / L);
-    return launch_op(back ? group_norm_back_kernel<ST, L, NV, WAVES> : group_norm_kernel<ST, L, NV, WAVES>, dim3((unsigned)grid), dim3(WAVES ? 64 * args.waves : 256), 0, stream, args);
+    return launch_op(back ? group_norm_back_kernel<ST, L, NV, WAVES, EXACT> : group_norm_kernel<ST, L, NV, WAVES, EXACT>, dim3((unsigned)grid), dim3(WAVES ? 64 * args.waves : 256), 0,
+                     stream, args);
+}
+template <typename ST, bool EXACT> hipError_t launch_group_norm_of(bool back, const GroupNormPlan &plan, hipStream_t stream, const GroupNormArgs &args)
+{
+    if (plan.waves > 1) return launch_team<ST, 64, group_most<ST>(), true, EXACT>(back, stream, args);
+    if (plan.nv > 1) return launch_team<ST, 64, 2, false, EXACT>(back, stream, args);
+    switch (plan.lanes) {
+    case 1: return launch_team<ST, 1, 1, false, EXACT>(back, stream, args);
+    case 2: return launch_team<ST, 2, 1, false, EXACT>(back, stream, args);
+    case 4: return launch_team<ST, 4, 1, false, EXACT>(back, stream, args);
+    case 8: return launch_team<ST, 8, 1, false, EXACT>(back, stream, args);
+    case 16: return launch_team<ST, 16, 1, false, EXACT>(back, stream, args);
+    case 32: return launch_team<ST, 32, 1, false, EXACT>(back, stream, args);
+    default: return launch_team<ST, 64, 1, false, EXACT>(back, stream, args);
+    }
 }
 template <typename ST> hipError_t launch_group_norm_with(bool back, const GroupNormPlan &plan, hipStream_t stream, const GroupNormArgs &args)
 {
-    if (plan.waves > 1) return launch_team<ST, 64, group_most<ST>(), true>(back, stream, args);
-    if (plan.nv > 1) return launch_team<ST, 64, 2, false>(back, stream, args);
-    switch (plan.lanes) {
-    case 1: return launch_team<ST, 1, 1, false>(back, stream, args);
-    case 2: return launch_team<ST, 2, 1, false>(back, stream, args);
-    case 4: return launch_team<ST, 4, 1, false>(back, stream, args);
-    case 8: return launch_team<ST, 8, 1, false>(back, stream, args);
-    case 16: return launch_team<ST, 16, 1, false>(back, stream, args);
-    case 32: return launch_team<ST, 32, 1, false>(back, stream, args);
-    default: return launch_team<ST, 64, 1, false>(back, stream, args);
-    }
+    return args.size % group_vec<ST>() == 0 ? launch_group_norm_of<ST, true>(back, plan, stream, args) : launch_group_norm_of<ST, false>(back, plan, stream, args);
 }
 #define SCANSCAM_DEFINE_GROUP_NORM_LAUNCH(ST)                                                                                                      \
     template <> hipError_t launch_group_norm<ST>(bool back, const GroupNormPlan &plan, hipStream_t stream, const GroupNormArgs &args)              \

@@ -336,7 +336,7 @@ int scanscam_attend_fwd(const scanscam_attend *a, void *stream)
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t err = hipSuccess;
     if (parts > 1) err = starts(args, false, kEnds, s);
-    if (err == hipSuccess) err = run(a->state_out != nullptr ? kOutputs : kOutputsOnce, a->sequences * a->heads * parts, s, args);
+    if (err == hipSuccess) err = run(a->state_out != nullptr ? kOutputs : kOutputsRounded, a->sequences * a->heads * parts, s, args);
     return code(err);
 }
 

@@ -74,10 +74,12 @@ __device__ __forceinline__ float4v mma(const float4v &a, const float4v &b, float
 }
 
 // Terms of the activations' type that a float32 factor is taken apart into where float32 results come from it (states that are handed over, gradients
-// of states and of decays): all 24 bits, 22 in fp16. What only 16-bit results come from has one: a rounding that is half of the result's own.
+// of states and of decays): all 24 bits, 22 in fp16. Where only 16-bit results come from it the state is read in one term, whose rounding is like the
+// result's own, and what is added to it has two (with one, results were 1.6 times as far from 64 bits as rounded ones are, with two 1.35 times).
 template <typename ST> constexpr int kTerms = 3;
 template <> inline constexpr int kTerms<_Float16> = 2;
 template <> inline constexpr int kTerms<float> = 1;
+template <typename ST> constexpr int kTermsRounded = sizeof(ST) == 2 ? 2 : 1;
 
 // fp16 has five bits of exponent: what is taken apart is first brought to a largest value of 2^14 in the wave, by a power of two, so that the second
 // term's smallest step is 2^-38 of it and nothing overflows.
@@ -110,6 +112,9 @@ template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(c
             float rest = x[e];
 #pragma unroll
             for (int t = 0; t < TERMS; t++) {
+                // (A product that is rounded to fp16 where it is made is rounded once; what is left must be what that rounding left, and not one's after the
+                // product was rounded to fp32: where the two differ, the next term would miss by a whole step.)
+                if constexpr (std::is_same_v<ST, _Float16>) asm("" : "+v"(rest));
                 const ST h = (ST)rest;
                 out[t][e] = h;
                 if (t + 1 < TERMS) rest -= (float)h;  // (an infinity becomes a NaN)
@@ -868,7 +873,7 @@ template <typename ST, int D> struct BackLds {
 template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forceinline__ void back_pass(const AttendArgs &args, float *lds)
 {
     constexpr bool BOTH = attend_both<D>();
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * back_waves<D>(), STEPS = C / KS, TT = C / 16, PER = KS / 16, TERMS = KEYS ? kTerms<ST> : 1;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * back_waves<D>(), STEPS = C / KS, TT = C / 16, PER = KS / 16, TERMS = KEYS ? kTerms<ST> : 1, TERMS_IN = KEYS ? kTerms<ST> : kTermsRounded<ST>;
     const scanscam_attend &a = args.a;
     const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % W, n16 = lane & 15, g = lane >> 4;
     float *at = lds;
@@ -1003,7 +1008,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                 if (g == 0) red[wave * C + s] = write;
             }
         }
-        H.template update<TERMS>(update_rows, inner, own, decays.upto, a.scale, decays.whole());
+        H.template update<TERMS_IN>(update_rows, inner, own, decays.upto, a.scale, decays.whole());
         if constexpr (KEYS) {
             const bool border = args.cross != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0;
             const int64_t at_border = border ? border_at(args, span.batch, t0, C, span.head) : 0;
@@ -1045,8 +1050,8 @@ template <typename ST, int D, int JK, int JV, bool EXACT> __global__ __launch_bo
 }
 
 // --- launches by type ---------------------------------------------------------------------------------------------------------------------
-// kOutputsOnce: no state is handed over, so that what is added to it is rounded to one term.
-enum AttendPass { kOutputs, kOutputsOnce, kQueries, kKeysAndValues, kEnds, kBackEnds };
+// kOutputsRounded: no state is handed over.
+enum AttendPass { kOutputs, kOutputsRounded, kQueries, kKeysAndValues, kEnds, kBackEnds };
 
 // Channels that a call's tiles have room for.
 inline int attend_width(const scanscam_attend &a)
@@ -1073,7 +1078,7 @@ template <auto Kernel, int WORDS> hipError_t launch_attend_units(int64_t units, 
 // Column tiles of a wave by the columns that there are: a head of up to 64 (of the 256 kind 128) leaves half of the waves' registers and products out.
 template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
 {
-    constexpr int threads = 64 * attend_waves<D>(), grad_threads = 64 * attend_waves<D, true>(), back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, T = kTerms<ST>;
+    constexpr int threads = 64 * attend_waves<D>(), grad_threads = 64 * attend_waves<D, true>(), back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, T = kTerms<ST>, R = kTermsRounded<ST>;
     constexpr int out = AttendLds<ST, D, false>::WORDS, grad = AttendLds<ST, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
     const bool k_half = ALL == 2 && args.a.K <= D / 2, v_half = ALL == 2 && args.a.V <= D / 2;
     const unsigned kinds = attend_both<D>() ? 1 : 2;
@@ -1081,9 +1086,9 @@ template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPa
     case kOutputs:
         return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, T, EXACT>, out>(units, 1, threads, stream, args)
                       : launch_attend_units<attend_kernel<ST, D, ALL, false, T, EXACT>, out>(units, 1, threads, stream, args);
-    case kOutputsOnce:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, 1, EXACT>, out>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, ALL, false, 1, EXACT>, out>(units, 1, threads, stream, args);
+    case kOutputsRounded:
+        return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, R, EXACT>, out>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, false, R, EXACT>, out>(units, 1, threads, stream, args);
     case kQueries:
         return k_half ? launch_attend_units<attend_kernel<ST, D, 1, true, T, EXACT>, grad>(units, 1, grad_threads, stream, args)
                       : launch_attend_units<attend_kernel<ST, D, D / 16 / attend_waves<D, true>(), true, T, EXACT>, grad>(units, 1, grad_threads, stream, args);

@@ -221,3 +221,19 @@ def test_group_norm_and_gradients(gpu, monkeypatch, dtype, rows, channels, group
             norm_close(a, w, f"gradient of {n}", terms=rows ** 0.5 if n in ("weight", "bias") else 1.0)
         else:
             assert a.float().abs().max() <= 2.0 ** -16 * 316.3 * float(gy.float().abs().max()) * 16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_float32_results_of_16_bits_are_float32_s(gpu, dtype):
+    """States and gradients of decays, over all values together: 2^-24 for each of a few additions on the way (512 tokens are 8 chunks), and no term of a product lost."""
+    v = make(12, dtype, 2, 512, 4, 128, 64, groups=2, state=True)
+    names = [n for n, t in v.items() if t is not None]
+    ref, dev = {n: wide(v[n]).requires_grad_() for n in names}, {n: v[n].to(gpu).requires_grad_() for n in names}
+    outs, grads = [], []
+    for call, leaves in ((baseline.naive_linear_attention, ref), (f.linear_attention, dev)):
+        y, state = call(**leaves, scale=0.1, return_state=True)
+        outs.append(state)
+        weights = [torch.linspace(-1, 1, t.numel(), dtype=torch.float64).view(t.shape) for t in (y, state)]
+        grads.append(torch.autograd.grad((y, state), [leaves["decay"], leaves["state"]], [w.to(dtype).to(t) if t is y else w.float().to(t) for w, t in zip(weights, (y, state))]))
+    for want, got in [outs] + list(zip(*grads)):
+        assert (got.detach().cpu().double() - want.detach()).norm() <= 1e-6 * want.detach().norm()

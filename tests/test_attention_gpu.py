@@ -225,7 +225,11 @@ def test_group_norm_and_gradients(gpu, monkeypatch, dtype, rows, channels, group
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_float32_results_of_16_bits_are_float32_s(gpu, dtype):
-    """States and gradients of decays, over all values together: 2^-24 for each of a few additions on the way (512 tokens are 8 chunks), and no term of a product lost."""
+    """
+    States and gradients of decays, over all values together: no term of a product is lost. What a token reads or writes is a sum whose products pass some 40
+    roundings of 2^-24, independent ones: 40^0.5 2^-24 = 3.8e-7 of it. A decay's gradient is a running sum of such terms over 8 chunks, of two kinds each, which
+    cancel to about the size of one: 16^0.5 as much, 1.5e-6, below 2^-19. (A product's second term that is missing costs 2^-11 of one product in some 10^4.)
+    """
     v = make(12, dtype, 2, 512, 4, 128, 64, groups=2, state=True)
     names = [n for n, t in v.items() if t is not None]
     ref, dev = {n: wide(v[n]).requires_grad_() for n in names}, {n: v[n].to(gpu).requires_grad_() for n in names}
@@ -236,4 +240,4 @@ def test_float32_results_of_16_bits_are_float32_s(gpu, dtype):
         weights = [torch.linspace(-1, 1, t.numel(), dtype=torch.float64).view(t.shape) for t in (y, state)]
         grads.append(torch.autograd.grad((y, state), [leaves["decay"], leaves["state"]], [w.to(dtype).to(t) if t is y else w.float().to(t) for w, t in zip(weights, (y, state))]))
     for want, got in [outs] + list(zip(*grads)):
-        assert (got.detach().cpu().double() - want.detach()).norm() <= 1e-6 * want.detach().norm()
+        assert (got.detach().cpu().double() - want.detach()).norm() <= 2.0 ** -19 * want.detach().norm()

@@ -94,10 +94,12 @@ __device__ __forceinline__ float most_of(float v)
     v = top(v, dpp_move<0x143, 0xc>(0.0f, v));
     return read_lane(v, 63);
 }
-// (zero, infinities and NaN are left at 1; the power's inverse is finite too)
-__device__ __forceinline__ float scale_to_fp16(float most)
+// `largest(finite)`: the wave's largest absolute value, or largest finite one: one that is not finite is no measure for the others. (The power's inverse is finite too.)
+template <typename F> __device__ __forceinline__ float scale_to_fp16(F largest)
 {
-    if (!(most > 1e-30f && most < __builtin_inff())) return 1.0f;
+    float most = largest(false);
+    if (__builtin_expect(!(most < __builtin_inff()), 0)) most = largest(true);
+    if (!(most > 1e-30f)) return 1.0f;
     return __builtin_ldexpf(1.0f, 14 - (int)(__builtin_bit_cast(uint32_t, most) >> 23) + 127);
 }
 
@@ -430,14 +432,19 @@ template <typename ST, int D, int JT, int WAVES> struct State {
     __device__ __forceinline__ float scale() const
     {
         if constexpr (!std::is_same_v<ST, _Float16>) return 1.0f;
-        float most = 0.0f;
+        return scale_to_fp16([&](bool finite) {
+            float most = 0.0f;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+            for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (int jt = 0; jt < JT; jt++)
+                for (int jt = 0; jt < JT; jt++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) most = __builtin_fmaxf(most, __builtin_fabsf(s[rt][jt][r]));
-        return scale_to_fp16(most_of(most));
+                    for (int r = 0; r < 4; r++) {
+                        const float v = __builtin_fabsf(s[rt][jt][r]);
+                        most = __builtin_fmaxf(most, finite && !(v < __builtin_inff()) ? 0.0f : v);
+                    }
+            return most_of(most);
+        });
     }
     // acc[tt][jt], columns: rows of `of` (tokens), rows: the state's columns: the state's product with them, times the power of two that is returned.
     template <int TERMS> __device__ __forceinline__ float times(Tile<ST, D> of, int rows, float4v (&acc)[C / 16][JT]) const
@@ -481,18 +488,23 @@ template <typename ST, int D, int JT, int WAVES> struct State {
         const int g = (threadIdx.x & 63) >> 4;
         float bring = 1.0f;
         if constexpr (std::is_same_v<ST, _Float16>) {
-            float most = 0.0f;
+            bring = scale_to_fp16([&](bool finite) {
+                float most = 0.0f;
 #pragma unroll
-            for (int step = 0; step < STEPS; step++)
+                for (int step = 0; step < STEPS; step++)
 #pragma unroll
-                for (int h = 0; h < PER; h++) {
-                    const float4v w = *reinterpret_cast<const float4v *>(weight + step * KS + 16 * h + 4 * g);
+                    for (int h = 0; h < PER; h++) {
+                        const float4v w = *reinterpret_cast<const float4v *>(weight + step * KS + 16 * h + 4 * g);
 #pragma unroll
-                    for (int jt = 0; jt < JT; jt++)
+                        for (int jt = 0; jt < JT; jt++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) most = __builtin_fmaxf(most, __builtin_fabsf((float)own[jt][step][4 * h + r] * (w[r] * factor)));
-                }
-            bring = scale_to_fp16(most_of(most));
+                            for (int r = 0; r < 4; r++) {
+                                const float v = __builtin_fabsf((float)own[jt][step][4 * h + r] * (w[r] * factor));
+                                most = __builtin_fmaxf(most, finite && !(v < __builtin_inff()) ? 0.0f : v);
+                            }
+                    }
+                return most_of(most);
+            });
             bring = bring < 1048576.0f ? bring : 1048576.0f;  // (the state is multiplied with it as well)
             factor *= bring;
         }
@@ -740,17 +752,27 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
 #pragma unroll
                     for (int r = 0; r < 4; r++) finite += sum[jt][r] * 0.0f;
                 if (__builtin_expect(__ballot(finite != 0.0f) != 0, 0)) {
-                    // A value that is not finite may be a later token's, times a score of zero: the tokens up to t alone.
+                    // A value that is not finite may be a later token's, times a score of zero. Where the tokens up to t alone give a finite sum it is the product's
+                    // without such values, in the same order as ever.
 #pragma unroll
                     for (int jt = 0; jt < JT; jt++) {
-                        sum[jt] = acc[tt][jt];
+                        float4v alone = acc[tt][jt], clean = acc[tt][jt];
                         for (int s = 0; s <= t; s++) {
                             float value[4];
                             Z.four(s, S.column(jt) + 4 * g, value);
                             const float p = scores.at(s, t);
 #pragma unroll
-                            for (int r = 0; r < 4; r++) sum[jt][r] += p * value[r];
+                            for (int r = 0; r < 4; r++) alone[r] += p * value[r];
                         }
+#pragma unroll
+                        for (int step = 0; step <= tt / PER; step++) {
+                            frag_t<ST> values = own[jt][step];
+#pragma unroll
+                            for (int e = 0; e < 4 * PER; e++) values[e] = __builtin_isfinite((float)values[e]) ? values[e] : (ST)0.0f;
+                            clean = mma(values, scores.operand(tt, step), clean);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; r++) sum[jt][r] = __builtin_isfinite(alone[r]) ? clean[r] : alone[r];
                     }
                     settle();
                 }

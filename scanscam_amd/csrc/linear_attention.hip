@@ -87,7 +87,8 @@ template <typename ST> __global__ __launch_bounds__(256) void shared_kernel(Shar
 }
 
 // One token: S = e^g S + k v^T, y = scale S^T q. Memory bounds it, the states read and written. A workgroup takes `width` columns of a head's
-// state; `lanes` lanes hold four columns each, and rows go round the workgroup, eight under way at once.
+// state; `lanes` lanes hold four columns each, and rows go round the workgroup, four
+// under way at once (256 x 16 states of 128 x 128 from HBM, 537 MB: 114 us, 4.7 TB/s; eight 123, sixteen 131, for more registers leave fewer waves).
 struct StepArgs {
     scanscam_attend_step a;
     int32_t lanes, pieces, each;
@@ -110,7 +111,7 @@ template <typename ST> __global__ __launch_bounds__(256) void attend_step_kernel
         return;
     }
     float *state = a.state + (slot * a.heads + head) * (int64_t)K * V + col;
-    constexpr int UNROLL = 8;
+    constexpr int UNROLL = 4;
     float4v s[UNROLL];
     const auto ask = [&](int i0) {
 #pragma unroll

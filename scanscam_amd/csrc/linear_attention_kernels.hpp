@@ -613,22 +613,16 @@ template <bool EXACT, typename ST> __device__ __forceinline__ void put4(ST *row,
 
 // Waves of a workgroup, or in the pass over keys and values of each of its kinds: four with up to two tiles of 16 columns each. (Eight waves of one tile
 // read the shared operands twice as often: [8, 4096, 16 x 128] in bf16 201 us forwards, 164 so.)
-#ifndef GWPS
-#define GWPS 2
-#endif
-#ifndef GW
-#define GW 4
-#endif
-template <int D, bool GRAD = false> constexpr int attend_waves() { return D == 256 ? 8 : GRAD && D == 128 ? GW : 4; }
+template <int D> constexpr int attend_waves() { return D == 256 ? 8 : 4; }
 
 // --- outputs (x, y, z = q, k, v) and, with GRAD, gradients of queries (x, y, z = do, v, k) with what decays read -----------------------
 template <typename ST, int D, bool GRAD> struct AttendLds {
-    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<D, GRAD>();
+    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<D>();
     static constexpr int WORDS = 3 * Tile<ST, D>::WORDS + Scores<ST>::WORDS + Decays<C>::WORDS + (GRAD ? W * C + 2 * W : 0);
 };
-template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global__ __launch_bounds__((64 * attend_waves<D, GRAD>()), (GRAD && D == 128 && GW == 8 ? GWPS : 2)) void attend_kernel(AttendArgs args)
+template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * attend_waves<D>(), 2) void attend_kernel(AttendArgs args)
 {
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D, GRAD>(), NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const scanscam_attend &a = args.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
@@ -828,9 +822,11 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
 template <typename ST, int D> struct EndsLds {
     static constexpr int WORDS = 2 * Tile<ST, D>::WORDS + Decays<Operand<ST>::CHUNK>::WORDS;
 };
-template <typename ST, int D, int JT, bool BACK, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * attend_waves<D>(), 2) void ends_kernel(AttendArgs args)
+// W waves of JT tiles each. (128 columns are eight waves of one tile, which leave each other twice as much to wait for: 61 us for the first three of four parts of
+// [8, 4096, 16 x 128] in bf16, 67 by four waves of two.)
+template <typename ST, int D, int JT, int W, bool BACK, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * W, D == 128 && W == 8 ? 4 : 2) void ends_kernel(AttendArgs args)
 {
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * W, STEPS = C / KS;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * W, STEPS = C / KS;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const scanscam_attend &a = args.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1097,33 +1093,35 @@ template <auto Kernel, int WORDS> hipError_t launch_attend_units(int64_t units, 
     return hipSuccess;
 }
 
-// Column tiles of a wave by the columns that there are: a head of up to 64 (of the 256 kind 128) leaves half of the waves' registers and products out.
+// Column tiles of a wave by the columns that there are: a head of up to 64 (of the 256 kind 128) leaves half of the waves' registers and products out
+// (whole vectors only: the other kernels are rare, and theirs are as many again).
 template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
 {
-    constexpr int threads = 64 * attend_waves<D>(), grad_threads = 64 * attend_waves<D, true>(), back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, T = kTerms<ST>, R = kTermsRounded<ST>;
+    constexpr int WAVES = attend_waves<D>(), EJ = D == 256 ? 2 : 1, EW = D / 16 / EJ;  // (EJ, EW: of the ends, whole)
+    constexpr int threads = 64 * WAVES, back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, HALF = EXACT ? 1 : ALL, T = kTerms<ST>, R = kTermsRounded<ST>;
     constexpr int out = AttendLds<ST, D, false>::WORDS, grad = AttendLds<ST, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
     const bool k_half = ALL == 2 && args.a.K <= D / 2, v_half = ALL == 2 && args.a.V <= D / 2;
     const unsigned kinds = attend_both<D>() ? 1 : 2;
     switch (pass) {
     case kOutputs:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, T, EXACT>, out>(units, 1, threads, stream, args)
+        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, false, T, EXACT>, out>(units, 1, threads, stream, args)
                       : launch_attend_units<attend_kernel<ST, D, ALL, false, T, EXACT>, out>(units, 1, threads, stream, args);
     case kOutputsRounded:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, 1, false, R, EXACT>, out>(units, 1, threads, stream, args)
+        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, false, R, EXACT>, out>(units, 1, threads, stream, args)
                       : launch_attend_units<attend_kernel<ST, D, ALL, false, R, EXACT>, out>(units, 1, threads, stream, args);
     case kQueries:
-        return k_half ? launch_attend_units<attend_kernel<ST, D, 1, true, T, EXACT>, grad>(units, 1, grad_threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, D / 16 / attend_waves<D, true>(), true, T, EXACT>, grad>(units, 1, grad_threads, stream, args);
+        return k_half ? launch_attend_units<attend_kernel<ST, D, HALF, true, T, EXACT>, grad>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, true, T, EXACT>, grad>(units, 1, threads, stream, args);
     case kKeysAndValues:  // (both are not halves at once)
-        if (k_half) return launch_attend_units<attend_back_kernel<ST, D, 1, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
-        if (v_half) return launch_attend_units<attend_back_kernel<ST, D, ALL, 1, EXACT>, back>(units, kinds, back_threads, stream, args);
+        if (k_half) return launch_attend_units<attend_back_kernel<ST, D, HALF, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
+        if (v_half) return launch_attend_units<attend_back_kernel<ST, D, ALL, HALF, EXACT>, back>(units, kinds, back_threads, stream, args);
         return launch_attend_units<attend_back_kernel<ST, D, ALL, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
     case kEnds:
-        return v_half ? launch_attend_units<ends_kernel<ST, D, 1, false, T, EXACT>, ends>(units, 1, threads, stream, args)
-                      : launch_attend_units<ends_kernel<ST, D, ALL, false, T, EXACT>, ends>(units, 1, threads, stream, args);
+        return v_half ? launch_attend_units<ends_kernel<ST, D, HALF, WAVES, false, T, EXACT>, ends>(units, 1, threads, stream, args)
+                      : launch_attend_units<ends_kernel<ST, D, EJ, EW, false, T, EXACT>, ends>(units, 1, 64 * EW, stream, args);
     default:
-        return k_half ? launch_attend_units<ends_kernel<ST, D, 1, true, T, EXACT>, ends>(units, 1, threads, stream, args)
-                      : launch_attend_units<ends_kernel<ST, D, ALL, true, T, EXACT>, ends>(units, 1, threads, stream, args);
+        return k_half ? launch_attend_units<ends_kernel<ST, D, HALF, WAVES, true, T, EXACT>, ends>(units, 1, threads, stream, args)
+                      : launch_attend_units<ends_kernel<ST, D, EJ, EW, true, T, EXACT>, ends>(units, 1, 64 * EW, stream, args);
     }
 }
 template <typename ST, int D> hipError_t launch_attend_of(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)

@@ -108,6 +108,25 @@ template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(c
     if constexpr (sizeof(ST) == 4) {
 #pragma unroll
         for (int e = 0; e < N; e++) out[0][e] = x[e];
+    } else if constexpr (std::is_same_v<ST, __bf16>) {
+        // Two at a time: one conversion makes both, and their 32 bits hold both floats (267 to 246 us of the gradients of queries below).
+        typedef float float2v __attribute__((ext_vector_type(2)));
+        typedef __bf16 pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            float2v rest = {x[e], x[e + 1]};
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+                const pair h = __builtin_convertvector(rest, pair);
+                out[t][e] = h[0];
+                out[t][e + 1] = h[1];
+                if (t + 1 < TERMS) {
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, h);
+                    rest[0] -= __builtin_bit_cast(float, bits << 16);  // (an infinity becomes a NaN)
+                    rest[1] -= __builtin_bit_cast(float, bits & 0xffff0000u);
+                }
+            }
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < N; e++) {
@@ -116,10 +135,10 @@ template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(c
             for (int t = 0; t < TERMS; t++) {
                 // (A product that is rounded to fp16 where it is made is rounded once; what is left must be what that rounding left, and not one's after the
                 // product was rounded to fp32: where the two differ, the next term would miss by a whole step.)
-                if constexpr (std::is_same_v<ST, _Float16>) asm("" : "+v"(rest));
+                asm("" : "+v"(rest));
                 const ST h = (ST)rest;
                 out[t][e] = h;
-                if (t + 1 < TERMS) rest -= (float)h;  // (an infinity becomes a NaN)
+                if (t + 1 < TERMS) rest -= (float)h;
             }
         }
     }

@@ -109,7 +109,7 @@ template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(c
 #pragma unroll
         for (int e = 0; e < N; e++) out[0][e] = x[e];
     } else if constexpr (std::is_same_v<ST, __bf16>) {
-        // Two at a time: one conversion makes both, and their 32 bits hold both floats (267 to 246 us of the gradients of queries below).
+        // Two at a time: one conversion makes both, and their 32 bits hold both floats (267 us of the gradients of queries below were 246).
         typedef float float2v __attribute__((ext_vector_type(2)));
         typedef __bf16 pair __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -589,30 +589,38 @@ __device__ __forceinline__ int64_t border_at(const AttendArgs &args, int64_t bat
     return (batch * args.most_borders + t / (kBorder * chunk)) * args.a.heads + head;
 }
 
-// The scores of a chunk in LDS, as operands: [tile of 16 columns][step of KS rows][lane] of 16 bytes each.
+// The scores of a chunk in LDS, as operands: [term][tile of 16 columns][step of KS rows][lane] of 16 bytes each. In 16 bits they have two terms:
+// the rounding of one is that of every result which it is the largest factor of, once more than the result's own.
 template <typename ST> struct Scores {
-    static constexpr int KS = Operand<ST>::KS, PER = KS / 16, C = Operand<ST>::CHUNK, STEPS = C / KS, WORDS = C * C * (int)sizeof(ST) / 4;
+    static constexpr int KS = Operand<ST>::KS, PER = KS / 16, C = Operand<ST>::CHUNK, STEPS = C / KS, TERMS = sizeof(ST) == 2 ? 2 : 1, ONE = C / 16 * STEPS * 64;
+    static constexpr int WORDS = TERMS * ONE * 4;
     frag_t<ST> *p;
-    __device__ __forceinline__ frag_t<ST> operand(int tile, int step) const { return p[(tile * STEPS + step) * 64 + (threadIdx.x & 63)]; }
+    __device__ __forceinline__ frag_t<ST> operand(int tile, int step, int term) const { return p[term * ONE + (tile * STEPS + step) * 64 + (threadIdx.x & 63)]; }
     // A 16 x 16 tile of rows row_tile * 16 ... and columns tile * 16 ...
     __device__ __forceinline__ void put(int tile, int row_tile, float4v v) const
     {
-        ST *at = reinterpret_cast<ST *>(p + (tile * STEPS + row_tile / PER) * 64 + (threadIdx.x & 63)) + row_tile % PER * 4;
         using raw_t = typename RawT<4 * sizeof(ST)>::type;
-        Elems<ST, 4> four;
+        const float f[4] = {v[0], v[1], v[2], v[3]};
+        frag_t<ST> terms[TERMS];
+        split<ST, TERMS>(f, terms);
 #pragma unroll
-        for (int r = 0; r < 4; r++) four.e[r] = (ST)v[r];
-        *reinterpret_cast<raw_t *>(at) = __builtin_bit_cast(raw_t, four);
+        for (int term = 0; term < TERMS; term++) {
+            Elems<ST, 4> four;
+#pragma unroll
+            for (int r = 0; r < 4; r++) four.e[r] = terms[term][r];
+            *reinterpret_cast<raw_t *>(reinterpret_cast<ST *>(p + term * ONE + (tile * STEPS + row_tile / PER) * 64 + (threadIdx.x & 63)) + row_tile % PER * 4) = __builtin_bit_cast(raw_t, four);
+        }
     }
     __device__ __forceinline__ float at(int row, int column) const
     {
-        const ST *e = reinterpret_cast<const ST *>(p + (column / 16 * STEPS + row / KS) * 64 + row % 16 / 4 * 16 + column % 16);
-        return (float)e[row % KS / 16 * 4 + row % 4];
+        const ST *e = reinterpret_cast<const ST *>(p + (column / 16 * STEPS + row / KS) * 64 + row % 16 / 4 * 16 + column % 16) + row % KS / 16 * 4 + row % 4;
+        const float most = (float)*e;
+        return TERMS == 2 && __builtin_isfinite(most) ? most + (float)e[ONE * (16 / sizeof(ST))] : most;
     }
     // Tiles beyond the diagonal that operands reach are zeros, and nobody writes them.
     __device__ __forceinline__ void clear() const
     {
-        for (int i = threadIdx.x; i < C / 16 * STEPS * 64; i += blockDim.x) reinterpret_cast<raw16 *>(p)[i] = raw16{0, 0, 0, 0};
+        for (int i = threadIdx.x; i < TERMS * ONE; i += blockDim.x) reinterpret_cast<raw16 *>(p)[i] = raw16{0, 0, 0, 0};
     }
 };
 
@@ -633,15 +641,18 @@ template <bool EXACT, typename ST> __device__ __forceinline__ void put4(ST *row,
 // Waves of a workgroup, or in the pass over keys and values of each of its kinds: four with up to two tiles of 16 columns each. (Eight waves of one tile
 // read the shared operands twice as often: [8, 4096, 16 x 128] in bf16 201 us forwards, 164 so.)
 template <int D> constexpr int attend_waves() { return D == 256 ? 8 : 4; }
+// Gradients of queries have a third more in registers. With three terms of 128 columns that is more than there are of them: eight waves of one tile take 269 us of
+// that layer, four 290. With two (fp16, [2, 4096, 32 x 128]) eight take 120 us, four 118.
+template <typename ST, int D> constexpr int query_waves() { return D == 128 && kTerms<ST> == 3 ? 8 : attend_waves<D>(); }
 
 // --- outputs (x, y, z = q, k, v) and, with GRAD, gradients of queries (x, y, z = do, v, k) with what decays read -----------------------
-template <typename ST, int D, bool GRAD> struct AttendLds {
-    static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<D>();
+template <typename ST, int W, int D, bool GRAD> struct AttendLds {
+    static constexpr int C = Operand<ST>::CHUNK;
     static constexpr int WORDS = 3 * Tile<ST, D>::WORDS + Scores<ST>::WORDS + Decays<C>::WORDS + (GRAD ? W * C + 2 * W : 0);
 };
-template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * attend_waves<D>(), 2) void attend_kernel(AttendArgs args)
+template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * W, 2) void attend_kernel(AttendArgs args)
 {
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const scanscam_attend &a = args.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
@@ -755,9 +766,12 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
             }
 #pragma unroll
             for (int step = 0; step <= tt / PER; step++) {
-                const frag_t<ST> p = scores.operand(tt, step);
 #pragma unroll
-                for (int jt = 0; jt < JT; jt++) sum[jt] = mma(own[jt][step], p, sum[jt]);
+                for (int term = Scores<ST>::TERMS; term-- > 0;) {
+                    const frag_t<ST> p = scores.operand(tt, step, term);
+#pragma unroll
+                    for (int jt = 0; jt < JT; jt++) sum[jt] = mma(own[jt][step], p, sum[jt]);
+                }
             }
             if constexpr (!GRAD) {
 #pragma unroll
@@ -782,7 +796,8 @@ template <typename ST, int D, int JT, bool GRAD, int TERMS, bool EXACT> __global
                             frag_t<ST> values = own[jt][step];
 #pragma unroll
                             for (int e = 0; e < 4 * PER; e++) values[e] = __builtin_isfinite((float)values[e]) ? values[e] : (ST)0.0f;
-                            clean = mma(values, scores.operand(tt, step), clean);
+#pragma unroll
+                            for (int term = Scores<ST>::TERMS; term-- > 0;) clean = mma(values, scores.operand(tt, step, term), clean);
                         }
 #pragma unroll
                         for (int r = 0; r < 4; r++) sum[jt][r] = __builtin_isfinite(alone[r]) ? clean[r] : alone[r];
@@ -1022,9 +1037,12 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
             }
 #pragma unroll
             for (int step = st / PER; step < STEPS; step++) {
-                const frag_t<ST> p = scores.operand(st, step);
 #pragma unroll
-                for (int jt = 0; jt < JT; jt++) acc[st][jt] = mma(own[jt][step], p, acc[st][jt]);
+                for (int term = Scores<ST>::TERMS; term-- > 0;) {
+                    const frag_t<ST> p = scores.operand(st, step, term);
+#pragma unroll
+                    for (int jt = 0; jt < JT; jt++) acc[st][jt] = mma(own[jt][step], p, acc[st][jt]);
+                }
             }
             if (s < n) {
                 const int64_t row = out_lane + (t0 + st * 16) * out_step;
@@ -1118,19 +1136,20 @@ template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPa
 {
     constexpr int WAVES = attend_waves<D>(), EJ = D == 256 ? 2 : 1, EW = D / 16 / EJ;  // (EJ, EW: of the ends, whole)
     constexpr int threads = 64 * WAVES, back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, HALF = EXACT ? 1 : ALL, T = kTerms<ST>, R = kTermsRounded<ST>;
-    constexpr int out = AttendLds<ST, D, false>::WORDS, grad = AttendLds<ST, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
+    constexpr int GW = query_waves<ST, D>(), GJ = D / 16 / GW;  // (of the queries' gradients, whole)
+    constexpr int out = AttendLds<ST, WAVES, D, false>::WORDS, grad_half = AttendLds<ST, WAVES, D, true>::WORDS, grad = AttendLds<ST, GW, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
     const bool k_half = ALL == 2 && args.a.K <= D / 2, v_half = ALL == 2 && args.a.V <= D / 2;
     const unsigned kinds = attend_both<D>() ? 1 : 2;
     switch (pass) {
     case kOutputs:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, false, T, EXACT>, out>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, ALL, false, T, EXACT>, out>(units, 1, threads, stream, args);
+        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, false, T, EXACT>, out>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, WAVES, false, T, EXACT>, out>(units, 1, threads, stream, args);
     case kOutputsRounded:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, false, R, EXACT>, out>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, ALL, false, R, EXACT>, out>(units, 1, threads, stream, args);
+        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, false, R, EXACT>, out>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, WAVES, false, R, EXACT>, out>(units, 1, threads, stream, args);
     case kQueries:
-        return k_half ? launch_attend_units<attend_kernel<ST, D, HALF, true, T, EXACT>, grad>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, ALL, true, T, EXACT>, grad>(units, 1, threads, stream, args);
+        return k_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, true, T, EXACT>, grad_half>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, GJ, GW, true, T, EXACT>, grad>(units, 1, 64 * GW, stream, args);
     case kKeysAndValues:  // (both are not halves at once)
         if (k_half) return launch_attend_units<attend_back_kernel<ST, D, HALF, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
         if (v_half) return launch_attend_units<attend_back_kernel<ST, D, ALL, HALF, EXACT>, back>(units, kinds, back_threads, stream, args);

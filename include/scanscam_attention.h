@@ -38,7 +38,7 @@ typedef struct scanscam_attend {
     const void *offsets; /* or NULL */
     int32_t offsets64, dtype, decay_dtype, decay_fixed;
     float scale;
-    int32_t parts;                 /* of time that a sequence is shared out in; 0: chosen */
+    int32_t parts;                 /* of time that a sequence of T tokens is shared out in; 0: chosen */
     scanscam_tokens q, k, v, y;
     scanscam_tokens decay;         /* or NULL */
     const float *state_in;         /* [sequences, heads, K, V], or NULL */

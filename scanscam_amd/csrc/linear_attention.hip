@@ -4,35 +4,44 @@
 
 namespace scanscam {
 
-// The states that parts start from, out of what each adds: in the parts' order, or from the last part on (gradients). AHEAD parts are asked for
-// together: one after the other each would be a trip to memory (128 parts of 4 heads: 37 us, 24 by sixteens).
-struct Joined {
-    float *ends;
-    const double *logs;
-    const float *from;  // [pairs][values], or NULL
-    int64_t pairs, pair0;
-    int32_t parts, values, back;
-};
-template <int AHEAD> __global__ __launch_bounds__(256) void join_kernel(Joined a)
+// The states at the borders between parts, out of what each adds: in the parts' order, or from the last part on (gradients). AHEAD borders are asked for
+// together: one after the other each would be a trip to memory (128 parts of 4 heads: 37 us, 24 by sixteens). A lane takes VALUES of them.
+template <int AHEAD, int VALUES, bool BACK> __global__ __launch_bounds__(256) void join_kernel(AttendArgs args)
 {
-    const int at = blockIdx.y * 256 + threadIdx.x;
-    const int64_t pair = a.pair0 + blockIdx.x;
-    if (at >= a.values) return;
-    float run = a.from == nullptr ? 0.0f : a.from[pair * a.values + at];
-    for (int i0 = 0; i0 < a.parts; i0 += AHEAD) {
-        float adds[AHEAD], decay[AHEAD];
-        const auto unit = [&](int i) { return pair * a.parts + (a.back ? a.parts - 1 - i : i); };
+    const scanscam_attend &a = args.a;
+    const int64_t pair = args.first + blockIdx.x, values = a.K * a.V, at = (int64_t)blockIdx.y * 256 * VALUES + threadIdx.x;
+    Span s;
+    s.sequence = pair / a.heads;
+    s.head = (int)(pair % a.heads);
+    s.parts = args.parts;
+    s.cut = s.sequence * (s.parts - 1);
+    if (a.offsets != nullptr && !count_parts(args, s.sequence, 0, s)) return;
+    const int borders = s.parts - 1;
+    if (borders == 0) return;
+    const float *given = BACK ? a.gstate_out : a.state_in;
+    float *ends = (BACK ? args.back_ends : args.ends) + at;
+    const double *logs = args.logs;
+    const auto border = [&](int i) { return cut_at(args, s, BACK ? borders - 1 - i : i); };
+    float run[VALUES];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {  // (the last one's was not computed)
-            const bool there = i0 + i + 1 < a.parts;
-            adds[i] = there ? a.ends[unit(i0 + i) * a.values + at] : 0.0f;
-            decay[i] = there ? exp2_(a.logs[unit(i0 + i)]) : 0.0f;
+    for (int v = 0; v < VALUES; v++) run[v] = given != nullptr && at + 256 * v < values ? given[pair * values + at + 256 * v] : 0.0f;
+    for (int i0 = 0; i0 < borders; i0 += AHEAD) {
+        float adds[AHEAD][VALUES], decay[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int there = i0 + i < borders ? i0 + i : borders - 1;
+            decay[i] = exp2_(logs[border(there)]);
+#pragma unroll
+            for (int v = 0; v < VALUES; v++) adds[i][v] = at + 256 * v < values ? ends[border(there) * values + 256 * v] : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
-            if (i0 + i < a.parts) {
-                a.ends[unit(i0 + i) * a.values + at] = run;
-                run = run * decay[i] + adds[i];
+            if (i0 + i < borders) {
+#pragma unroll
+                for (int v = 0; v < VALUES; v++) {
+                    run[v] = run[v] * decay[i] + adds[i][v];
+                    if (at + 256 * v < values) ends[border(i0 + i) * values + 256 * v] = run[v];
+                }
             }
     }
 }
@@ -43,8 +52,9 @@ template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(A
 {
     const scanscam_attend &a = args.a;
     AttendArgs whole = args;
-    whole.parts = 1;
-    const Span span = span_of(whole, args.first + blockIdx.x, C);
+    whole.per = 0;
+    Span span;
+    if (!span_of(whole, args.first + blockIdx.x, C, span)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __shared__ double over[kBorder];
     const int64_t chunks = (span.length + C - 1) / C, base = span.head * args.tokens + span.batch * a.T;
@@ -55,7 +65,7 @@ template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(A
         const double reads = sums_upto(read), writes = sums_upto(write), all_reads = read_lane(reads, 63), all_writes = read_lane(writes, 63);
         if (lane == 0) over[wave] = all_reads - all_writes;
         __syncthreads();
-        double end = first + kBorder < chunks ? args.cross[border_at(args, span.batch, span.from + (first + kBorder) * C, C, span.head)] : args.last[span.unit];
+        double end = first + kBorder < chunks ? args.cross[border_at(args, span.batch, span.from + (first + kBorder) * C, C, span.head)] : args.last[args.first + blockIdx.x];
         for (int w = 0; w < wave; w++) end += over[w];
         if (there) args.decays[(span.batch * a.T + t) * a.heads + span.head] = (float)((end - all_writes) + (all_reads - reads + read) + (writes - write));
         __syncthreads();
@@ -207,14 +217,42 @@ int check_attend(const scanscam_attend *a, bool back)
 
 int chunk_of(const scanscam_attend &a) { return a.dtype == SCANSCAM_F32 ? Operand<float>::CHUNK : Operand<__bf16>::CHUNK; }
 
-int parts_of(const scanscam_attend &a)
+// How time is shared out. Parts cost a second pass over keys and values, and states at their borders; they are for calls with fewer heads of sequences
+// than it takes to fill the card, two workgroups on each of 256 CUs: up to 512 parts of no less than four chunks. ([8, 4096, 16 x 128] in bf16 with gradients
+// by 1, 2, 4, 8 parts: 1.74, 1.16, 0.99, 1.09 ms; 30001 tokens of four heads in float32 by 64, 128: 425, 416 us.)
+// Of sequences behind each other the host knows all tokens only. Their parts have one length, which makes 384 of all tokens, and the sequences' last ones, shorter as
+// they are, come on top: 8021 tokens of 13 sequences of 16 heads, from equal ones to one with two thirds of the tokens, 99 - 109 us; with 512 114 - 124,
+// 256 117 - 125, and in one part each 114 - 492. A sequence that is no longer than a part is one, and costs an empty workgroup in either of the passes more.
+// (Sequences enough fill the card by themselves, and every workgroup would count them.)
+struct Plan {
+    int64_t per;                         // tokens of a part, whole chunks; 0: all of the sequence
+    int64_t units, borders;              // heads of parts; borders between parts, at most
+    int parts;                           // of a sequence of T tokens
+};
+Plan plan_of(const scanscam_attend &a)
 {
-    if (a.parts > 0) return a.parts;
-    const int64_t pairs = a.sequences * a.heads, chunks = ceil_div(a.T, chunk_of(a));
-    if (pairs == 0 || pairs >= 256) return 1;
-    int64_t parts = 512 / pairs;
-    parts = parts < chunks / 4 ? parts : chunks / 4;
-    return parts < 2 ? 1 : (int)parts;
+    const int chunk = chunk_of(a);
+    const int64_t pairs = a.sequences * a.heads, chunks = ceil_div(a.T, chunk);
+    Plan p{0, pairs, 0, 1};
+    if (a.offsets != nullptr && a.sequences != 1) {
+        int64_t per = a.parts > 0 ? ceil_div(chunks, a.parts) : ceil_div(chunks * a.heads, 384);
+        if (a.parts == 0) per = pairs >= 4096 ? chunks : per < 4 ? 4 : per;
+        if (per < 1 || per * chunk > a.T) return p;
+        p.per = per * chunk;
+        p.borders = a.T / p.per;
+        p.units = (a.sequences + p.borders) * a.heads;
+        p.parts = (int)ceil_div(chunks, per);
+        return p;
+    }
+    int64_t parts = a.parts;
+    if (parts == 0 && pairs > 0 && pairs < 256) parts = 512 / pairs < chunks / 4 ? 512 / pairs : chunks / 4;
+    if (parts < 2) return p;
+    p.per = ceil_div(chunks, parts) * chunk;
+    if (p.per == 0) p.per = chunk;
+    p.parts = (int)parts;
+    p.borders = a.sequences * (parts - 1);
+    p.units = pairs * parts;
+    return p;
 }
 
 // What the workspace holds, in order; each piece begins on 16 bytes.
@@ -222,8 +260,8 @@ struct Pieces {
     size_t ends, back_ends, logs, reads, writes, inside, last, borders, cross, part_q, part_k, decays, bytes;
     int64_t most_borders;
 };
-int64_t ends_values(const scanscam_attend &a, int parts) { return a.sequences * a.heads * parts * a.K * a.V; }
-Pieces pieces_of(const scanscam_attend &a, bool back, int parts)
+int64_t ends_values(const scanscam_attend &a, const Plan &plan) { return plan.borders * a.heads * a.K * a.V; }
+Pieces pieces_of(const scanscam_attend &a, bool back, const Plan &plan)
 {
     Pieces p{};
     const auto take = [&](bool there, int64_t count, size_t size) {
@@ -231,11 +269,11 @@ Pieces pieces_of(const scanscam_attend &a, bool back, int parts)
         if (there) p.bytes += ((size_t)count * size + 15) / 16 * 16;
         return at;
     };
-    const int64_t pairs = a.sequences * a.heads, values = ends_values(a, parts), tokens = a.batch * a.T;
-    p.ends = take(parts > 1 && !back, values, 4);  // (a backward call has the forward one's)
-    p.logs = take(parts > 1, pairs * parts, 8);
+    const int64_t pairs = a.sequences * a.heads, values = ends_values(a, plan), tokens = a.batch * a.T;
+    p.ends = take(!back, values, 4);  // (a backward call has the forward one's)
+    p.logs = take(true, plan.borders * a.heads, 8);
     if (!back) return p;
-    p.back_ends = take(parts > 1, values, 4);
+    p.back_ends = take(true, values, 4);
     p.reads = take(true, tokens * a.heads, 4);
     p.writes = take(true, tokens * a.heads, 4);
     p.inside = take(true, tokens * a.heads, 4);
@@ -259,16 +297,25 @@ hipError_t run(AttendPass pass, int64_t units, hipStream_t stream, const AttendA
     }
 }
 
-// The states that parts start from.
-hipError_t starts(const AttendArgs &args, bool back, AttendPass pass, hipStream_t stream)
+// The states at the borders between parts.
+template <int AHEAD, int VALUES> hipError_t join_with(const AttendArgs &args, bool back, int64_t pairs, hipStream_t stream)
 {
-    const scanscam_attend &a = args.a;
-    const int64_t pairs = a.sequences * a.heads;
-    hipError_t err = run(pass, pairs * args.parts, stream, args);
-    Joined j{back ? args.back_ends : args.ends, args.logs, back ? a.gstate_out : a.state_in, pairs, 0, args.parts, (int32_t)(a.K * a.V), back};
+    const dim3 grid((unsigned)pairs, (unsigned)ceil_div(args.a.K * args.a.V, 256 * VALUES));
+    return launch_op(back ? join_kernel<AHEAD, VALUES, true> : join_kernel<AHEAD, VALUES, false>, grid, dim3(256), 0, stream, args);
+}
+hipError_t starts(AttendArgs args, bool back, AttendPass pass, int64_t units, hipStream_t stream)
+{
+    const int64_t pairs = args.a.sequences * args.a.heads;
+    hipError_t err = run(pass, units, stream, args);
     constexpr int64_t most = 1 << 22;
-    for (; j.pair0 < pairs && err == hipSuccess; j.pair0 += most)
-        err = launch_op(args.parts <= 4 ? join_kernel<4> : join_kernel<16>, dim3((unsigned)(pairs - j.pair0 < most ? pairs - j.pair0 : most), (unsigned)ceil_div(a.K * a.V, 256)), dim3(256), 0, stream, j);
+    // Four values a lane where their states are half a million or more: there are workgroups enough without. (Packed prompts' 208 states of 128 x 128: 21 us, 56 by one;
+    // four parts of 128 of them 10 us, 16 by one; 127 parts of four of 48 x 72 33 us, 19 by one.)
+    const bool many = pairs * args.a.K * args.a.V >= 1 << 19, few = args.parts <= 4;
+    for (args.first = 0; args.first < pairs && err == hipSuccess; args.first += most) {
+        const int64_t now = pairs - args.first < most ? pairs - args.first : most;
+        if (few) err = many ? join_with<4, 4>(args, back, now, stream) : join_with<4, 1>(args, back, now, stream);
+        else err = many ? join_with<16, 4>(args, back, now, stream) : join_with<16, 1>(args, back, now, stream);
+    }
     return err;
 }
 
@@ -309,35 +356,36 @@ extern "C" {
 
 size_t scanscam_attend_saved_bytes(const scanscam_attend *a)
 {
-    const int parts = sizes_fit(a) ? parts_of(*a) : 1;
-    return parts > 1 ? (size_t)ends_values(*a, parts) * sizeof(float) : 0;
+    return sizes_fit(a) ? (size_t)ends_values(*a, plan_of(*a)) * sizeof(float) : 0;
 }
 
 size_t scanscam_attend_workspace_bytes(const scanscam_attend *a, int direction)
 {
-    return sizes_fit(a) ? pieces_of(*a, direction == SCANSCAM_BACKWARD, parts_of(*a)).bytes : 0;
+    return sizes_fit(a) ? pieces_of(*a, direction == SCANSCAM_BACKWARD, plan_of(*a)).bytes : 0;
 }
 
 int scanscam_attend_fwd(const scanscam_attend *a, void *stream)
 {
     SCANSCAM_CHECK(check_attend(a, false));
     if (a->sequences == 0 || a->heads == 0 || (a->batch * a->T == 0 && a->state_out == nullptr)) return SCANSCAM_OK;
-    const int parts = parts_of(*a);
-    const Pieces at = pieces_of(*a, false, parts);
+    const Plan plan = plan_of(*a);
+    const Pieces at = pieces_of(*a, false, plan);
     if (at.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < at.bytes)) return SCANSCAM_EWORKSPACE;
     if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
     char *w = static_cast<char *>(a->workspace);
     AttendArgs args{};
     args.a = *a;
     args.tokens = a->batch * a->T;
-    args.parts = parts;
+    args.per = plan.per;
+    args.parts = plan.parts;
+    args.cuts = plan.borders;
     args.each = (int32_t)(a->heads / a->groups);
     args.ends = a->saved != nullptr ? static_cast<float *>(a->saved) : reinterpret_cast<float *>(w + at.ends);
     args.logs = reinterpret_cast<double *>(w + at.logs);
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t err = hipSuccess;
-    if (parts > 1) err = starts(args, false, kEnds, s);
-    if (err == hipSuccess) err = run(a->state_out != nullptr ? kOutputs : kOutputsRounded, a->sequences * a->heads * parts, s, args);
+    if (plan.borders > 0) err = starts(args, false, kEnds, plan.units, s);
+    if (err == hipSuccess) err = run(a->state_out != nullptr ? kOutputs : kOutputsRounded, plan.units, s, args);
     return code(err);
 }
 
@@ -349,16 +397,18 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     if (a->heads == 0) return SCANSCAM_OK;
     if (a->sequences == 0 || (a->batch * a->T == 0 && a->gstate_in == nullptr))
         return a->gdecay != nullptr && a->decay_fixed ? code(column_sum({nullptr, 0, 0, {a->gdecay}, {a->heads}}, s)) : SCANSCAM_OK;
-    const int parts = parts_of(*a);
-    const Pieces at = pieces_of(*a, true, parts);
+    const Plan plan = plan_of(*a);
+    const Pieces at = pieces_of(*a, true, plan);
     if (at.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < at.bytes)) return SCANSCAM_EWORKSPACE;
     if (misaligned(a->workspace, 16)) return SCANSCAM_EALIGN;
-    if (parts > 1 && a->saved == nullptr) return SCANSCAM_EINVAL;
+    if (plan.borders > 0 && a->saved == nullptr) return SCANSCAM_EINVAL;
     char *w = static_cast<char *>(a->workspace);
     AttendArgs args{};
     args.a = *a;
     args.tokens = a->batch * a->T;
-    args.parts = parts;
+    args.per = plan.per;
+    args.parts = plan.parts;
+    args.cuts = plan.borders;
     args.each = (int32_t)(a->heads / a->groups);
     args.ends = static_cast<float *>(a->saved);
     args.back_ends = reinterpret_cast<float *>(w + at.back_ends);
@@ -381,9 +431,9 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     }
     const int64_t pairs = a->sequences * a->heads;
     hipError_t err = hipSuccess;
-    if (parts > 1) err = starts(args, true, kBackEnds, s);
-    if (err == hipSuccess) err = run(kQueries, pairs * parts, s, args);
-    if (err == hipSuccess) err = run(kKeysAndValues, pairs * parts, s, args);
+    if (plan.borders > 0) err = starts(args, true, kBackEnds, plan.units, s);
+    if (err == hipSuccess) err = run(kQueries, plan.units, s, args);
+    if (err == hipSuccess) err = run(kKeysAndValues, plan.units, s, args);
     if (a->gdecay != nullptr && err == hipSuccess) {
         constexpr int64_t most = 1 << 21;
         for (args.first = 0; args.first < pairs && err == hipSuccess; args.first += most) {

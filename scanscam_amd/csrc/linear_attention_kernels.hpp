@@ -40,9 +40,12 @@ struct AttendArgs {
     scanscam_attend a;
     int64_t first;            // the first unit of this launch; a unit is a part of a head of a sequence
     int64_t tokens;           // batch * T
-    int32_t parts, each;      // parts of a sequence, heads that share queries and keys
-    float *ends, *back_ends;  // [sequences][heads][parts][K][V]: what a part adds to the state; then the state that it starts from
-    double *logs;             // [sequences][heads][parts]: the part's sum of decays
+    int64_t per, cuts;        // tokens of a part, whole chunks (0: all of the sequence); borders between parts that there is room for
+    int32_t parts, each;      // parts of a sequence of T tokens, heads that share queries and keys
+    // [heads][border between parts][K][V]: what the part before it (gradients: behind it) adds to the state, then the state there; and [heads][border between parts],
+    // the sum of that part's decays. The borders of a sequence follow each other, those of all sequences too.
+    float *ends, *back_ends;
+    double *logs;
     float *reads, *writes, *inside;  // [heads][tokens]: R[t], W[t], and the sum of M[t,s] over s less that of M[s,t]
     double *last;             // [sequences][heads]: <gradient of the last state, last state>
     float *borders;           // [border][heads]: the state at a border, tile by tile as the lanes hold it
@@ -260,18 +263,11 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
 // The tokens that a workgroup goes through: a part of a sequence, of whole chunks but for the last.
 struct Span {
     int64_t sequence, batch, from, begin, end, length;  // from, begin and end: tokens of the batch element; from and length: of the sequence
-    int head, part;
-    int64_t unit;
+    int64_t cut;  // the first of the sequence's borders between parts
+    int head, part, parts;
 };
-__device__ __forceinline__ Span span_of(const AttendArgs &args, int64_t unit, int chunk)
+__device__ __forceinline__ void span_of_sequence(const scanscam_attend &a, Span &s)
 {
-    const scanscam_attend &a = args.a;
-    Span s;
-    s.unit = unit;
-    s.part = (int)(unit % args.parts);
-    const int64_t rest = unit / args.parts;
-    s.head = (int)(rest % a.heads);
-    s.sequence = rest / a.heads;
     int64_t from = 0, to = a.T;
     s.batch = s.sequence;
     if (a.offsets != nullptr) {
@@ -281,10 +277,80 @@ __device__ __forceinline__ Span span_of(const AttendArgs &args, int64_t unit, in
     }
     s.from = from;
     s.length = to - from;
-    const int64_t chunks = (s.length + chunk - 1) / chunk, per = (chunks + args.parts - 1) / args.parts * chunk;
-    s.begin = from + (s.part * per < s.length ? s.part * per : s.length);
-    s.end = from + ((s.part + 1) * per < s.length ? (s.part + 1) * per : s.length);
-    return s;
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane)
+{
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)v, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (int64_t)(hi << 32 | lo);
+}
+// Parts of sequences of different lengths: a long one has more. Every wave counts for itself, 64 sequences at a time: those of the sequences before `sequence`, or where
+// that is negative before the one that part `slot` of all belongs to, which s then holds (false if there is none, or no room for its borders).
+__device__ __forceinline__ bool count_parts(const AttendArgs &args, int64_t sequence, int64_t slot, Span &s)
+{
+    const scanscam_attend &a = args.a;
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0;
+    for (int64_t first = 0; first < a.sequences; first += 64) {
+        Span at;
+        at.sequence = first + lane;
+        int64_t parts = 0;
+        if (at.sequence < a.sequences) {
+            span_of_sequence(a, at);
+            const int64_t whole = (at.length + args.per - 1) / args.per;
+            parts = whole < 1 ? 1 : whole;
+        }
+        int64_t upto = parts;
+#pragma unroll
+        for (int step = 1; step < 64; step *= 2) {
+            const int64_t other = __shfl_up(upto, step, 64);
+            if (lane >= step) upto += other;
+        }
+        const uint64_t found = __ballot(sequence >= 0 ? at.sequence == sequence : at.sequence < a.sequences && before + upto > slot);
+        if (found != 0) {
+            const int there = __builtin_ctzll(found);
+            s.parts = (int)lane_of(parts, there);
+            s.sequence = first + there;
+            before += lane_of(upto, there) - s.parts;
+            s.part = (int)(slot - before);
+            s.cut = before - s.sequence;
+            return s.cut + s.parts - 1 <= args.cuts;  // (always, but with offsets that go back)
+        }
+        before += lane_of(upto, 63);
+    }
+    return false;
+}
+// The span of a unit; false if there is none.
+__device__ __forceinline__ bool span_of(const AttendArgs &args, int64_t unit, int chunk, Span &s)
+{
+    const scanscam_attend &a = args.a;
+    // (Parts are next to each other: heads of the same tokens, which can share lines of memory, would be on different XCDs. 30001 tokens of 4 heads of 48 and 72
+    // in float32, with gradients: 450 us, 428 so.)
+    if (args.per == 0 || a.offsets == nullptr) {
+        s.parts = args.per == 0 ? 1 : args.parts;
+        s.part = (int)(unit % s.parts);
+        s.head = (int)(unit / s.parts % a.heads);
+        s.sequence = unit / s.parts / a.heads;
+        s.cut = s.sequence * (s.parts - 1);
+    } else {
+        const int64_t slots = a.sequences + args.cuts;
+        s.head = (int)(unit / slots);
+        if (!count_parts(args, -1, unit % slots, s)) return false;
+    }
+    span_of_sequence(a, s);
+    const int64_t per = args.per == 0 ? s.length : args.per;
+    s.begin = s.from + (s.part * per < s.length ? s.part * per : s.length);
+    s.end = s.from + ((s.part + 1) * per < s.length ? (s.part + 1) * per : s.length);
+    return true;
+}
+__device__ __forceinline__ int64_t cut_at(const AttendArgs &args, const Span &s, int i) { return s.head * args.cuts + s.cut + i; }
+// Where the state lies that a part starts from: the given one, or that at the border before it (gradients: behind it).
+__device__ __forceinline__ const float *start_of(const AttendArgs &args, const Span &s, bool back)
+{
+    const scanscam_attend &a = args.a;
+    const int64_t values = (int64_t)a.K * a.V;
+    if (s.part != (back ? s.parts - 1 : 0)) return (back ? args.back_ends : args.ends) + cut_at(args, s, s.part - (back ? 0 : 1)) * values;
+    const float *given = back ? a.gstate_out : a.state_in;
+    return given == nullptr ? nullptr : given + (s.sequence * a.heads + s.head) * values;
 }
 
 template <typename ST> __device__ __forceinline__ const ST *tensor_at(const scanscam_tokens &t, const Span &s, int64_t head)
@@ -664,7 +730,8 @@ template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> _
     float *red = GRAD ? take(W * C) : nullptr;
     double *last = GRAD ? reinterpret_cast<double *>(take(2 * W)) : nullptr;
 
-    const Span span = span_of(args, args.first + blockIdx.x, C);
+    Span span;
+    if (!span_of(args, args.first + blockIdx.x, C, span)) return;
     const int64_t shared = span.head / args.each;
     const int K = (int)a.K, V = (int)a.V;
     const scanscam_tokens &xt = GRAD ? a.gy : a.q, &yt = GRAD ? a.v : a.k, &zt = GRAD ? a.k : a.v;
@@ -681,7 +748,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> _
 
     State<ST, D, JT, W> S;
     S.wave = wave;
-    S.read(args.parts > 1 ? args.ends + span.unit * K * V : a.state_in == nullptr ? nullptr : a.state_in + pair * K * V, inner, outer, row_step, col_step);
+    S.read(start_of(args, span, false), inner, outer, row_step, col_step);
     scores.clear();
 
     Staged<ST, D, NT, EXACT> sx(x, xt.token, inner), sy(y, yt.token, inner), sz(z, zt.token, outer);
@@ -835,7 +902,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> _
             }
         }
     }
-    if (span.part == args.parts - 1) {
+    if (span.part == span.parts - 1) {
         if constexpr (!GRAD) {
             if (a.state_out != nullptr) S.write(a.state_out + pair * K * V, inner, outer, row_step, col_step);
         } else if (args.last != nullptr) {
@@ -867,8 +934,8 @@ template <typename ST, int D, int JT, int W, bool BACK, int TERMS, bool EXACT> _
     Tile<ST, D> Y{reinterpret_cast<ST *>(lds)}, Z{reinterpret_cast<ST *>(lds + Tile<ST, D>::WORDS)};
     float *rest = lds + 2 * Tile<ST, D>::WORDS;
     Decays<C> decays{reinterpret_cast<double *>(rest), rest + 2 * C, rest + 3 * C};
-    const Span span = span_of(args, args.first + blockIdx.x, C);
-    if (span.part == (BACK ? 0 : args.parts - 1)) return;  // (nothing starts from its end)
+    Span span;
+    if (!span_of(args, args.first + blockIdx.x, C, span) || span.part == (BACK ? 0 : span.parts - 1)) return;  // (nothing starts from the last one's end)
     const int K = (int)a.K, V = (int)a.V;
     const scanscam_tokens &yt = BACK ? a.gy : a.k, &zt = BACK ? a.q : a.v;
     const int64_t shared = span.head / args.each;
@@ -908,8 +975,9 @@ template <typename ST, int D, int JT, int W, bool BACK, int TERMS, bool EXACT> _
         S.template update<TERMS>(Y, inner, own, BACK ? decays.upto : decays.after, BACK ? a.scale : 1.0f, decays.whole());
         __syncthreads();
     }
-    S.write((BACK ? args.back_ends : args.ends) + span.unit * K * V, inner, outer, row_step, col_step);
-    if (threadIdx.x == 0) args.logs[span.unit] = whole;
+    const int64_t border = cut_at(args, span, span.part - (BACK ? 1 : 0));
+    S.write((BACK ? args.back_ends : args.ends) + border * K * V, inner, outer, row_step, col_step);
+    if (threadIdx.x == 0) args.logs[border] = whole;
 }
 
 // --- gradients of keys and values, backwards in time ------------------------------------------------------------------------------------
@@ -940,7 +1008,8 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
     double *over = reinterpret_cast<double *>(take(2 * W));
     float *rows = take(TT * C), *cols = take(TT * C);  // sums of M over each tile's rows and columns
 
-    const Span span = span_of(args, args.first + blockIdx.x, C);
+    Span span;
+    if (!span_of(args, args.first + blockIdx.x, C, span)) return;
     const int64_t shared = span.head / args.each, pair = span.sequence * a.heads + span.head;
     const int K = (int)a.K, V = (int)a.V;
     const ST *q = tensor_at<ST>(a.q, span, shared), *k = tensor_at<ST>(a.k, span, shared), *v = tensor_at<ST>(a.v, span, span.head), *o = tensor_at<ST>(a.gy, span, span.head);
@@ -953,7 +1022,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
 
     State<ST, D, JT, W> H;
     H.wave = wave;
-    H.read(args.parts > 1 ? args.back_ends + span.unit * K * V : a.gstate_out == nullptr ? nullptr : a.gstate_out + pair * K * V, inner, outer, row_step, col_step);
+    H.read(start_of(args, span, true), inner, outer, row_step, col_step);
     of_keys.clear();
     if constexpr (BOTH) of_values.clear();
 

@@ -241,3 +241,17 @@ def test_float32_results_of_16_bits_are_float32_s(gpu, dtype):
         grads.append(torch.autograd.grad((y, state), [leaves["decay"], leaves["state"]], [w.to(dtype).to(t) if t is y else w.float().to(t) for w, t in zip(weights, (y, state))]))
     for want, got in [outs] + list(zip(*grads)):
         assert (got.detach().cpu().double() - want.detach()).norm() <= 2.0 ** -19 * want.detach().norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("parts", [0, 7, 45, 200])
+def test_long_and_short_sequences_behind_each_other(gpu, monkeypatch, dtype, parts):
+    """A long one is shared out in more parts than a short one."""
+    test_attention_and_gradients(gpu, monkeypatch, dtype, 0, 0, 2, 32, 24, {"lengths": [1, 0, 900, 64, 3, 2000, 130, 0], "state": True}, parts, False)
+
+
+def test_more_sequences_than_a_wave_counts_at_once(gpu, monkeypatch):
+    lengths = [(7 * i) % 40 for i in range(150)]
+    lengths[70], lengths[149] = 700, 300
+    test_attention_and_gradients(gpu, monkeypatch, torch.bfloat16, 0, 0, 2, 16, 20, {"lengths": lengths, "state": True}, 0, True)
+    test_attention_and_gradients(gpu, monkeypatch, torch.bfloat16, 0, 0, 2, 16, 20, {"lengths": lengths, "state": True}, 20, False)

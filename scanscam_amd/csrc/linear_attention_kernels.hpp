@@ -83,7 +83,7 @@ __device__ __forceinline__ float4v mma(const float4v &a, const float4v &b, float
 
 // Terms of the activations' type that a float32 factor is taken apart into where float32 results come from it (states that are handed over, gradients
 // of states and of decays): all 24 bits, 22 in fp16. Where only 16-bit results come from it the state is read in one term, whose rounding is like the
-// result's own, and what is added to it has two (with one, results were 1.6 times as far from 64 bits as rounded ones are, with two 1.35 times).
+// result's own, and what is added to it has two (with one, results were up to 1.6 times as far from 64 bits as rounded ones are, with two and two of the scores 1.3 times).
 template <typename ST> constexpr int kTerms = 3;
 template <> inline constexpr int kTerms<_Float16> = 2;
 template <> inline constexpr int kTerms<float> = 1;

@@ -212,7 +212,7 @@ template <typename ST, int D, int NT, bool EXACT> struct Staged {
     int64_t stride;
     int d, col, drop;  // (drop: elements of this lane's vector that come before its column)
     // Where a row ends inside a vector the vector is the row's last whole one, and what of it belongs to the lane before is shifted out on the way to LDS: loads under a
-    // condition of the lanes are waited for one after the other ([25, 656, 5 heads of 194 and 27] in bf16: 237 us that way, 198 this way).
+    // condition of the lanes are waited for one after the other ([25, 656, 5 heads of 194 and 27] in bf16: 237 us that way, 198 this way, before halves).
     __device__ __forceinline__ Staged(const ST *base, int64_t token_stride, int channels) : stride(token_stride), d(channels)
     {
         col = threadIdx.x % ROW * VE;
@@ -1223,12 +1223,12 @@ template <auto Kernel, int WORDS> hipError_t launch_attend_units(int64_t units, 
     return hipSuccess;
 }
 
-// Column tiles of a wave by the columns that there are: a head of up to 64 (of the 256 kind 128) leaves half of the waves' registers and products out
-// (whole vectors only: the other kernels are rare, and theirs are as many again).
+// Column tiles of a wave by the columns that there are: a head of up to 64 (of the 256 kind 128) leaves half of the waves' registers and products out.
 template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPass pass, int64_t units, hipStream_t stream, const AttendArgs &args)
 {
     constexpr int WAVES = attend_waves<D>(), EJ = D == 256 ? 2 : 1, EW = D / 16 / EJ;  // (EJ, EW: of the ends, whole)
-    constexpr int threads = 64 * WAVES, back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, HALF = EXACT ? 1 : ALL, T = kTerms<ST>, R = kTermsRounded<ST>;
+    // HALF: column tiles of a wave for a side that fills no more than half of them ([25, 656, 5 heads of 194 and 27] in bf16: 88 us, 198 with all).
+    constexpr int threads = 64 * WAVES, back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, HALF = 1, T = kTerms<ST>, R = kTermsRounded<ST>;
     constexpr int GW = query_waves<ST, D>(), GJ = D / 16 / GW;  // (of the queries' gradients, whole)
     constexpr int out = AttendLds<ST, WAVES, D, false>::WORDS, grad_half = AttendLds<ST, WAVES, D, true>::WORDS, grad = AttendLds<ST, GW, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
     const bool k_half = ALL == 2 && args.a.K <= D / 2, v_half = ALL == 2 && args.a.V <= D / 2;

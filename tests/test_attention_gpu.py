@@ -255,3 +255,11 @@ def test_more_sequences_than_a_wave_counts_at_once(gpu, monkeypatch):
     lengths[70], lengths[149] = 700, 300
     test_attention_and_gradients(gpu, monkeypatch, torch.bfloat16, 0, 0, 2, 16, 20, {"lengths": lengths, "state": True}, 0, True)
     test_attention_and_gradients(gpu, monkeypatch, torch.bfloat16, 0, 0, 2, 16, 20, {"lengths": lengths, "state": True}, 20, False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,V", [(200, 27), (61, 199), (101, 30), (5, 90), (130, 3)])
+@pytest.mark.parametrize("T,parts", [(70, 0), (203, 2)])
+def test_one_side_half_as_wide_or_less(gpu, monkeypatch, dtype, K, V, T, parts):
+    """Waves hold half as many columns where a side leaves half of them empty."""
+    test_attention_and_gradients(gpu, monkeypatch, dtype, 2, T, 2, K, V, {"groups": 1, "state": True}, parts, False)

@@ -385,7 +385,7 @@ int scanscam_attend_fwd(const scanscam_attend *a, void *stream)
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t err = hipSuccess;
     if (plan.borders > 0) err = starts(args, false, kEnds, plan.units, s);
-    if (err == hipSuccess) err = run(a->state_out != nullptr ? kOutputs : kOutputsRounded, plan.units, s, args);
+    if (err == hipSuccess) err = run(kOutputs, plan.units, s, args);
     return code(err);
 }
 

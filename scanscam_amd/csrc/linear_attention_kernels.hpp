@@ -27,7 +27,7 @@
 //
 // What bounds it: neither memory nor the matrix unit, but the chain of a chunk (loads to LDS, scores, a barrier, sums, the state's update, a barrier) in few waves,
 // for a state's columns and a chunk's operands leave registers for two waves a SIMD. [8, 4096, 16 x 128] in bf16, in four parts: ends of parts 60 us, outputs
-// 140 (of 537 MB, 3.8 TB/s; the kernel's products are 40 us of the matrix unit), ends backwards 72, gradients of queries 268, of keys and values 402, decays 10.
+// 161 (of 537 MB, 3.3 TB/s), ends backwards 72, gradients of queries 267, of keys and values 418, decays 10.
 // In counters the matrix unit is busy for a fifth of these, the vector unit (terms, decays, addresses) for a third.
 #pragma once
 
@@ -82,8 +82,8 @@ __device__ __forceinline__ float4v mma(const float4v &a, const float4v &b, float
 }
 
 // Terms of the activations' type that a float32 factor is taken apart into where float32 results come from it (states that are handed over, gradients
-// of states and of decays): all 24 bits, 22 in fp16. Where only 16-bit results come from it the state is read in one term, whose rounding is like the
-// result's own, and what is added to it has two (with one, results were up to 1.6 times as far from 64 bits as rounded ones are, with two and two of the scores 1.3 times).
+// of states and of decays): all 24 bits, 22 in fp16. Where only 16-bit results come from it, two: 2^-17 of it is lost, and results are as far from 64 bits as ones that
+// are rounded once (with the state in one term they were 1.2 to 1.3 times as far, and outputs 141 us of [8, 4096, 16 x 128] in bf16 for 161, keys and values 401 for 418).
 template <typename ST> constexpr int kTerms = 3;
 template <> inline constexpr int kTerms<_Float16> = 2;
 template <> inline constexpr int kTerms<float> = 1;
@@ -729,9 +729,9 @@ template <typename ST, int W, int D, bool GRAD> struct AttendLds {
     static constexpr int C = Operand<ST>::CHUNK;
     static constexpr int WORDS = 3 * Tile<ST, D>::WORDS + Scores<ST>::WORDS + Decays<C>::WORDS + (GRAD ? W * C + 2 * W : 0);
 };
-template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> __global__ __launch_bounds__(64 * W, 2) void attend_kernel(AttendArgs args)
+template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ __launch_bounds__(64 * W, 2) void attend_kernel(AttendArgs args)
 {
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, NT = 64 * W, STEPS = C / KS, TT = C / 16, PER = KS / 16, TERMS = kTerms<ST>;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const scanscam_attend &a = args.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g = lane >> 4;
@@ -818,7 +818,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, int TERMS, bool EXACT> _
             scores.put(tt, st, p);
         }
         float4v acc[TT][JT];
-        const float factor = a.scale / S.template times<GRAD ? TERMS : 1>(X, inner, acc);
+        const float factor = a.scale / S.template times<GRAD ? TERMS : kTermsRounded<ST>>(X, inner, acc);
         if constexpr (GRAD)
             if (args.borders != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0)
                 S.keep(args.borders + border_at(args, span.batch, t0, C, span.head) * D * D, inner, outer);
@@ -1017,7 +1017,7 @@ template <typename ST, int D> struct BackLds {
 template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forceinline__ void back_pass(const AttendArgs &args, float *lds)
 {
     constexpr bool BOTH = attend_both<D>();
-    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * back_waves<D>(), STEPS = C / KS, TT = C / 16, PER = KS / 16, TERMS = KEYS ? kTerms<ST> : 1, TERMS_IN = KEYS ? kTerms<ST> : kTermsRounded<ST>;
+    constexpr int C = Operand<ST>::CHUNK, KS = Operand<ST>::KS, W = attend_waves<D>(), NT = 64 * back_waves<D>(), STEPS = C / KS, TT = C / 16, PER = KS / 16, TERMS = KEYS ? kTerms<ST> : kTermsRounded<ST>;
     const scanscam_attend &a = args.a;
     const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all % W, n16 = lane & 15, g = lane >> 4;
     float *at = lds;
@@ -1156,7 +1156,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                 if (g == 0) red[wave * C + s] = write;
             }
         }
-        H.template update<TERMS_IN>(update_rows, inner, own, decays.upto, a.scale, decays.whole());
+        H.template update<TERMS>(update_rows, inner, own, decays.upto, a.scale, decays.whole());
         if constexpr (KEYS) {
             const bool border = args.cross != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0;
             const int64_t at_border = border ? border_at(args, span.batch, t0, C, span.head) : 0;
@@ -1198,8 +1198,7 @@ template <typename ST, int D, int JK, int JV, bool EXACT> __global__ __launch_bo
 }
 
 // --- launches by type ---------------------------------------------------------------------------------------------------------------------
-// kOutputsRounded: no state is handed over.
-enum AttendPass { kOutputs, kOutputsRounded, kQueries, kKeysAndValues, kEnds, kBackEnds };
+enum AttendPass { kOutputs, kQueries, kKeysAndValues, kEnds, kBackEnds };
 
 // Channels that a call's tiles have room for.
 inline int attend_width(const scanscam_attend &a)
@@ -1228,21 +1227,18 @@ template <typename ST, int D, bool EXACT> hipError_t launch_attend_with(AttendPa
 {
     constexpr int WAVES = attend_waves<D>(), EJ = D == 256 ? 2 : 1, EW = D / 16 / EJ;  // (EJ, EW: of the ends, whole)
     // HALF: column tiles of a wave for a side that fills no more than half of them ([25, 656, 5 heads of 194 and 27] in bf16: 88 us, 198 with all).
-    constexpr int threads = 64 * WAVES, back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, HALF = 1, T = kTerms<ST>, R = kTermsRounded<ST>;
+    constexpr int threads = 64 * WAVES, back_threads = 64 * back_waves<D>(), ALL = D == 64 ? 1 : 2, HALF = 1, T = kTerms<ST>;
     constexpr int GW = query_waves<ST, D>(), GJ = D / 16 / GW;  // (of the queries' gradients, whole)
     constexpr int out = AttendLds<ST, WAVES, D, false>::WORDS, grad_half = AttendLds<ST, WAVES, D, true>::WORDS, grad = AttendLds<ST, GW, D, true>::WORDS, back = BackLds<ST, D>::WORDS, ends = EndsLds<ST, D>::WORDS;
     const bool k_half = ALL == 2 && args.a.K <= D / 2, v_half = ALL == 2 && args.a.V <= D / 2;
     const unsigned kinds = attend_both<D>() ? 1 : 2;
     switch (pass) {
     case kOutputs:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, false, T, EXACT>, out>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, ALL, WAVES, false, T, EXACT>, out>(units, 1, threads, stream, args);
-    case kOutputsRounded:
-        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, false, R, EXACT>, out>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, ALL, WAVES, false, R, EXACT>, out>(units, 1, threads, stream, args);
+        return v_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, false, EXACT>, out>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, ALL, WAVES, false, EXACT>, out>(units, 1, threads, stream, args);
     case kQueries:
-        return k_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, true, T, EXACT>, grad_half>(units, 1, threads, stream, args)
-                      : launch_attend_units<attend_kernel<ST, D, GJ, GW, true, T, EXACT>, grad>(units, 1, 64 * GW, stream, args);
+        return k_half ? launch_attend_units<attend_kernel<ST, D, HALF, WAVES, true, EXACT>, grad_half>(units, 1, threads, stream, args)
+                      : launch_attend_units<attend_kernel<ST, D, GJ, GW, true, EXACT>, grad>(units, 1, 64 * GW, stream, args);
     case kKeysAndValues:  // (both are not halves at once)
         if (k_half) return launch_attend_units<attend_back_kernel<ST, D, HALF, ALL, EXACT>, back>(units, kinds, back_threads, stream, args);
         if (v_half) return launch_attend_units<attend_back_kernel<ST, D, ALL, HALF, EXACT>, back>(units, kinds, back_threads, stream, args);

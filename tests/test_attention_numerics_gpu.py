@@ -1,0 +1,70 @@
+"""
+The attention's kernels where numbers are small, large, or of very different sizes: against the plain loops in float64 on the same stored inputs.
+
+Bounds. With A the sum of an output's products' absolute values (as in test_attention_gpu.py) and h half a unit in the last place of the activations' type, relative:
+  * a float32 factor of a product is taken apart into terms of the type, two at least: 2^-17 (bf16) or 2^-22 (fp16) of it is lost, at up to two places of a chain
+    of products (what is added to a state, and the state or the score that is read): TERMS A;
+  * in fp32 a product is rounded once for each addition on its way, at most K + V + C + 2 T of them and some 64 of exponentials and factors: (600 + 2 T) 2^-24 A;
+  * a result in 16 bits is rounded once: h |want|, in fp16 2^-25 at least (half of its smallest step).
+"""
+import math
+
+import pytest
+import torch
+
+import scanscam_amd as f
+from scanscam_amd import attention, baseline
+from test_attention_gpu import HALF, make, sizes, wide
+
+pytestmark = pytest.mark.gpu
+
+TERMS = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -21}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def call(attend, given, names, scale, gy=None, gs=None):
+    """(y, new state, gradients by name); ``gs`` None: no gradient of the new state."""
+    y, new = attend(**given, scale=scale, return_state=True)
+    if gy is None:
+        return y.detach(), new.detach(), {}
+    outs, weights = ([y], [gy]) if gs is None else ([y, new], [gy, gs])
+    grads = torch.autograd.grad(outs, [given[n] for n in names], weights, allow_unused=True)
+    return y.detach(), new.detach(), {n: torch.zeros_like(given[n]) if t is None else t for n, t in zip(names, grads)}
+
+
+def results(gpu, given, scale, gy=None, gs=None):
+    """The kernels' results, what is right, and A of each."""
+    names = [n for n, t in given.items() if t is not None and n != "offsets"]
+    out = []
+    for attend, of, weight in ((f.linear_attention, lambda t, n: t.to(gpu), lambda t: t.to(gpu)), (baseline.naive_linear_attention, lambda t, n: wide(t), wide),
+                               (baseline.naive_linear_attention, lambda t, n: sizes(wide(t), n), lambda t: wide(t).abs())):
+        own = {n: None if t is None else of(t, n).requires_grad_() if n in names and gy is not None else of(t, n) for n, t in given.items()}
+        out.append(call(attend, own, names, scale, None if gy is None else weight(gy), None if gs is None else weight(gs)))
+    return out
+
+
+def near(got, want, total, dtype, T, what):
+    """``total``: A."""
+    assert got.shape == want.shape and torch.isfinite(got).all(), what
+    half = HALF[got.dtype]
+    got, want, total = got.detach().cpu().double(), want.detach().cpu().double(), total.detach().cpu().double()
+    bound = 1.01 * half * want.abs() + ((600 + 2 * T) * 2.0 ** -24 + TERMS[dtype]) * total + (2.0 ** -25 if half == HALF[torch.float16] else 0.0)
+    over = (got - want).abs() - bound
+    at = int(over.argmax())
+    assert not (over > 0).any(), f"{what}: {float((got - want).abs().max()):.3e} off; at {at}: {float(got.flatten()[at])} for {float(want.flatten()[at])}, bound {float(bound.flatten()[at]):.3e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K,V,T,groups", [(64, 64, 300, 2), (128, 128, 200, 1), (128, 64, 130, 2), (256, 200, 100, 1), (33, 97, 140, 2)])
+@pytest.mark.parametrize("parts", [0, 2])
+def test_results_in_16_bits_are_rounded_once(gpu, monkeypatch, dtype, K, V, T, groups, parts):
+    """Whatever is asked for besides: outputs have the same bits with a state handed back, with gradients, and without either."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    v, scale = make(23, dtype, 2, T, 2, K, V, groups=groups, pace=0.02, state=True), K ** -0.5
+    gy = torch.randn(v["v"].shape, generator=torch.Generator().manual_seed(24)).to(dtype)
+    got, want, total = results(gpu, v, scale, gy)
+    near(got[0], want[0], total[0], dtype, T, "y")
+    for n in ("q", "k", "v"):
+        near(got[2][n], want[2][n], total[2][n], dtype, T, f"gradient of {n}")
+    alone = f.linear_attention(**{n: t if t is None else t.to(gpu) for n, t in v.items()}, scale=scale)
+    assert torch.equal(alone, got[0])

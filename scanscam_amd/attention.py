@@ -147,7 +147,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
         raise TypeError(f"{what}: state must be float32, got {state.dtype}")
     if v.device.type != "cuda":
         return baseline.naive_linear_attention(q, k, v, decay, scale=scale, state=state, offsets=offsets, return_state=return_state)
-    _check_sizes(what, heads * max(K, V), v.shape[0] * v.shape[1], sequences)
+    _check_sizes(what, max(heads * max(K, V), q.shape[2] * K), v.shape[0] * v.shape[1], sequences)
     if _needs_node(q, k, v, decay, state):
         y, new = LinearAttention.apply(q, k, v, decay, state, offsets, float(scale), bool(return_state))
     else:

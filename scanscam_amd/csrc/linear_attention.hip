@@ -72,21 +72,21 @@ template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(A
     }
 }
 
-// Gradients of shared queries or keys: over the heads that share them, in order.
+// Gradients of shared queries or keys: over the heads that share them, in order (of no heads they are zero).
 struct Shared {
-    const float *part;  // [tokens][heads][K]
+    const float *part;  // [tokens][groups * each][K]
     scanscam_tokens out;
     int64_t tokens, T, token0;
-    int32_t heads, each, K, dtype;
+    int32_t groups, each, K;
 };
 template <typename ST> __global__ __launch_bounds__(256) void shared_kernel(Shared a)
 {
-    const int fours = (a.K + 3) / 4, groups = a.heads / a.each, row = groups * fours;
+    const int fours = (a.K + 3) / 4, row = a.groups * fours;
     const int64_t index = (int64_t)blockIdx.x * 256 + threadIdx.x, token = a.token0 + index / row;
     if (token >= a.tokens) return;
     const int rest = (int)(index % row), group = rest / fours, at = rest % fours * 4, count = a.K - at;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const float *p = a.part + (token * a.heads + (int64_t)group * a.each) * a.K + at;
+    const float *p = a.part + (token * a.groups + group) * a.each * a.K + at;
     for (int h = 0; h < a.each; h++, p += a.K) {
         float f[4];
         load_part<float, 4>(p, count, f);
@@ -321,13 +321,24 @@ hipError_t starts(AttendArgs args, bool back, AttendPass pass, int64_t units, hi
 
 template <typename ST> hipError_t join_shared(Shared s, hipStream_t stream)
 {
-    const int64_t row = (int64_t)(s.heads / s.each) * ceil_div(s.K, 4), most = (int64_t(1) << 31) / row;
+    const int64_t row = (int64_t)s.groups * ceil_div(s.K, 4), most = (int64_t(1) << 31) / row;
     const int64_t all = s.tokens;
     hipError_t err = hipSuccess;
     for (; s.token0 < all && err == hipSuccess; s.token0 += most) {
         const int64_t now = all - s.token0 < most ? all - s.token0 : most;
         s.tokens = s.token0 + now;
         err = launch_op(shared_kernel<ST>, dim3((unsigned)ceil_div(now * row, 256)), dim3(256), 0, stream, s);
+    }
+    return err;
+}
+
+// Gradients of queries and keys out of the heads' (each: heads that share one).
+hipError_t join_both(const scanscam_attend &a, int32_t each, const float *part_q, const float *part_k, hipStream_t stream)
+{
+    hipError_t err = hipSuccess;
+    for (int i = 0; i < 2 && err == hipSuccess; i++) {
+        const Shared sum{i == 0 ? part_q : part_k, i == 0 ? a.gq : a.gk, a.batch * a.T, a.T, 0, (int32_t)a.groups, each, (int32_t)a.K};
+        err = a.dtype == SCANSCAM_F32 ? join_shared<float>(sum, stream) : a.dtype == SCANSCAM_BF16 ? join_shared<__bf16>(sum, stream) : join_shared<_Float16>(sum, stream);
     }
     return err;
 }
@@ -394,7 +405,12 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     SCANSCAM_CHECK(check_attend(a, true));
     if (a->gdecay != nullptr && a->decay.p == nullptr) return SCANSCAM_EINVAL;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (a->heads == 0) return SCANSCAM_OK;
+    if (a->heads == 0) {
+        if (a->batch * a->T == 0) return SCANSCAM_OK;
+        if (a->groups > kMostChannels / a->K) return SCANSCAM_EINVAL;
+        for (const scanscam_tokens *t : {&a->gq, &a->gk}) SCANSCAM_CHECK(check_tokens(*t, activation_size(a->dtype)));
+        return code(join_both(*a, 0, nullptr, nullptr, s));
+    }
     if (a->sequences == 0 || (a->batch * a->T == 0 && a->gstate_in == nullptr))
         return a->gdecay != nullptr && a->decay_fixed ? code(column_sum({nullptr, 0, 0, {a->gdecay}, {a->heads}}, s)) : SCANSCAM_OK;
     const Plan plan = plan_of(*a);
@@ -443,12 +459,7 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
         }
         if (a->decay_fixed && err == hipSuccess) err = column_sum({args.decays, args.tokens, a->heads, {a->gdecay}, {a->heads}}, s);
     }
-    if (args.each > 1 && err == hipSuccess) {
-        for (int i = 0; i < 2 && err == hipSuccess; i++) {
-            const Shared sum{i == 0 ? args.part_q : args.part_k, i == 0 ? a->gq : a->gk, args.tokens, a->T, 0, (int32_t)a->heads, args.each, (int32_t)a->K, a->dtype};
-            err = a->dtype == SCANSCAM_F32 ? join_shared<float>(sum, s) : a->dtype == SCANSCAM_BF16 ? join_shared<__bf16>(sum, s) : join_shared<_Float16>(sum, s);
-        }
-    }
+    if (args.each > 1 && err == hipSuccess) err = join_both(*a, args.each, args.part_q, args.part_k, s);
     return code(err);
 }
 

@@ -126,7 +126,6 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
     :param return_state: hand back the states after the last tokens as well, in float32
     :return: y, [batch, T, heads, V], or ``(y, state)``. Differentiable in every tensor but ``offsets``. Products are taken in the activations'
         type and added up in float32; what float32 results come from (states, gradients of states and float32 decays) is not rounded to 16 bits.
-        In float16 the scaled and decayed product of a query and a key (backwards also of a gradient and a value) has to be below 65504 to be finite.
         Values that are not finite reach the tokens after them and nothing before them; in gradients they may also reach the neighbouring 63 tokens
         of their own head and sequence, and the decays before them.
     """

@@ -27,7 +27,7 @@
 //
 // What bounds it: neither memory nor the matrix unit, but the chain of a chunk (loads to LDS, scores, a barrier, sums, the state's update, a barrier) in few waves,
 // for a state's columns and a chunk's operands leave registers for two waves a SIMD. [8, 4096, 16 x 128] in bf16, in four parts: ends of parts 60 us, outputs
-// 161 (of 537 MB, 3.3 TB/s), ends backwards 72, gradients of queries 267, of keys and values 418, decays 10.
+// 153 (of 537 MB, 3.5 TB/s), ends backwards 72, gradients of queries 259, of keys and values 401, decays 10.
 // In counters the matrix unit is busy for a fifth of these, the vector unit (terms, decays, addresses) for a third.
 #pragma once
 
@@ -83,7 +83,7 @@ __device__ __forceinline__ float4v mma(const float4v &a, const float4v &b, float
 
 // Terms of the activations' type that a float32 factor is taken apart into where float32 results come from it (states that are handed over, gradients
 // of states and of decays): all 24 bits, 22 in fp16. Where only 16-bit results come from it, two: 2^-17 of it is lost, and results are as far from 64 bits as ones that
-// are rounded once (with the state in one term they were 1.2 to 1.3 times as far, and outputs 141 us of [8, 4096, 16 x 128] in bf16 for 161, keys and values 401 for 418).
+// are rounded once (with the state in one term they were 1.2 to 1.3 times as far, and outputs 141 us of [8, 4096, 16 x 128] in bf16 for 161).
 template <typename ST> constexpr int kTerms = 3;
 template <> inline constexpr int kTerms<_Float16> = 2;
 template <> inline constexpr int kTerms<float> = 1;
@@ -454,6 +454,14 @@ __device__ __forceinline__ int later(int v)
     return v;
 }
 
+// The same for one of the wave. (With heads over 128 channels a wave has one unit of scores at most, whose addresses would be made before the loop and lie in memory:
+// [4, 4096, 8 x 256 x 256] in bf16 380 us for outputs and 1018 for gradients of keys and values, 295 and 804 so.)
+__device__ __forceinline__ int later_uniform(int v)
+{
+    asm volatile("" : "+s"(v));
+    return v;
+}
+
 // A wave's columns of a state: all rows, in accumulators. Column tile jt of wave w is the state's tile jt * WAVES + w. Products go over the rows that
 // there are, 64 at a time.
 template <typename ST, int D, int JT, int WAVES> struct State {
@@ -670,10 +678,14 @@ __device__ __forceinline__ int64_t border_at(const AttendArgs &args, int64_t bat
 
 // The scores of a chunk in LDS, as operands: [term][tile of 16 columns][step of KS rows][lane] of 16 bytes each. In 16 bits they have two terms:
 // the rounding of one is that of every result which it is the largest factor of, once more than the result's own.
+// In fp16 a token's scores of a step are multiplied with a power of two that brings the largest of them to 2^14, as states are, and sums of products with them by its
+// inverse: scores below 2^-14 would be rounded in steps of 2^-24 otherwise, and lost below 2^-25 (queries and keys of 3e-4: outputs 19 % off), and past 65504 infinite.
 template <typename ST> struct Scores {
-    static constexpr int KS = Operand<ST>::KS, PER = KS / 16, C = Operand<ST>::CHUNK, STEPS = C / KS, TERMS = sizeof(ST) == 2 ? 2 : 1, ONE = C / 16 * STEPS * 64;
-    static constexpr int WORDS = TERMS * ONE * 4;
+    static constexpr bool SCALED = std::is_same_v<ST, _Float16>;
+    static constexpr int KS = Operand<ST>::KS, PER = KS / 16, C = Operand<ST>::CHUNK, TT = C / 16, STEPS = C / KS, TERMS = sizeof(ST) == 2 ? 2 : 1, ONE = TT * STEPS * 64;
+    static constexpr int SCALES = SCALED ? STEPS * C : 0, WORDS = TERMS * ONE * 4 + SCALES, UNITS = STEPS * (TT + PER) / 2;
     frag_t<ST> *p;
+    __device__ __forceinline__ float *unscale(int step) const { return reinterpret_cast<float *>(p + TERMS * ONE) + step * C; }
     __device__ __forceinline__ frag_t<ST> operand(int tile, int step, int term) const { return p[term * ONE + (tile * STEPS + step) * 64 + (threadIdx.x & 63)]; }
     // A 16 x 16 tile of rows row_tile * 16 ... and columns tile * 16 ...
     __device__ __forceinline__ void put(int tile, int row_tile, float4v v) const
@@ -693,21 +705,63 @@ template <typename ST> struct Scores {
     __device__ __forceinline__ float at(int row, int column) const
     {
         const ST *e = reinterpret_cast<const ST *>(p + (column / 16 * STEPS + row / KS) * 64 + row % 16 / 4 * 16 + column % 16) + row % KS / 16 * 4 + row % 4;
-        const float most = (float)*e;
-        return TERMS == 2 && __builtin_isfinite(most) ? most + (float)e[ONE * (16 / sizeof(ST))] : most;
+        const float most = (float)*e, back = SCALED ? unscale(row / KS)[column] : 1.0f;
+        return (TERMS == 2 && __builtin_isfinite(most) ? most + (float)e[ONE * (16 / sizeof(ST))] : most) * back;
     }
-    // Tiles beyond the diagonal that operands reach are zeros, and nobody writes them.
-    __device__ __forceinline__ void clear() const
+    // The scores of a step's PER row tiles by 16 columns (zeros beyond the diagonal), which lie lane by lane: lane 16 g + n has four rows of column n.
+    __device__ __forceinline__ void put_step(int tile, int step, float4v (&v)[PER]) const
     {
-        for (int i = threadIdx.x; i < TERMS * ONE; i += blockDim.x) reinterpret_cast<raw16 *>(p)[i] = raw16{0, 0, 0, 0};
+        if constexpr (SCALED) {
+            float most = 0.0f;
+#pragma unroll
+            for (int h = 0; h < PER; h++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float x = __builtin_fabsf(v[h][r]);
+                    most = __builtin_fmaxf(most, x < __builtin_inff() ? x : 0.0f);  // (what is not finite is no measure for the others)
+                }
+            most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+            most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+            const int up = most > 1e-30f ? 14 + 127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23) : 0;
+            const float factor = __builtin_bit_cast(float, (uint32_t)(127 + up) << 23);
+#pragma unroll
+            for (int h = 0; h < PER; h++) v[h] *= factor;
+            if ((threadIdx.x & 63) < 16) unscale(step)[tile * 16 + (threadIdx.x & 63)] = __builtin_bit_cast(float, (uint32_t)(127 - up) << 23);
+        }
+#pragma unroll
+        for (int h = 0; h < PER; h++) put(tile, step * PER + h, v[h]);
+    }
+    // sum += (rows of `own`) x (tile's column of scores), over a step.
+    template <int JT> __device__ __forceinline__ void times(const frag_t<ST> (&own)[JT][STEPS], int tile, int step, float4v (&sum)[JT]) const
+    {
+        float4v part[JT];
+#pragma unroll
+        for (int jt = 0; jt < JT; jt++) part[jt] = SCALED ? float4v{0, 0, 0, 0} : sum[jt];
+#pragma unroll
+        for (int term = TERMS; term-- > 0;) {
+            const frag_t<ST> f = operand(tile, step, term);
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++) part[jt] = mma(own[jt][step], f, part[jt]);
+        }
+        const float back = SCALED ? unscale(step)[tile * 16 + (threadIdx.x & 15)] : 1.0f;
+#pragma unroll
+        for (int jt = 0; jt < JT; jt++) sum[jt] = SCALED ? sum[jt] + part[jt] * back : part[jt];
     }
 };
 
-// The id-th pair (i, j) with j <= i.
-__device__ __forceinline__ void pair_of(int id, int &i, int &j)
+// The id-th column tile and step of scores that products reach: those of PER row tiles first, so that waves which take two take a whole one and one of a single tile.
+// (Row tiles up to the diagonal; for those from it on both count from the other end.)
+template <typename ST> __device__ __forceinline__ void unit_of(int id, int &tile, int &step)
 {
-    i = id < 1 ? 0 : id < 3 ? 1 : id < 6 ? 2 : 3;
-    j = id - i * (i + 1) / 2;
+    if constexpr (Operand<ST>::KS / 16 == 2) {
+        static_assert(Operand<ST>::CHUNK == 64, "four column tiles of two steps");
+        tile = id < 2 ? 3 : id == 2 ? 2 : id == 3 ? 1 : id == 4 ? 2 : 0;
+        step = id == 1 || id == 4 ? 1 : 0;
+    } else {
+        static_assert(Operand<ST>::CHUNK == 32, "two column tiles of two steps");
+        tile = id < 2 ? 1 : 0;
+        step = id == 1 ? 1 : 0;
+    }
 }
 
 // Four neighbouring values of a token's output. EXACT: `cols` is a multiple of four.
@@ -762,7 +816,6 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
     State<ST, D, JT, W> S;
     S.wave = wave;
     S.read(start_of(args, span, false), inner, outer, row_step, col_step);
-    scores.clear();
 
     Staged<ST, D, NT, EXACT> sx(x, xt.token, inner), sy(y, yt.token, inner), sz(z, zt.token, outer);
     uint32_t decay = 0;
@@ -805,17 +858,24 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
         if (t0 + C < span.end) ask(t0 + C);
 
         // Scores: tiles of 16 tokens s (rows) by 16 tokens t (columns), t >= s. (The first wave, which has the decays, is not among those with one more.)
-        for (int id = (wave + 2) % W; id < TT * (TT + 1) / 2; id += W) {
-            int tt, st;
-            pair_of(id, tt, st);
-            float4v p = score(Y, st * 16, X, tt * 16, inner);
+        for (int id = D == 256 ? later_uniform((wave + 2) % W) : (wave + 2) % W; id < Scores<ST>::UNITS; id += W) {
+            int tt, step;
+            unit_of<ST>(id, tt, step);
             const double upto = decays.sums[tt * 16 + n16];
+            float4v p[PER];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int s = st * 16 + 4 * g + r, t = tt * 16 + n16;
-                p[r] = s <= t ? p[r] * (exp2_(upto - decays.sums[s]) * a.scale) : 0.0f;
+            for (int h = 0; h < PER; h++) {
+                const int st = step * PER + h;
+                p[h] = float4v{0, 0, 0, 0};
+                if (st > tt) continue;
+                p[h] = score(Y, st * 16, X, tt * 16, inner);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int s = st * 16 + 4 * g + r, t = tt * 16 + n16;
+                    p[h][r] = s <= t ? p[h][r] * (exp2_(upto - decays.sums[s]) * a.scale) : 0.0f;
+                }
             }
-            scores.put(tt, st, p);
+            scores.put_step(tt, step, p);
         }
         float4v acc[TT][JT];
         const float factor = a.scale / S.template times<GRAD ? TERMS : kTermsRounded<ST>>(X, inner, acc);
@@ -856,14 +916,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
                 sum[jt] = acc[tt][jt];
             }
 #pragma unroll
-            for (int step = 0; step <= tt / PER; step++) {
-#pragma unroll
-                for (int term = Scores<ST>::TERMS; term-- > 0;) {
-                    const frag_t<ST> p = scores.operand(tt, step, term);
-#pragma unroll
-                    for (int jt = 0; jt < JT; jt++) sum[jt] = mma(own[jt][step], p, sum[jt]);
-                }
-            }
+            for (int step = 0; step <= tt / PER; step++) scores.times(own, tt, step, sum);
             if constexpr (!GRAD) {
 #pragma unroll
                 for (int jt = 0; jt < JT; jt++)
@@ -872,9 +925,21 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
                 if (__builtin_expect(__ballot(finite != 0.0f) != 0, 0)) {
                     // A value that is not finite may be a later token's, times a score of zero. Where the tokens up to t alone give a finite sum it is the product's
                     // without such values, in the same order as ever.
+                    float4v clean[JT];
+#pragma unroll
+                    for (int jt = 0; jt < JT; jt++) clean[jt] = acc[tt][jt];
+#pragma unroll
+                    for (int step = 0; step <= tt / PER; step++) {
+                        frag_t<ST> values[JT][STEPS];
+#pragma unroll
+                        for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                            for (int e = 0; e < 4 * PER; e++) values[jt][step][e] = __builtin_isfinite((float)own[jt][step][e]) ? own[jt][step][e] : (ST)0.0f;
+                        scores.times(values, tt, step, clean);
+                    }
 #pragma unroll
                     for (int jt = 0; jt < JT; jt++) {
-                        float4v alone = acc[tt][jt], clean = acc[tt][jt];
+                        float4v alone = acc[tt][jt];
                         for (int s = 0; s <= t; s++) {
                             float value[4];
                             Z.four(s, S.column(jt) + 4 * g, value);
@@ -883,15 +948,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
                             for (int r = 0; r < 4; r++) alone[r] += p * value[r];
                         }
 #pragma unroll
-                        for (int step = 0; step <= tt / PER; step++) {
-                            frag_t<ST> values = own[jt][step];
-#pragma unroll
-                            for (int e = 0; e < 4 * PER; e++) values[e] = __builtin_isfinite((float)values[e]) ? values[e] : (ST)0.0f;
-#pragma unroll
-                            for (int term = Scores<ST>::TERMS; term-- > 0;) clean = mma(values, scores.operand(tt, step, term), clean);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; r++) sum[jt][r] = __builtin_isfinite(alone[r]) ? clean[r] : alone[r];
+                        for (int r = 0; r < 4; r++) sum[jt][r] = __builtin_isfinite(alone[r]) ? clean[jt][r] : alone[r];
                     }
                     settle();
                 }
@@ -1047,8 +1104,6 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
     State<ST, D, JT, W> H;
     H.wave = wave;
     H.read(start_of(args, span, true), inner, outer, row_step, col_step);
-    of_keys.clear();
-    if constexpr (BOTH) of_values.clear();
 
     Staged<ST, D, NT, EXACT> sq(q, a.q.token, K), sk(k, a.k.token, K), sv(v, a.v.token, V), so(o, a.gy.token, V);
     uint32_t decay = 0;
@@ -1076,32 +1131,40 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
 
         // Scores: tiles of 16 tokens t (rows) by 16 tokens s (columns), t >= s, and of both M.
         if (!BOTH || !KEYS) {
-            for (int id = (wave + 2) % W; id < TT * (TT + 1) / 2; id += W) {
-                int tt, st;
-                pair_of(id, tt, st);
-                float4v p{0, 0, 0, 0}, other{0, 0, 0, 0};
-                if (BOTH || KEYS) p = score(O, tt * 16, Vt, st * 16, V);
-                other = score(Q, tt * 16, Kt, st * 16, K);
+            for (int id = D == 256 ? later_uniform((wave + 2) % W) : (wave + 2) % W; id < Scores<ST>::UNITS; id += W) {
+                int st, step;
+                unit_of<ST>(id, st, step);
+                st = TT - 1 - st;
+                step = STEPS - 1 - step;
                 const double from_s = decays.sums[st * 16 + n16];
-                float over_t = 0.0f;
+                float4v p[PER], other[PER];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int s = st * 16 + n16, t = tt * 16 + 4 * g + r;
-                    const float w = exp2_(decays.sums[t] - from_s) * a.scale;
-                    if (BOTH || KEYS) {
-                        const float m = s < t ? p[r] * other[r] * w : 0.0f, over_s = row_sum(m);
-                        over_t += m;
-                        if (n16 == 15) rows[st * C + t] = over_s;
+                for (int h = 0; h < PER; h++) {
+                    const int tt = step * PER + h;
+                    p[h] = other[h] = float4v{0, 0, 0, 0};
+                    if (tt < st) continue;
+                        if (BOTH || KEYS) p[h] = score(O, tt * 16, Vt, st * 16, V);
+                    other[h] = score(Q, tt * 16, Kt, st * 16, K);
+                    float over_t = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int s = st * 16 + n16, t = tt * 16 + 4 * g + r;
+                        const float w = exp2_(decays.sums[t] - from_s) * a.scale;
+                        if (BOTH || KEYS) {
+                            const float m = s < t ? p[h][r] * other[h][r] * w : 0.0f, over_s = row_sum(m);
+                            over_t += m;
+                            if (n16 == 15) rows[st * C + t] = over_s;
+                        }
+                        p[h][r] = s <= t ? p[h][r] * w : 0.0f;
+                        other[h][r] = s <= t ? other[h][r] * w : 0.0f;
                     }
-                    p[r] = s <= t ? p[r] * w : 0.0f;
-                    other[r] = s <= t ? other[r] * w : 0.0f;
+                    if (BOTH || KEYS) {
+                        over_t = column_sum4(over_t);
+                        if (g == 0) cols[tt * C + st * 16 + n16] = over_t;
+                    }
                 }
-                if (BOTH || KEYS) {
-                    over_t = column_sum4(over_t);
-                    if (g == 0) cols[tt * C + st * 16 + n16] = over_t;
-                    of_keys.put(st, tt, p);
-                }
-                if (BOTH || !KEYS) of_values.put(st, tt, other);
+                if (BOTH || KEYS) of_keys.put_step(st, step, p);
+                if (BOTH || !KEYS) of_values.put_step(st, step, other);
             }
         }
         float4v acc[TT][JT];
@@ -1129,14 +1192,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                 }
             }
 #pragma unroll
-            for (int step = st / PER; step < STEPS; step++) {
-#pragma unroll
-                for (int term = Scores<ST>::TERMS; term-- > 0;) {
-                    const frag_t<ST> p = scores.operand(st, step, term);
-#pragma unroll
-                    for (int jt = 0; jt < JT; jt++) acc[st][jt] = mma(own[jt][step], p, acc[st][jt]);
-                }
-            }
+            for (int step = st / PER; step < STEPS; step++) scores.times(own, st, step, acc[st]);
             if (s < n) {
                 const int64_t row = out_lane + (t0 + st * 16) * out_step;
 #pragma unroll

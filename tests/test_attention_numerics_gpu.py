@@ -68,3 +68,22 @@ def test_results_in_16_bits_are_rounded_once(gpu, monkeypatch, dtype, K, V, T, g
         near(got[2][n], want[2][n], total[2][n], dtype, T, f"gradient of {n}")
     alone = f.linear_attention(**{n: t if t is None else t.to(gpu) for n, t in v.items()}, scale=scale)
     assert torch.equal(alone, got[0])
+
+
+
+@pytest.mark.parametrize("qk,vs,gs", [(1e-3, 100.0, 1.0), (3e-4, 1000.0, 0.1), (1e-4, 6000.0, 0.01), (1.0, 1.0, 1e-5), (1.0, 1.0, 1e-6), (40.0, 10.0, 1e-3)])
+@pytest.mark.parametrize("K,V,T,parts", [(128, 128, 64, 0), (64, 48, 150, 2), (200, 256, 70, 0)])
+def test_products_of_small_and_large_values_in_fp16(gpu, monkeypatch, qk, vs, gs, K, V, T, parts):
+    """Products of queries and keys, or of gradients and values, far below fp16's smallest steps, or past its largest value, where results are neither."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    v, scale = make(21, torch.float16, 1, T, 2, K, V, groups=1, pace=0.02), 1.0 if qk < 1 else K ** -0.5
+    v["q"], v["k"], v["v"] = (v["q"].float() * qk).half(), (v["k"].float() * qk).half(), (v["v"].float() * vs).half()
+    if qk > 1:
+        scale = 1e-3  # (products of 40 x 40 x 128 are more than fp16 holds; what comes of them is not)
+        v["q"] *= 4
+    gy = (torch.randn(v["v"].shape, generator=torch.Generator().manual_seed(22)) * gs).half()
+    got, want, total = results(gpu, v, scale, gy)
+    near(got[0], want[0], total[0], torch.float16, T, "y")
+    near(got[1], want[1], total[1], torch.float16, T, "state")
+    for n in ("q", "k", "v"):
+        near(got[2][n], want[2][n], total[2][n], torch.float16, T, f"gradient of {n}")

@@ -534,23 +534,26 @@ template <typename ST, int D, int JT, int WAVES> struct State {
                 }
         return sum;
     }
+    // The wave's largest absolute value, or finite one.
+    __device__ __forceinline__ float largest(bool finite) const
+    {
+        float most = 0.0f;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int jt = 0; jt < JT; jt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float v = __builtin_fabsf(s[rt][jt][r]);
+                    most = __builtin_fmaxf(most, finite && !(v < __builtin_inff()) ? 0.0f : v);
+                }
+        return most_of(most);
+    }
     // The power of two that the state is multiplied with in operands.
     __device__ __forceinline__ float scale() const
     {
         if constexpr (!std::is_same_v<ST, _Float16>) return 1.0f;
-        return scale_to_fp16([&](bool finite) {
-            float most = 0.0f;
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                for (int jt = 0; jt < JT; jt++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float v = __builtin_fabsf(s[rt][jt][r]);
-                        most = __builtin_fmaxf(most, finite && !(v < __builtin_inff()) ? 0.0f : v);
-                    }
-            return most_of(most);
-        });
+        return scale_to_fp16([&](bool finite) { return largest(finite); });
     }
     // acc[tt][jt], columns: rows of `of` (tokens), rows: the state's columns: the state's product with them, times the power of two that is returned.
     template <int TERMS> __device__ __forceinline__ float times(Tile<ST, D> of, int rows, float4v (&acc)[C / 16][JT]) const
@@ -611,7 +614,13 @@ template <typename ST, int D, int JT, int WAVES> struct State {
                     }
                 return most_of(most);
             });
-            bring = bring < 1048576.0f ? bring : 1048576.0f;  // (the state is multiplied with it as well)
+            // The state is multiplied with it as well, and must stay finite.
+            const float all = largest(false), most = (all < __builtin_inff() ? all : largest(true)) * decay;
+            bring = bring < 1048576.0f ? bring : 1048576.0f;
+            if (__builtin_expect(!(most < 0x1p105f), 0)) {
+                const float room = most < __builtin_inff() ? __builtin_ldexpf(1.0f, 126 + 127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23)) : 1.0f;
+                bring = bring < room ? bring : room;
+            }
             factor *= bring;
         }
 #pragma unroll

@@ -87,3 +87,27 @@ def test_products_of_small_and_large_values_in_fp16(gpu, monkeypatch, qk, vs, gs
     near(got[1], want[1], total[1], torch.float16, T, "state")
     for n in ("q", "k", "v"):
         near(got[2][n], want[2][n], total[2][n], torch.float16, T, f"gradient of {n}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("parts", [0, 2])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -6])
+def test_states_grow_as_far_as_float32_holds_them(gpu, monkeypatch, dtype, parts, size):
+    """Decays above zero: states of some 1e36, and gradients of states as large, to which tokens before and after add as little as ever."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    T = 200
+    v = make(25, dtype, 1, T, 2, 48, 64, state=True)
+    v["v"], v["q"] = (v["v"].float() * size).to(dtype), (v["q"].float() * size).to(dtype)
+    v["decay"] = torch.zeros(1, T, 2)
+    v["decay"][:, 65:135] = 83.0 / 70
+    g = torch.Generator().manual_seed(26)
+    gy, gs = torch.randn(v["v"].shape, generator=g).to(dtype), torch.randn(v["state"].shape, generator=g)
+    found = []
+    for attend, of, weight in ((f.linear_attention, lambda t, n: t.to(gpu), lambda t: t.to(gpu)), (baseline.naive_linear_attention, lambda t, n: wide(t), wide),
+                               (baseline.naive_linear_attention, lambda t, n: sizes(wide(t), n), lambda t: wide(t).abs())):
+        given = {n: t if t is None else of(t, n).requires_grad_(n == "state") for n, t in v.items()}
+        y, new = attend(**given, return_state=True)  # (what queries read of it is more than fp16 holds)
+        found.append((new.detach(), *torch.autograd.grad((y, new), given["state"], (weight(gy), weight(gs)))))
+    for got, want, total, what in zip(*found, ("state", "gradient of the state")):
+        assert want.abs().max() > 1e36
+        near(got, want, total, dtype, T, what)

@@ -25,7 +25,7 @@ extern "C" {
  * heads / groups neighbouring heads of v each; q, k are [batch, T, groups, K], v, y [batch, T, heads, V], K and V 1 ... 256.
  * decay: logs of the decays, [batch, T, heads] of type `decay_dtype`, unit-stride along the heads (`group` is not looked at), or
  * [heads] where `decay_fixed` is set (strides 0), or NULL (no decay). -infinity forgets everything. Logs above 0 let states
- * grow, as far as fp32 holds them.
+ * grow, as far as fp32 holds them and the exponential of what the logs of any 64 neighbouring tokens sum up to.
  *
  * `saved`: for a backward call, the states that its parts of time start from (scanscam_attend_saved_bytes, which may be 0). The
  * workspace (scanscam_attend_workspace_bytes) is for calls that share the time of a sequence out over

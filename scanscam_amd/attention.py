@@ -120,7 +120,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
     :param q, k: [batch, T, groups, K], shared by heads / groups neighbouring heads each; 1 to 256 channels
     :param v: [batch, T, heads, V], 1 to 256 channels
     :param decay: logs of the decays, [batch, T, heads], or [heads] for one of each head, of any of the three types; none without. They are
-        meant to be 0 at most (-infinity forgets everything); above, states grow as far as float32 holds them.
+        meant to be 0 at most (-infinity forgets everything); above, states grow as far as float32 holds them, and what the logs of any
+        64 neighbouring tokens sum up to has to be 80 at most: where float32 does not hold its exponential results are not finite.
     :param state: [sequences, heads, K, V] in float32, the states before the first tokens (zeros if not given)
     :param offsets: the first token of each of several packed sequences, and the end
     :param return_state: hand back the states after the last tokens as well, in float32

@@ -27,10 +27,13 @@ template <int AHEAD, int VALUES, bool BACK> __global__ __launch_bounds__(256) vo
     for (int v = 0; v < VALUES; v++) run[v] = given != nullptr && at + 256 * v < values ? given[pair * values + at + 256 * v] : 0.0f;
     for (int i0 = 0; i0 < borders; i0 += AHEAD) {
         float adds[AHEAD][VALUES], decay[AHEAD];
+        int power[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const int there = i0 + i < borders ? i0 + i : borders - 1;
-            decay[i] = exp2_(logs[border(there)]);
+            const double log = logs[border(there)], whole = __builtin_floor(log < -4096.0 ? -4096.0 : log > 4096.0 ? 4096.0 : log);
+            power[i] = (int)whole;  // (a power past float32's, where decays are above zero: the state may be small, or zero)
+            decay[i] = exp2_(log < -4096.0 || log > 4096.0 ? 0.0 : log - whole);
 #pragma unroll
             for (int v = 0; v < VALUES; v++) adds[i][v] = at + 256 * v < values ? ends[border(there) * values + 256 * v] : 0.0f;
         }
@@ -39,7 +42,7 @@ template <int AHEAD, int VALUES, bool BACK> __global__ __launch_bounds__(256) vo
             if (i0 + i < borders) {
 #pragma unroll
                 for (int v = 0; v < VALUES; v++) {
-                    run[v] = run[v] * decay[i] + adds[i][v];
+                    run[v] = __builtin_ldexpf(run[v] * decay[i], power[i]) + adds[i][v];
                     if (at + 256 * v < values) ends[border(i0 + i) * values + 256 * v] = run[v];
                 }
             }

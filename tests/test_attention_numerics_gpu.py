@@ -111,3 +111,27 @@ def test_states_grow_as_far_as_float32_holds_them(gpu, monkeypatch, dtype, parts
     for got, want, total, what in zip(*found, ("state", "gradient of the state")):
         assert want.abs().max() > 1e36
         near(got, want, total, dtype, T, what)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("parts", [0, 2, 3])
+def test_decays_of_a_part_grow_past_float32_where_states_do_not(gpu, monkeypatch, dtype, parts):
+    """Over hundreds of tokens decays may grow by more than float32 holds: a state of zero, and a gradient of zero, stay what they are."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    T = 900
+    v = make(27, dtype, 1, T, 2, 40, 24)
+    v["decay"] *= 0.01
+    v["decay"][:, :256] = 0.5  # e^128 in 256 tokens that add nothing
+    v["k"][:, :256] = 0
+    got, want, total = results(gpu, v, 0.2)
+    near(got[0], want[0], total[0], dtype, T, "y")
+    near(got[1], want[1], total[1], dtype, T, "state")
+    v = make(28, dtype, 1, T, 2, 40, 24)
+    v["decay"] *= 0.01
+    v["decay"][:, 640:] = 0.5  # and in as many that are not read, of a state that is zero
+    v["decay"][:, 639] = -math.inf
+    v["k"][:, 639:] = v["q"][:, 639:] = 0
+    gy = torch.randn(v["v"].shape, generator=torch.Generator().manual_seed(29)).to(dtype)
+    got, want, total = results(gpu, v, 0.2, gy)
+    for n in ("q", "k", "v"):
+        near(got[2][n], want[2][n], total[2][n], dtype, T, f"gradient of {n}")

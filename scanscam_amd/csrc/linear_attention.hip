@@ -59,18 +59,26 @@ template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(A
     Span span;
     if (!span_of(whole, args.first + blockIdx.x, C, span)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __shared__ double over[kBorder];
+    __shared__ double all_reads[kBorder], all_writes[kBorder];
+    __shared__ bool closed[kBorder];
     const int64_t chunks = (span.length + C - 1) / C, base = span.head * args.tokens + span.batch * a.T;
     for (int64_t first = (int64_t)blockIdx.y * kBorder; first < chunks; first += (int64_t)gridDim.y * kBorder) {
         const int64_t c = first + kBorder - 1 - wave, t = span.begin + c * C + lane;
         const bool there = lane < C && t < span.end;
-        const double read = there ? (double)args.reads[base + t] + (double)args.inside[base + t] : 0.0, write = there ? args.writes[base + t] : 0.0;
-        const double reads = sums_upto(read), writes = sums_upto(write), all_reads = read_lane(reads, 63), all_writes = read_lane(writes, 63);
-        if (lane == 0) over[wave] = all_reads - all_writes;
+        const double read = there ? args.reads[base + t] : 0.0, write = there ? args.writes[base + t] : 0.0, pair = there ? args.inside[base + t] : 0.0;
+        const double reads = sums_upto(read), writes = sums_upto(write), pairs = sums_upto(pair), all_pairs = read_lane(pairs, 63), decay = read_lane(sums_upto(decay_of(a, decay_at(a, span, t, there))), 63);
+        if (lane == 63) {
+            all_reads[wave] = reads;
+            all_writes[wave] = writes;
+            closed[wave] = exp2_(decay) == 0.0f;  // (as for the states: nothing passes the chunk)
+        }
         __syncthreads();
         double end = first + kBorder < chunks ? args.cross[border_at(args, span.batch, span.from + (first + kBorder) * C, C, span.head)] : args.last[args.first + blockIdx.x];
-        for (int w = 0; w < wave; w++) end += over[w];
-        if (there) args.decays[(span.batch * a.T + t) * a.heads + span.head] = (float)((end - all_writes) + (all_reads - reads + read) + (writes - write));
+        for (int w = 0; w < wave; w++) end = (closed[w] ? 0.0 : end - all_writes[w]) + all_reads[w];
+        const double past = closed[wave] ? 0.0 : end - all_writes[wave];
+        if (there)
+            args.decays[(span.batch * a.T + t) * a.heads + span.head] =
+                (float)(past + (all_reads[wave] - reads + read) + (writes - write) + (all_pairs - pairs + pair));
         __syncthreads();
     }
 }
@@ -279,7 +287,7 @@ Pieces pieces_of(const scanscam_attend &a, bool back, const Plan &plan)
     p.back_ends = take(true, values, 4);
     p.reads = take(true, tokens * a.heads, 4);
     p.writes = take(true, tokens * a.heads, 4);
-    p.inside = take(true, tokens * a.heads, 4);
+    p.inside = take(true, tokens * a.heads, 8);
     p.last = take(true, pairs, 8);
     p.most_borders = a.T / (kBorder * chunk_of(a)) + 1;
     const int64_t borders = a.T > kBorder * chunk_of(a) ? a.batch * p.most_borders * a.heads : 0, width = attend_width(a);
@@ -435,7 +443,7 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     if (a->gdecay != nullptr) {
         args.reads = reinterpret_cast<float *>(w + at.reads);
         args.writes = reinterpret_cast<float *>(w + at.writes);
-        args.inside = reinterpret_cast<float *>(w + at.inside);
+        args.inside = reinterpret_cast<double *>(w + at.inside);
         args.last = reinterpret_cast<double *>(w + at.last);
         args.most_borders = at.most_borders;
         if (at.cross > at.borders) {  // (some sequence may have one)

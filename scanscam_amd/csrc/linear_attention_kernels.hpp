@@ -10,13 +10,15 @@
 //   S'   = e^G[end] S + sum over s of e^(G[end]-G[s]) k[s] v[s]^T.
 // dq is the same with (do, v, k) in place of (q, k, v), dk and dv the same backwards in time with (v, do, q) and (k, q, do).
 //
-// The gradient of a decay is summed up from what passes it, never from differences of what does not: inside of a chunk the pairs
-// s < t, M[t,s] = e^(G[t]-G[s]) (q[t] k[s]) (do[t] v[s]), in fp32; across its borders R[t] = q[t] (what dq[t] takes from S) and
+// The gradient of a decay is summed up from what passes it: inside of a chunk the pairs
+// s < t, M[t,s] = e^(G[t]-G[s]) (q[t] k[s]) (do[t] v[s]); across its borders R[t] = q[t] (what dq[t] takes from S) and
 // W[s] = k[s] (what dk[s] takes from H). With X[c] = e^G[end] <H, S>, which passes the whole chunk,
 //   dg[t] = X[c] + sum over u >= t of R[u] + sum over s < t of W[s] + sum over s < t <= u of M[u,s],
 //   X[c] + sum of W = X[c+1] + sum of the next chunk's R  (both are the product of state and gradient at the border),
-// so that X follows from a border on without either state. What the sums' roundings leave in it grows with the chunks: at every eighth border the
-// pass over queries stores its state, and the pass over keys takes the product anew. W and R are fp32's: states go into products in several terms.
+// so that X follows from a border on without either state, in 64 bits. R, W and M are fp32's: what their roundings leave in X, some 2^-24 of the products on the way
+// from the border, stays also where X is much smaller than these; it is zero where the chunk's decays let nothing through. To keep the way short, at every eighth border the
+// pass over queries stores its state, and the pass over keys takes the product anew. The sums of M are differences of sums over rows and columns, which leave 2^-53 of them.
+// W and R are fp32's: states go into products in several terms.
 //
 // Layout. A workgroup takes a head of a sequence (or of a part of it) through its chunks. A wave holds all rows of its own columns of the
 // state in the matrix unit's accumulators; these are, as they lie, operands of the next product: with lane = 16 g + n a 16 x 16 tile
@@ -51,7 +53,8 @@ struct AttendArgs {
     // the sum of that part's decays. The borders of a sequence follow each other, those of all sequences too.
     float *ends, *back_ends;
     double *logs;
-    float *reads, *writes, *inside;  // [heads][tokens]: R[t], W[t], and the sum of M[t,s] over s less that of M[s,t]
+    float *reads, *writes;    // [heads][tokens]: R[t] and W[t]
+    double *inside;           // [heads][tokens]: the sum of M[t,s] over s less that of M[s,t]
     double *last;             // [sequences][heads]: <gradient of the last state, last state>
     float *borders;           // [border][heads]: the state at a border, tile by tile as the lanes hold it
     double *cross;            // [border][heads]: its product with the gradient there
@@ -423,16 +426,16 @@ template <int C> struct Decays {
 };
 
 // sum over 16 neighbouring lanes, in the last of them
-__device__ __forceinline__ float row_sum(float v)
+__device__ __forceinline__ double row_sum(double v)
 {
-    v += dpp_move<0x111, 0xf>(0.0f, v);
-    v += dpp_move<0x112, 0xf>(0.0f, v);
-    v += dpp_move<0x114, 0xf>(0.0f, v);
-    v += dpp_move<0x118, 0xf>(0.0f, v);
+    v += dpp_move<0x111, 0xf>(0.0, v);
+    v += dpp_move<0x112, 0xf>(0.0, v);
+    v += dpp_move<0x114, 0xf>(0.0, v);
+    v += dpp_move<0x118, 0xf>(0.0, v);
     return v;
 }
 // sum over the four lanes that hold the same column, in all of them
-__device__ __forceinline__ float column_sum4(float v)
+template <typename T> __device__ __forceinline__ T column_sum4(T v)
 {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
@@ -1078,7 +1081,7 @@ template <int D> constexpr bool attend_both() { return D < 256; }
 template <int D> constexpr int back_waves() { return attend_waves<D>() * (attend_both<D>() ? 2 : 1); }
 template <typename ST, int D> struct BackLds {
     static constexpr int C = Operand<ST>::CHUNK, W = attend_waves<D>();
-    static constexpr int WORDS = 4 * Tile<ST, D>::WORDS + (attend_both<D>() ? 2 : 1) * Scores<ST>::WORDS + Decays<C>::WORDS + W * C + 2 * W + 2 * (C / 16) * C;
+    static constexpr int WORDS = 4 * Tile<ST, D>::WORDS + (attend_both<D>() ? 2 : 1) * Scores<ST>::WORDS + Decays<C>::WORDS + W * C + 2 * W + 4 * (C / 16) * C;
 };
 template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forceinline__ void back_pass(const AttendArgs &args, float *lds)
 {
@@ -1096,7 +1099,8 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
     Decays<C> decays{reinterpret_cast<double *>(take(2 * C)), take(C), take(C)};
     float *red = take(W * C);
     double *over = reinterpret_cast<double *>(take(2 * W));
-    float *rows = take(TT * C), *cols = take(TT * C);  // sums of M over each tile's rows and columns
+    // Sums of M over each tile's rows and columns, in 64 bits: their differences are sums over pairs that pass a token, of which the others' must leave nothing.
+    double *rows = reinterpret_cast<double *>(take(2 * TT * C)), *cols = reinterpret_cast<double *>(take(2 * TT * C));
 
     Span span;
     if (!span_of(args, args.first + blockIdx.x, C, span)) return;
@@ -1154,13 +1158,13 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                     if (tt < st) continue;
                         if (BOTH || KEYS) p[h] = score(O, tt * 16, Vt, st * 16, V);
                     other[h] = score(Q, tt * 16, Kt, st * 16, K);
-                    float over_t = 0.0f;
+                    double over_t = 0.0;
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int s = st * 16 + n16, t = tt * 16 + 4 * g + r;
                         const float w = exp2_(decays.sums[t] - from_s) * a.scale;
                         if (BOTH || KEYS) {
-                            const float m = s < t ? p[h][r] * other[h][r] * w : 0.0f, over_s = row_sum(m);
+                            const double m = s < t ? p[h][r] * other[h][r] * w : 0.0f, over_s = row_sum(m);
                             over_t += m;
                             if (n16 == 15) rows[st * C + t] = over_s;
                         }
@@ -1239,7 +1243,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                 float write = 0.0f;
                 for (int w = 0; w < W; w++) write += red[w * C + threadIdx.x];
                 const int t = threadIdx.x;
-                float inside = 0.0f;
+                double inside = 0.0;
                 for (int st = 0; st <= t / 16; st++) inside += rows[st * C + t];
                 for (int tt = t / 16; tt < TT; tt++) inside -= cols[tt * C + t];
                 const int64_t at = span.head * args.tokens + span.batch * a.T + t0 + t;

@@ -135,3 +135,54 @@ def test_decays_of_a_part_grow_past_float32_where_states_do_not(gpu, monkeypatch
     got, want, total = results(gpu, v, 0.2, gy)
     for n in ("q", "k", "v"):
         near(got[2][n], want[2][n], total[2][n], dtype, T, f"gradient of {n}")
+
+
+def passing(total, decay, dtype, begin=0, end=None):
+    """
+    A decay's gradient is the product of state and gradient that passes its chunk, and what passes the token and not the whole chunk. The former comes from the
+    product at the next border, eight chunks on at most, less what the tokens between it write and more what they read: what these sums' roundings leave is relative to the largest product on the way, but no
+    more than what state and gradient can have as a product: nothing where the chunk's decays let nothing through. That largest product by token, in units of A.
+    """
+    chunk = 32 if dtype == torch.float32 else 64
+    end = total.shape[1] if end is None else end
+    out = torch.zeros_like(total)
+    chunks = (end - begin + chunk - 1) // chunk
+    most = torch.zeros_like(total[:, 0])
+    for c in range(chunks - 1, -1, -1):
+        a, b = begin + c * chunk, min(begin + (c + 1) * chunk, end)
+        if (c + 1) % 8 == 0:  # a border behind this chunk
+            most = total[:, b:min(b + 1, end)].amax(1) if b < end else torch.zeros_like(most)
+        here = torch.maximum(most, total[:, a:b].amax(1))
+        closed = torch.isinf(decay[:, a:b]).any(1)
+        out[:, a:b] = torch.where(closed, 0.0, here)[:, None]
+        most = torch.where(closed, total[:, a], here)
+    return out
+
+
+def near_decays(got, want, total, decay, dtype, T, what, spans=None):
+    """``spans``: first tokens and ends of packed sequences."""
+    got, want, total = (t.detach().cpu().double() for t in (got, want, total))
+    assert torch.isfinite(got).all()
+    noise = torch.zeros_like(total)
+    for a, b in spans or [(0, total.shape[1])]:
+        noise[:, a:b] = passing(total, decay, dtype, a, b)[:, a:b]
+    bound = ((600 + 2 * T) * 2.0 ** -24 + TERMS[dtype]) * (total + noise) + 2.0 ** -44 * total.max() + 1.01 * HALF[torch.float32] * want.abs()
+    over = (got - want).abs() - bound
+    at = int(over.argmax())
+    assert not (over > 0).any(), f"{what}: at {at} of {tuple(got.shape)}: {float(got.flatten()[at])} for {float(want.flatten()[at])}, bound {float(bound.flatten()[at]):.3e}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,cut", [(64, 20), (40, 39), (700, 300), (1200, 511), (1200, 512)])
+@pytest.mark.parametrize("strong", [-math.inf, -90.0])
+@pytest.mark.parametrize("K,V", [(64, 64), (24, 128)])
+def test_a_decay_s_gradient_is_of_what_passes_it(gpu, dtype, T, cut, strong, K, V):
+    """Where a decay lets nothing through its gradient is nothing, however large what later tokens read and write."""
+    v = make(31, dtype, 1, T, 2, K, V, pace=0.01)
+    v["decay"][0, cut] = strong
+    later = min(cut + 12, T - 1)
+    v["v"][:, later:] = (v["v"][:, later:].float() * 100).to(dtype)
+    gy = torch.randn(v["v"].shape, generator=torch.Generator().manual_seed(32)).to(dtype)
+    got, want, total = results(gpu, v, K ** -0.5, gy)
+    shown = torch.where(v["decay"] < -80, -math.inf, v["decay"])  # (e^-90 is 2^-130: of products below 2^60, nothing that the bound's last term does not hold)
+    near_decays(got[2]["decay"], want[2]["decay"], total[2]["decay"], shown, dtype, T, "gradient of the decays")

@@ -20,20 +20,17 @@ template <int AHEAD, int VALUES, bool BACK> __global__ __launch_bounds__(256) vo
     if (borders == 0) return;
     const float *given = BACK ? a.gstate_out : a.state_in;
     float *ends = (BACK ? args.back_ends : args.ends) + at;
-    const double *logs = args.logs;
     const auto border = [&](int i) { return cut_at(args, s, BACK ? borders - 1 - i : i); };
     float run[VALUES];
 #pragma unroll
     for (int v = 0; v < VALUES; v++) run[v] = given != nullptr && at + 256 * v < values ? given[pair * values + at + 256 * v] : 0.0f;
     for (int i0 = 0; i0 < borders; i0 += AHEAD) {
-        float adds[AHEAD][VALUES], decay[AHEAD];
-        int power[AHEAD];
+        float adds[AHEAD][VALUES];
+        AttendArgs::Power decay[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const int there = i0 + i < borders ? i0 + i : borders - 1;
-            const double log = logs[border(there)], whole = __builtin_floor(log < -4096.0 ? -4096.0 : log > 4096.0 ? 4096.0 : log);
-            power[i] = (int)whole;  // (a power past float32's, where decays are above zero: the state may be small, or zero)
-            decay[i] = exp2_(log < -4096.0 || log > 4096.0 ? 0.0 : log - whole);
+            decay[i] = args.powers[border(there)];
 #pragma unroll
             for (int v = 0; v < VALUES; v++) adds[i][v] = at + 256 * v < values ? ends[border(there) * values + 256 * v] : 0.0f;
         }
@@ -42,7 +39,7 @@ template <int AHEAD, int VALUES, bool BACK> __global__ __launch_bounds__(256) vo
             if (i0 + i < borders) {
 #pragma unroll
                 for (int v = 0; v < VALUES; v++) {
-                    run[v] = __builtin_ldexpf(run[v] * decay[i], power[i]) + adds[i][v];
+                    run[v] = __builtin_ldexpf(run[v] * decay[i].rest, decay[i].whole) + adds[i][v];
                     if (at + 256 * v < values) ends[border(i0 + i) * values + 256 * v] = run[v];
                 }
             }
@@ -268,7 +265,7 @@ Plan plan_of(const scanscam_attend &a)
 
 // What the workspace holds, in order; each piece begins on 16 bytes.
 struct Pieces {
-    size_t ends, back_ends, logs, reads, writes, inside, last, borders, cross, part_q, part_k, decays, bytes;
+    size_t ends, back_ends, powers, reads, writes, inside, last, borders, cross, part_q, part_k, decays, bytes;
     int64_t most_borders;
 };
 int64_t ends_values(const scanscam_attend &a, const Plan &plan) { return plan.borders * a.heads * a.K * a.V; }
@@ -282,7 +279,7 @@ Pieces pieces_of(const scanscam_attend &a, bool back, const Plan &plan)
     };
     const int64_t pairs = a.sequences * a.heads, values = ends_values(a, plan), tokens = a.batch * a.T;
     p.ends = take(!back, values, 4);  // (a backward call has the forward one's)
-    p.logs = take(true, plan.borders * a.heads, 8);
+    p.powers = take(true, plan.borders * a.heads, sizeof(AttendArgs::Power));
     if (!back) return p;
     p.back_ends = take(true, values, 4);
     p.reads = take(true, tokens * a.heads, 4);
@@ -403,7 +400,7 @@ int scanscam_attend_fwd(const scanscam_attend *a, void *stream)
     args.cuts = plan.borders;
     args.each = (int32_t)(a->heads / a->groups);
     args.ends = a->saved != nullptr ? static_cast<float *>(a->saved) : reinterpret_cast<float *>(w + at.ends);
-    args.logs = reinterpret_cast<double *>(w + at.logs);
+    args.powers = reinterpret_cast<AttendArgs::Power *>(w + at.powers);
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t err = hipSuccess;
     if (plan.borders > 0) err = starts(args, false, kEnds, plan.units, s);
@@ -439,7 +436,7 @@ int scanscam_attend_bwd(const scanscam_attend *a, void *stream)
     args.each = (int32_t)(a->heads / a->groups);
     args.ends = static_cast<float *>(a->saved);
     args.back_ends = reinterpret_cast<float *>(w + at.back_ends);
-    args.logs = reinterpret_cast<double *>(w + at.logs);
+    args.powers = reinterpret_cast<AttendArgs::Power *>(w + at.powers);
     if (a->gdecay != nullptr) {
         args.reads = reinterpret_cast<float *>(w + at.reads);
         args.writes = reinterpret_cast<float *>(w + at.writes);

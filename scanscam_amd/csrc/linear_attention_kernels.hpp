@@ -50,9 +50,12 @@ struct AttendArgs {
     int64_t per, cuts;        // tokens of a part, whole chunks (0: all of the sequence); borders between parts that there is room for
     int32_t parts, each;      // parts of a sequence of T tokens, heads that share queries and keys
     // [heads][border between parts][K][V]: what the part before it (gradients: behind it) adds to the state, then the state there; and [heads][border between parts],
-    // the sum of that part's decays. The borders of a sequence follow each other, those of all sequences too.
+    // that part's decay. The borders of a sequence follow each other, those of all sequences too.
     float *ends, *back_ends;
-    double *logs;
+    struct Power {
+        float rest;     // rest 2^whole, a part's decay: of logs above zero float32 may not hold it
+        int32_t whole;
+    } *powers;
     float *reads, *writes;    // [heads][tokens]: R[t] and W[t]
     double *inside;           // [heads][tokens]: the sum of M[t,s] over s less that of M[s,t]
     double *last;             // [sequences][heads]: <gradient of the last state, last state>
@@ -1070,7 +1073,10 @@ template <typename ST, int D, int JT, int W, bool BACK, int TERMS, bool EXACT> _
     }
     const int64_t border = cut_at(args, span, span.part - (BACK ? 1 : 0));
     S.write((BACK ? args.back_ends : args.ends) + border * K * V, inner, outer, row_step, col_step);
-    if (threadIdx.x == 0) args.logs[border] = whole;
+    if (threadIdx.x == 0) {
+        const double power = __builtin_floor(whole < -4096.0 ? -4096.0 : whole > 4096.0 ? 4096.0 : whole);
+        args.powers[border] = {exp2_(whole < -4096.0 || whole > 4096.0 ? 0.0 : whole - power), (int32_t)power};
+    }
 }
 
 // --- gradients of keys and values, backwards in time ------------------------------------------------------------------------------------

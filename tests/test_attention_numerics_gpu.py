@@ -186,3 +186,43 @@ def test_a_decay_s_gradient_is_of_what_passes_it(gpu, dtype, T, cut, strong, K, 
     got, want, total = results(gpu, v, K ** -0.5, gy)
     shown = torch.where(v["decay"] < -80, -math.inf, v["decay"])  # (e^-90 is 2^-130: of products below 2^60, nothing that the bound's last term does not hold)
     near_decays(got[2]["decay"], want[2]["decay"], total[2]["decay"], shown, dtype, T, "gradient of the decays")
+
+
+# (more than eight chunks: decays' gradients take the product of state and gradient anew at each eighth border, with states that another pass stored)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,V,lengths", [(128, 128, None), (128, 64, [1100, 0, 37, 600]), (64, 128, None), (256, 256, None), (130, 40, [3, 1070]), (40, 250, None)])
+def test_gradients_of_decays_past_borders_of_wide_heads(gpu, monkeypatch, dtype, K, V, lengths):
+    T = sum(lengths) if lengths else 1100
+    heads = 1 if K * V > 128 * 128 else 2
+    v = make(33, dtype, 1, T, heads, K, V, groups=1, lengths=lengths, state=True, pace=0.002)
+    gy = torch.randn(v["v"].shape, generator=torch.Generator().manual_seed(34)).to(dtype)
+    gs = torch.randn(v["state"].shape, generator=torch.Generator().manual_seed(35))
+    got, want, total = results(gpu, v, K ** -0.5, gy, gs)
+    ends = [0] + torch.tensor(lengths).cumsum(0).tolist() if lengths else [0, T]
+    spans = list(zip(ends, ends[1:]))
+    for parts in (0, 1, 3):
+        monkeypatch.setattr(attention, "_parts", parts)
+        names = [n for n, t in v.items() if t is not None and n != "offsets"]
+        dev = {n: None if t is None else t.to(gpu).requires_grad_(n != "offsets") for n, t in v.items()}
+        y, new, grads = call(f.linear_attention, dev, names, K ** -0.5, gy.to(gpu), gs.to(gpu))
+        near(y, want[0], total[0], dtype, T, f"y, {parts} parts")
+        near(new, want[1], total[1], dtype, T, f"state, {parts} parts")
+        for n in ("q", "k", "v", "state"):
+            near(grads[n], want[2][n], total[2][n], dtype, T, f"gradient of {n}, {parts} parts")
+        near_decays(grads["decay"], want[2]["decay"], total[2]["decay"], v["decay"], dtype, T, f"gradient of decays, {parts} parts", spans)
+
+
+@pytest.mark.parametrize("dtype,T,K,V,decay", [(torch.bfloat16, 1500, 128, 64, "head"), (torch.float32, 1100, 64, 128, "head"), (torch.float32, 17000, 4, 4, "token"), (torch.float32, 17000, 4, 4, "head")])
+def test_gradients_of_decays_over_many_tokens(gpu, dtype, T, K, V, decay):
+    """Decays of heads are sums over more than 1024 tokens; and more than 64 times eight chunks of one sequence."""
+    v = make(36, dtype, 1, T, 2, K, V, decay="token", pace=0.002)
+    if decay == "head":
+        v["decay"] = v["decay"][0, 0].clone()
+    gy = torch.randn(v["v"].shape, generator=torch.Generator().manual_seed(37)).to(dtype)
+    got, want, total = results(gpu, v, K ** -0.5, gy)
+    for n in ("q", "k", "v"):
+        near(got[2][n], want[2][n], total[2][n], dtype, T, f"gradient of {n}")
+    if decay == "head":  # (sums over the tokens in float32 at up to 64 in a row: the products' own roundings are more)
+        near(got[2]["decay"], want[2]["decay"], total[2]["decay"], dtype, T, "gradient of the decays")
+    else:
+        near_decays(got[2]["decay"], want[2]["decay"], total[2]["decay"], v["decay"], dtype, T, "gradient of the decays")

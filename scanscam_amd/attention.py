@@ -8,6 +8,7 @@ Tensors, types, packed sequences, single tokens' slots and recorded calls are as
 counterpart in the reference, whose one operator is the scan.
 """
 import ctypes
+import operator
 from typing import Optional, Tuple, Union
 
 import torch
@@ -88,6 +89,12 @@ def _launching(what: str):
     return _lib()
 
 
+def _number(what: str, name: str, value) -> float:
+    if isinstance(value, torch.Tensor) and value.requires_grad and torch.is_grad_enabled():
+        raise TypeError(f"{what}: {name} is a number and has no gradient, got a tensor that requires one")
+    return float(value)
+
+
 # --------------------------------------------------------------------------------------------------------- linear attention
 def _check_heads(what: str, q, k, v, decay, lead: int) -> None:
     """``lead``: 2 for [batch, T, heads, ...], 1 for [rows, heads, ...]."""
@@ -122,6 +129,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
     :param decay: logs of the decays, [batch, T, heads], or [heads] for one of each head, of any of the three types; none without. They are
         meant to be 0 at most (-infinity forgets everything); above, states grow as far as float32 holds them, and what the logs of any
         64 neighbouring tokens sum up to has to be 80 at most: where float32 does not hold its exponential results are not finite.
+    :param scale: a number (to train it, multiply q with it)
     :param state: [sequences, heads, K, V] in float32, the states before the first tokens (zeros if not given)
     :param offsets: the first token of each of several packed sequences, and the end
     :param return_state: hand back the states after the last tokens as well, in float32
@@ -138,6 +146,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
         if out is not None:
             return out
     what = "linear_attention"
+    scale = _number(what, "scale", scale)
     _check_heads(what, q, k, v, decay, 2)
     _check_devices(what, v, (("q", q), ("k", k), ("decay", decay), ("state", state), ("offsets", offsets)))
     sequences = _check_offsets(what, v, offsets)
@@ -149,7 +158,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, decay: O
         return baseline.naive_linear_attention(q, k, v, decay, scale=scale, state=state, offsets=offsets, return_state=return_state)
     _check_sizes(what, max(heads * max(K, V), q.shape[2] * K), v.shape[0] * v.shape[1], sequences)
     if _needs_node(q, k, v, decay, state):
-        y, new = LinearAttention.apply(q, k, v, decay, state, offsets, float(scale), bool(return_state))
+        y, new = LinearAttention.apply(q, k, v, decay, state, offsets, scale, bool(return_state))
     else:
         y, new, _, _ = _attend_forward(q, k, v, decay, state, offsets, scale, return_state, False)
     return (y, new) if return_state else y
@@ -254,6 +263,7 @@ def linear_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
         if out is not None:
             return out
     what = "linear_attention_step"
+    scale = _number(what, "scale", scale)
     _check_heads(what, q, k, v, decay, 1)
     _check_devices(what, v, (("state", state), ("q", q), ("k", k), ("decay", decay), ("slots", slots)))
     rows, heads, V = v.shape
@@ -270,7 +280,7 @@ def linear_attention_step(state: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
         return baseline.naive_linear_attention_step(state, q, k, v, decay, scale=scale, slots=slots)
     _check_sizes(what, heads * max(q.shape[2], V), rows)
     if torch.jit.is_tracing():
-        return LinearAttentionStep.apply(state, q, k, v, decay, slots, float(scale))
+        return LinearAttentionStep.apply(state, q, k, v, decay, slots, scale)
     return _attend_step(state, q, k, v, decay, slots, scale)
 
 
@@ -324,7 +334,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         if out is not None:
             return out
     what = "group_norm"
-    groups = int(groups)
+    groups, eps = operator.index(groups), _number(what, "eps", eps)
     if x.dim() < 1 or groups < 1 or x.shape[-1] % groups:
         raise AssertionError(f"{what}: x must be [..., channels] with channels shared out evenly to the groups, got shape {tuple(x.shape)} and {groups} groups")
     if x.shape[-1] // groups > _MOST_GROUP:
@@ -338,7 +348,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         return baseline.naive_group_norm(x, groups, weight, bias, z, eps=eps, activation=activation)
     _check_sizes(what, x.shape[-1], x.shape[:-1].numel())
     if _needs_node(x, weight, bias, z):
-        return GroupNorm.apply(x, groups, weight, bias, z, float(eps), activation)
+        return GroupNorm.apply(x, groups, weight, bias, z, eps, activation)
     return _group_norm_forward(x, groups, weight, bias, z, eps, activation)[0]
 
 

@@ -1284,9 +1284,13 @@ struct GroupNormBackward : torch::autograd::Function<GroupNormBackward> {
     }
 };
 
-// A number, or not covered.
+// A number, or not covered (a tensor is one with a gradient, perhaps).
 double number(Arguments &in, int i)
 {
+    if (!PyFloat_Check(in.args[i]) && !PyLong_Check(in.args[i])) {
+        in.ok = false;
+        return 0.0;
+    }
     const double v = PyFloat_AsDouble(in.args[i]);
     if (PyErr_Occurred()) {
         PyErr_Clear();

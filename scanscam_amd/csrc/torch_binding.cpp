@@ -438,6 +438,12 @@ struct Operators {
 
 constexpr int64_t kMostStates = 256, kMostTaps = 8, kMostNormChannels = 32768;
 
+// A state was written in place: its version says so, where it has one (tensors made in inference mode do not, and outside of it the count would raise, after the launch).
+void written(const at::Tensor &state)
+{
+    if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
+
 // The arguments of one call, looked at one after the other; `ok` says whether it is covered so far.
 // An output that the kernels write whole, without the dispatcher's part of at::empty() (0.8 us each against 0.45; modes and the tracer have been asked for).
 at::Tensor output(at::IntArrayRef sizes, at::ScalarType type, at::Device device) { return at::detail::empty_cuda(sizes, type, device, std::nullopt); }
@@ -1001,7 +1007,7 @@ PyObject *conv_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     at::Tensor y = in.empty(x.sizes(), x.scalar_type());
     a.y = in.tokens(y, 1);
     SCANSCAM_LAUNCH(operators.conv_step(&a, in.stream()), "conv_step_fwd")
-    state.unsafeGetTensorImpl()->bump_version();  // (written in place)
+    written(state);
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }
@@ -1108,7 +1114,7 @@ PyObject *selective_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     at::Tensor y = in.empty(x.sizes(), x.scalar_type());
     a.y = in.tokens(y, 1);
     SCANSCAM_LAUNCH(operators.selective_step(&a, in.stream()), "selective_step_fwd")
-    state.unsafeGetTensorImpl()->bump_version();
+    written(state);
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }
@@ -1391,7 +1397,7 @@ PyObject *attend_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     at::Tensor y = in.empty(v.sizes(), v.scalar_type());
     a.y = in.tokens(y, 1);
     SCANSCAM_LAUNCH(attention.step(&a, in.stream()), "attend_step_fwd")
-    state.unsafeGetTensorImpl()->bump_version();
+    written(state);
     return THPVariable_Wrap(std::move(y));
     END_HANDLE_TH_ERRORS
 }

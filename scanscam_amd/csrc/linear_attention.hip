@@ -226,12 +226,15 @@ int check_attend(const scanscam_attend *a, bool back)
 int chunk_of(const scanscam_attend &a) { return a.dtype == SCANSCAM_F32 ? Operand<float>::CHUNK : Operand<__bf16>::CHUNK; }
 
 // How time is shared out. Parts cost a second pass over keys and values, and states at their borders; they are for calls with fewer heads of sequences
-// than it takes to fill the card, two workgroups on each of 256 CUs: up to 512 parts of no less than four chunks. ([8, 4096, 16 x 128] in bf16 with gradients
-// by 1, 2, 4, 8 parts: 1.74, 1.16, 0.99, 1.09 ms; 30001 tokens of four heads in float32 by 64, 128: 425, 416 us.)
+// than it takes to fill the card: up to 512 parts of no less than four chunks. ([8, 4096, 16 x 128] in bf16 with gradients
+// by 1, 2, 4, 8 parts: 1.74, 1.16, 0.99, 1.09 ms; 30001 tokens of four heads in float32 by 64, 128: 425, 416 us.) 512 is two workgroups on each of 256 CUs, which holds for the
+// forward pass of up to 128 channels. Backwards, and of more channels, a CU has one, so that where two parts make no round of workgroups fewer one part is better:
+// [12, 2048, 16 x 128] in bf16 with gradients takes 940 us by the rule's two and 820 by one; [8, 2048, 8 x 256 x 256] 1810 by its eight and 1530 by four.
 // Of sequences behind each other the host knows all tokens only. Their parts have one length, which makes 384 of all tokens, and the sequences' last ones, shorter as
-// they are, come on top: 8021 tokens of 13 sequences of 16 heads, from equal ones to one with two thirds of the tokens, 99 - 109 us; with 512 114 - 124,
+// they are, come on top: 8021 tokens of 13 sequences of 16 heads, from equal ones to one with two thirds of the tokens, 99 - 113 us; with 512 114 - 124,
 // 256 117 - 125, and in one part each 114 - 492. A sequence that is no longer than a part is one, and costs an empty workgroup in either of the passes more.
-// (Heads of sequences enough fill the card by themselves; and every workgroup counts the sequences, 64 in a trip to memory.)
+// Every workgroup counts the sequences, 64 in a trip to memory: more than 256 are not shared out, nor heads of sequences that fill the card by themselves
+// (6000 tokens and 299 short sequences of four heads: 550 us; with 249 short ones 115).
 struct Plan {
     int64_t per;                         // tokens of a part, whole chunks; 0: all of the sequence
     int64_t units, borders;              // heads of parts; borders between parts, at most

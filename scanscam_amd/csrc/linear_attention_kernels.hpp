@@ -29,8 +29,8 @@
 //
 // What bounds it: neither memory nor the matrix unit, but the chain of a chunk (loads to LDS, scores, a barrier, sums, the state's update, a barrier) in few waves,
 // for a state's columns and a chunk's operands leave registers for two waves a SIMD. [8, 4096, 16 x 128] in bf16, in four parts: ends of parts 60 us, outputs
-// 153 (of 537 MB, 3.5 TB/s), ends backwards 72, gradients of queries 259, of keys and values 401, decays 10.
-// In counters the matrix unit is busy for a fifth of these, the vector unit (terms, decays, addresses) for a third.
+// 154 (of 537 MB, 3.5 TB/s; 566 by the counters), ends backwards 73, gradients of queries 258, of keys and values 410, decays 12.
+// In counters the matrix unit is busy for 26 % of the time forwards and for 18 to 20 % of the gradients' kernels, the vector unit (terms, decays, addresses) for 41 and 33 to 36 %.
 #pragma once
 
 #include "ops_common.hpp"
@@ -123,7 +123,7 @@ template <typename ST, int TERMS, int N> __device__ __forceinline__ void split(c
 #pragma unroll
         for (int e = 0; e < N; e++) out[0][e] = x[e];
     } else if constexpr (std::is_same_v<ST, __bf16>) {
-        // Two at a time: one conversion makes both, and their 32 bits hold both floats (267 us of the gradients of queries below were 246).
+        // Two at a time: one conversion makes both, and their 32 bits hold both floats (gradients of queries of the layer above 246 us, 267 one at a time).
         typedef float float2v __attribute__((ext_vector_type(2)));
         typedef __bf16 pair __attribute__((ext_vector_type(2)));
 #pragma unroll

@@ -1074,8 +1074,10 @@ template <typename ST, int D, int JT, int W, bool BACK, int TERMS, bool EXACT> _
     const int64_t border = cut_at(args, span, span.part - (BACK ? 1 : 0));
     S.write((BACK ? args.back_ends : args.ends) + border * K * V, inner, outer, row_step, col_step);
     if (threadIdx.x == 0) {
-        const double power = __builtin_floor(whole < -4096.0 ? -4096.0 : whole > 4096.0 ? 4096.0 : whole);
-        args.powers[border] = {exp2_(whole < -4096.0 || whole > 4096.0 ? 0.0 : whole - power), (int32_t)power};
+        // (the rest is 1 at most, so that the product with it stays finite)
+        const bool held = whole >= -4096.0 && whole <= 4096.0;
+        const double power = __builtin_ceil(held ? whole : whole < 0.0 ? -4096.0 : 4096.0);
+        args.powers[border] = {exp2_(held ? whole - power : 0.0), (int32_t)power};
     }
 }
 
@@ -1162,7 +1164,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                     const int tt = step * PER + h;
                     p[h] = other[h] = float4v{0, 0, 0, 0};
                     if (tt < st) continue;
-                        if (BOTH || KEYS) p[h] = score(O, tt * 16, Vt, st * 16, V);
+                    if (BOTH || KEYS) p[h] = score(O, tt * 16, Vt, st * 16, V);
                     other[h] = score(Q, tt * 16, Kt, st * 16, K);
                     double over_t = 0.0;
 #pragma unroll

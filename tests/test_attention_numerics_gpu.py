@@ -226,3 +226,22 @@ def test_gradients_of_decays_over_many_tokens(gpu, dtype, T, K, V, decay):
         near(got[2]["decay"], want[2]["decay"], total[2]["decay"], dtype, T, "gradient of the decays")
     else:
         near_decays(got[2]["decay"], want[2]["decay"], total[2]["decay"], v["decay"], dtype, T, "gradient of the decays")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("parts", [0, 3])
+def test_states_near_float32_s_largest_value(gpu, monkeypatch, dtype, parts):
+    """They decay a little, in one part or from part to part, and stay finite on the way."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    T = 200
+    v = make(38, dtype, 1, T, 2, 24, 16, state=True)
+    v["q"] *= 0
+    v["state"] = v["state"].sign() * 3.2e38
+    v["decay"] = torch.full((1, T, 2), -1e-3)
+    gs = v["state"].flip(-1).contiguous()
+    given = {n: t if t is None else t.to(gpu).requires_grad_(n == "state") for n, t in v.items()}
+    _, new = f.linear_attention(**given, return_state=True)
+    back, = torch.autograd.grad(new, given["state"], gs.to(gpu))
+    want = v["state"].double() * math.exp(-1e-3 * T)
+    near(new, want, want.abs(), dtype, T, "state")
+    near(back, want.flip(-1), want.abs(), dtype, T, "gradient of the state")

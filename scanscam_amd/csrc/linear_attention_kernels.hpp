@@ -596,9 +596,9 @@ template <typename ST, int D, int JT, int WAVES> struct State {
         }
         return factor;
     }
-    // s = decay s + sum over the chunk's tokens of from[t] (weight[t] factor own[t])^T
+    // s = decay s + sum over the chunk's tokens of from[t] (weight[t] factor own[t])^T; scaled: what times() or scale() of this state returned
     template <int TERMS>
-    __device__ __forceinline__ void update(Tile<ST, D> from, int rows, const frag_t<ST> (&own)[JT][STEPS], const float *weight, float factor, float decay)
+    __device__ __forceinline__ void update(Tile<ST, D> from, int rows, const frag_t<ST> (&own)[JT][STEPS], const float *weight, float factor, float decay, float scaled)
     {
         const int g = (threadIdx.x & 63) >> 4;
         float bring = 1.0f;
@@ -621,7 +621,7 @@ template <typename ST, int D, int JT, int WAVES> struct State {
                 return most_of(most);
             });
             // The state is multiplied with it as well, and must stay finite.
-            const float all = largest(false), most = (all < __builtin_inff() ? all : largest(true)) * decay;
+            const float most = 32768.0f / scaled * decay;
             bring = bring < 1048576.0f ? bring : 1048576.0f;
             if (__builtin_expect(!(most < 0x1p105f), 0)) {
                 const float room = most < __builtin_inff() ? __builtin_ldexpf(1.0f, 126 + 127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23)) : 1.0f;
@@ -893,7 +893,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
             scores.put_step(tt, step, p);
         }
         float4v acc[TT][JT];
-        const float factor = a.scale / S.template times<GRAD ? TERMS : kTermsRounded<ST>>(X, inner, acc);
+        const float scaled = S.template times<GRAD ? TERMS : kTermsRounded<ST>>(X, inner, acc), factor = a.scale / scaled;
         if constexpr (GRAD)
             if (args.borders != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0)
                 S.keep(args.borders + border_at(args, span.batch, t0, C, span.head) * D * D, inner, outer);
@@ -987,7 +987,7 @@ template <typename ST, int D, int JT, int W, bool GRAD, bool EXACT> __global__ _
                 if (g == 0) red[wave * C + t] = read;
             }
         }
-        S.template update<TERMS>(Y, inner, own, decays.after, 1.0f, decays.whole());
+        S.template update<TERMS>(Y, inner, own, decays.after, 1.0f, decays.whole(), scaled);
         __syncthreads();
         if constexpr (GRAD) {
             if (threadIdx.x < (unsigned)n && args.reads != nullptr) {
@@ -1068,7 +1068,7 @@ template <typename ST, int D, int JT, int W, bool BACK, int TERMS, bool EXACT> _
         for (int jt = 0; jt < JT; jt++)
 #pragma unroll
             for (int step = 0; step < STEPS; step++) own[jt][step] = Z.columns(S.column(jt), step * KS);
-        S.template update<TERMS>(Y, inner, own, BACK ? decays.upto : decays.after, BACK ? a.scale : 1.0f, decays.whole());
+        S.template update<TERMS>(Y, inner, own, BACK ? decays.upto : decays.after, BACK ? a.scale : 1.0f, decays.whole(), S.scale());
         __syncthreads();
     }
     const int64_t border = cut_at(args, span, span.part - (BACK ? 1 : 0));
@@ -1189,7 +1189,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
             }
         }
         float4v acc[TT][JT];
-        const float unscale = 1.0f / H.template times<TERMS>(inter, inner, acc);
+        const float scaled = H.template times<TERMS>(inter, inner, acc), unscale = 1.0f / scaled;
         frag_t<ST> own[JT][STEPS];
 #pragma unroll
         for (int jt = 0; jt < JT; jt++)
@@ -1233,7 +1233,7 @@ template <typename ST, int D, int JT, bool KEYS, bool EXACT> __device__ __forcei
                 if (g == 0) red[wave * C + s] = write;
             }
         }
-        H.template update<TERMS>(update_rows, inner, own, decays.upto, a.scale, decays.whole());
+        H.template update<TERMS>(update_rows, inner, own, decays.upto, a.scale, decays.whole(), scaled);
         if constexpr (KEYS) {
             const bool border = args.cross != nullptr && t0 > span.from && (t0 - span.from) % (kBorder * C) == 0;
             const int64_t at_border = border ? border_at(args, span.batch, t0, C, span.head) : 0;

@@ -622,9 +622,8 @@ template <typename ST, int D, int JT, int WAVES> struct State {
             });
             // The state is multiplied with it as well, and must stay finite.
             const float most = 32768.0f / scaled * decay;
-            bring = bring < 1048576.0f ? bring : 1048576.0f;
-            if (__builtin_expect(!(most < 0x1p105f), 0)) {
-                const float room = most < __builtin_inff() ? __builtin_ldexpf(1.0f, 126 + 127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23)) : 1.0f;
+            if (__builtin_expect(!(most * bring < 0x1p126f), 0)) {
+                const float room = most < __builtin_inff() ? __builtin_ldexpf(1.0f, 125 + 127 - (int)(__builtin_bit_cast(uint32_t, most) >> 23)) : 1.0f;
                 bring = bring < room ? bring : room;
             }
             factor *= bring;

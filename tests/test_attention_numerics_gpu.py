@@ -245,3 +245,18 @@ def test_states_near_float32_s_largest_value(gpu, monkeypatch, dtype, parts):
     want = v["state"].double() * math.exp(-1e-3 * T)
     near(new, want, want.abs(), dtype, T, "state")
     near(back, want.flip(-1), want.abs(), dtype, T, "gradient of the state")
+
+
+@pytest.mark.parametrize("K,V,T,parts", [(3, 3, 17, 0), (64, 32, 142, 2), (130, 200, 60, 0)])
+def test_small_additions_to_states_in_fp16(gpu, monkeypatch, K, V, T, parts):
+    """Gradients of states that nothing but the far ends of a strong decay adds to, and small states: as small as they are."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    v = make(39, torch.float16, 1, T, 2, K, V, state=True, pace=0.01)
+    v["state"] *= 1e-12
+    v["decay"][:, 0] = -25.0  # (what reaches the first state is e^-25)
+    v["v"] = (v["v"].float() * 1e-3).half()
+    g = torch.Generator().manual_seed(40)
+    gy, gs = torch.randn(v["v"].shape, generator=g).half(), torch.randn(v["state"].shape, generator=g) * 1e-12
+    got, want, total = results(gpu, v, K ** -0.5, gy, gs)
+    near(got[1], want[1], total[1], torch.float16, T, "state")
+    near(got[2]["state"], want[2]["state"], total[2]["state"], torch.float16, T, "gradient of the state")

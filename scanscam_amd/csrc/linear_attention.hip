@@ -67,7 +67,7 @@ template <int C> __global__ __launch_bounds__(64 * kBorder) void decays_kernel(A
         if (lane == 63) {
             all_reads[wave] = reads;
             all_writes[wave] = writes;
-            closed[wave] = exp2_(decay) == 0.0f;  // (as for the states: nothing passes the chunk)
+            closed[wave] = exp2_(decay) == 0.0f || (c == 0 && a.state_in == nullptr);  // (as for the states: nothing passes the chunk, or there is nothing before it)
         }
         __syncthreads();
         double end = first + kBorder < chunks ? args.cross[border_at(args, span.batch, span.from + (first + kBorder) * C, C, span.head)] : args.last[args.first + blockIdx.x];

@@ -260,3 +260,20 @@ def test_small_additions_to_states_in_fp16(gpu, monkeypatch, K, V, T, parts):
     got, want, total = results(gpu, v, K ** -0.5, gy, gs)
     near(got[1], want[1], total[1], torch.float16, T, "state")
     near(got[2]["state"], want[2]["state"], total[2]["state"], torch.float16, T, "gradient of the state")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths", [[1, 1, 0, 1], [1, 90, 5, 300, 64], [700, 3]])
+@pytest.mark.parametrize("parts", [0, 2])
+def test_a_first_token_s_decay_has_no_gradient_without_a_state(gpu, monkeypatch, dtype, lengths, parts):
+    """There is nothing that it lets through, whatever the last states' gradients are."""
+    monkeypatch.setattr(attention, "_parts", parts)
+    v = make(41, dtype, 0, 0, 2, 40, 56, lengths=lengths, pace=0.01)
+    given = {n: t if t is None else t.to(gpu).requires_grad_(n != "offsets") for n, t in v.items()}
+    y, new = f.linear_attention(**given, return_state=True)
+    g = torch.Generator().manual_seed(42)
+    gy, gs = torch.randn(y.shape, generator=g).to(dtype).to(gpu), torch.randn(new.shape, generator=g).to(gpu)
+    grad, = torch.autograd.grad((y, new), given["decay"], (gy, gs))
+    first = [int(o) for o, n in zip(v["offsets"], lengths) if n > 0]
+    assert grad[0, first].abs().max() <= 2.0 ** -44 * 40 * 56 * 300  # (sums in 64 bits of pairs, of as many products of some 1 each)
+    assert all(n < 2 or grad[0, int(o) + 1:int(o) + n].abs().max() > 1e-3 for o, n in zip(v["offsets"], lengths))
